@@ -18,6 +18,7 @@ enum DeviceError : int32_t {
   kDevErrTimeout = 1,       // an mbarrier wait ran out of time
   kDevErrExpertId = 2,      // an expert id outside [0, E)
   kDevErrNoTier = 4,        // a routed expert that no tier holds
+  kDevErrOffsets = 8,       // group offsets that decrease or leave the rows
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {

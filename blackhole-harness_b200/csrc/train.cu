@@ -1,0 +1,660 @@
+// train.cu — the memory-bound operators of training a MoE layer's 16-bit
+// experts: SwiGLU with the routing weight (forward and backward) and the global
+// gradient norm with clipping.
+#include <algorithm>
+#include <atomic>
+#include <cstdarg>
+#include <cmath>
+#include <cstdio>
+#include <type_traits>
+#include <vector>
+
+#include "internal.cuh"
+#include "ptx.cuh"
+
+namespace hexmoe {
+namespace {
+
+int arg_error(const char* fmt, ...) {
+  char buf[256];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return report_error(HEXMOE_E_ARG, buf);
+}
+
+bool known_dtype(int32_t dt) { return dt == HEXMOE_F32 || dt == HEXMOE_BF16 || dt == HEXMOE_F16; }
+size_t dtype_bytes(int32_t dt) { return dt == HEXMOE_F32 ? 4 : 2; }
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __half>) return __half2float(v);
+  else return __bfloat162float(v);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float v) {
+  if constexpr (std::is_same_v<T, float>) return v;
+  else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(v);
+  else return __float2bfloat16_rn(v);
+}
+
+// V consecutive elements as one register load or store of up to 16 bytes.
+template <int BYTES>
+struct RawOf;
+template <> struct RawOf<16> { using type = uint4; };
+template <> struct RawOf<8> { using type = uint2; };
+template <> struct RawOf<4> { using type = uint32_t; };
+template <> struct RawOf<2> { using type = uint16_t; };
+
+template <typename T, int V>
+struct Vec {
+  using Raw = typename RawOf<static_cast<int>(sizeof(T)) * V>::type;
+  static constexpr int kWords = sizeof(Raw) < 4 ? 1 : sizeof(Raw) / 4;
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&x)[V]) {
+    if constexpr (V == 1 && sizeof(T) == 2) {
+      x[0] = to_f32(reinterpret_cast<const T&>(r));
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        if constexpr (std::is_same_v<T, float>) {
+          x[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same_v<T, __half>) {
+          const float2 f = __half22float2(reinterpret_cast<const __half2&>(w[i]));
+          x[2 * i] = f.x;
+          x[2 * i + 1] = f.y;
+        } else {
+          x[2 * i] = __uint_as_float(w[i] << 16);
+          x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+      }
+    }
+  }
+  static __device__ __forceinline__ Raw pack(const float (&x)[V]) {
+    Raw r;
+    if constexpr (V == 1 && sizeof(T) == 2) {
+      const T t = from_f32<T>(x[0]);
+      r = reinterpret_cast<const uint16_t&>(t);
+    } else {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        if constexpr (std::is_same_v<T, float>) {
+          w[i] = __float_as_uint(x[i]);
+        } else if constexpr (std::is_same_v<T, __half>) {
+          const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+          w[i] = reinterpret_cast<const uint32_t&>(h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+          w[i] = reinterpret_cast<const uint32_t&>(h);
+        }
+      }
+    }
+    return r;
+  }
+};
+
+cudaLaunchConfig_t launch_config(dim3 grid, int threads, cudaStream_t st, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr->val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// ------------------------------------------------------------------- SwiGLU
+// act = w silu(g) u on rows [g | u], silu(g) = g s, s = 1 / (1 + e^-g), and with
+// d = dL/dact
+//   dg = w d u (s + silu(g) (1 - s)),  du = w d silu(g),  dw = sum_i d silu(g) u
+// Bound by HBM: 3 values of traffic per activation forward, 5 backward.  TPR
+// threads take a row (a warp for common widths, a block's 128 for wide rows or
+// few of them, 4 or 8 for narrow ones), so that the sum of dw stays in one
+// thread group and is added in a fixed order; each thread has kUnroll 16-byte
+// loads per operand in flight.
+constexpr int kSwigluThreads = 256;
+constexpr int kUnroll = 3;   // three 16-byte pieces a lane cover 768 16-bit values a warp
+
+struct SwigluParams {
+  const void* h;        // [rows, 2 * inter]
+  const void* dact;     // backward: [rows, inter]
+  const float* weight;  // [rows] or null
+  void* out;            // forward: act [rows, inter]; backward: dh [rows, 2 * inter]
+  float* dweight;       // backward: [rows] or null
+  int64_t rows, ld_h, ld_dact, ld_out;
+  int32_t inter;
+};
+
+// s and silu(g).  16-bit types round the result to 2^-9 or 2^-12: the fast
+// exponential and reciprocal (about 2^-21) vanish in that.  f32 uses expf and
+// the rounded divide.
+template <typename T>
+__device__ __forceinline__ void sigmoid_silu(float g, float& s, float& silu) {
+  if constexpr (std::is_same_v<T, float>) {
+    s = 1.f / (1.f + expf(-g));
+  } else {
+    s = __fdividef(1.f, 1.f + __expf(-g));
+  }
+  silu = g * s;
+}
+
+template <typename T, int V, int TPR, bool BWD>
+__global__ void __launch_bounds__(kSwigluThreads) swiglu_kernel(const SwigluParams p) {
+  using VecT = Vec<T, V>;
+  using Raw = typename VecT::Raw;
+  constexpr int kRows = kSwigluThreads / TPR;
+  const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + slot;
+  pdl_wait();
+  const bool live = row < p.rows;
+  float sum = 0.f;
+  if (live) {
+    const T* g_row = static_cast<const T*>(p.h) + row * p.ld_h;
+    const T* u_row = g_row + p.inter;
+    const T* d_row = BWD ? static_cast<const T*>(p.dact) + row * p.ld_dact : nullptr;
+    T* o_row = static_cast<T*>(p.out) + row * p.ld_out;
+    const float w = p.weight ? p.weight[row] : 1.f;
+    const int n = p.inter / V;
+    for (int c0 = lane; c0 < n; c0 += TPR * kUnroll) {
+      Raw g[kUnroll], u[kUnroll], d[kUnroll];
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) {
+        const int c = c0 + i * TPR;
+        if (c < n) {
+          g[i] = reinterpret_cast<const Raw*>(g_row)[c];
+          u[i] = reinterpret_cast<const Raw*>(u_row)[c];
+          if constexpr (BWD) d[i] = reinterpret_cast<const Raw*>(d_row)[c];
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) {
+        const int c = c0 + i * TPR;
+        if (c >= n) continue;
+        float gf[V], uf[V], df[V], a[V], b[V];
+        VecT::unpack(g[i], gf);
+        VecT::unpack(u[i], uf);
+        if constexpr (BWD) VecT::unpack(d[i], df);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          float s, silu;
+          sigmoid_silu<T>(gf[j], s, silu);
+          if constexpr (BWD) {
+            sum += df[j] * silu * uf[j];
+            const float dw = df[j] * w;
+            a[j] = dw * uf[j] * (s + silu * (1.f - s));
+            b[j] = dw * silu;
+          } else {
+            a[j] = silu * w * uf[j];   // a weight of zero comes before the product that may overflow
+          }
+        }
+        reinterpret_cast<Raw*>(o_row)[c] = VecT::pack(a);
+        if constexpr (BWD) reinterpret_cast<Raw*>(o_row + p.inter)[c] = VecT::pack(b);
+      }
+    }
+  }
+  if constexpr (BWD) {
+    if (p.dweight) {   // uniform over the grid: every thread takes part
+#pragma unroll
+      for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if constexpr (TPR > 32) {
+        __shared__ float part[kSwigluThreads / 32];
+        if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < TPR / 32; ++i) sum += part[slot * (TPR / 32) + i];
+      }
+      if (live && lane == 0) p.dweight[row] = sum;
+    }
+  }
+}
+
+template <typename T, int V, int TPR, bool BWD>
+cudaError_t launch_swiglu_one(const SwigluParams& p, cudaStream_t st) {
+  const int64_t blocks = (p.rows + kSwigluThreads / TPR - 1) / (kSwigluThreads / TPR);
+  if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  cudaLaunchAttribute attr;
+  const cudaLaunchConfig_t cfg = launch_config(dim3(static_cast<unsigned>(blocks)), kSwigluThreads, st, &attr);
+  return cudaLaunchKernelEx(&cfg, swiglu_kernel<T, V, TPR, BWD>, p);
+}
+
+template <typename T, int V, bool BWD>
+cudaError_t launch_swiglu_vec(const SwigluParams& p, cudaStream_t st) {
+  const int n = p.inter / V;
+  if (n <= 4 * kUnroll) return launch_swiglu_one<T, V, 4, BWD>(p, st);
+  if (n <= 8 * kUnroll) return launch_swiglu_one<T, V, 8, BWD>(p, st);
+  if (n <= 32 * kUnroll || p.rows >= 8192) return launch_swiglu_one<T, V, 32, BWD>(p, st);
+  return launch_swiglu_one<T, V, 128, BWD>(p, st);
+}
+
+template <typename T, bool BWD>
+cudaError_t launch_swiglu_type(const SwigluParams& p, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  auto aligned = [](const void* q, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld * static_cast<int64_t>(sizeof(T)) % 16 == 0;
+  };
+  const bool vec = p.inter % V == 0 && aligned(p.h, p.ld_h) && aligned(p.out, p.ld_out) &&
+                   (!BWD || aligned(p.dact, p.ld_dact));
+  return vec ? launch_swiglu_vec<T, V, BWD>(p, st) : launch_swiglu_vec<T, 1, BWD>(p, st);
+}
+
+int run_swiglu(const char* what, const SwigluParams& p, int32_t dtype, bool bwd, void* stream) {
+  if (!known_dtype(dtype)) return report_error(HEXMOE_E_DTYPE, "swiglu: bad dtype");
+  if (p.rows < 0 || p.inter <= 0 || p.inter > (1 << 30)) return arg_error("%s: rows %lld, inter %d", what, static_cast<long long>(p.rows), p.inter);
+  if (p.ld_h < 2ll * p.inter || p.ld_out < (bwd ? 2ll : 1ll) * p.inter || (bwd && p.ld_dact < p.inter))
+    return arg_error("%s: a row stride is shorter than its row", what);
+  if (p.rows == 0) return HEXMOE_OK;
+  if (!p.h || !p.out || (bwd && !p.dact)) return arg_error("%s: null pointer", what);
+  const size_t z = dtype_bytes(dtype);
+  if (reinterpret_cast<uintptr_t>(p.h) % z || reinterpret_cast<uintptr_t>(p.out) % z ||
+      reinterpret_cast<uintptr_t>(p.dact) % z || reinterpret_cast<uintptr_t>(p.weight) % 4 ||
+      reinterpret_cast<uintptr_t>(p.dweight) % 4)
+    return arg_error("%s: a pointer is not aligned to its element", what);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    return bwd ? launch_swiglu_type<T, true>(p, st) : launch_swiglu_type<T, false>(p, st);
+  };
+  const cudaError_t e = dtype == HEXMOE_F32 ? go(float{}) : dtype == HEXMOE_F16 ? go(__half{}) : go(__nv_bfloat16{});
+  return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
+}
+
+// ------------------------------------------- gradient norm and clipping
+// norm = sqrt(sum x^2) (or max |x|) over a list of tensors, then
+// out = x min(1, max_norm / (norm + 1e-6)).  Bound by HBM: a read for the norm
+// and, where something is scaled or copied, a read and a write.  Two kernels:
+// partial sums per block, then every block adds all partials in the same order
+// (one result, whatever the order of the blocks) and scales.  The tensor list
+// travels as a kernel parameter, so nothing of it is kept between calls.  Each
+// block owns a run of consecutive chunks and the second kernel walks it
+// backwards: what the first one read last is still in L2.
+constexpr int kClipThreads = 256;
+constexpr int kClipPerSm = 4;
+constexpr int kClipChunk = 8192;   // values; a multiple of every vector's
+constexpr int kClipSmallList = 64;
+constexpr int kClipList = 1000;    // 32 bytes an entry: just under the 32764 bytes of parameters
+
+struct ClipEntry {
+  const void* src;
+  void* dst;
+  int64_t n;
+  uint32_t first;   // its first chunk
+  int16_t src_type, dst_type;
+};
+template <int CAP>
+struct ClipTable {
+  int32_t count;
+  uint32_t chunks;
+  ClipEntry e[CAP];
+};
+
+// Sum of squares of up to 8 values, exact to f32 rounding at every magnitude:
+// where the plain sum overflows or has lost small values to underflow, the
+// values are scaled by a power of two first.
+template <int V>
+__device__ __forceinline__ double square_sum(const float (&x)[V]) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) s = fmaf(x[i], x[i], s);
+  if (s > 1e-25f && s < 3e38f) return static_cast<double>(s);
+  const float f = s <= 1e-25f ? 0x1p100f : 0x1p-64f;
+  const double back = s <= 1e-25f ? 0x1p-200 : 0x1p128;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) s = fmaf(x[i] * f, x[i] * f, s);
+  return static_cast<double>(s) * back;
+}
+
+// |x| as bits: integer order is the order of magnitudes, with NaN above infinity.
+template <int V>
+__device__ __forceinline__ uint32_t max_bits(const float (&x)[V]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) m = max(m, __float_as_uint(x[i]) & 0x7fffffffu);
+  return m;
+}
+
+template <bool INF>
+struct ClipAcc {
+  double sum = 0;
+  uint32_t big = 0;
+  template <int V>
+  __device__ __forceinline__ void add(const float (&x)[V]) {
+    if constexpr (INF) big = max(big, max_bits(x));
+    else sum += square_sum(x);
+  }
+};
+
+// The `count` values of a chunk into the accumulator, by one block.
+template <typename T, bool INF>
+__device__ __forceinline__ void clip_read(const T* src, int count, ClipAcc<INF>& acc) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int U = 4;
+  // head: the values before the first 16-byte boundary
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(src) % 16 / sizeof(T));
+  const int head = min(count, off ? V - off : 0);
+  if (threadIdx.x < head) {
+    const float x[1] = {to_f32(src[threadIdx.x])};
+    acc.add(x);
+  }
+  const int n = (count - head) / V;
+  using Raw = typename Vec<T, V>::Raw;
+  const Raw* v = reinterpret_cast<const Raw*>(src + head);
+  for (int c0 = threadIdx.x; c0 < n; c0 += kClipThreads * U) {
+    Raw r[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (c0 + i * kClipThreads < n) r[i] = v[c0 + i * kClipThreads];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (c0 + i * kClipThreads >= n) continue;
+      float x[V];
+      Vec<T, V>::unpack(r[i], x);
+      acc.add(x);
+    }
+  }
+  const int tail = head + n * V + threadIdx.x;
+  if (tail < count) {
+    const float x[1] = {to_f32(src[tail])};
+    acc.add(x);
+  }
+}
+
+// dst = src * c over the `count` values of a chunk, by one block.  Vectors where
+// source and destination share their place within a vector (every in-place
+// call), else one value at a time.  Not inlined: nine pairs of types in one
+// kernel body spill.
+template <typename T, typename D>
+__device__ __noinline__ void clip_scale(const T* src, D* dst, int count, float c) {
+  constexpr int V = 16 / (sizeof(T) > sizeof(D) ? sizeof(T) : sizeof(D));   // 16 bytes of the wider type
+  constexpr int U = 4;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(src) % (V * sizeof(T)) / sizeof(T));
+  if (static_cast<int>(reinterpret_cast<uintptr_t>(dst) % (V * sizeof(D)) / sizeof(D)) != off) {
+    for (int i = threadIdx.x; i < count; i += kClipThreads) dst[i] = from_f32<D>(to_f32(src[i]) * c);
+    return;
+  }
+  const int head = min(count, off ? V - off : 0);
+  if (threadIdx.x < head) dst[threadIdx.x] = from_f32<D>(to_f32(src[threadIdx.x]) * c);
+  const int n = (count - head) / V;
+  using Raw = typename Vec<T, V>::Raw;
+  using RawD = typename Vec<D, V>::Raw;
+  const Raw* v = reinterpret_cast<const Raw*>(src + head);
+  RawD* o = reinterpret_cast<RawD*>(dst + head);
+  for (int c0 = threadIdx.x; c0 < n; c0 += kClipThreads * U) {
+    Raw r[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (c0 + i * kClipThreads < n) r[i] = v[c0 + i * kClipThreads];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      if (c0 + i * kClipThreads >= n) continue;
+      float x[V];
+      Vec<T, V>::unpack(r[i], x);
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[j] *= c;
+      o[c0 + i * kClipThreads] = Vec<D, V>::pack(x);
+    }
+  }
+  const int tail = head + n * V + threadIdx.x;
+  if (tail < count) dst[tail] = from_f32<D>(to_f32(src[tail]) * c);
+}
+
+// The entry that holds chunk c.
+template <int CAP>
+__device__ __forceinline__ int clip_entry(const ClipTable<CAP>& t, uint32_t c) {
+  int lo = 0, hi = t.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (t.e[mid].first <= c) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Block b's chunks of `chunks`, with the grid's blocks sharing them evenly.
+__device__ __forceinline__ void clip_run(uint32_t chunks, uint32_t& a, uint32_t& b) {
+  a = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * blockIdx.x / gridDim.x);
+  b = static_cast<uint32_t>(static_cast<uint64_t>(chunks) * (blockIdx.x + 1) / gridDim.x);
+}
+
+template <int CAP, bool INF>
+__global__ void __launch_bounds__(kClipThreads, kClipPerSm)
+    clip_norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* partial) {
+  pdl_wait();
+  pdl_launch_dependents();
+  uint32_t c, end;
+  clip_run(t.chunks, c, end);
+  ClipAcc<INF> acc;
+  if (c < end) {
+    int i = clip_entry(t, c);
+    for (; c < end; ++c) {
+      while (i + 1 < t.count && t.e[i + 1].first <= c) ++i;
+      const ClipEntry& e = t.e[i];
+      const int64_t a = static_cast<int64_t>(c - e.first) * kClipChunk;
+      const int count = static_cast<int>(min(e.n - a, static_cast<int64_t>(kClipChunk)));
+      if (e.src_type == HEXMOE_F32) clip_read(static_cast<const float*>(e.src) + a, count, acc);
+      else if (e.src_type == HEXMOE_F16) clip_read(static_cast<const __half*>(e.src) + a, count, acc);
+      else clip_read(static_cast<const __nv_bfloat16*>(e.src) + a, count, acc);
+    }
+  }
+  __shared__ double part[kClipThreads / 32];
+  if constexpr (INF) acc.sum = static_cast<double>(__uint_as_float(__reduce_max_sync(0xffffffffu, acc.big)));
+  else
+    for (int o = 16; o > 0; o >>= 1) acc.sum += __shfl_xor_sync(0xffffffffu, acc.sum, o);
+  if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = acc.sum;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = part[0];
+    for (int i = 1; i < kClipThreads / 32; ++i) {
+      if constexpr (INF) s = s != s || part[i] <= s ? s : part[i];   // a NaN stays
+      else s += part[i];
+    }
+    partial[blockIdx.x] = s;
+  }
+}
+
+template <int CAP, bool INF>
+__global__ void __launch_bounds__(kClipThreads, kClipPerSm)
+    clip_scale_kernel(const __grid_constant__ ClipTable<CAP> t, const double* partial, int32_t partials,
+                      float max_norm, int32_t copies, float* norm_out) {
+  pdl_wait();
+  __shared__ double part[kClipThreads];
+  double s = 0;
+  for (int i = threadIdx.x; i < partials; i += kClipThreads) {
+    const double v = partial[i];
+    if constexpr (INF) s = s != s || v <= s ? s : v;
+    else s += v;
+  }
+  part[threadIdx.x] = s;
+  __syncthreads();
+#pragma unroll
+  for (int o = kClipThreads / 2; o > 0; o >>= 1) {
+    if (threadIdx.x < o) {
+      const double v = part[threadIdx.x + o];
+      if constexpr (INF) part[threadIdx.x] = part[threadIdx.x] != part[threadIdx.x] || v <= part[threadIdx.x] ? part[threadIdx.x] : v;
+      else part[threadIdx.x] += v;
+    }
+    __syncthreads();
+  }
+  const float norm = static_cast<float>(INF ? part[0] : sqrt(part[0]));
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = norm;
+  float coef = isinf(max_norm) ? 1.f : max_norm / (norm + 1e-6f);
+  if (coef > 1.f) coef = 1.f;                // a NaN stays
+  if (coef == 1.f && !copies) return;        // in place and within the norm: nothing changes
+  uint32_t c0, c;
+  clip_run(t.chunks, c0, c);
+  if (c0 == c) return;
+  int i = clip_entry(t, c - 1);
+  while (c-- > c0) {
+    while (t.e[i].first > c) --i;
+    const ClipEntry& e = t.e[i];
+    if (coef == 1.f && e.dst == e.src) continue;
+    const int64_t a = static_cast<int64_t>(c - e.first) * kClipChunk;
+    const int count = static_cast<int>(min(e.n - a, static_cast<int64_t>(kClipChunk)));
+    auto to = [&](auto* src) {
+      if (e.dst_type == HEXMOE_F32) clip_scale(src, static_cast<float*>(e.dst) + a, count, coef);
+      else if (e.dst_type == HEXMOE_F16) clip_scale(src, static_cast<__half*>(e.dst) + a, count, coef);
+      else clip_scale(src, static_cast<__nv_bfloat16*>(e.dst) + a, count, coef);
+    };
+    if (e.src_type == HEXMOE_F32) to(static_cast<const float*>(e.src) + a);
+    else if (e.src_type == HEXMOE_F16) to(static_cast<const __half*>(e.src) + a);
+    else to(static_cast<const __nv_bfloat16*>(e.src) + a);
+  }
+}
+
+int clip_grid(uint32_t chunks, int sms) {
+  return static_cast<int>(std::max<uint32_t>(1, std::min<uint32_t>(chunks, kClipPerSm * sms)));
+}
+
+template <int CAP, bool INF>
+cudaError_t launch_clip(const std::vector<ClipEntry>& list, double* partial, int sms, float max_norm, bool copies,
+                        float* norm_out, cudaStream_t st) {
+  const size_t groups = std::max<size_t>(1, (list.size() + CAP - 1) / CAP);
+  int32_t partials = 0;
+  ClipTable<CAP> t;
+  auto fill = [&](size_t g) {
+    const size_t a = g * CAP, b = std::min(list.size(), a + CAP);
+    t.count = static_cast<int32_t>(b - a);
+    t.chunks = 0;
+    for (size_t i = a; i < b; ++i) {
+      t.e[i - a] = list[i];
+      t.e[i - a].first = t.chunks;
+      t.chunks += static_cast<uint32_t>((list[i].n + kClipChunk - 1) / kClipChunk);
+    }
+    return clip_grid(t.chunks, sms);
+  };
+  cudaLaunchAttribute attr;
+  for (size_t g = 0; g < groups; ++g) {
+    const int grid = fill(g);
+    const cudaLaunchConfig_t cfg = launch_config(dim3(grid), kClipThreads, st, &attr);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, clip_norm_kernel<CAP, INF>, t, partial + partials);
+    if (e != cudaSuccess) return e;
+    partials += grid;
+  }
+  for (size_t g = groups; g-- > 0;) {   // the table still holds the last group
+    const int grid = g + 1 == groups ? clip_grid(t.chunks, sms) : fill(g);
+    const cudaLaunchConfig_t cfg = launch_config(dim3(grid), kClipThreads, st, &attr);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, clip_scale_kernel<CAP, INF>, t, static_cast<const double*>(partial),
+                                             partials, max_norm, static_cast<int32_t>(copies), g == 0 ? norm_out : nullptr);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+int current_sms(int* sms) {
+  static std::atomic<int> cached[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return report_cuda_error(e, "cudaGetDevice");
+  if (dev < 0 || dev >= 64) return report_error(HEXMOE_E_DEVICE, "device ordinal out of range");
+  if (!cached[dev].load(std::memory_order_relaxed)) {
+    int v = 0;
+    e = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return report_cuda_error(e, "cudaDeviceGetAttribute");
+    cached[dev].store(v, std::memory_order_relaxed);
+  }
+  *sms = cached[dev].load(std::memory_order_relaxed);
+  return HEXMOE_OK;
+}
+
+constexpr int kClipMaxSms = 256;   // what the workspace is sized for
+
+}  // namespace
+}  // namespace hexmoe
+
+using namespace hexmoe;
+
+extern "C" {
+
+int hexmoe_swiglu(const void* h, int32_t dtype, int64_t rows, int32_t inter, int64_t ld_h, const float* row_weights,
+                  void* act, int64_t ld_act, void* stream) {
+  SwigluParams p{};
+  p.h = h; p.weight = row_weights; p.out = act;
+  p.rows = rows; p.ld_h = ld_h; p.ld_out = ld_act; p.inter = inter;
+  return run_swiglu("hexmoe_swiglu", p, dtype, false, stream);
+}
+
+int hexmoe_swiglu_backward(const void* dact, int64_t ld_dact, const void* h, int64_t ld_h, int32_t dtype, int64_t rows,
+                           int32_t inter, const float* row_weights, void* dh, int64_t ld_dh, float* drow_weights,
+                           void* stream) {
+  SwigluParams p{};
+  p.h = h; p.dact = dact; p.weight = row_weights; p.out = dh; p.dweight = drow_weights;
+  p.rows = rows; p.ld_h = ld_h; p.ld_dact = ld_dact; p.ld_out = ld_dh; p.inter = inter;
+  return run_swiglu("hexmoe_swiglu_backward", p, dtype, true, stream);
+}
+
+size_t hexmoe_clip_grad_norm_workspace_bytes(int32_t tensors) {
+  if (tensors < 0) return 0;
+  const size_t groups = tensors <= kClipSmallList ? 1 : (static_cast<size_t>(tensors) + kClipList - 1) / kClipList;
+  return groups * kClipPerSm * kClipMaxSms * sizeof(double);
+}
+
+int hexmoe_clip_grad_norm(int32_t tensors, const void* const* src, const int64_t* counts, const int32_t* src_dtypes,
+                          void* const* dst, const int32_t* dst_dtypes, float max_norm, int32_t inf_norm,
+                          float* norm_out, void* workspace, size_t workspace_bytes, void* stream) {
+  if (tensors < 0) return arg_error("hexmoe_clip_grad_norm: %d tensors", tensors);
+  if (!(max_norm >= 0.f)) return arg_error("hexmoe_clip_grad_norm: max_norm must be at least 0");
+  if (!norm_out || !workspace || (tensors && (!src || !counts || !src_dtypes || (dst && !dst_dtypes))))
+    return arg_error("hexmoe_clip_grad_norm: null pointer");
+  if (reinterpret_cast<uintptr_t>(workspace) % 8 || reinterpret_cast<uintptr_t>(norm_out) % 4)
+    return arg_error("hexmoe_clip_grad_norm: workspace or norm not aligned");
+  const size_t need = hexmoe_clip_grad_norm_workspace_bytes(tensors);
+  if (workspace_bytes < need)
+    return arg_error("hexmoe_clip_grad_norm: workspace %zu bytes < %zu needed", workspace_bytes, need);
+  int sms = 0;
+  if (int rc = current_sms(&sms)) return rc;
+  sms = std::min(sms, kClipMaxSms);
+  try {
+    std::vector<ClipEntry> list;
+    struct Span {
+      uintptr_t a, b;
+      bool written;
+    };
+    std::vector<Span> spans;
+    list.reserve(tensors);
+    spans.reserve(2 * static_cast<size_t>(tensors));
+    bool copies = false;
+    for (int32_t i = 0; i < tensors; ++i) {
+      const int32_t st = src_dtypes[i], dt = dst ? dst_dtypes[i] : st;
+      if (!known_dtype(st) || !known_dtype(dt)) return report_error(HEXMOE_E_DTYPE, "hexmoe_clip_grad_norm: bad dtype");
+      if (counts[i] < 0 || counts[i] > (1ll << 40)) return arg_error("hexmoe_clip_grad_norm: tensor %d has %lld values", i, static_cast<long long>(counts[i]));
+      if (counts[i] == 0) continue;
+      void* d = dst ? dst[i] : const_cast<void*>(src[i]);
+      if (!src[i] || !d) return arg_error("hexmoe_clip_grad_norm: null pointer");
+      const uintptr_t sa = reinterpret_cast<uintptr_t>(src[i]), da = reinterpret_cast<uintptr_t>(d);
+      if (sa % dtype_bytes(st) || da % dtype_bytes(dt)) return arg_error("hexmoe_clip_grad_norm: tensor %d is not aligned to its element", i);
+      list.push_back({src[i], d, counts[i], 0, static_cast<int16_t>(st), static_cast<int16_t>(dt)});
+      spans.push_back({da, da + counts[i] * dtype_bytes(dt), true});
+      if (sa != da) spans.push_back({sa, sa + counts[i] * dtype_bytes(st), false});
+      else if (st != dt) return arg_error("hexmoe_clip_grad_norm: tensor %d is written in place with another dtype", i);
+      copies |= sa != da;
+    }
+    // a value that is written may be reached through one entry only: overlapping
+    // entries would be scaled twice, or read after they were scaled
+    std::sort(spans.begin(), spans.end(), [](const Span& x, const Span& y) { return x.a < y.a; });
+    uintptr_t any_end = 0, written_end = 0;
+    for (const Span& s : spans) {
+      if (s.a < written_end || (s.written && s.a < any_end)) return arg_error("hexmoe_clip_grad_norm: tensors overlap");
+      any_end = std::max(any_end, s.b);
+      if (s.written) written_end = std::max(written_end, s.b);
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    double* partial = static_cast<double*>(workspace);
+    const bool small = tensors <= kClipSmallList;
+    const cudaError_t e =
+        inf_norm ? (small ? launch_clip<kClipSmallList, true>(list, partial, sms, max_norm, copies, norm_out, st)
+                          : launch_clip<kClipList, true>(list, partial, sms, max_norm, copies, norm_out, st))
+                 : (small ? launch_clip<kClipSmallList, false>(list, partial, sms, max_norm, copies, norm_out, st)
+                          : launch_clip<kClipList, false>(list, partial, sms, max_norm, copies, norm_out, st));
+    return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, "hexmoe_clip_grad_norm");
+  } catch (const std::exception&) {
+    return report_error(HEXMOE_E_ARG, "hexmoe_clip_grad_norm: out of host memory");
+  }
+}
+
+}  // extern "C"

@@ -355,6 +355,78 @@ HEXMOE_API int hexmoe_quantize(const float* W, int32_t n, int32_t out, int32_t i
                                uint8_t* block_scale_out, float* expert_scale_out, float* levels_out,
                                void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Training a layer's experts in 16 bits.  No counterpart in the reference's
+ * runtime, which only serves; these are what stands between hexmoe_dequant (the
+ * 16-bit stacks of a layer's experts) and hexmoe_quantize (which takes them back,
+ * with Hessians): the products of routed rows with their experts' matrices and
+ * their gradients, the activation between them, and the clipping of the
+ * gradients.
+ *
+ * Rows lie in expert order: group e is rows offsets[e] .. offsets[e+1]-1 of
+ * `rows`, offsets [experts + 1] in offsets_dtype on the device (1..2048 experts,
+ * any group empty, rows < 2^31 - 512).  Offsets that decrease or leave 0..rows
+ * are clamped (each to at least the one before) and set bit 8 of the device
+ * error word.  Sums are held in fp32 and rounded once; the results do not depend
+ * on the order in which blocks run.  x, w, dy and out must not overlap.
+ * ------------------------------------------------------------------------- */
+
+/* The offsets of a plan (hexmoe_align): offsets[e] = block_m times the number
+ * of its blocks with an expert below e, so that group e holds expert e's run of
+ * plan rows, padding included (none at block_m 1).  expert_ids [max_blocks], npp
+ * [1] as align writes them; offsets int32 [num_experts + 1]. */
+HEXMOE_API int hexmoe_group_offsets(const int32_t* expert_ids, int64_t max_blocks, const int32_t* npp, int32_t block_m,
+                                    int32_t num_experts, int32_t* offsets, void* stream);
+
+/* Products of ragged groups.  w [experts, n, k]: row stride ld_w, stride_w
+ * elements from one expert to the next.  For every row r of group e
+ *   transpose = 0:  out[r, :n] = x[r, :k] W[e]^T
+ *   transpose = 1:  out[r, :k] = x[r, :n] W[e]     (the gradient of the rows)
+ * Rows of no group (before offsets[0], from offsets[experts] on) are set to zero.
+ * x, w: BF16 or F16; out: the same or F32.  Any n, k >= 1 and strides; bases and
+ * strides that are multiples of 16 bytes run on the tensor-memory kernels. */
+HEXMOE_API int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int64_t stride_w,
+                                 int32_t dtype, int64_t rows, int32_t experts, int32_t n, int32_t k, int32_t transpose,
+                                 const void* offsets, int32_t offsets_dtype, void* out, int64_t ld_out,
+                                 int32_t out_dtype, void* stream);
+
+/* Weight gradients out[e] = sum over the rows r of group e of dy[r, :n]^T
+ * x[r, :k], out [experts, n, k] (zero for an empty group); with dy = x the
+ * Hessians x_e^T x_e that GPTQ rounding takes.  accumulate != 0 adds to what out
+ * holds (rounded once, after the addition).  dy, x: BF16 or F16; out: the same or F32. */
+HEXMOE_API int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int32_t dtype,
+                                    int64_t rows, int32_t experts, int32_t n, int32_t k, const void* offsets,
+                                    int32_t offsets_dtype, void* out, int64_t ld_out, int64_t stride_out,
+                                    int32_t out_dtype, int32_t accumulate, void* stream);
+
+/* SwiGLU of rows h = [gate | up] (h [rows, 2 * inter], row stride ld_h):
+ *   act[r, i] = silu(gate[r, i]) * up[r, i] * row_weights[r]
+ * (row_weights [rows] f32, NULL for 1), and its gradient
+ *   dgate = w d up (s + silu (1 - s)), dup = w d silu, drow_weights[r] = sum_i d silu up
+ * with d = dact, s = sigmoid(gate); drow_weights may be NULL.  dh may be h
+ * itself.  All of one dtype (F32, BF16, F16), computed in fp32. */
+HEXMOE_API int hexmoe_swiglu(const void* h, int32_t dtype, int64_t rows, int32_t inter, int64_t ld_h,
+                             const float* row_weights, void* act, int64_t ld_act, void* stream);
+HEXMOE_API int hexmoe_swiglu_backward(const void* dact, int64_t ld_dact, const void* h, int64_t ld_h, int32_t dtype,
+                                      int64_t rows, int32_t inter, const float* row_weights, void* dh, int64_t ld_dh,
+                                      float* drow_weights, void* stream);
+
+/* The norm of all values of a list of tensors (src, counts, src_dtypes: host
+ * arrays of `tensors` entries; contiguous values on the device), and the values
+ * scaled to a largest norm:
+ *   norm_out = sqrt(sum x^2), or max |x| with inf_norm != 0  (f32, on the device)
+ *   dst      = src * min(1, max_norm / (norm_out + 1e-6))
+ * dst = NULL scales in place; otherwise dst / dst_dtypes give every tensor's
+ * destination.  Partial sums are kept in fp64, squares never overflow.  A norm
+ * that is infinite or NaN scales by 0 or NaN; max_norm = infinity scales by 1.
+ * Written tensors must not overlap each other or another entry's source.
+ * workspace: hexmoe_clip_grad_norm_workspace_bytes(tensors), 8-byte aligned. */
+HEXMOE_API size_t hexmoe_clip_grad_norm_workspace_bytes(int32_t tensors);
+HEXMOE_API int hexmoe_clip_grad_norm(int32_t tensors, const void* const* src, const int64_t* counts,
+                                     const int32_t* src_dtypes, void* const* dst, const int32_t* dst_dtypes,
+                                     float max_norm, int32_t inf_norm, float* norm_out, void* workspace,
+                                     size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
