@@ -6,8 +6,13 @@
 #include <cstdio>
 #include <type_traits>
 
+#include <atomic>
+#include <mutex>
+
+#include <cudaTypedefs.h>
+
 #include "internal.cuh"
-#include "ptx.cuh"
+#include "pair.cuh"
 
 namespace hexmoe {
 namespace {
@@ -102,6 +107,15 @@ __device__ __forceinline__ uint16_t round16(float v, bool bf16) {
 }
 __device__ __forceinline__ float widen16(uint16_t v, bool bf16) {
   return bf16 ? __bfloat162float(__ushort_as_bfloat16(v)) : __half2float(__ushort_as_half(v));
+}
+
+__device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
+  if (bf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return reinterpret_cast<const uint32_t&>(v);
+  }
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return reinterpret_cast<const uint32_t&>(v);
 }
 
 // 64 rows x 32 reduction values into registers (16 a thread), zero outside the
@@ -268,6 +282,471 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
   offsets[e] = static_cast<int32_t>(lo * bm);
 }
 
+// ------------------------------------------------------------ tensor-memory kernel
+// Persistent pairs of CTAs over tiles of one group.  Every tile is one 256-row M
+// side by up to 256 N columns of fp32 accumulators in tensor memory (two such
+// accumulators, so that a tile's epilogue runs under the next one's products),
+// fed by a ring of 64-wide reduction steps that TMA fills, 32 KB a CTA and step.
+//   rows (y = x W^T, dx = dy W)  M side: the matrix's output features, N side: the
+//         group's rows.  N is a multiple of 32 chosen per tile, so a group of 341
+//         rows takes two tiles of 192, not two of 256, and a group of 5 rows one
+//         of 32: the weights stream once at full width whatever the group's size.
+//   weight gradient              M side: n, N side: k, reduction over the group's
+//         rows.  The last step of a group zeroes the rows that follow it, in both
+//         operands (they are another group's, and may hold anything).
+// Operand majors: x and dy rows are reduction-major (K) in the row products, as
+// is W for y; W for dx, and both operands of the weight gradient, are stored with
+// the reduction outermost and go to the tensor core as MN-major tiles.
+//
+// 12 warps a CTA: 0 loads, 1 issues the products (the leader's), 2 zeroes tails
+// (weight gradient), 4..11 write results.  Each walks the groups' offsets by
+// itself, so that no size is known on the host.
+constexpr int kStages = 6;
+constexpr int kStepK = 64;
+constexpr uint32_t kOperandBytes = 128 * kStepK * 2;   // one operand's share of a CTA and step
+constexpr uint32_t kChunkBytes = kOperandBytes / 2;    // 64 rows of an MN-major operand
+constexpr int kPairThreads = 384;
+constexpr int kWriters = 8;
+constexpr uint32_t kAccCols = 256;
+constexpr uint32_t kStoreBytes = 4096;                 // a writer's staging tile: 32 lines of 128 B
+constexpr uint32_t kPairSmem = 1024 + kStages * 2 * kOperandBytes + kWriters * kStoreBytes + 1024;
+constexpr int kBoxes = 4;                              // row boxes of 16, 32, 64, 128
+
+enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2 };
+
+struct PairParams {
+  CUtensorMap a;             // W (3-D: reduction or features, ..., expert) or dy
+  CUtensorMap b[kBoxes];     // the rows, by box height; weight gradient: [0] is x
+  CUtensorMap out;           // weight gradient: boxes of 32 rows x 128 B
+  Groups g;
+  int32_t m_len;             // M side: output features / n
+  int32_t n_len;             // weight gradient: k
+  int32_t red;               // row products: reduction length
+  int32_t m_tiles, n_tiles, tile_n;   // n_tiles, tile_n: weight gradient
+  void* dst;
+  int64_t ld, stride_e;
+  int32_t f32, bf16, accumulate, tma_out;
+  int32_t* dev_err;
+};
+
+// One tile: expert, its rows [begin, end), M offset, N offset (a row offset in the
+// row products) and width, real rows.
+struct Tile {
+  int32_t e, m0, n0, width, steps, tail;
+  int64_t row0;
+  int32_t valid;
+};
+
+template <int MODE>
+struct Walker {
+  int32_t base = -32;
+  int64_t carry = 0, lo = 0;
+  int32_t upto = 0, mine = 0, total = 0;
+  int64_t begin = 0, end = 0;
+  bool bad = false;
+
+  __device__ __forceinline__ bool find(const PairParams& p, int32_t tile, Tile& t) {
+    while (tile >= total) {
+      if (base + 32 >= p.g.experts) return false;
+      base += 32;
+      const GroupScan s = scan_groups(p.g, base, carry);
+      bad |= s.bad;
+      begin = s.begin;
+      end = s.end;
+      if (base == 0) lo = __shfl_sync(0xffffffffu, begin, 0);
+      const int lane = threadIdx.x % 32;
+      if constexpr (MODE == kWgrad) mine = base + lane < p.g.experts ? p.m_tiles * p.n_tiles : 0;
+      else mine = static_cast<int32_t>((end - begin + kAccCols - 1) / kAccCols) * p.m_tiles;
+      upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int32_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      upto += total;
+      total = __shfl_sync(0xffffffffu, upto, 31);
+    }
+    const int src = __ffs(__ballot_sync(0xffffffffu, tile < upto)) - 1;
+    const int64_t b = __shfl_sync(0xffffffffu, begin, src), e = __shfl_sync(0xffffffffu, end, src);
+    const int32_t local = tile - __shfl_sync(0xffffffffu, upto - mine, src);
+    t.e = base + src;
+    if constexpr (MODE == kWgrad) {
+      t.m0 = local / p.n_tiles * 256;
+      t.n0 = local % p.n_tiles * p.tile_n;
+      t.width = p.tile_n;
+      t.row0 = b;
+      t.valid = 0;
+      t.steps = static_cast<int32_t>((e - b + kStepK - 1) / kStepK);
+      t.tail = static_cast<int32_t>((e - b) % kStepK);
+    } else {
+      const int32_t size = static_cast<int32_t>(e - b), tiles = (size + 255) / 256;
+      const int32_t width = ((size + tiles - 1) / tiles + 31) / 32 * 32;
+      t.m0 = local / tiles * 256;
+      t.n0 = local % tiles * width;
+      t.width = width;
+      t.row0 = b + t.n0;
+      t.valid = min(width, size - t.n0);
+      t.steps = (p.red + kStepK - 1) / kStepK;
+      t.tail = p.red % kStepK;
+    }
+    return true;
+  }
+};
+
+struct PairCtrl {
+  uint64_t full[kStages], empty[kStages], tail[kStages];
+  uint64_t acc_full[2], acc_empty[2], done;
+  uint32_t tmem;
+  int abort;
+};
+
+template <int MODE>
+__global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
+    grouped_pair_kernel(const __grid_constant__ PairParams p) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* base = raw + (1024 - smem_u32(raw) % 1024) % 1024;
+  uint8_t* ring = base;
+  uint8_t* staging = ring + kStages * 2 * kOperandBytes;
+  PairCtrl* c = reinterpret_cast<PairCtrl*>(staging + kWriters * kStoreBytes);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  volatile int* abort = &c->abort;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&c->full[i], 2);    // one arrival of each CTA
+      mbar_init(&c->empty[i], 1);   // the products' commit
+      mbar_init(&c->tail[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&c->acc_full[i], 1);
+      mbar_init(&c->acc_empty[i], 2 * kWriters);
+    }
+    mbar_init(&c->done, 1);
+    c->abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 2) pair_tmem_alloc(&c->tmem, 512);
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = c->tmem;
+  pdl_wait();
+
+  const int32_t first = blockIdx.x / 2, stride = gridDim.x / 2;
+  Walker<MODE> walk;
+  Tile t;
+  if (warp == 0) {
+    // ---------------------------------------------------------------- loads
+    uint32_t it = 0;
+    bool ok = true;
+    for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
+      if (lane == 0) {
+        const int32_t half = t.width / 2;
+        int box = 0;
+        while (16 << box < half) ++box;
+        const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128;
+        const uint32_t bytes = kOperandBytes + (MODE == kWgrad ? kOperandBytes : (16u << box) * kStepK * 2);
+        for (int32_t s = 0; s < t.steps; ++s, ++it) {
+          const uint32_t st = it % kStages;
+          if (!pair_wait(&c->empty[st], (it / kStages + 1) & 1, abort, p.dev_err)) { ok = false; break; }
+          uint8_t* a = ring + st * 2 * kOperandBytes;
+          uint8_t* b = a + kOperandBytes;
+          // a step whose rows past the group's end are still to be zeroed lands on this CTA's own barrier
+          const bool fix = MODE == kWgrad && s + 1 == t.steps && t.tail % 16 != 0;
+          const uint32_t bar = fix ? peer_addr(&c->tail[st], rank) : peer_addr(&c->full[st], 0);
+          pair_arrive_expect_tx(bar, bytes);
+          if constexpr (MODE == kRowsK) {
+            pair_load_3d(a, &p.a, bar, s * kStepK, m, t.e);
+          } else if constexpr (MODE == kRowsMN) {
+            pair_load_3d(a, &p.a, bar, m, s * kStepK, t.e);
+            pair_load_3d(a + kChunkBytes, &p.a, bar, m + 64, s * kStepK, t.e);
+          } else {
+            const int32_t y = static_cast<int32_t>(t.row0) + s * kStepK;
+            pair_load_2d(a, &p.a, bar, m, y);
+            pair_load_2d(a + kChunkBytes, &p.a, bar, m + 64, y);
+          }
+          if constexpr (MODE == kWgrad) {
+            const int32_t y = static_cast<int32_t>(t.row0) + s * kStepK, x = t.n0 + static_cast<int32_t>(rank) * half;
+            pair_load_2d(b, &p.b[0], bar, x, y);
+            pair_load_2d(b + kChunkBytes, &p.b[0], bar, x + 64, y);
+          } else {
+            pair_load_2d(b, &p.b[box], bar, s * kStepK, static_cast<int32_t>(t.row0) + static_cast<int32_t>(rank) * half);
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+    if (walk.bad && blockIdx.x == 0) atomicOr(p.dev_err, kDevErrOffsets);
+    if (ok && lane == 0) {   // the last steps are released to both CTAs before either leaves
+      for (uint32_t back = 0; back < kStages && back < it; ++back) {
+        const uint32_t j = it - 1 - back;
+        pair_wait(&c->empty[j % kStages], (j / kStages) & 1, abort, p.dev_err);
+      }
+    }
+    if (*abort && lane == 0 && leader) {   // copies of both CTAs still in flight: wait for them, with a limit
+      int ignore = 0;
+      for (uint32_t back = 0; back < kStages && back < it; ++back) {
+        const uint32_t j = it - 1 - back;
+        mbar_wait(&c->full[j % kStages], (j / kStages) & 1, &ignore, p.dev_err);
+      }
+    }
+  } else if (warp == 1 && leader) {
+    // ------------------------------------------------------------- products
+    uint32_t it = 0, n = 0;
+    bool ok = true;
+    for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
+      if (t.steps == 0) continue;   // an empty group's gradient: zeros, without an accumulator
+      if (lane == 0) {
+        const uint32_t buf = n % 2, acc = tmem + buf * kAccCols;
+        const uint32_t idesc = umma_idesc(p.bf16, 256, t.width) | (MODE != kRowsK ? kIdescMajorA : 0) |
+                               (MODE == kWgrad ? kIdescMajorB : 0);
+        ok = pair_wait(&c->acc_empty[buf], (n / 2 + 1) & 1, abort, p.dev_err);
+        tc_fence_after();
+        for (int32_t s = 0; ok && s < t.steps; ++s, ++it) {
+          const uint32_t st = it % kStages;
+          ok = pair_wait(&c->full[st], (it / kStages) & 1, abort, p.dev_err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t a = smem_u32(ring + st * 2 * kOperandBytes), b = a + kOperandBytes;
+          const uint64_t da = MODE == kRowsK ? sw128_desc(a) : sw128_mn_desc(a, kChunkBytes);
+          const uint64_t db = MODE == kWgrad ? sw128_mn_desc(b, kChunkBytes) : sw128_desc(b);
+          const int subs = s + 1 == t.steps && t.tail ? (t.tail + 15) / 16 : kStepK / 16;
+          for (int k = 0; k < subs; ++k)
+            pair_umma_f16(acc, da + k * (MODE == kRowsK ? 2 : 128), db + k * (MODE == kWgrad ? 128 : 2), idesc, s | k);
+          pair_umma_commit(&c->empty[st]);
+        }
+        if (ok) pair_umma_commit(&c->acc_full[buf]);
+      }
+      ++n;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+    }
+    if (*abort && lane == 0) {   // products in flight end before their tensor memory goes
+      int ignore = 0;
+      pair_umma_commit(&c->done);
+      mbar_wait(&c->done, 0, &ignore, p.dev_err);
+    }
+  } else if (warp == 2 && MODE == kWgrad) {
+    // ---------------------------------------------------------------- tails
+    uint32_t it = 0;
+    int uses = 0;   // lane s: how many tails stage s has held
+    bool ok = true;
+    for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
+      it += t.steps;
+      if (t.tail % 16 == 0) continue;
+      const uint32_t st = (it - 1) % kStages;
+      ok = mbar_wait(&c->tail[st], __shfl_sync(0xffffffffu, uses, st) & 1, abort, p.dev_err);
+      ok = __all_sync(0xffffffffu, ok);
+      if (lane == static_cast<int>(st)) ++uses;
+      uint4* a = reinterpret_cast<uint4*>(ring + st * 2 * kOperandBytes);
+      const int zeros = (16 - t.tail % 16) * 8;   // 16-byte pieces in the lines to clear, per 64-row chunk
+      for (int i = lane; ok && i < 4 * zeros; i += 32)
+        a[i / zeros * (kChunkBytes / 16) + t.tail * 8 + i % zeros] = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) pair_arrive(peer_addr(&c->full[st], 0));
+    }
+  } else if (warp >= 4) {
+    // -------------------------------------------------------------- results
+    const int quad = warp % 4, part = (warp - 4) / 4;
+    uint8_t* stage = staging + (warp - 4) * kStoreBytes;
+    uint32_t n = 0;
+    bool ok = true;
+    for (int32_t tile = first; walk.find(p, tile, t); tile += stride) {
+      const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;   // this warp's 32 M rows
+      const uint32_t acc = tmem + (n % 2) * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16);
+      if (t.steps) {
+        ok = __all_sync(0xffffffffu, pair_wait(&c->acc_full[n % 2], (n / 2) & 1, abort, p.dev_err));
+        if (!ok) break;
+        tc_fence_after();
+      }
+      if (m < p.m_len) {
+        if constexpr (MODE != kWgrad) {
+          // lane = feature, column = row of the group: a warp's store is 32 features of one row
+          const int32_t f = m + lane;
+          for (int32_t col = part * 32; col < t.valid; col += 64) {
+            uint32_t r[32];
+            tmem_ld32(acc + col, r);
+            tmem_ld_wait();
+            const int32_t rows = min(32, t.valid - col);
+            if (f < p.m_len) {
+              const int64_t at = (t.row0 + col) * p.ld + f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                if (j >= rows) break;
+                if (p.f32) static_cast<float*>(p.dst)[at + j * p.ld] = __uint_as_float(r[j]);
+                else static_cast<uint16_t*>(p.dst)[at + j * p.ld] = round16(__uint_as_float(r[j]), p.bf16);
+              }
+            }
+            __syncwarp();
+          }
+        } else if (t.steps || !p.accumulate) {
+          // lane = n, column = k: 128-byte lines through shared memory, stored by TMA, which cuts them at
+          // the matrix's edges; outputs that TMA cannot address are written by element
+          const int32_t wide = p.tma_out && !p.f32 ? 64 : 32;
+          for (int32_t col = part * wide; col < t.width && t.n0 + col < p.n_len; col += 2 * wide) {
+            if (p.tma_out) {
+              if (lane == 0) bulk_wait_read();
+              __syncwarp();
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h * 32 >= wide) break;
+              uint32_t r[32];
+              if (t.steps) {
+                tmem_ld32(acc + col + h * 32, r);
+                tmem_ld_wait();
+              } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) r[j] = 0;
+              }
+              if (!p.tma_out) {
+                const int64_t at = t.e * p.stride_e + (m + lane) * p.ld + t.n0 + col;
+                const int32_t left = m + lane < p.m_len ? min(32, p.n_len - t.n0 - col) : 0;
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                  if (j >= left) continue;
+                  float v = __uint_as_float(r[j]);
+                  if (p.f32) {
+                    float* o = static_cast<float*>(p.dst) + at + j;
+                    *o = p.accumulate ? *o + v : v;
+                  } else {
+                    uint16_t* o = static_cast<uint16_t*>(p.dst) + at + j;
+                    if (p.accumulate) v += widen16(*o, p.bf16);
+                    *o = round16(v, p.bf16);
+                  }
+                }
+              } else if (p.f32) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                  *reinterpret_cast<uint4*>(stage + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                      make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+              } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                  uint32_t w[4];
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    w[i] = pack16(__uint_as_float(r[8 * q + 2 * i]), __uint_as_float(r[8 * q + 2 * i + 1]), p.bf16);
+                  *reinterpret_cast<uint4*>(stage + lane * 128 + (((h * 4 + q) ^ (lane & 7)) << 4)) =
+                      make_uint4(w[0], w[1], w[2], w[3]);
+                }
+              }
+            }
+            if (p.tma_out) {
+              fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                if (p.accumulate) tma_add_3d(&p.out, stage, t.n0 + col, m, t.e);
+                else tma_store_3d(&p.out, stage, t.n0 + col, m, t.e);
+                bulk_commit();
+              }
+            }
+          }
+        }
+      }
+      if (t.steps) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) pair_arrive(peer_addr(&c->acc_empty[n % 2], 0));
+        ++n;
+      }
+    }
+    if constexpr (MODE == kWgrad) {
+      if (p.tma_out && lane == 0) bulk_wait_all();
+    } else if (ok) {   // rows of no group
+      const int64_t gap = walk.lo + (p.g.rows - walk.carry);
+      for (int64_t i = blockIdx.x; i < gap; i += gridDim.x) {
+        const int64_t at = (i < walk.lo ? i : i - walk.lo + walk.carry) * p.ld;
+        for (int32_t f = threadIdx.x - 128; f < p.m_len; f += kWriters * 32) {
+          if (p.f32) static_cast<float*>(p.dst)[at + f] = 0.f;
+          else static_cast<uint16_t*>(p.dst)[at + f] = 0;
+        }
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();
+  if (warp == 2) pair_tmem_free(tmem, 512);
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* q = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &q, 12000, cudaEnableDefault, &r) == cudaSuccess &&
+        r == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(q);
+  });
+  return fn;
+}
+
+// [outer][rows][cols] with row pitch and outer stride in bytes (dims = 2 leaves
+// the outer one away), 128-byte swizzle.
+int make_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int dims, uint64_t cols, uint64_t rows,
+             uint64_t outer, uint64_t pitch, uint64_t stride, uint32_t box_cols, uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return report_error(HEXMOE_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t size[3] = {cols, rows, outer}, strides[2] = {pitch, stride};
+  const cuuint32_t box[3] = {box_cols, box_rows, 1}, step[3] = {1, 1, 1};
+  const CUresult r = fn(m, dt, dims, const_cast<void*>(base), size, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return HEXMOE_OK;
+  char buf[96];
+  snprintf(buf, sizeof(buf), "grouped product: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
+  return report_error(HEXMOE_E_CUDA, buf);
+}
+
+// Whether TMA can address a matrix: base and strides in multiples of 16 bytes.
+bool tma_rows(const void* p, int64_t ld, int64_t size) {
+  return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && ld * size < (1ll << 40);
+}
+bool tma_stack(const void* p, int64_t ld, int64_t stride, int64_t size, int32_t count) {
+  return tma_rows(p, ld, size) &&
+         (count == 1 || (stride * size % 16 == 0 && stride >= ld && stride * size < (1ll << 40)));
+}
+
+int sm_count(int* sms) {
+  static std::atomic<int> cached[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return report_cuda_error(e, "cudaGetDevice");
+  if (dev < 0 || dev >= 64) return report_error(HEXMOE_E_DEVICE, "device ordinal out of range");
+  int v = cached[dev].load(std::memory_order_acquire);
+  if (!v) {   // first call on this device: the kernels' shared memory as well
+    for (const void* k : {reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad>)}) {
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
+      if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
+    }
+    e = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return report_cuda_error(e, "cudaDeviceGetAttribute");
+    cached[dev].store(v, std::memory_order_release);
+  }
+  *sms = v;
+  return HEXMOE_OK;
+}
+
+template <int MODE>
+cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(sms / 2, tiles))));
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE>, p);
+}
+
 int check_groups(const char* what, int64_t rows, int32_t experts, const void* offsets, int32_t offsets_dtype) {
   if (offsets_dtype != HEXMOE_I32 && offsets_dtype != HEXMOE_I64) return report_error(HEXMOE_E_DTYPE, "offsets are I32 or I64");
   if (rows < 0 || rows >= (1ll << 31) - 512) return arg_error("%s: %lld rows", what, static_cast<long long>(rows));
@@ -323,8 +802,33 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
     return arg_error("%s: null pointer, or one not aligned to its element", what);
   int32_t* dev_err = device_error_word();
   if (!dev_err) return report_error(HEXMOE_E_CUDA, "device error word unavailable");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const Groups groups = {offsets, offsets_dtype == HEXMOE_I64, experts, rows};
+  if (tma_rows(x, ld_x, 2) && tma_stack(w, ld_w, stride_w, 2, experts)) {
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    PairParams q{};
+    q.g = groups;
+    q.m_len = width_out; q.red = width_in;
+    q.m_tiles = (width_out + 255) / 256;
+    q.dst = out; q.ld = ld_out;
+    q.f32 = out_dtype == HEXMOE_F32; q.bf16 = dtype == HEXMOE_BF16;
+    q.dev_err = dev_err;
+    const int64_t tiles = (rows / 256 + std::min<int64_t>(experts, rows)) * q.m_tiles;
+    if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
+    const CUtensorMapDataType dt = q.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if (int rc = make_map(&q.a, w, dt, 3, k, n, experts, 2 * ld_w, experts == 1 ? 2 * ld_w : 2 * stride_w, 64,
+                          transpose ? 64 : 128))
+      return rc;
+    // box heights up to half the widest tile that these rows can make
+    const int64_t half = (std::min<int64_t>(rows, 256) + 31) / 32 * 16;
+    for (int i = 0; i < kBoxes && (i == 0 || (8 << i) < half); ++i)
+      if (int rc = make_map(&q.b[i], x, dt, 2, width_in, rows, 1, 2 * ld_x, 0, 64, 16u << i)) return rc;
+    const cudaError_t e = transpose ? launch_pair<kRowsMN>(q, tiles, sms, st) : launch_pair<kRowsK>(q, tiles, sms, st);
+    return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
+  }
   PlainParams p{};
-  p.g = {offsets, offsets_dtype == HEXMOE_I64, experts, rows};
+  p.g = groups;
   p.a = static_cast<const uint16_t*>(x); p.a_i = ld_x; p.a_r = 1;
   p.b = static_cast<const uint16_t*>(w); p.b_e = stride_w;
   p.b_j = transpose ? 1 : ld_w; p.b_r = transpose ? ld_w : 1;
@@ -333,7 +837,7 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
   p.j_tiles = (width_out + kPlainTile - 1) / kPlainTile;
   p.dev_err = dev_err;
   const int64_t row_tiles = rows / kPlainTile + std::min<int64_t>(experts, rows);
-  const cudaError_t e = launch_plain(p, false, row_tiles * p.j_tiles, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_plain(p, false, row_tiles * p.j_tiles, st);
   return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
 }
 
@@ -351,8 +855,37 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
     return arg_error("%s: null pointer, or one not aligned to its element", what);
   int32_t* dev_err = device_error_word();
   if (!dev_err) return report_error(HEXMOE_E_CUDA, "device error word unavailable");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const Groups groups = {offsets, offsets_dtype == HEXMOE_I64, experts, rows};
+  if (rows > 0 && tma_rows(dy, ld_dy, 2) && tma_rows(x, ld_x, 2)) {
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    PairParams q{};
+    q.g = groups;
+    q.m_len = n; q.n_len = k;
+    q.m_tiles = (n + 255) / 256;
+    q.n_tiles = (k + 255) / 256;
+    q.tile_n = ((k + q.n_tiles - 1) / q.n_tiles + 63) / 64 * 64;
+    q.dst = out; q.ld = ld_out; q.stride_e = stride_out;
+    q.f32 = out_dtype == HEXMOE_F32; q.bf16 = dtype == HEXMOE_BF16; q.accumulate = accumulate != 0;
+    q.dev_err = dev_err;
+    const int64_t tiles = static_cast<int64_t>(experts) * q.m_tiles * q.n_tiles;
+    if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
+    const CUtensorMapDataType dt = q.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if (int rc = make_map(&q.a, dy, dt, 2, n, rows, 1, 2 * ld_dy, 0, 64, 64)) return rc;
+    if (int rc = make_map(&q.b[0], x, dt, 2, k, rows, 1, 2 * ld_x, 0, 64, 64)) return rc;
+    // a 16-bit sum is rounded once: that of an addition to out cannot be left to TMA, which rounds before and after
+    const int64_t z = q.f32 ? 4 : 2;
+    q.tma_out = tma_stack(out, ld_out, stride_out, z, experts) && (q.f32 || !q.accumulate);
+    if (q.tma_out)
+      if (int rc = make_map(&q.out, out, q.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dt, 3, k, n, experts, z * ld_out,
+                            experts == 1 ? z * ld_out : z * stride_out, q.f32 ? 32 : 64, 32))
+        return rc;
+    const cudaError_t e = launch_pair<kWgrad>(q, tiles, sms, st);
+    return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
+  }
   PlainParams p{};
-  p.g = {offsets, offsets_dtype == HEXMOE_I64, experts, rows};
+  p.g = groups;
   p.a = static_cast<const uint16_t*>(dy); p.a_i = 1; p.a_r = ld_dy;
   p.b = static_cast<const uint16_t*>(x); p.b_j = 1; p.b_r = ld_x;
   p.i_len = n; p.j_len = k;
@@ -362,7 +895,7 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
   p.j_tiles = (k + kPlainTile - 1) / kPlainTile;
   p.dev_err = dev_err;
   const int64_t blocks = static_cast<int64_t>(experts) * p.i_tiles * p.j_tiles;
-  const cudaError_t e = launch_plain(p, true, blocks, static_cast<cudaStream_t>(stream));
+  const cudaError_t e = launch_plain(p, true, blocks, st);
   return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
 }
 

@@ -51,7 +51,7 @@ template <> struct RawOf<2> { using type = uint16_t; };
 template <typename T, int V>
 struct Vec {
   using Raw = typename RawOf<static_cast<int>(sizeof(T)) * V>::type;
-  static constexpr int kWords = sizeof(Raw) < 4 ? 1 : sizeof(Raw) / 4;
+  [[maybe_unused]] static constexpr int kWords = static_cast<int>(sizeof(Raw) / 4);
   static __device__ __forceinline__ void unpack(const Raw& r, float (&x)[V]) {
     if constexpr (V == 1 && sizeof(T) == 2) {
       x[0] = to_f32(reinterpret_cast<const T&>(r));
