@@ -449,7 +449,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         const uint32_t bytes = kOperandBytes + (MODE == kWgrad ? kOperandBytes : (16u << box) * kStepK * 2);
         for (int32_t s = 0; s < t.steps; ++s, ++it) {
           const uint32_t st = it % kStages;
-          if (!pair_wait(&c->empty[st], (it / kStages + 1) & 1, abort, p.dev_err)) { ok = false; break; }
+          if (!mbar_wait(&c->empty[st], (it / kStages + 1) & 1, abort, p.dev_err)) { ok = false; break; }
           uint8_t* a = ring + st * 2 * kOperandBytes;
           uint8_t* b = a + kOperandBytes;
           // a step whose rows past the group's end are still to be zeroed lands on this CTA's own barrier
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     if (ok && lane == 0) {   // the last steps are released to both CTAs before either leaves
       for (uint32_t back = 0; back < kStages && back < it; ++back) {
         const uint32_t j = it - 1 - back;
-        pair_wait(&c->empty[j % kStages], (j / kStages) & 1, abort, p.dev_err);
+        mbar_wait(&c->empty[j % kStages], (j / kStages) & 1, abort, p.dev_err);
       }
     }
     if (*abort && lane == 0 && leader) {   // copies of both CTAs still in flight: wait for them, with a limit
@@ -501,11 +501,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         const uint32_t buf = n % 2, acc = tmem + buf * kAccCols;
         const uint32_t idesc = umma_idesc(p.bf16, 256, t.width) | (MODE != kRowsK ? kIdescMajorA : 0) |
                                (MODE == kWgrad ? kIdescMajorB : 0);
-        ok = pair_wait(&c->acc_empty[buf], (n / 2 + 1) & 1, abort, p.dev_err);
+        ok = mbar_wait(&c->acc_empty[buf], (n / 2 + 1) & 1, abort, p.dev_err);
         tc_fence_after();
         for (int32_t s = 0; ok && s < t.steps; ++s, ++it) {
           const uint32_t st = it % kStages;
-          ok = pair_wait(&c->full[st], (it / kStages) & 1, abort, p.dev_err);
+          ok = MODE == kWgrad && s + 1 == t.steps && t.tail % 16   // both CTAs' zeroed rows
+                   ? pair_wait(&c->full[st], (it / kStages) & 1, abort, p.dev_err)
+                   : mbar_wait(&c->full[st], (it / kStages) & 1, abort, p.dev_err);
           if (!ok) break;
           tc_fence_after();
           const uint32_t a = smem_u32(ring + st * 2 * kOperandBytes), b = a + kOperandBytes;
@@ -544,7 +546,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         a[i / zeros * (kChunkBytes / 16) + t.tail * 8 + i % zeros] = make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) pair_arrive(peer_addr(&c->full[st], 0));
+      if (lane == 0) pair_arrive_release(peer_addr(&c->full[st], 0));
     }
   } else if (warp >= 4) {
     // -------------------------------------------------------------- results
@@ -556,7 +558,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;   // this warp's 32 M rows
       const uint32_t acc = tmem + (n % 2) * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16);
       if (t.steps) {
-        ok = __all_sync(0xffffffffu, pair_wait(&c->acc_full[n % 2], (n / 2) & 1, abort, p.dev_err));
+        ok = __all_sync(0xffffffffu, mbar_wait(&c->acc_full[n % 2], (n / 2) & 1, abort, p.dev_err));
         if (!ok) break;
         tc_fence_after();
       }
