@@ -20,31 +20,32 @@ inputs' device, synchronise nothing and can be captured in CUDA graphs.
 
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
 
 import torch
 
 from blackhole_b200 import _lib
-from blackhole_b200.hex_moe import _DT, _aligned, _ptr, _stream, align, combine_rows
+from blackhole_b200.hex_moe import _DT, _aligned, _ptr, align, combine_rows
 
 _16BIT = (torch.bfloat16, torch.float16)
 _INDEX = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 
 
-class _On:
-    """torch.cuda.device(dev), at no cost where dev is current already."""
+_raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream() without building a Stream object
 
-    def __init__(self, dev: torch.device):
-        self.guard = None if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *args):
-        if self.guard is not None:
-            self.guard.__exit__(*args)
+def _run(name: str, dev: torch.device, *args) -> None:
+    """One C call on dev's current stream (with dev current), its status raised as an exception."""
+    fn = getattr(_lib.lib, name)
+    index = dev.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _rows2d(t: torch.Tensor, what: str) -> torch.Tensor:
@@ -110,12 +111,8 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, transpos
     res = _output(out, (R, K if transpose else N), x.dtype, out_dtype, x.device, "grouped_mm")
     to = res if res.stride(1) == 1 and res.stride(0) >= res.shape[1] else torch.empty_like(
         res, memory_format=torch.contiguous_format)
-    with _On(x.device):
-        rc = _lib.lib.hexmoe_grouped_mm(_ptr(x), x.stride(0), _ptr(w), w.stride(1), w.stride(0), _DT[x.dtype], R, E, N,
-                                        K, transpose, _ptr(offsets), _INDEX[offsets.dtype], _ptr(to), to.stride(0),
-                                        _DT[to.dtype], _stream(x.device))
-    if rc:
-        _lib.check(rc, "hexmoe_grouped_mm")
+    _run("hexmoe_grouped_mm", x.device, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(1), w.stride(0), _DT[x.dtype],
+         R, E, N, K, transpose, offsets.data_ptr(), _INDEX[offsets.dtype], to.data_ptr(), to.stride(0), _DT[to.dtype])
     return res if to is res else res.copy_(to)
 
 
@@ -142,12 +139,9 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out_
         to = res.contiguous()
     else:
         to = torch.empty_like(res, memory_format=torch.contiguous_format)
-    with _On(x.device):
-        rc = _lib.lib.hexmoe_grouped_wgrad(_ptr(dy), dy.stride(0), _ptr(x), x.stride(0), _DT[x.dtype], R, E, N, K,
-                                           _ptr(offsets), _INDEX[offsets.dtype], _ptr(to), to.stride(1), to.stride(0),
-                                           _DT[to.dtype], accumulate, _stream(x.device))
-    if rc:
-        _lib.check(rc, "hexmoe_grouped_wgrad")
+    _run("hexmoe_grouped_wgrad", x.device, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), _DT[x.dtype], R, E, N,
+         K, offsets.data_ptr(), _INDEX[offsets.dtype], to.data_ptr(), to.stride(1), to.stride(0), _DT[to.dtype],
+         accumulate)
     return res if to is res else res.copy_(to)
 
 
@@ -171,11 +165,8 @@ def swiglu(h: torch.Tensor, row_weights: torch.Tensor | None = None) -> torch.Te
         raise ValueError(f"h must be [R, 2 * I], got {tuple(h.shape)}")
     row_weights = _check_row_weights(row_weights, R, h.device)
     act = torch.empty(R, width // 2, dtype=h.dtype, device=h.device)
-    with _On(h.device):
-        rc = _lib.lib.hexmoe_swiglu(_ptr(h), _DT[h.dtype], R, width // 2, h.stride(0), _ptr(row_weights), _ptr(act),
-                                    width // 2, _stream(h.device))
-    if rc:
-        _lib.check(rc, "hexmoe_swiglu")
+    _run("hexmoe_swiglu", h.device, h.data_ptr(), _DT[h.dtype], R, width // 2, h.stride(0), _ptr(row_weights),
+         act.data_ptr(), width // 2)
     return act
 
 
@@ -197,11 +188,8 @@ def swiglu_backward(dact: torch.Tensor, h: torch.Tensor, row_weights: torch.Tens
     h, dact = _rows2d(h, "h"), _rows2d(dact, "dact")
     dh = torch.empty(R, 2 * I, dtype=h.dtype, device=h.device) if out is None else out
     dw = None if row_weights is None else torch.empty(R, dtype=torch.float32, device=h.device)
-    with _On(h.device):
-        rc = _lib.lib.hexmoe_swiglu_backward(_ptr(dact), dact.stride(0), _ptr(h), h.stride(0), _DT[h.dtype], R, I,
-                                             _ptr(row_weights), _ptr(dh), dh.stride(0), _ptr(dw), _stream(h.device))
-    if rc:
-        _lib.check(rc, "hexmoe_swiglu_backward")
+    _run("hexmoe_swiglu_backward", h.device, dact.data_ptr(), dact.stride(0), h.data_ptr(), h.stride(0), _DT[h.dtype], R,
+         I, _ptr(row_weights), dh.data_ptr(), dh.stride(0), _ptr(dw))
     return dh, dw
 
 
@@ -246,12 +234,8 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
         raise ValueError(f"max_norm must be at least 0, got {max_norm}")
     if out is not None:
         out = [out] if isinstance(out, torch.Tensor) else list(out)
-        if len(out) != len(grads):
-            raise ValueError(f"out holds {len(out)} tensors, grads {len(grads)}")
-        for g, o in zip(grads, out):
-            if (g is None) != (o is None) or g is not None and (
-                    o.shape != g.shape or o.stride() != g.stride() or o.device != g.device):
-                raise ValueError("every tensor of out must have its gradient's shape, strides and device")
+        if len(out) != len(grads) or any((g is None) != (o is None) for g, o in zip(grads, out)):
+            raise ValueError("out must hold a tensor for every gradient")
         out = [o for o in out if o is not None]
     grads = [g for g in grads if g is not None]
     if not grads:
@@ -259,10 +243,14 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     dev = grads[0].device
     if dev.type != "cuda":
         raise ValueError("clip_grad_norm runs on CUDA only")
-    for g in grads:
-        if g.device != dev:
-            raise ValueError(f"clip_grad_norm: tensors on {dev} and {g.device}")
-    if not all(map(_dense, grads)):
+    held = grads if out is None else grads + out
+    if {t.get_device() for t in held} != {dev.index}:
+        raise ValueError(f"clip_grad_norm: not every tensor is on {dev}")
+    if out is not None and [g.shape for g in grads] != [o.shape for o in out]:
+        raise ValueError("every tensor of out must have its gradient's shape")
+    if not all([t.is_contiguous() for t in held]):
+        if out is not None and [g.stride() for g in grads] != [o.stride() for o in out]:
+            raise ValueError("every tensor of out must have its gradient's strides")
         grads = [r for g in grads for r in _runs(g)]
         if len(grads) > _CLIP_RUNS:
             raise ValueError(f"clip_grad_norm: the tensors fall into {len(grads)} runs of memory (at most {_CLIP_RUNS})")
@@ -270,21 +258,18 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
             out = [r for o in out for r in _runs(o)]
     n = len(grads)
     try:
-        types = [_DT[g.dtype] for g in grads]
-        out_types = None if out is None else [_DT[o.dtype] for o in out]
+        types = array("i", [_DT[g.dtype] for g in grads])
+        out_types = None if out is None else array("i", [_DT[o.dtype] for o in out])
     except KeyError as e:
         raise ValueError(f"clip_grad_norm: unsupported dtype {e.args[0]}") from None
-    ptrs, i32 = ctypes.c_void_p * n, ctypes.c_int32 * n
+    ptrs, counts = array("Q", [g.data_ptr() for g in grads]), array("q", [g.numel() for g in grads])
+    out_ptrs = None if out is None else array("Q", [o.data_ptr() for o in out])
     norm = torch.empty((), dtype=torch.float32, device=dev)
     nbytes = _lib.lib.hexmoe_clip_grad_norm_workspace_bytes(n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    with _On(dev):
-        rc = _lib.lib.hexmoe_clip_grad_norm(
-            n, ptrs(*[g.data_ptr() for g in grads]), (ctypes.c_int64 * n)(*[g.numel() for g in grads]), i32(*types),
-            None if out is None else ptrs(*[o.data_ptr() for o in out]), None if out is None else i32(*out_types),
-            max_norm, norm_type == math.inf, _ptr(norm), _ptr(ws), nbytes, _stream(dev))
-    if rc:
-        _lib.check(rc, "hexmoe_clip_grad_norm")
+    at = lambda a: None if a is None else a.buffer_info()[0]  # noqa: E731
+    _run("hexmoe_clip_grad_norm", dev, n, at(ptrs), at(counts), at(types), at(out_ptrs), at(out_types), max_norm,
+         norm_type == math.inf, norm.data_ptr(), ws.data_ptr(), nbytes)
     return norm
 
 
@@ -297,10 +282,7 @@ def expert_plan(topk_ids: torch.Tensor, num_experts: int) -> tuple[torch.Tensor,
     sid, eid, npp = align(topk_ids.reshape(-1), num_experts, 1)
     S, dev = topk_ids.numel(), sid.device
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-    with _On(dev):
-        rc = _lib.lib.hexmoe_group_offsets(_ptr(eid), eid.numel(), _ptr(npp), 1, num_experts, _ptr(offsets),
-                                           _stream(dev))
-    _lib.check(rc, "hexmoe_group_offsets")
+    _run("hexmoe_group_offsets", dev, _ptr(eid), eid.numel(), _ptr(npp), 1, num_experts, _ptr(offsets))
     rows = torch.full((S + 1,), -1, dtype=torch.int32, device=dev)
     rows[sid.long()] = torch.arange(sid.numel(), dtype=torch.int32, device=dev)
     return offsets, sid, rows[:S], (sid, eid, npp)
@@ -312,10 +294,8 @@ def _gather(x: torch.Tensor, topk: int, num_experts: int, plan: tuple) -> torch.
     sid, _, npp = plan
     x = _aligned(x)
     xs = torch.empty(sid.numel(), x.shape[1], dtype=x.dtype, device=x.device)
-    with _On(x.device):
-        rc = _lib.lib.hexmoe_gather(_ptr(x), _DT[x.dtype], x.shape[0], x.shape[1], topk, num_experts, _ptr(sid),
-                                    _ptr(npp), 1, _ptr(xs), _stream(x.device))
-    _lib.check(rc, "hexmoe_gather")
+    _run("hexmoe_gather", x.device, _ptr(x), _DT[x.dtype], x.shape[0], x.shape[1], topk, num_experts, _ptr(sid), _ptr(npp),
+         1, _ptr(xs))
     return xs
 
 

@@ -438,23 +438,22 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   Tile t;
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
-    uint32_t it = 0;
+    uint32_t it = 0, st = 0, phase = 1;
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
-      if (lane == 0) {
-        const int32_t half = t.width / 2;
-        int box = 0;
-        while (16 << box < half) ++box;
-        const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128;
-        const uint32_t bytes = kOperandBytes + (MODE == kWgrad ? kOperandBytes : (16u << box) * kStepK * 2);
-        for (int32_t s = 0; s < t.steps; ++s, ++it) {
-          const uint32_t st = it % kStages;
-          if (!mbar_wait(&c->empty[st], (it / kStages + 1) & 1, abort, p.dev_err)) { ok = false; break; }
-          uint8_t* a = ring + st * 2 * kOperandBytes;
-          uint8_t* b = a + kOperandBytes;
-          // a step whose rows past the group's end are still to be zeroed lands on this CTA's own barrier
-          const bool fix = MODE == kWgrad && s + 1 == t.steps && t.tail % 16 != 0;
-          const uint32_t bar = fix ? peer_addr(&c->tail[st], rank) : peer_addr(&c->full[st], 0);
+      const int32_t half = t.width / 2;
+      int box = 0;
+      while (16 << box < half) ++box;
+      const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128;
+      const uint32_t bytes = kOperandBytes + (MODE == kWgrad ? kOperandBytes : (16u << box) * kStepK * 2);
+      for (int32_t s = 0; s < t.steps; ++s, ++it) {
+        if (!mbar_wait(&c->empty[st], phase, abort, p.dev_err)) { ok = false; break; }
+        uint8_t* a = ring + st * 2 * kOperandBytes;
+        uint8_t* b = a + kOperandBytes;
+        // a step whose rows past the group's end are still to be zeroed lands on this CTA's own barrier
+        const bool fix = MODE == kWgrad && s + 1 == t.steps && t.tail % 16 != 0;
+        const uint32_t bar = fix ? peer_addr(&c->tail[st], rank) : peer_addr(&c->full[st], 0);
+        if (elect_one()) {
           pair_arrive_expect_tx(bar, bytes);
           if constexpr (MODE == kRowsK) {
             pair_load_3d(a, &p.a, bar, s * kStepK, m, t.e);
@@ -474,8 +473,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             pair_load_2d(b, &p.b[box], bar, s * kStepK, static_cast<int32_t>(t.row0) + static_cast<int32_t>(rank) * half);
           }
         }
+        __syncwarp();
+        if (++st == kStages) { st = 0; phase ^= 1; }
       }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = __all_sync(0xffffffffu, ok);
     }
     if (walk.bad && blockIdx.x == 0) atomicOr(p.dev_err, kDevErrOffsets);
     if (ok && lane == 0) {   // the last steps are released to both CTAs before either leaves
@@ -493,35 +494,39 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     }
   } else if (warp == 1 && leader) {
     // ------------------------------------------------------------- products
-    uint32_t it = 0, n = 0;
+    uint32_t n = 0, st = 0, phase = 0;
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
       if (t.steps == 0) continue;   // an empty group's gradient: zeros, without an accumulator
-      if (lane == 0) {
-        const uint32_t buf = n % 2, acc = tmem + buf * kAccCols;
-        const uint32_t idesc = umma_idesc(p.bf16, 256, t.width) | (MODE != kRowsK ? kIdescMajorA : 0) |
-                               (MODE == kWgrad ? kIdescMajorB : 0);
-        ok = mbar_wait(&c->acc_empty[buf], (n / 2 + 1) & 1, abort, p.dev_err);
+      const uint32_t buf = n % 2, acc = tmem + buf * kAccCols;
+      const uint32_t idesc = umma_idesc(p.bf16, 256, t.width) | (MODE != kRowsK ? kIdescMajorA : 0) |
+                             (MODE == kWgrad ? kIdescMajorB : 0);
+      ok = mbar_wait(&c->acc_empty[buf], (n / 2 + 1) & 1, abort, p.dev_err);
+      for (int32_t s = 0; ok && s < t.steps; ++s) {
+        const bool last = s + 1 == t.steps;
+        ok = MODE == kWgrad && last && t.tail % 16   // both CTAs' zeroed rows
+                 ? pair_wait(&c->full[st], phase, abort, p.dev_err)
+                 : mbar_wait(&c->full[st], phase, abort, p.dev_err);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         tc_fence_after();
-        for (int32_t s = 0; ok && s < t.steps; ++s, ++it) {
-          const uint32_t st = it % kStages;
-          ok = MODE == kWgrad && s + 1 == t.steps && t.tail % 16   // both CTAs' zeroed rows
-                   ? pair_wait(&c->full[st], (it / kStages) & 1, abort, p.dev_err)
-                   : mbar_wait(&c->full[st], (it / kStages) & 1, abort, p.dev_err);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t a = smem_u32(ring + st * 2 * kOperandBytes), b = a + kOperandBytes;
-          const uint64_t da = MODE == kRowsK ? sw128_desc(a) : sw128_mn_desc(a, kChunkBytes);
-          const uint64_t db = MODE == kWgrad ? sw128_mn_desc(b, kChunkBytes) : sw128_desc(b);
-          const int subs = s + 1 == t.steps && t.tail ? (t.tail + 15) / 16 : kStepK / 16;
-          for (int k = 0; k < subs; ++k)
-            pair_umma_f16(acc, da + k * (MODE == kRowsK ? 2 : 128), db + k * (MODE == kWgrad ? 128 : 2), idesc, s | k);
+        const uint32_t a = smem_u32(ring + st * 2 * kOperandBytes), b = a + kOperandBytes;
+        const uint64_t da = MODE == kRowsK ? sw128_desc(a) : sw128_mn_desc(a, kChunkBytes);
+        const uint64_t db = MODE == kWgrad ? sw128_mn_desc(b, kChunkBytes) : sw128_desc(b);
+        const int subs = last && t.tail ? (t.tail + 15) / 16 : kStepK / 16;
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < kStepK / 16; ++k)
+            if (k < subs)
+              pair_umma_f16(acc, da + k * (MODE == kRowsK ? 2 : 128), db + k * (MODE == kWgrad ? 128 : 2), idesc, s | k);
           pair_umma_commit(&c->empty[st]);
+          if (last) pair_umma_commit(&c->acc_full[buf]);
         }
-        if (ok) pair_umma_commit(&c->acc_full[buf]);
+        __syncwarp();
+        if (++st == kStages) { st = 0; phase ^= 1; }
       }
       ++n;
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = __all_sync(0xffffffffu, ok);
     }
     if (*abort && lane == 0) {   // products in flight end before their tensor memory goes
       int ignore = 0;

@@ -7,6 +7,18 @@
 
 namespace hexmoe {
 
+// True in one lane of a converged warp.  tcgen05 and TMA instructions take their
+// operands from uniform registers: behind this test the compiler knows that one
+// lane runs, where behind `lane == 0` it guards every one of them.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
