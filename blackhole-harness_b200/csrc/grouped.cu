@@ -118,6 +118,39 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi, bool bf16) {
   return reinterpret_cast<const uint32_t&>(v);
 }
 
+// fp32 bits rounded to 16: pairs into one word each (the first half of r), or each
+// into its own.  One branch on the type, none per value.
+template <int N>
+__device__ __forceinline__ void pack_pairs(uint32_t (&r)[N], bool bf16) {
+  if (bf16) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) r[i] = pack16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) r[i] = pack16(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]), false);
+  }
+}
+__device__ __forceinline__ void pack_each(uint32_t (&r)[32], bool bf16) {
+  if (bf16) {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = round16(__uint_as_float(r[i]), true);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 32; ++i) r[i] = round16(__uint_as_float(r[i]), false);
+  }
+}
+// The first `count` (all from 8 on, none below 1) of 8 16-bit values.
+__device__ __forceinline__ void store_8(uint16_t* dst, const uint4& v, int count) {
+  if (count >= 8) {
+    *reinterpret_cast<uint4*>(dst) = v;
+    return;
+  }
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < count) dst[i] = static_cast<uint16_t>(w[i / 2] >> (i % 2 * 16));
+}
+
 // 64 rows x 32 reduction values into registers (16 a thread), zero outside the
 // given extents; consecutive threads walk the dimension of unit stride.
 __device__ __forceinline__ void plain_fetch(uint16_t (&v)[16], const uint16_t* base, int64_t s_i, int64_t s_r,
@@ -301,15 +334,16 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 // 12 warps a CTA: 0 loads, 1 issues the products (the leader's), 2 zeroes tails
 // (weight gradient), 4..11 write results.  Each walks the groups' offsets by
 // itself, so that no size is known on the host.
-constexpr int kStages = 6;
+constexpr int kMaxStages = 6;
 constexpr int kStepK = 64;
 constexpr uint32_t kOperandBytes = 128 * kStepK * 2;   // one operand's share of a CTA and step
 constexpr uint32_t kChunkBytes = kOperandBytes / 2;    // 64 rows of an MN-major operand
 constexpr int kPairThreads = 384;
 constexpr int kWriters = 8;
 constexpr uint32_t kAccCols = 256;
-constexpr uint32_t kStoreBytes = 4096;                 // a writer's staging tile: 32 lines of 128 B
-constexpr uint32_t kPairSmem = 1024 + kStages * 2 * kOperandBytes + kWriters * kStoreBytes + 1024;
+constexpr uint32_t kStoreBytes = 2048;                 // a staging tile: 32 lines of 64 B, two for each writer
+constexpr uint32_t kRingBytes = 12 * kOperandBytes;    // 6 steps of A and B, or 4 of A and two Bs
+constexpr uint32_t kPairSmem = 1024 + kRingBytes + 2 * kWriters * kStoreBytes + 1024;
 constexpr int kBoxes = 4;                              // row boxes of 16, 32, 64, 128
 
 enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2 };
@@ -317,7 +351,7 @@ enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2 };
 struct PairParams {
   CUtensorMap a;             // W (3-D: reduction or features, ..., expert) or dy
   CUtensorMap b[kBoxes];     // the rows, by box height; weight gradient: [0] is x
-  CUtensorMap out;           // weight gradient: boxes of 32 rows x 128 B
+  CUtensorMap out;           // boxes of 32 rows x 64 B
   Groups g;
   int32_t m_len;             // M side: output features / n
   int32_t n_len;             // weight gradient: k
@@ -329,16 +363,18 @@ struct PairParams {
   int32_t* dev_err;
 };
 
-// One tile: expert, its rows [begin, end), M offset, N offset (a row offset in the
-// row products) and width, real rows.
+// One tile: expert, M offset, N offset (a row offset within the group in the row
+// products) and width, of `parts` accumulators side by side; row0 its first row,
+// valid its real rows; steps of the reduction, the last one of `tail` (0: full).
 struct Tile {
-  int32_t e, m0, n0, width, steps, tail;
+  int32_t e, m0, n0, width, parts, steps, tail;
   int64_t row0;
   int32_t valid;
 };
 
-template <int MODE>
+template <int MODE, bool WIDE>
 struct Walker {
+  static constexpr int32_t kSpan = WIDE ? 512 : 256;   // most rows of a tile
   int32_t base = -32;
   int64_t carry = 0, lo = 0;
   int32_t upto = 0, mine = 0, total = 0;
@@ -356,7 +392,7 @@ struct Walker {
       if (base == 0) lo = __shfl_sync(0xffffffffu, begin, 0);
       const int lane = threadIdx.x % 32;
       if constexpr (MODE == kWgrad) mine = base + lane < p.g.experts ? p.m_tiles * p.n_tiles : 0;
-      else mine = static_cast<int32_t>((end - begin + kAccCols - 1) / kAccCols) * p.m_tiles;
+      else mine = static_cast<int32_t>((end - begin + kSpan - 1) / kSpan) * p.m_tiles;
       upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -374,18 +410,20 @@ struct Walker {
       t.m0 = local / p.n_tiles * 256;
       t.n0 = local % p.n_tiles * p.tile_n;
       t.width = p.tile_n;
+      t.parts = 1;
       t.row0 = b;
       t.valid = 0;
       t.steps = static_cast<int32_t>((e - b + kStepK - 1) / kStepK);
       t.tail = static_cast<int32_t>((e - b) % kStepK);
     } else {
-      const int32_t size = static_cast<int32_t>(e - b), tiles = (size + 255) / 256;
-      const int32_t width = ((size + tiles - 1) / tiles + 31) / 32 * 32;
+      const int32_t size = static_cast<int32_t>(e - b), tiles = (size + kSpan - 1) / kSpan;
+      const int32_t span = (size + tiles - 1) / tiles;
+      t.parts = WIDE && span > 256 ? 2 : 1;
+      t.width = ((span + t.parts - 1) / t.parts + 31) / 32 * 32;
       t.m0 = local / tiles * 256;
-      t.n0 = local % tiles * width;
-      t.width = width;
+      t.n0 = local % tiles * t.parts * t.width;
       t.row0 = b + t.n0;
-      t.valid = min(width, size - t.n0);
+      t.valid = min(t.parts * t.width, size - t.n0);
       t.steps = (p.red + kStepK - 1) / kStepK;
       t.tail = p.red % kStepK;
     }
@@ -394,26 +432,27 @@ struct Walker {
 };
 
 struct PairCtrl {
-  uint64_t full[kStages], empty[kStages], tail[kStages];
+  uint64_t full[kMaxStages], empty[kMaxStages], tail[kMaxStages];
   uint64_t acc_full[2], acc_empty[2], done;
   uint32_t tmem;
   int abort;
 };
 
-template <int MODE>
+template <int MODE, bool WIDE>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     grouped_pair_kernel(const __grid_constant__ PairParams p) {
+  constexpr uint32_t kStages = WIDE ? 4 : 6, kStageBytes = (WIDE ? 3 : 2) * kOperandBytes;
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (1024 - smem_u32(raw) % 1024) % 1024;
   uint8_t* ring = base;
-  uint8_t* staging = ring + kStages * 2 * kOperandBytes;
-  PairCtrl* c = reinterpret_cast<PairCtrl*>(staging + kWriters * kStoreBytes);
+  uint8_t* staging = ring + kRingBytes;
+  PairCtrl* c = reinterpret_cast<PairCtrl*>(staging + 2 * kWriters * kStoreBytes);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
   volatile int* abort = &c->abort;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
+    for (int i = 0; i < kMaxStages; ++i) {
       mbar_init(&c->full[i], 2);    // one arrival of each CTA
       mbar_init(&c->empty[i], 1);   // the products' commit
       mbar_init(&c->tail[i], 1);
@@ -434,7 +473,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   pdl_wait();
 
   const int32_t first = blockIdx.x / 2, stride = gridDim.x / 2;
-  Walker<MODE> walk;
+  Walker<MODE, WIDE> walk;
   Tile t;
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
@@ -442,13 +481,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
       const int32_t half = t.width / 2;
-      int box = 0;
-      while (16 << box < half) ++box;
       const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128;
-      const uint32_t bytes = kOperandBytes + (MODE == kWgrad ? kOperandBytes : (16u << box) * kStepK * 2);
+      const uint32_t bytes =
+          kOperandBytes + (MODE == kWgrad ? kOperandBytes : static_cast<uint32_t>(t.parts * half) * kStepK * 2);
       for (int32_t s = 0; s < t.steps; ++s, ++it) {
         if (!mbar_wait(&c->empty[st], phase, abort, p.dev_err)) { ok = false; break; }
-        uint8_t* a = ring + st * 2 * kOperandBytes;
+        uint8_t* a = ring + st * kStageBytes;
         uint8_t* b = a + kOperandBytes;
         // a step whose rows past the group's end are still to be zeroed lands on this CTA's own barrier
         const bool fix = MODE == kWgrad && s + 1 == t.steps && t.tail % 16 != 0;
@@ -470,7 +508,20 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             pair_load_2d(b, &p.b[0], bar, x, y);
             pair_load_2d(b + kChunkBytes, &p.b[0], bar, x + 64, y);
           } else {
-            pair_load_2d(b, &p.b[box], bar, s * kStepK, static_cast<int32_t>(t.row0) + static_cast<int32_t>(rank) * half);
+#pragma unroll
+            for (int part = 0; part < (WIDE ? 2 : 1); ++part) {
+              if (part >= t.parts) break;
+              uint8_t* to = b + part * kOperandBytes;
+              int32_t y = static_cast<int32_t>(t.row0) + part * t.width + static_cast<int32_t>(rank) * half;
+#pragma unroll
+              for (int i = kBoxes - 1; i >= 0; --i) {   // the rows' number in boxes of 128, 64, 32, 16
+                if (half & (16 << i)) {
+                  pair_load_2d(to, &p.b[i], bar, s * kStepK, y);
+                  to += (16 << i) * kStepK * 2;
+                  y += 16 << i;
+                }
+              }
+            }
           }
         }
         __syncwarp();
@@ -498,34 +549,37 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
       if (t.steps == 0) continue;   // an empty group's gradient: zeros, without an accumulator
-      const uint32_t buf = n % 2, acc = tmem + buf * kAccCols;
       const uint32_t idesc = umma_idesc(p.bf16, 256, t.width) | (MODE != kRowsK ? kIdescMajorA : 0) |
                              (MODE == kWgrad ? kIdescMajorB : 0);
-      ok = mbar_wait(&c->acc_empty[buf], (n / 2 + 1) & 1, abort, p.dev_err);
       for (int32_t s = 0; ok && s < t.steps; ++s) {
         const bool last = s + 1 == t.steps;
-        ok = MODE == kWgrad && last && t.tail % 16   // both CTAs' zeroed rows
-                 ? pair_wait(&c->full[st], phase, abort, p.dev_err)
-                 : mbar_wait(&c->full[st], phase, abort, p.dev_err);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        const uint32_t a = smem_u32(ring + st * 2 * kOperandBytes), b = a + kOperandBytes;
+        ok = mbar_wait(&c->full[st], phase, abort, p.dev_err);
+        const uint32_t a = smem_u32(ring + st * kStageBytes);
         const uint64_t da = MODE == kRowsK ? sw128_desc(a) : sw128_mn_desc(a, kChunkBytes);
-        const uint64_t db = MODE == kWgrad ? sw128_mn_desc(b, kChunkBytes) : sw128_desc(b);
         const int subs = last && t.tail ? (t.tail + 15) / 16 : kStepK / 16;
-        if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < kStepK / 16; ++k)
-            if (k < subs)
-              pair_umma_f16(acc, da + k * (MODE == kRowsK ? 2 : 128), db + k * (MODE == kWgrad ? 128 : 2), idesc, s | k);
-          pair_umma_commit(&c->empty[st]);
-          if (last) pair_umma_commit(&c->acc_full[buf]);
+        for (int part = 0; part < (WIDE ? 2 : 1); ++part) {
+          if (part >= t.parts) break;
+          const uint32_t buf = (n + part) % 2, acc = tmem + buf * kAccCols;
+          if (s == 0) ok = ok && mbar_wait(&c->acc_empty[buf], ((n + part) / 2 + 1) & 1, abort, p.dev_err);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t b = a + (1 + part) * kOperandBytes;
+          const uint64_t db = MODE == kWgrad ? sw128_mn_desc(b, kChunkBytes) : sw128_desc(b);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kStepK / 16; ++k)
+              if (k < subs)
+                pair_umma_f16(acc, da + k * (MODE == kRowsK ? 2 : 128), db + k * (MODE == kWgrad ? 128 : 2), idesc, s | k);
+            if (part + 1 == t.parts) pair_umma_commit(&c->empty[st]);
+            if (last) pair_umma_commit(&c->acc_full[buf]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
         if (++st == kStages) { st = 0; phase ^= 1; }
       }
-      ++n;
+      n += t.parts;
       ok = __all_sync(0xffffffffu, ok);
     }
     if (*abort && lane == 0) {   // products in flight end before their tensor memory goes
@@ -545,22 +599,24 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       ok = mbar_wait(&c->tail[st], __shfl_sync(0xffffffffu, uses, st) & 1, abort, p.dev_err);
       ok = __all_sync(0xffffffffu, ok);
       if (lane == static_cast<int>(st)) ++uses;
-      uint4* a = reinterpret_cast<uint4*>(ring + st * 2 * kOperandBytes);
+      uint4* a = reinterpret_cast<uint4*>(ring + st * kStageBytes);
       const int zeros = (16 - t.tail % 16) * 8;   // 16-byte pieces in the lines to clear, per 64-row chunk
       for (int i = lane; ok && i < 4 * zeros; i += 32)
         a[i / zeros * (kChunkBytes / 16) + t.tail * 8 + i % zeros] = make_uint4(0, 0, 0, 0);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) pair_arrive_release(peer_addr(&c->full[st], 0));
+      if (lane == 0) pair_arrive_zeroed(peer_addr(&c->full[st], 0));
     }
   } else if (warp >= 4) {
     // -------------------------------------------------------------- results
     const int quad = warp % 4, part = (warp - 4) / 4;
-    uint8_t* stage = staging + (warp - 4) * kStoreBytes;
+    uint8_t* stages = staging + (warp - 4) * 2 * kStoreBytes;
+    uint32_t flip = 0;
     uint32_t n = 0;
     bool ok = true;
     for (int32_t tile = first; walk.find(p, tile, t); tile += stride) {
       const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;   // this warp's 32 M rows
+      for (int part_n = 0; part_n < (WIDE ? t.parts : 1); ++part_n) {
       const uint32_t acc = tmem + (n % 2) * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16);
       if (t.steps) {
         ok = __all_sync(0xffffffffu, mbar_wait(&c->acc_full[n % 2], (n / 2) & 1, abort, p.dev_err));
@@ -569,85 +625,119 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       }
       if (m < p.m_len) {
         if constexpr (MODE != kWgrad) {
-          // lane = feature, column = row of the group: a warp's store is 32 features of one row
-          const int32_t f = m + lane;
-          for (int32_t col = part * 32; col < t.valid; col += 64) {
-            uint32_t r[32];
-            tmem_ld32(acc + col, r);
-            tmem_ld_wait();
-            const int32_t rows = min(32, t.valid - col);
-            if (f < p.m_len) {
-              const int64_t at = (t.row0 + col) * p.ld + f;
+          const int32_t valid = min(t.width, t.valid - part_n * t.width);
+          const int64_t row0 = t.row0 + part_n * t.width;
+          for (int32_t col = part * 32; col < valid; col += 64) {
+            const int32_t rows = min(32, valid - col);
+            if (p.tma_out) {
+              // tensor memory holds a feature a lane and a row a column: 8 x 8 fragments are stored transposed,
+              // into lines of 32 features of one row, and a full tile of 32 rows leaves by TMA
+              uint8_t* stage = stages + (flip ^= 1) * kStoreBytes;
+              uint32_t lo[16], hi[16];
+              tmem_ld_fragments(acc + col, lo);
+              tmem_ld_fragments(acc + col + (16u << 16), hi);
+              if (lane == 0) bulk_wait_read_1();
+              __syncwarp();
+              tmem_ld_wait();
+              pack_pairs(lo, p.bf16);
+              pack_pairs(hi, p.bf16);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                if (j >= rows) break;
-                if (p.f32) static_cast<float*>(p.dst)[at + j * p.ld] = __uint_as_float(r[j]);
-                else static_cast<uint16_t*>(p.dst)[at + j * p.ld] = round16(__uint_as_float(r[j]), p.bf16);
+              for (int i = 0; i < 4; ++i) {
+                const int line = 8 * i + lane % 8;
+                stmatrix_t(smem_u32(stage) + line * 64 + ((lane / 8 ^ (line >> 1 & 3)) << 4), lo[2 * i], lo[2 * i + 1],
+                           hi[2 * i], hi[2 * i + 1]);
               }
+              if (rows == 32) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) tma_store_2d(&p.out, stage, m, static_cast<int32_t>(row0) + col);
+              } else {   // the group's last rows: the next ones are another group's
+                __syncwarp();
+                uint16_t* dst = static_cast<uint16_t*>(p.dst) + (row0 + col) * p.ld + m;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int line = 8 * i + lane / 4, q = lane % 4;
+                  const uint4 v = *reinterpret_cast<const uint4*>(stage + line * 64 + ((q ^ (line >> 1 & 3)) << 4));
+                  if (line < rows) store_8(dst + line * p.ld + q * 8, v, p.m_len - m - q * 8);
+                }
+                __syncwarp();
+              }
+              if (lane == 0) bulk_commit();
+            } else {
+              // lane = feature, register = row: a warp's store is 32 features of one row
+              uint32_t r[32];
+              tmem_ld32(acc + col, r);
+              tmem_ld_wait();
+              const int32_t count = m + lane < p.m_len ? rows : 0;
+              const int64_t at = (row0 + col) * p.ld + m + lane;
+              if (p.f32) {
+                float* dst = static_cast<float*>(p.dst) + at;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (j < count) dst[j * p.ld] = __uint_as_float(r[j]);
+              } else {
+                uint16_t* dst = static_cast<uint16_t*>(p.dst) + at;
+                pack_each(r, p.bf16);
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (j < count) dst[j * p.ld] = static_cast<uint16_t>(r[j]);
+              }
+              __syncwarp();
             }
-            __syncwarp();
           }
         } else if (t.steps || !p.accumulate) {
-          // lane = n, column = k: 128-byte lines through shared memory, stored by TMA, which cuts them at
-          // the matrix's edges; outputs that TMA cannot address are written by element
-          const int32_t wide = p.tma_out && !p.f32 ? 64 : 32;
-          for (int32_t col = part * wide; col < t.width && t.n0 + col < p.n_len; col += 2 * wide) {
-            if (p.tma_out) {
-              if (lane == 0) bulk_wait_read();
-              __syncwarp();
-            }
+          // lane = n, column = k: 64-byte lines through shared memory, stored by TMA, which cuts them at the
+          // matrix's edges; outputs that TMA cannot address are written by element
+          for (int32_t col = part * 32; col < t.width && t.n0 + col < p.n_len; col += 64) {
+            uint32_t r[32];
+            if (t.steps) {
+              tmem_ld32(acc + col, r);
+              tmem_ld_wait();
+            } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              if (h * 32 >= wide) break;
-              uint32_t r[32];
-              if (t.steps) {
-                tmem_ld32(acc + col + h * 32, r);
-                tmem_ld_wait();
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) r[j] = 0;
-              }
-              if (!p.tma_out) {
-                const int64_t at = t.e * p.stride_e + (m + lane) * p.ld + t.n0 + col;
-                const int32_t left = m + lane < p.m_len ? min(32, p.n_len - t.n0 - col) : 0;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  if (j >= left) continue;
-                  float v = __uint_as_float(r[j]);
-                  if (p.f32) {
-                    float* o = static_cast<float*>(p.dst) + at + j;
-                    *o = p.accumulate ? *o + v : v;
-                  } else {
-                    uint16_t* o = static_cast<uint16_t*>(p.dst) + at + j;
-                    if (p.accumulate) v += widen16(*o, p.bf16);
-                    *o = round16(v, p.bf16);
-                  }
-                }
-              } else if (p.f32) {
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                  *reinterpret_cast<uint4*>(stage + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-                      make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
-              } else {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  uint32_t w[4];
-#pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    w[i] = pack16(__uint_as_float(r[8 * q + 2 * i]), __uint_as_float(r[8 * q + 2 * i + 1]), p.bf16);
-                  *reinterpret_cast<uint4*>(stage + lane * 128 + (((h * 4 + q) ^ (lane & 7)) << 4)) =
-                      make_uint4(w[0], w[1], w[2], w[3]);
-                }
-              }
+              for (int j = 0; j < 32; ++j) r[j] = 0;
             }
             if (p.tma_out) {
-              fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                if (p.accumulate) tma_add_3d(&p.out, stage, t.n0 + col, m, t.e);
-                else tma_store_3d(&p.out, stage, t.n0 + col, m, t.e);
-                bulk_commit();
+              if (!p.f32) pack_pairs(r, p.bf16);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {   // 16 words a line: 32 columns of 16 bits, or 16 of f32 twice
+                if (h == 1 && !p.f32) break;
+                uint8_t* stage = stages + (flip ^= 1) * kStoreBytes;
+                if (lane == 0) bulk_wait_read_1();
+                __syncwarp();
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                  *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = make_uint4(
+                      r[16 * h + 4 * q], r[16 * h + 4 * q + 1], r[16 * h + 4 * q + 2], r[16 * h + 4 * q + 3]);
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  if (p.accumulate) tma_add_3d(&p.out, stage, t.n0 + col + 16 * h, m, t.e);
+                  else tma_store_3d(&p.out, stage, t.n0 + col + 16 * h, m, t.e);
+                  bulk_commit();
+                }
               }
+            } else {
+              const int64_t at = t.e * p.stride_e + (m + lane) * p.ld + t.n0 + col;
+              const int32_t count = m + lane < p.m_len ? min(32, p.n_len - t.n0 - col) : 0;
+              if (p.f32) {
+                float* dst = static_cast<float*>(p.dst) + at;
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (j < count) dst[j] = __uint_as_float(r[j]) + (p.accumulate ? dst[j] : 0.f);
+              } else {
+                uint16_t* dst = static_cast<uint16_t*>(p.dst) + at;
+                if (p.accumulate) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j)
+                    if (j < count) r[j] = __float_as_uint(__uint_as_float(r[j]) + widen16(dst[j], p.bf16));
+                }
+                pack_each(r, p.bf16);
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (j < count) dst[j] = static_cast<uint16_t>(r[j]);
+              }
+              __syncwarp();
             }
           }
         }
@@ -658,10 +748,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         if (lane == 0) pair_arrive(peer_addr(&c->acc_empty[n % 2], 0));
         ++n;
       }
+      }
+      if (!ok) break;
     }
-    if constexpr (MODE == kWgrad) {
-      if (p.tma_out && lane == 0) bulk_wait_all();
-    } else if (ok) {   // rows of no group
+    if (p.tma_out && lane == 0) bulk_wait_all();
+    if (MODE != kWgrad && ok) {   // rows of no group
       const int64_t gap = walk.lo + (p.g.rows - walk.carry);
       for (int64_t i = blockIdx.x; i < gap; i += gridDim.x) {
         const int64_t at = (i < walk.lo ? i : i - walk.lo + walk.carry) * p.ld;
@@ -692,16 +783,16 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 // [outer][rows][cols] with row pitch and outer stride in bytes (dims = 2 leaves
-// the outer one away), 128-byte swizzle.
+// the outer one away).
 int make_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int dims, uint64_t cols, uint64_t rows,
-             uint64_t outer, uint64_t pitch, uint64_t stride, uint32_t box_cols, uint32_t box_rows) {
+             uint64_t outer, uint64_t pitch, uint64_t stride, uint32_t box_cols, uint32_t box_rows,
+             CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   auto fn = encode_fn();
   if (!fn) return report_error(HEXMOE_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const cuuint64_t size[3] = {cols, rows, outer}, strides[2] = {pitch, stride};
   const cuuint32_t box[3] = {box_cols, box_rows, 1}, step[3] = {1, 1, 1};
   const CUresult r = fn(m, dt, dims, const_cast<void*>(base), size, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) return HEXMOE_OK;
   char buf[96];
   snprintf(buf, sizeof(buf), "grouped product: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));
@@ -725,9 +816,11 @@ int sm_count(int* sms) {
   if (dev < 0 || dev >= 64) return report_error(HEXMOE_E_DEVICE, "device ordinal out of range");
   int v = cached[dev].load(std::memory_order_acquire);
   if (!v) {   // first call on this device: the kernels' shared memory as well
-    for (const void* k : {reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad>)}) {
+    for (const void* k : {reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, false>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, true>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, false>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, true>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, false>)}) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
       if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
     }
@@ -739,7 +832,7 @@ int sm_count(int* sms) {
   return HEXMOE_OK;
 }
 
-template <int MODE>
+template <int MODE, bool WIDE>
 cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(sms / 2, tiles))));
@@ -751,7 +844,7 @@ cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE>, p);
+  return cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, WIDE>, p);
 }
 
 int check_groups(const char* what, int64_t rows, int32_t experts, const void* offsets, int32_t offsets_dtype) {
@@ -829,9 +922,17 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
       return rc;
     // box heights up to half the widest tile that these rows can make
     const int64_t half = (std::min<int64_t>(rows, 256) + 31) / 32 * 16;
-    for (int i = 0; i < kBoxes && (i == 0 || (8 << i) < half); ++i)
+    for (int i = 0; i < kBoxes && 16 << i <= half; ++i)
       if (int rc = make_map(&q.b[i], x, dt, 2, width_in, rows, 1, 2 * ld_x, 0, 64, 16u << i)) return rc;
-    const cudaError_t e = transpose ? launch_pair<kRowsMN>(q, tiles, sms, st) : launch_pair<kRowsK>(q, tiles, sms, st);
+    q.tma_out = !q.f32 && tma_rows(out, ld_out, 2);
+    if (q.tma_out)
+      if (int rc = make_map(&q.out, out, dt, 2, width_out, rows, 1, 2 * ld_out, 0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
+        return rc;
+    const bool wide = rows / 512 * q.m_tiles >= 2 * sms;
+    const cudaError_t e = wide ? (transpose ? launch_pair<kRowsMN, true>(q, tiles, sms, st)
+                                            : launch_pair<kRowsK, true>(q, tiles, sms, st))
+                               : (transpose ? launch_pair<kRowsMN, false>(q, tiles, sms, st)
+                                            : launch_pair<kRowsK, false>(q, tiles, sms, st));
     return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
   }
   PlainParams p{};
@@ -886,9 +987,10 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
     q.tma_out = tma_stack(out, ld_out, stride_out, z, experts) && (q.f32 || !q.accumulate);
     if (q.tma_out)
       if (int rc = make_map(&q.out, out, q.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dt, 3, k, n, experts, z * ld_out,
-                            experts == 1 ? z * ld_out : z * stride_out, q.f32 ? 32 : 64, 32))
+                            experts == 1 ? z * ld_out : z * stride_out, q.f32 ? 16 : 32, 32,
+                            CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
-    const cudaError_t e = launch_pair<kWgrad>(q, tiles, sms, st);
+    const cudaError_t e = launch_pair<kWgrad, false>(q, tiles, sms, st);
     return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
   }
   PlainParams p{};

@@ -34,12 +34,14 @@ __device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
   return a;
 }
-// Arrivals on a barrier of either CTA.  release orders this thread's earlier
-// writes before it, for which the hardware waits until they are performed (about
-// 0.7 us a time in a loop that loads); the relaxed ones are for arrivals that
-// publish no write of this thread: byte counts of loads, accumulators read.
-__device__ __forceinline__ void pair_arrive_release(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// Arrivals on a barrier of either CTA.  A release at cluster scope makes the
+// hardware wait for all of this thread's memory operations (about 0.5 us in a loop
+// that loads), so none is used.  The relaxed forms publish no write of this thread:
+// byte counts of loads, accumulators read.  pair_arrive_zeroed follows writes to
+// this CTA's shared memory that only this SM's tensor core reads, and that
+// fence.proxy.async has already ordered before its reads.
+__device__ __forceinline__ void pair_arrive_zeroed(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void pair_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -48,34 +50,6 @@ __device__ __forceinline__ void pair_arrive_expect_tx(uint32_t bar, uint32_t byt
   asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ bool pair_try_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-// mbar_wait (ptx.cuh) for a barrier on which the other CTA publishes writes.
-__device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* dev_err) {
-  if (pair_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer();
-  for (uint32_t i = 1;; ++i) {
-    if (pair_try_wait(bar, parity)) return true;
-    if ((i & 15) == 0) {
-      if (*abort) return false;
-      if (globaltimer() - t0 > kWaitTimeoutNs) {
-        *abort = 1;
-        atomicOr(dev_err, kDevErrTimeout);
-        return false;
-      }
-    }
-  }
-}
-
 // Box loads into this CTA's shared memory that complete on `bar`, a cluster
 // address: this CTA's barrier or the other CTA's.
 __device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {
@@ -100,6 +74,12 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void*
                "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
                : "memory");
 }
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(smem_u32(src)), "r"(x), "r"(y)
+               : "memory");
+}
 __device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, const void* src, int32_t x, int32_t y, int32_t z) {
   asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(map)),
@@ -107,7 +87,8 @@ __device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, const void* s
                : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void bulk_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+// All but the newest of this thread's groups have read their shared memory.
+__device__ __forceinline__ void bulk_wait_read_1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 __device__ __forceinline__ void pair_tmem_alloc(uint32_t* dst_smem, uint32_t ncols) {  // one warp of each CTA
@@ -149,6 +130,25 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
         "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
+}
+
+// 16 lanes x 32 columns as 8 x 8 fragments: for column block i (8 columns), r[4i],
+// r[4i+1] hold columns 8i + 2q, 8i + 2q + 1 of lane g, r[4i+2], r[4i+3] of lane
+// g + 8 (thread 4g + q).
+__device__ __forceinline__ void tmem_ld_fragments(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Four 8 x 8 matrices of 16-bit values, transposed on the way: thread t gives the
+// address of line t % 8 of matrix t / 8.
+__device__ __forceinline__ void stmatrix_t(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b),
+               "r"(c), "r"(d)
+               : "memory");
 }
 
 // Shared-memory matrix descriptor of an MN-major tile in 128-byte swizzle: the
