@@ -431,6 +431,135 @@ struct Walker {
   }
 };
 
+// Writes 32 x 32 pieces of an accumulator: one writer warp's M rows by 32 columns.
+template <int MODE>
+struct Writer {
+  const PairParams& p;
+  uint8_t* stages;   // two staging tiles of 32 lines of 64 B (the 16-byte pieces of a line permuted as SWIZZLE_64B)
+  int lane;
+  int32_t e = 0, m = 0, cols = 0;   // expert; first M row; columns there are
+  int64_t n0 = 0;                   // column 0 in the output: row products: its row; weight gradient: its column
+  uint32_t flip = 0;
+
+  __device__ __forceinline__ uint8_t* next_stage() {
+    flip ^= 1;
+    if (lane == 0) bulk_wait_read_1();
+    __syncwarp();
+    return stages + flip * kStoreBytes;
+  }
+  // Row products that leave by TMA take fragments, everything else a row of 32 columns a lane.
+  __device__ __forceinline__ void load(uint32_t acc, uint32_t (&r)[32]) const {
+    if (MODE != kWgrad && p.tma_out) {
+      tmem_ld_fragments<0>(acc, r);
+      tmem_ld_fragments<16>(acc + (16u << 16), r);
+    } else {
+      tmem_ld32(acc, r);
+    }
+  }
+  __device__ __forceinline__ void write(int32_t col, uint32_t (&r)[32]) {
+    if constexpr (MODE == kWgrad) write_gradient(col, r);
+    else if (p.tma_out) write_rows(col, r);
+    else write_elements(col, r);
+  }
+
+  // Tensor memory holds a feature a lane and a row a column: 8 x 8 fragments are
+  // stored transposed, into lines of 32 features of one row, and a full tile of 32
+  // rows leaves by TMA.
+  __device__ __forceinline__ void write_rows(int32_t col, uint32_t (&r)[32]) {
+    const int32_t rows = min(32, cols - col);
+    uint8_t* stage = next_stage();
+    pack_pairs(r, p.bf16);   // words 0..7: lanes 0..15, 8..15: lanes 16..31
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int line = 8 * i + lane % 8;
+      stmatrix_t(smem_u32(stage) + line * 64 + ((lane / 8 ^ (line >> 1 & 3)) << 4), r[2 * i], r[2 * i + 1], r[8 + 2 * i],
+                 r[8 + 2 * i + 1]);
+    }
+    if (rows == 32) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) tma_store_2d(&p.out, stage, m, static_cast<int32_t>(n0) + col);
+    } else {   // the group's last rows: the next ones are another group's
+      __syncwarp();
+      uint16_t* dst = static_cast<uint16_t*>(p.dst) + (n0 + col) * p.ld + m;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int line = 8 * i + lane / 4, q = lane % 4;
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + line * 64 + ((q ^ (line >> 1 & 3)) << 4));
+        if (line < rows) store_8(dst + line * p.ld + q * 8, v, p.m_len - m - q * 8);
+      }
+      __syncwarp();
+    }
+    if (lane == 0) bulk_commit();
+  }
+
+  // f32 rows, and outputs that TMA cannot address: lane = feature, register = row,
+  // a warp's store is 32 features of one row.
+  __device__ __forceinline__ void write_elements(int32_t col, uint32_t (&r)[32]) const {
+    const int32_t rows = m + lane < p.m_len ? min(32, cols - col) : 0;
+    const int64_t at = (n0 + col) * p.ld + m + lane;
+    if (p.f32) {
+      float* dst = static_cast<float*>(p.dst) + at;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < rows) dst[j * p.ld] = __uint_as_float(r[j]);
+    } else {
+      uint16_t* dst = static_cast<uint16_t*>(p.dst) + at;
+      pack_each(r, p.bf16);
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < rows) dst[j * p.ld] = static_cast<uint16_t>(r[j]);
+    }
+    __syncwarp();
+  }
+
+  // lane = n, register = k: 64-byte lines through shared memory, stored by TMA,
+  // which cuts them at the matrix's edges; by element where TMA cannot.
+  __device__ __forceinline__ void write_gradient(int32_t col, uint32_t (&r)[32]) {
+    if (p.tma_out) {
+      if (!p.f32) pack_pairs(r, p.bf16);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {   // 16 words a line: 32 columns of 16 bits, or 16 of f32 twice
+        if (h == 1 && !p.f32) break;
+        uint8_t* stage = next_stage();
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
+              make_uint4(r[16 * h + 4 * q], r[16 * h + 4 * q + 1], r[16 * h + 4 * q + 2], r[16 * h + 4 * q + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          const int32_t x = static_cast<int32_t>(n0) + col + 16 * h;
+          if (p.accumulate) tma_add_3d(&p.out, stage, x, m, e);
+          else tma_store_3d(&p.out, stage, x, m, e);
+          bulk_commit();
+        }
+      }
+      return;
+    }
+    const int64_t at = e * p.stride_e + (m + lane) * p.ld + n0 + col;
+    const int32_t count = m + lane < p.m_len ? min(32, cols - col) : 0;
+    if (p.f32) {
+      float* dst = static_cast<float*>(p.dst) + at;
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < count) dst[j] = __uint_as_float(r[j]) + (p.accumulate ? dst[j] : 0.f);
+    } else {
+      uint16_t* dst = static_cast<uint16_t*>(p.dst) + at;
+      if (p.accumulate) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < count) r[j] = __float_as_uint(__uint_as_float(r[j]) + widen16(dst[j], p.bf16));
+      }
+      pack_each(r, p.bf16);
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (j < count) dst[j] = static_cast<uint16_t>(r[j]);
+    }
+    __syncwarp();
+  }
+};
+
 struct PairCtrl {
   uint64_t full[kMaxStages], empty[kMaxStages], tail[kMaxStages];
   uint64_t acc_full[2], acc_empty[2], done;
@@ -609,147 +738,53 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     }
   } else if (warp >= 4) {
     // -------------------------------------------------------------- results
-    const int quad = warp % 4, part = (warp - 4) / 4;
-    uint8_t* stages = staging + (warp - 4) * 2 * kStoreBytes;
-    uint32_t flip = 0;
+    const int quad = warp % 4, part = (warp - 4) / 4;   // 32 of the CTA's M rows, every other 32 columns
+    Writer<MODE> out{p, staging + (warp - 4) * 2 * kStoreBytes, lane};
     uint32_t n = 0;
     bool ok = true;
-    for (int32_t tile = first; walk.find(p, tile, t); tile += stride) {
-      const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;   // this warp's 32 M rows
-      for (int part_n = 0; part_n < (WIDE ? t.parts : 1); ++part_n) {
-      const uint32_t acc = tmem + (n % 2) * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16);
-      if (t.steps) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&c->acc_full[n % 2], (n / 2) & 1, abort, p.dev_err));
+    for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
+      out.e = t.e;
+      out.m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
+      for (int acc_n = 0; acc_n < (WIDE ? t.parts : 1); ++acc_n) {
+        const int32_t cols = MODE == kWgrad ? min(t.width, p.n_len - t.n0) : min(t.width, t.valid - acc_n * t.width);
+        const int chunks = out.m < p.m_len && cols > part * 32 ? (cols - part * 32 + 63) / 64 : 0;
+        out.cols = cols;
+        out.n0 = MODE == kWgrad ? t.n0 : t.row0 + acc_n * t.width;
+        uint32_t r0[32], r1[32];
+        if (t.steps == 0) {   // an empty group's gradient
+          if (p.accumulate) continue;
+          for (int i = 0; i < chunks; ++i) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) r0[j] = 0;
+            out.write(part * 32 + 64 * i, r0);
+          }
+          continue;
+        }
+        const uint32_t buf = n % 2, acc = tmem + buf * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16) + part * 32;
+        ok = __all_sync(0xffffffffu, mbar_wait(&c->acc_full[buf], (n / 2) & 1, abort, p.dev_err));
         if (!ok) break;
         tc_fence_after();
-      }
-      if (m < p.m_len) {
-        if constexpr (MODE != kWgrad) {
-          const int32_t valid = min(t.width, t.valid - part_n * t.width);
-          const int64_t row0 = t.row0 + part_n * t.width;
-          for (int32_t col = part * 32; col < valid; col += 64) {
-            const int32_t rows = min(32, valid - col);
-            if (p.tma_out) {
-              // tensor memory holds a feature a lane and a row a column: 8 x 8 fragments are stored transposed,
-              // into lines of 32 features of one row, and a full tile of 32 rows leaves by TMA
-              uint8_t* stage = stages + (flip ^= 1) * kStoreBytes;
-              uint32_t lo[16], hi[16];
-              tmem_ld_fragments(acc + col, lo);
-              tmem_ld_fragments(acc + col + (16u << 16), hi);
-              if (lane == 0) bulk_wait_read_1();
-              __syncwarp();
-              tmem_ld_wait();
-              pack_pairs(lo, p.bf16);
-              pack_pairs(hi, p.bf16);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int line = 8 * i + lane % 8;
-                stmatrix_t(smem_u32(stage) + line * 64 + ((lane / 8 ^ (line >> 1 & 3)) << 4), lo[2 * i], lo[2 * i + 1],
-                           hi[2 * i], hi[2 * i + 1]);
-              }
-              if (rows == 32) {
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) tma_store_2d(&p.out, stage, m, static_cast<int32_t>(row0) + col);
-              } else {   // the group's last rows: the next ones are another group's
-                __syncwarp();
-                uint16_t* dst = static_cast<uint16_t*>(p.dst) + (row0 + col) * p.ld + m;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const int line = 8 * i + lane / 4, q = lane % 4;
-                  const uint4 v = *reinterpret_cast<const uint4*>(stage + line * 64 + ((q ^ (line >> 1 & 3)) << 4));
-                  if (line < rows) store_8(dst + line * p.ld + q * 8, v, p.m_len - m - q * 8);
-                }
-                __syncwarp();
-              }
-              if (lane == 0) bulk_commit();
-            } else {
-              // lane = feature, register = row: a warp's store is 32 features of one row
-              uint32_t r[32];
-              tmem_ld32(acc + col, r);
-              tmem_ld_wait();
-              const int32_t count = m + lane < p.m_len ? rows : 0;
-              const int64_t at = (row0 + col) * p.ld + m + lane;
-              if (p.f32) {
-                float* dst = static_cast<float*>(p.dst) + at;
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (j < count) dst[j * p.ld] = __uint_as_float(r[j]);
-              } else {
-                uint16_t* dst = static_cast<uint16_t*>(p.dst) + at;
-                pack_each(r, p.bf16);
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (j < count) dst[j * p.ld] = static_cast<uint16_t>(r[j]);
-              }
-              __syncwarp();
-            }
-          }
-        } else if (t.steps || !p.accumulate) {
-          // lane = n, column = k: 64-byte lines through shared memory, stored by TMA, which cuts them at the
-          // matrix's edges; outputs that TMA cannot address are written by element
-          for (int32_t col = part * 32; col < t.width && t.n0 + col < p.n_len; col += 64) {
-            uint32_t r[32];
-            if (t.steps) {
-              tmem_ld32(acc + col, r);
-              tmem_ld_wait();
-            } else {
-#pragma unroll
-              for (int j = 0; j < 32; ++j) r[j] = 0;
-            }
-            if (p.tma_out) {
-              if (!p.f32) pack_pairs(r, p.bf16);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {   // 16 words a line: 32 columns of 16 bits, or 16 of f32 twice
-                if (h == 1 && !p.f32) break;
-                uint8_t* stage = stages + (flip ^= 1) * kStoreBytes;
-                if (lane == 0) bulk_wait_read_1();
-                __syncwarp();
-#pragma unroll
-                for (int q = 0; q < 4; ++q)
-                  *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = make_uint4(
-                      r[16 * h + 4 * q], r[16 * h + 4 * q + 1], r[16 * h + 4 * q + 2], r[16 * h + 4 * q + 3]);
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                  if (p.accumulate) tma_add_3d(&p.out, stage, t.n0 + col + 16 * h, m, t.e);
-                  else tma_store_3d(&p.out, stage, t.n0 + col + 16 * h, m, t.e);
-                  bulk_commit();
-                }
-              }
-            } else {
-              const int64_t at = t.e * p.stride_e + (m + lane) * p.ld + t.n0 + col;
-              const int32_t count = m + lane < p.m_len ? min(32, p.n_len - t.n0 - col) : 0;
-              if (p.f32) {
-                float* dst = static_cast<float*>(p.dst) + at;
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (j < count) dst[j] = __uint_as_float(r[j]) + (p.accumulate ? dst[j] : 0.f);
-              } else {
-                uint16_t* dst = static_cast<uint16_t*>(p.dst) + at;
-                if (p.accumulate) {
-#pragma unroll
-                  for (int j = 0; j < 32; ++j)
-                    if (j < count) r[j] = __float_as_uint(__uint_as_float(r[j]) + widen16(dst[j], p.bf16));
-                }
-                pack_each(r, p.bf16);
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (j < count) dst[j] = static_cast<uint16_t>(r[j]);
-              }
-              __syncwarp();
-            }
-          }
+        ++n;
+        // a chunk is written while the next one's load is under way; the accumulator is free once the last is read
+        auto release = [&] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) pair_arrive(peer_addr(&c->acc_empty[buf], 0));
+        };
+        if (chunks == 0) release();
+        else out.load(acc, r0);
+        for (int i = 0; i < chunks; i += 2) {
+          tmem_ld_wait_for(r0);
+          if (i + 1 < chunks) out.load(acc + 64 * (i + 1), r1);
+          else release();
+          out.write(part * 32 + 64 * i, r0);
+          if (i + 1 == chunks) break;
+          tmem_ld_wait_for(r1);
+          if (i + 2 < chunks) out.load(acc + 64 * (i + 2), r0);
+          else release();
+          out.write(part * 32 + 64 * (i + 1), r1);
         }
       }
-      if (t.steps) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) pair_arrive(peer_addr(&c->acc_empty[n % 2], 0));
-        ++n;
-      }
-      }
-      if (!ok) break;
     }
     if (p.tma_out && lane == 0) bulk_wait_all();
     if (MODE != kWgrad && ok) {   // rows of no group
@@ -928,7 +963,10 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
     if (q.tma_out)
       if (int rc = make_map(&q.out, out, dt, 2, width_out, rows, 1, 2 * ld_out, 0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
-    const bool wide = rows / 512 * q.m_tiles >= 2 * sms;
+    // Two accumulators a tile where groups of 257..512 rows are the rule (the matrix is then loaded once a
+    // group, not twice: 96 x 341 rows, 1536 x 2048: 182 us against 194) and still fill the machine; with
+    // larger groups the drain between tiles costs more than it saves (8192^2 x 2048: 180 us against 174).
+    const bool wide = rows > 256ll * experts && rows <= 512ll * experts && experts * q.m_tiles >= sms;
     const cudaError_t e = wide ? (transpose ? launch_pair<kRowsMN, true>(q, tiles, sms, st)
                                             : launch_pair<kRowsK, true>(q, tiles, sms, st))
                                : (transpose ? launch_pair<kRowsMN, false>(q, tiles, sms, st)

@@ -86,6 +86,13 @@ __device__ __forceinline__ void tma_add_3d(const CUtensorMap* map, const void* s
                "r"(smem_u32(src)), "r"(x), "r"(y), "r"(z)
                : "memory");
 }
+// A box on its way into L2 ahead of its load.
+__device__ __forceinline__ void tma_prefetch_3d(const CUtensorMap* map, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.prefetch.tensor.3d.L2.global [%0, {%1, %2, %3}];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // All but the newest of this thread's groups have read their shared memory.
 __device__ __forceinline__ void bulk_wait_read_1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
@@ -135,13 +142,25 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
 // 16 lanes x 32 columns as 8 x 8 fragments: for column block i (8 columns), r[4i],
 // r[4i+1] hold columns 8i + 2q, 8i + 2q + 1 of lane g, r[4i+2], r[4i+3] of lane
 // g + 8 (thread 4g + q).
-__device__ __forceinline__ void tmem_ld_fragments(uint32_t taddr, uint32_t (&r)[16]) {
+template <int FIRST>
+__device__ __forceinline__ void tmem_ld_fragments(uint32_t taddr, uint32_t (&r)[32]) {   // into r[FIRST..FIRST+15]
   asm volatile(
       "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "=r"(r[FIRST + 0]), "=r"(r[FIRST + 1]), "=r"(r[FIRST + 2]), "=r"(r[FIRST + 3]), "=r"(r[FIRST + 4]), "=r"(r[FIRST + 5]), "=r"(r[FIRST + 6]), "=r"(r[FIRST + 7]), "=r"(r[FIRST + 8]),
+        "=r"(r[FIRST + 9]), "=r"(r[FIRST + 10]), "=r"(r[FIRST + 11]), "=r"(r[FIRST + 12]), "=r"(r[FIRST + 13]), "=r"(r[FIRST + 14]), "=r"(r[FIRST + 15])
       : "r"(taddr)
       : "memory");
+}
+// Waits for this thread's tensor-memory loads, and names the registers of the one
+// whose values are used next: none of their uses can move before the wait, while
+// registers of a load still in flight stay out of it.
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                 "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                 "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                 "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
 // Four 8 x 8 matrices of 16-bit values, transposed on the way: thread t gives the
 // address of line t % 8 of matrix t / 8.
