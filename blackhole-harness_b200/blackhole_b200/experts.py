@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import math
 from array import array
+from operator import attrgetter
 
 import torch
 
@@ -33,59 +34,76 @@ _INDEX = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream() without building a Stream object
+_current_device = torch.cuda.current_device
 
 
-def _run(name: str, dev: torch.device, *args) -> None:
+def _run(fn, dev: torch.device, *args) -> None:
     """One C call on dev's current stream (with dev current), its status raised as an exception."""
-    fn = getattr(_lib.lib, name)
     index = dev.index
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
             rc = fn(*args, _raw_stream(index))
     if rc:
-        _lib.check(rc, name)
+        _lib.check(rc, fn.__name__)
 
 
-def _rows2d(t: torch.Tensor, what: str) -> torch.Tensor:
-    """t as a matrix whose rows are contiguous (a copy only where they are not)."""
+def _rows2d(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int]:
+    """t as a matrix whose rows are contiguous (a copy only where they are not), and its row stride."""
     if t.dim() != 2:
         raise ValueError(f"{what} must be a matrix, got {tuple(t.shape)}")
+    ld, step = t.stride()
     # a row stride shorter than a row (an expanded or overlapping view) is no stride the kernels take
-    return t if (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) >= t.shape[1] else t.contiguous()
+    if ld < t.shape[1] or (step != 1 and t.shape[1] != 1):
+        t = t.contiguous()
+        ld = max(t.stride(0), t.shape[1])
+    return t, ld
 
 
-def _check_groups(offsets: torch.Tensor, experts: int, dev: torch.device) -> torch.Tensor:
-    if offsets.dtype not in _INDEX or offsets.dim() != 1 or offsets.shape[0] != experts + 1:
+def _check_groups(offsets: torch.Tensor, experts: int, dev: torch.device) -> tuple[torch.Tensor, int]:
+    """offsets, checked, and their type's code."""
+    code = _INDEX.get(offsets.dtype)
+    if code is None or offsets.shape != (experts + 1,):
         raise ValueError(f"offsets must be int32 or int64 [{experts + 1}], got {offsets.dtype} {tuple(offsets.shape)}")
     if offsets.device != dev:
         raise ValueError(f"offsets are on {offsets.device}, the rows on {dev}")
-    return offsets.contiguous()
+    return offsets.contiguous(), code
 
 
-def _check_16bit(what: str, *tensors: torch.Tensor) -> None:
+def _check_16bit(what: str, *tensors: torch.Tensor) -> int:
+    """The code of the tensors' type, which is one."""
     t0 = tensors[0]
+    dtype, dev = t0.dtype, t0.device
     for t in tensors:
         if not t.is_cuda:
             raise ValueError(f"{what} runs on CUDA only")
-        if t.device != t0.device:
-            raise ValueError(f"{what}: tensors on {t0.device} and {t.device}")
-        if t.dtype not in _16BIT or t.dtype != t0.dtype:
-            raise ValueError(f"{what} takes bf16 or fp16 tensors of one type, got {t0.dtype} and {t.dtype}")
+        if t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+        if t.dtype != dtype:
+            raise ValueError(f"{what} takes bf16 or fp16 tensors of one type, got {dtype} and {t.dtype}")
+    if dtype not in _16BIT:
+        raise ValueError(f"{what} takes bf16 or fp16 tensors, got {dtype}")
+    return _DT[dtype]
 
 
-def _output(out, shape: tuple, dtype, out_dtype, dev, what: str) -> torch.Tensor:
-    """The caller's `out`, checked, or a new tensor of out_dtype (dtype unless given)."""
+def _output(out, shape: tuple, like: torch.Tensor, out_dtype, what: str) -> torch.Tensor:
+    """The caller's `out`, checked, or a new tensor of out_dtype (like's unless given)."""
+    dtype = like.dtype
     if out is None:
-        out_dtype = out_dtype or dtype
-        if out_dtype not in (dtype, torch.float32):
+        if out_dtype is None or out_dtype == dtype:
+            return like.new_empty(shape)
+        if out_dtype != torch.float32:
             raise ValueError(f"{what}: out_dtype must be {dtype} or float32")
-        return torch.empty(shape, dtype=out_dtype, device=dev)
-    if tuple(out.shape) != shape or out.device != dev or out.dtype not in (dtype, torch.float32) or (
+        return like.new_empty(shape, dtype=out_dtype)
+    if out.shape != shape or out.device != like.device or out.dtype not in (dtype, torch.float32) or (
             out_dtype is not None and out_dtype != out.dtype):
-        raise ValueError(f"{what}: out must be {dtype} or float32 {list(shape)} on {dev}")
+        raise ValueError(f"{what}: out must be {dtype} or float32 {list(shape)} on {like.device}")
     return out
+
+
+_grouped_mm, _grouped_wgrad = _lib.lib.hexmoe_grouped_mm, _lib.lib.hexmoe_grouped_wgrad
+_swiglu, _swiglu_backward = _lib.lib.hexmoe_swiglu, _lib.lib.hexmoe_swiglu_backward
 
 
 def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, transpose: bool = False,
@@ -93,26 +111,33 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, transpos
     """x[r] W[e]^T for every row r of group e: x [R, K], w [E, N, K] -> [R, N]; with transpose
     x[r] W[e]: x [R, N] -> [R, K].  Rows of no group come back as zero.  bf16 or fp16, the
     result in the same type or (out_dtype, out) float32."""
+    code = _check_16bit("grouped_mm", x, w)
     if w.dim() != 3:
         raise ValueError(f"w must be [E, N, K], got {tuple(w.shape)}")
-    _check_16bit("grouped_mm", x, w)
-    x = _rows2d(x, "x")
+    x, ld_x = _rows2d(x, "x")
     E, N, K = w.shape
-    offsets = _check_groups(offsets, E, x.device)
+    dev = x.device
+    offsets, index_code = _check_groups(offsets, E, dev)
     R, width = x.shape
     if width != (N if transpose else K):
         raise ValueError(f"x has {width} columns, w is {tuple(w.shape)} (transpose={transpose})")
-    if w.stride(2) != 1 or w.stride(1) < K:
+    stride_w, ld_w, step = w.stride()
+    if step != 1 or ld_w < K:
         # a transposed view of [E, K, N] is that stack, used the other way round
-        if w.stride(1) == 1 and w.stride(2) >= N:
-            w, N, K, transpose = w.transpose(1, 2), K, N, not transpose
+        if ld_w == 1 and step >= N:
+            ld_w, N, K, transpose = step, K, N, not transpose
         else:
             w = w.contiguous()
-    res = _output(out, (R, K if transpose else N), x.dtype, out_dtype, x.device, "grouped_mm")
-    to = res if res.stride(1) == 1 and res.stride(0) >= res.shape[1] else torch.empty_like(
-        res, memory_format=torch.contiguous_format)
-    _run("hexmoe_grouped_mm", x.device, x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(1), w.stride(0), _DT[x.dtype],
-         R, E, N, K, transpose, offsets.data_ptr(), _INDEX[offsets.dtype], to.data_ptr(), to.stride(0), _DT[to.dtype])
+            stride_w, ld_w = N * K, K
+    width = K if transpose else N
+    res = to = _output(out, (R, width), x, out_dtype, "grouped_mm")
+    ld = width
+    if out is not None:
+        ld = res.stride(0)
+        if ld < width or res.stride(1) != 1:
+            to, ld = torch.empty_like(res, memory_format=torch.contiguous_format), width
+    _run(_grouped_mm, dev, x.data_ptr(), ld_x, w.data_ptr(), ld_w, stride_w, code, R, E, N, K, transpose,
+         offsets.data_ptr(), index_code, to.data_ptr(), ld, _DT[to.dtype])
     return res if to is res else res.copy_(to)
 
 
@@ -121,8 +146,8 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out_
     """dW[e] = dy_e^T x_e over the rows of every group: dy [R, N], x [R, K] -> [E, N, K] (zero for
     an empty group), in their type or float32.  accumulate adds to `out`.  With dy = x these
     are the Hessians that quant.quantize_stack(H=...) takes."""
-    _check_16bit("grouped_wgrad", dy, x)
-    dy, x = _rows2d(dy, "dy"), _rows2d(x, "x")
+    code = _check_16bit("grouped_wgrad", dy, x)
+    (dy, ld_dy), (x, ld_x) = _rows2d(dy, "dy"), _rows2d(x, "x")
     if dy.shape[0] != x.shape[0]:
         raise ValueError(f"dy has {dy.shape[0]} rows, x {x.shape[0]}")
     if accumulate and out is None:
@@ -130,18 +155,18 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out_
     E = offsets.shape[0] - 1 if offsets.dim() == 1 else 0
     if E < 1:
         raise ValueError("offsets must be [experts + 1]")
-    offsets = _check_groups(offsets, E, x.device)
-    R, N, K = x.shape[0], dy.shape[1], x.shape[1]
-    res = _output(out, (E, N, K), x.dtype, out_dtype, x.device, "grouped_wgrad")
-    if res.stride(2) == 1 and res.stride(1) >= K and res.stride(0) >= (N - 1) * res.stride(1) + K:
-        to = res
-    elif accumulate:
-        to = res.contiguous()
-    else:
-        to = torch.empty_like(res, memory_format=torch.contiguous_format)
-    _run("hexmoe_grouped_wgrad", x.device, dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), _DT[x.dtype], R, E, N,
-         K, offsets.data_ptr(), _INDEX[offsets.dtype], to.data_ptr(), to.stride(1), to.stride(0), _DT[to.dtype],
-         accumulate)
+    dev = x.device
+    offsets, index_code = _check_groups(offsets, E, dev)
+    (R, K), N = x.shape, dy.shape[1]
+    res = to = _output(out, (E, N, K), x, out_dtype, "grouped_wgrad")
+    stride, ld = N * K, K
+    if out is not None:
+        stride, ld, step = res.stride()
+        if step != 1 or ld < K or stride < (N - 1) * ld + K:
+            to = res.contiguous() if accumulate else torch.empty_like(res, memory_format=torch.contiguous_format)
+            stride, ld = N * K, K
+    _run(_grouped_wgrad, dev, dy.data_ptr(), ld_dy, x.data_ptr(), ld_x, code, R, E, N, K, offsets.data_ptr(), index_code,
+         to.data_ptr(), ld, stride, _DT[to.dtype], accumulate)
     return res if to is res else res.copy_(to)
 
 
@@ -159,14 +184,14 @@ def swiglu(h: torch.Tensor, row_weights: torch.Tensor | None = None) -> torch.Te
         raise ValueError("swiglu runs on CUDA only")
     if h.dtype not in _DT:
         raise ValueError(f"unsupported dtype {h.dtype}")
-    h = _rows2d(h, "h")
+    h, ld = _rows2d(h, "h")
     R, width = h.shape
     if width % 2 or not width:
         raise ValueError(f"h must be [R, 2 * I], got {tuple(h.shape)}")
-    row_weights = _check_row_weights(row_weights, R, h.device)
-    act = torch.empty(R, width // 2, dtype=h.dtype, device=h.device)
-    _run("hexmoe_swiglu", h.device, h.data_ptr(), _DT[h.dtype], R, width // 2, h.stride(0), _ptr(row_weights),
-         act.data_ptr(), width // 2)
+    dev, inter = h.device, width // 2
+    row_weights = _check_row_weights(row_weights, R, dev)
+    act = h.new_empty((R, inter))
+    _run(_swiglu, dev, h.data_ptr(), _DT[h.dtype], R, inter, ld, _ptr(row_weights), act.data_ptr(), inter)
     return act
 
 
@@ -184,12 +209,13 @@ def swiglu_backward(dact: torch.Tensor, h: torch.Tensor, row_weights: torch.Tens
     if out is not None and (out.shape != h.shape or out.dtype != h.dtype or out.device != h.device
                             or out.stride(1) != 1 or out.stride(0) < 2 * I):
         raise ValueError(f"out must be {h.dtype} {list(h.shape)} with contiguous rows")
-    row_weights = _check_row_weights(row_weights, R, h.device)
-    h, dact = _rows2d(h, "h"), _rows2d(dact, "dact")
-    dh = torch.empty(R, 2 * I, dtype=h.dtype, device=h.device) if out is None else out
-    dw = None if row_weights is None else torch.empty(R, dtype=torch.float32, device=h.device)
-    _run("hexmoe_swiglu_backward", h.device, dact.data_ptr(), dact.stride(0), h.data_ptr(), h.stride(0), _DT[h.dtype], R,
-         I, _ptr(row_weights), dh.data_ptr(), dh.stride(0), _ptr(dw))
+    dev = h.device
+    row_weights = _check_row_weights(row_weights, R, dev)
+    (h, ld_h), (dact, ld_dact) = _rows2d(h, "h"), _rows2d(dact, "dact")
+    dh = h.new_empty((R, 2 * I)) if out is None else out
+    dw = None if row_weights is None else row_weights.new_empty(R)
+    _run(_swiglu_backward, dev, dact.data_ptr(), ld_dact, h.data_ptr(), ld_h, _DT[h.dtype], R, I, _ptr(row_weights),
+         dh.data_ptr(), 2 * I if out is None else out.stride(0), _ptr(dw))
     return dh, dw
 
 
@@ -217,7 +243,22 @@ def _runs(t: torch.Tensor):
         yield from _runs(t.select(d, i))
 
 
+def _type_codes(tensors: list) -> array:
+    dtypes = list(map(_get_dtype, tensors))
+    try:
+        if dtypes.count(dtypes[0]) == len(dtypes):
+            return array("i", [_DT[dtypes[0]]]) * len(dtypes)
+        return array("i", [_DT[t] for t in dtypes])
+    except KeyError as e:
+        raise ValueError(f"clip_grad_norm: unsupported dtype {e.args[0]}") from None
+
+
 _CLIP_RUNS = 1 << 16
+# called by map() over a model's gradients: the host's share of a small model's clipping
+_get_device, _is_contiguous, _data_ptr, _numel = (torch.Tensor.get_device, torch.Tensor.is_contiguous,
+                                                  torch.Tensor.data_ptr, torch.Tensor.numel)
+_get_shape, _get_dtype = attrgetter("shape"), attrgetter("dtype")
+_clip_grad_norm, _clip_workspace_bytes = _lib.lib.hexmoe_clip_grad_norm, _lib.lib.hexmoe_clip_grad_norm_workspace_bytes
 
 
 def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None) -> torch.Tensor:
@@ -244,11 +285,11 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     if dev.type != "cuda":
         raise ValueError("clip_grad_norm runs on CUDA only")
     held = grads if out is None else grads + out
-    if {t.get_device() for t in held} != {dev.index}:
+    if set(map(_get_device, held)) != {dev.index}:
         raise ValueError(f"clip_grad_norm: not every tensor is on {dev}")
-    if out is not None and [g.shape for g in grads] != [o.shape for o in out]:
+    if out is not None and list(map(_get_shape, grads)) != list(map(_get_shape, out)):
         raise ValueError("every tensor of out must have its gradient's shape")
-    if not all([t.is_contiguous() for t in held]):
+    if not all(map(_is_contiguous, held)):
         if out is not None and [g.stride() for g in grads] != [o.stride() for o in out]:
             raise ValueError("every tensor of out must have its gradient's strides")
         grads = [r for g in grads for r in _runs(g)]
@@ -257,20 +298,18 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
         if out is not None:
             out = [r for o in out for r in _runs(o)]
     n = len(grads)
-    try:
-        types = array("i", [_DT[g.dtype] for g in grads])
-        out_types = None if out is None else array("i", [_DT[o.dtype] for o in out])
-    except KeyError as e:
-        raise ValueError(f"clip_grad_norm: unsupported dtype {e.args[0]}") from None
-    ptrs, counts = array("Q", [g.data_ptr() for g in grads]), array("q", [g.numel() for g in grads])
-    out_ptrs = None if out is None else array("Q", [o.data_ptr() for o in out])
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    nbytes = _lib.lib.hexmoe_clip_grad_norm_workspace_bytes(n)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    at = lambda a: None if a is None else a.buffer_info()[0]  # noqa: E731
-    _run("hexmoe_clip_grad_norm", dev, n, at(ptrs), at(counts), at(types), at(out_ptrs), at(out_types), max_norm,
-         norm_type == math.inf, norm.data_ptr(), ws.data_ptr(), nbytes)
-    return norm
+    types = _type_codes(grads)
+    ptrs, counts = array("Q", map(_data_ptr, grads)), array("q", map(_numel, grads))
+    if out is None:
+        out_ptr = out_types_ptr = None
+    else:
+        out_types, out_ptrs = _type_codes(out), array("Q", map(_data_ptr, out))
+        out_ptr, out_types_ptr = out_ptrs.buffer_info()[0], out_types.buffer_info()[0]
+    nbytes = _clip_workspace_bytes(n)
+    ws = torch.empty(nbytes // 4 + 1, dtype=torch.float32, device=dev)   # the partial sums, then the norm
+    _run(_clip_grad_norm, dev, n, ptrs.buffer_info()[0], counts.buffer_info()[0], types.buffer_info()[0], out_ptr,
+         out_types_ptr, max_norm, norm_type == math.inf, ws.data_ptr() + nbytes, ws.data_ptr(), nbytes)
+    return ws[nbytes // 4]
 
 
 def expert_plan(topk_ids: torch.Tensor, num_experts: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, tuple]:
@@ -282,7 +321,7 @@ def expert_plan(topk_ids: torch.Tensor, num_experts: int) -> tuple[torch.Tensor,
     sid, eid, npp = align(topk_ids.reshape(-1), num_experts, 1)
     S, dev = topk_ids.numel(), sid.device
     offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-    _run("hexmoe_group_offsets", dev, _ptr(eid), eid.numel(), _ptr(npp), 1, num_experts, _ptr(offsets))
+    _run(_lib.lib.hexmoe_group_offsets, dev, _ptr(eid), eid.numel(), _ptr(npp), 1, num_experts, _ptr(offsets))
     rows = torch.full((S + 1,), -1, dtype=torch.int32, device=dev)
     rows[sid.long()] = torch.arange(sid.numel(), dtype=torch.int32, device=dev)
     return offsets, sid, rows[:S], (sid, eid, npp)
@@ -294,7 +333,7 @@ def _gather(x: torch.Tensor, topk: int, num_experts: int, plan: tuple) -> torch.
     sid, _, npp = plan
     x = _aligned(x)
     xs = torch.empty(sid.numel(), x.shape[1], dtype=x.dtype, device=x.device)
-    _run("hexmoe_gather", x.device, _ptr(x), _DT[x.dtype], x.shape[0], x.shape[1], topk, num_experts, _ptr(sid), _ptr(npp),
+    _run(_lib.lib.hexmoe_gather, x.device, _ptr(x), _DT[x.dtype], x.shape[0], x.shape[1], topk, num_experts, _ptr(sid), _ptr(npp),
          1, _ptr(xs))
     return xs
 

@@ -334,7 +334,7 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 // 12 warps a CTA: 0 loads, 1 issues the products (the leader's), 2 zeroes tails
 // (weight gradient), 4..11 write results.  Each walks the groups' offsets by
 // itself, so that no size is known on the host.
-constexpr int kMaxStages = 6;
+constexpr int kMaxStages = 10;
 constexpr int kStepK = 64;
 constexpr uint32_t kOperandBytes = 128 * kStepK * 2;   // one operand's share of a CTA and step
 constexpr uint32_t kChunkBytes = kOperandBytes / 2;    // 64 rows of an MN-major operand
@@ -347,6 +347,13 @@ constexpr uint32_t kPairSmem = 1024 + kRingBytes + 2 * kWriters * kStoreBytes + 
 constexpr int kBoxes = 4;                              // row boxes of 16, 32, 64, 128
 
 enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2 };
+
+// Shapes of a tile's N side and of the ring that fits it.
+//   kOne     up to 256 columns: 6 steps of 32 KB
+//   kTwo     up to 512 in two accumulators: 4 steps of 48 KB
+//   kNarrow  up to 64: 10 steps of 20 KB, the matrix's share of each as large as in the others: with a
+//            handful of rows the matrix streams, and what counts is how much of it is on its way
+enum PairShape { kOne = 0, kTwo = 1, kNarrow = 2 };
 
 struct PairParams {
   CUtensorMap a;             // W (3-D: reduction or features, ..., expert) or dy
@@ -372,9 +379,10 @@ struct Tile {
   int32_t valid;
 };
 
-template <int MODE, bool WIDE>
+template <int MODE, int SHAPE>
 struct Walker {
-  static constexpr int32_t kSpan = WIDE ? 512 : 256;   // most rows of a tile
+  static constexpr bool kWide = SHAPE == kTwo;
+  static constexpr int32_t kSpan = SHAPE == kTwo ? 512 : SHAPE == kNarrow ? 64 : 256;   // most rows of a tile
   int32_t base = -32;
   int64_t carry = 0, lo = 0;
   int32_t upto = 0, mine = 0, total = 0;
@@ -418,7 +426,7 @@ struct Walker {
     } else {
       const int32_t size = static_cast<int32_t>(e - b), tiles = (size + kSpan - 1) / kSpan;
       const int32_t span = (size + tiles - 1) / tiles;
-      t.parts = WIDE && span > 256 ? 2 : 1;
+      t.parts = kWide && span > 256 ? 2 : 1;
       t.width = ((span + t.parts - 1) / t.parts + 31) / 32 * 32;
       t.m0 = local / tiles * 256;
       t.n0 = local % tiles * t.parts * t.width;
@@ -567,10 +575,13 @@ struct PairCtrl {
   int abort;
 };
 
-template <int MODE, bool WIDE>
+template <int MODE, int SHAPE>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     grouped_pair_kernel(const __grid_constant__ PairParams p) {
-  constexpr uint32_t kStages = WIDE ? 4 : 6, kStageBytes = (WIDE ? 3 : 2) * kOperandBytes;
+  constexpr bool WIDE = SHAPE == kTwo;
+  constexpr uint32_t kStages = SHAPE == kTwo ? 4 : SHAPE == kNarrow ? 9 : 6;
+  constexpr uint32_t kStageBytes = kOperandBytes * (SHAPE == kTwo ? 12 : SHAPE == kNarrow ? 5 : 8) / 4;
+  static_assert(kStages <= kMaxStages && kStages * kStageBytes <= kRingBytes);
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (1024 - smem_u32(raw) % 1024) % 1024;
   uint8_t* ring = base;
@@ -600,9 +611,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   tc_fence_after();
   const uint32_t tmem = c->tmem;
   pdl_wait();
+  pdl_launch_dependents();   // one wave: whoever waits for this grid may take its place on the SMs as they fall free
 
   const int32_t first = blockIdx.x / 2, stride = gridDim.x / 2;
-  Walker<MODE, WIDE> walk;
+  Walker<MODE, SHAPE> walk;
   Tile t;
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
@@ -851,11 +863,13 @@ int sm_count(int* sms) {
   if (dev < 0 || dev >= 64) return report_error(HEXMOE_E_DEVICE, "device ordinal out of range");
   int v = cached[dev].load(std::memory_order_acquire);
   if (!v) {   // first call on this device: the kernels' shared memory as well
-    for (const void* k : {reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, false>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, true>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, false>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, true>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, false>)}) {
+    for (const void* k : {reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kOne>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kTwo>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kNarrow>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kOne>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kTwo>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kNarrow>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, kOne>)}) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
       if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
     }
@@ -867,7 +881,7 @@ int sm_count(int* sms) {
   return HEXMOE_OK;
 }
 
-template <int MODE, bool WIDE>
+template <int MODE, int SHAPE>
 cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(sms / 2, tiles))));
@@ -879,7 +893,7 @@ cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, WIDE>, p);
+  return cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, SHAPE>, p);
 }
 
 int check_groups(const char* what, int64_t rows, int32_t experts, const void* offsets, int32_t offsets_dtype) {
@@ -960,17 +974,22 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
     for (int i = 0; i < kBoxes && 16 << i <= half; ++i)
       if (int rc = make_map(&q.b[i], x, dt, 2, width_in, rows, 1, 2 * ld_x, 0, 64, 16u << i)) return rc;
     q.tma_out = !q.f32 && tma_rows(out, ld_out, 2);
-    if (q.tma_out)
+    if (q.tma_out && rows >= 32)   // no full tile of 32 rows otherwise
       if (int rc = make_map(&q.out, out, dt, 2, width_out, rows, 1, 2 * ld_out, 0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
     // Two accumulators a tile where groups of 257..512 rows are the rule (the matrix is then loaded once a
     // group, not twice: 96 x 341 rows, 1536 x 2048: 182 us against 194) and still fill the machine; with
     // larger groups the drain between tiles costs more than it saves (8192^2 x 2048: 180 us against 174).
     const bool wide = rows > 256ll * experts && rows <= 512ll * experts && experts * q.m_tiles >= sms;
-    const cudaError_t e = wide ? (transpose ? launch_pair<kRowsMN, true>(q, tiles, sms, st)
-                                            : launch_pair<kRowsK, true>(q, tiles, sms, st))
-                               : (transpose ? launch_pair<kRowsMN, false>(q, tiles, sms, st)
-                                            : launch_pair<kRowsK, false>(q, tiles, sms, st));
+    const PairShape shape = rows <= 64 ? kNarrow : wide ? kTwo : kOne;
+    auto launch = [&](auto mode) {
+      constexpr int MODE = decltype(mode)::value;
+      return shape == kNarrow ? launch_pair<MODE, kNarrow>(q, tiles, sms, st)
+             : shape == kTwo  ? launch_pair<MODE, kTwo>(q, tiles, sms, st)
+                              : launch_pair<MODE, kOne>(q, tiles, sms, st);
+    };
+    const cudaError_t e = transpose ? launch(std::integral_constant<int, kRowsMN>{})
+                                    : launch(std::integral_constant<int, kRowsK>{});
     return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
   }
   PlainParams p{};
@@ -1028,7 +1047,7 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
                             experts == 1 ? z * ld_out : z * stride_out, q.f32 ? 16 : 32, 32,
                             CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
-    const cudaError_t e = launch_pair<kWgrad, false>(q, tiles, sms, st);
+    const cudaError_t e = launch_pair<kWgrad, kOne>(q, tiles, sms, st);
     return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
   }
   PlainParams p{};
