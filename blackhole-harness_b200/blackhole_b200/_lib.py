@@ -28,7 +28,8 @@ EXPORTS = (
     "hexmoe_ep_init", "hexmoe_ep_handle", "hexmoe_ep_connect", "hexmoe_ep_workspace_bytes", "hexmoe_ep_dispatch",
     "hexmoe_ep_experts", "hexmoe_ep_combine", "hexmoe_ep_forward", "hexmoe_ep_destroy",
     "hexmoe_quantize_workspace_bytes", "hexmoe_quantize",
-    "hexmoe_group_offsets", "hexmoe_grouped_mm", "hexmoe_grouped_wgrad", "hexmoe_swiglu", "hexmoe_swiglu_backward",
+    "hexmoe_group_offsets", "hexmoe_grouped_mm_workspace_bytes", "hexmoe_grouped_mm",
+    "hexmoe_grouped_wgrad_workspace_bytes", "hexmoe_grouped_wgrad", "hexmoe_swiglu", "hexmoe_swiglu_backward",
     "hexmoe_clip_grad_norm_workspace_bytes", "hexmoe_clip_grad_norm",
 )
 EP_MAX_WORLD = 8          # HEXMOE_EP_MAX_WORLD
@@ -93,9 +94,11 @@ def _load() -> ctypes.CDLL:
                                            P]),
         "hexmoe_group_offsets": (ctypes.c_int, [P, I64_, P, I32_, I32_, P, P]),
         "hexmoe_grouped_mm": (ctypes.c_int, [P, I64_, P, I64_, I64_, I32_, I64_, I32_, I32_, I32_, I32_, P, I32_, P,
-                                             I64_, I32_, P]),
+                                             I64_, I32_, P, SZ, P]),
+        "hexmoe_grouped_mm_workspace_bytes": (SZ, [I64_, I32_, I32_, I32_, I32_]),
+        "hexmoe_grouped_wgrad_workspace_bytes": (SZ, [I64_, I32_, I32_, I32_]),
         "hexmoe_grouped_wgrad": (ctypes.c_int, [P, I64_, P, I64_, I32_, I64_, I32_, I32_, I32_, P, I32_, P, I64_, I64_,
-                                                I32_, I32_, P]),
+                                                I32_, I32_, P, SZ, P]),
         "hexmoe_swiglu": (ctypes.c_int, [P, I32_, I64_, I32_, I64_, P, P, I64_, P]),
         "hexmoe_swiglu_backward": (ctypes.c_int, [P, I64_, P, I64_, I32_, I64_, I32_, P, P, I64_, P, P]),
         "hexmoe_clip_grad_norm_workspace_bytes": (SZ, [I32_]),

@@ -364,17 +364,19 @@ struct PairParams {
   int32_t n_len;             // weight gradient: k
   int32_t red;               // row products: reduction length
   int32_t m_tiles, n_tiles, tile_n;   // n_tiles, tile_n: weight gradient
-  void* dst;
-  int64_t ld, stride_e;
+  int32_t splits;            // runs that the reduction of a tile is cut into
+  void* dst;                 // splits > 1: fp32 partials, one result a run
+  int64_t ld, stride_e, stride_split;
   int32_t f32, bf16, accumulate, tma_out;
   int32_t* dev_err;
 };
 
 // One tile: expert, M offset, N offset (a row offset within the group in the row
 // products) and width, of `parts` accumulators side by side; row0 its first row,
-// valid its real rows; steps of the reduction, the last one of `tail` (0: full).
+// valid its real rows; steps of the reduction from `first` on, the last one of
+// `tail` (0: full); split: the run of the reduction that these are.
 struct Tile {
-  int32_t e, m0, n0, width, parts, steps, tail;
+  int32_t e, m0, n0, width, parts, first, steps, tail, split;
   int64_t row0;
   int32_t valid;
 };
@@ -389,7 +391,8 @@ struct Walker {
   int64_t begin = 0, end = 0;
   bool bad = false;
 
-  __device__ __forceinline__ bool find(const PairParams& p, int32_t tile, Tile& t) {
+  __device__ __forceinline__ bool find(const PairParams& p, int32_t unit, Tile& t) {
+    const int32_t tile = p.splits > 1 ? unit / p.splits : unit;
     while (tile >= total) {
       if (base + 32 >= p.g.experts) return false;
       base += 32;
@@ -435,6 +438,14 @@ struct Walker {
       t.steps = (p.red + kStepK - 1) / kStepK;
       t.tail = p.red % kStepK;
     }
+    t.first = t.split = 0;
+    if (p.splits > 1) {
+      t.split = unit - tile * p.splits;
+      const int32_t steps = t.steps;
+      t.first = steps * t.split / p.splits;
+      t.steps = steps * (t.split + 1) / p.splits - t.first;
+      if (t.first + t.steps != steps) t.tail = 0;
+    }
     return true;
   }
 };
@@ -445,7 +456,7 @@ struct Writer {
   const PairParams& p;
   uint8_t* stages;   // two staging tiles of 32 lines of 64 B (the 16-byte pieces of a line permuted as SWIZZLE_64B)
   int lane;
-  int32_t e = 0, m = 0, cols = 0;   // expert; first M row; columns there are
+  int32_t e = 0, m = 0, cols = 0;   // which result (expert, run of the reduction); first M row; columns there are
   int64_t n0 = 0;                   // column 0 in the output: row products: its row; weight gradient: its column
   uint32_t flip = 0;
 
@@ -505,7 +516,7 @@ struct Writer {
   // a warp's store is 32 features of one row.
   __device__ __forceinline__ void write_elements(int32_t col, uint32_t (&r)[32]) const {
     const int32_t rows = m + lane < p.m_len ? min(32, cols - col) : 0;
-    const int64_t at = (n0 + col) * p.ld + m + lane;
+    const int64_t at = e * p.stride_split + (n0 + col) * p.ld + m + lane;
     if (p.f32) {
       float* dst = static_cast<float*>(p.dst) + at;
 #pragma unroll
@@ -632,20 +643,21 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         // a step whose rows past the group's end are still to be zeroed lands on this CTA's own barrier
         const bool fix = MODE == kWgrad && s + 1 == t.steps && t.tail % 16 != 0;
         const uint32_t bar = fix ? peer_addr(&c->tail[st], rank) : peer_addr(&c->full[st], 0);
+        const int32_t r = (t.first + s) * kStepK;   // where the step begins in the reduction
         if (elect_one()) {
           pair_arrive_expect_tx(bar, bytes);
           if constexpr (MODE == kRowsK) {
-            pair_load_3d(a, &p.a, bar, s * kStepK, m, t.e);
+            pair_load_3d(a, &p.a, bar, r, m, t.e);
           } else if constexpr (MODE == kRowsMN) {
-            pair_load_3d(a, &p.a, bar, m, s * kStepK, t.e);
-            pair_load_3d(a + kChunkBytes, &p.a, bar, m + 64, s * kStepK, t.e);
+            pair_load_3d(a, &p.a, bar, m, r, t.e);
+            pair_load_3d(a + kChunkBytes, &p.a, bar, m + 64, r, t.e);
           } else {
-            const int32_t y = static_cast<int32_t>(t.row0) + s * kStepK;
+            const int32_t y = static_cast<int32_t>(t.row0) + r;
             pair_load_2d(a, &p.a, bar, m, y);
             pair_load_2d(a + kChunkBytes, &p.a, bar, m + 64, y);
           }
           if constexpr (MODE == kWgrad) {
-            const int32_t y = static_cast<int32_t>(t.row0) + s * kStepK, x = t.n0 + static_cast<int32_t>(rank) * half;
+            const int32_t y = static_cast<int32_t>(t.row0) + r, x = t.n0 + static_cast<int32_t>(rank) * half;
             pair_load_2d(b, &p.b[0], bar, x, y);
             pair_load_2d(b + kChunkBytes, &p.b[0], bar, x + 64, y);
           } else {
@@ -657,7 +669,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
 #pragma unroll
               for (int i = kBoxes - 1; i >= 0; --i) {   // the rows' number in boxes of 128, 64, 32, 16
                 if (half & (16 << i)) {
-                  pair_load_2d(to, &p.b[i], bar, s * kStepK, y);
+                  pair_load_2d(to, &p.b[i], bar, r, y);
                   to += (16 << i) * kStepK * 2;
                   y += 16 << i;
                 }
@@ -755,7 +767,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     uint32_t n = 0;
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
-      out.e = t.e;
+      out.e = MODE == kWgrad ? t.split * p.g.experts + t.e : t.split;
       out.m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
       for (int acc_n = 0; acc_n < (WIDE ? t.parts : 1); ++acc_n) {
         const int32_t cols = MODE == kWgrad ? min(t.width, p.n_len - t.n0) : min(t.width, t.valid - acc_n * t.width);
@@ -801,8 +813,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     if (p.tma_out && lane == 0) bulk_wait_all();
     if (MODE != kWgrad && ok) {   // rows of no group
       const int64_t gap = walk.lo + (p.g.rows - walk.carry);
-      for (int64_t i = blockIdx.x; i < gap; i += gridDim.x) {
-        const int64_t at = (i < walk.lo ? i : i - walk.lo + walk.carry) * p.ld;
+      for (int64_t j = blockIdx.x; j < gap * p.splits; j += gridDim.x) {
+        const int64_t i = j % gap, at = j / gap * p.stride_split + (i < walk.lo ? i : i - walk.lo + walk.carry) * p.ld;
         for (int32_t f = threadIdx.x - 128; f < p.m_len; f += kWriters * 32) {
           if (p.f32) static_cast<float*>(p.dst)[at + f] = 0.f;
           else static_cast<uint16_t*>(p.dst)[at + f] = 0;
@@ -896,6 +908,88 @@ cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_
   return cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, SHAPE>, p);
 }
 
+// ------------------------------------------------------------------- splits
+// Products of few tiles leave most pairs idle while a few walk a long reduction:
+// their reduction is cut into `splits` runs of steps, each with an fp32 partial
+// result in the workspace, which a second kernel adds in order and rounds.
+constexpr int kPairsPlanned = 74;   // pairs of a B200; what the split is planned for
+constexpr int kMaxSplits = 16;
+
+// Runs for `tiles` tiles of `steps` steps.  A step takes about 0.2 us and the second
+// kernel about 3: cutting pays from some 16 steps saved on.
+int plan_splits(int64_t tiles, int64_t steps) {
+  const int64_t s = std::min<int64_t>({kPairsPlanned / std::max<int64_t>(tiles, 1), steps / 4, kMaxSplits});
+  return s >= 2 && steps - steps / s >= 16 ? static_cast<int>(s) : 1;
+}
+int64_t row_tiles(int64_t rows, int32_t experts, int32_t m_len) {
+  return (rows / 256 + std::min<int64_t>(experts, rows)) * ((m_len + 255) / 256);
+}
+int64_t pitch4(int64_t n) { return (n + 3) / 4 * 4; }   // f32 rows of whole 16-byte pieces
+int rows_splits(int64_t rows, int32_t experts, int32_t m_len, int32_t red) {
+  return plan_splits(row_tiles(rows, experts, m_len), (red + kStepK - 1) / kStepK);
+}
+int wgrad_splits(int64_t rows, int32_t experts, int32_t n, int32_t k) {
+  return plan_splits(static_cast<int64_t>(experts) * ((n + 255) / 256) * ((k + 255) / 256), rows / experts / kStepK);
+}
+
+struct JoinParams {
+  const float* part;   // [splits][rows][pitch]
+  int64_t rows, pitch;
+  int32_t splits, cols;
+  void* out;           // row r: matrix r / inner, its row r % inner
+  int64_t ld, stride;
+  int32_t inner, f32, bf16, accumulate, vec;
+};
+
+__global__ void __launch_bounds__(256) grouped_join_kernel(const JoinParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int32_t pieces = static_cast<int32_t>(p.pitch / 4);
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= p.rows * pieces) return;
+  const int64_t row = i / pieces;
+  const int32_t col = static_cast<int32_t>(i % pieces) * 4;
+  float v[4] = {};
+  for (int s = 0; s < p.splits; ++s) {
+    const float4 f = __ldg(reinterpret_cast<const float4*>(p.part + (s * p.rows + row) * p.pitch + col));
+    v[0] += f.x;
+    v[1] += f.y;
+    v[2] += f.z;
+    v[3] += f.w;
+  }
+  const int64_t at = row / p.inner * p.stride + row % p.inner * p.ld + col;
+  const int count = min(4, p.cols - col);
+  if (p.f32) {
+    float* o = static_cast<float*>(p.out) + at;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < count) o[j] = p.accumulate ? o[j] + v[j] : v[j];
+  } else {
+    uint16_t* o = static_cast<uint16_t*>(p.out) + at;
+    if (p.vec && !p.accumulate && count == 4) {
+      *reinterpret_cast<uint2*>(o) = make_uint2(pack16(v[0], v[1], p.bf16), pack16(v[2], v[3], p.bf16));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j < count) o[j] = round16(p.accumulate ? widen16(o[j], p.bf16) + v[j] : v[j], p.bf16);
+    }
+  }
+}
+
+cudaError_t launch_join(const JoinParams& p, cudaStream_t st) {
+  const int64_t blocks = (p.rows * (p.pitch / 4) + 255) / 256;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, grouped_join_kernel, p);
+}
+
 int check_groups(const char* what, int64_t rows, int32_t experts, const void* offsets, int32_t offsets_dtype) {
   if (offsets_dtype != HEXMOE_I32 && offsets_dtype != HEXMOE_I64) return report_error(HEXMOE_E_DTYPE, "offsets are I32 or I64");
   if (rows < 0 || rows >= (1ll << 31) - 512) return arg_error("%s: %lld rows", what, static_cast<long long>(rows));
@@ -935,9 +1029,22 @@ int hexmoe_group_offsets(const int32_t* expert_ids, int64_t max_blocks, const in
   return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, "hexmoe_group_offsets");
 }
 
+size_t hexmoe_grouped_mm_workspace_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k, int32_t transpose) {
+  if (rows <= 0 || experts <= 0 || n <= 0 || k <= 0) return 0;
+  const int32_t width_out = transpose ? k : n, splits = rows_splits(rows, experts, width_out, transpose ? n : k);
+  return splits > 1 ? splits * rows * pitch4(width_out) * sizeof(float) : 0;
+}
+
+size_t hexmoe_grouped_wgrad_workspace_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k) {
+  if (rows <= 0 || experts <= 0 || n <= 0 || k <= 0) return 0;
+  const int32_t splits = wgrad_splits(rows, experts, n, k);
+  return splits > 1 ? splits * static_cast<size_t>(experts) * n * pitch4(k) * sizeof(float) : 0;
+}
+
 int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int64_t stride_w, int32_t dtype,
                       int64_t rows, int32_t experts, int32_t n, int32_t k, int32_t transpose, const void* offsets,
-                      int32_t offsets_dtype, void* out, int64_t ld_out, int32_t out_dtype, void* stream) {
+                      int32_t offsets_dtype, void* out, int64_t ld_out, int32_t out_dtype, void* workspace,
+                      size_t workspace_bytes, void* stream) {
   const char* what = "hexmoe_grouped_mm";
   if (!is16(dtype)) return report_error(HEXMOE_E_DTYPE, "hexmoe_grouped_mm: x and w are BF16 or F16");
   if (out_dtype != dtype && out_dtype != HEXMOE_F32) return report_error(HEXMOE_E_DTYPE, "hexmoe_grouped_mm: out is of x's dtype or F32");
@@ -953,6 +1060,8 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
   if (!dev_err) return report_error(HEXMOE_E_CUDA, "device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Groups groups = {offsets, offsets_dtype == HEXMOE_I64, experts, rows};
+  const bool f32 = out_dtype == HEXMOE_F32, bf16 = dtype == HEXMOE_BF16;
+  if (workspace && off_by(workspace, 16)) return arg_error("%s: workspace not 16-byte aligned", what);
   if (tma_rows(x, ld_x, 2) && tma_stack(w, ld_w, stride_w, 2, experts)) {
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
@@ -960,12 +1069,18 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
     q.g = groups;
     q.m_len = width_out; q.red = width_in;
     q.m_tiles = (width_out + 255) / 256;
-    q.dst = out; q.ld = ld_out;
-    q.f32 = out_dtype == HEXMOE_F32; q.bf16 = dtype == HEXMOE_BF16;
+    q.splits = rows_splits(rows, experts, width_out, width_in);
+    const int64_t pitch = pitch4(width_out);
+    if (workspace_bytes < q.splits * rows * pitch * sizeof(float) || !workspace) q.splits = 1;
+    const bool split = q.splits > 1;
+    q.dst = split ? workspace : out;
+    q.ld = split ? pitch : ld_out;
+    q.stride_split = rows * pitch;
+    q.f32 = split || f32; q.bf16 = bf16;
     q.dev_err = dev_err;
-    const int64_t tiles = (rows / 256 + std::min<int64_t>(experts, rows)) * q.m_tiles;
+    const int64_t tiles = row_tiles(rows, experts, width_out) * q.splits;
     if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
-    const CUtensorMapDataType dt = q.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (int rc = make_map(&q.a, w, dt, 3, k, n, experts, 2 * ld_w, experts == 1 ? 2 * ld_w : 2 * stride_w, 64,
                           transpose ? 64 : 128))
       return rc;
@@ -988,8 +1103,16 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
              : shape == kTwo  ? launch_pair<MODE, kTwo>(q, tiles, sms, st)
                               : launch_pair<MODE, kOne>(q, tiles, sms, st);
     };
-    const cudaError_t e = transpose ? launch(std::integral_constant<int, kRowsMN>{})
-                                    : launch(std::integral_constant<int, kRowsK>{});
+    cudaError_t e = transpose ? launch(std::integral_constant<int, kRowsMN>{})
+                              : launch(std::integral_constant<int, kRowsK>{});
+    if (e == cudaSuccess && split) {
+      JoinParams j{};
+      j.part = static_cast<const float*>(workspace);
+      j.rows = rows; j.pitch = pitch; j.splits = q.splits; j.cols = width_out;
+      j.out = out; j.ld = ld_out; j.inner = static_cast<int32_t>(rows);
+      j.f32 = f32; j.bf16 = bf16; j.vec = ld_out % 4 == 0 && !off_by(out, 8);
+      e = launch_join(j, st);
+    }
     return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
   }
   PlainParams p{};
@@ -998,17 +1121,18 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
   p.b = static_cast<const uint16_t*>(w); p.b_e = stride_w;
   p.b_j = transpose ? 1 : ld_w; p.b_r = transpose ? ld_w : 1;
   p.j_len = width_out; p.r_len = width_in;
-  p.out = out; p.out_i = ld_out; p.out_f32 = out_dtype == HEXMOE_F32; p.bf16 = dtype == HEXMOE_BF16;
+  p.out = out; p.out_i = ld_out; p.out_f32 = f32; p.bf16 = bf16;
   p.j_tiles = (width_out + kPlainTile - 1) / kPlainTile;
   p.dev_err = dev_err;
-  const int64_t row_tiles = rows / kPlainTile + std::min<int64_t>(experts, rows);
-  const cudaError_t e = launch_plain(p, false, row_tiles * p.j_tiles, st);
+  const int64_t plain_tiles = rows / kPlainTile + std::min<int64_t>(experts, rows);
+  const cudaError_t e = launch_plain(p, false, plain_tiles * p.j_tiles, st);
   return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
 }
 
 int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int32_t dtype, int64_t rows,
                          int32_t experts, int32_t n, int32_t k, const void* offsets, int32_t offsets_dtype, void* out,
-                         int64_t ld_out, int64_t stride_out, int32_t out_dtype, int32_t accumulate, void* stream) {
+                         int64_t ld_out, int64_t stride_out, int32_t out_dtype, int32_t accumulate, void* workspace,
+                         size_t workspace_bytes, void* stream) {
   const char* what = "hexmoe_grouped_wgrad";
   if (!is16(dtype)) return report_error(HEXMOE_E_DTYPE, "hexmoe_grouped_wgrad: dy and x are BF16 or F16");
   if (out_dtype != dtype && out_dtype != HEXMOE_F32) return report_error(HEXMOE_E_DTYPE, "hexmoe_grouped_wgrad: out is of x's dtype or F32");
@@ -1022,6 +1146,8 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
   if (!dev_err) return report_error(HEXMOE_E_CUDA, "device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const Groups groups = {offsets, offsets_dtype == HEXMOE_I64, experts, rows};
+  const bool f32 = out_dtype == HEXMOE_F32, bf16 = dtype == HEXMOE_BF16;
+  if (workspace && off_by(workspace, 16)) return arg_error("%s: workspace not 16-byte aligned", what);
   if (rows > 0 && tma_rows(dy, ld_dy, 2) && tma_rows(x, ld_x, 2)) {
     int sms = 0;
     if (int rc = sm_count(&sms)) return rc;
@@ -1031,23 +1157,37 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
     q.m_tiles = (n + 255) / 256;
     q.n_tiles = (k + 255) / 256;
     q.tile_n = ((k + q.n_tiles - 1) / q.n_tiles + 63) / 64 * 64;
-    q.dst = out; q.ld = ld_out; q.stride_e = stride_out;
-    q.f32 = out_dtype == HEXMOE_F32; q.bf16 = dtype == HEXMOE_BF16; q.accumulate = accumulate != 0;
+    q.splits = wgrad_splits(rows, experts, n, k);
+    const int64_t pitch = pitch4(k), lines = static_cast<int64_t>(experts) * n;
+    if (workspace_bytes < q.splits * lines * pitch * sizeof(float) || !workspace) q.splits = 1;
+    const bool split = q.splits > 1;
+    q.dst = split ? workspace : out;
+    q.ld = split ? pitch : ld_out;
+    q.stride_e = split ? n * pitch : stride_out;
+    q.f32 = split || f32; q.bf16 = bf16; q.accumulate = accumulate && !split;
     q.dev_err = dev_err;
-    const int64_t tiles = static_cast<int64_t>(experts) * q.m_tiles * q.n_tiles;
+    const int64_t tiles = static_cast<int64_t>(experts) * q.m_tiles * q.n_tiles * q.splits;
     if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
-    const CUtensorMapDataType dt = q.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (int rc = make_map(&q.a, dy, dt, 2, n, rows, 1, 2 * ld_dy, 0, 64, 64)) return rc;
     if (int rc = make_map(&q.b[0], x, dt, 2, k, rows, 1, 2 * ld_x, 0, 64, 64)) return rc;
     // a 16-bit sum is rounded once: that of an addition to out cannot be left to TMA, which rounds before and after
-    const int64_t z = q.f32 ? 4 : 2;
-    q.tma_out = tma_stack(out, ld_out, stride_out, z, experts) && (q.f32 || !q.accumulate);
+    const int64_t z = q.f32 ? 4 : 2, results = static_cast<int64_t>(experts) * q.splits;
+    q.tma_out = tma_stack(q.dst, q.ld, q.stride_e, z, static_cast<int32_t>(results)) && (q.f32 || !q.accumulate);
     if (q.tma_out)
-      if (int rc = make_map(&q.out, out, q.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dt, 3, k, n, experts, z * ld_out,
-                            experts == 1 ? z * ld_out : z * stride_out, q.f32 ? 16 : 32, 32,
-                            CU_TENSOR_MAP_SWIZZLE_64B))
+      if (int rc = make_map(&q.out, q.dst, q.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dt, 3, k, n, results, z * q.ld,
+                            results == 1 ? z * q.ld : z * q.stride_e, q.f32 ? 16 : 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
-    const cudaError_t e = launch_pair<kWgrad, kOne>(q, tiles, sms, st);
+    cudaError_t e = launch_pair<kWgrad, kOne>(q, tiles, sms, st);
+    if (e == cudaSuccess && split) {
+      JoinParams j{};
+      j.part = static_cast<const float*>(workspace);
+      j.rows = lines; j.pitch = pitch; j.splits = q.splits; j.cols = k;
+      j.out = out; j.ld = ld_out; j.stride = stride_out; j.inner = n;
+      j.f32 = f32; j.bf16 = bf16; j.accumulate = accumulate != 0;
+      j.vec = ld_out % 4 == 0 && stride_out % 4 == 0 && !off_by(out, 8);
+      e = launch_join(j, st);
+    }
     return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
   }
   PlainParams p{};
@@ -1056,7 +1196,7 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
   p.b = static_cast<const uint16_t*>(x); p.b_j = 1; p.b_r = ld_x;
   p.i_len = n; p.j_len = k;
   p.out = out; p.out_i = ld_out; p.out_e = stride_out;
-  p.out_f32 = out_dtype == HEXMOE_F32; p.accumulate = accumulate; p.bf16 = dtype == HEXMOE_BF16;
+  p.out_f32 = f32; p.accumulate = accumulate; p.bf16 = bf16;
   p.i_tiles = (n + kPlainTile - 1) / kPlainTile;
   p.j_tiles = (k + kPlainTile - 1) / kPlainTile;
   p.dev_err = dev_err;

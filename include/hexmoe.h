@@ -384,20 +384,28 @@ HEXMOE_API int hexmoe_group_offsets(const int32_t* expert_ids, int64_t max_block
  *   transpose = 1:  out[r, :k] = x[r, :n] W[e]     (the gradient of the rows)
  * Rows of no group (before offsets[0], from offsets[experts] on) are set to zero.
  * x, w: BF16 or F16; out: the same or F32.  Any n, k >= 1 and strides; bases and
- * strides that are multiples of 16 bytes run on the tensor-memory kernels. */
+ * strides that are multiples of 16 bytes run on the tensor-memory kernels.
+ * workspace (16-byte aligned): hexmoe_grouped_mm_workspace_bytes, 0 for most
+ * sizes.  With it, few tiles share a long reduction; without it (NULL or too
+ * small) each walks its own, with the same result up to the order of the sums. */
+HEXMOE_API size_t hexmoe_grouped_mm_workspace_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k,
+                                                    int32_t transpose);
 HEXMOE_API int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, int64_t stride_w,
                                  int32_t dtype, int64_t rows, int32_t experts, int32_t n, int32_t k, int32_t transpose,
                                  const void* offsets, int32_t offsets_dtype, void* out, int64_t ld_out,
-                                 int32_t out_dtype, void* stream);
+                                 int32_t out_dtype, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Weight gradients out[e] = sum over the rows r of group e of dy[r, :n]^T
  * x[r, :k], out [experts, n, k] (zero for an empty group); with dy = x the
  * Hessians x_e^T x_e that GPTQ rounding takes.  accumulate != 0 adds to what out
- * holds (rounded once, after the addition).  dy, x: BF16 or F16; out: the same or F32. */
+ * holds (rounded once, after the addition).  dy, x: BF16 or F16; out: the same or
+ * F32.  workspace: as for hexmoe_grouped_mm. */
+HEXMOE_API size_t hexmoe_grouped_wgrad_workspace_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k);
 HEXMOE_API int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int32_t dtype,
                                     int64_t rows, int32_t experts, int32_t n, int32_t k, const void* offsets,
                                     int32_t offsets_dtype, void* out, int64_t ld_out, int64_t stride_out,
-                                    int32_t out_dtype, int32_t accumulate, void* stream);
+                                    int32_t out_dtype, int32_t accumulate, void* workspace, size_t workspace_bytes,
+                                    void* stream);
 
 /* SwiGLU of rows h = [gate | up] (h [rows, 2 * inter], row stride ld_h):
  *   act[r, i] = silu(gate[r, i]) * up[r, i] * row_weights[r]

@@ -197,6 +197,59 @@ def test_grouped_wgrad_rows_outside_and_parts(widths):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("n,k", [(200, 2056), (2056, 200), (1000, 1048)])
+def test_grouped_mm_long_reduction_of_few_tiles(n, k, transpose, out_dtype):
+    """Few tiles share the reduction (a workspace is asked for); rows before and after the groups stay zero."""
+    sizes, first, rows = [70, 0, 1], 3, 80
+    width = n if transpose else k
+    if width >= 2000:
+        assert _lib.lib.hexmoe_grouped_mm_workspace_bytes(rows, 3, n, k, transpose) > 0
+    x, w = normal((rows, width), BF16, 25), normal((3, n, k), BF16, 26, 0.05)
+    off = offsets_of(sizes, first)
+    want, mass = mm_reference(x, w, off, transpose, rows)
+    got = experts.grouped_mm(x.to(DEV), w.to(DEV), off.to(DEV), transpose=transpose, out_dtype=out_dtype)
+    assert not got[:first].any() and not got[first + 71:].any()
+    assert_sum(got, want, mass, width, out_dtype)
+    assert torch.equal(got, experts.grouped_mm(x.to(DEV), w.to(DEV), off.to(DEV), transpose=transpose, out_dtype=out_dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("sizes", [[5000], [4000, 0, 3], [2111, 2050]], ids=str)
+def test_grouped_wgrad_long_reduction_of_few_tiles(sizes, out_dtype):
+    """One group's rows shared by several runs, groups shorter than the runs are many, sums added to out."""
+    E, n, k = len(sizes), 72, 130
+    assert _lib.lib.hexmoe_grouped_wgrad_workspace_bytes(sum(sizes), E, n, k) > 0
+    dy, x = normal((sum(sizes), n), BF16, 27), normal((sum(sizes), k + 6), BF16, 28)
+    off = offsets_of(sizes)
+    want, mass = wgrad_reference(dy, x[:, :k], off)
+    xd = x.to(DEV)[:, :k]
+    assert_sum(experts.grouped_wgrad(dy.to(DEV), xd, off.to(DEV), out_dtype=out_dtype), want, mass, max(sizes), out_dtype)
+    base = normal((E, n, k), out_dtype, 29)
+    out = experts.grouped_wgrad(dy.to(DEV), xd, off.to(DEV), out=base.to(DEV), accumulate=True)
+    assert_sum(out, want + base.double(), mass + base.double().abs(), max(sizes) + 1, out_dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("sizes", [[1], [0, 3, 0, 1], [32], [9, 17, 6], [1] * 20, [0] * 40 + [8] + [0] * 30 + [16]], ids=str)
+def test_grouped_mm_few_rows(sizes, transpose):
+    """A decode step's rows, past one pass over a matrix, with gaps on both sides; fp16; widths off the block sizes."""
+    n, k, first = 200, 1352, 32 - sum(sizes) if sum(sizes) > 30 else 1
+    rows = min(32, first + sum(sizes) + 1)
+    width = n if transpose else k
+    x, w = normal((rows, width), F16, 38), normal((len(sizes), n, k), F16, 39, 0.1)
+    x[:first] = float("nan")
+    off = offsets_of(sizes, first)
+    want, mass = mm_reference(x, w, off, transpose, rows)
+    for out_dtype in (F16, F32):
+        got = experts.grouped_mm(x.to(DEV), w.to(DEV), off.to(DEV), transpose=transpose, out_dtype=out_dtype)
+        assert_sum(got, want, mass, width, out_dtype)
+
+
+@pytest.mark.gpu
 def test_grouped_products_repeat_bit_for_bit():
     sizes = [0, 300, 41, 5, 600]
     off = offsets_of(sizes).to(DEV)
@@ -554,7 +607,7 @@ def test_refusals_without_a_gpu():
     L, P = _lib.lib, ctypes.c_void_p(256)
     odd = ctypes.c_void_p(257)
     mm = lambda **a: L.hexmoe_grouped_mm(*{**dict(x=P, ldx=8, w=P, ldw=8, sw=64, dt=1, rows=4, E=2, n=8, k=8, tr=0, off=P,  # noqa: E731
-                                                  odt=0, out=P, ldo=8, outdt=1, st=None), **a}.values())
+                                                  odt=0, out=P, ldo=8, outdt=1, ws=None, nws=0, st=None), **a}.values())
     for bad in (dict(n=0), dict(k=-1), dict(rows=-1), dict(E=0), dict(E=2049), dict(ldx=7), dict(ldw=7), dict(ldo=7),
                 dict(x=None), dict(w=None), dict(out=None), dict(off=None), dict(x=odd), dict(off=odd), dict(rows=2 ** 31)):
         assert mm(**bad) == _lib.HEXMOE_E_ARG, bad
@@ -562,7 +615,7 @@ def test_refusals_without_a_gpu():
         assert mm(**bad) == _lib.HEXMOE_E_DTYPE, bad
     assert mm(rows=0) == _lib.HEXMOE_OK
     wg = lambda **a: L.hexmoe_grouped_wgrad(*{**dict(dy=P, lddy=8, x=P, ldx=8, dt=1, rows=4, E=2, n=8, k=8, off=P, odt=0,  # noqa: E731
-                                                     out=P, ldo=8, so=64, outdt=1, acc=0, st=None), **a}.values())
+                                                     out=P, ldo=8, so=64, outdt=1, acc=0, ws=None, nws=0, st=None), **a}.values())
     for bad in (dict(n=0), dict(rows=-1), dict(E=0), dict(lddy=7), dict(ldx=7), dict(ldo=7), dict(so=63), dict(out=None),
                 dict(dy=None), dict(off=None), dict(out=odd)):
         assert wg(**bad) == _lib.HEXMOE_E_ARG, bad
