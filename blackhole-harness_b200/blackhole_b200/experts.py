@@ -26,7 +26,7 @@ from operator import attrgetter
 
 import torch
 
-from blackhole_b200 import _lib
+from blackhole_b200 import _call, _lib   # _call: the same calls without Python's share, None where it passes
 from blackhole_b200.hex_moe import _DT, _aligned, _ptr, align, combine_rows
 
 _16BIT = (torch.bfloat16, torch.float16)
@@ -118,6 +118,10 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, transpos
     """x[r] W[e]^T for every row r of group e: x [R, K], w [E, N, K] -> [R, N]; with transpose
     x[r] W[e]: x [R, N] -> [R, K].  Rows of no group come back as zero.  bf16 or fp16, the
     result in the same type or (out_dtype, out) float32."""
+    if out is None and out_dtype is None:
+        res = _call.grouped_mm(x, w, offsets, transpose)
+        if res is not None:
+            return res
     code = _check_16bit("grouped_mm", x, w)
     if w.dim() != 3:
         raise ValueError(f"w must be [E, N, K], got {tuple(w.shape)}")
@@ -156,6 +160,10 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out_
     """dW[e] = dy_e^T x_e over the rows of every group: dy [R, N], x [R, K] -> [E, N, K] (zero for
     an empty group), in their type or float32.  accumulate adds to `out`.  With dy = x these
     are the Hessians that quant.quantize_stack(H=...) takes."""
+    if out is None and not accumulate and (out_dtype is None or out_dtype in (torch.float32, x.dtype)):
+        res = _call.grouped_wgrad(dy, x, offsets, out_dtype == torch.float32)
+        if res is not None:
+            return res
     code = _check_16bit("grouped_wgrad", dy, x)
     (dy, ld_dy), (x, ld_x) = _rows2d(dy, "dy"), _rows2d(x, "x")
     if dy.shape[0] != x.shape[0]:
@@ -193,6 +201,9 @@ def _check_row_weights(row_weights, rows: int, dev: torch.device):
 
 def swiglu(h: torch.Tensor, row_weights: torch.Tensor | None = None) -> torch.Tensor:
     """silu(gate) * up * row_weights of rows h [R, 2I] = [gate | up] -> [R, I] (f32, bf16 or fp16)."""
+    act = _call.swiglu(h, row_weights)
+    if act is not None:
+        return act
     if not h.is_cuda:
         raise ValueError("swiglu runs on CUDA only")
     if h.dtype not in _DT:
@@ -212,6 +223,10 @@ def swiglu_backward(dact: torch.Tensor, h: torch.Tensor, row_weights: torch.Tens
                     out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
     """The gradient of swiglu(h, row_weights) for dact [R, I]: dh [R, 2I], and that of row_weights
     (float32 [R]; None without them).  out takes dh; it may be h itself."""
+    if out is None:
+        both = _call.swiglu_backward(dact, h, row_weights)
+        if both is not None:
+            return both
     if not h.is_cuda or not dact.is_cuda:
         raise ValueError("swiglu_backward runs on CUDA only")
     if h.dtype not in _DT or dact.dtype != h.dtype or dact.device != h.device:
@@ -294,6 +309,9 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     grads = [g for g in grads if g is not None]
     if not grads:
         raise ValueError("clip_grad_norm: no gradients")
+    norm = _call.clip_grad_norm(grads, out, max_norm, norm_type == math.inf)
+    if norm is not None:
+        return norm
     dev = grads[0].device
     if dev.type != "cuda":
         raise ValueError("clip_grad_norm runs on CUDA only")
