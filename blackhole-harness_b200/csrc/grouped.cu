@@ -334,7 +334,7 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 // 12 warps a CTA: 0 loads, 1 issues the products (the leader's), 2 zeroes tails
 // (weight gradient), 4..11 write results.  Each walks the groups' offsets by
 // itself, so that no size is known on the host.
-constexpr int kMaxStages = 10;
+constexpr int kMaxStages = 6;
 constexpr int kStepK = 64;
 constexpr uint32_t kOperandBytes = 128 * kStepK * 2;   // one operand's share of a CTA and step
 constexpr uint32_t kChunkBytes = kOperandBytes / 2;    // 64 rows of an MN-major operand
@@ -351,9 +351,12 @@ enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2 };
 // Shapes of a tile's N side and of the ring that fits it.
 //   kOne     up to 256 columns: 6 steps of 32 KB
 //   kTwo     up to 512 in two accumulators: 4 steps of 48 KB
-//   kNarrow  up to 64: 10 steps of 20 KB, the matrix's share of each as large as in the others: with a
-//            handful of rows the matrix streams, and what counts is how much of it is on its way
+//   kNarrow  up to 64: 4 steps of 40 KB, 128 wide: with a handful of rows the matrix streams, and the ring holds
+//            as much of it as it can.  Waiting for a step, issuing its products and committing them
+//            takes the issuing warp some 450 cycles, more than narrow products run: twice the step
+//            (one token on 96 experts, 1536 x 2048: 64 wide 14.5 us, 128 wide 13.2).
 enum PairShape { kOne = 0, kTwo = 1, kNarrow = 2 };
+constexpr int subs_of(int shape) { return shape == kNarrow ? 2 : 1; }   // 64-wide blocks of a step
 
 struct PairParams {
   CUtensorMap a;             // W (3-D: reduction or features, ..., expert) or dy
@@ -383,8 +386,7 @@ struct Tile {
 
 template <int MODE, int SHAPE>
 struct Walker {
-  static constexpr bool kWide = SHAPE == kTwo;
-  static constexpr int32_t kSpan = SHAPE == kTwo ? 512 : SHAPE == kNarrow ? 64 : 256;   // most rows of a tile
+  [[maybe_unused]] static constexpr int32_t kSpan = SHAPE == kTwo ? 512 : SHAPE == kNarrow ? 64 : 256;   // most rows of a tile
   int32_t base = -32;
   int64_t carry = 0, lo = 0;
   int32_t upto = 0, mine = 0, total = 0;
@@ -429,14 +431,15 @@ struct Walker {
     } else {
       const int32_t size = static_cast<int32_t>(e - b), tiles = (size + kSpan - 1) / kSpan;
       const int32_t span = (size + tiles - 1) / tiles;
-      t.parts = kWide && span > 256 ? 2 : 1;
+      t.parts = SHAPE == kTwo && span > 256 ? 2 : 1;
       t.width = ((span + t.parts - 1) / t.parts + 31) / 32 * 32;
       t.m0 = local / tiles * 256;
       t.n0 = local % tiles * t.parts * t.width;
       t.row0 = b + t.n0;
       t.valid = min(t.parts * t.width, size - t.n0);
-      t.steps = (p.red + kStepK - 1) / kStepK;
-      t.tail = p.red % kStepK;
+      constexpr int32_t kWidth = kStepK * subs_of(SHAPE);
+      t.steps = (p.red + kWidth - 1) / kWidth;
+      t.tail = p.red % kWidth;
     }
     t.first = t.split = 0;
     if (p.splits > 1) {
@@ -462,7 +465,7 @@ struct Writer {
 
   __device__ __forceinline__ uint8_t* next_stage() {
     flip ^= 1;
-    if (lane == 0) bulk_wait_read_1();
+    if (elect_one()) bulk_wait_read_1();
     __syncwarp();
     return stages + flip * kStoreBytes;
   }
@@ -497,7 +500,10 @@ struct Writer {
     if (rows == 32) {
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) tma_store_2d(&p.out, stage, m, static_cast<int32_t>(n0) + col);
+      if (elect_one()) {
+        tma_store_2d(&p.out, stage, m, static_cast<int32_t>(n0) + col);
+        bulk_commit();
+      }
     } else {   // the group's last rows: the next ones are another group's
       __syncwarp();
       uint16_t* dst = static_cast<uint16_t*>(p.dst) + (n0 + col) * p.ld + m;
@@ -508,8 +514,8 @@ struct Writer {
         if (line < rows) store_8(dst + line * p.ld + q * 8, v, p.m_len - m - q * 8);
       }
       __syncwarp();
+      if (elect_one()) bulk_commit();   // an empty group, for the count of next_stage()
     }
-    if (lane == 0) bulk_commit();
   }
 
   // f32 rows, and outputs that TMA cannot address: lane = feature, register = row,
@@ -547,7 +553,7 @@ struct Writer {
               make_uint4(r[16 * h + 4 * q], r[16 * h + 4 * q + 1], r[16 * h + 4 * q + 2], r[16 * h + 4 * q + 3]);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) {
+        if (elect_one()) {
           const int32_t x = static_cast<int32_t>(n0) + col + 16 * h;
           if (p.accumulate) tma_add_3d(&p.out, stage, x, m, e);
           else tma_store_3d(&p.out, stage, x, m, e);
@@ -590,8 +596,10 @@ template <int MODE, int SHAPE>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     grouped_pair_kernel(const __grid_constant__ PairParams p) {
   constexpr bool WIDE = SHAPE == kTwo;
-  constexpr uint32_t kStages = SHAPE == kTwo ? 4 : SHAPE == kNarrow ? 9 : 6;
-  constexpr uint32_t kStageBytes = kOperandBytes * (SHAPE == kTwo ? 12 : SHAPE == kNarrow ? 5 : 8) / 4;
+  constexpr int kSubs = subs_of(SHAPE);
+  constexpr uint32_t kStages = SHAPE == kOne ? 6 : 4;
+  constexpr uint32_t kBBytes = SHAPE == kNarrow ? kOperandBytes / 4 : kOperandBytes;   // B of a 64-wide block
+  constexpr uint32_t kStageBytes = kSubs * (kOperandBytes + (WIDE ? 2 : 1) * kBBytes);
   static_assert(kStages <= kMaxStages && kStages * kStageBytes <= kRingBytes);
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (1024 - smem_u32(raw) % 1024) % 1024;
@@ -639,42 +647,50 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       for (int32_t s = 0; s < t.steps; ++s, ++it) {
         if (!mbar_wait(&c->empty[st], phase, abort, p.dev_err)) { ok = false; break; }
         uint8_t* a = ring + st * kStageBytes;
-        uint8_t* b = a + kOperandBytes;
+        uint8_t* b = a + kSubs * kOperandBytes;
         // a step whose rows past the group's end are still to be zeroed lands on this CTA's own barrier
-        const bool fix = MODE == kWgrad && s + 1 == t.steps && t.tail % 16 != 0;
+        const bool last = s + 1 == t.steps;
+        const bool fix = MODE == kWgrad && last && t.tail % 16 != 0;
         const uint32_t bar = fix ? peer_addr(&c->tail[st], rank) : peer_addr(&c->full[st], 0);
-        const int32_t r = (t.first + s) * kStepK;   // where the step begins in the reduction
+        const int subs = kSubs > 1 && last && t.tail ? (t.tail + kStepK - 1) / kStepK : kSubs;
         if (elect_one()) {
-          pair_arrive_expect_tx(bar, bytes);
-          if constexpr (MODE == kRowsK) {
-            pair_load_3d(a, &p.a, bar, r, m, t.e);
-          } else if constexpr (MODE == kRowsMN) {
-            pair_load_3d(a, &p.a, bar, m, r, t.e);
-            pair_load_3d(a + kChunkBytes, &p.a, bar, m + 64, r, t.e);
-          } else {
-            const int32_t y = static_cast<int32_t>(t.row0) + r;
-            pair_load_2d(a, &p.a, bar, m, y);
-            pair_load_2d(a + kChunkBytes, &p.a, bar, m + 64, y);
-          }
-          if constexpr (MODE == kWgrad) {
-            const int32_t y = static_cast<int32_t>(t.row0) + r, x = t.n0 + static_cast<int32_t>(rank) * half;
-            pair_load_2d(b, &p.b[0], bar, x, y);
-            pair_load_2d(b + kChunkBytes, &p.b[0], bar, x + 64, y);
-          } else {
+          pair_arrive_expect_tx(bar, subs * bytes);
 #pragma unroll
-            for (int part = 0; part < (WIDE ? 2 : 1); ++part) {
-              if (part >= t.parts) break;
-              uint8_t* to = b + part * kOperandBytes;
-              int32_t y = static_cast<int32_t>(t.row0) + part * t.width + static_cast<int32_t>(rank) * half;
+          for (int sub = 0; sub < kSubs; ++sub) {
+            if (sub >= subs) break;
+            const int32_t r = ((t.first + s) * kSubs + sub) * kStepK;   // where the block begins in the reduction
+            if constexpr (MODE == kRowsK) {
+              pair_load_3d(a, &p.a, bar, r, m, t.e);
+            } else if constexpr (MODE == kRowsMN) {
+              pair_load_3d(a, &p.a, bar, m, r, t.e);
+              pair_load_3d(a + kChunkBytes, &p.a, bar, m + 64, r, t.e);
+            } else {
+              const int32_t y = static_cast<int32_t>(t.row0) + r;
+              pair_load_2d(a, &p.a, bar, m, y);
+              pair_load_2d(a + kChunkBytes, &p.a, bar, m + 64, y);
+            }
+            if constexpr (MODE == kWgrad) {
+              const int32_t y = static_cast<int32_t>(t.row0) + r, x = t.n0 + static_cast<int32_t>(rank) * half;
+              pair_load_2d(b, &p.b[0], bar, x, y);
+              pair_load_2d(b + kChunkBytes, &p.b[0], bar, x + 64, y);
+            } else {
 #pragma unroll
-              for (int i = kBoxes - 1; i >= 0; --i) {   // the rows' number in boxes of 128, 64, 32, 16
-                if (half & (16 << i)) {
-                  pair_load_2d(to, &p.b[i], bar, r, y);
-                  to += (16 << i) * kStepK * 2;
-                  y += 16 << i;
+              for (int part = 0; part < (WIDE ? 2 : 1); ++part) {
+                if (part >= t.parts) break;
+                uint8_t* to = b + part * kOperandBytes;
+                int32_t y = static_cast<int32_t>(t.row0) + part * t.width + static_cast<int32_t>(rank) * half;
+#pragma unroll
+                for (int i = kBoxes - 1; i >= 0; --i) {   // the rows' number in boxes of 128, 64, 32, 16
+                  if (half & (16 << i)) {
+                    pair_load_2d(to, &p.b[i], bar, r, y);
+                    to += (16 << i) * kStepK * 2;
+                    y += 16 << i;
+                  }
                 }
               }
             }
+            a += kOperandBytes;
+            b += kBBytes;
           }
         }
         __syncwarp();
@@ -709,7 +725,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         ok = mbar_wait(&c->full[st], phase, abort, p.dev_err);
         const uint32_t a = smem_u32(ring + st * kStageBytes);
         const uint64_t da = MODE == kRowsK ? sw128_desc(a) : sw128_mn_desc(a, kChunkBytes);
-        const int subs = last && t.tail ? (t.tail + 15) / 16 : kStepK / 16;
+        const int count = last && t.tail ? (t.tail + 15) / 16 : kSubs * kStepK / 16;   // products of 16
 #pragma unroll
         for (int part = 0; part < (WIDE ? 2 : 1); ++part) {
           if (part >= t.parts) break;
@@ -718,13 +734,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
-          const uint32_t b = a + (1 + part) * kOperandBytes;
+          const uint32_t b = a + kSubs * kOperandBytes + part * kOperandBytes;
           const uint64_t db = MODE == kWgrad ? sw128_mn_desc(b, kChunkBytes) : sw128_desc(b);
           if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < kStepK / 16; ++k)
-              if (k < subs)
-                pair_umma_f16(acc, da + k * (MODE == kRowsK ? 2 : 128), db + k * (MODE == kWgrad ? 128 : 2), idesc, s | k);
+            for (int k = 0; k < kSubs * kStepK / 16; ++k)   // the next 64-wide block of an operand: its bytes / 16 on
+              if (k < count)
+                pair_umma_f16(acc, da + k % 4 * (MODE == kRowsK ? 2 : 128) + k / 4 * (kOperandBytes >> 4),
+                              db + k % 4 * (MODE == kWgrad ? 128 : 2) + k / 4 * (kBBytes >> 4), idesc, s | k);
             if (part + 1 == t.parts) pair_umma_commit(&c->empty[st]);
             if (last) pair_umma_commit(&c->acc_full[buf]);
           }
@@ -810,7 +827,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         }
       }
     }
-    if (p.tma_out && lane == 0) bulk_wait_all();
+    if (p.tma_out && elect_one()) bulk_wait_all();
     if (MODE != kWgrad && ok) {   // rows of no group
       const int64_t gap = walk.lo + (p.g.rows - walk.carry);
       for (int64_t j = blockIdx.x; j < gap * p.splits; j += gridDim.x) {

@@ -7,7 +7,8 @@
 
 namespace hexmoe {
 
-// True in one lane of a converged warp.  tcgen05 and TMA instructions take their
+// True in one lane of a converged warp, always the same one (so that bulk groups
+// are committed and waited for by one thread).  tcgen05 and TMA instructions take their
 // operands from uniform registers: behind this test the compiler knows that one
 // lane runs, where behind `lane == 0` it guards every one of them.
 __device__ __forceinline__ bool elect_one() {
