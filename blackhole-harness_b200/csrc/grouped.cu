@@ -355,8 +355,12 @@ enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2 };
 //            as much of it as it can.  Waiting for a step, issuing its products and committing them
 //            takes the issuing warp some 450 cycles, more than narrow products run: twice the step
 //            (one token on 96 experts, 1536 x 2048: 64 wide 14.5 us, 128 wide 13.2).
-enum PairShape { kOne = 0, kTwo = 1, kNarrow = 2 };
-constexpr int subs_of(int shape) { return shape == kNarrow ? 2 : 1; }   // 64-wide blocks of a step
+//   kMiddle  up to 128: 4 steps of 48 KB, 128 wide
+enum PairShape { kOne = 0, kTwo = 1, kNarrow = 2, kMiddle = 3 };
+constexpr int subs_of(int shape) { return shape >= kNarrow ? 2 : 1; }   // 64-wide blocks of a step
+constexpr int span_of(int shape) {                                      // most rows of a tile
+  return shape == kTwo ? 512 : shape == kNarrow ? 64 : shape == kMiddle ? 128 : 256;
+}
 
 struct PairParams {
   CUtensorMap a;             // W (3-D: reduction or features, ..., expert) or dy
@@ -386,7 +390,6 @@ struct Tile {
 
 template <int MODE, int SHAPE>
 struct Walker {
-  [[maybe_unused]] static constexpr int32_t kSpan = SHAPE == kTwo ? 512 : SHAPE == kNarrow ? 64 : 256;   // most rows of a tile
   int32_t base = -32;
   int64_t carry = 0, lo = 0;
   int32_t upto = 0, mine = 0, total = 0;
@@ -394,6 +397,7 @@ struct Walker {
   bool bad = false;
 
   __device__ __forceinline__ bool find(const PairParams& p, int32_t unit, Tile& t) {
+    constexpr int32_t kSpan = span_of(SHAPE);
     const int32_t tile = p.splits > 1 ? unit / p.splits : unit;
     while (tile >= total) {
       if (base + 32 >= p.g.experts) return false;
@@ -598,7 +602,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   constexpr bool WIDE = SHAPE == kTwo;
   constexpr int kSubs = subs_of(SHAPE);
   constexpr uint32_t kStages = SHAPE == kOne ? 6 : 4;
-  constexpr uint32_t kBBytes = SHAPE == kNarrow ? kOperandBytes / 4 : kOperandBytes;   // B of a 64-wide block
+  constexpr uint32_t kBBytes = SHAPE == kNarrow ? kOperandBytes / 4 : SHAPE == kMiddle ? kOperandBytes / 2 : kOperandBytes;   // B of a 64-wide block
   constexpr uint32_t kStageBytes = kSubs * (kOperandBytes + (WIDE ? 2 : 1) * kBBytes);
   static_assert(kStages <= kMaxStages && kStages * kStageBytes <= kRingBytes);
   extern __shared__ uint8_t raw[];
@@ -895,6 +899,8 @@ int sm_count(int* sms) {
     for (const void* k : {reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kOne>),
                           reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kTwo>),
                           reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kNarrow>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kMiddle>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kMiddle>),
                           reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kOne>),
                           reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kTwo>),
                           reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kNarrow>),
@@ -938,10 +944,22 @@ int plan_splits(int64_t tiles, int64_t steps) {
   const int64_t s = std::min<int64_t>({kPairsPlanned / std::max<int64_t>(tiles, 1), steps / 4, kMaxSplits});
   return s >= 2 && steps - steps / s >= 16 ? static_cast<int>(s) : 1;
 }
-int64_t row_tiles(int64_t rows, int32_t experts, int32_t m_len) {
-  return (rows / 256 + std::min<int64_t>(experts, rows)) * ((m_len + 255) / 256);
-}
 int64_t pitch4(int64_t n) { return (n + 3) / 4 * 4; }   // f32 rows of whole 16-byte pieces
+
+// The shape for groups of this mean size.  Steps 128 wide pay up to tiles of 128 columns (32 experts x 30
+// rows x 512 x 2048: 11.9 us against 14.3).  Two accumulators a tile where groups of 257..512 rows are the
+// rule (the matrix is then loaded once a group, not twice: 96 x 341 rows, 1536 x 2048: 182 us against
+// 194) and still fill the machine; with larger groups the drain between tiles costs more than it saves
+// (8192^2 x 2048: 180 us against 174).
+PairShape rows_shape(int64_t rows, int32_t experts, int32_t m_len) {
+  if (rows <= 64 || rows <= 32ll * experts) return kNarrow;
+  if (rows <= 128 || rows <= 96ll * experts) return kMiddle;
+  const bool fills = static_cast<int64_t>(experts) * ((m_len + 255) / 256) >= 2 * kPairsPlanned;
+  return rows > 256ll * experts && rows <= 512ll * experts && fills ? kTwo : kOne;
+}
+int64_t row_tiles(int64_t rows, int32_t experts, int32_t m_len) {   // at most
+  return (rows / span_of(rows_shape(rows, experts, m_len)) + std::min<int64_t>(experts, rows)) * ((m_len + 255) / 256);
+}
 int rows_splits(int64_t rows, int32_t experts, int32_t m_len, int32_t red) {
   return plan_splits(row_tiles(rows, experts, m_len), (red + kStepK - 1) / kStepK);
 }
@@ -1109,16 +1127,13 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
     if (q.tma_out && rows >= 32)   // no full tile of 32 rows otherwise
       if (int rc = make_map(&q.out, out, dt, 2, width_out, rows, 1, 2 * ld_out, 0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
-    // Two accumulators a tile where groups of 257..512 rows are the rule (the matrix is then loaded once a
-    // group, not twice: 96 x 341 rows, 1536 x 2048: 182 us against 194) and still fill the machine; with
-    // larger groups the drain between tiles costs more than it saves (8192^2 x 2048: 180 us against 174).
-    const bool wide = rows > 256ll * experts && rows <= 512ll * experts && experts * q.m_tiles >= sms;
-    const PairShape shape = rows <= 64 ? kNarrow : wide ? kTwo : kOne;
+    const PairShape shape = rows_shape(rows, experts, width_out);
     auto launch = [&](auto mode) {
       constexpr int MODE = decltype(mode)::value;
-      return shape == kNarrow ? launch_pair<MODE, kNarrow>(q, tiles, sms, st)
-             : shape == kTwo  ? launch_pair<MODE, kTwo>(q, tiles, sms, st)
-                              : launch_pair<MODE, kOne>(q, tiles, sms, st);
+      return shape == kNarrow   ? launch_pair<MODE, kNarrow>(q, tiles, sms, st)
+             : shape == kMiddle ? launch_pair<MODE, kMiddle>(q, tiles, sms, st)
+             : shape == kTwo    ? launch_pair<MODE, kTwo>(q, tiles, sms, st)
+                                : launch_pair<MODE, kOne>(q, tiles, sms, st);
     };
     cudaError_t e = transpose ? launch(std::integral_constant<int, kRowsMN>{})
                               : launch(std::integral_constant<int, kRowsK>{});
