@@ -380,12 +380,14 @@ struct PairParams {
 
 // One tile: expert, M offset, N offset (a row offset within the group in the row
 // products) and width, of `parts` accumulators side by side; row0 its first row,
-// valid its real rows; steps of the reduction from `first` on, the last one of
+// valid its real columns; steps of the reduction from `first` on, the last one of
 // `tail` (0: full); split: the run of the reduction that these are.
 struct Tile {
   int32_t e, m0, n0, width, parts, first, steps, tail, split;
   int64_t row0;
   int32_t valid;
+  // The columns of accumulator i: what is left of the tile, in whole 32s (341 rows: 192 and 160).
+  __device__ __forceinline__ int32_t columns(int i) const { return min(width, (valid - i * width + 31) / 32 * 32); }
 };
 
 template <int MODE, int SHAPE>
@@ -426,10 +428,9 @@ struct Walker {
     if constexpr (MODE == kWgrad) {
       t.m0 = local / p.n_tiles * 256;
       t.n0 = local % p.n_tiles * p.tile_n;
-      t.width = p.tile_n;
+      t.width = t.valid = p.tile_n;
       t.parts = 1;
       t.row0 = b;
-      t.valid = 0;
       t.steps = static_cast<int32_t>((e - b + kStepK - 1) / kStepK);
       t.tail = static_cast<int32_t>((e - b) % kStepK);
     } else {
@@ -644,10 +645,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     uint32_t it = 0, st = 0, phase = 1;
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
-      const int32_t half = t.width / 2;
+      const int32_t halves[2] = {t.columns(0) / 2, WIDE && t.parts > 1 ? t.columns(1) / 2 : 0};
       const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128;
       const uint32_t bytes =
-          kOperandBytes + (MODE == kWgrad ? kOperandBytes : static_cast<uint32_t>(t.parts * half) * kStepK * 2);
+          kOperandBytes + (MODE == kWgrad ? kOperandBytes : static_cast<uint32_t>(halves[0] + halves[1]) * kStepK * 2);
       for (int32_t s = 0; s < t.steps; ++s, ++it) {
         if (!mbar_wait(&c->empty[st], phase, abort, p.dev_err)) { ok = false; break; }
         uint8_t* a = ring + st * kStageBytes;
@@ -674,13 +675,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
               pair_load_2d(a + kChunkBytes, &p.a, bar, m + 64, y);
             }
             if constexpr (MODE == kWgrad) {
-              const int32_t y = static_cast<int32_t>(t.row0) + r, x = t.n0 + static_cast<int32_t>(rank) * half;
+              const int32_t y = static_cast<int32_t>(t.row0) + r, x = t.n0 + static_cast<int32_t>(rank) * halves[0];
               pair_load_2d(b, &p.b[0], bar, x, y);
               pair_load_2d(b + kChunkBytes, &p.b[0], bar, x + 64, y);
             } else {
 #pragma unroll
               for (int part = 0; part < (WIDE ? 2 : 1); ++part) {
                 if (part >= t.parts) break;
+                const int32_t half = halves[part];
                 uint8_t* to = b + part * kOperandBytes;
                 int32_t y = static_cast<int32_t>(t.row0) + part * t.width + static_cast<int32_t>(rank) * half;
 #pragma unroll
@@ -722,8 +724,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
       if (t.steps == 0) continue;   // an empty group's gradient: zeros, without an accumulator
-      const uint32_t idesc = umma_idesc(p.bf16, 256, t.width) | (MODE != kRowsK ? kIdescMajorA : 0) |
-                             (MODE == kWgrad ? kIdescMajorB : 0);
+      constexpr uint32_t kMajors = (MODE != kRowsK ? kIdescMajorA : 0) | (MODE == kWgrad ? kIdescMajorB : 0);
+      const uint32_t idescs[2] = {umma_idesc(p.bf16, 256, t.columns(0)) | kMajors,
+                                  WIDE && t.parts > 1 ? umma_idesc(p.bf16, 256, t.columns(1)) | kMajors : 0};
       for (int32_t s = 0; ok && s < t.steps; ++s) {
         const bool last = s + 1 == t.steps;
         ok = mbar_wait(&c->full[st], phase, abort, p.dev_err);
@@ -745,7 +748,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             for (int k = 0; k < kSubs * kStepK / 16; ++k)   // the next 64-wide block of an operand: its bytes / 16 on
               if (k < count)
                 pair_umma_f16(acc, da + k % 4 * (MODE == kRowsK ? 2 : 128) + k / 4 * (kOperandBytes >> 4),
-                              db + k % 4 * (MODE == kWgrad ? 128 : 2) + k / 4 * (kBBytes >> 4), idesc, s | k);
+                              db + k % 4 * (MODE == kWgrad ? 128 : 2) + k / 4 * (kBBytes >> 4), idescs[part], s | k);
             if (part + 1 == t.parts) pair_umma_commit(&c->empty[st]);
             if (last) pair_umma_commit(&c->acc_full[buf]);
           }
@@ -1170,6 +1173,7 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
   if (out_dtype != dtype && out_dtype != HEXMOE_F32) return report_error(HEXMOE_E_DTYPE, "hexmoe_grouped_wgrad: out is of x's dtype or F32");
   if (int rc = check_groups(what, rows, experts, offsets, offsets_dtype)) return rc;
   if (n <= 0 || k <= 0 || n > (1 << 24) || k > (1 << 24)) return arg_error("%s: n %d, k %d", what, n, k);
+  if (rows >= 1ll << 28) return arg_error("%s: %lld rows", what, static_cast<long long>(rows));
   if (ld_dy < n || ld_x < k || ld_out < k || stride_out < static_cast<int64_t>(n - 1) * ld_out + k)
     return arg_error("%s: a stride is shorter than what it spans", what);
   if (!out || (rows && (!dy || !x)) || off_by(dy, 2) || off_by(x, 2) || off_by(out, out_dtype == HEXMOE_F32 ? 4 : 2))

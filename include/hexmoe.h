@@ -399,7 +399,7 @@ HEXMOE_API int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int
  * x[r, :k], out [experts, n, k] (zero for an empty group); with dy = x the
  * Hessians x_e^T x_e that GPTQ rounding takes.  accumulate != 0 adds to what out
  * holds (rounded once, after the addition).  dy, x: BF16 or F16; out: the same or
- * F32.  workspace: as for hexmoe_grouped_mm. */
+ * F32.  Fewer than 2^28 rows.  workspace: as for hexmoe_grouped_mm. */
 HEXMOE_API size_t hexmoe_grouped_wgrad_workspace_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k);
 HEXMOE_API int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int32_t dtype,
                                     int64_t rows, int32_t experts, int32_t n, int32_t k, const void* offsets,
