@@ -388,6 +388,7 @@ class _ExpertMLP(torch.autograd.Function):
         return combine_rows(grouped_mm(act, w2, offsets), T, k, rows)
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
         xs, h, act, weight, offsets, rows, w13, w2, *plan = ctx.saved_tensors
         T, k = ctx.tokens, ctx.topk

@@ -556,6 +556,47 @@ def test_expert_mlp(tokens, E, k, H, I):
 
 
 @pytest.mark.gpu
+def test_expert_mlp_without_tokens_and_with_bad_ids():
+    """No tokens; ids of no expert: they add nothing, have no gradient, and set the device error word."""
+    from blackhole_b200.hex_moe import device_status
+    w13, w2 = normal((4, 64, 32), BF16, 73).to(DEV).requires_grad_(), normal((4, 32, 32), BF16, 74).to(DEV).requires_grad_()
+    out = experts.expert_mlp(torch.zeros(0, 32, dtype=BF16, device=DEV), torch.zeros(0, 2, device=DEV),
+                             torch.zeros(0, 2, dtype=torch.int64, device=DEV), w13, w2)
+    out.sum().backward()
+    assert out.shape == (0, 32) and not w13.grad.any() and not w2.grad.any()
+    x, weights = normal((5, 32), BF16, 75).to(DEV).requires_grad_(), torch.rand(5, 2, device=DEV).requires_grad_()
+    ids = torch.tensor([[0, 1], [2, -1], [4, 3], [3, 0], [9, -7]], device=DEV)
+    out = experts.expert_mlp(x, weights, ids, w13, w2)
+    out.backward(torch.ones_like(out).expand_as(out))
+    assert device_status(0) & 2
+    good = (ids >= 0) & (ids < 4)
+    assert not weights.grad[~good].any() and weights.grad[good].all() and not out[4].any() and not x.grad[4].any()
+    same = experts.expert_mlp(x, torch.where(good, weights, 0), ids.clamp(0, 3), w13, w2)
+    assert torch.equal(same, out)
+
+
+@pytest.mark.gpu
+def test_ordinary_calls_and_the_checked_ones_agree():
+    """What _call takes and what goes through Python's checks is the same call: an `out` sends it there."""
+    off = offsets_of([40, 0, 88]).to(DEV)
+    x, w, dy = normal((128, 72), BF16, 76).to(DEV), normal((3, 136, 72), BF16, 77).to(DEV), normal((128, 136), BF16, 78).to(DEV)
+    out = torch.empty(128, 136, dtype=BF16, device=DEV)
+    assert torch.equal(experts.grouped_mm(x, w, off), experts.grouped_mm(x, w, off, out=out))
+    dw = torch.empty(3, 136, 72, device=DEV)
+    assert torch.equal(experts.grouped_wgrad(dy, x, off, out_dtype=F32), experts.grouped_wgrad(dy, x, off, out=dw))
+    weight, dact = torch.rand(128, device=DEV), dy[:, :68].contiguous()
+    dh, dweight = experts.swiglu_backward(dact, dy, weight)
+    again, dweight2 = experts.swiglu_backward(dact, dy, weight, out=torch.empty_like(dy))
+    assert torch.equal(dh, again) and torch.equal(dweight, dweight2)
+    strided = torch.randn(256, device=DEV)[::2]
+    assert torch.equal(experts.swiglu(dy, strided), experts.swiglu(dy, strided.contiguous()))
+    a, b = torch.randn(50, device=DEV), torch.randn(7, 9, device=DEV)
+    want = experts.clip_grad_norm([a.clone(), b.clone()], 1.0)
+    got = experts.clip_grad_norm([a, b.t().contiguous().t()], 1.0)
+    assert abs(float(want) - float(got)) <= 2.0 ** -22 * float(want)
+
+
+@pytest.mark.gpu
 def test_expert_mlp_equals_hex_moe_on_dequantized_stacks():
     """On the stacks that dequant_all makes, the training layer and the HEX layer agree to the layer's tolerance."""
     from blackhole_b200.hex_moe import HexTier, dequant_all, hex_moe
@@ -600,6 +641,18 @@ def test_operators_on_another_stream():
         assert float(norm) > 1.0 and float(got.float().norm()) < 1.01
     side.synchronize()
     assert abs(float(want.float().norm()) - float(norm)) <= 2.0 ** -20 * float(norm)
+
+
+@pytest.mark.gpu
+def test_healing_example():
+    """The operators together: what training and the Hessians are for shows on held-out rows."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("heal_experts", ROOT / "examples" / "heal_experts.py")
+    heal = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(heal)
+    got = heal.main(steps=80)
+    assert got["pruned and healed"] < got["pruned"]
+    assert got["pruned, healed and quantized"] < got["pruned and quantized"] < got["pruned and quantized to the nearest level"]
 
 
 # ------------------------------------------------------------------ refusals
