@@ -436,12 +436,13 @@ struct Walker {
     } else {
       const int32_t size = static_cast<int32_t>(e - b), tiles = (size + kSpan - 1) / kSpan;
       const int32_t span = (size + tiles - 1) / tiles;
-      t.parts = SHAPE == kTwo && span > 256 ? 2 : 1;
-      t.width = ((span + t.parts - 1) / t.parts + 31) / 32 * 32;
+      const int32_t parts = SHAPE == kTwo && span > 256 ? 2 : 1;
+      t.width = ((span + parts - 1) / parts + 31) / 32 * 32;
       t.m0 = local / tiles * 256;
-      t.n0 = local % tiles * t.parts * t.width;
+      t.n0 = local % tiles * parts * t.width;
       t.row0 = b + t.n0;
-      t.valid = min(t.parts * t.width, size - t.n0);
+      t.valid = min(parts * t.width, size - t.n0);
+      t.parts = t.valid > t.width ? 2 : 1;   // the last tile of a group may end within its first accumulator
       constexpr int32_t kWidth = kStepK * subs_of(SHAPE);
       t.steps = (p.red + kWidth - 1) / kWidth;
       t.tail = p.red % kWidth;

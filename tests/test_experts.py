@@ -250,6 +250,30 @@ def test_grouped_mm_few_rows(sizes, transpose):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("transpose", [False, True])
+def test_grouped_mm_uneven_groups_of_a_training_step(transpose):
+    """Mean group sizes between 257 and 512, groups far from the mean: tiles of two accumulators, the
+    last of a group ending within the first (1, 256), at its end and just past it."""
+    E, n, k = 80, 264, 72     # two 256-row M sides an expert: enough tiles to fill the machine
+    if transpose:
+        n, k = k, n
+    sizes = [4097, 4096, 513, 512, 511, 257, 256, 255, 1, 0, 769, 1025, 1024, 300, 2049, 641] + [205] * 64
+    assert 256 * E < sum(sizes) <= 512 * E
+    rows, width = sum(sizes), n if transpose else k
+    g = torch.Generator(device=DEV).manual_seed(82)
+    x = torch.randn(rows, width, generator=g, device=DEV).to(BF16)
+    w = torch.randn(E, n, k, generator=g, device=DEV).mul(0.1).to(BF16)
+    off = offsets_of(sizes)
+    got = experts.grouped_mm(x, w, off.to(DEV), transpose=transpose)
+    xd, wd, at = x.double(), w.double(), off.tolist()
+    want, mass = torch.zeros_like(got, dtype=torch.float64), torch.zeros_like(got, dtype=torch.float64)
+    for e in range(E):
+        r, m = slice(at[e], at[e + 1]), wd[e] if transpose else wd[e].t()
+        want[r], mass[r] = xd[r] @ m, xd[r].abs() @ m.abs()
+    assert_sum(got, want.cpu(), mass.cpu(), width, BF16)
+
+
+@pytest.mark.gpu
 def test_grouped_products_repeat_bit_for_bit():
     sizes = [0, 300, 41, 5, 600]
     off = offsets_of(sizes).to(DEV)
