@@ -40,7 +40,8 @@ __device__ __forceinline__ T from_f32(float v) {
   else return __float2bfloat16_rn(v);
 }
 
-// V consecutive elements as one register load or store of up to 16 bytes.
+// V consecutive elements as one register load or store of up to 16 bytes; their
+// 32-bit words by value (an address taken would put them into local memory).
 template <int BYTES>
 struct RawOf;
 template <> struct RawOf<16> { using type = uint4; };
@@ -48,51 +49,60 @@ template <> struct RawOf<8> { using type = uint2; };
 template <> struct RawOf<4> { using type = uint32_t; };
 template <> struct RawOf<2> { using type = uint16_t; };
 
+__device__ __forceinline__ uint32_t word(const uint4& r, int i) { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }
+__device__ __forceinline__ uint32_t word(const uint2& r, int i) { return i == 0 ? r.x : r.y; }
+__device__ __forceinline__ uint32_t word(const uint32_t& r, int) { return r; }
+__device__ __forceinline__ void from_words(uint4& r, const uint32_t (&w)[4]) { r = make_uint4(w[0], w[1], w[2], w[3]); }
+__device__ __forceinline__ void from_words(uint2& r, const uint32_t (&w)[4]) { r = make_uint2(w[0], w[1]); }
+__device__ __forceinline__ void from_words(uint32_t& r, const uint32_t (&w)[4]) { r = w[0]; }
+
 template <typename T, int V>
 struct Vec {
   using Raw = typename RawOf<static_cast<int>(sizeof(T)) * V>::type;
-  [[maybe_unused]] static constexpr int kWords = static_cast<int>(sizeof(Raw) / 4);
-  static __device__ __forceinline__ void unpack(const Raw& r, float (&x)[V]) {
-    if constexpr (V == 1 && sizeof(T) == 2) {
-      x[0] = to_f32(reinterpret_cast<const T&>(r));
-    } else {
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+  static __device__ __forceinline__ void unpack(Raw r, float (&x)[V]) {
+    if constexpr (std::is_same_v<T, float>) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        if constexpr (std::is_same_v<T, float>) {
-          x[i] = __uint_as_float(w[i]);
-        } else if constexpr (std::is_same_v<T, __half>) {
-          const float2 f = __half22float2(reinterpret_cast<const __half2&>(w[i]));
-          x[2 * i] = f.x;
-          x[2 * i + 1] = f.y;
+      for (int i = 0; i < V; ++i) x[i] = __uint_as_float(word(r, i));
+    } else if constexpr (V == 1) {
+      if constexpr (std::is_same_v<T, __half>) x[0] = __half2float(__ushort_as_half(r));
+      else x[0] = __bfloat162float(__ushort_as_bfloat16(r));
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const uint32_t w = word(r, i);
+        if constexpr (std::is_same_v<T, __half>) {
+          x[2 * i] = __half2float(__ushort_as_half(static_cast<uint16_t>(w)));
+          x[2 * i + 1] = __half2float(__ushort_as_half(static_cast<uint16_t>(w >> 16)));
         } else {
-          x[2 * i] = __uint_as_float(w[i] << 16);
-          x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+          x[2 * i] = __uint_as_float(w << 16);
+          x[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
         }
       }
     }
   }
   static __device__ __forceinline__ Raw pack(const float (&x)[V]) {
-    Raw r;
     if constexpr (V == 1 && sizeof(T) == 2) {
-      const T t = from_f32<T>(x[0]);
-      r = reinterpret_cast<const uint16_t&>(t);
+      if constexpr (std::is_same_v<T, __half>) return __half_as_ushort(__float2half_rn(x[0]));
+      else return __bfloat16_as_ushort(__float2bfloat16_rn(x[0]));
     } else {
-      uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+      uint32_t w[4] = {};
+      constexpr int kWords = static_cast<int>(sizeof(Raw) / 4);
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
         if constexpr (std::is_same_v<T, float>) {
           w[i] = __float_as_uint(x[i]);
         } else if constexpr (std::is_same_v<T, __half>) {
-          const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-          w[i] = reinterpret_cast<const uint32_t&>(h);
+          w[i] = __half_as_ushort(__float2half_rn(x[2 * i])) |
+                 static_cast<uint32_t>(__half_as_ushort(__float2half_rn(x[2 * i + 1]))) << 16;
         } else {
           const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
-          w[i] = reinterpret_cast<const uint32_t&>(h);
+          w[i] = __bfloat16_as_ushort(h.x) | static_cast<uint32_t>(__bfloat16_as_ushort(h.y)) << 16;
         }
       }
+      Raw r;
+      from_words(r, w);
+      return r;
     }
-    return r;
   }
 };
 
@@ -274,9 +284,12 @@ int run_swiglu(const char* what, const SwigluParams& p, int32_t dtype, bool bwd,
 // blocks move through the chunks side by side, the second kernel backwards: what
 // the first one read last is still in L2.
 constexpr int kClipThreads = 256;
-constexpr int kClipPerSm = 3;      // with 16384-value chunks, 604 M bf16 values copied: 578 us; 2, 4, 5 an SM: 678, 606, 790
+// Blocks an SM, with two loads in flight a thread in the scaling and four in the norm: more requests under
+// way than this mix reads and writes too finely for HBM.  604 M bf16 values copied: 566 us; with four
+// loads in the scaling 578, with 3 or 5 blocks 596 and 627 (300 M f32: 560; 579, 604, 616).
+constexpr int kClipPerSm = 4;
 // Values of a chunk: long runs for HBM, but enough chunks for every block of a short list
-// (40 tensors of 1.5 M values in all: 4096 values 9.6 us, 16384 17.7).
+// (40 tensors of 1.5 M values in all: 4096 values 8.0 us, 16384 17.7).
 constexpr int kClipChunk = 16384, kClipShortChunk = 4096;
 constexpr int64_t kClipShort = 16 << 20;
 constexpr int kClipSmallList = 64;
@@ -287,7 +300,6 @@ struct ClipEntry {
   void* dst;
   int64_t n;
   uint32_t first;   // its first chunk
-  int16_t src_type, dst_type;
 };
 template <int CAP>
 struct ClipTable {
@@ -371,12 +383,11 @@ __device__ __forceinline__ void clip_read(const T* src, int count, ClipAcc<INF>&
 
 // dst = src * c over the `count` values of a chunk, by one block.  Vectors where
 // source and destination share their place within a vector (every in-place
-// call), else one value at a time.  Not inlined: nine pairs of types in one
-// kernel body spill.
+// call), else one value at a time.
 template <typename T, typename D>
-__device__ __noinline__ void clip_scale(const T* src, D* dst, int count, float c) {
+__device__ __forceinline__ void clip_scale(const T* src, D* dst, int count, float c) {
   constexpr int V = 16 / (sizeof(T) > sizeof(D) ? sizeof(T) : sizeof(D));   // 16 bytes of the wider type
-  constexpr int U = 4;
+  constexpr int U = 2;
   const int off = static_cast<int>(reinterpret_cast<uintptr_t>(src) % (V * sizeof(T)) / sizeof(T));
   if (static_cast<int>(reinterpret_cast<uintptr_t>(dst) % (V * sizeof(D)) / sizeof(D)) != off) {
     for (int i = threadIdx.x; i < count; i += kClipThreads) dst[i] = from_f32<D>(to_f32(src[i]) * c);
@@ -420,7 +431,7 @@ __device__ __forceinline__ int clip_entry(const ClipTable<CAP>& t, uint32_t c) {
   return lo;
 }
 
-template <int CAP, bool INF>
+template <typename T, int CAP, bool INF>
 __global__ void __launch_bounds__(kClipThreads, kClipPerSm)
     clip_norm_kernel(const __grid_constant__ ClipTable<CAP> t, double* partial) {
   pdl_wait();
@@ -433,9 +444,7 @@ __global__ void __launch_bounds__(kClipThreads, kClipPerSm)
       const ClipEntry& e = t.e[i];
       const int64_t a = static_cast<int64_t>(c - e.first) * t.chunk;
       const int count = static_cast<int>(min(e.n - a, static_cast<int64_t>(t.chunk)));
-      if (e.src_type == HEXMOE_F32) clip_read(static_cast<const float*>(e.src) + a, count, acc);
-      else if (e.src_type == HEXMOE_F16) clip_read(static_cast<const __half*>(e.src) + a, count, acc);
-      else clip_read(static_cast<const __nv_bfloat16*>(e.src) + a, count, acc);
+      clip_read(static_cast<const T*>(e.src) + a, count, acc);
     }
   }
   __shared__ double part[kClipThreads / 32];
@@ -454,7 +463,7 @@ __global__ void __launch_bounds__(kClipThreads, kClipPerSm)
   }
 }
 
-template <int CAP, bool INF>
+template <typename T, typename D, int CAP, bool INF>
 __global__ void __launch_bounds__(kClipThreads, kClipPerSm)
     clip_scale_kernel(const __grid_constant__ ClipTable<CAP> t, const double* partial, int32_t partials,
                       float max_norm, int32_t copies, float* norm_out) {
@@ -490,14 +499,7 @@ __global__ void __launch_bounds__(kClipThreads, kClipPerSm)
     if (coef == 1.f && e.dst == e.src) continue;
     const int64_t a = static_cast<int64_t>(c - e.first) * t.chunk;
     const int count = static_cast<int>(min(e.n - a, static_cast<int64_t>(t.chunk)));
-    auto to = [&](auto* src) {
-      if (e.dst_type == HEXMOE_F32) clip_scale(src, static_cast<float*>(e.dst) + a, count, coef);
-      else if (e.dst_type == HEXMOE_F16) clip_scale(src, static_cast<__half*>(e.dst) + a, count, coef);
-      else clip_scale(src, static_cast<__nv_bfloat16*>(e.dst) + a, count, coef);
-    };
-    if (e.src_type == HEXMOE_F32) to(static_cast<const float*>(e.src) + a);
-    else if (e.src_type == HEXMOE_F16) to(static_cast<const __half*>(e.src) + a);
-    else to(static_cast<const __nv_bfloat16*>(e.src) + a);
+    clip_scale(static_cast<const T*>(e.src) + a, static_cast<D*>(e.dst) + a, count, coef);
   }
 }
 
@@ -505,39 +507,68 @@ int clip_grid(uint32_t chunks, int sms) {
   return static_cast<int>(std::max<uint32_t>(1, std::min<uint32_t>(chunks, kClipPerSm * sms)));
 }
 
-template <int CAP, bool INF>
-cudaError_t launch_clip(const std::vector<ClipEntry>& list, double* partial, int sms, float max_norm, bool copies,
-                        float* norm_out, cudaStream_t st) {
-  const size_t groups = std::max<size_t>(1, (list.size() + CAP - 1) / CAP);
+// The tensors of one pair of types, and what a call passes along its launches.
+struct ClipCall {
+  std::vector<ClipEntry> lists[3][3];   // [source type][destination type]
+  double* partial;
   int32_t partials = 0;
-  ClipTable<CAP> t;
-  int64_t values = 0;
-  for (const ClipEntry& e : list) values += e.n;
-  t.chunk = values < kClipShort ? kClipShortChunk : kClipChunk;
-  auto fill = [&](size_t g) {
-    const size_t a = g * CAP, b = std::min(list.size(), a + CAP);
-    t.count = static_cast<int32_t>(b - a);
-    t.chunks = 0;
-    for (size_t i = a; i < b; ++i) {
-      t.e[i - a] = list[i];
-      t.e[i - a].first = t.chunks;
-      t.chunks += static_cast<uint32_t>((list[i].n + t.chunk - 1) / t.chunk);
-    }
-    return clip_grid(t.chunks, sms);
-  };
-  cudaLaunchAttribute attr;
-  for (size_t g = 0; g < groups; ++g) {
-    const int grid = fill(g);
-    const cudaLaunchConfig_t cfg = launch_config(dim3(grid), kClipThreads, st, &attr);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, clip_norm_kernel<CAP, INF>, t, partial + partials);
-    if (e != cudaSuccess) return e;
-    partials += grid;
+  int32_t chunk, copies;
+  int sms;
+  float max_norm;
+  float* norm_out;
+  cudaStream_t st;
+};
+
+template <int CAP>
+int fill_table(ClipTable<CAP>& t, const std::vector<ClipEntry>& list, size_t from, const ClipCall& c) {
+  const size_t to = std::min(list.size(), from + CAP);
+  t.count = static_cast<int32_t>(to - from);
+  t.chunks = 0;
+  t.chunk = c.chunk;
+  for (size_t i = from; i < to; ++i) {
+    t.e[i - from] = list[i];
+    t.e[i - from].first = t.chunks;
+    t.chunks += static_cast<uint32_t>((list[i].n + t.chunk - 1) / t.chunk);
   }
-  for (size_t g = groups; g-- > 0;) {   // the table still holds the last group
-    const int grid = g + 1 == groups ? clip_grid(t.chunks, sms) : fill(g);
-    const cudaLaunchConfig_t cfg = launch_config(dim3(grid), kClipThreads, st, &attr);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, clip_scale_kernel<CAP, INF>, t, static_cast<const double*>(partial),
-                                             partials, max_norm, static_cast<int32_t>(copies), g == 0 ? norm_out : nullptr);
+  return clip_grid(t.chunks, c.sms);
+}
+
+// All norm kernels of the call, then all scale kernels, the lists in the reverse order.
+template <typename T, typename D, int CAP, bool INF>
+cudaError_t launch_clip_list(const std::vector<ClipEntry>& list, bool scale, ClipCall& c) {
+  ClipTable<CAP> t;
+  cudaLaunchAttribute attr;
+  const size_t tables = (list.size() + CAP - 1) / CAP;
+  for (size_t i = 0; i < tables; ++i) {
+    const int grid = fill_table(t, list, (scale ? tables - 1 - i : i) * CAP, c);
+    const cudaLaunchConfig_t cfg = launch_config(dim3(grid), kClipThreads, c.st, &attr);
+    cudaError_t e;
+    if (scale) {
+      e = cudaLaunchKernelEx(&cfg, clip_scale_kernel<T, D, CAP, INF>, t, static_cast<const double*>(c.partial), c.partials,
+                             c.max_norm, c.copies, c.norm_out);
+    } else {
+      e = cudaLaunchKernelEx(&cfg, clip_norm_kernel<T, CAP, INF>, t, c.partial + c.partials);
+      c.partials += grid;
+    }
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+template <int CAP, bool INF>
+cudaError_t launch_clip(ClipCall& c) {
+  for (int i = 0; i < 18; ++i) {
+    const bool scale = i >= 9;
+    const int pair = scale ? 17 - i : i, src = pair / 3, dst = pair % 3;
+    const std::vector<ClipEntry>& list = c.lists[src][dst];
+    auto to = [&](auto s) {
+      using T = decltype(s);
+      return dst == HEXMOE_F32   ? launch_clip_list<T, float, CAP, INF>(list, scale, c)
+             : dst == HEXMOE_F16 ? launch_clip_list<T, __half, CAP, INF>(list, scale, c)
+                                 : launch_clip_list<T, __nv_bfloat16, CAP, INF>(list, scale, c);
+    };
+    if (list.empty()) continue;
+    const cudaError_t e = src == HEXMOE_F32 ? to(float{}) : src == HEXMOE_F16 ? to(__half{}) : to(__nv_bfloat16{});
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -587,7 +618,8 @@ int hexmoe_swiglu_backward(const void* dact, int64_t ld_dact, const void* h, int
 
 size_t hexmoe_clip_grad_norm_workspace_bytes(int32_t tensors) {
   if (tensors < 0) return 0;
-  const size_t groups = tensors <= kClipSmallList ? 1 : (static_cast<size_t>(tensors) + kClipList - 1) / kClipList;
+  // launches of the norm: one for every pair of types, more for lists past a table's length
+  const size_t groups = std::max(1, std::min(tensors, 9)) + static_cast<size_t>(tensors) / kClipList;
   return groups * kClipPerSm * kClipMaxSms * sizeof(double);
 }
 
@@ -607,15 +639,14 @@ int hexmoe_clip_grad_norm(int32_t tensors, const void* const* src, const int64_t
   if (int rc = current_sms(&sms)) return rc;
   sms = std::min(sms, kClipMaxSms);
   try {
-    std::vector<ClipEntry> list;
     struct Span {
       uintptr_t a, b;
       bool written;
     };
     std::vector<Span> spans;
-    list.reserve(tensors);
     spans.reserve(2 * static_cast<size_t>(tensors));
-    bool copies = false;
+    ClipCall call{};
+    int64_t values = 0;
     for (int32_t i = 0; i < tensors; ++i) {
       const int32_t st = src_dtypes[i], dt = dst ? dst_dtypes[i] : st;
       if (!known_dtype(st) || !known_dtype(dt)) return report_error(HEXMOE_E_DTYPE, "hexmoe_clip_grad_norm: bad dtype");
@@ -625,11 +656,12 @@ int hexmoe_clip_grad_norm(int32_t tensors, const void* const* src, const int64_t
       if (!src[i] || !d) return arg_error("hexmoe_clip_grad_norm: null pointer");
       const uintptr_t sa = reinterpret_cast<uintptr_t>(src[i]), da = reinterpret_cast<uintptr_t>(d);
       if (sa % dtype_bytes(st) || da % dtype_bytes(dt)) return arg_error("hexmoe_clip_grad_norm: tensor %d is not aligned to its element", i);
-      list.push_back({src[i], d, counts[i], 0, static_cast<int16_t>(st), static_cast<int16_t>(dt)});
+      call.lists[st][dt].push_back({src[i], d, counts[i], 0});
+      values += counts[i];
       spans.push_back({da, da + counts[i] * dtype_bytes(dt), true});
       if (sa != da) spans.push_back({sa, sa + counts[i] * dtype_bytes(st), false});
       else if (st != dt) return arg_error("hexmoe_clip_grad_norm: tensor %d is written in place with another dtype", i);
-      copies |= sa != da;
+      call.copies |= sa != da;
     }
     // a value that is written may be reached through one entry only: overlapping
     // entries would be scaled twice, or read after they were scaled
@@ -640,14 +672,19 @@ int hexmoe_clip_grad_norm(int32_t tensors, const void* const* src, const int64_t
       any_end = std::max(any_end, s.b);
       if (s.written) written_end = std::max(written_end, s.b);
     }
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    double* partial = static_cast<double*>(workspace);
+    call.partial = static_cast<double*>(workspace);
+    call.chunk = values < kClipShort ? kClipShortChunk : kClipChunk;
+    call.sms = sms;
+    call.max_norm = max_norm;
+    call.norm_out = norm_out;
+    call.st = static_cast<cudaStream_t>(stream);
+    if (values == 0) {   // no values: a norm of 0
+      const cudaError_t e = cudaMemsetAsync(norm_out, 0, sizeof(float), call.st);
+      return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, "hexmoe_clip_grad_norm");
+    }
     const bool small = tensors <= kClipSmallList;
-    const cudaError_t e =
-        inf_norm ? (small ? launch_clip<kClipSmallList, true>(list, partial, sms, max_norm, copies, norm_out, st)
-                          : launch_clip<kClipList, true>(list, partial, sms, max_norm, copies, norm_out, st))
-                 : (small ? launch_clip<kClipSmallList, false>(list, partial, sms, max_norm, copies, norm_out, st)
-                          : launch_clip<kClipList, false>(list, partial, sms, max_norm, copies, norm_out, st));
+    const cudaError_t e = inf_norm ? (small ? launch_clip<kClipSmallList, true>(call) : launch_clip<kClipList, true>(call))
+                                   : (small ? launch_clip<kClipSmallList, false>(call) : launch_clip<kClipList, false>(call));
     return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, "hexmoe_clip_grad_norm");
   } catch (const std::exception&) {
     return report_error(HEXMOE_E_ARG, "hexmoe_clip_grad_norm: out of host memory");
