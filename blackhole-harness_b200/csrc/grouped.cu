@@ -72,7 +72,8 @@ __device__ __forceinline__ GroupScan scan_groups(const Groups& g, int base, int6
 // out(i, j) = sum_r A(i, r) B(j, r) over operands with any element strides:
 // 64 x 64 tiles, mma.sync over 32-wide reduction steps staged in shared memory
 // with element loads.  It takes what the TMA kernels cannot address (a base or
-// row stride that is no multiple of 16 bytes).
+// row stride that is no multiple of 16 bytes); bound by those loads (weight gradient of
+// 32768 rows, 96 x 1536 x 2048: 5.8 ms, where the tensor-memory kernel takes 0.2).
 constexpr int kPlainTile = 64, kPlainK = 32, kPlainThreads = 128, kPlainPitch = kPlainK + 8;
 
 struct PlainParams {
@@ -334,6 +335,11 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 // 12 warps a CTA: 0 loads, 1 issues the products (the leader's), 2 zeroes tails
 // (weight gradient), 4..11 write results.  Each walks the groups' offsets by
 // itself, so that no size is known on the host.
+//
+// Measured, bf16, 96 experts, 1536 x 2048: 512 rows 91 us (HBM, 6.7 TB/s); 32768 rows
+// 174..184 us (1120..1180 TFLOP/s; HBM and tensor cores, each of which alone takes
+// 145); the weight gradient of those 194..203 us (604 MB written, which takes a
+// plain fill 157).  A single product of 8192 x 8192 x 2048: 174 us (1580 TFLOP/s).
 constexpr int kMaxStages = 6;
 constexpr int kStepK = 64;
 constexpr uint32_t kOperandBytes = 128 * kStepK * 2;   // one operand's share of a CTA and step
@@ -938,7 +944,9 @@ cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_
 // ------------------------------------------------------------------- splits
 // Products of few tiles leave most pairs idle while a few walk a long reduction:
 // their reduction is cut into `splits` runs of steps, each with an fp32 partial
-// result in the workspace, which a second kernel adds in order and rounds.
+// result in the workspace, which a second kernel adds in order and rounds (4
+// experts x 75 rows x 512 x 4096: 11.6 us instead of 19.5; weight gradient of 2 x
+// 4000 rows, 256 x 512: 14.6 instead of 24.9).
 constexpr int kPairsPlanned = 74;   // pairs of a B200; what the split is planned for
 constexpr int kMaxSplits = 16;
 
