@@ -52,19 +52,22 @@ __device__ __forceinline__ GroupScan scan_groups(const Groups& g, int base, int6
   const int64_t raw0 = raw_offset(g, min(e, g.experts)), raw1 = raw_offset(g, min(e + 1, g.experts));
   GroupScan s;
   s.bad = in && (raw0 < 0 || raw1 < raw0 || raw1 > g.rows);
-  int64_t end = max(raw1 < 0 ? 0 : raw1 > g.rows ? g.rows : raw1, carry);
-  int64_t first = raw0 < 0 ? 0 : raw0 > g.rows ? g.rows : raw0;
-  if (lane == 0) end = max(end, max(first, carry));
+  s.begin = raw0;
+  s.end = raw1;
+  if (__any_sync(0xffffffffu, s.bad || raw0 < carry)) {   // something to clamp, here or in the groups before
+    int64_t end = max(raw1 < 0 ? 0 : raw1 > g.rows ? g.rows : raw1, carry);
+    const int64_t first = max(raw0 < 0 ? 0 : raw0 > g.rows ? g.rows : raw0, carry);
+    if (lane == 0) end = max(end, first);
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {   // running maximum
-    const int64_t v = __shfl_up_sync(0xffffffffu, end, o);
-    if (lane >= o) end = max(end, v);
+    for (int o = 1; o < 32; o <<= 1) {   // running maximum
+      const int64_t v = __shfl_up_sync(0xffffffffu, end, o);
+      if (lane >= o) end = max(end, v);
+    }
+    const int64_t begin = __shfl_up_sync(0xffffffffu, end, 1);
+    s.begin = lane == 0 ? first : begin;
+    s.end = end;
   }
-  int64_t begin = __shfl_up_sync(0xffffffffu, end, 1);
-  if (lane == 0) begin = max(first, carry);
-  carry = __shfl_sync(0xffffffffu, end, 31);
-  s.begin = begin;
-  s.end = end;
+  carry = __shfl_sync(0xffffffffu, s.end, 31);
   return s;
 }
 
@@ -622,21 +625,25 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
   volatile int* abort = &c->abort;
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < kMaxStages; ++i) {
-      mbar_init(&c->full[i], 2);    // one arrival of each CTA
-      mbar_init(&c->empty[i], 1);   // the products' commit
-      mbar_init(&c->tail[i], 1);
+  if (warp == 0) {   // a barrier a lane
+    if (lane < kMaxStages) {
+      mbar_init(&c->full[lane], 2);    // one arrival of each CTA
+      mbar_init(&c->empty[lane], 1);   // the products' commit
+      mbar_init(&c->tail[lane], 1);
+    } else if (lane < kMaxStages + 2) {
+      mbar_init(&c->acc_full[lane - kMaxStages], 1);
+      mbar_init(&c->acc_empty[lane - kMaxStages], 2 * kWriters);
+    } else if (lane == kMaxStages + 2) {
+      mbar_init(&c->done, 1);
+      c->abort = 0;
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&c->acc_full[i], 1);
-      mbar_init(&c->acc_empty[i], 2 * kWriters);
-    }
-    mbar_init(&c->done, 1);
-    c->abort = 0;
     fence_mbar_init();
-  }
-  if (warp == 2) pair_tmem_alloc(&c->tmem, 512);
+  } else if (warp == 1) {
+    if (lane == 0) {
+      prefetch_tmap(&p.a);
+      prefetch_tmap(&p.b[0]);
+    }
+  } else if (warp == 2) pair_tmem_alloc(&c->tmem, 512);
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
