@@ -350,9 +350,9 @@ constexpr uint32_t kChunkBytes = kOperandBytes / 2;    // 64 rows of an MN-major
 constexpr int kPairThreads = 384;
 constexpr int kWriters = 8;
 constexpr uint32_t kAccCols = 256;
-constexpr uint32_t kStoreBytes = 2048;                 // a staging tile: 32 lines of 64 B, two for each writer
-constexpr uint32_t kRingBytes = 12 * kOperandBytes;    // 6 steps of A and B, or 4 of A and two Bs
-constexpr uint32_t kPairSmem = 1024 + kRingBytes + 2 * kWriters * kStoreBytes + 1024;
+constexpr uint32_t kStoreBytes = 2048;                 // a writer's staging tile: 32 lines of 64 B
+constexpr uint32_t kRingBytes = 200 * 1024;            // 6 steps of A and B, 4 of A and two Bs, 5 narrow ones
+constexpr uint32_t kPairSmem = 1024 + kRingBytes + kWriters * kStoreBytes + 1024;
 constexpr int kBoxes = 4;                              // row boxes of 16, 32, 64, 128
 
 enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2 };
@@ -360,10 +360,10 @@ enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2 };
 // Shapes of a tile's N side and of the ring that fits it.
 //   kOne     up to 256 columns: 6 steps of 32 KB
 //   kTwo     up to 512 in two accumulators: 4 steps of 48 KB
-//   kNarrow  up to 64: 4 steps of 40 KB, 128 wide: with a handful of rows the matrix streams, and the ring holds
+//   kNarrow  up to 64: 5 steps of 40 KB, 128 wide: with a handful of rows the matrix streams, and the ring holds
 //            as much of it as it can.  Waiting for a step, issuing its products and committing them
 //            takes the issuing warp some 450 cycles, more than narrow products run: twice the step
-//            (one token on 96 experts, 1536 x 2048: 64 wide 14.5 us, 128 wide 13.2).
+//            (one token on 96 experts, 1536 x 2048: 64 wide 14.5 us, 128 wide 13.1, 12.6 with the fifth step).
 //   kMiddle  up to 128: 4 steps of 48 KB, 128 wide
 enum PairShape { kOne = 0, kTwo = 1, kNarrow = 2, kMiddle = 3 };
 constexpr int subs_of(int shape) { return shape >= kNarrow ? 2 : 1; }   // 64-wide blocks of a step
@@ -472,17 +472,15 @@ struct Walker {
 template <int MODE>
 struct Writer {
   const PairParams& p;
-  uint8_t* stages;   // two staging tiles of 32 lines of 64 B (the 16-byte pieces of a line permuted as SWIZZLE_64B)
+  uint8_t* stage;    // 32 lines of 64 B (the 16-byte pieces of a line permuted as SWIZZLE_64B)
   int lane;
   int32_t e = 0, m = 0, cols = 0;   // which result (expert, run of the reduction); first M row; columns there are
   int64_t n0 = 0;                   // column 0 in the output: row products: its row; weight gradient: its column
-  uint32_t flip = 0;
 
-  __device__ __forceinline__ uint8_t* next_stage() {
-    flip ^= 1;
-    if (elect_one()) bulk_wait_read_1();
+  // The staging tile is free once the store before has read it.
+  __device__ __forceinline__ void stage_free() const {
+    if (elect_one()) bulk_wait_read();
     __syncwarp();
-    return stages + flip * kStoreBytes;
   }
   // Row products that leave by TMA take fragments, everything else a row of 32 columns a lane.
   __device__ __forceinline__ void load(uint32_t acc, uint32_t (&r)[32]) const {
@@ -504,8 +502,8 @@ struct Writer {
   // rows leaves by TMA.
   __device__ __forceinline__ void write_rows(int32_t col, uint32_t (&r)[32]) {
     const int32_t rows = min(32, cols - col);
-    uint8_t* stage = next_stage();
     pack_pairs(r, p.bf16);   // words 0..7: lanes 0..15, 8..15: lanes 16..31
+    stage_free();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int line = 8 * i + lane % 8;
@@ -529,7 +527,6 @@ struct Writer {
         if (line < rows) store_8(dst + line * p.ld + q * 8, v, p.m_len - m - q * 8);
       }
       __syncwarp();
-      if (elect_one()) bulk_commit();   // an empty group, for the count of next_stage()
     }
   }
 
@@ -561,7 +558,7 @@ struct Writer {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {   // 16 words a line: 32 columns of 16 bits, or 16 of f32 twice
         if (h == 1 && !p.f32) break;
-        uint8_t* stage = next_stage();
+        stage_free();
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
@@ -612,7 +609,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     grouped_pair_kernel(const __grid_constant__ PairParams p) {
   constexpr bool WIDE = SHAPE == kTwo;
   constexpr int kSubs = subs_of(SHAPE);
-  constexpr uint32_t kStages = SHAPE == kOne ? 6 : 4;
+  constexpr uint32_t kStages = SHAPE == kOne ? 6 : SHAPE == kNarrow ? 5 : 4;
   constexpr uint32_t kBBytes = SHAPE == kNarrow ? kOperandBytes / 4 : SHAPE == kMiddle ? kOperandBytes / 2 : kOperandBytes;   // B of a 64-wide block
   constexpr uint32_t kStageBytes = kSubs * (kOperandBytes + (WIDE ? 2 : 1) * kBBytes);
   static_assert(kStages <= kMaxStages && kStages * kStageBytes <= kRingBytes);
@@ -620,7 +617,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   uint8_t* base = raw + (1024 - smem_u32(raw) % 1024) % 1024;
   uint8_t* ring = base;
   uint8_t* staging = ring + kRingBytes;
-  PairCtrl* c = reinterpret_cast<PairCtrl*>(staging + 2 * kWriters * kStoreBytes);
+  PairCtrl* c = reinterpret_cast<PairCtrl*>(staging + kWriters * kStoreBytes);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
@@ -801,7 +798,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   } else if (warp >= 4) {
     // -------------------------------------------------------------- results
     const int quad = warp % 4, part = (warp - 4) / 4;   // 32 of the CTA's M rows, every other 32 columns
-    Writer<MODE> out{p, staging + (warp - 4) * 2 * kStoreBytes, lane};
+    Writer<MODE> out{p, staging + (warp - 4) * kStoreBytes, lane};
     uint32_t n = 0;
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
