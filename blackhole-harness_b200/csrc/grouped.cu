@@ -949,16 +949,26 @@ cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_
 // Products of few tiles leave most pairs idle while a few walk a long reduction:
 // their reduction is cut into `splits` runs of steps, each with an fp32 partial
 // result in the workspace, which a second kernel adds in order and rounds (4
-// experts x 75 rows x 512 x 4096: 11.6 us instead of 19.5; weight gradient of 2 x
-// 4000 rows, 256 x 512: 14.6 instead of 24.9).
+// experts x 75 rows x 512 x 4096: 11.3 us instead of 14.1; weight gradient of 2 x
+// 4000 rows, 256 x 512: 12.5 instead of 23.8).
 constexpr int kPairsPlanned = 74;   // pairs of a B200; what the split is planned for
 constexpr int kMaxSplits = 16;
 
-// Runs for `tiles` tiles of `steps` steps.  A step takes about 0.2 us and the second
-// kernel about 3: cutting pays from some 16 steps saved on.
-int plan_splits(int64_t tiles, int64_t steps) {
-  const int64_t s = std::min<int64_t>({kPairsPlanned / std::max<int64_t>(tiles, 1), steps / 4, kMaxSplits});
-  return s >= 2 && steps - steps / s >= 16 ? static_cast<int>(s) : 1;
+// Runs for `tiles` tiles of `steps` steps and `values` results, by what they take: about 0.2 us a step, 2.5 for
+// the second kernel, and the fp32 partials written and read at some 6 MB a us (of its own measure, 500 rows x
+// 2048 x 2048: 1 run 14.4 us, 4 runs 15.6; 200 rows x 1024 x 1536 of 4 experts: 7.9 and 9.0).
+int plan_splits(int64_t tiles, int64_t steps, int64_t values) {
+  const int64_t most = std::min<int64_t>({kPairsPlanned / std::max<int64_t>(tiles, 1), steps / 4, kMaxSplits});
+  int best = 1;
+  double least = 0.2 * static_cast<double>(steps);
+  for (int s = 2; s <= most; ++s) {
+    const double t = 0.2 * static_cast<double>((steps + s - 1) / s) + 2.5 + 8e-6 / 6 * static_cast<double>(s * values);
+    if (t < least) {
+      least = t;
+      best = s;
+    }
+  }
+  return best;
 }
 int64_t pitch4(int64_t n) { return (n + 3) / 4 * 4; }   // f32 rows of whole 16-byte pieces
 
@@ -977,10 +987,11 @@ int64_t row_tiles(int64_t rows, int32_t experts, int32_t m_len) {   // at most
   return (rows / span_of(rows_shape(rows, experts, m_len)) + std::min<int64_t>(experts, rows)) * ((m_len + 255) / 256);
 }
 int rows_splits(int64_t rows, int32_t experts, int32_t m_len, int32_t red) {
-  return plan_splits(row_tiles(rows, experts, m_len), (red + kStepK - 1) / kStepK);
+  return plan_splits(row_tiles(rows, experts, m_len), (red + kStepK - 1) / kStepK, rows * m_len);
 }
 int wgrad_splits(int64_t rows, int32_t experts, int32_t n, int32_t k) {
-  return plan_splits(static_cast<int64_t>(experts) * ((n + 255) / 256) * ((k + 255) / 256), rows / experts / kStepK);
+  return plan_splits(static_cast<int64_t>(experts) * ((n + 255) / 256) * ((k + 255) / 256), rows / experts / kStepK,
+                     static_cast<int64_t>(experts) * n * k);
 }
 
 struct JoinParams {
