@@ -954,15 +954,17 @@ cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_
 constexpr int kPairsPlanned = 74;   // pairs of a B200; what the split is planned for
 constexpr int kMaxSplits = 16;
 
-// Runs for `tiles` tiles of `steps` steps and `values` results, by what they take: about 0.2 us a step, 2.5 for
-// the second kernel, and the fp32 partials written and read at some 6 MB a us (of its own measure, 500 rows x
-// 2048 x 2048: 1 run 14.4 us, 4 runs 15.6; 200 rows x 1024 x 1536 of 4 experts: 7.9 and 9.0).
-int plan_splits(int64_t tiles, int64_t steps, int64_t values) {
+// Runs for `tiles` tiles of `steps` steps and `values` results, by what they take: step_us a step (0.28 with 256
+// columns, 0.17 with up to 128), about 2.5 us for the second kernel, and the fp32 partials written and read at
+// some 6 MB a us (500 rows x 2048 x 2048: 1 run 14.4 us, 4 runs 15.6; 200 rows x 1024 x 1536 of 4 experts: 7.9
+// and 9.0; weight gradient of 5 x 1185 rows, 112 x 1208: 2 runs 17.3, 1 run 20.3).
+int plan_splits(int64_t tiles, int64_t steps, double step_us, int64_t values) {
   const int64_t most = std::min<int64_t>({kPairsPlanned / std::max<int64_t>(tiles, 1), steps / 4, kMaxSplits});
   int best = 1;
-  double least = 0.2 * static_cast<double>(steps);
+  double least = step_us * static_cast<double>(steps);
   for (int s = 2; s <= most; ++s) {
-    const double t = 0.2 * static_cast<double>((steps + s - 1) / s) + 2.5 + 8e-6 / 6 * static_cast<double>(s * values);
+    const double t = step_us * static_cast<double>((steps + s - 1) / s) + 2.5 +
+                     8e-6 / 6 * static_cast<double>(s * values);
     if (t < least) {
       least = t;
       best = s;
@@ -987,11 +989,12 @@ int64_t row_tiles(int64_t rows, int32_t experts, int32_t m_len) {   // at most
   return (rows / span_of(rows_shape(rows, experts, m_len)) + std::min<int64_t>(experts, rows)) * ((m_len + 255) / 256);
 }
 int rows_splits(int64_t rows, int32_t experts, int32_t m_len, int32_t red) {
-  return plan_splits(row_tiles(rows, experts, m_len), (red + kStepK - 1) / kStepK, rows * m_len);
+  return plan_splits(row_tiles(rows, experts, m_len), (red + kStepK - 1) / kStepK,
+                     span_of(rows_shape(rows, experts, m_len)) >= 256 ? 0.28 : 0.17, rows * m_len);
 }
 int wgrad_splits(int64_t rows, int32_t experts, int32_t n, int32_t k) {
   return plan_splits(static_cast<int64_t>(experts) * ((n + 255) / 256) * ((k + 255) / 256), rows / experts / kStepK,
-                     static_cast<int64_t>(experts) * n * k);
+                     0.28, static_cast<int64_t>(experts) * n * k);
 }
 
 struct JoinParams {
