@@ -955,7 +955,7 @@ constexpr int kPairsPlanned = 74;   // pairs of a B200; what the split is planne
 constexpr int kMaxSplits = 16;
 
 // Runs for `tiles` tiles of `steps` steps and `values` results, by what they take: step_us a step (0.28 with 256
-// columns, 0.17 with up to 128), about 2.5 us for the second kernel, and the fp32 partials written and read at
+// columns, 0.14 with up to 128), about 2.5 us for the second kernel, and the fp32 partials written and read at
 // some 6 MB a us (500 rows x 2048 x 2048: 1 run 14.4 us, 4 runs 15.6; 200 rows x 1024 x 1536 of 4 experts: 7.9
 // and 9.0; weight gradient of 5 x 1185 rows, 112 x 1208: 2 runs 17.3, 1 run 20.3).
 int plan_splits(int64_t tiles, int64_t steps, double step_us, int64_t values) {
@@ -974,23 +974,27 @@ int plan_splits(int64_t tiles, int64_t steps, double step_us, int64_t values) {
 }
 int64_t pitch4(int64_t n) { return (n + 3) / 4 * 4; }   // f32 rows of whole 16-byte pieces
 
+// Most tiles that rows in groups can make with a shape.
+int64_t row_tiles(int64_t rows, int32_t experts, int32_t m_len, PairShape shape) {
+  return (rows / span_of(shape) + std::min<int64_t>(experts, rows)) * ((m_len + 255) / 256);
+}
 // The shape for groups of this mean size.  Steps 128 wide pay up to tiles of 128 columns (32 experts x 30
-// rows x 512 x 2048: 11.9 us against 14.3).  Two accumulators a tile where groups of 257..512 rows are the
-// rule (the matrix is then loaded once a group, not twice: 96 x 341 rows, 1536 x 2048: 182 us against
-// 194) and still fill the machine; with larger groups the drain between tiles costs more than it saves
-// (8192^2 x 2048: 180 us against 174).
+// rows x 512 x 2048: 11.9 us against 14.3), and narrower tiles wherever every one of them still has a pair of
+// its own (1511 rows, 192 x 1472: 7.6 us narrow, 8.0 middle, 11.4 one; 3296 rows of 2 experts, 512 x 872, 106 tiles
+// narrow: 9.3, 7.8, 9.6; 484 rows of 3, 3872 x 3768, 96 tiles middle: 37.0 middle, 26.9 one).  Two accumulators a
+// tile where groups of 257..512 rows are the rule (the matrix is then loaded once a group, not twice: 96 x 341
+// rows, 1536 x 2048: 182 us against 194) and still fill the machine; with larger groups the drain between tiles
+// costs more than it saves (8192^2 x 2048: 180 us against 174).
 PairShape rows_shape(int64_t rows, int32_t experts, int32_t m_len) {
-  if (rows <= 64 || rows <= 32ll * experts) return kNarrow;
-  if (rows <= 128 || rows <= 96ll * experts) return kMiddle;
+  if (rows <= 64 || rows <= 32ll * experts || row_tiles(rows, experts, m_len, kNarrow) <= kPairsPlanned) return kNarrow;
+  if (rows <= 128 || rows <= 96ll * experts || row_tiles(rows, experts, m_len, kMiddle) <= kPairsPlanned) return kMiddle;
   const bool fills = static_cast<int64_t>(experts) * ((m_len + 255) / 256) >= 2 * kPairsPlanned;
   return rows > 256ll * experts && rows <= 512ll * experts && fills ? kTwo : kOne;
 }
-int64_t row_tiles(int64_t rows, int32_t experts, int32_t m_len) {   // at most
-  return (rows / span_of(rows_shape(rows, experts, m_len)) + std::min<int64_t>(experts, rows)) * ((m_len + 255) / 256);
-}
 int rows_splits(int64_t rows, int32_t experts, int32_t m_len, int32_t red) {
-  return plan_splits(row_tiles(rows, experts, m_len), (red + kStepK - 1) / kStepK,
-                     span_of(rows_shape(rows, experts, m_len)) >= 256 ? 0.28 : 0.17, rows * m_len);
+  const PairShape shape = rows_shape(rows, experts, m_len);
+  return plan_splits(row_tiles(rows, experts, m_len, shape), (red + kStepK - 1) / kStepK,
+                     span_of(shape) >= 256 ? 0.28 : 0.14, rows * m_len);
 }
 int wgrad_splits(int64_t rows, int32_t experts, int32_t n, int32_t k) {
   return plan_splits(static_cast<int64_t>(experts) * ((n + 255) / 256) * ((k + 255) / 256), rows / experts / kStepK,
@@ -1143,7 +1147,8 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
     q.stride_split = rows * pitch;
     q.f32 = split || f32; q.bf16 = bf16;
     q.dev_err = dev_err;
-    const int64_t tiles = row_tiles(rows, experts, width_out) * q.splits;
+    const PairShape shape = rows_shape(rows, experts, width_out);
+    const int64_t tiles = row_tiles(rows, experts, width_out, shape) * q.splits;
     if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (int rc = make_map(&q.a, w, dt, 3, k, n, experts, 2 * ld_w, experts == 1 ? 2 * ld_w : 2 * stride_w, 64,
@@ -1157,7 +1162,6 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
     if (q.tma_out && rows >= 32)   // no full tile of 32 rows otherwise
       if (int rc = make_map(&q.out, out, dt, 2, width_out, rows, 1, 2 * ld_out, 0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
-    const PairShape shape = rows_shape(rows, experts, width_out);
     auto launch = [&](auto mode) {
       constexpr int MODE = decltype(mode)::value;
       return shape == kNarrow   ? launch_pair<MODE, kNarrow>(q, tiles, sms, st)
