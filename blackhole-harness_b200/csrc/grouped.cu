@@ -434,14 +434,15 @@ struct Walker {
     const int64_t b = __shfl_sync(0xffffffffu, begin, src), e = __shfl_sync(0xffffffffu, end, src);
     const int32_t local = tile - __shfl_sync(0xffffffffu, upto - mine, src);
     t.e = base + src;
+    constexpr int32_t kWidth = kStepK * subs_of(SHAPE);
     if constexpr (MODE == kWgrad) {
       t.m0 = local / p.n_tiles * 256;
       t.n0 = local % p.n_tiles * p.tile_n;
       t.width = t.valid = p.tile_n;
       t.parts = 1;
       t.row0 = b;
-      t.steps = static_cast<int32_t>((e - b + kStepK - 1) / kStepK);
-      t.tail = static_cast<int32_t>((e - b) % kStepK);
+      t.steps = static_cast<int32_t>((e - b + kWidth - 1) / kWidth);
+      t.tail = static_cast<int32_t>((e - b) % kWidth);
     } else {
       const int32_t size = static_cast<int32_t>(e - b), tiles = (size + kSpan - 1) / kSpan;
       const int32_t span = (size + tiles - 1) / tiles;
@@ -452,7 +453,6 @@ struct Walker {
       t.row0 = b + t.n0;
       t.valid = min(parts * t.width, size - t.n0);
       t.parts = t.valid > t.width ? 2 : 1;   // the last tile of a group may end within its first accumulator
-      constexpr int32_t kWidth = kStepK * subs_of(SHAPE);
       t.steps = (p.red + kWidth - 1) / kWidth;
       t.tail = p.red % kWidth;
     }
@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       const int32_t halves[2] = {t.columns(0) / 2, WIDE && t.parts > 1 ? t.columns(1) / 2 : 0};
       const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128;
       const uint32_t bytes =
-          kOperandBytes + (MODE == kWgrad ? kOperandBytes : static_cast<uint32_t>(halves[0] + halves[1]) * kStepK * 2);
+          kOperandBytes + (MODE == kWgrad ? kBBytes : static_cast<uint32_t>(halves[0] + halves[1]) * kStepK * 2);
       for (int32_t s = 0; s < t.steps; ++s, ++it) {
         if (!mbar_wait(&c->empty[st], phase, abort, p.dev_err)) { ok = false; break; }
         uint8_t* a = ring + st * kStageBytes;
@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             if constexpr (MODE == kWgrad) {
               const int32_t y = static_cast<int32_t>(t.row0) + r, x = t.n0 + static_cast<int32_t>(rank) * halves[0];
               pair_load_2d(b, &p.b[0], bar, x, y);
-              pair_load_2d(b + kChunkBytes, &p.b[0], bar, x + 64, y);
+              if constexpr (kBBytes > kChunkBytes) pair_load_2d(b + kChunkBytes, &p.b[0], bar, x + 64, y);
             } else {
 #pragma unroll
               for (int part = 0; part < (WIDE ? 2 : 1); ++part) {
@@ -787,10 +787,15 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       ok = mbar_wait(&c->tail[st], __shfl_sync(0xffffffffu, uses, st) & 1, abort, p.dev_err);
       ok = __all_sync(0xffffffffu, ok);
       if (lane == static_cast<int>(st)) ++uses;
-      uint4* a = reinterpret_cast<uint4*>(ring + st * kStageBytes);
-      const int zeros = (16 - t.tail % 16) * 8;   // 16-byte pieces in the lines to clear, per 64-row chunk
-      for (int i = lane; ok && i < 4 * zeros; i += 32)
-        a[i / zeros * (kChunkBytes / 16) + t.tail * 8 + i % zeros] = make_uint4(0, 0, 0, 0);
+      const uint32_t sub = t.tail / kStepK;
+      uint8_t* a = ring + st * kStageBytes + sub * kOperandBytes;
+      uint8_t* b = ring + st * kStageBytes + kSubs * kOperandBytes + sub * kBBytes;
+      const int zeros = (16 - t.tail % 16) * 8;   // 16-byte pieces in the lines to clear, per 64-column chunk
+      for (int i = lane; ok && i < static_cast<int>(2 + kBBytes / kChunkBytes) * zeros; i += 32) {
+        const uint32_t chunk = i / zeros;
+        uint8_t* at = chunk < 2 ? a + chunk * kChunkBytes : b + (chunk - 2) * kChunkBytes;
+        reinterpret_cast<uint4*>(at)[t.tail % kStepK * 8 + i % zeros] = make_uint4(0, 0, 0, 0);
+      }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) pair_arrive_zeroed(peer_addr(&c->full[st], 0));
@@ -918,7 +923,8 @@ int sm_count(int* sms) {
                           reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kOne>),
                           reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kTwo>),
                           reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kNarrow>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, kOne>)}) {
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, kOne>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, kMiddle>)}) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
       if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
     }
@@ -955,20 +961,20 @@ constexpr int kPairsPlanned = 74;   // pairs of a B200; what the split is planne
 constexpr int kMaxSplits = 16;
 
 // Runs for `tiles` tiles of `steps` steps and `values` results, by what they take: step_us a step (0.28 with 256
-// columns, 0.14 with up to 128), about 2.5 us for the second kernel, and the fp32 partials written and read at
+// columns, 0.14 with up to 128, 0.15 to 0.3 for a weight gradient's, by how its rows lie in memory), about 2.5 us for the second kernel, and the fp32 partials written and read at
 // some 6 MB a us (500 rows x 2048 x 2048: 1 run 14.4 us, 4 runs 15.6; 200 rows x 1024 x 1536 of 4 experts: 7.9
 // and 9.0; weight gradient of 5 x 1185 rows, 112 x 1208: 2 runs 17.3, 1 run 20.3).
-int plan_splits(int64_t tiles, int64_t steps, double step_us, int64_t values) {
+struct SplitPlan {
+  int splits;
+  double us;
+};
+SplitPlan plan_splits(int64_t tiles, int64_t steps, double step_us, int64_t values) {
   const int64_t most = std::min<int64_t>({kPairsPlanned / std::max<int64_t>(tiles, 1), steps / 4, kMaxSplits});
-  int best = 1;
-  double least = step_us * static_cast<double>(steps);
+  SplitPlan best = {1, step_us * static_cast<double>(steps)};
   for (int s = 2; s <= most; ++s) {
-    const double t = step_us * static_cast<double>((steps + s - 1) / s) + 2.5 +
-                     8e-6 / 6 * static_cast<double>(s * values);
-    if (t < least) {
-      least = t;
-      best = s;
-    }
+    const double us = step_us * static_cast<double>((steps + s - 1) / s) + 2.5 +
+                      8e-6 / 6 * static_cast<double>(s * values);
+    if (us < best.us) best = {s, us};
   }
   return best;
 }
@@ -994,11 +1000,28 @@ PairShape rows_shape(int64_t rows, int32_t experts, int32_t m_len) {
 int rows_splits(int64_t rows, int32_t experts, int32_t m_len, int32_t red) {
   const PairShape shape = rows_shape(rows, experts, m_len);
   return plan_splits(row_tiles(rows, experts, m_len, shape), (red + kStepK - 1) / kStepK,
-                     span_of(shape) >= 256 ? 0.28 : 0.14, rows * m_len);
+                     span_of(shape) >= 256 ? 0.28 : 0.14, rows * m_len)
+      .splits;
+}
+int64_t wgrad_tiles(int32_t experts, int32_t n, int32_t k, PairShape shape) {
+  return static_cast<int64_t>(experts) * ((n + 255) / 256) * ((k + span_of(shape) - 1) / span_of(shape));
+}
+SplitPlan wgrad_plan(int64_t rows, int32_t experts, int32_t n, int32_t k, PairShape shape) {
+  return plan_splits(wgrad_tiles(experts, n, k, shape), rows / experts / kStepK, shape == kOne ? 0.28 : 0.2,
+                     static_cast<int64_t>(experts) * n * k);
+}
+// Tiles of 128 columns and steps of 128 rows where each tile still has a pair of its own, or where there are no more
+// columns (2790 rows of 9 groups, 256 x 128: 6.2 us against 6.6; 8192 rows, 512 x 512: 23.8 against 42.1; 15244 rows
+// of 77, 120 x 112: 12.8 against 15.1).  With more tiles than pairs they lose (1125 rows of 4, 432 x 3712: 10.9 us
+// against 9.4), and where twice as wide ones may share a reduction that these may not (20787 rows of 3,
+// 120 x 2232: 43.2 against 34.2).
+PairShape wgrad_shape(int64_t rows, int32_t experts, int32_t n, int32_t k) {
+  if (k <= span_of(kMiddle)) return kMiddle;
+  if (wgrad_tiles(experts, n, k, kMiddle) > kPairsPlanned) return kOne;
+  return wgrad_plan(rows, experts, n, k, kMiddle).us <= wgrad_plan(rows, experts, n, k, kOne).us ? kMiddle : kOne;
 }
 int wgrad_splits(int64_t rows, int32_t experts, int32_t n, int32_t k) {
-  return plan_splits(static_cast<int64_t>(experts) * ((n + 255) / 256) * ((k + 255) / 256), rows / experts / kStepK,
-                     0.28, static_cast<int64_t>(experts) * n * k);
+  return wgrad_plan(rows, experts, n, k, wgrad_shape(rows, experts, n, k)).splits;
 }
 
 struct JoinParams {
@@ -1222,7 +1245,8 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
     q.g = groups;
     q.m_len = n; q.n_len = k;
     q.m_tiles = (n + 255) / 256;
-    q.n_tiles = (k + 255) / 256;
+    const PairShape shape = wgrad_shape(rows, experts, n, k);
+    q.n_tiles = (k + span_of(shape) - 1) / span_of(shape);
     q.tile_n = ((k + q.n_tiles - 1) / q.n_tiles + 63) / 64 * 64;
     q.splits = wgrad_splits(rows, experts, n, k);
     const int64_t pitch = pitch4(k), lines = static_cast<int64_t>(experts) * n;
@@ -1233,7 +1257,7 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
     q.stride_e = split ? n * pitch : stride_out;
     q.f32 = split || f32; q.bf16 = bf16; q.accumulate = accumulate && !split;
     q.dev_err = dev_err;
-    const int64_t tiles = static_cast<int64_t>(experts) * q.m_tiles * q.n_tiles * q.splits;
+    const int64_t tiles = wgrad_tiles(experts, n, k, shape) * q.splits;
     if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
     if (int rc = make_map(&q.a, dy, dt, 2, n, rows, 1, 2 * ld_dy, 0, 64, 64)) return rc;
@@ -1245,7 +1269,8 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
       if (int rc = make_map(&q.out, q.dst, q.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dt, 3, k, n, results, z * q.ld,
                             results == 1 ? z * q.ld : z * q.stride_e, q.f32 ? 16 : 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
-    cudaError_t e = launch_pair<kWgrad, kOne>(q, tiles, sms, st);
+    cudaError_t e = shape == kOne ? launch_pair<kWgrad, kOne>(q, tiles, sms, st)
+                                  : launch_pair<kWgrad, kMiddle>(q, tiles, sms, st);
     if (e == cudaSuccess && split) {
       JoinParams j{};
       j.part = static_cast<const float*>(workspace);
