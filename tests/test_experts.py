@@ -197,6 +197,44 @@ def test_grouped_wgrad_rows_outside_and_parts(widths):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("width", [1000, 2600])
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("sizes", ["tile edges", "pair edges", "large"], ids=str)
+def test_grouped_mm_of_many_tiles(sizes, transpose, width):
+    """More tiles than pairs of SMs at one width of tile or another; what surrounds the groups is not a number."""
+    sizes, red, first = SIZES[sizes], 136, 3
+    n, k = (red, width) if transpose else (width, red)
+    rows = first + sum(sizes) + 2
+    x, w = normal((rows, red), BF16, 61), normal((len(sizes), n, k), BF16, 62, 0.1)
+    x[:first], x[-2:] = float("nan"), float("inf")
+    off = offsets_of(sizes, first)
+    want, mass = mm_reference(x, w, off, transpose, rows)
+    got = experts.grouped_mm(x.to(DEV), w.to(DEV), off.to(DEV), transpose=transpose)
+    assert not got[:first].any() and not got[-2:].any()
+    assert_sum(got, want, mass, red, BF16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [F16, F32], ids=str)
+@pytest.mark.parametrize("sizes", ["tile edges", "pair edges", "empty ends"], ids=str)
+def test_grouped_wgrad_of_many_tiles(sizes, out_dtype):
+    """More tiles than pairs of SMs; each group's neighbours are not numbers when its turn comes."""
+    sizes, n, k, first = SIZES[sizes], 520, 584, 5
+    rows = first + sum(sizes) + 70
+    dy, x = torch.full((rows, n), float("inf"), dtype=F16), torch.full((rows, k), float("nan"), dtype=F16)
+    dy[first:first + sum(sizes)], x[first:first + sum(sizes)] = normal((sum(sizes), n), F16, 63), normal((sum(sizes), k), F16, 64)
+    off = offsets_of(sizes, first)
+    want, mass = wgrad_reference(dy, x, off)
+    got = experts.grouped_wgrad(dy.to(DEV), x.to(DEV), off.to(DEV), out_dtype=out_dtype)
+    assert_sum(got, want, mass, max(sizes), out_dtype)
+    bad = max(range(len(sizes)), key=lambda e: sizes[e])
+    x[off[bad]:off[bad + 1]] = float("nan")
+    got2 = experts.grouped_wgrad(dy.to(DEV), x.to(DEV), off.to(DEV), out_dtype=out_dtype)
+    rest = [e for e in range(len(sizes)) if e != bad]
+    assert got2[bad].isnan().all() and torch.equal(got2[rest], got[rest])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("out_dtype", [BF16, F32], ids=str)
 @pytest.mark.parametrize("transpose", [False, True])
 @pytest.mark.parametrize("n,k", [(200, 2056), (2056, 200), (1000, 1048)])
