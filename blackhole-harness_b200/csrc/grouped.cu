@@ -1181,7 +1181,8 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
     const int64_t half = (std::min<int64_t>(rows, 256) + 31) / 32 * 16;
     for (int i = 0; i < kBoxes && 16 << i <= half; ++i)
       if (int rc = make_map(&q.b[i], x, dt, 2, width_in, rows, 1, 2 * ld_x, 0, 64, 16u << i)) return rc;
-    q.tma_out = !q.f32 && tma_rows(out, ld_out, 2);
+    // a TMA store ends at a multiple of 16 bytes: it would write over what stands behind a row that does not
+    q.tma_out = !q.f32 && tma_rows(out, ld_out, 2) && width_out % 8 == 0;
     if (q.tma_out && rows >= 32)   // no full tile of 32 rows otherwise
       if (int rc = make_map(&q.out, out, dt, 2, width_out, rows, 1, 2 * ld_out, 0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
@@ -1264,7 +1265,9 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
     if (int rc = make_map(&q.b[0], x, dt, 2, k, rows, 1, 2 * ld_x, 0, 64, 64)) return rc;
     // a 16-bit sum is rounded once: that of an addition to out cannot be left to TMA, which rounds before and after
     const int64_t z = q.f32 ? 4 : 2, results = static_cast<int64_t>(experts) * q.splits;
-    q.tma_out = tma_stack(q.dst, q.ld, q.stride_e, z, static_cast<int32_t>(results)) && (q.f32 || !q.accumulate);
+    // (and a store ends at a multiple of 16 bytes, with zeros in what a row lacks: the partials have room for that)
+    q.tma_out = tma_stack(q.dst, q.ld, q.stride_e, z, static_cast<int32_t>(results)) && (split || k * z % 16 == 0) &&
+                (q.f32 || !q.accumulate);
     if (q.tma_out)
       if (int rc = make_map(&q.out, q.dst, q.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dt, 3, k, n, results, z * q.ld,
                             results == 1 ? z * q.ld : z * q.stride_e, q.f32 ? 16 : 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))

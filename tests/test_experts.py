@@ -234,6 +234,51 @@ def test_grouped_wgrad_of_many_tiles(sizes, out_dtype):
     assert got2[bad].isnan().all() and torch.equal(got2[rest], got[rest])
 
 
+def padded(t, fill):
+    """t as a view into rows that are some elements longer (a multiple of 16 bytes), which hold `fill`."""
+    width = t.shape[-1] // 8 * 8 + 8
+    buf = torch.full((*t.shape[:-1], width), fill, dtype=t.dtype, device=DEV)
+    view = buf[..., :t.shape[-1]]
+    view.copy_(t)
+    return buf, view
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("E,rows,n,k", [(3, 70, 301, 67), (2, 900, 45, 133), (9, 2000, 1501, 99), (20, 6000, 2100, 77)])
+def test_grouped_mm_of_odd_widths_in_padded_rows(E, rows, n, k, transpose):
+    """Rows of an odd width, 16-byte strides and not-a-number between them: neither read nor written over."""
+    r = np.random.RandomState(E)
+    sizes = np.bincount(r.randint(0, E, rows), minlength=E)
+    if transpose:
+        n, k = k, n
+    x, w = normal((rows, n if transpose else k), BF16, 67), normal((E, n, k), BF16, 68, 0.1)
+    off = offsets_of(sizes)
+    want, mass = mm_reference(x, w, off, transpose, rows)
+    buf, out = padded(torch.zeros(rows, k if transpose else n, dtype=BF16), 5.0)
+    experts.grouped_mm(padded(x, float("nan"))[1], padded(w, float("nan"))[1], off.to(DEV), transpose=transpose, out=out)
+    assert_sum(out, want, mass, n if transpose else k, BF16)
+    assert (buf[:, out.shape[1]:] == 5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("E,rows,n,k", [(2, 70, 129, 67), (12, 700, 301, 355), (40, 1500, 77, 499), (1, 5000, 97, 131)])
+def test_grouped_wgrad_of_odd_widths_in_padded_rows(E, rows, n, k, out_dtype):
+    """The same of gradients: what stands between the rows of a view is nobody's."""
+    r = np.random.RandomState(E)
+    sizes = np.bincount(r.randint(0, E, rows), minlength=E)
+    dy, x, off = normal((rows, n), BF16, 69), normal((rows, k), BF16, 70), offsets_of(sizes)
+    want, mass = wgrad_reference(dy, x, off)
+    buf, out = padded(torch.zeros(E, n, k, dtype=out_dtype), 5.0)
+    ins = padded(dy, float("nan"))[1], padded(x, float("nan"))[1]
+    experts.grouped_wgrad(*ins, off.to(DEV), out=out)
+    assert_sum(out, want, mass, max(sizes), out_dtype)
+    assert (buf[..., k:] == 5).all()
+    experts.grouped_wgrad(*ins, off.to(DEV), out=out, accumulate=True)
+    assert (buf[..., k:] == 5).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("out_dtype", [BF16, F32], ids=str)
 @pytest.mark.parametrize("transpose", [False, True])
