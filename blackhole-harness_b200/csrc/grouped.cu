@@ -328,9 +328,10 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 //         group's rows.  N is a multiple of 32 chosen per tile, so a group of 341
 //         rows takes two tiles of 192, not two of 256, and a group of 5 rows one
 //         of 32: the weights stream once at full width whatever the group's size.
-//   weight gradient              M side: n, N side: k, reduction over the group's
-//         rows.  The last step of a group zeroes the rows that follow it, in both
-//         operands (they are another group's, and may hold anything).
+//   weight gradient              M side: n, N side: k (or the other way about, kWgradT,
+//         where n would fill its 256s badly), reduction over the group's rows.  The last
+//         step of a group zeroes the rows that follow it, in both operands (they are
+//         another group's, and may hold anything).
 // Operand majors: x and dy rows are reduction-major (K) in the row products, as
 // is W for y; W for dx, and both operands of the weight gradient, are stored with
 // the reduction outermost and go to the tensor core as MN-major tiles.
@@ -355,7 +356,7 @@ constexpr uint32_t kRingBytes = 200 * 1024;            // 6 steps of A and B, 4 
 constexpr uint32_t kPairSmem = 1024 + kRingBytes + kWriters * kStoreBytes + 1024;
 constexpr int kBoxes = 4;                              // row boxes of 16, 32, 64, 128
 
-enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2 };
+enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2, kWgradT = 3 };   // kWgradT: M side k, N side n
 
 // Shapes of a tile's N side and of the ring that fits it.
 //   kOne     up to 256 columns: 6 steps of 32 KB
@@ -372,12 +373,12 @@ constexpr int span_of(int shape) {                                      // most 
 }
 
 struct PairParams {
-  CUtensorMap a;             // W (3-D: reduction or features, ..., expert) or dy
-  CUtensorMap b[kBoxes];     // the rows, by box height; weight gradient: [0] is x
-  CUtensorMap out;           // boxes of 32 rows x 64 B
+  CUtensorMap a;             // W (3-D: reduction or features, ..., expert); weight gradient: dy, or x in kWgradT
+  CUtensorMap b[kBoxes];     // the rows, by box height; weight gradient: [0] is the other of x and dy
+  CUtensorMap out;           // boxes of 32 rows x 64 B; f32 of kWgradT: 16 rows x 128 B
   Groups g;
-  int32_t m_len;             // M side: output features / n
-  int32_t n_len;             // weight gradient: k
+  int32_t m_len;             // M side: output features; weight gradient: n, or k in kWgradT
+  int32_t n_len;             // weight gradient: k, or n in kWgradT
   int32_t red;               // row products: reduction length
   int32_t m_tiles, n_tiles, tile_n;   // n_tiles, tile_n: weight gradient
   int32_t splits;            // runs that the reduction of a tile is cut into
@@ -419,7 +420,7 @@ struct Walker {
       end = s.end;
       if (base == 0) lo = __shfl_sync(0xffffffffu, begin, 0);
       const int lane = threadIdx.x % 32;
-      if constexpr (MODE == kWgrad) mine = base + lane < p.g.experts ? p.m_tiles * p.n_tiles : 0;
+      if constexpr (MODE >= kWgrad) mine = base + lane < p.g.experts ? p.m_tiles * p.n_tiles : 0;
       else mine = static_cast<int32_t>((end - begin + kSpan - 1) / kSpan) * p.m_tiles;
       upto = mine;
 #pragma unroll
@@ -435,7 +436,7 @@ struct Walker {
     const int32_t local = tile - __shfl_sync(0xffffffffu, upto - mine, src);
     t.e = base + src;
     constexpr int32_t kWidth = kStepK * subs_of(SHAPE);
-    if constexpr (MODE == kWgrad) {
+    if constexpr (MODE >= kWgrad) {
       t.m0 = local / p.n_tiles * 256;
       t.n0 = local % p.n_tiles * p.tile_n;
       t.width = t.valid = p.tile_n;
@@ -472,7 +473,7 @@ struct Walker {
 template <int MODE>
 struct Writer {
   const PairParams& p;
-  uint8_t* stage;    // 32 lines of 64 B (the 16-byte pieces of a line permuted as SWIZZLE_64B)
+  uint8_t* stage;    // 32 lines of 64 B (their 16-byte pieces permuted as SWIZZLE_64B), or 16 plain ones of 128 B
   int lane;
   int32_t e = 0, m = 0, cols = 0;   // which result (expert, run of the reduction); first M row; columns there are
   int64_t n0 = 0;                   // column 0 in the output: row products: its row; weight gradient: its column
@@ -484,7 +485,7 @@ struct Writer {
   }
   // Row products that leave by TMA take fragments, everything else a row of 32 columns a lane.
   __device__ __forceinline__ void load(uint32_t acc, uint32_t (&r)[32]) const {
-    if (MODE != kWgrad && p.tma_out) {
+    if (MODE != kWgrad && p.tma_out && (MODE < kWgrad || !p.f32)) {
       tmem_ld_fragments<0>(acc, r);
       tmem_ld_fragments<16>(acc + (16u << 16), r);
     } else {
@@ -493,13 +494,14 @@ struct Writer {
   }
   __device__ __forceinline__ void write(int32_t col, uint32_t (&r)[32]) {
     if constexpr (MODE == kWgrad) write_gradient(col, r);
+    else if (MODE == kWgradT && p.tma_out && p.f32) write_lines(col, r);
     else if (p.tma_out) write_rows(col, r);
     else write_elements(col, r);
   }
 
   // Tensor memory holds a feature a lane and a row a column: 8 x 8 fragments are
   // stored transposed, into lines of 32 features of one row, and a full tile of 32
-  // rows leaves by TMA.
+  // rows leaves by TMA (a weight gradient's always does: its matrix ends at n, not at a neighbour).
   __device__ __forceinline__ void write_rows(int32_t col, uint32_t (&r)[32]) {
     const int32_t rows = min(32, cols - col);
     pack_pairs(r, p.bf16);   // words 0..7: lanes 0..15, 8..15: lanes 16..31
@@ -510,11 +512,12 @@ struct Writer {
       stmatrix_t(smem_u32(stage) + line * 64 + ((lane / 8 ^ (line >> 1 & 3)) << 4), r[2 * i], r[2 * i + 1], r[8 + 2 * i],
                  r[8 + 2 * i + 1]);
     }
-    if (rows == 32) {
+    if (MODE == kWgradT || rows == 32) {
       fence_proxy_async_smem();
       __syncwarp();
       if (elect_one()) {
-        tma_store_2d(&p.out, stage, m, static_cast<int32_t>(n0) + col);
+        if constexpr (MODE == kWgradT) tma_store_3d(&p.out, stage, m, static_cast<int32_t>(n0) + col, e);
+        else tma_store_2d(&p.out, stage, m, static_cast<int32_t>(n0) + col);
         bulk_commit();
       }
     } else {   // the group's last rows: the next ones are another group's
@@ -530,18 +533,43 @@ struct Writer {
     }
   }
 
+  // f32 of a transposed gradient, lane = k, register = n: 16 lines of 128 bytes at a time.
+  __device__ __forceinline__ void write_lines(int32_t col, uint32_t (&r)[32]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (16 * h >= cols - col) break;
+      stage_free();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) reinterpret_cast<uint32_t*>(stage)[32 * j + lane] = r[16 * h + j];
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (elect_one()) {
+        const int32_t y = static_cast<int32_t>(n0) + col + 16 * h;
+        if (p.accumulate) tma_add_3d(&p.out, stage, m, y, e);
+        else tma_store_3d(&p.out, stage, m, y, e);
+        bulk_commit();
+      }
+    }
+  }
+
   // f32 rows, and outputs that TMA cannot address: lane = feature, register = row,
   // a warp's store is 32 features of one row.
   __device__ __forceinline__ void write_elements(int32_t col, uint32_t (&r)[32]) const {
     const int32_t rows = m + lane < p.m_len ? min(32, cols - col) : 0;
-    const int64_t at = e * p.stride_split + (n0 + col) * p.ld + m + lane;
+    const int64_t at = e * (MODE == kWgradT ? p.stride_e : p.stride_split) + (n0 + col) * p.ld + m + lane;
+    const bool add = MODE == kWgradT && p.accumulate;
     if (p.f32) {
       float* dst = static_cast<float*>(p.dst) + at;
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (j < rows) dst[j * p.ld] = __uint_as_float(r[j]);
+        if (j < rows) dst[j * p.ld] = __uint_as_float(r[j]) + (add ? dst[j * p.ld] : 0.f);
     } else {
       uint16_t* dst = static_cast<uint16_t*>(p.dst) + at;
+      if (add) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j)
+          if (j < rows) r[j] = __float_as_uint(__uint_as_float(r[j]) + widen16(dst[j * p.ld], p.bf16));
+      }
       pack_each(r, p.bf16);
 #pragma unroll
       for (int j = 0; j < 32; ++j)
@@ -610,7 +638,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   constexpr bool WIDE = SHAPE == kTwo;
   constexpr int kSubs = subs_of(SHAPE);
   constexpr uint32_t kStages = SHAPE == kOne ? 6 : SHAPE == kNarrow ? 5 : 4;
-  constexpr uint32_t kBBytes = SHAPE == kNarrow ? kOperandBytes / 4 : SHAPE == kMiddle ? kOperandBytes / 2 : kOperandBytes;   // B of a 64-wide block
+  constexpr uint32_t kBBytes = kOperandBytes / (SHAPE == kNarrow ? 4 : SHAPE == kMiddle ? 2 : 1);   // B of a 64-wide block
   constexpr uint32_t kStageBytes = kSubs * (kOperandBytes + (WIDE ? 2 : 1) * kBBytes);
   static_assert(kStages <= kMaxStages && kStages * kStageBytes <= kRingBytes);
   extern __shared__ uint8_t raw[];
@@ -659,14 +687,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       const int32_t halves[2] = {t.columns(0) / 2, WIDE && t.parts > 1 ? t.columns(1) / 2 : 0};
       const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128;
       const uint32_t bytes =
-          kOperandBytes + (MODE == kWgrad ? kBBytes : static_cast<uint32_t>(halves[0] + halves[1]) * kStepK * 2);
+          kOperandBytes + (MODE >= kWgrad ? kBBytes : static_cast<uint32_t>(halves[0] + halves[1]) * kStepK * 2);
       for (int32_t s = 0; s < t.steps; ++s, ++it) {
         if (!mbar_wait(&c->empty[st], phase, abort, p.dev_err)) { ok = false; break; }
         uint8_t* a = ring + st * kStageBytes;
         uint8_t* b = a + kSubs * kOperandBytes;
         // a step whose rows past the group's end are still to be zeroed lands on this CTA's own barrier
         const bool last = s + 1 == t.steps;
-        const bool fix = MODE == kWgrad && last && t.tail % 16 != 0;
+        const bool fix = MODE >= kWgrad && last && t.tail % 16 != 0;
         const uint32_t bar = fix ? peer_addr(&c->tail[st], rank) : peer_addr(&c->full[st], 0);
         const int subs = kSubs > 1 && last && t.tail ? (t.tail + kStepK - 1) / kStepK : kSubs;
         if (elect_one()) {
@@ -685,7 +713,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
               pair_load_2d(a, &p.a, bar, m, y);
               pair_load_2d(a + kChunkBytes, &p.a, bar, m + 64, y);
             }
-            if constexpr (MODE == kWgrad) {
+            if constexpr (MODE >= kWgrad) {
               const int32_t y = static_cast<int32_t>(t.row0) + r, x = t.n0 + static_cast<int32_t>(rank) * halves[0];
               pair_load_2d(b, &p.b[0], bar, x, y);
               if constexpr (kBBytes > kChunkBytes) pair_load_2d(b + kChunkBytes, &p.b[0], bar, x + 64, y);
@@ -735,7 +763,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
       if (t.steps == 0) continue;   // an empty group's gradient: zeros, without an accumulator
-      constexpr uint32_t kMajors = (MODE != kRowsK ? kIdescMajorA : 0) | (MODE == kWgrad ? kIdescMajorB : 0);
+      constexpr uint32_t kMajors = (MODE != kRowsK ? kIdescMajorA : 0) | (MODE >= kWgrad ? kIdescMajorB : 0);
       const uint32_t idescs[2] = {umma_idesc(p.bf16, 256, t.columns(0)) | kMajors,
                                   WIDE && t.parts > 1 ? umma_idesc(p.bf16, 256, t.columns(1)) | kMajors : 0};
       for (int32_t s = 0; ok && s < t.steps; ++s) {
@@ -753,13 +781,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           if (!ok) break;
           tc_fence_after();
           const uint32_t b = a + kSubs * kOperandBytes + part * kOperandBytes;
-          const uint64_t db = MODE == kWgrad ? sw128_mn_desc(b, kChunkBytes) : sw128_desc(b);
+          const uint64_t db = MODE >= kWgrad ? sw128_mn_desc(b, kChunkBytes) : sw128_desc(b);
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kSubs * kStepK / 16; ++k)   // the next 64-wide block of an operand: its bytes / 16 on
               if (k < count)
                 pair_umma_f16(acc, da + k % 4 * (MODE == kRowsK ? 2 : 128) + k / 4 * (kOperandBytes >> 4),
-                              db + k % 4 * (MODE == kWgrad ? 128 : 2) + k / 4 * (kBBytes >> 4), idescs[part], s | k);
+                              db + k % 4 * (MODE >= kWgrad ? 128 : 2) + k / 4 * (kBBytes >> 4), idescs[part], s | k);
             if (part + 1 == t.parts) pair_umma_commit(&c->empty[st]);
             if (last) pair_umma_commit(&c->acc_full[buf]);
           }
@@ -775,7 +803,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       pair_umma_commit(&c->done);
       mbar_wait(&c->done, 0, &ignore, p.dev_err);
     }
-  } else if (warp == 2 && MODE == kWgrad) {
+  } else if (warp == 2 && MODE >= kWgrad) {
     // ---------------------------------------------------------------- tails
     uint32_t it = 0;
     int uses = 0;   // lane s: how many tails stage s has held
@@ -807,13 +835,13 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     uint32_t n = 0;
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
-      out.e = MODE == kWgrad ? t.split * p.g.experts + t.e : t.split;
+      out.e = MODE >= kWgrad ? t.split * p.g.experts + t.e : t.split;
       out.m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
       for (int acc_n = 0; acc_n < (WIDE ? t.parts : 1); ++acc_n) {
-        const int32_t cols = MODE == kWgrad ? min(t.width, p.n_len - t.n0) : min(t.width, t.valid - acc_n * t.width);
+        const int32_t cols = MODE >= kWgrad ? min(t.width, p.n_len - t.n0) : min(t.width, t.valid - acc_n * t.width);
         const int chunks = out.m < p.m_len && cols > part * 32 ? (cols - part * 32 + 63) / 64 : 0;
         out.cols = cols;
-        out.n0 = MODE == kWgrad ? t.n0 : t.row0 + acc_n * t.width;
+        out.n0 = MODE >= kWgrad ? t.n0 : t.row0 + acc_n * t.width;
         uint32_t r0[32], r1[32];
         if (t.steps == 0) {   // an empty group's gradient
           if (p.accumulate) continue;
@@ -851,7 +879,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       }
     }
     if (p.tma_out && elect_one()) bulk_wait_all();
-    if (MODE != kWgrad && ok) {   // rows of no group
+    if (MODE < kWgrad && ok) {   // rows of no group
       const int64_t gap = walk.lo + (p.g.rows - walk.carry);
       for (int64_t j = blockIdx.x; j < gap * p.splits; j += gridDim.x) {
         const int64_t i = j % gap, at = j / gap * p.stride_split + (i < walk.lo ? i : i - walk.lo + walk.carry) * p.ld;
@@ -924,7 +952,9 @@ int sm_count(int* sms) {
                           reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kTwo>),
                           reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kNarrow>),
                           reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, kOne>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, kMiddle>)}) {
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, kMiddle>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgradT, kOne>),
+                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgradT, kMiddle>)}) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
       if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
     }
@@ -961,8 +991,8 @@ constexpr int kPairsPlanned = 74;   // pairs of a B200; what the split is planne
 constexpr int kMaxSplits = 16;
 
 // Runs for `tiles` tiles of `steps` steps and `values` results, by what they take: step_us a step (0.28 with 256
-// columns, 0.14 with up to 128, 0.15 to 0.3 for a weight gradient's, by how its rows lie in memory), about 2.5 us for the second kernel, and the fp32 partials written and read at
-// some 6 MB a us (500 rows x 2048 x 2048: 1 run 14.4 us, 4 runs 15.6; 200 rows x 1024 x 1536 of 4 experts: 7.9
+// columns, 0.14 with up to 128, 0.15 to 0.3 for a weight gradient's, by how its rows lie in memory), about
+// 2.5 us for the second kernel, and the fp32 partials written and read at some 6 MB a us (500 rows x 2048 x 2048: 1 run 14.4 us, 4 runs 15.6; 200 rows x 1024 x 1536 of 4 experts: 7.9
 // and 9.0; weight gradient of 5 x 1185 rows, 112 x 1208: 2 runs 17.3, 1 run 20.3).
 struct SplitPlan {
   int splits;
@@ -1003,25 +1033,41 @@ int rows_splits(int64_t rows, int32_t experts, int32_t m_len, int32_t red) {
                      span_of(shape) >= 256 ? 0.28 : 0.14, rows * m_len)
       .splits;
 }
-int64_t wgrad_tiles(int32_t experts, int32_t n, int32_t k, PairShape shape) {
-  return static_cast<int64_t>(experts) * ((n + 255) / 256) * ((k + span_of(shape) - 1) / span_of(shape));
+int64_t wgrad_tiles(int32_t experts, int32_t m_len, int32_t n_len, PairShape shape) {
+  return static_cast<int64_t>(experts) * ((m_len + 255) / 256) * ((n_len + span_of(shape) - 1) / span_of(shape));
 }
-SplitPlan wgrad_plan(int64_t rows, int32_t experts, int32_t n, int32_t k, PairShape shape) {
-  return plan_splits(wgrad_tiles(experts, n, k, shape), rows / experts / kStepK, shape == kOne ? 0.28 : 0.2,
-                     static_cast<int64_t>(experts) * n * k);
+SplitPlan wgrad_plan(int64_t rows, int32_t experts, int32_t m_len, int32_t n_len, PairShape shape) {
+  return plan_splits(wgrad_tiles(experts, m_len, n_len, shape), rows / experts / kStepK, shape == kOne ? 0.28 : 0.2,
+                     static_cast<int64_t>(experts) * m_len * n_len);
 }
 // Tiles of 128 columns and steps of 128 rows where each tile still has a pair of its own, or where there are no more
 // columns (2790 rows of 9 groups, 256 x 128: 6.2 us against 6.6; 8192 rows, 512 x 512: 23.8 against 42.1; 15244 rows
 // of 77, 120 x 112: 12.8 against 15.1).  With more tiles than pairs they lose (1125 rows of 4, 432 x 3712: 10.9 us
 // against 9.4), and where twice as wide ones may share a reduction that these may not (20787 rows of 3,
 // 120 x 2232: 43.2 against 34.2).
-PairShape wgrad_shape(int64_t rows, int32_t experts, int32_t n, int32_t k) {
-  if (k <= span_of(kMiddle)) return kMiddle;
-  if (wgrad_tiles(experts, n, k, kMiddle) > kPairsPlanned) return kOne;
-  return wgrad_plan(rows, experts, n, k, kMiddle).us <= wgrad_plan(rows, experts, n, k, kOne).us ? kMiddle : kOne;
+PairShape wgrad_shape(int64_t rows, int32_t experts, int32_t m_len, int32_t n_len) {
+  if (n_len <= span_of(kMiddle)) return kMiddle;
+  if (wgrad_tiles(experts, m_len, n_len, kMiddle) > kPairsPlanned) return kOne;
+  const double middle = wgrad_plan(rows, experts, m_len, n_len, kMiddle).us;
+  return middle <= wgrad_plan(rows, experts, m_len, n_len, kOne).us ? kMiddle : kOne;
+}
+// Whether x's columns are the M side and dy's the N side (kWgradT) rather than the other way about: where that pads
+// the matrix by less, and it counts because there are more tiles than pairs (2084 rows of 84 groups, 88 x 1336: 14.3
+// us against 19.4; 14 rows of 90, 352 x 1464: 24.9 against 29.3) or because the runs of a split get shorter (20787
+// rows of 3, 120 x 2232: 27.7 against 33.9).  Elsewhere it gains nothing (3378 rows, 352 x 2136: 16.8 against 15.8).
+bool wgrad_swaps(int64_t rows, int32_t experts, int32_t n, int32_t k) {
+  const auto area = [](int64_t m_len, int64_t n_len) { return (m_len + 255) / 256 * 256 * ((n_len + 63) / 64 * 64); };
+  if (10 * area(k, n) >= 9 * area(n, k)) return false;
+  if (wgrad_tiles(experts, n, k, kMiddle) > kPairsPlanned) return true;
+  const auto us = [&](int32_t m_len, int32_t n_len) {
+    return wgrad_plan(rows, experts, m_len, n_len, wgrad_shape(rows, experts, m_len, n_len)).us;
+  };
+  return us(k, n) < us(n, k);
 }
 int wgrad_splits(int64_t rows, int32_t experts, int32_t n, int32_t k) {
-  return wgrad_plan(rows, experts, n, k, wgrad_shape(rows, experts, n, k)).splits;
+  const bool swap = wgrad_swaps(rows, experts, n, k);
+  const int32_t m_len = swap ? k : n, n_len = swap ? n : k;
+  return wgrad_plan(rows, experts, m_len, n_len, wgrad_shape(rows, experts, m_len, n_len)).splits;
 }
 
 struct JoinParams {
@@ -1244,11 +1290,12 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
     if (int rc = sm_count(&sms)) return rc;
     PairParams q{};
     q.g = groups;
-    q.m_len = n; q.n_len = k;
-    q.m_tiles = (n + 255) / 256;
-    const PairShape shape = wgrad_shape(rows, experts, n, k);
-    q.n_tiles = (k + span_of(shape) - 1) / span_of(shape);
-    q.tile_n = ((k + q.n_tiles - 1) / q.n_tiles + 63) / 64 * 64;
+    const bool swap = wgrad_swaps(rows, experts, n, k);
+    q.m_len = swap ? k : n; q.n_len = swap ? n : k;
+    q.m_tiles = (q.m_len + 255) / 256;
+    const PairShape shape = wgrad_shape(rows, experts, q.m_len, q.n_len);
+    q.n_tiles = (q.n_len + span_of(shape) - 1) / span_of(shape);
+    q.tile_n = ((q.n_len + q.n_tiles - 1) / q.n_tiles + 63) / 64 * 64;
     q.splits = wgrad_splits(rows, experts, n, k);
     const int64_t pitch = pitch4(k), lines = static_cast<int64_t>(experts) * n;
     if (workspace_bytes < q.splits * lines * pitch * sizeof(float) || !workspace) q.splits = 1;
@@ -1258,11 +1305,11 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
     q.stride_e = split ? n * pitch : stride_out;
     q.f32 = split || f32; q.bf16 = bf16; q.accumulate = accumulate && !split;
     q.dev_err = dev_err;
-    const int64_t tiles = wgrad_tiles(experts, n, k, shape) * q.splits;
+    const int64_t tiles = wgrad_tiles(experts, q.m_len, q.n_len, shape) * q.splits;
     if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if (int rc = make_map(&q.a, dy, dt, 2, n, rows, 1, 2 * ld_dy, 0, 64, 64)) return rc;
-    if (int rc = make_map(&q.b[0], x, dt, 2, k, rows, 1, 2 * ld_x, 0, 64, 64)) return rc;
+    if (int rc = make_map(swap ? &q.b[0] : &q.a, dy, dt, 2, n, rows, 1, 2 * ld_dy, 0, 64, 64)) return rc;
+    if (int rc = make_map(swap ? &q.a : &q.b[0], x, dt, 2, k, rows, 1, 2 * ld_x, 0, 64, 64)) return rc;
     // a 16-bit sum is rounded once: that of an addition to out cannot be left to TMA, which rounds before and after
     const int64_t z = q.f32 ? 4 : 2, results = static_cast<int64_t>(experts) * q.splits;
     // (and a store ends at a multiple of 16 bytes, with zeros in what a row lacks: the partials have room for that)
@@ -1270,10 +1317,13 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
                 (q.f32 || !q.accumulate);
     if (q.tma_out)
       if (int rc = make_map(&q.out, q.dst, q.f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dt, 3, k, n, results, z * q.ld,
-                            results == 1 ? z * q.ld : z * q.stride_e, q.f32 ? 16 : 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
+                            results == 1 ? z * q.ld : z * q.stride_e, q.f32 && !swap ? 16 : 32, q.f32 && swap ? 16 : 32,
+                            q.f32 && swap ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
-    cudaError_t e = shape == kOne ? launch_pair<kWgrad, kOne>(q, tiles, sms, st)
-                                  : launch_pair<kWgrad, kMiddle>(q, tiles, sms, st);
+    cudaError_t e = swap ? shape == kOne ? launch_pair<kWgradT, kOne>(q, tiles, sms, st)
+                                         : launch_pair<kWgradT, kMiddle>(q, tiles, sms, st)
+                    : shape == kOne ? launch_pair<kWgrad, kOne>(q, tiles, sms, st)
+                                    : launch_pair<kWgrad, kMiddle>(q, tiles, sms, st);
     if (e == cudaSuccess && split) {
       JoinParams j{};
       j.part = static_cast<const float*>(workspace);

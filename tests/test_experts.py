@@ -234,6 +234,30 @@ def test_grouped_wgrad_of_many_tiles(sizes, out_dtype):
     assert got2[bad].isnan().all() and torch.equal(got2[rest], got[rest])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("ld", [1096, 1091])
+@pytest.mark.parametrize("out_dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("n,k", [(72, 1088), (264, 1000), (300, 1091)])
+def test_grouped_wgrad_with_x_on_the_wide_side(n, k, out_dtype, ld):
+    """A narrow n beside a wide k, in more tiles than pairs: rows of k by TMA and by element, summed, with empty groups."""
+    sizes = [3, 0, 65, 200, 16, 1, 130, 0, 64, 9, 17, 33]
+    dy, x = normal((sum(sizes) + 2, n), BF16, 65), normal((sum(sizes) + 2, k), BF16, 66)
+    dy[-2:], x[-2:] = float("nan"), float("inf")
+    off = offsets_of(sizes)
+    want, mass = wgrad_reference(dy, x, off)
+    out = torch.full((len(sizes), n, ld), 5.0, dtype=out_dtype, device=DEV)
+    xd = torch.zeros(sum(sizes) + 2, 1096, dtype=BF16, device=DEV)
+    dyd = torch.zeros(sum(sizes) + 2, (n + 7) // 8 * 8, dtype=BF16, device=DEV)
+    dyd[:, :n], xd[:, :k] = dy.to(DEV), x.to(DEV)
+    experts.grouped_wgrad(dyd[:, :n], xd[:, :k], off.to(DEV), out=out[:, :, :k])
+    assert_sum(out[:, :, :k], want, mass, max(sizes), out_dtype)
+    assert (out[:, :, k:] == 5).all()
+    base = out[:, :, :k].double().cpu()
+    experts.grouped_wgrad(dyd[:, :n], xd[:, :k], off.to(DEV), out=out[:, :, :k], accumulate=True)
+    assert_sum(out[:, :, :k], want + base, mass + base.abs(), max(sizes) + 1, out_dtype)
+    assert (out[:, :, k:] == 5).all()
+
+
 def padded(t, fill):
     """t as a view into rows that are some elements longer (a multiple of 16 bytes), which hold `fill`."""
     width = t.shape[-1] // 8 * 8 + 8
