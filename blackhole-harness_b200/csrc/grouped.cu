@@ -984,16 +984,15 @@ cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_
 // ------------------------------------------------------------------- splits
 // Products of few tiles leave most pairs idle while a few walk a long reduction:
 // their reduction is cut into `splits` runs of steps, each with an fp32 partial
-// result in the workspace, which a second kernel adds in order and rounds (4
-// experts x 75 rows x 512 x 4096: 11.3 us instead of 14.1; weight gradient of 2 x
-// 4000 rows, 256 x 512: 12.5 instead of 23.8).
+// result in the workspace, which a second kernel adds in order and rounds.
 constexpr int kPairsPlanned = 74;   // pairs of a B200; what the split is planned for
 constexpr int kMaxSplits = 16;
 
 // Runs for `tiles` tiles of `steps` steps and `values` results, by what they take: step_us a step (0.28 with 256
 // columns, 0.14 with up to 128, 0.15 to 0.3 for a weight gradient's, by how its rows lie in memory), about
-// 2.5 us for the second kernel, and the fp32 partials written and read at some 6 MB a us (500 rows x 2048 x 2048: 1 run 14.4 us, 4 runs 15.6; 200 rows x 1024 x 1536 of 4 experts: 7.9
-// and 9.0; weight gradient of 5 x 1185 rows, 112 x 1208: 2 runs 17.3, 1 run 20.3).
+// 1 us for the second kernel and 0.2 a run, and the fp32 partials written and read at some 6 MB a us (6 rows, 776 x
+// 1624: 1, 2, 4, 8 runs 9.0, 8.8, 7.8, 8.1 us; 300 rows of 4 groups, 512 x 4096: 13.5, 11.9, 10.7, 11.7; 500 rows,
+// 2048 x 2048: 10.0, 14.8, 17.0, 23.1; weight gradient of 2 x 4000 rows, 256 x 512: 13.9, 12.1, 10.4, 12.2).
 struct SplitPlan {
   int splits;
   double us;
@@ -1002,7 +1001,7 @@ SplitPlan plan_splits(int64_t tiles, int64_t steps, double step_us, int64_t valu
   const int64_t most = std::min<int64_t>({kPairsPlanned / std::max<int64_t>(tiles, 1), steps / 4, kMaxSplits});
   SplitPlan best = {1, step_us * static_cast<double>(steps)};
   for (int s = 2; s <= most; ++s) {
-    const double us = step_us * static_cast<double>((steps + s - 1) / s) + 2.5 +
+    const double us = step_us * static_cast<double>((steps + s - 1) / s) + 1 + 0.2 * s +
                       8e-6 / 6 * static_cast<double>(s * values);
     if (us < best.us) best = {s, us};
   }
@@ -1037,7 +1036,7 @@ int64_t wgrad_tiles(int32_t experts, int32_t m_len, int32_t n_len, PairShape sha
   return static_cast<int64_t>(experts) * ((m_len + 255) / 256) * ((n_len + span_of(shape) - 1) / span_of(shape));
 }
 SplitPlan wgrad_plan(int64_t rows, int32_t experts, int32_t m_len, int32_t n_len, PairShape shape) {
-  return plan_splits(wgrad_tiles(experts, m_len, n_len, shape), rows / experts / kStepK, shape == kOne ? 0.28 : 0.2,
+  return plan_splits(wgrad_tiles(experts, m_len, n_len, shape), rows / experts / kStepK, shape == kOne ? 0.28 : 0.17,
                      static_cast<int64_t>(experts) * m_len * n_len);
 }
 // Tiles of 128 columns and steps of 128 rows where each tile still has a pair of its own, or where there are no more
@@ -1088,8 +1087,9 @@ __global__ void __launch_bounds__(256) grouped_join_kernel(const JoinParams p) {
   const int64_t row = i / pieces;
   const int32_t col = static_cast<int32_t>(i % pieces) * 4;
   float v[4] = {};
+#pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
-    const float4 f = __ldg(reinterpret_cast<const float4*>(p.part + (s * p.rows + row) * p.pitch + col));
+    const float4 f = *reinterpret_cast<const float4*>(p.part + (s * p.rows + row) * p.pitch + col);
     v[0] += f.x;
     v[1] += f.y;
     v[2] += f.z;
