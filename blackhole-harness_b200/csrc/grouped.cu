@@ -989,20 +989,21 @@ constexpr int kPairsPlanned = 74;   // pairs of a B200; what the split is planne
 constexpr int kMaxSplits = 16;
 
 // Runs for `tiles` tiles of `steps` steps and `values` results, by what they take: step_us a step (0.28 with 256
-// columns, 0.14 with up to 128, 0.15 to 0.3 for a weight gradient's, by how its rows lie in memory), about
-// 1 us for the second kernel and 0.2 a run, and the fp32 partials written and read at some 6 MB a us (6 rows, 776 x
-// 1624: 1, 2, 4, 8 runs 9.0, 8.8, 7.8, 8.1 us; 300 rows of 4 groups, 512 x 4096: 13.5, 11.9, 10.7, 11.7; 500 rows,
-// 2048 x 2048: 10.0, 14.8, 17.0, 23.1; weight gradient of 2 x 4000 rows, 256 x 512: 13.9, 12.1, 10.4, 12.2).
+// columns, 0.14 with up to 128, 0.15 to 0.3 for a weight gradient's, by how its rows lie in memory), value_us for
+// an fp32 partial written and read (row products write theirs without TMA), some 1.2 us for the second
+// kernel and 0.15 a run.  With 1, 2, 4, 8 runs: 6 rows, 776 x 1624: 9.0, 8.8, 7.8, 8.1 us; 300 rows of 4 groups, 512 x
+// 4096: 13.5, 11.9, 10.7, 11.7; 500 rows, 2048 x 2048: 10.0, 14.8, 17.0, 23.1; weight gradient of 2 x 4000 rows,
+// 256 x 512: 13.9, 12.1, 10.4, 12.2.
 struct SplitPlan {
   int splits;
   double us;
 };
-SplitPlan plan_splits(int64_t tiles, int64_t steps, double step_us, int64_t values) {
+SplitPlan plan_splits(int64_t tiles, int64_t steps, double step_us, int64_t values, double value_us) {
   const int64_t most = std::min<int64_t>({kPairsPlanned / std::max<int64_t>(tiles, 1), steps / 4, kMaxSplits});
   SplitPlan best = {1, step_us * static_cast<double>(steps)};
   for (int s = 2; s <= most; ++s) {
-    const double us = step_us * static_cast<double>((steps + s - 1) / s) + 1 + 0.2 * s +
-                      8e-6 / 6 * static_cast<double>(s * values);
+    const double us = step_us * static_cast<double>((steps + s - 1) / s) + 1.2 + 0.15 * s +
+                      value_us * static_cast<double>(s * values);
     if (us < best.us) best = {s, us};
   }
   return best;
@@ -1029,7 +1030,7 @@ PairShape rows_shape(int64_t rows, int32_t experts, int32_t m_len) {
 int rows_splits(int64_t rows, int32_t experts, int32_t m_len, int32_t red) {
   const PairShape shape = rows_shape(rows, experts, m_len);
   return plan_splits(row_tiles(rows, experts, m_len, shape), (red + kStepK - 1) / kStepK,
-                     span_of(shape) >= 256 ? 0.28 : 0.14, rows * m_len)
+                     span_of(shape) >= 256 ? 0.28 : 0.14, rows * m_len, 3.3e-6)
       .splits;
 }
 int64_t wgrad_tiles(int32_t experts, int32_t m_len, int32_t n_len, PairShape shape) {
@@ -1037,7 +1038,7 @@ int64_t wgrad_tiles(int32_t experts, int32_t m_len, int32_t n_len, PairShape sha
 }
 SplitPlan wgrad_plan(int64_t rows, int32_t experts, int32_t m_len, int32_t n_len, PairShape shape) {
   return plan_splits(wgrad_tiles(experts, m_len, n_len, shape), rows / experts / kStepK, shape == kOne ? 0.28 : 0.17,
-                     static_cast<int64_t>(experts) * m_len * n_len);
+                     static_cast<int64_t>(experts) * m_len * n_len, 1.7e-6);
 }
 // Tiles of 128 columns and steps of 128 rows where each tile still has a pair of its own, or where there are no more
 // columns (2790 rows of 9 groups, 256 x 128: 6.2 us against 6.6; 8192 rows, 512 x 512: 23.8 against 42.1; 15244 rows
