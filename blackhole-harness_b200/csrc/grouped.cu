@@ -341,8 +341,8 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 // itself, so that no size is known on the host.
 //
 // Measured, bf16, 96 experts, 1536 x 2048: 512 rows 91 us (HBM, 6.7 TB/s); 32768 rows
-// 174..184 us (1120..1180 TFLOP/s; HBM and tensor cores, each of which alone takes
-// 145); the weight gradient of those 194..203 us (604 MB written, which takes a
+// 174..186 us (1110..1180 TFLOP/s; HBM and tensor cores, each of which alone takes
+// 145); the weight gradient of those 194..207 us (604 MB written, which takes a
 // plain fill 157).  A single product of 8192 x 8192 x 2048: 174 us (1580 TFLOP/s).
 constexpr int kMaxStages = 6;
 constexpr int kStepK = 64;
@@ -1041,7 +1041,7 @@ SplitPlan wgrad_plan(int64_t rows, int32_t experts, int32_t m_len, int32_t n_len
                      static_cast<int64_t>(experts) * m_len * n_len, 1.7e-6);
 }
 // Tiles of 128 columns and steps of 128 rows where each tile still has a pair of its own, or where there are no more
-// columns (2790 rows of 9 groups, 256 x 128: 6.2 us against 6.6; 8192 rows, 512 x 512: 23.8 against 42.1; 15244 rows
+// columns (2790 rows of 9 groups, 256 x 128: 6.2 us against 6.6; 8192 rows, 512 x 512, unsplit: 23.8 against 42.1; 15244 rows
 // of 77, 120 x 112: 12.8 against 15.1).  With more tiles than pairs they lose (1125 rows of 4, 432 x 3712: 10.9 us
 // against 9.4), and where twice as wide ones may share a reduction that these may not (20787 rows of 3,
 // 120 x 2232: 43.2 against 34.2).
