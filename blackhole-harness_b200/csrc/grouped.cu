@@ -1041,10 +1041,10 @@ SplitPlan wgrad_plan(int64_t rows, int32_t experts, int32_t m_len, int32_t n_len
                      static_cast<int64_t>(experts) * m_len * n_len, 1.7e-6);
 }
 // Tiles of 128 columns and steps of 128 rows where each tile still has a pair of its own, or where there are no more
-// columns (2790 rows of 9 groups, 256 x 128: 6.2 us against 6.6; 8192 rows, 512 x 512, unsplit: 23.8 against 42.1; 15244 rows
-// of 77, 120 x 112: 12.8 against 15.1).  With more tiles than pairs they lose (1125 rows of 4, 432 x 3712: 10.9 us
-// against 9.4), and where twice as wide ones may share a reduction that these may not (20787 rows of 3,
-// 120 x 2232: 43.2 against 34.2).
+// columns (2790 rows of 9 groups, 256 x 128: 6.2 us against 6.6; 8192 rows, 512 x 512, unsplit: 23.8 against 42.1;
+// 15244 rows of 77, 120 x 112: 12.8 against 15.1).  With more tiles than pairs they lose (1125 rows of 4, 432 x 3712:
+// 10.9 us against 9.4), and where twice as wide ones may share a reduction that these may not (20787 rows of 3,
+// 120 x 2232 with n on the M side: 43.2 against 34.2).
 PairShape wgrad_shape(int64_t rows, int32_t experts, int32_t m_len, int32_t n_len) {
   if (n_len <= span_of(kMiddle)) return kMiddle;
   if (wgrad_tiles(experts, m_len, n_len, kMiddle) > kPairsPlanned) return kOne;
