@@ -689,7 +689,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       const uint32_t bytes =
           kOperandBytes + (MODE >= kWgrad ? kBBytes : static_cast<uint32_t>(halves[0] + halves[1]) * kStepK * 2);
       for (int32_t s = 0; s < t.steps; ++s, ++it) {
-        if (!mbar_wait(&c->empty[st], phase, abort, p.dev_err)) { ok = false; break; }
+        ok = warp_wait(&c->empty[st], phase, abort, p.dev_err);
+        if (!ok) break;
         uint8_t* a = ring + st * kStageBytes;
         uint8_t* b = a + kSubs * kOperandBytes;
         // a step whose rows past the group's end are still to be zeroed lands on this CTA's own barrier
@@ -741,7 +742,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         __syncwarp();
         if (++st == kStages) { st = 0; phase ^= 1; }
       }
-      ok = __all_sync(0xffffffffu, ok);
     }
     if (walk.bad && blockIdx.x == 0) atomicOr(p.dev_err, kDevErrOffsets);
     if (ok && lane == 0) {   // the last steps are released to both CTAs before either leaves
@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
                                   WIDE && t.parts > 1 ? umma_idesc(p.bf16, 256, t.columns(1)) | kMajors : 0};
       for (int32_t s = 0; ok && s < t.steps; ++s) {
         const bool last = s + 1 == t.steps;
-        ok = mbar_wait(&c->full[st], phase, abort, p.dev_err);
+        ok = warp_wait(&c->full[st], phase, abort, p.dev_err);
         const uint32_t a = smem_u32(ring + st * kStageBytes);
         const uint64_t da = MODE == kRowsK ? sw128_desc(a) : sw128_mn_desc(a, kChunkBytes);
         const int count = last && t.tail ? (t.tail + 15) / 16 : kSubs * kStepK / 16;   // products of 16
@@ -776,8 +776,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         for (int part = 0; part < (WIDE ? 2 : 1); ++part) {
           if (part >= t.parts) break;
           const uint32_t buf = (n + part) % 2, acc = tmem + buf * kAccCols;
-          if (s == 0) ok = ok && mbar_wait(&c->acc_empty[buf], ((n + part) / 2 + 1) & 1, abort, p.dev_err);
-          ok = __all_sync(0xffffffffu, ok);
+          if (s == 0) ok = ok && warp_wait(&c->acc_empty[buf], ((n + part) / 2 + 1) & 1, abort, p.dev_err);
           if (!ok) break;
           tc_fence_after();
           const uint32_t b = a + kSubs * kOperandBytes + part * kOperandBytes;
@@ -796,7 +795,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         if (++st == kStages) { st = 0; phase ^= 1; }
       }
       n += t.parts;
-      ok = __all_sync(0xffffffffu, ok);
     }
     if (*abort && lane == 0) {   // products in flight end before their tensor memory goes
       int ignore = 0;
@@ -812,8 +810,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       it += t.steps;
       if (t.tail % 16 == 0) continue;
       const uint32_t st = (it - 1) % kStages;
-      ok = mbar_wait(&c->tail[st], __shfl_sync(0xffffffffu, uses, st) & 1, abort, p.dev_err);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = warp_wait(&c->tail[st], __shfl_sync(0xffffffffu, uses, st) & 1, abort, p.dev_err);
       if (lane == static_cast<int>(st)) ++uses;
       const uint32_t sub = t.tail / kStepK;
       uint8_t* a = ring + st * kStageBytes + sub * kOperandBytes;
@@ -853,7 +850,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           continue;
         }
         const uint32_t buf = n % 2, acc = tmem + buf * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16) + part * 32;
-        ok = __all_sync(0xffffffffu, mbar_wait(&c->acc_full[buf], (n / 2) & 1, abort, p.dev_err));
+        ok = warp_wait(&c->acc_full[buf], (n / 2) & 1, abort, p.dev_err);
         if (!ok) break;
         tc_fence_after();
         ++n;

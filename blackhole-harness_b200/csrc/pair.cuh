@@ -20,6 +20,11 @@ __device__ __forceinline__ bool elect_one() {
       : "=r"(ok));
   return ok != 0;
 }
+// A wait of a whole warp: true in all lanes or in none.  Where a wait runs out its lanes may disagree (one gives up
+// as another's poll succeeds); parted, they would meet in different warp-wide operations and hang.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* dev_err) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, dev_err));
+}
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));

@@ -1,0 +1,29 @@
+"""What the pair kernel's warps owe one another, read from its source: faults here would show as a hang or
+as a race, which no run may be made to show."""
+
+from __future__ import annotations
+
+import re
+
+from conftest import ROOT
+
+CSRC = ROOT / "blackhole-harness_b200" / "csrc"
+
+
+def kernel_lines():
+    """The lines of grouped_pair_kernel, without comments."""
+    src = (CSRC / "grouped.cu").read_text()
+    body = src[src.index("grouped_pair_kernel(const __grid_constant__"):src.index("encode_fn()")]
+    return [re.sub(r"//.*", "", line) for line in body.splitlines()]
+
+
+def test_a_warp_gives_up_as_one():
+    """Lanes that disagree on a wait that ran out must not part ways before a warp-wide operation: every wait
+    of a whole warp votes, and a bare wait stands only where a single lane runs."""
+    lines = kernel_lines()
+    bare = [i for i, line in enumerate(lines) if re.search(r"(?<!\w)mbar_wait\(", line)]
+    for i in bare:
+        assert any("lane == 0" in line for line in lines[max(0, i - 5):i]), lines[i]
+    assert sum("warp_wait(" in line for line in lines) >= 5
+    helper = (CSRC / "pair.cuh").read_text()
+    assert re.search(r"bool warp_wait\([^{]*\{\s*return __all_sync\(0xffffffffu, mbar_wait\(", helper)
