@@ -682,6 +682,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
     uint32_t it = 0, st = 0, phase = 1;
+    uint32_t tails = 0, tail_odd = 0;   // a bit a stage: whether it has held a tail, whether an odd number of them
     bool ok = true;
     for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
       const int32_t halves[2] = {t.columns(0) / 2, WIDE && t.parts > 1 ? t.columns(1) / 2 : 0};
@@ -697,6 +698,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         const bool last = s + 1 == t.steps;
         const bool fix = MODE >= kWgrad && last && t.tail % 16 != 0;
         const uint32_t bar = fix ? peer_addr(&c->tail[st], rank) : peer_addr(&c->full[st], 0);
+        if (fix) { tails |= 1u << st; tail_odd ^= 1u << st; }
         const int subs = kSubs > 1 && last && t.tail ? (t.tail + kStepK - 1) / kStepK : kSubs;
         if (elect_one()) {
           pair_arrive_expect_tx(bar, subs * bytes);
@@ -756,6 +758,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         const uint32_t j = it - 1 - back;
         mbar_wait(&c->full[j % kStages], (j / kStages) & 1, &ignore, p.dev_err);
       }
+    }
+    if (MODE >= kWgrad && *abort && lane == 0) {   // and, in each CTA, for the tails, which land on its own barriers
+      int ignore = 0;
+      for (uint32_t j = 0; j < kStages; ++j)
+        if (tails >> j & 1) mbar_wait(&c->tail[j], ~tail_odd >> j & 1, &ignore, p.dev_err);
     }
   } else if (warp == 1 && leader) {
     // ------------------------------------------------------------- products

@@ -27,3 +27,11 @@ def test_a_warp_gives_up_as_one():
     assert sum("warp_wait(" in line for line in lines) >= 5
     helper = (CSRC / "pair.cuh").read_text()
     assert re.search(r"bool warp_wait\([^{]*\{\s*return __all_sync\(0xffffffffu, mbar_wait\(", helper)
+
+
+def test_a_kernel_that_gives_up_waits_for_its_copies():
+    """After a wait that ran out no CTA may leave while copies still land in its shared memory: the leader waits
+    for the steps of both CTAs, each CTA for the tails, which complete on barriers of its own."""
+    text = "\n".join(kernel_lines())
+    for barrier, guard in (("full", r"\*abort && lane == 0 && leader"), ("tail", r"\*abort && lane == 0\)")):
+        assert re.search(guard + r"[^}]*mbar_wait\(&c->" + barrier + r"\[[^}]*&ignore", text), barrier
