@@ -177,7 +177,7 @@ __device__ __forceinline__ void plain_stage(uint16_t (*tile)[kPlainPitch], const
 
 template <bool WGRAD>
 __global__ void __launch_bounds__(kPlainThreads) grouped_plain_kernel(const PlainParams p) {
-  __shared__ uint16_t ta[kPlainTile][kPlainPitch], tb[kPlainTile][kPlainPitch];
+  __shared__ __align__(16) uint16_t ta[kPlainTile][kPlainPitch], tb[kPlainTile][kPlainPitch];   // read as 32-bit words
   __shared__ int64_t s_begin, s_end;
   __shared__ int s_expert;
   __shared__ int64_t s_lo, s_hi;

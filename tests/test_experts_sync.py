@@ -35,3 +35,11 @@ def test_a_kernel_that_gives_up_waits_for_its_copies():
     text = "\n".join(kernel_lines())
     for barrier, guard in (("full", r"\*abort && lane == 0 && leader"), ("tail", r"\*abort && lane == 0\)")):
         assert re.search(guard + r"[^}]*mbar_wait\(&c->" + barrier + r"\[[^}]*&ignore", text), barrier
+
+
+def test_shared_arrays_read_as_words_are_aligned():
+    """An array of 16-bit elements is only sure of 2 bytes: one that is read as wider words says its alignment."""
+    for name in ("grouped.cu", "train.cu"):
+        src = re.sub(r"//.*", "", (CSRC / name).read_text())
+        for line in re.findall(r"(?<!extern )__shared__[^;]*\buint(?:8|16)_t\b[^;]*;", src):
+            assert "__align__(16)" in line, line
