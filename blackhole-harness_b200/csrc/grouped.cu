@@ -776,6 +776,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       for (int32_t s = 0; ok && s < t.steps; ++s) {
         const bool last = s + 1 == t.steps;
         ok = warp_wait(&c->full[st], phase, abort, p.dev_err);
+        if (MODE >= kWgrad && ok && last && t.tail % 16 != 0) pair_acquire(&c->full[st], phase);   // both CTAs' zeroed rows
         const uint32_t a = smem_u32(ring + st * kStageBytes);
         const uint64_t da = MODE == kRowsK ? sw128_desc(a) : sw128_mn_desc(a, kChunkBytes);
         const int count = last && t.tail ? (t.tail + 15) / 16 : kSubs * kStepK / 16;   // products of 16
@@ -830,7 +831,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) pair_arrive_zeroed(peer_addr(&c->full[st], 0));
+      if (lane == 0) pair_arrive_release(peer_addr(&c->full[st], 0));
     }
   } else if (warp >= 4) {
     // -------------------------------------------------------------- results

@@ -42,12 +42,21 @@ __device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
 }
 // Arrivals on a barrier of either CTA.  A release at cluster scope makes the
 // hardware wait for all of this thread's memory operations (about 0.5 us in a loop
-// that loads), so none is used.  The relaxed forms publish no write of this thread:
-// byte counts of loads, accumulators read.  pair_arrive_zeroed follows writes to
-// this CTA's shared memory that only this SM's tensor core reads, and that
-// fence.proxy.async has already ordered before its reads.
-__device__ __forceinline__ void pair_arrive_zeroed(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+// that loads), so the loops use relaxed forms, which publish no write of this thread:
+// byte counts of loads, accumulators read.  pair_arrive_release publishes writes to
+// this CTA's shared memory (once a group: its zeroed rows) to the thread of either CTA
+// that waits and then calls pair_acquire; the writes themselves pass fence.proxy.async
+// first, as the pair's tensor cores read them.
+__device__ __forceinline__ void pair_arrive_release(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// After a wait for the phase of this parity: sees what was released to the barrier by either CTA.
+__device__ __forceinline__ void pair_acquire(uint64_t* bar, uint32_t parity) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
+      "r"(parity)
+      : "memory");
 }
 __device__ __forceinline__ void pair_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");

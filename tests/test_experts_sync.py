@@ -43,3 +43,14 @@ def test_shared_arrays_read_as_words_are_aligned():
         src = re.sub(r"//.*", "", (CSRC / name).read_text())
         for line in re.findall(r"(?<!extern )__shared__[^;]*\buint(?:8|16)_t\b[^;]*;", src):
             assert "__align__(16)" in line, line
+
+
+def test_zeroed_rows_are_published_to_the_pair():
+    """The rows that one CTA clears are read by a product that the other issues: released and acquired at the
+    scope of both."""
+    text = "\n".join(kernel_lines())
+    helper = (CSRC / "pair.cuh").read_text()
+    assert "mbarrier.arrive.release.cluster" in helper.split("void pair_arrive_release(")[1][:200]
+    assert ".acquire.cluster" in helper.split("void pair_acquire(")[1][:250]
+    assert re.search(r"fence_proxy_async_smem\(\);\s*__syncwarp\(\);\s*if \(lane == 0\) pair_arrive_release", text)
+    assert re.search(r"warp_wait\(&c->full\[st\][^;]*;\s*if \(MODE >= kWgrad && ok && last && t.tail % 16 != 0\) pair_acquire", text)
