@@ -141,16 +141,24 @@ struct SwigluParams {
   int32_t inter;
 };
 
-// s and silu(g).  16-bit types round the result to 2^-9 or 2^-12: the fast
-// exponential and reciprocal (about 2^-21) vanish in that.  f32 uses expf and
-// the rounded divide.
+// s, 1 - s and silu(g), from e = exp(-|g|): with 1 + e in 1..2 neither end of the range overflows (1 / (1 + e^-g)
+// is zero from g = -88.7 on, from -87.3 with the fast divide, where silu is still a normal value down to -91).
+// 16-bit types round the result to 2^-9 or 2^-12: the fast exponential (2 + 1.173 |g| units of 2^-23: 2^-16 at |g|
+// = 88) and divide (2 units) vanish in that.  f32 uses expf and the rounded divide.  Below g = -87.3 e is no
+// normal value and has an error of up to 2^-150 instead.
 template <typename T>
-__device__ __forceinline__ void sigmoid_silu(float g, float& s, float& silu) {
+__device__ __forceinline__ void sigmoid_silu(float g, float& s, float& rest, float& silu) {
+  float e, r;
   if constexpr (std::is_same_v<T, float>) {
-    s = 1.f / (1.f + expf(-g));
+    e = expf(-fabsf(g));
+    r = 1.f / (1.f + e);
   } else {
-    s = __fdividef(1.f, 1.f + __expf(-g));
+    e = __expf(-fabsf(g));
+    r = __fdividef(1.f, 1.f + e);
   }
+  const float er = e * r;
+  s = g < 0.f ? er : r;
+  rest = g < 0.f ? r : er;
   silu = g * s;
 }
 
@@ -192,12 +200,12 @@ __global__ void __launch_bounds__(kSwigluThreads) swiglu_kernel(const SwigluPara
         if constexpr (BWD) VecT::unpack(d[i], df);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          float s, silu;
-          sigmoid_silu<T>(gf[j], s, silu);
+          float s, rest, silu;
+          sigmoid_silu<T>(gf[j], s, rest, silu);
           if constexpr (BWD) {
             sum += df[j] * silu * uf[j];
             const float dw = df[j] * w;
-            a[j] = dw * uf[j] * (s + silu * (1.f - s));
+            a[j] = dw * uf[j] * (s + silu * rest);
             b[j] = dw * silu;
           } else {
             a[j] = silu * w * uf[j];   // a weight of zero comes before the product that may overflow
