@@ -63,3 +63,18 @@ def test_swiglu_of_infinite_and_undefined_gates(dtype):
     h = torch.cat([gate, torch.full((4,), 2.0)])[None].to(dtype)
     act = experts.swiglu(h.to(DEV))[0].float().cpu()
     assert act[0] == math.inf and act[2].isnan() and act[3].isfinite() and not act[1].abs() > 0   # 0 or, as inf / inf, NaN
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+def test_swiglu_of_tiny_gates(dtype):
+    """silu(g) is g / 2 near zero, down to the type's smallest values."""
+    tiny = torch.tensor([2.0 ** -e for e in (list(range(10, 150, 7)) if dtype != F16 else list(range(5, 25)))])
+    gate = torch.cat([tiny, -tiny]).to(dtype)
+    h = torch.cat([gate, torch.ones_like(gate)])[None]
+    want = swiglu_reference(h, None)
+    got = experts.swiglu(h.to(DEV)).double().cpu()
+    assert ((got - want).abs() <= (32 * 2.0 ** -23 + 1.01 * ROUND[dtype]) * want.abs() + HALF_STEP[dtype] + 2.0 ** -149).all()
+    dh, _ = experts.swiglu_backward(torch.ones(1, len(gate), dtype=dtype, device=DEV), h.to(DEV))
+    want = swiglu_reference(h, None, torch.ones(1, len(gate), dtype=dtype))[0]
+    assert ((dh.double().cpu() - want).abs() <= (32 * 2.0 ** -23 + 1.01 * ROUND[dtype]) * want.abs() + HALF_STEP[dtype] + 2.0 ** -149).all()
