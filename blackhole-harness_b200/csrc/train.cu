@@ -129,7 +129,11 @@ cudaLaunchConfig_t launch_config(dim3 grid, int threads, cudaStream_t st, cudaLa
 // loads per operand in flight.  32768 x 768 bf16 with weights: forward 24.2 us (6.24
 // TB/s), backward 41.0 us (6.15 TB/s).
 constexpr int kSwigluThreads = 256;
-constexpr int kUnroll = 3;   // three 16-byte pieces a lane cover 768 16-bit values a warp
+// 16-byte pieces a lane has in flight: three cover 768 16-bit values a warp.  With 1, 2, 3, 4 (bf16, forward and
+// backward, us): 32768 x 768: 23.5 + 38.8, 25.5 + 41.9, 24.6 + 41.5, 26.4 + 43.0; 32768 x 96: 8.0 + 12.8, 4.9 + 7.2, 4.6
+// + 6.9, 4.5 + 7.5; 8191 x 517 (by element): 11.2 + 16.8, 9.1 + 14.2, 8.8 + 12.2, 7.7 + 12.6; f32 32768 x 768: 46.8 + 77.7,
+// 45.6 + 76.0, 45.6 + 75.4, 48.3 + 75.4.
+constexpr int kUnroll = 3;
 
 struct SwigluParams {
   const void* h;        // [rows, 2 * inter]
@@ -246,6 +250,16 @@ cudaError_t launch_swiglu_one(const SwigluParams& p, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, swiglu_kernel<T, V, TPR, BWD>, p);
 }
 
+// The threads of a row: as few as cover it with kUnroll pieces each, a block's half for wide rows unless there are
+// enough rows that a warp each fills the machine.  bf16, forward and backward, us, with 4, 8, 32, 128 threads a row:
+//   32768 x 64     3.2 + 5.3    3.2 + 5.8    8.2 + 16.4   17 + 54     (4 taken)
+//   32768 x 96     4.6 + 6.9    5.1 + 8.0    9.3 + 17.0   18 + 56     (4)
+//   65536 x 200   15.9 + 27.5  14.5 + 26.4  19.9 + 41.0   40 + 133    (32: one piece past the 24 of 8 threads)
+//   512 x 768      9.7 + 12.6   5.4 + 7.0    2.2 + 2.6    1.8 + 2.2   (32)
+//   512 x 4096      53 + 67      27 + 36     7.7 + 10.7   3.6 + 5.3   (128)
+//   4096 x 4096     67 + 84      36 + 47    18.3 + 34.6  18.4 + 30.9  (128)
+//   8192 x 4096     73 + 93      47 + 64    37.0 + 58.3  34.2 + 57.3  (32)
+//   16384 x 1536    36 + 50      27 + 52    24.8 + 40.5  30.3 + 54.7  (32)
 template <typename T, int V, bool BWD>
 cudaError_t launch_swiglu_vec(const SwigluParams& p, cudaStream_t st) {
   const int n = p.inter / V;
