@@ -71,6 +71,16 @@ __device__ __forceinline__ GroupScan scan_groups(const Groups& g, int base, int6
   return s;
 }
 
+// The tensor core's fp32 sums cut where an fp32 addition rounds, once for every 16 products: the error grows with the
+// length of a sum, always towards zero.  Results in fp32 therefore take no more than kRunLength products from one
+// accumulator and add the runs in fp32.  x^T x of 500, 2000, 8000, 60000 rows, relative to its diagonal: 1e-6, 6e-6, 5e-6,
+// 5e-6 (in one accumulator 1e-6, 6e-6, 2.7e-5, 3.3e-4; a plain fp32 product 3e-7, 1e-6, 1e-6, 4e-6 or, values of one
+// sign, 1.3e-5).  What it costs is the additions, which L2 takes at 2.5 TB/s: f32 gradient of 8 x 8192 rows, 2048 x 2048:
+// 419 us against 374, 60000 rows 393 against 339 (446 with runs of 1024); rows of 8192 to f32, 4 x 2048 x 1536: 174
+// against 154.  16-bit results are rounded to 2^-9 or 2^-12 at the end and keep one accumulator: 5e-6 at 2000 products,
+// 2.7e-5 at 8000.
+constexpr int kRunLength = 2048;
+
 // ---------------------------------------------------------------- plain kernel
 // out(i, j) = sum_r A(i, r) B(j, r) over operands with any element strides:
 // 64 x 64 tiles, mma.sync over 32-wide reduction steps staged in shared memory
@@ -237,7 +247,18 @@ __global__ void __launch_bounds__(kPlainThreads) grouped_plain_kernel(const Plai
   const int64_t i_left = WGRAD ? p.i_len - i0 : end - begin, j_left = p.j_len - j0;
   const int64_t reds = WGRAD ? end - begin : p.r_len;
   const int wi = warp / 2 * 32, wj = warp % 2 * 32, g = lane / 4, q = lane % 4;
-  float acc[2][4][4] = {};
+  float acc[2][4][4] = {}, sum[2][4][4] = {};
+  auto flush = [&] {
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < 4; ++n)
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          sum[m][n][h] += acc[m][n][h];
+          acc[m][n][h] = 0.f;
+        }
+  };
   uint16_t va[16], vb[16];
   plain_fetch(va, a, p.a_i, p.a_r, i_left, reds);
   plain_fetch(vb, b, p.b_j, p.b_r, j_left, reds);
@@ -266,7 +287,9 @@ __global__ void __launch_bounds__(kPlainThreads) grouped_plain_kernel(const Plai
         for (int m = 0; m < 2; ++m) mma_16816(acc[m][n], fa[m], b0, b1, p.bf16);
       }
     }
+    if (r / kPlainK % (kRunLength / kPlainK) == kRunLength / kPlainK - 1) flush();
   }
+  flush();
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -276,7 +299,7 @@ __global__ void __launch_bounds__(kPlainThreads) grouped_plain_kernel(const Plai
         const int i = wi + m * 16 + g + (h >> 1) * 8, j = wj + n * 8 + q * 2 + (h & 1);
         if (i >= i_left || j >= j_left) continue;
         const int64_t at = WGRAD ? e * p.out_e + (i0 + i) * p.out_i + j0 + j : (begin + i) * p.out_i + j0 + j;
-        float v = acc[m][n][h];
+        float v = sum[m][n][h];
         if (p.out_f32) {
           float* o = static_cast<float*>(p.out) + at;
           *o = p.accumulate ? *o + v : v;
@@ -381,7 +404,8 @@ struct PairParams {
   int32_t n_len;             // weight gradient: k, or n in kWgradT
   int32_t red;               // row products: reduction length
   int32_t m_tiles, n_tiles, tile_n;   // n_tiles, tile_n: weight gradient
-  int32_t splits;            // runs that the reduction of a tile is cut into
+  int32_t splits;            // runs that the reduction of a tile is cut into, over several pairs
+  int32_t run;               // RUNS: most steps that one accumulator sums
   void* dst;                 // splits > 1: fp32 partials, one result a run
   int64_t ld, stride_e, stride_split;
   int32_t f32, bf16, accumulate, tma_out;
@@ -396,17 +420,44 @@ struct Tile {
   int32_t e, m0, n0, width, parts, first, steps, tail, split;
   int64_t row0;
   int32_t valid;
+  bool add;   // to what the runs before it have written
   // The columns of accumulator i: what is left of the tile, in whole 32s (341 rows: 192 and 160).
   __device__ __forceinline__ int32_t columns(int i) const { return min(width, (valid - i * width + 31) / 32 * 32); }
 };
 
-template <int MODE, int SHAPE>
+// RUNS: f32 results whose reduction may pass kRunLength.  Kernels without it are 4 % faster (16-bit gradient of 96 x
+// 1536 x 2048, 341 rows: 248 us against 260 with the runs looked for).
+template <int MODE, int SHAPE, bool RUNS>
 struct Walker {
   int32_t base = -32;
   int64_t carry = 0, lo = 0;
   int32_t upto = 0, mine = 0, total = 0;
   int64_t begin = 0, end = 0;
   bool bad = false;
+  int32_t left = 0, per = 0, end_tail = 0;   // of the tile's steps: to come, in a run, and its last one
+
+  // The next run of a tile's reduction: all of it, or with RUNS pieces of at most p.run steps one after the other.
+  __device__ __forceinline__ bool next(const PairParams& p, int32_t& unit, int32_t stride, Tile& t) {
+    if (!RUNS || left == 0) {
+      if (!find(p, unit, t)) return false;
+      unit += stride;
+      if constexpr (!RUNS) return true;
+      t.add = false;
+      per = left = t.steps;
+      end_tail = t.tail;
+      if (left > p.run) {
+        const int32_t runs = (left + p.run - 1) / p.run;
+        per = (left + runs - 1) / runs;
+      }
+    } else {
+      t.first += t.steps;
+      t.add = true;
+    }
+    t.steps = min(per, left);
+    left -= t.steps;
+    t.tail = left ? 0 : end_tail;
+    return true;
+  }
 
   __device__ __forceinline__ bool find(const PairParams& p, int32_t unit, Tile& t) {
     constexpr int32_t kSpan = span_of(SHAPE);
@@ -470,22 +521,30 @@ struct Walker {
 };
 
 // Writes 32 x 32 pieces of an accumulator: one writer warp's M rows by 32 columns.
-template <int MODE>
+template <int MODE, bool RUNS>
 struct Writer {
   const PairParams& p;
   uint8_t* stage;    // 32 lines of 64 B (their 16-byte pieces permuted as SWIZZLE_64B), or 16 plain ones of 128 B
   int lane;
   int32_t e = 0, m = 0, cols = 0;   // which result (expert, run of the reduction); first M row; columns there are
+  bool add = false;                 // to what is there
   int64_t n0 = 0;                   // column 0 in the output: row products: its row; weight gradient: its column
 
+  // An f32 result, or its addition without waiting for what is there.  Each value has one writer, whose additions
+  // to an address keep their order.
+  __device__ __forceinline__ void put(float* dst, float v) const {
+    if (add) atomicAdd(dst, v);
+    else *dst = v;
+  }
   // The staging tile is free once the store before has read it.
   __device__ __forceinline__ void stage_free() const {
     if (elect_one()) bulk_wait_read();
     __syncwarp();
   }
+  __device__ __forceinline__ bool f32() const { return RUNS || p.f32; }
   // Row products that leave by TMA take fragments, everything else a row of 32 columns a lane.
   __device__ __forceinline__ void load(uint32_t acc, uint32_t (&r)[32]) const {
-    if (MODE != kWgrad && p.tma_out && (MODE < kWgrad || !p.f32)) {
+    if (MODE != kWgrad && p.tma_out && (MODE < kWgrad || !f32())) {
       tmem_ld_fragments<0>(acc, r);
       tmem_ld_fragments<16>(acc + (16u << 16), r);
     } else {
@@ -494,7 +553,7 @@ struct Writer {
   }
   __device__ __forceinline__ void write(int32_t col, uint32_t (&r)[32]) {
     if constexpr (MODE == kWgrad) write_gradient(col, r);
-    else if (MODE == kWgradT && p.tma_out && p.f32) write_lines(col, r);
+    else if (MODE == kWgradT && p.tma_out && f32()) write_lines(col, r);
     else if (p.tma_out) write_rows(col, r);
     else write_elements(col, r);
   }
@@ -545,7 +604,7 @@ struct Writer {
       __syncwarp();
       if (elect_one()) {
         const int32_t y = static_cast<int32_t>(n0) + col + 16 * h;
-        if (p.accumulate) tma_add_3d(&p.out, stage, m, y, e);
+        if (add) tma_add_3d(&p.out, stage, m, y, e);
         else tma_store_3d(&p.out, stage, m, y, e);
         bulk_commit();
       }
@@ -557,12 +616,11 @@ struct Writer {
   __device__ __forceinline__ void write_elements(int32_t col, uint32_t (&r)[32]) const {
     const int32_t rows = m + lane < p.m_len ? min(32, cols - col) : 0;
     const int64_t at = e * (MODE == kWgradT ? p.stride_e : p.stride_split) + (n0 + col) * p.ld + m + lane;
-    const bool add = MODE == kWgradT && p.accumulate;
-    if (p.f32) {
+    if (f32()) {
       float* dst = static_cast<float*>(p.dst) + at;
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (j < rows) dst[j * p.ld] = __uint_as_float(r[j]) + (add ? dst[j * p.ld] : 0.f);
+        if (j < rows) put(dst + j * p.ld, __uint_as_float(r[j]));
     } else {
       uint16_t* dst = static_cast<uint16_t*>(p.dst) + at;
       if (add) {
@@ -582,10 +640,10 @@ struct Writer {
   // which cuts them at the matrix's edges; by element where TMA cannot.
   __device__ __forceinline__ void write_gradient(int32_t col, uint32_t (&r)[32]) {
     if (p.tma_out) {
-      if (!p.f32) pack_pairs(r, p.bf16);
+      if (!f32()) pack_pairs(r, p.bf16);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {   // 16 words a line: 32 columns of 16 bits, or 16 of f32 twice
-        if (h == 1 && !p.f32) break;
+        if (h == 1 && !f32()) break;
         stage_free();
 #pragma unroll
         for (int q = 0; q < 4; ++q)
@@ -595,7 +653,7 @@ struct Writer {
         __syncwarp();
         if (elect_one()) {
           const int32_t x = static_cast<int32_t>(n0) + col + 16 * h;
-          if (p.accumulate) tma_add_3d(&p.out, stage, x, m, e);
+          if (add) tma_add_3d(&p.out, stage, x, m, e);
           else tma_store_3d(&p.out, stage, x, m, e);
           bulk_commit();
         }
@@ -604,14 +662,14 @@ struct Writer {
     }
     const int64_t at = e * p.stride_e + (m + lane) * p.ld + n0 + col;
     const int32_t count = m + lane < p.m_len ? min(32, cols - col) : 0;
-    if (p.f32) {
+    if (f32()) {
       float* dst = static_cast<float*>(p.dst) + at;
 #pragma unroll
       for (int j = 0; j < 32; ++j)
-        if (j < count) dst[j] = __uint_as_float(r[j]) + (p.accumulate ? dst[j] : 0.f);
+        if (j < count) put(dst + j, __uint_as_float(r[j]));
     } else {
       uint16_t* dst = static_cast<uint16_t*>(p.dst) + at;
-      if (p.accumulate) {
+      if (add) {
 #pragma unroll
         for (int j = 0; j < 32; ++j)
           if (j < count) r[j] = __float_as_uint(__uint_as_float(r[j]) + widen16(dst[j], p.bf16));
@@ -632,7 +690,7 @@ struct PairCtrl {
   int abort;
 };
 
-template <int MODE, int SHAPE>
+template <int MODE, int SHAPE, bool RUNS>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     grouped_pair_kernel(const __grid_constant__ PairParams p) {
   constexpr bool WIDE = SHAPE == kTwo;
@@ -677,14 +735,14 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   pdl_launch_dependents();   // one wave: whoever waits for this grid may take its place on the SMs as they fall free
 
   const int32_t first = blockIdx.x / 2, stride = gridDim.x / 2;
-  Walker<MODE, SHAPE> walk;
+  Walker<MODE, SHAPE, RUNS> walk;
   Tile t;
   if (warp == 0) {
     // ---------------------------------------------------------------- loads
     uint32_t it = 0, st = 0, phase = 1;
     uint32_t tails = 0, tail_odd = 0;   // a bit a stage: whether it has held a tail, whether an odd number of them
     bool ok = true;
-    for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
+    for (int32_t tile = first; ok && walk.next(p, tile, stride, t);) {
       const int32_t halves[2] = {t.columns(0) / 2, WIDE && t.parts > 1 ? t.columns(1) / 2 : 0};
       const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128;
       const uint32_t bytes =
@@ -768,7 +826,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     // ------------------------------------------------------------- products
     uint32_t n = 0, st = 0, phase = 0;
     bool ok = true;
-    for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
+    for (int32_t tile = first; ok && walk.next(p, tile, stride, t);) {
       if (t.steps == 0) continue;   // an empty group's gradient: zeros, without an accumulator
       constexpr uint32_t kMajors = (MODE != kRowsK ? kIdescMajorA : 0) | (MODE >= kWgrad ? kIdescMajorB : 0);
       const uint32_t idescs[2] = {umma_idesc(p.bf16, 256, t.columns(0)) | kMajors,
@@ -814,7 +872,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     uint32_t it = 0;
     int uses = 0;   // lane s: how many tails stage s has held
     bool ok = true;
-    for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
+    for (int32_t tile = first; ok && walk.next(p, tile, stride, t);) {
       it += t.steps;
       if (t.tail % 16 == 0) continue;
       const uint32_t st = (it - 1) % kStages;
@@ -836,12 +894,17 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   } else if (warp >= 4) {
     // -------------------------------------------------------------- results
     const int quad = warp % 4, part = (warp - 4) / 4;   // 32 of the CTA's M rows, every other 32 columns
-    Writer<MODE> out{p, staging + (warp - 4) * kStoreBytes, lane};
+    Writer<MODE, RUNS> out{p, staging + (warp - 4) * kStoreBytes, lane};
     uint32_t n = 0;
     bool ok = true;
-    for (int32_t tile = first; ok && walk.find(p, tile, t); tile += stride) {
+    for (int32_t tile = first; ok && walk.next(p, tile, stride, t);) {
       out.e = MODE >= kWgrad ? t.split * p.g.experts + t.e : t.split;
       out.m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
+      out.add = p.accumulate || (RUNS && t.add);
+      if (RUNS && t.add && p.tma_out) {   // the stores of the run before have arrived: additions to the same values stay in order
+        if (elect_one()) bulk_wait_all();
+        __syncwarp();
+      }
       for (int acc_n = 0; acc_n < (WIDE ? t.parts : 1); ++acc_n) {
         const int32_t cols = MODE >= kWgrad ? min(t.width, p.n_len - t.n0) : min(t.width, t.valid - acc_n * t.width);
         const int chunks = out.m < p.m_len && cols > part * 32 ? (cols - part * 32 + 63) / 64 : 0;
@@ -940,6 +1003,10 @@ bool tma_stack(const void* p, int64_t ld, int64_t stride, int64_t size, int32_t 
          (count == 1 || (stride * size % 16 == 0 && stride >= ld && stride * size < (1ll << 40)));
 }
 
+#define PAIR_KERNELS(MODE, SHAPE)                                             \
+  reinterpret_cast<const void*>(grouped_pair_kernel<MODE, SHAPE, false>), \
+      reinterpret_cast<const void*>(grouped_pair_kernel<MODE, SHAPE, true>)
+
 int sm_count(int* sms) {
   static std::atomic<int> cached[64] = {};
   int dev = 0;
@@ -948,18 +1015,10 @@ int sm_count(int* sms) {
   if (dev < 0 || dev >= 64) return report_error(HEXMOE_E_DEVICE, "device ordinal out of range");
   int v = cached[dev].load(std::memory_order_acquire);
   if (!v) {   // first call on this device: the kernels' shared memory as well
-    for (const void* k : {reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kOne>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kTwo>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kNarrow>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsK, kMiddle>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kMiddle>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kOne>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kTwo>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kRowsMN, kNarrow>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, kOne>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgrad, kMiddle>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgradT, kOne>),
-                          reinterpret_cast<const void*>(grouped_pair_kernel<kWgradT, kMiddle>)}) {
+    for (const void* k : {PAIR_KERNELS(kRowsK, kOne), PAIR_KERNELS(kRowsK, kTwo), PAIR_KERNELS(kRowsK, kNarrow),
+                          PAIR_KERNELS(kRowsK, kMiddle), PAIR_KERNELS(kRowsMN, kOne), PAIR_KERNELS(kRowsMN, kTwo),
+                          PAIR_KERNELS(kRowsMN, kNarrow), PAIR_KERNELS(kRowsMN, kMiddle), PAIR_KERNELS(kWgrad, kOne),
+                          PAIR_KERNELS(kWgrad, kMiddle), PAIR_KERNELS(kWgradT, kOne), PAIR_KERNELS(kWgradT, kMiddle)}) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
       if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
     }
@@ -983,7 +1042,8 @@ cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, SHAPE>, p);
+  return p.run ? cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, SHAPE, true>, p)
+               : cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, SHAPE, false>, p);
 }
 
 // ------------------------------------------------------------------- splits
@@ -1223,6 +1283,7 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
     q.f32 = split || f32; q.bf16 = bf16;
     q.dev_err = dev_err;
     const PairShape shape = rows_shape(rows, experts, width_out);
+    q.run = f32 && width_in > kRunLength ? kRunLength / (kStepK * subs_of(shape)) : 0;
     const int64_t tiles = row_tiles(rows, experts, width_out, shape) * q.splits;
     if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
@@ -1310,6 +1371,7 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
     q.ld = split ? pitch : ld_out;
     q.stride_e = split ? n * pitch : stride_out;
     q.f32 = split || f32; q.bf16 = bf16; q.accumulate = accumulate && !split;
+    q.run = f32 && rows > kRunLength ? kRunLength / (kStepK * subs_of(shape)) : 0;
     q.dev_err = dev_err;
     const int64_t tiles = wgrad_tiles(experts, q.m_len, q.n_len, shape) * q.splits;
     if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);

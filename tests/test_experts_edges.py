@@ -8,7 +8,7 @@ import math
 import numpy as np
 import pytest
 import torch
-from test_experts import (BF16, DEV, F16, F32, ROUND, assert_sum, device_word, normal, offsets_of,  # noqa: F401
+from test_experts import (BF16, DEV, F16, F32, ROUND, assert_sum, device_word, mm_reference, normal, offsets_of,  # noqa: F401
                           swiglu_reference, wgrad_reference)
 
 from blackhole_b200 import experts
@@ -78,3 +78,94 @@ def test_swiglu_of_tiny_gates(dtype):
     dh, _ = experts.swiglu_backward(torch.ones(1, len(gate), dtype=dtype, device=DEV), h.to(DEV))
     want = swiglu_reference(h, None, torch.ones(1, len(gate), dtype=dtype))[0]
     assert ((dh.double().cpu() - want).abs() <= (32 * 2.0 ** -23 + 1.01 * ROUND[dtype]) * want.abs() + HALF_STEP[dtype] + 2.0 ** -149).all()
+
+
+# ------------------------------------------------------------------ long sums
+RUN = 2048   # the most products that one accumulator of an f32 result sums (16 at a time)
+
+
+def run_bound(terms):
+    """Of a sum of `terms` positive products of even size, relative.  One addition of 16 products is off by at most a unit
+    in the last place (2^-23) of a sum that has grown to half on average; the runs are added in f32 (2^-24 each, on half
+    the sum on average); some units for the ends."""
+    return (min(terms, RUN) / 16 / 2 + 8) * 2.0 ** -23 + (terms / RUN / 2 + 1) * 2.0 ** -24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hessian", [False, True])
+@pytest.mark.parametrize("rows", [500, 8000, 60_000])
+@pytest.mark.parametrize("E,n,k", [(1, 72, 136), (40, 256, 512), (90, 72, 264), (2, 9, 11)])
+def test_f32_gradients_do_not_lose_bits_with_length(E, n, k, rows, hessian):
+    """The error of a sum of one sign stays below what a lost row would take from it, however long the group: tiles alone
+    and shared, x on either side, by TMA and by element."""
+    if hessian:
+        n = k
+    sizes = [rows] + [17] * (E - 1)
+    g = torch.Generator(device=DEV).manual_seed(83)
+    draw = lambda width: (1 + torch.rand(sum(sizes), width, generator=g, device=DEV) / 4).to(BF16)  # noqa: E731
+    x = draw(k)
+    dy = x if hessian else draw(n)
+    off = offsets_of(sizes).to(DEV)
+    assert run_bound(rows) < 0.7 / rows
+    want = dy[:rows].double().t() @ x[:rows].double()
+    out = experts.grouped_wgrad(dy, x, off, out_dtype=F32)
+    assert float(((out[0].double() - want).abs() / want).max()) <= run_bound(rows)
+    base = torch.full_like(out, 1000.0)
+    experts.grouped_wgrad(dy, x, off, out=base, accumulate=True)
+    assert float(((base[0].double() - want - 1000).abs() / (want + 1000)).max()) <= run_bound(rows) + 2.0 ** -23
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("rows", [3, 100, 700, 40_000])
+@pytest.mark.parametrize("width", [2048, 32768, 32766])
+def test_f32_row_products_do_not_lose_bits_with_width(rows, width, transpose):
+    """The same along the reduction of the row products."""
+    out_width = 72
+    g = torch.Generator(device=DEV).manual_seed(84)
+    draw = lambda *shape: (1 + torch.rand(*shape, generator=g, device=DEV) / 4).to(BF16)  # noqa: E731
+    x, w = draw(rows, width), draw(2, *((width, out_width) if transpose else (out_width, width)))
+    off = offsets_of([rows // 2, rows - rows // 2]).to(DEV)
+    got = experts.grouped_mm(x, w, off, transpose=transpose, out_dtype=F32)
+    for e, (a, b) in enumerate([(0, rows // 2), (rows // 2, rows)]):
+        want = x[a:b].double() @ (w[e].double() if transpose else w[e].double().t())
+        assert not len(want) or float(((got[a:b].double() - want).abs() / want).max()) <= run_bound(width)
+
+
+# whole numbers: every sum is exact in f32, so a row that is lost or taken twice shows whatever the length
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("n,k", [(72, 130), (264, 520), (88, 1336)])
+@pytest.mark.parametrize("sizes", [[5000], [4000, 0, 3], [2111, 2050], [1, 15, 16, 17, 63, 64, 65, 2047, 2048, 2049, 2064, 4097],
+                                   [33] * 70], ids=lambda s: f"{len(s)} groups of {s[0]}")
+def test_whole_numbers_keep_every_row(sizes, n, k, out_dtype):
+    g = torch.Generator().manual_seed(85)
+    first, rows = 3, sum(sizes) + 70
+    dy, x = (torch.randint(-3, 4, (rows, w), generator=g).float() for w in (n, k))
+    dy[:first], x[:first] = math.nan, math.inf      # what no group holds
+    dy[first + sum(sizes):], x[first + sum(sizes):] = math.inf, math.nan
+    off = offsets_of(sizes, first)
+    want, _ = wgrad_reference(dy, x, off)
+    assert want.abs().max() < 2 ** 24
+    dyd, xd, offd = dy.to(BF16).to(DEV), x.to(BF16).to(DEV), off.to(DEV)
+    got = experts.grouped_wgrad(dyd, xd, offd, out_dtype=out_dtype)
+    assert torch.equal(got.cpu(), want.to(out_dtype))
+    base = torch.randint(-100, 101, want.shape, generator=g).to(out_dtype)
+    out = experts.grouped_wgrad(dyd, xd, offd, out=base.to(DEV), accumulate=True)
+    assert torch.equal(out.cpu(), (want + base.double()).to(out_dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("transpose", [False, True])
+@pytest.mark.parametrize("out_dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("n,k", [(200, 2056), (2056, 200), (1000, 3004)])
+@pytest.mark.parametrize("sizes", [[1], [70, 0, 1], [300, 257, 512, 2]], ids=str)
+def test_whole_numbers_keep_every_column(sizes, n, k, out_dtype, transpose):
+    g = torch.Generator().manual_seed(86)
+    rows = sum(sizes)
+    x = torch.randint(-3, 4, (rows, n if transpose else k), generator=g).float()
+    w = torch.randint(-3, 4, (len(sizes), n, k), generator=g).float()
+    off = offsets_of(sizes)
+    want, _ = mm_reference(x, w, off, transpose, rows)
+    got = experts.grouped_mm(x.to(BF16).to(DEV), w.to(BF16).to(DEV), off.to(DEV), transpose=transpose, out_dtype=out_dtype)
+    assert torch.equal(got.cpu(), want.to(out_dtype))
