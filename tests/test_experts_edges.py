@@ -8,7 +8,7 @@ import math
 import numpy as np
 import pytest
 import torch
-from test_experts import (BF16, DEV, F16, F32, ROUND, assert_sum, device_word, mm_reference, normal, offsets_of,  # noqa: F401
+from test_experts import (BF16, DEV, F16, F32, ROUND, assert_sum, device_word, mm_reference, normal, offsets_of, padded,  # noqa: F401
                           swiglu_reference, wgrad_reference)
 
 from blackhole_b200 import experts
@@ -169,3 +169,34 @@ def test_whole_numbers_keep_every_column(sizes, n, k, out_dtype, transpose):
     want, _ = mm_reference(x, w, off, transpose, rows)
     got = experts.grouped_mm(x.to(BF16).to(DEV), w.to(BF16).to(DEV), off.to(DEV), transpose=transpose, out_dtype=out_dtype)
     assert torch.equal(got.cpu(), want.to(out_dtype))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("E,rows,n,k", [(2, 70, 129, 67), (12, 700, 301, 355), (40, 1500, 77, 499), (1, 5000, 97, 131)])
+def test_gradients_are_added_to_odd_rows(E, rows, n, k, out_dtype):
+    """What stands in rows whose width is no multiple of 16 bytes is added to, exactly (whole numbers), and nothing beside."""
+    g = torch.Generator().manual_seed(87)
+    sizes = np.bincount(np.random.RandomState(E).randint(0, E, rows), minlength=E)
+    dy, x = (torch.randint(-3, 4, (rows, w), generator=g).to(BF16) for w in (n, k))
+    off = offsets_of(sizes)
+    base = torch.randint(-100, 101, (E, n, k), generator=g).to(out_dtype)
+    want = (wgrad_reference(dy, x, off)[0] + base.double()).to(out_dtype)
+    buf, out = padded(base, 5.0)
+    ins = padded(dy, math.nan)[1], padded(x, math.nan)[1]
+    experts.grouped_wgrad(*ins, off.to(DEV), out=out, accumulate=True)
+    assert torch.equal(out.cpu(), want) and (buf[..., k:] == 5).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("off", [[0, 20, 10, 32], [0, 8, 16, 40], [-4, 8, 16, 32], [0, 2 ** 40, 7, 9]], ids=str)
+def test_gradients_of_offsets_that_do_not_fit(off):
+    """The gradient of offsets that are clamped is that of the clamped ones."""
+    from blackhole_b200.hex_moe import device_status
+    x, off = normal((32, 64), BF16, 88).to(DEV), torch.tensor(off)
+    got = experts.grouped_wgrad(x, x, off.to(DEV), out_dtype=F32)
+    assert device_status(0) == 8
+    fixed = torch.cummax(off.clamp(0, 32), 0).values
+    assert torch.equal(got, experts.grouped_wgrad(x, x, fixed.to(DEV), out_dtype=F32))
+    want, mass = wgrad_reference(x.cpu(), x.cpu(), fixed)
+    assert_sum(got, want, mass, 32, F32)
