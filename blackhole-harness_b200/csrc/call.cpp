@@ -8,8 +8,9 @@
 // arguments, allocates what the call needs, makes it on the current stream and
 // returns the result; or it returns None, having done nothing, where anything is
 // out of the ordinary (another device than the current one, a stride that wants a
-// copy, a type or shape that does not fit, an error of the call), and experts.py
-// takes the call from there, with its checks and messages.
+// copy, a type or shape that does not fit, arguments that the call refuses), and
+// experts.py takes the call from there, with its checks and messages.  A call that
+// failed on the way, with some of its work perhaps done, raises.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -21,6 +22,8 @@
 #include <cmath>
 #include <exception>
 #include <optional>
+#include <stdexcept>
+#include <string>
 #include <vector>
 
 #include "hexmoe.h"
@@ -56,7 +59,15 @@ at::Tensor workspace(size_t bytes, const at::Tensor& like) {
   return at::empty({static_cast<int64_t>(bytes)}, like.options().dtype(at::kByte));
 }
 
-// C++ exceptions (an allocation that fails) become Python's.
+// Whether a call refused its arguments, before any work.  Any other failure may have come after a launch: made once
+// more, the call could scale what it has scaled already.
+bool refused(int rc, const char* what) {
+  if (rc == HEXMOE_OK) return false;
+  if (rc == HEXMOE_E_ARG || rc == HEXMOE_E_DTYPE) return true;
+  throw std::runtime_error(std::string(what) + ": " + hexmoe_last_error());
+}
+
+// C++ exceptions (an allocation or a launch that fails) become Python's.
 template <typename F>
 PyObject* guarded(F&& f) {
   try {
@@ -87,10 +98,10 @@ PyObject* grouped_mm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const size_t bytes = hexmoe_grouped_mm_workspace_bytes(R, E, N, K, transpose);
     at::Tensor ws;
     if (bytes) ws = workspace(bytes, *x);
-    if (hexmoe_grouped_mm(x->data_ptr(), x->stride(0), w->data_ptr(), w->stride(1), w->stride(0), code, R, E, N, K,
-                          transpose, off->data_ptr(), index, out.data_ptr(), width, code, bytes ? ws.data_ptr() : nullptr,
-                          bytes, stream_of(*x)))
-      Py_RETURN_NONE;
+    const int rc = hexmoe_grouped_mm(x->data_ptr(), x->stride(0), w->data_ptr(), w->stride(1), w->stride(0), code, R,
+                                     E, N, K, transpose, off->data_ptr(), index, out.data_ptr(), width, code,
+                                     bytes ? ws.data_ptr() : nullptr, bytes, stream_of(*x));
+    if (refused(rc, "hexmoe_grouped_mm")) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
   });
 }
@@ -112,10 +123,10 @@ PyObject* grouped_wgrad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const size_t bytes = hexmoe_grouped_wgrad_workspace_bytes(R, E, N, K);
     at::Tensor ws;
     if (bytes) ws = workspace(bytes, *x);
-    if (hexmoe_grouped_wgrad(dy->data_ptr(), dy->stride(0), x->data_ptr(), x->stride(0), code, R, E, N, K, off->data_ptr(),
-                             index, out.data_ptr(), K, N * K, f32 ? HEXMOE_F32 : code, 0, bytes ? ws.data_ptr() : nullptr,
-                             bytes, stream_of(*x)))
-      Py_RETURN_NONE;
+    const int rc = hexmoe_grouped_wgrad(dy->data_ptr(), dy->stride(0), x->data_ptr(), x->stride(0), code, R, E, N, K,
+                                        off->data_ptr(), index, out.data_ptr(), K, N * K, f32 ? HEXMOE_F32 : code, 0,
+                                        bytes ? ws.data_ptr() : nullptr, bytes, stream_of(*x));
+    if (refused(rc, "hexmoe_grouped_wgrad")) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));
   });
 }
@@ -142,9 +153,9 @@ PyObject* swiglu(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       Py_RETURN_NONE;
     const int64_t rows = h->size(0), inter = h->size(1) / 2;
     at::Tensor act = at::empty({rows, inter}, h->options());
-    if (hexmoe_swiglu(h->data_ptr(), code_of(h->scalar_type()), rows, inter, h->stride(0), weights, act.data_ptr(), inter,
-                      stream_of(*h)))
-      Py_RETURN_NONE;
+    const int rc = hexmoe_swiglu(h->data_ptr(), code_of(h->scalar_type()), rows, inter, h->stride(0), weights,
+                                 act.data_ptr(), inter, stream_of(*h));
+    if (refused(rc, "hexmoe_swiglu")) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(act));
   });
 }
@@ -161,10 +172,10 @@ PyObject* swiglu_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int64_t rows = dact->size(0), inter = dact->size(1);
     at::Tensor dh = at::empty({rows, 2 * inter}, h->options()), dw;
     if (weights || a[2] != Py_None) dw = at::empty({rows}, h->options().dtype(at::kFloat));
-    if (hexmoe_swiglu_backward(dact->data_ptr(), dact->stride(0), h->data_ptr(), h->stride(0), code_of(h->scalar_type()),
-                               rows, inter, weights, dh.data_ptr(), 2 * inter,
-                               dw.defined() ? dw.data_ptr<float>() : nullptr, stream_of(*h)))
-      Py_RETURN_NONE;
+    const int rc = hexmoe_swiglu_backward(dact->data_ptr(), dact->stride(0), h->data_ptr(), h->stride(0),
+                                          code_of(h->scalar_type()), rows, inter, weights, dh.data_ptr(), 2 * inter,
+                                          dw.defined() ? dw.data_ptr<float>() : nullptr, stream_of(*h));
+    if (refused(rc, "hexmoe_swiglu_backward")) Py_RETURN_NONE;
     PyObject* first = THPVariable_Wrap(std::move(dh));
     if (!first) return nullptr;
     PyObject* second = Py_None;
@@ -219,10 +230,11 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const double max_norm = PyFloat_AS_DOUBLE(a[2]);
     const size_t bytes = hexmoe_clip_grad_norm_workspace_bytes(static_cast<int32_t>(n));
     at::Tensor norm = at::empty({}, first->options().dtype(at::kFloat)), ws = workspace(bytes, *first);
-    if (hexmoe_clip_grad_norm(static_cast<int32_t>(n), src.data(), counts.data(), types.data(), copies ? dst.data() : nullptr,
-                              copies ? dst_types.data() : nullptr, static_cast<float>(max_norm), a[3] == Py_True,
-                              norm.data_ptr<float>(), ws.data_ptr(), bytes, stream_of(*first)))
-      Py_RETURN_NONE;
+    const int rc = hexmoe_clip_grad_norm(static_cast<int32_t>(n), src.data(), counts.data(), types.data(),
+                                         copies ? dst.data() : nullptr, copies ? dst_types.data() : nullptr,
+                                         static_cast<float>(max_norm), a[3] == Py_True, norm.data_ptr<float>(),
+                                         ws.data_ptr(), bytes, stream_of(*first));
+    if (refused(rc, "hexmoe_clip_grad_norm")) Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(norm));
   });
 }

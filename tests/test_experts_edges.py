@@ -4,15 +4,20 @@ to lose a row in, what happens to a call that fails half way, and what autograd 
 from __future__ import annotations
 
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
 import torch
+from conftest import ROOT
 from test_experts import (BF16, DEV, F16, F32, ROUND, assert_sum, device_word, mm_reference, normal, offsets_of, padded,  # noqa: F401
                           swiglu_reference, wgrad_reference)
 
 from blackhole_b200 import experts
 
+PACKAGE = ROOT / "blackhole-harness_b200"
 # smallest distance between values, halved: what a result near zero may be off by
 HALF_STEP = {BF16: 2.0 ** -134, F16: 2.0 ** -25, F32: 2.0 ** -150}
 LARGEST = {BF16: 3.3895e38, F16: 65504.0, F32: 3.4028234e38}
@@ -200,3 +205,24 @@ def test_gradients_of_offsets_that_do_not_fit(off):
     assert torch.equal(got, experts.grouped_wgrad(x, x, fixed.to(DEV), out_dtype=F32))
     want, mass = wgrad_reference(x.cpu(), x.cpu(), fixed)
     assert_sum(got, want, mass, 32, F32)
+
+
+# ------------------------------------------------------------------ calls and autograd
+FAILING = r"""
+extern "C" int hexmoe_clip_grad_norm() { return 3; }                         // HEXMOE_E_CUDA
+extern "C" const char* hexmoe_last_error() { return "a launch that failed"; }
+"""
+
+
+@pytest.mark.gpu
+def test_a_failed_clipping_is_not_made_again(tmp_path):
+    """After a launch that failed some lists may have been scaled: the call raises and is not repeated."""
+    (tmp_path / "failing.cpp").write_text(FAILING)
+    lib = tmp_path / "failing.so"
+    subprocess.run(["g++", "-shared", "-fPIC", "-o", lib, tmp_path / "failing.cpp"], check=True)
+    code = ("import torch\nfrom blackhole_b200 import experts\ng = torch.ones(4, device='cuda')\n"
+            "try:\n    experts.clip_grad_norm([g], 0.5)\nexcept RuntimeError as e:\n    assert 'a launch that failed' in str(e), e\n"
+            "else:\n    raise SystemExit('the call was made again')\nassert g.tolist() == [1.0] * 4, g\n")
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=PACKAGE,
+                          env={**os.environ, "LD_PRELOAD": str(lib)})
+    assert done.returncode == 0, done.stdout + done.stderr
