@@ -26,8 +26,14 @@ from operator import attrgetter
 
 import torch
 
-from blackhole_b200 import _call, _lib   # _call: the same calls without Python's share, None where it passes
+from blackhole_b200 import _lib
 from blackhole_b200.hex_moe import _DT, _aligned, _ptr, align, combine_rows
+
+try:
+    from blackhole_b200 import _call   # the same calls without Python's share, None where it passes
+except ImportError:   # not built, or built for another torch: every call goes through Python and libhexmoe.so
+    class _call:
+        grouped_mm = grouped_wgrad = swiglu = swiglu_backward = clip_grad_norm = staticmethod(lambda *args: None)
 
 _16BIT = (torch.bfloat16, torch.float16)
 _INDEX = {torch.int32: _lib.I32, torch.int64: _lib.I64}

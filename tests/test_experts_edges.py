@@ -226,3 +226,31 @@ def test_a_failed_clipping_is_not_made_again(tmp_path):
     done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=PACKAGE,
                           env={**os.environ, "LD_PRELOAD": str(lib)})
     assert done.returncode == 0, done.stdout + done.stderr
+
+
+def test_the_operators_import_without_the_call_module():
+    """_call.so is bound to one torch and one Python; libhexmoe.so is not, and every call has a path to it in Python."""
+    code = ("import sys\nsys.modules['blackhole_b200._call'] = None\nimport torch\nfrom blackhole_b200 import experts\n"
+            "try:\n    experts.swiglu(torch.zeros(2, 4))\nexcept ValueError as e:\n    assert 'CUDA' in str(e)\nelse:\n    raise SystemExit(1)\n")
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120, cwd=PACKAGE)
+    assert done.returncode == 0, done.stderr
+
+
+@pytest.mark.gpu
+def test_calls_without_the_call_module_are_the_same(monkeypatch):
+    off = offsets_of([40, 0, 88]).to(DEV)
+    x, w, dy = normal((128, 72), BF16, 89).to(DEV), normal((3, 136, 72), BF16, 90).to(DEV), normal((128, 136), BF16, 91).to(DEV)
+    weight, grads = torch.rand(128, device=DEV), [normal((300, 7), F32, 92).to(DEV), normal((9,), BF16, 93).to(DEV)]
+
+    def calls():
+        out = [torch.empty_like(t) for t in grads]
+        norm = experts.clip_grad_norm(grads, 1.0, out=out)
+        return [experts.grouped_mm(x, w, off), experts.grouped_mm(dy, w, off, transpose=True), experts.grouped_wgrad(dy, x, off),
+                experts.grouped_wgrad(dy, x, off, out_dtype=F32), experts.swiglu(dy, weight),
+                *experts.swiglu_backward(dy[:, :68].contiguous(), dy, weight), norm, *out]
+
+    with_it = calls()
+    none = type("none", (), {name: staticmethod(lambda *args: None) for name in
+                             ("grouped_mm", "grouped_wgrad", "swiglu", "swiglu_backward", "clip_grad_norm")})
+    monkeypatch.setattr(experts, "_call", none)
+    assert all(torch.equal(a, b) for a, b in zip(with_it, calls(), strict=True))
