@@ -236,6 +236,13 @@ def test_the_operators_import_without_the_call_module():
     assert done.returncode == 0, done.stderr
 
 
+def test_the_library_builds_without_headers_of_python_and_torch():
+    done = subprocess.run(["make", "-n", "-B", "PYTHON=false", "all"], capture_output=True, text=True, timeout=60, cwd=PACKAGE)
+    assert done.returncode == 0 and "libhexmoe.so" in done.stdout and "call.cpp" not in done.stdout, done.stderr
+    done = subprocess.run(["make", "-n", "-B", f"PYTHON={sys.executable}", "all"], capture_output=True, text=True, timeout=120, cwd=PACKAGE)
+    assert done.returncode == 0 and "call.cpp" in done.stdout, done.stderr
+
+
 @pytest.mark.gpu
 def test_calls_without_the_call_module_are_the_same(monkeypatch):
     off = offsets_of([40, 0, 88]).to(DEV)
