@@ -41,6 +41,7 @@ _INDEX = {torch.int32: _lib.I32, torch.int64: _lib.I64}
 
 _raw_stream = torch._C._cuda_getCurrentRawStream   # current_stream() without building a Stream object
 _current_device = torch.cuda.current_device
+_written = torch.autograd.graph.increment_version   # tells autograd, which may hold the tensor, that it changed
 
 
 def _run(fn, dev: torch.device, *args) -> None:
@@ -158,7 +159,11 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, transpos
         ws, nbytes = _workspace(_lib.lib.hexmoe_grouped_mm_workspace_bytes(R, E, N, K, transpose), x)
     _run(_grouped_mm, dev, x.data_ptr(), ld_x, w.data_ptr(), ld_w, stride_w, code, R, E, N, K, transpose,
          offsets.data_ptr(), index_code, to.data_ptr(), ld, _DT[to.dtype], _ptr(ws), nbytes)
-    return res if to is res else res.copy_(to)
+    if to is not res:
+        res.copy_(to)
+    elif out is not None:
+        _written(out)
+    return res
 
 
 def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out_dtype: torch.dtype | None = None,
@@ -194,7 +199,11 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out_
         ws, nbytes = _workspace(_lib.lib.hexmoe_grouped_wgrad_workspace_bytes(R, E, N, K), x)
     _run(_grouped_wgrad, dev, dy.data_ptr(), ld_dy, x.data_ptr(), ld_x, code, R, E, N, K, offsets.data_ptr(), index_code,
          to.data_ptr(), ld, stride, _DT[to.dtype], accumulate, _ptr(ws), nbytes)
-    return res if to is res else res.copy_(to)
+    if to is not res:
+        res.copy_(to)
+    elif out is not None:
+        _written(out)
+    return res
 
 
 def _check_row_weights(row_weights, rows: int, dev: torch.device):
@@ -250,6 +259,8 @@ def swiglu_backward(dact: torch.Tensor, h: torch.Tensor, row_weights: torch.Tens
     dw = None if row_weights is None else row_weights.new_empty(R)
     _run(_swiglu_backward, dev, dact.data_ptr(), ld_dact, h.data_ptr(), ld_h, _DT[h.dtype], R, I, _ptr(row_weights),
          dh.data_ptr(), 2 * I if out is None else out.stride(0), _ptr(dw))
+    if out is not None:
+        _written(out)
     return dh, dw
 
 
@@ -321,7 +332,7 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     dev = grads[0].device
     if dev.type != "cuda":
         raise ValueError("clip_grad_norm runs on CUDA only")
-    held = grads if out is None else grads + out
+    held, written = grads if out is None else grads + out, grads if out is None else out
     if set(map(_get_device, held)) != {dev.index}:
         raise ValueError(f"clip_grad_norm: not every tensor is on {dev}")
     if out is not None and list(map(_get_shape, grads)) != list(map(_get_shape, out)):
@@ -346,6 +357,7 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     ws = torch.empty(nbytes // 4 + 1, dtype=torch.float32, device=dev)   # the partial sums, then the norm
     _run(_clip_grad_norm, dev, n, ptrs.buffer_info()[0], counts.buffer_info()[0], types.buffer_info()[0], out_ptr,
          out_types_ptr, max_norm, norm_type == math.inf, ws.data_ptr() + nbytes, ws.data_ptr(), nbytes)
+    _written(written)
     return ws[nbytes // 4]
 
 

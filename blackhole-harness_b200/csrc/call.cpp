@@ -235,6 +235,10 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                                          static_cast<float>(max_norm), a[3] == Py_True, norm.data_ptr<float>(),
                                          ws.data_ptr(), bytes, stream_of(*first));
     if (refused(rc, "hexmoe_clip_grad_norm")) Py_RETURN_NONE;
+    for (Py_ssize_t i = 0; i < n; ++i) {   // autograd, which may hold what was written, looks at its version
+      const at::Tensor& written = *tensor(PyList_GET_ITEM(a[copies], i));
+      if (!written.is_inference()) written.unsafeGetTensorImpl()->bump_version();
+    }
     return THPVariable_Wrap(std::move(norm));
   });
 }

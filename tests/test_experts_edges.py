@@ -261,3 +261,33 @@ def test_calls_without_the_call_module_are_the_same(monkeypatch):
                              ("grouped_mm", "grouped_wgrad", "swiglu", "swiglu_backward", "clip_grad_norm")})
     monkeypatch.setattr(experts, "_call", none)
     assert all(torch.equal(a, b) for a, b in zip(with_it, calls(), strict=True))
+
+
+@pytest.mark.gpu
+def test_autograd_sees_what_is_written():
+    """A tensor that is written to has a new version, so that a backward pass that kept its old values refuses them."""
+    off = offsets_of([40, 0, 88]).to(DEV)
+    x, w, dy = normal((128, 72), BF16, 94).to(DEV), normal((3, 136, 72), BF16, 95).to(DEV), normal((128, 136), BF16, 96).to(DEV)
+    wide, grads = torch.zeros(128, 140, dtype=BF16, device=DEV), [torch.ones(9, device=DEV), torch.ones(5, dtype=BF16, device=DEV)]
+    strided = torch.ones(6, 8, device=DEV)[:, :5]
+    with torch.inference_mode():
+        kept = torch.ones(4, device=DEV)
+    cases = [([wide], lambda: experts.grouped_mm(x, w, off, out=wide[:, :136])),
+             ([w], lambda: experts.grouped_wgrad(dy, x, off, out=w, accumulate=True)),
+             ([dy], lambda: experts.swiglu_backward(dy[:, :68].contiguous(), dy, out=dy)),
+             (grads, lambda: experts.clip_grad_norm(grads, 1.0)), ([strided], lambda: experts.clip_grad_norm([strided], 1.0)),
+             (grads, lambda: experts.clip_grad_norm([torch.ones_like(t) for t in grads], 1.0, out=grads))]
+    for written, call in cases:
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > v for t, v in zip(written, before))
+    experts.clip_grad_norm([kept], 1.0)      # a tensor without versions
+    assert float(kept.norm()) < 1.01
+    source = [torch.ones(9, device=DEV)]
+    experts.clip_grad_norm(source, 1.0, out=[torch.empty(9, device=DEV)])
+    assert source[0]._version == 0           # only read
+    leaf = torch.zeros(9, device=DEV, requires_grad=True)
+    held = leaf.exp()
+    experts.clip_grad_norm([held.detach()], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        held.sum().backward()
