@@ -986,8 +986,15 @@ int make_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int dims,
   if (!fn) return report_error(HEXMOE_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   const cuuint64_t size[3] = {cols, rows, outer}, strides[2] = {pitch, stride};
   const cuuint32_t box[3] = {box_cols, box_rows, 1}, step[3] = {1, 1, 1};
-  const CUresult r = fn(m, dt, dims, const_cast<void*>(base), size, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return fn(m, dt, dims, const_cast<void*>(base), size, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {   // a host thread that has launched nothing yet: runtime calls bind it, this one does not
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
   if (r == CUDA_SUCCESS) return HEXMOE_OK;
   char buf[96];
   snprintf(buf, sizeof(buf), "grouped product: cuTensorMapEncodeTiled failed (%d)", static_cast<int>(r));

@@ -7,6 +7,7 @@ import math
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 import numpy as np
 import pytest
@@ -291,3 +292,18 @@ def test_autograd_sees_what_is_written():
     experts.clip_grad_norm([held.detach()], 0.1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         held.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["grouped_mm", "transpose", "grouped_wgrad"])
+def test_a_product_may_be_a_threads_first_call(name):
+    """A host thread that has launched nothing has no CUDA context of its own (autograd's and a server's worker threads)."""
+    off = offsets_of([40, 0, 88]).to(DEV)
+    x, w, dy = normal((128, 72), BF16, 104).to(DEV), normal((3, 136, 72), BF16, 105).to(DEV), normal((128, 136), BF16, 106).to(DEV)
+    call = {"grouped_mm": lambda: experts.grouped_mm(x, w, off), "transpose": lambda: experts.grouped_mm(dy, w, off, transpose=True),
+            "grouped_wgrad": lambda: experts.grouped_wgrad(dy, x, off)}[name]
+    want = call().clone()     # and its memory is at hand: the thread's call allocates nothing from the driver
+    torch.cuda.synchronize()
+    with ThreadPoolExecutor(1) as pool:
+        got = pool.submit(call).result()
+    assert torch.equal(got, want)
