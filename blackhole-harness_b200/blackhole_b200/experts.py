@@ -16,6 +16,10 @@ Rows lie in expert order: group e is rows offsets[e] .. offsets[e + 1] - 1
 (expert_plan makes them from a router's ids).  Inputs must be CUDA tensors on an
 sm_100 device; there is no CPU path.  Calls run on the current stream of the
 inputs' device, synchronise nothing and can be captured in CUDA graphs.
+
+grouped_mm, grouped_wgrad, swiglu and expert_mlp are differentiable (once).  What is written
+into an `out` stays outside autograd's graph, as do swiglu_backward and clip_grad_norm, and
+an `out` overlaps no input (swiglu_backward's may be h).
 """
 
 from __future__ import annotations
@@ -109,6 +113,11 @@ def _output(out, shape: tuple, like: torch.Tensor, out_dtype, what: str) -> torc
     return out
 
 
+def _recorded(*tensors) -> bool:
+    """Whether autograd is to see the call."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 _FEW_TILES = 37   # the library asks for a workspace only where at most so many 256 x 256 tiles share the machine
 
 
@@ -120,15 +129,71 @@ _grouped_mm, _grouped_wgrad = _lib.lib.hexmoe_grouped_mm, _lib.lib.hexmoe_groupe
 _swiglu, _swiglu_backward = _lib.lib.hexmoe_swiglu, _lib.lib.hexmoe_swiglu_backward
 
 
+class _GroupedMM(torch.autograd.Function):
+    """y = x W^T: dx = dy W, dW[e] = dy_e^T x_e; with transpose y = x W: dx = dy W^T, dW[e] = x_e^T dy_e.  The
+    gradient of an f32 result is rounded to the 16 bits that the products take."""
+
+    @staticmethod
+    def forward(ctx, x, w, offsets, transpose, out_dtype):
+        ctx.save_for_backward(x, w, offsets)
+        ctx.transpose = transpose
+        return grouped_mm(x, w, offsets, transpose, out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, offsets = ctx.saved_tensors
+        dy = dy.to(x.dtype)
+        dx = grouped_mm(dy, w, offsets, not ctx.transpose) if ctx.needs_input_grad[0] else None
+        dw = None
+        if ctx.needs_input_grad[1]:
+            dw = grouped_wgrad(x, dy, offsets) if ctx.transpose else grouped_wgrad(dy, x, offsets)
+        return dx, dw, None, None, None
+
+
+class _GroupedWgrad(torch.autograd.Function):
+    """dW[e] = dy_e^T x_e: with its gradient G, ddy = x G^T and dx = dy G.  G is rounded as above."""
+
+    @staticmethod
+    def forward(ctx, dy, x, offsets, out_dtype):
+        ctx.save_for_backward(dy, x, offsets)
+        return grouped_wgrad(dy, x, offsets, out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        dy, x, offsets = ctx.saved_tensors
+        g = g.to(x.dtype)
+        ddy = grouped_mm(x, g, offsets) if ctx.needs_input_grad[0] else None
+        return ddy, grouped_mm(dy, g, offsets, transpose=True) if ctx.needs_input_grad[1] else None, None, None
+
+
+class _SwiGLU(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, row_weights):
+        ctx.save_for_backward(h, row_weights)
+        return swiglu(h, row_weights)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dact):
+        return swiglu_backward(dact, *ctx.saved_tensors)
+
+
 def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, transpose: bool = False,
                out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """x[r] W[e]^T for every row r of group e: x [R, K], w [E, N, K] -> [R, N]; with transpose
     x[r] W[e]: x [R, N] -> [R, K].  Rows of no group come back as zero.  bf16 or fp16, the
-    result in the same type or (out_dtype, out) float32."""
+    result in the same type or (out_dtype, out) float32.  Differentiable in x and w; with
+    `out`, where they require grad, an error."""
     if out is None and out_dtype is None:
         res = _call.grouped_mm(x, w, offsets, transpose)
         if res is not None:
             return res
+    if _recorded(x, w):
+        if out is not None:
+            raise RuntimeError("grouped_mm: x or w requires grad, and what is written into out is not differentiable")
+        return _GroupedMM.apply(x, w, offsets, transpose, out_dtype)
     code = _check_16bit("grouped_mm", x, w)
     if w.dim() != 3:
         raise ValueError(f"w must be [E, N, K], got {tuple(w.shape)}")
@@ -170,11 +235,14 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out_
                   out: torch.Tensor | None = None, accumulate: bool = False) -> torch.Tensor:
     """dW[e] = dy_e^T x_e over the rows of every group: dy [R, N], x [R, K] -> [E, N, K] (zero for
     an empty group), in their type or float32.  accumulate adds to `out`.  With dy = x these
-    are the Hessians that quant.quantize_stack(H=...) takes."""
+    are the Hessians that quant.quantize_stack(H=...) takes.  Differentiable without `out`; sums
+    in `out` are statistics or gradients, and keep no graph."""
     if out is None and not accumulate and (out_dtype is None or out_dtype in (torch.float32, x.dtype)):
         res = _call.grouped_wgrad(dy, x, offsets, out_dtype == torch.float32)
         if res is not None:
             return res
+    if out is None and not accumulate and _recorded(dy, x):
+        return _GroupedWgrad.apply(dy, x, offsets, out_dtype)
     code = _check_16bit("grouped_wgrad", dy, x)
     (dy, ld_dy), (x, ld_x) = _rows2d(dy, "dy"), _rows2d(x, "x")
     if dy.shape[0] != x.shape[0]:
@@ -215,10 +283,13 @@ def _check_row_weights(row_weights, rows: int, dev: torch.device):
 
 
 def swiglu(h: torch.Tensor, row_weights: torch.Tensor | None = None) -> torch.Tensor:
-    """silu(gate) * up * row_weights of rows h [R, 2I] = [gate | up] -> [R, I] (f32, bf16 or fp16)."""
+    """silu(gate) * up * row_weights of rows h [R, 2I] = [gate | up] -> [R, I] (f32, bf16 or fp16),
+    differentiable in both."""
     act = _call.swiglu(h, row_weights)
     if act is not None:
         return act
+    if _recorded(h, row_weights):
+        return _SwiGLU.apply(h, row_weights)
     if not h.is_cuda:
         raise ValueError("swiglu runs on CUDA only")
     if h.dtype not in _DT:
@@ -237,7 +308,7 @@ def swiglu(h: torch.Tensor, row_weights: torch.Tensor | None = None) -> torch.Te
 def swiglu_backward(dact: torch.Tensor, h: torch.Tensor, row_weights: torch.Tensor | None = None,
                     out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor | None]:
     """The gradient of swiglu(h, row_weights) for dact [R, I]: dh [R, 2I], and that of row_weights
-    (float32 [R]; None without them).  out takes dh; it may be h itself."""
+    (float32 [R]; None without them).  out takes dh; it may be h itself.  Not differentiable itself."""
     if out is None:
         both = _call.swiglu_backward(dact, h, row_weights)
         if both is not None:

@@ -8,13 +8,14 @@
 // arguments, allocates what the call needs, makes it on the current stream and
 // returns the result; or it returns None, having done nothing, where anything is
 // out of the ordinary (another device than the current one, a stride that wants a
-// copy, a type or shape that does not fit, arguments that the call refuses), and
+// copy, a type or shape that does not fit, inputs that autograd follows, arguments that the call refuses), and
 // experts.py takes the call from there, with its checks and messages.  A call that
 // failed on the way, with some of its work perhaps done, raises.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -46,6 +47,8 @@ int code_of(at::ScalarType t) {
 bool here(const at::Tensor& t) {
   return t.is_cuda() && t.layout() == at::kStrided && t.get_device() == c10::cuda::current_device();
 }
+// Autograd is to see a call with this input.
+bool recorded(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
 void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 bool matrix(const at::Tensor& t) { return t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= t.size(1); }
 
@@ -85,7 +88,8 @@ PyObject* grouped_mm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
     const at::Tensor *x = n_args == 4 ? tensor(a[0]) : nullptr, *w = x ? tensor(a[1]) : nullptr,
                      *off = w ? tensor(a[2]) : nullptr;
-    if (!off || !here(*x) || !here(*w) || x->scalar_type() != w->scalar_type() || !matrix(*x) || w->dim() != 3)
+    if (!off || !here(*x) || !here(*w) || x->scalar_type() != w->scalar_type() || !matrix(*x) || w->dim() != 3 ||
+        recorded(*x) || recorded(*w))
       Py_RETURN_NONE;
     const int code = code_of(x->scalar_type()), transpose = a[3] == Py_True;
     const int64_t E = w->size(0), N = w->size(1), K = w->size(2), R = x->size(0);
@@ -112,7 +116,7 @@ PyObject* grouped_wgrad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor *dy = n_args == 4 ? tensor(a[0]) : nullptr, *x = dy ? tensor(a[1]) : nullptr,
                      *off = x ? tensor(a[2]) : nullptr;
     if (!off || !here(*dy) || !here(*x) || dy->scalar_type() != x->scalar_type() || !matrix(*dy) || !matrix(*x) ||
-        off->dim() != 1 || off->size(0) < 2)
+        off->dim() != 1 || off->size(0) < 2 || recorded(*dy) || recorded(*x))
       Py_RETURN_NONE;
     const int code = code_of(x->scalar_type());
     const int64_t E = off->size(0) - 1, N = dy->size(1), K = x->size(1), R = x->size(0);
@@ -149,7 +153,8 @@ PyObject* swiglu(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor* h = n_args == 2 ? tensor(a[0]) : nullptr;
     const float* weights = nullptr;
     if (!h || !here(*h) || code_of(h->scalar_type()) < 0 || !matrix(*h) || h->size(1) % 2 || !h->size(1) ||
-        h->size(1) > (1 << 30) || !row_weights(a[1], h->size(0), &weights))
+        h->size(1) > (1 << 30) || !row_weights(a[1], h->size(0), &weights) || recorded(*h) ||
+        (weights && recorded(*tensor(a[1]))))
       Py_RETURN_NONE;
     const int64_t rows = h->size(0), inter = h->size(1) / 2;
     at::Tensor act = at::empty({rows, inter}, h->options());

@@ -307,3 +307,72 @@ def test_a_product_may_be_a_threads_first_call(name):
     with ThreadPoolExecutor(1) as pool:
         got = pool.submit(call).result()
     assert torch.equal(got, want)
+
+
+def grads_of(call, *inputs):
+    """The call's result, its gradient for a drawn one of the result, and that."""
+    leaves = [t.detach().clone().requires_grad_() for t in inputs]
+    out = call(*leaves)
+    assert out.requires_grad
+    d = normal(tuple(out.shape), out.dtype, 97).to(DEV)
+    return [out.detach(), *torch.autograd.grad(out, leaves, d)], d
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("out_dtype", [None, F32], ids=str)
+def test_operators_inside_a_graph(out_dtype):
+    """Called on inputs that require grad, the operators hand on gradients: those of the operators themselves."""
+    sizes = [40, 0, 88]
+    off = offsets_of(sizes).to(DEV)
+    x, w, dy = normal((130, 72), BF16, 98).to(DEV), normal((3, 136, 72), BF16, 99, 0.1).to(DEV), normal((130, 136), BF16, 100).to(DEV)
+    (y, dx, dw), d = grads_of(lambda a, b: experts.grouped_mm(a, b, off, out_dtype=out_dtype), x, w)
+    d = d.to(BF16)
+    assert torch.equal(y, experts.grouped_mm(x, w, off, out_dtype=out_dtype)) and dx.dtype == dw.dtype == BF16
+    assert torch.equal(dx, experts.grouped_mm(d, w, off, transpose=True)) and torch.equal(dw, experts.grouped_wgrad(d, x, off))
+    want, mass = wgrad_reference(d.cpu(), x.cpu(), off.cpu())
+    assert_sum(dw, want, mass, max(sizes), BF16)
+    (y, dx, dw), d = grads_of(lambda a, b: experts.grouped_mm(a, b, off, transpose=True, out_dtype=out_dtype), dy, w)
+    d = d.to(BF16)
+    assert torch.equal(dx, experts.grouped_mm(d, w, off)) and torch.equal(dw, experts.grouped_wgrad(dy, d, off))
+    want, mass = mm_reference(d.cpu(), w.cpu(), off.cpu(), False, 130)
+    assert_sum(dx, want, mass, 72, BF16)
+    (dw, ddy, dx), g = grads_of(lambda a, b: experts.grouped_wgrad(a, b, off, out_dtype=out_dtype), dy, x)
+    g = g.to(BF16)
+    assert torch.equal(ddy, experts.grouped_mm(x, g, off)) and torch.equal(dx, experts.grouped_mm(dy, g, off, transpose=True))
+    # one of the inputs alone, and one input twice: H = x^T x has the gradient x (G + G^T)
+    leaf = x.clone().requires_grad_()
+    experts.grouped_mm(leaf, w, off).float().sum().backward()
+    assert torch.equal(leaf.grad, experts.grouped_mm(torch.ones_like(dy), w, off, transpose=True))
+    (h, dx), g = grads_of(lambda a: experts.grouped_wgrad(a, a, off, out_dtype=F32), x)
+    want, mass = mm_reference(x.cpu(), (g.to(BF16).double() + g.to(BF16).double().transpose(1, 2)).cpu(), off.cpu(), False, 130)
+    # two products, each rounded to bf16, and their sum
+    both, mass2 = mm_reference(x.cpu().abs(), (g.abs().double() + g.abs().double().transpose(1, 2)).cpu(), off.cpu(), False, 130)
+    assert ((dx.double().cpu() - want).abs() <= 3 * 2.0 ** -8 * mass2).all()
+
+
+@pytest.mark.gpu
+def test_swiglu_inside_a_graph():
+    h, weight = normal((50, 96), BF16, 101).to(DEV), torch.rand(50, device=DEV)
+    (act, dh, dw), d = grads_of(experts.swiglu, h, weight)
+    assert torch.equal(act, experts.swiglu(h, weight))
+    assert all(torch.equal(a, b) for a, b in zip((dh, dw), experts.swiglu_backward(d, h, weight)))
+    (act, dh), d = grads_of(experts.swiglu, h)
+    assert torch.equal(dh, experts.swiglu_backward(d, h)[0])
+    leaf = weight.clone().requires_grad_()
+    experts.swiglu(h, leaf).float().sum().backward()
+    assert torch.equal(leaf.grad, experts.swiglu_backward(torch.ones_like(d), h, weight)[1])
+
+
+@pytest.mark.gpu
+def test_calls_outside_the_graph():
+    """Without grad mode nothing is recorded; a product into `out` says that it cannot be; sums in `out` are not."""
+    off = offsets_of([40, 0, 88]).to(DEV)
+    x, w = normal((128, 72), BF16, 102).to(DEV).requires_grad_(), normal((3, 136, 72), BF16, 103).to(DEV)
+    out, h = torch.empty(128, 136, dtype=BF16, device=DEV), torch.zeros(3, 72, 72, device=DEV)
+    with pytest.raises(RuntimeError, match="requires grad"):
+        experts.grouped_mm(x, w, off, out=out)
+    assert experts.grouped_wgrad(x, x, off, out=h, accumulate=True) is h and not h.requires_grad
+    with torch.no_grad():
+        assert not experts.grouped_mm(x, w, off).requires_grad and not experts.grouped_mm(x, w, off, out=out).requires_grad
+        assert torch.equal(h, experts.grouped_wgrad(x, x, off, out_dtype=F32))
+    assert not experts.grouped_mm(x.detach(), w, off).requires_grad
