@@ -118,9 +118,6 @@ def _recorded(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-_FEW_TILES = 37   # the library asks for a workspace only where at most so many 256 x 256 tiles share the machine
-
-
 def _workspace(nbytes: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int]:
     return (torch.empty(nbytes, dtype=torch.uint8, device=like.device), nbytes) if nbytes else (None, 0)
 
@@ -219,9 +216,7 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor, transpos
         ld = res.stride(0)
         if ld < width or res.stride(1) != 1:
             to, ld = torch.empty_like(res, memory_format=torch.contiguous_format), width
-    ws, nbytes = None, 0
-    if -(-width // 256) * (min(E, R) + R // 256) <= _FEW_TILES:
-        ws, nbytes = _workspace(_lib.lib.hexmoe_grouped_mm_workspace_bytes(R, E, N, K, transpose), x)
+    ws, nbytes = _workspace(_lib.lib.hexmoe_grouped_mm_workspace_bytes(R, E, N, K, transpose), x)
     _run(_grouped_mm, dev, x.data_ptr(), ld_x, w.data_ptr(), ld_w, stride_w, code, R, E, N, K, transpose,
          offsets.data_ptr(), index_code, to.data_ptr(), ld, _DT[to.dtype], _ptr(ws), nbytes)
     if to is not res:
@@ -262,9 +257,7 @@ def grouped_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor, out_
         if step != 1 or ld < K or stride < (N - 1) * ld + K:
             to = res.contiguous() if accumulate else torch.empty_like(res, memory_format=torch.contiguous_format)
             stride, ld = N * K, K
-    ws, nbytes = None, 0
-    if E * -(-N // 256) * -(-K // 256) <= _FEW_TILES:
-        ws, nbytes = _workspace(_lib.lib.hexmoe_grouped_wgrad_workspace_bytes(R, E, N, K), x)
+    ws, nbytes = _workspace(_lib.lib.hexmoe_grouped_wgrad_workspace_bytes(R, E, N, K), x)
     _run(_grouped_wgrad, dev, dy.data_ptr(), ld_dy, x.data_ptr(), ld_x, code, R, E, N, K, offsets.data_ptr(), index_code,
          to.data_ptr(), ld, stride, _DT[to.dtype], accumulate, _ptr(ws), nbytes)
     if to is not res:

@@ -376,3 +376,23 @@ def test_calls_outside_the_graph():
         assert not experts.grouped_mm(x, w, off).requires_grad and not experts.grouped_mm(x, w, off, out=out).requires_grad
         assert torch.equal(h, experts.grouped_wgrad(x, x, off, out_dtype=F32))
     assert not experts.grouped_mm(x.detach(), w, off).requires_grad
+
+
+@pytest.mark.gpu
+def test_the_library_alone_plans_the_workspace(monkeypatch):
+    """Whatever the size, the library is asked, and gets what it asks for: no rule of its plan is kept on this side."""
+    from blackhole_b200 import _lib
+    sizes = [3] * 120
+    off, asked, given = offsets_of(sizes).to(DEV), [], []
+    x, dy = normal((360, 264), BF16, 107).to(DEV), normal((360, 520), BF16, 108).to(DEV)
+    w = normal((120, 520, 264), BF16, 109).to(DEV)
+    want = experts.grouped_mm(x, w, off), experts.grouped_wgrad(dy, x, off)
+    for name in ("hexmoe_grouped_mm_workspace_bytes", "hexmoe_grouped_wgrad_workspace_bytes"):
+        monkeypatch.setattr(_lib.lib, name, lambda *args: asked.append(args) or 4096)
+    held = experts._workspace
+    monkeypatch.setattr(experts, "_workspace", lambda nbytes, like: given.append(nbytes) or held(nbytes, like))
+    outs = torch.empty_like(want[0]), torch.empty_like(want[1])
+    experts.grouped_mm(x, w, off, out=outs[0])
+    experts.grouped_wgrad(dy, x, off, out=outs[1])
+    assert [a[:4] for a in asked] == [(360, 120, 520, 264)] * 2 and given == [4096] * 2
+    assert all(torch.equal(a, b) for a, b in zip(outs, want))
