@@ -345,11 +345,16 @@ def _runs(t: torch.Tensor):
     if t.numel() == 0 or _dense(t):
         yield t
         return
-    if 0 in t.stride():
+    if 0 in (st for st, size in zip(t.stride(), t.shape) if size > 1):
         raise ValueError("clip_grad_norm: an expanded tensor holds a value more than once")
     d = max(range(t.dim()), key=lambda i: t.stride(i) if t.shape[i] > 1 else -1)
     for i in range(t.shape[d]):
         yield from _runs(t.select(d, i))
+
+
+def _places(t: torch.Tensor) -> list:
+    """Where t's values stand: the strides of the dimensions that have any."""
+    return [(st, size) for st, size in zip(t.stride(), t.shape) if size != 1] if t.numel() else []
 
 
 def _type_codes(tensors: list) -> array:
@@ -402,7 +407,7 @@ def clip_grad_norm(grads, max_norm: float, norm_type: float = 2.0, out=None) -> 
     if out is not None and list(map(_get_shape, grads)) != list(map(_get_shape, out)):
         raise ValueError("every tensor of out must have its gradient's shape")
     if not all(map(_is_contiguous, held)):
-        if out is not None and [g.stride() for g in grads] != [o.stride() for o in out]:
+        if out is not None and list(map(_places, grads)) != list(map(_places, out)):
             raise ValueError("every tensor of out must have its gradient's strides")
         grads = [r for g in grads for r in _runs(g)]
         if len(grads) > _CLIP_RUNS:

@@ -396,3 +396,19 @@ def test_the_library_alone_plans_the_workspace(monkeypatch):
     experts.grouped_wgrad(dy, x, off, out=outs[1])
     assert [a[:4] for a in asked] == [(360, 120, 520, 264)] * 2 and given == [4096] * 2
     assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.gpu
+def test_clipping_does_not_look_at_strides_of_single_entries():
+    """The stride of a dimension of one entry, or of a tensor without values, says nothing about where values stand."""
+    base, into = normal((4, 6), F32, 110).to(DEV), torch.full((4, 6), 9.0, device=DEV)
+    grads = [base.as_strided((1, 4, 1, 3), (0, 6, 0, 2)), torch.empty(0, 6, device=DEV)[:, ::2]]
+    out = [into.as_strided((1, 4, 1, 3), (7, 6, 1, 2)), torch.empty(0, 3, device=DEV)]
+    part = base[:, ::2].clone()
+    norm = experts.clip_grad_norm(grads, 1.0, out=out)
+    assert abs(float(norm) - float(part.double().norm())) <= 2.0 ** -22 * float(norm)
+    torch.testing.assert_close(into[:, ::2], part / part.norm(), rtol=1e-5, atol=0)
+    assert (into[:, 1::2] == 9).all() and torch.equal(base[:, ::2], part)
+    assert torch.equal(experts.clip_grad_norm(grads, 1.0), norm) and torch.equal(base[:, ::2], into[:, ::2])
+    with pytest.raises(ValueError, match="strides"):
+        experts.clip_grad_norm([base[:, ::2]], 1.0, out=[torch.empty(4, 3, device=DEV)])
