@@ -314,7 +314,7 @@ def swiglu_backward(dact: torch.Tensor, h: torch.Tensor, row_weights: torch.Tens
         raise ValueError(f"h must be [R, 2 * I] and dact [R, I], got {tuple(h.shape)} and {tuple(dact.shape)}")
     R, I = dact.shape
     if out is not None and (out.shape != h.shape or out.dtype != h.dtype or out.device != h.device
-                            or out.stride(1) != 1 or out.stride(0) < 2 * I):
+                            or out.stride(1) != 1 or (R > 1 and out.stride(0) < 2 * I)):
         raise ValueError(f"out must be {h.dtype} {list(h.shape)} with contiguous rows")
     dev = h.device
     row_weights = _check_row_weights(row_weights, R, dev)
@@ -322,7 +322,7 @@ def swiglu_backward(dact: torch.Tensor, h: torch.Tensor, row_weights: torch.Tens
     dh = h.new_empty((R, 2 * I)) if out is None else out
     dw = None if row_weights is None else row_weights.new_empty(R)
     _run(_swiglu_backward, dev, dact.data_ptr(), ld_dact, h.data_ptr(), ld_h, _DT[h.dtype], R, I, _ptr(row_weights),
-         dh.data_ptr(), 2 * I if out is None else out.stride(0), _ptr(dw))
+         dh.data_ptr(), 2 * I if out is None else max(out.stride(0), 2 * I), _ptr(dw))
     if out is not None:
         _written(out)
     return dh, dw

@@ -412,3 +412,14 @@ def test_clipping_does_not_look_at_strides_of_single_entries():
     assert torch.equal(experts.clip_grad_norm(grads, 1.0), norm) and torch.equal(base[:, ::2], into[:, ::2])
     with pytest.raises(ValueError, match="strides"):
         experts.clip_grad_norm([base[:, ::2]], 1.0, out=[torch.empty(4, 3, device=DEV)])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [0, 1])
+def test_swiglu_backward_into_a_single_row(rows):
+    """A single row has no row stride to be refused for."""
+    h, dact, weight = normal((rows, 48), BF16, 111).to(DEV), normal((rows, 24), BF16, 112).to(DEV), torch.rand(rows, device=DEV)
+    out = torch.zeros(48, dtype=BF16, device=DEV).as_strided((rows, 48), (1, 1))
+    dh, dw = experts.swiglu_backward(dact, h, weight, out=out)
+    want = experts.swiglu_backward(dact, h, weight)
+    assert dh is out and torch.equal(dh, want[0]) and torch.equal(dw, want[1])
