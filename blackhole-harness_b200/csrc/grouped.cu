@@ -359,8 +359,8 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 // is W for y; W for dx, and both operands of the weight gradient, are stored with
 // the reduction outermost and go to the tensor core as MN-major tiles.
 //
-// 12 warps a CTA: 0 loads, 1 issues the products (the leader's), 2 zeroes tails
-// (weight gradient), 4..11 write results.  Each walks the groups' offsets by
+// 12 warps a CTA: 0 loads, 1 issues the products (the leader's), 2 and 3 zero tails
+// (weight gradient, the leader's), 4..11 write results.  Each walks the groups' offsets by
 // itself, so that no size is known on the host.
 //
 // Measured, bf16, 96 experts, 1536 x 2048: 512 rows 91 us (HBM, 6.7 TB/s); 32768 rows
@@ -712,7 +712,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     if (lane < kMaxStages) {
       mbar_init(&c->full[lane], 2);    // one arrival of each CTA
       mbar_init(&c->empty[lane], 1);   // the products' commit
-      mbar_init(&c->tail[lane], 1);
+      mbar_init(&c->tail[lane], 2);
     } else if (lane < kMaxStages + 2) {
       mbar_init(&c->acc_full[lane - kMaxStages], 1);
       mbar_init(&c->acc_empty[lane - kMaxStages], 2 * kWriters);
@@ -752,10 +752,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         if (!ok) break;
         uint8_t* a = ring + st * kStageBytes;
         uint8_t* b = a + kSubs * kOperandBytes;
-        // a step whose rows past the group's end are still to be zeroed lands on this CTA's own barrier
+        // a step whose rows past the group's end are still to be zeroed lands on another barrier
         const bool last = s + 1 == t.steps;
         const bool fix = MODE >= kWgrad && last && t.tail % 16 != 0;
-        const uint32_t bar = fix ? peer_addr(&c->tail[st], rank) : peer_addr(&c->full[st], 0);
+        const uint32_t bar = peer_addr(fix ? &c->tail[st] : &c->full[st], 0);
         if (fix) { tails |= 1u << st; tail_odd ^= 1u << st; }
         const int subs = kSubs > 1 && last && t.tail ? (t.tail + kStepK - 1) / kStepK : kSubs;
         if (elect_one()) {
@@ -817,7 +817,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         mbar_wait(&c->full[j % kStages], (j / kStages) & 1, &ignore, p.dev_err);
       }
     }
-    if (MODE >= kWgrad && *abort && lane == 0) {   // and, in each CTA, for the tails, which land on its own barriers
+    if (MODE >= kWgrad && *abort && lane == 0 && leader) {   // and for the steps that land on the tails' barriers
       int ignore = 0;
       for (uint32_t j = 0; j < kStages; ++j)
         if (tails >> j & 1) mbar_wait(&c->tail[j], ~tail_odd >> j & 1, &ignore, p.dev_err);
@@ -834,7 +834,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       for (int32_t s = 0; ok && s < t.steps; ++s) {
         const bool last = s + 1 == t.steps;
         ok = warp_wait(&c->full[st], phase, abort, p.dev_err);
-        if (MODE >= kWgrad && ok && last && t.tail % 16 != 0) pair_acquire(&c->full[st], phase);   // both CTAs' zeroed rows
         const uint32_t a = smem_u32(ring + st * kStageBytes);
         const uint64_t da = MODE == kRowsK ? sw128_desc(a) : sw128_mn_desc(a, kChunkBytes);
         const int count = last && t.tail ? (t.tail + 15) / 16 : kSubs * kStepK / 16;   // products of 16
@@ -867,8 +866,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       pair_umma_commit(&c->done);
       mbar_wait(&c->done, 0, &ignore, p.dev_err);
     }
-  } else if (warp == 2 && MODE >= kWgrad) {
+  } else if ((warp == 2 || warp == 3) && MODE >= kWgrad && leader) {
     // ---------------------------------------------------------------- tails
+    // A warp for each CTA's shared memory, both in the leader: what they clear reaches the products by way of an
+    // arrival in their own CTA.  A warp in either CTA would have to release to the other (96 x 1536 x 2048, 341 rows: 235
+    // us against 218; without clearing anything 204).
+    const uint32_t cta = warp - 2;
     uint32_t it = 0;
     int uses = 0;   // lane s: how many tails stage s has held
     bool ok = true;
@@ -879,17 +882,19 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       ok = warp_wait(&c->tail[st], __shfl_sync(0xffffffffu, uses, st) & 1, abort, p.dev_err);
       if (lane == static_cast<int>(st)) ++uses;
       const uint32_t sub = t.tail / kStepK;
-      uint8_t* a = ring + st * kStageBytes + sub * kOperandBytes;
-      uint8_t* b = ring + st * kStageBytes + kSubs * kOperandBytes + sub * kBBytes;
+      const uint8_t* a = ring + st * kStageBytes + sub * kOperandBytes;
+      const uint8_t* b = ring + st * kStageBytes + kSubs * kOperandBytes + sub * kBBytes;
       const int zeros = (16 - t.tail % 16) * 8;   // 16-byte pieces in the lines to clear, per 64-column chunk
-      for (int i = lane; ok && i < static_cast<int>(2 + kBBytes / kChunkBytes) * zeros; i += 32) {
-        const uint32_t chunk = i / zeros;
-        uint8_t* at = chunk < 2 ? a + chunk * kChunkBytes : b + (chunk - 2) * kChunkBytes;
-        reinterpret_cast<uint4*>(at)[t.tail % kStepK * 8 + i % zeros] = make_uint4(0, 0, 0, 0);
+      constexpr uint32_t kChunks = 2 + kBBytes / kChunkBytes;
+#pragma unroll
+      for (uint32_t chunk = 0; chunk < kChunks; ++chunk) {
+        const uint32_t at =
+            peer_addr(chunk < 2 ? a + chunk * kChunkBytes : b + (chunk - 2) * kChunkBytes, cta) + t.tail % kStepK * 128;
+        for (int i = lane; ok && i < zeros; i += 32) pair_store_zeros(at + 16 * i);
       }
-      fence_proxy_async_smem();
+      fence_proxy_async();
       __syncwarp();
-      if (lane == 0) pair_arrive_release(peer_addr(&c->full[st], 0));
+      if (ok && lane == 0) mbar_arrive(&c->full[st]);
     }
   } else if (warp >= 4) {
     // -------------------------------------------------------------- results

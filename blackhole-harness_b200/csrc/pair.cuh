@@ -42,22 +42,8 @@ __device__ __forceinline__ uint32_t peer_addr(const void* p, uint32_t rank) {
 }
 // Arrivals on a barrier of either CTA.  A release at cluster scope makes the
 // hardware wait for all of this thread's memory operations (about 0.5 us in a loop
-// that loads), so the loops use relaxed forms, which publish no write of this thread:
-// byte counts of loads, accumulators read.  pair_arrive_release publishes writes to
-// this CTA's shared memory (once a group: its zeroed rows) to the thread of either CTA
-// that waits and then calls pair_acquire; the writes themselves pass fence.proxy.async
-// first, as the pair's tensor cores read them.
-__device__ __forceinline__ void pair_arrive_release(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// After a wait for the phase of this parity: sees what was released to the barrier by either CTA.
-__device__ __forceinline__ void pair_acquire(uint64_t* bar, uint32_t parity) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%0], %1;\n\t}" ::"r"(smem_u32(bar)),
-      "r"(parity)
-      : "memory");
-}
+// that loads), so these are relaxed and publish no write of this thread: byte
+// counts of loads, accumulators read.
 __device__ __forceinline__ void pair_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -65,6 +51,12 @@ __device__ __forceinline__ void pair_arrive_expect_tx(uint32_t bar, uint32_t byt
   asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                : "memory");
 }
+// 16 bytes of zeros at a shared-memory address of either CTA.
+__device__ __forceinline__ void pair_store_zeros(uint32_t addr) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(addr), "r"(0) : "memory");
+}
+// This thread's writes to shared memory, of either CTA, come before what async operations read after it.
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async;" ::: "memory"); }
 // Box loads into this CTA's shared memory that complete on `bar`, a cluster
 // address: this CTA's barrier or the other CTA's.
 __device__ __forceinline__ void pair_load_2d(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y) {

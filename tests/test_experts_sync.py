@@ -30,10 +30,10 @@ def test_a_warp_gives_up_as_one():
 
 
 def test_a_kernel_that_gives_up_waits_for_its_copies():
-    """After a wait that ran out no CTA may leave while copies still land in its shared memory: the leader waits
-    for the steps of both CTAs, each CTA for the tails, which complete on barriers of its own."""
+    """After a wait that ran out neither CTA may leave while copies still land in its shared memory: the leader, on whose
+    barriers both CTAs' copies complete, waits for the steps and for the tails."""
     text = "\n".join(kernel_lines())
-    for barrier, guard in (("full", r"\*abort && lane == 0 && leader"), ("tail", r"\*abort && lane == 0\)")):
+    for barrier, guard in (("full", r"\*abort && lane == 0 && leader"), ("tail", r"\*abort && lane == 0 && leader")):
         assert re.search(guard + r"[^}]*mbar_wait\(&c->" + barrier + r"\[[^}]*&ignore", text), barrier
 
 
@@ -45,12 +45,12 @@ def test_shared_arrays_read_as_words_are_aligned():
             assert "__align__(16)" in line, line
 
 
-def test_zeroed_rows_are_published_to_the_pair():
-    """The rows that one CTA clears are read by a product that the other issues: released and acquired at the
-    scope of both."""
+def test_zeroed_rows_are_published_to_the_product():
+    """The rows that are cleared are read by a product that the leader issues.  No arrival here releases to the other CTA,
+    so the leader's warps clear them in both, behind copies that complete in the leader, and arrive in the leader."""
     text = "\n".join(kernel_lines())
-    helper = (CSRC / "pair.cuh").read_text()
-    assert "mbarrier.arrive.release.cluster" in helper.split("void pair_arrive_release(")[1][:200]
-    assert ".acquire.cluster" in helper.split("void pair_acquire(")[1][:250]
-    assert re.search(r"fence_proxy_async_smem\(\);\s*__syncwarp\(\);\s*if \(lane == 0\) pair_arrive_release", text)
-    assert re.search(r"warp_wait\(&c->full\[st\][^;]*;\s*if \(MODE >= kWgrad && ok && last && t.tail % 16 != 0\) pair_acquire", text)
+    assert ".release.cluster" not in (CSRC / "pair.cuh").read_text().split("cluster_sync")[1].split("}", 1)[1]
+    assert re.search(r"peer_addr\(fix \? &c->tail\[st\] : &c->full\[st\], 0\)", text)
+    role = text[text.index("(warp == 2 || warp == 3) && MODE >= kWgrad && leader"):text.index("warp >= 4")]
+    assert re.search(r"warp_wait\(&c->tail\[st\].*pair_store_zeros.*fence_proxy_async\(\);\s*__syncwarp\(\);\s*"
+                     r"if \(ok && lane == 0\) mbar_arrive\(&c->full\[st\]\)", role, re.S)
