@@ -870,7 +870,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     // ---------------------------------------------------------------- tails
     // A warp for each CTA's shared memory, both in the leader: what they clear reaches the products by way of an
     // arrival in their own CTA.  A warp in either CTA would have to release to the other (96 x 1536 x 2048, 341 rows: 235
-    // us against 218; without clearing anything 204).
+    // us against 214, or 219 with the wide fence in both; without clearing anything 205, mostly for want of the fence).
     const uint32_t cta = warp - 2;
     uint32_t it = 0;
     int uses = 0;   // lane s: how many tails stage s has held
@@ -892,7 +892,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             peer_addr(chunk < 2 ? a + chunk * kChunkBytes : b + (chunk - 2) * kChunkBytes, cta) + t.tail % kStepK * 128;
         for (int i = lane; ok && i < zeros; i += 32) pair_store_zeros(at + 16 * i);
       }
-      fence_proxy_async();
+      if (cta == 0) fence_proxy_async_smem();
+      else fence_proxy_async();
       __syncwarp();
       if (ok && lane == 0) mbar_arrive(&c->full[st]);
     }

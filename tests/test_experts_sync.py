@@ -52,5 +52,5 @@ def test_zeroed_rows_are_published_to_the_product():
     assert ".release.cluster" not in (CSRC / "pair.cuh").read_text().split("cluster_sync")[1].split("}", 1)[1]
     assert re.search(r"peer_addr\(fix \? &c->tail\[st\] : &c->full\[st\], 0\)", text)
     role = text[text.index("(warp == 2 || warp == 3) && MODE >= kWgrad && leader"):text.index("warp >= 4")]
-    assert re.search(r"warp_wait\(&c->tail\[st\].*pair_store_zeros.*fence_proxy_async\(\);\s*__syncwarp\(\);\s*"
-                     r"if \(ok && lane == 0\) mbar_arrive\(&c->full\[st\]\)", role, re.S)
+    assert re.search(r"warp_wait\(&c->tail\[st\].*pair_store_zeros.*if \(cta == 0\) fence_proxy_async_smem\(\);\s*"
+                     r"else fence_proxy_async\(\);\s*__syncwarp\(\);\s*if \(ok && lane == 0\) mbar_arrive\(&c->full\[st\]\)", role, re.S)
