@@ -363,10 +363,11 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 // (weight gradient, the leader's), 4..11 write results.  Each walks the groups' offsets by
 // itself, so that no size is known on the host.
 //
-// Measured, bf16, 96 experts, 1536 x 2048: 512 rows 91 us (HBM, 6.7 TB/s); 32768 rows
-// 174..186 us (1110..1180 TFLOP/s; HBM and tensor cores, each of which alone takes
-// 145); the weight gradient of those 194..207 us (604 MB written, which takes a
-// plain fill 157).  A single product of 8192 x 8192 x 2048: 174 us (1580 TFLOP/s).
+// Measured, bf16, 96 experts, 1536 x 2048, a call at a time and (in brackets) back to back, where the power cap
+// lowers the clock at the same number of cycles: 512 rows 91..93 us (93: HBM, 6.5 TB/s); 32768 rows 174..178 us
+// (206..228 at 1.12 GHz; HBM and tensor cores, each of which alone takes 145); the weight gradient of those 203..209 us
+// (229..260 at 1.27 GHz; tensor cores 52 % busy, 604 MB written, which takes a plain fill 157).  A single product of
+// 8192 x 8192 x 2048: 174 us (1580 TFLOP/s).
 constexpr int kMaxStages = 6;
 constexpr int kStepK = 64;
 constexpr uint32_t kOperandBytes = 128 * kStepK * 2;   // one operand's share of a CTA and step

@@ -126,8 +126,8 @@ cudaLaunchConfig_t launch_config(dim3 grid, int threads, cudaStream_t st, cudaLa
 // threads take a row (a warp for common widths, a block's 128 for wide rows or
 // few of them, 4 or 8 for narrow ones), so that the sum of dw stays in one
 // thread group and is added in a fixed order; each thread has kUnroll 16-byte
-// loads per operand in flight.  32768 x 768 bf16 with weights: forward 24.2 us (6.24
-// TB/s), backward 41.0 us (6.15 TB/s).
+// loads per operand in flight.  32768 x 768 bf16 with weights: forward 23.6 us (6.4
+// TB/s), backward 40.8 us (6.2 TB/s).
 constexpr int kSwigluThreads = 256;
 // 16-byte pieces a lane has in flight: three cover 768 16-bit values a warp.  With 1, 2, 3, 4 (bf16, forward and
 // backward, us): 32768 x 768: 23.5 + 38.8, 25.5 + 41.9, 24.6 + 41.5, 26.4 + 43.0; 32768 x 96: 8.0 + 12.8, 4.9 + 7.2, 4.6
