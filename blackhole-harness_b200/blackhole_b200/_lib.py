@@ -14,8 +14,9 @@ from pathlib import Path
 LIB_PATH = Path(__file__).resolve().parent / "libhexmoe.so"
 
 HEXMOE_OK, HEXMOE_E_ARG, HEXMOE_E_DTYPE, HEXMOE_E_CUDA, HEXMOE_E_UNSUPPORTED, HEXMOE_E_DEVICE = range(6)
-F32, BF16, F16 = 0, 1, 2
+F32, BF16, F16, I8 = 0, 1, 2, 3
 I32, I64 = 0, 1
+SOFTMAX, SIGMOID = 0, 1
 MAX_TIERS = 4
 NOALLOC_SCRATCH_BYTES = 32 << 20   # HEXMOE_NOALLOC_SCRATCH_BYTES in include/hexmoe.h
 
@@ -30,7 +31,9 @@ EXPORTS = (
     "hexmoe_quantize_workspace_bytes", "hexmoe_quantize",
     "hexmoe_group_offsets", "hexmoe_grouped_mm_workspace_bytes", "hexmoe_grouped_mm",
     "hexmoe_grouped_wgrad_workspace_bytes", "hexmoe_grouped_wgrad", "hexmoe_swiglu", "hexmoe_swiglu_backward",
-    "hexmoe_clip_grad_norm_workspace_bytes", "hexmoe_clip_grad_norm",
+    "hexmoe_clip_grad_norm_workspace_bytes", "hexmoe_clip_grad_norm", "hexmoe_route", "hexmoe_route_backward",
+    "hexmoe_quantize_rows", "hexmoe_grouped_mm_int8_workspace_bytes", "hexmoe_grouped_mm_int8",
+    "hexmoe_int8_forward_workspace_bytes", "hexmoe_int8_forward",
 )
 EP_MAX_WORLD = 8          # HEXMOE_EP_MAX_WORLD
 EP_HANDLE_BYTES = 64      # HEXMOE_EP_HANDLE_BYTES
@@ -103,6 +106,17 @@ def _load() -> ctypes.CDLL:
         "hexmoe_swiglu_backward": (ctypes.c_int, [P, I64_, P, I64_, I32_, I64_, I32_, P, P, I64_, P, P]),
         "hexmoe_clip_grad_norm_workspace_bytes": (SZ, [I32_]),
         "hexmoe_clip_grad_norm": (ctypes.c_int, [I32_, P, P, P, P, P, ctypes.c_float, I32_, P, P, SZ, P]),
+        "hexmoe_route": (ctypes.c_int, [P, I32_, I64_, I64_, I32_, I32_, I32_, P, I32_, I32_, I32_, I32_, ctypes.c_float,
+                                        P, P, P]),
+        "hexmoe_route_backward": (ctypes.c_int, [P, P, I32_, I64_, I64_, I32_, I32_, P, I32_, I32_, I32_, ctypes.c_float,
+                                                 P, I64_, P]),
+        "hexmoe_quantize_rows": (ctypes.c_int, [P, I32_, I64_, I64_, I32_, P, I64_, P, P]),
+        "hexmoe_grouped_mm_int8_workspace_bytes": (SZ, [I64_, I32_, I32_, I32_, I32_]),
+        "hexmoe_grouped_mm_int8": (ctypes.c_int, [P, I32_, I64_, P, P, I64_, I64_, P, I64_, I32_, I32_, I32_, P, I32_, P,
+                                                  I64_, I32_, P, SZ, P]),
+        "hexmoe_int8_forward_workspace_bytes": (SZ, [I64_, I32_, I32_, I32_, I32_]),
+        "hexmoe_int8_forward": (ctypes.c_int, [P, I32_, I64_, I64_, I32_, I32_, I32_, P, P, I32_, I32_, P, I64_, I64_, P,
+                                               P, I64_, I64_, P, P, I32_, P, SZ, P]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)

@@ -30,13 +30,14 @@ int arg_error(const char* fmt, ...) {
 // and to no less than the one before, so that whatever the array holds the
 // groups are disjoint row ranges.  `bad` says that something was clamped.
 struct Groups {
-  const void* offsets;   // int32 or int64 [experts + 1]
+  const void* offsets;   // int32 or int64 [experts + 1]; null (8-bit products): one group of all rows
   int32_t is64;
   int32_t experts;
   int64_t rows;
 };
 
 __device__ __forceinline__ int64_t raw_offset(const Groups& g, int e) {
+  if (!g.offsets) return e ? g.rows : 0;
   return g.is64 ? static_cast<const int64_t*>(g.offsets)[e] : static_cast<const int32_t*>(g.offsets)[e];
 }
 
@@ -380,7 +381,11 @@ constexpr uint32_t kRingBytes = 200 * 1024;            // 6 steps of A and B, 4 
 constexpr uint32_t kPairSmem = 1024 + kRingBytes + kWriters * kStoreBytes + 1024;
 constexpr int kBoxes = 4;                              // row boxes of 16, 32, 64, 128
 
-enum PairMode { kRowsK = 0, kRowsMN = 1, kWgrad = 2, kWgradT = 3 };   // kWgradT: M side k, N side n
+// kInt8: y = x W^T of 8-bit integers with scales; kInt8Glu: SwiGLU of such products with gate and up rows; kWgradT: M
+// side k, N side n.
+enum PairMode { kRowsK = 0, kRowsMN = 1, kInt8 = 2, kInt8Glu = 3, kWgrad = 4, kWgradT = 5 };
+constexpr bool is_int8(int mode) { return mode == kInt8 || mode == kInt8Glu; }
+constexpr bool k_major(int mode) { return mode == kRowsK || is_int8(mode); }   // the matrix as it lies is reduction-major
 
 // Shapes of a tile's N side and of the ring that fits it.
 //   kOne     up to 256 columns: 6 steps of 32 KB
@@ -403,7 +408,10 @@ struct PairParams {
   Groups g;
   int32_t m_len;             // M side: output features; weight gradient: n, or k in kWgradT
   int32_t n_len;             // weight gradient: k, or n in kWgradT
-  int32_t red;               // row products: reduction length
+  int32_t red;               // row products: reduction length (8-bit: in pairs)
+  int32_t out_len;           // row products: columns of the result
+  const float* x_scale;      // 8-bit products: [rows]
+  const float* w_scale;      // [experts, matrix rows]
   int32_t m_tiles, n_tiles, tile_n;   // n_tiles, tile_n: weight gradient
   int32_t splits;            // runs that the reduction of a tile is cut into, over several pairs
   int32_t run;               // RUNS: most steps that one accumulator sums
@@ -530,6 +538,40 @@ struct Writer {
   int32_t e = 0, m = 0, cols = 0;   // which result (expert, run of the reduction); first M row; columns there are
   bool add = false;                 // to what is there
   int64_t n0 = 0;                   // column 0 in the output: row products: its row; weight gradient: its column
+  float w_scale = 0.f;              // 8-bit products: of this lane's matrix row
+
+  // The lane's matrix row is one of the tile's: kInt8 in order, kInt8Glu 8 of gate, the 8 of up.
+  __device__ __forceinline__ void load_w_scale(int32_t expert) {
+    if constexpr (MODE == kInt8) {
+      w_scale = m + lane < p.m_len ? p.w_scale[static_cast<int64_t>(expert) * p.m_len + m + lane] : 0.f;
+    } else if constexpr (MODE == kInt8Glu) {
+      const int32_t f = m / 2 + lane / 16 * 8 + lane % 8;
+      w_scale = f < p.out_len ? p.w_scale[static_cast<int64_t>(expert) * p.m_len + (lane % 16 < 8 ? 0 : p.out_len) + f] : 0.f;
+    }
+  }
+  // The scale of row `col + lane` of the tile, read while the accumulator is.
+  __device__ __forceinline__ float load_x_scale(int32_t col) const {
+    if constexpr (is_int8(MODE)) return col + lane < cols ? p.x_scale[n0 + col + lane] : 0.f;
+    return 0.f;
+  }
+  // int32 sums as scaled f32 values, in place.  Fragments: register 16 h + 4 i + 2 b + c is matrix row 16 h + 8 b + g
+  // and tile row 8 i + 2 q + c.
+  __device__ __forceinline__ void scale_fragments(uint32_t (&r)[32], float x) const {
+    const int g = lane / 4, q = lane % 4;
+    float ws[4], xs[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ws[i] = __shfl_sync(0xffffffffu, w_scale, g + 8 * i);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) xs[i] = __shfl_sync(0xffffffffu, x, i / 2 * 8 + 2 * q + i % 2);
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      r[j] = __float_as_uint(static_cast<float>(static_cast<int32_t>(r[j])) * (ws[j / 16 * 2 + j / 2 % 2] * xs[j / 4 % 4 * 2 + j % 2]));
+  }
+  __device__ __forceinline__ void scale_columns(uint32_t (&r)[32], float x) const {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      r[j] = __float_as_uint(static_cast<float>(static_cast<int32_t>(r[j])) * (w_scale * __shfl_sync(0xffffffffu, x, j)));
+  }
 
   // An f32 result, or its addition without waiting for what is there.  Each value has one writer, whose additions
   // to an address keep their order.
@@ -545,15 +587,20 @@ struct Writer {
   __device__ __forceinline__ bool f32() const { return RUNS || p.f32; }
   // Row products that leave by TMA take fragments, everything else a row of 32 columns a lane.
   __device__ __forceinline__ void load(uint32_t acc, uint32_t (&r)[32]) const {
-    if (MODE != kWgrad && p.tma_out && (MODE < kWgrad || !f32())) {
+    if (MODE == kInt8Glu || (MODE != kWgrad && p.tma_out && (MODE < kWgrad || !f32()))) {
       tmem_ld_fragments<0>(acc, r);
       tmem_ld_fragments<16>(acc + (16u << 16), r);
     } else {
       tmem_ld32(acc, r);
     }
   }
-  __device__ __forceinline__ void write(int32_t col, uint32_t (&r)[32]) {
+  __device__ __forceinline__ void write(int32_t col, uint32_t (&r)[32], float x) {
+    if constexpr (MODE == kInt8) {
+      if (p.tma_out) scale_fragments(r, x);
+      else scale_columns(r, x);
+    }
     if constexpr (MODE == kWgrad) write_gradient(col, r);
+    else if constexpr (MODE == kInt8Glu) write_glu(col, r, x);
     else if (MODE == kWgradT && p.tma_out && f32()) write_lines(col, r);
     else if (p.tma_out) write_rows(col, r);
     else write_elements(col, r);
@@ -588,6 +635,42 @@ struct Writer {
         const int line = 8 * i + lane / 4, q = lane % 4;
         const uint4 v = *reinterpret_cast<const uint4*>(stage + line * 64 + ((q ^ (line >> 1 & 3)) << 4));
         if (line < rows) store_8(dst + line * p.ld + q * 8, v, p.m_len - m - q * 8);
+      }
+      __syncwarp();
+    }
+  }
+
+  // silu(gate) up of the scaled products, f32: 16 features of 32 rows, lines of 64 bytes, stored by TMA where the
+  // rows are all the group's.  (The next product's rows are quantized from these values: rounded to 16 bits here they would land on
+  // other whole numbers often enough to double the layer's error.)
+  __device__ __forceinline__ void write_glu(int32_t col, uint32_t (&r)[32], float x) {
+    scale_fragments(r, x);
+    const int32_t rows = min(32, cols - col), f = m / 2;
+    const int g = lane / 4, q = lane % 4;
+    stage_free();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {   // j = 8 h + 2 i + c
+      const int h = j / 8, line = j % 8 / 2 * 8 + 2 * q + j % 2, at = 16 * h + j % 8 / 2 * 4 + j % 2;
+      const float gate = __uint_as_float(r[at]), up = __uint_as_float(r[at + 2]);
+      const float act = gate / (1.f + __expf(-gate)) * up;
+      const int feature = 8 * h + g;
+      *reinterpret_cast<float*>(stage + line * 64 + ((feature / 4 ^ (line >> 1 & 3)) << 4) + feature % 4 * 4) = act;
+    }
+    if (rows == 32) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (elect_one()) {
+        tma_store_2d(&p.out, stage, f, static_cast<int32_t>(n0) + col);
+        bulk_commit();
+      }
+    } else {   // the group's last rows: the next ones are another group's
+      __syncwarp();
+      float* dst = static_cast<float*>(p.dst) + (n0 + col) * p.ld + f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int line = 8 * i + lane / 4;
+        const float4 v = *reinterpret_cast<const float4*>(stage + line * 64 + ((q ^ (line >> 1 & 3)) << 4));
+        if (line < rows) *reinterpret_cast<float4*>(dst + line * p.ld + q * 4) = v;
       }
       __syncwarp();
     }
@@ -767,6 +850,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             const int32_t r = ((t.first + s) * kSubs + sub) * kStepK;   // where the block begins in the reduction
             if constexpr (MODE == kRowsK) {
               pair_load_3d(a, &p.a, bar, r, m, t.e);
+            } else if constexpr (MODE == kInt8) {
+              pair_load_3d(a, &p.a, bar, 2 * r, m, t.e);
+            } else if constexpr (MODE == kInt8Glu) {   // 8 rows of gate, the 8 of up, and so on
+              pair_load_5d(a, &p.a, bar, 2 * r, 0, 0, m / 16, t.e);
             } else if constexpr (MODE == kRowsMN) {
               pair_load_3d(a, &p.a, bar, m, r, t.e);
               pair_load_3d(a + kChunkBytes, &p.a, bar, m + 64, r, t.e);
@@ -789,7 +876,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
 #pragma unroll
                 for (int i = kBoxes - 1; i >= 0; --i) {   // the rows' number in boxes of 128, 64, 32, 16
                   if (half & (16 << i)) {
-                    pair_load_2d(to, &p.b[i], bar, r, y);
+                    pair_load_2d(to, &p.b[i], bar, is_int8(MODE) ? 2 * r : r, y);
                     to += (16 << i) * kStepK * 2;
                     y += 16 << i;
                   }
@@ -829,15 +916,17 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     bool ok = true;
     for (int32_t tile = first; ok && walk.next(p, tile, stride, t);) {
       if (t.steps == 0) continue;   // an empty group's gradient: zeros, without an accumulator
-      constexpr uint32_t kMajors = (MODE != kRowsK ? kIdescMajorA : 0) | (MODE >= kWgrad ? kIdescMajorB : 0);
-      const uint32_t idescs[2] = {umma_idesc(p.bf16, 256, t.columns(0)) | kMajors,
-                                  WIDE && t.parts > 1 ? umma_idesc(p.bf16, 256, t.columns(1)) | kMajors : 0};
+      constexpr uint32_t kMajors = (!k_major(MODE) ? kIdescMajorA : 0) | (MODE >= kWgrad ? kIdescMajorB : 0);
+      auto idesc = [&](int32_t columns) {
+        return is_int8(MODE) ? umma_idesc_i8(256, columns) : umma_idesc(p.bf16, 256, columns) | kMajors;
+      };
+      const uint32_t idescs[2] = {idesc(t.columns(0)), WIDE && t.parts > 1 ? idesc(t.columns(1)) : 0};
       for (int32_t s = 0; ok && s < t.steps; ++s) {
         const bool last = s + 1 == t.steps;
         ok = warp_wait(&c->full[st], phase, abort, p.dev_err);
         const uint32_t a = smem_u32(ring + st * kStageBytes);
-        const uint64_t da = MODE == kRowsK ? sw128_desc(a) : sw128_mn_desc(a, kChunkBytes);
-        const int count = last && t.tail ? (t.tail + 15) / 16 : kSubs * kStepK / 16;   // products of 16
+        const uint64_t da = k_major(MODE) ? sw128_desc(a) : sw128_mn_desc(a, kChunkBytes);
+        const int count = last && t.tail ? (t.tail + 15) / 16 : kSubs * kStepK / 16;   // products of 16 (8-bit: 32)
 #pragma unroll
         for (int part = 0; part < (WIDE ? 2 : 1); ++part) {
           if (part >= t.parts) break;
@@ -850,9 +939,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < kSubs * kStepK / 16; ++k)   // the next 64-wide block of an operand: its bytes / 16 on
-              if (k < count)
-                pair_umma_f16(acc, da + k % 4 * (MODE == kRowsK ? 2 : 128) + k / 4 * (kOperandBytes >> 4),
-                              db + k % 4 * (MODE >= kWgrad ? 128 : 2) + k / 4 * (kBBytes >> 4), idescs[part], s | k);
+              if (k < count) {
+                const uint64_t ka = da + k % 4 * (k_major(MODE) ? 2 : 128) + k / 4 * (kOperandBytes >> 4);
+                const uint64_t kb = db + k % 4 * (MODE >= kWgrad ? 128 : 2) + k / 4 * (kBBytes >> 4);
+                if constexpr (is_int8(MODE)) pair_umma_i8(acc, ka, kb, idescs[part], s | k);
+                else pair_umma_f16(acc, ka, kb, idescs[part], s | k);
+              }
             if (part + 1 == t.parts) pair_umma_commit(&c->empty[st]);
             if (last) pair_umma_commit(&c->acc_full[buf]);
           }
@@ -908,6 +1000,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       out.e = MODE >= kWgrad ? t.split * p.g.experts + t.e : t.split;
       out.m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
       out.add = p.accumulate || (RUNS && t.add);
+      if constexpr (is_int8(MODE)) out.load_w_scale(t.e);
       if (RUNS && t.add && p.tma_out) {   // the stores of the run before have arrived: additions to the same values stay in order
         if (elect_one()) bulk_wait_all();
         __syncwarp();
@@ -923,11 +1016,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           for (int i = 0; i < chunks; ++i) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) r0[j] = 0;
-            out.write(part * 32 + 64 * i, r0);
+            out.write(part * 32 + 64 * i, r0, 0.f);
           }
           continue;
         }
         const uint32_t buf = n % 2, acc = tmem + buf * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16) + part * 32;
+        float x0 = out.load_x_scale(part * 32);   // read while the products run
         ok = warp_wait(&c->acc_full[buf], (n / 2) & 1, abort, p.dev_err);
         if (!ok) break;
         tc_fence_after();
@@ -938,18 +1032,21 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           __syncwarp();
           if (lane == 0) pair_arrive(peer_addr(&c->acc_empty[buf], 0));
         };
+        const int32_t col = part * 32;
         if (chunks == 0) release();
         else out.load(acc, r0);
         for (int i = 0; i < chunks; i += 2) {
           tmem_ld_wait_for(r0);
+          const float x1 = i + 1 < chunks ? out.load_x_scale(col + 64 * (i + 1)) : 0.f;
           if (i + 1 < chunks) out.load(acc + 64 * (i + 1), r1);
           else release();
-          out.write(part * 32 + 64 * i, r0);
+          out.write(col + 64 * i, r0, x0);
           if (i + 1 == chunks) break;
           tmem_ld_wait_for(r1);
+          x0 = i + 2 < chunks ? out.load_x_scale(col + 64 * (i + 2)) : 0.f;
           if (i + 2 < chunks) out.load(acc + 64 * (i + 2), r0);
           else release();
-          out.write(part * 32 + 64 * (i + 1), r1);
+          out.write(col + 64 * (i + 1), r1, x1);
         }
       }
     }
@@ -958,7 +1055,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       const int64_t gap = walk.lo + (p.g.rows - walk.carry);
       for (int64_t j = blockIdx.x; j < gap * p.splits; j += gridDim.x) {
         const int64_t i = j % gap, at = j / gap * p.stride_split + (i < walk.lo ? i : i - walk.lo + walk.carry) * p.ld;
-        for (int32_t f = threadIdx.x - 128; f < p.m_len; f += kWriters * 32) {
+        for (int32_t f = threadIdx.x - 128; f < p.out_len; f += kWriters * 32) {
           if (p.f32) static_cast<float*>(p.dst)[at + f] = 0.f;
           else static_cast<uint16_t*>(p.dst)[at + f] = 0;
         }
@@ -984,15 +1081,11 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// [outer][rows][cols] with row pitch and outer stride in bytes (dims = 2 leaves
-// the outer one away).
-int make_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int dims, uint64_t cols, uint64_t rows,
-             uint64_t outer, uint64_t pitch, uint64_t stride, uint32_t box_cols, uint32_t box_rows,
-             CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+int encode_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int dims, const cuuint64_t* size,
+               const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
   auto fn = encode_fn();
   if (!fn) return report_error(HEXMOE_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-  const cuuint64_t size[3] = {cols, rows, outer}, strides[2] = {pitch, stride};
-  const cuuint32_t box[3] = {box_cols, box_rows, 1}, step[3] = {1, 1, 1};
+  const cuuint32_t step[5] = {1, 1, 1, 1, 1};
   auto encode = [&] {
     return fn(m, dt, dims, const_cast<void*>(base), size, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -1008,6 +1101,16 @@ int make_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int dims,
   return report_error(HEXMOE_E_CUDA, buf);
 }
 
+// [outer][rows][cols] with row pitch and outer stride in bytes (dims = 2 leaves
+// the outer one away).
+int make_map(CUtensorMap* m, const void* base, CUtensorMapDataType dt, int dims, uint64_t cols, uint64_t rows,
+             uint64_t outer, uint64_t pitch, uint64_t stride, uint32_t box_cols, uint32_t box_rows,
+             CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
+  const cuuint64_t size[3] = {cols, rows, outer}, strides[2] = {pitch, stride};
+  const cuuint32_t box[3] = {box_cols, box_rows, 1};
+  return encode_map(m, base, dt, dims, size, strides, box, swizzle);
+}
+
 // Whether TMA can address a matrix: base and strides in multiples of 16 bytes.
 bool tma_rows(const void* p, int64_t ld, int64_t size) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld * size % 16 == 0 && ld * size < (1ll << 40);
@@ -1021,6 +1124,8 @@ bool tma_stack(const void* p, int64_t ld, int64_t stride, int64_t size, int32_t 
   reinterpret_cast<const void*>(grouped_pair_kernel<MODE, SHAPE, false>), \
       reinterpret_cast<const void*>(grouped_pair_kernel<MODE, SHAPE, true>)
 
+#define INT8_KERNEL(MODE, SHAPE) reinterpret_cast<const void*>(grouped_pair_kernel<MODE, SHAPE, false>)
+
 int sm_count(int* sms) {
   static std::atomic<int> cached[64] = {};
   int dev = 0;
@@ -1032,7 +1137,10 @@ int sm_count(int* sms) {
     for (const void* k : {PAIR_KERNELS(kRowsK, kOne), PAIR_KERNELS(kRowsK, kTwo), PAIR_KERNELS(kRowsK, kNarrow),
                           PAIR_KERNELS(kRowsK, kMiddle), PAIR_KERNELS(kRowsMN, kOne), PAIR_KERNELS(kRowsMN, kTwo),
                           PAIR_KERNELS(kRowsMN, kNarrow), PAIR_KERNELS(kRowsMN, kMiddle), PAIR_KERNELS(kWgrad, kOne),
-                          PAIR_KERNELS(kWgrad, kMiddle), PAIR_KERNELS(kWgradT, kOne), PAIR_KERNELS(kWgradT, kMiddle)}) {
+                          PAIR_KERNELS(kWgrad, kMiddle), PAIR_KERNELS(kWgradT, kOne), PAIR_KERNELS(kWgradT, kMiddle),
+                          INT8_KERNEL(kInt8, kOne), INT8_KERNEL(kInt8, kTwo), INT8_KERNEL(kInt8, kNarrow),
+                          INT8_KERNEL(kInt8, kMiddle), INT8_KERNEL(kInt8Glu, kOne), INT8_KERNEL(kInt8Glu, kTwo),
+                          INT8_KERNEL(kInt8Glu, kNarrow), INT8_KERNEL(kInt8Glu, kMiddle)}) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
       if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
     }
@@ -1056,8 +1164,9 @@ cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return p.run ? cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, SHAPE, true>, p)
-               : cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, SHAPE, false>, p);
+  if constexpr (!is_int8(MODE))   // 8-bit products are summed exactly, however many
+    if (p.run) return cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, SHAPE, true>, p);
+  return cudaLaunchKernelEx(&cfg, grouped_pair_kernel<MODE, SHAPE, false>, p);
 }
 
 // ------------------------------------------------------------------- splits
@@ -1220,7 +1329,91 @@ int check_groups(const char* what, int64_t rows, int32_t experts, const void* of
 bool is16(int32_t dt) { return dt == HEXMOE_BF16 || dt == HEXMOE_F16; }
 bool off_by(const void* p, size_t z) { return reinterpret_cast<uintptr_t>(p) % z != 0; }
 
+// The tensor map of [gate | up] matrices as the SwiGLU product reads them: 128 bytes of the reduction of 8 gate rows, the 8
+// up rows of the same features, the next 8 gate rows ...  In an accumulator's 16-lane fragments gate and up of a feature
+// then are registers of one thread.
+int make_glu_map(CUtensorMap* m, const int8_t* w, int64_t k, int64_t inter, int64_t experts, int64_t ld, int64_t stride) {
+  const cuuint64_t size[5] = {static_cast<cuuint64_t>(k), 8, 2, static_cast<cuuint64_t>(inter / 8), static_cast<cuuint64_t>(experts)};
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(ld), static_cast<cuuint64_t>(inter * ld), static_cast<cuuint64_t>(8 * ld),
+                                 static_cast<cuuint64_t>(stride)};
+  const cuuint32_t box[5] = {128, 8, 2, 8, 1};
+  return encode_map(m, w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, size, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 }  // namespace
+
+size_t int8_partial_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k) {
+  const int splits = rows_splits(rows, experts, n, (k + 1) / 2);
+  return splits > 1 ? splits * rows * pitch4(n) * sizeof(float) : 0;
+}
+
+bool int8_rows(const void* p, int64_t ld) { return tma_rows(p, ld, 1); }
+bool int8_stack(const void* p, int64_t ld, int64_t stride, int32_t count) { return tma_stack(p, ld, stride, 1, count); }
+
+int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
+  int32_t* dev_err = device_error_word();
+  if (!dev_err) return report_error(HEXMOE_E_CUDA, "device error word unavailable");
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  PairParams q{};
+  q.g = {d.offsets, d.offsets64, d.experts, d.rows};
+  q.m_len = d.n;
+  q.out_len = d.glu ? d.n / 2 : d.n;
+  q.red = (d.k + 1) / 2;
+  q.m_tiles = (d.n + 255) / 256;
+  q.x_scale = d.x_scale;
+  q.w_scale = d.w_scale;
+  q.splits = d.glu ? 1 : rows_splits(d.rows, d.experts, d.n, q.red);
+  const int64_t pitch = pitch4(d.n);
+  if (d.workspace_bytes < q.splits * d.rows * pitch * sizeof(float) || !d.workspace) q.splits = 1;
+  const bool split = q.splits > 1, f32 = d.out_dtype == HEXMOE_F32, bf16 = d.out_dtype == HEXMOE_BF16;
+  q.dst = split ? d.workspace : d.out;
+  q.ld = split ? pitch : d.ld_out;
+  q.stride_split = d.rows * pitch;
+  q.f32 = split || f32; q.bf16 = bf16;
+  q.dev_err = dev_err;
+  const PairShape shape = rows_shape(d.rows, d.experts, d.n);
+  const int64_t tiles = row_tiles(d.rows, d.experts, d.n, shape) * q.splits;
+  if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
+  constexpr CUtensorMapDataType kBytes = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  if (int rc = d.glu ? make_glu_map(&q.a, d.w, d.k, q.out_len, d.experts, d.ld_w, d.experts == 1 ? d.ld_w : d.stride_w)
+                     : make_map(&q.a, d.w, kBytes, 3, d.k, d.n, d.experts, d.ld_w, d.experts == 1 ? d.ld_w : d.stride_w, 128, 128))
+    return rc;
+  const int64_t half = (std::min<int64_t>(d.rows, 256) + 31) / 32 * 16;
+  for (int i = 0; i < kBoxes && 16 << i <= half; ++i)
+    if (int rc = make_map(&q.b[i], d.x, kBytes, 2, d.k, d.rows, 1, d.ld_x, 0, 128, 16u << i)) return rc;
+  if (d.glu) {
+    q.tma_out = 1;
+    if (d.rows >= 32)
+      if (int rc = make_map(&q.out, d.out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, q.out_len, d.rows, 1, 4 * d.ld_out, 0, 16, 32,
+                            CU_TENSOR_MAP_SWIZZLE_64B))
+        return rc;
+  } else {
+    q.tma_out = !q.f32 && tma_rows(d.out, d.ld_out, 2) && d.n % 8 == 0;
+    if (q.tma_out && d.rows >= 32)
+      if (int rc = make_map(&q.out, d.out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, d.n,
+                            d.rows, 1, 2 * d.ld_out, 0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
+        return rc;
+  }
+  auto launch = [&](auto mode) {
+    constexpr int MODE = decltype(mode)::value;
+    return shape == kNarrow   ? launch_pair<MODE, kNarrow>(q, tiles, sms, st)
+           : shape == kMiddle ? launch_pair<MODE, kMiddle>(q, tiles, sms, st)
+           : shape == kTwo    ? launch_pair<MODE, kTwo>(q, tiles, sms, st)
+                              : launch_pair<MODE, kOne>(q, tiles, sms, st);
+  };
+  cudaError_t e = d.glu ? launch(std::integral_constant<int, kInt8Glu>{}) : launch(std::integral_constant<int, kInt8>{});
+  if (e == cudaSuccess && split) {
+    JoinParams j{};
+    j.part = static_cast<const float*>(d.workspace);
+    j.rows = d.rows; j.pitch = pitch; j.splits = q.splits; j.cols = d.n;
+    j.out = d.out; j.ld = d.ld_out; j.inner = static_cast<int32_t>(d.rows);
+    j.f32 = f32; j.bf16 = bf16; j.vec = d.ld_out % 4 == 0 && !off_by(d.out, 8);
+    e = launch_join(j, st);
+  }
+  return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
+}
+
 }  // namespace hexmoe
 
 using namespace hexmoe;
@@ -1285,7 +1478,7 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
     if (int rc = sm_count(&sms)) return rc;
     PairParams q{};
     q.g = groups;
-    q.m_len = width_out; q.red = width_in;
+    q.m_len = q.out_len = width_out; q.red = width_in;
     q.m_tiles = (width_out + 255) / 256;
     q.splits = rows_splits(rows, experts, width_out, width_in);
     const int64_t pitch = pitch4(width_out);

@@ -1,0 +1,521 @@
+// int8.cu — a MoE layer's experts in 8-bit integers: rows quantized with a scale each, the plan that puts
+// routed tokens into expert order, and the layer made of them and the products in grouped.cu.
+#include <algorithm>
+#include <cstdarg>
+#include <cstdio>
+#include <type_traits>
+
+#include <cooperative_groups.h>
+
+#include "internal.cuh"
+#include "ptx.cuh"
+
+namespace hexmoe {
+namespace {
+
+namespace cg = cooperative_groups;
+
+int arg_error(const char* fmt, ...) {
+  char buf[256];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  return report_error(HEXMOE_E_ARG, buf);
+}
+
+constexpr unsigned kAll = 0xffffffffu;
+constexpr int64_t kMaxSum = 131071;   // products of -128 and -128 that an int32 holds
+
+cudaLaunchConfig_t launch_config(dim3 grid, int threads, size_t smem, cudaStream_t st, cudaLaunchAttribute* attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr->val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cfg;
+}
+
+// ------------------------------------------------------------------- rows to 8 bits
+// scale = max |x| / 127, q = round(127 x / max |x|), ties to even, of every row.  The quotient is that of real numbers: it
+// is computed in f32, which is off by less than 2^-16 at 127, and where that leaves a border in doubt, in f64
+// (127 x is exact there, and half a step is met exactly: x = max / 2 is 63.5).  A row of zeros has scale 0; one that holds
+// an infinity or NaN has scale NaN and zeros, so that what is made of it is NaN.
+// Bound by HBM.  TPR threads take a row and keep its first kPieces 16-byte pieces each in registers; what a longer row has
+// behind those is read again.
+constexpr int kRowThreads = 256;
+constexpr int kPieces = 8;
+
+struct RowsParams {
+  const void* x;
+  int64_t ld_x, rows;
+  int32_t cols;
+  int8_t* q;              // [rows, ld_q], or with `places` [places..., ld_q]
+  int64_t ld_q;
+  float* scale;
+  const float* factor;    // [rows], what every scale is multiplied with; or null
+  const int32_t* count;   // on the device: rows that exist, of `rows`; or null
+  // The layer's tokens, each to the rows of its topk slots: slot s has row places[s] (-1: none), and its
+  // routing weight is copied to row_weight.
+  const int32_t* places;
+  int32_t topk;
+  const float* weights;
+  float* row_weight;
+};
+
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& v, float (&x)[16 / sizeof(T)]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same_v<T, float>) {
+      x[i] = __uint_as_float(w[i]);
+    } else if constexpr (std::is_same_v<T, __half>) {
+      x[2 * i] = __half2float(__ushort_as_half(static_cast<uint16_t>(w[i])));
+      x[2 * i + 1] = __half2float(__ushort_as_half(static_cast<uint16_t>(w[i] >> 16)));
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
+// Values a piece: 16 bytes of them, or one (rows that are not aligned to 16 bytes, or of odd lengths).
+template <typename T, bool VEC>
+struct Piece {
+  static constexpr int kValues = VEC ? 16 / sizeof(T) : 1;
+  float x[kValues];
+  __device__ __forceinline__ void load(const T* row, int i) {
+    if constexpr (VEC) {
+      unpack<T>(reinterpret_cast<const uint4*>(row)[i], x);
+    } else {
+      if constexpr (std::is_same_v<T, float>) x[0] = row[i];
+      else if constexpr (std::is_same_v<T, __half>) x[0] = __half2float(row[i]);
+      else x[0] = __bfloat162float(row[i]);
+    }
+  }
+};
+
+struct RowScale {
+  float largest, inverse;
+  bool plain;   // f32 is enough but for borders
+  __device__ __forceinline__ explicit RowScale(uint32_t bits) {
+    largest = __uint_as_float(bits);
+    plain = largest > 1e-30f && largest < 1e30f;
+    inverse = plain ? 127.f / largest : 0.f;
+  }
+  __device__ __forceinline__ bool finite() const { return __float_as_uint(largest) < 0x7f800000u; }
+  __device__ __forceinline__ float scale() const { return finite() ? largest / 127.f : __uint_as_float(0x7fc00000u); }
+  __device__ __forceinline__ int32_t operator()(float x) const {
+    const float t = x * inverse, r = rintf(t);
+    if (plain && fabsf(t - r) < 0.49998f) return static_cast<int32_t>(r);
+    if (!finite() || largest == 0.f) return 0;
+    return static_cast<int32_t>(rint(static_cast<double>(x) * 127.0 / static_cast<double>(largest)));
+  }
+};
+
+template <typename T, bool VEC, int TPR>
+__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsParams p) {
+  using P = Piece<T, VEC>;
+  constexpr int kRows = kRowThreads / TPR, V = P::kValues;
+  __shared__ uint32_t part[kRowThreads / 32];
+  const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + slot;
+  pdl_wait();
+  pdl_launch_dependents();
+  const bool live = row < p.rows && (!p.count || row < *p.count);
+  const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
+  const int n = p.cols / V;
+  P held[kPieces];
+  uint32_t bits = 0;
+  auto see = [&](const P& v) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) bits = max(bits, __float_as_uint(v.x[j]) & 0x7fffffffu);
+  };
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      if (lane + i * TPR < n) held[i].load(x, lane + i * TPR);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      if (lane + i * TPR < n) see(held[i]);
+    for (int c = lane + kPieces * TPR; c < n; c += TPR) {
+      P v;
+      v.load(x, c);
+      see(v);
+    }
+  }
+#pragma unroll
+  for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(kAll, bits, o));
+  if constexpr (TPR > 32) {
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = bits;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < TPR / 32; ++i) bits = max(bits, part[slot * (TPR / 32) + i]);
+  }
+  if (!live) return;
+  const RowScale to(bits);
+  auto write = [&](const P& v, int c) {
+    int32_t q[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) q[j] = to(v.x[j]);
+    uint32_t w[2] = {};
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[j / 4] |= (static_cast<uint32_t>(q[j]) & 0xffu) << j % 4 * 8;
+    auto put = [&](int64_t at) {
+      int8_t* dst = p.q + at * p.ld_q + static_cast<int64_t>(c) * V;
+      if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+      else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
+      else *dst = static_cast<int8_t>(q[0]);
+    };
+    if (!p.places) {
+      put(row);
+    } else {
+      for (int j = 0; j < p.topk; ++j) {
+        const int32_t at = p.places[row * p.topk + j];
+        if (at >= 0) put(at);
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i)
+    if (lane + i * TPR < n) write(held[i], lane + i * TPR);
+  for (int c = lane + kPieces * TPR; c < n; c += TPR) {
+    P v;
+    v.load(x, c);
+    write(v, c);
+  }
+  if (!p.places) {
+    if (lane == 0) p.scale[row] = p.factor ? to.scale() * p.factor[row] : to.scale();
+  } else {
+    for (int j = lane; j < p.topk; j += TPR) {
+      const int32_t at = p.places[row * p.topk + j];
+      if (at < 0) continue;
+      p.scale[at] = to.scale();
+      p.row_weight[at] = p.weights[row * p.topk + j];
+    }
+  }
+}
+
+template <typename T, bool VEC>
+cudaError_t launch_rows_vec(const RowsParams& p, cudaStream_t st) {
+  const int n = p.cols / Piece<T, VEC>::kValues;
+  auto go = [&](auto tpr, auto* kernel) {
+    constexpr int kRows = kRowThreads / decltype(tpr)::value;
+    const int64_t blocks = (p.rows + kRows - 1) / kRows;
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = launch_config(dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, st, &attr);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+  };
+  if (n <= 8 * kPieces) return go(std::integral_constant<int, 8>{}, quantize_rows_kernel<T, VEC, 8>);
+  if (n <= 32 * kPieces) return go(std::integral_constant<int, 32>{}, quantize_rows_kernel<T, VEC, 32>);
+  return go(std::integral_constant<int, 256>{}, quantize_rows_kernel<T, VEC, 256>);
+}
+
+template <typename T>
+cudaError_t launch_rows_type(const RowsParams& p, cudaStream_t st) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = p.cols % V == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ld_x % V == 0 &&
+                   reinterpret_cast<uintptr_t>(p.q) % V == 0 && p.ld_q % V == 0;
+  return vec ? launch_rows_vec<T, true>(p, st) : launch_rows_vec<T, false>(p, st);
+}
+
+cudaError_t launch_rows(const RowsParams& p, int32_t dtype, cudaStream_t st) {
+  if (p.rows == 0) return cudaSuccess;
+  return dtype == HEXMOE_F32   ? launch_rows_type<float>(p, st)
+         : dtype == HEXMOE_F16 ? launch_rows_type<__half>(p, st)
+                               : launch_rows_type<__nv_bfloat16>(p, st);
+}
+
+// ------------------------------------------------------------------- plan
+// The rows of routed slots in expert order: offsets[e] (exclusive counts) and every slot's row.  Within an expert the
+// rows come in whatever order the counting finds: no value of the layer depends on it (a row's sums are whole
+// numbers and its own).  One cluster: each CTA counts its slots in shared memory, the counts of the CTAs before it come
+// over distributed shared memory, and nothing has to be cleared or handed on between kernels.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanCtas = 8;
+constexpr int kMaxExperts = 2048;
+
+__global__ void __launch_bounds__(kPlanThreads, 1)
+    plan_kernel(const void* ids, int32_t ids64, int64_t slots, int32_t experts, int32_t* offsets, int32_t* places,
+                int32_t* dev_err) {
+  __shared__ int32_t hist[kMaxExperts], first[kMaxExperts], sums[32];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
+  pdl_wait();
+  pdl_launch_dependents();
+  for (int e = threadIdx.x; e < experts; e += kPlanThreads) hist[e] = 0;
+  __syncthreads();
+  const int64_t chunk = (slots + ctas - 1) / ctas, begin = rank * chunk, end = min(begin + chunk, slots);
+  auto expert = [&](int64_t s) -> int64_t {
+    const int64_t e = ids64 ? static_cast<const int64_t*>(ids)[s] : static_cast<const int32_t*>(ids)[s];
+    return e >= 0 && e < experts ? e : -1;
+  };
+  bool bad = false;
+  for (int64_t s = begin + threadIdx.x; s < end; s += kPlanThreads) {
+    const int64_t e = expert(s);
+    places[s] = e < 0 ? -1 : atomicAdd(&hist[e], 1);
+    bad |= e < 0;
+  }
+  if (bad) atomicOr(dev_err, kDevErrExpertId);
+  cluster.sync();
+  // every CTA: each expert's count over all of them, and before this one
+  const int per = (experts + kPlanThreads - 1) / kPlanThreads;   // 1 or 2 a thread
+  int32_t total[2] = {}, before[2] = {}, mine = 0;
+  for (int i = 0; i < per; ++i) {
+    const int e = static_cast<int>(threadIdx.x) * per + i;
+    if (e >= experts) break;
+    for (int c = 0; c < ctas; ++c) {
+      const int32_t v = cluster.map_shared_rank(hist, c)[e];
+      total[i] += v;
+      if (c < rank) before[i] += v;
+    }
+    mine += total[i];
+  }
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int32_t upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int32_t v = __shfl_up_sync(kAll, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) sums[warp] = upto;
+  __syncthreads();
+  if (warp == 0) {
+    int32_t v = sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int32_t u = __shfl_up_sync(kAll, v, o);
+      if (lane >= o) v += u;
+    }
+    sums[lane] = v;
+  }
+  __syncthreads();
+  int32_t at = upto - mine + (warp ? sums[warp - 1] : 0);
+  for (int i = 0; i < per; ++i) {
+    const int e = static_cast<int>(threadIdx.x) * per + i;
+    if (e >= experts) break;
+    first[e] = at + before[i];
+    if (rank == 0) offsets[e] = at;
+    at += total[i];
+    if (rank == 0 && e == experts - 1) offsets[experts] = at;
+  }
+  cluster.sync();   // `first` is whole, and no CTA leaves while its counts are read
+  for (int64_t s = begin + threadIdx.x; s < end; s += kPlanThreads) {
+    const int64_t e = expert(s);
+    if (e >= 0) places[s] += first[e];
+  }
+}
+
+cudaError_t launch_plan(const void* ids, int32_t ids64, int64_t slots, int32_t experts, int32_t* offsets, int32_t* places,
+                        int32_t* dev_err, cudaStream_t st) {
+  cudaLaunchAttribute attr[2];
+  const int ctas = slots > 2 * kPlanThreads ? kPlanCtas : 1;
+  cudaLaunchConfig_t cfg = launch_config(dim3(ctas), kPlanThreads, 0, st, attr);
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, plan_kernel, ids, ids64, slots, experts, offsets, places, dev_err);
+}
+
+bool is16(int32_t dt) { return dt == HEXMOE_BF16 || dt == HEXMOE_F16; }
+bool known_dtype(int32_t dt) { return dt == HEXMOE_F32 || is16(dt); }
+bool off_by(const void* p, size_t z) { return reinterpret_cast<uintptr_t>(p) % z != 0; }
+int64_t pitch16(int64_t n) { return (n + 15) / 16 * 16; }
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+// The parts of a workspace one after the other.
+struct Carve {
+  uint8_t* base;
+  size_t used = 0;
+  template <typename T>
+  T* take(size_t count) {
+    T* p = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += round256(count * sizeof(T));
+    return p;
+  }
+};
+
+struct MmScratch {
+  int8_t* q;
+  float* scale;
+  uint8_t* partial;
+  size_t partial_bytes, used;
+  MmScratch(void* ws, int64_t rows, int32_t experts, int32_t n, int32_t k, bool quantizes) {
+    Carve c{static_cast<uint8_t*>(ws)};
+    q = c.take<int8_t>(quantizes ? rows * pitch16(k) : 0);
+    scale = c.take<float>(quantizes ? rows : 0);
+    partial_bytes = int8_partial_bytes(rows, experts, n, k);
+    partial = c.take<uint8_t>(partial_bytes);
+    used = c.used;
+  }
+};
+
+struct LayerScratch {
+  int32_t *offsets, *places;
+  float *x_scale, *weight, *act, *act_scale;
+  int8_t *xq, *actq;
+  uint8_t *y, *partial;
+  size_t partial_bytes, used;
+  LayerScratch(void* ws, int64_t slots, int32_t experts, int32_t hidden, int32_t inter) {
+    Carve c{static_cast<uint8_t*>(ws)};
+    offsets = c.take<int32_t>(experts + 1);
+    places = c.take<int32_t>(slots);
+    x_scale = c.take<float>(slots);
+    weight = c.take<float>(slots);
+    act_scale = c.take<float>(slots);
+    xq = c.take<int8_t>(slots * hidden);
+    act = c.take<float>(slots * inter);
+    actq = c.take<int8_t>(slots * inter);
+    y = c.take<uint8_t>(2 * slots * hidden);
+    partial_bytes = int8_partial_bytes(slots, experts, hidden, inter);
+    partial = c.take<uint8_t>(partial_bytes);
+    used = c.used;
+  }
+};
+
+}  // namespace
+}  // namespace hexmoe
+
+using namespace hexmoe;
+
+extern "C" {
+
+int hexmoe_quantize_rows(const void* x, int32_t x_dtype, int64_t ld_x, int64_t rows, int32_t cols, int8_t* q, int64_t ld_q,
+                         float* scale, void* stream) {
+  const char* what = "hexmoe_quantize_rows";
+  if (!known_dtype(x_dtype)) return report_error(HEXMOE_E_DTYPE, "hexmoe_quantize_rows: bad dtype");
+  if (rows < 0 || cols <= 0 || cols > (1 << 30)) return arg_error("%s: rows %lld, cols %d", what, static_cast<long long>(rows), cols);
+  if (ld_x < cols || ld_q < cols) return arg_error("%s: a row stride is shorter than its row", what);
+  if (rows == 0) return HEXMOE_OK;
+  if (!x || !q || !scale || off_by(x, x_dtype == HEXMOE_F32 ? 4 : 2) || off_by(scale, 4))
+    return arg_error("%s: null pointer, or one not aligned to its element", what);
+  RowsParams p{};
+  p.x = x; p.ld_x = ld_x; p.rows = rows; p.cols = cols; p.q = q; p.ld_q = ld_q; p.scale = scale;
+  const cudaError_t e = launch_rows(p, x_dtype, static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
+}
+
+size_t hexmoe_grouped_mm_int8_workspace_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k, int32_t x_dtype) {
+  if (rows <= 0 || experts <= 0 || n <= 0 || k <= 0) return 0;
+  return MmScratch(nullptr, rows, experts, n, k, x_dtype != HEXMOE_I8).used;
+}
+
+int hexmoe_grouped_mm_int8(const void* x, int32_t x_dtype, int64_t ld_x, const float* x_scale, const int8_t* w, int64_t ld_w,
+                           int64_t stride_w, const float* w_scale, int64_t rows, int32_t experts, int32_t n, int32_t k,
+                           const void* offsets, int32_t offsets_dtype, void* out, int64_t ld_out, int32_t out_dtype,
+                           void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "hexmoe_grouped_mm_int8";
+  const bool quantizes = x_dtype != HEXMOE_I8;
+  if ((quantizes && !known_dtype(x_dtype)) || !known_dtype(out_dtype))
+    return report_error(HEXMOE_E_DTYPE, "hexmoe_grouped_mm_int8: x is I8, F32, BF16 or F16, out F32, BF16 or F16");
+  if (offsets_dtype != HEXMOE_I32 && offsets_dtype != HEXMOE_I64) return report_error(HEXMOE_E_DTYPE, "offsets are I32 or I64");
+  if (rows < 0 || rows >= (1ll << 31) - 512) return arg_error("%s: %lld rows", what, static_cast<long long>(rows));
+  if (experts <= 0 || experts > kMaxExperts) return arg_error("%s: %d experts outside 1..%d", what, experts, kMaxExperts);
+  if (n <= 0 || n > (1 << 24) || k <= 0 || k > kMaxSum)
+    return arg_error("%s: n %d, k %d (at most %lld, or a sum may leave int32)", what, n, k, static_cast<long long>(kMaxSum));
+  if (!offsets && experts != 1) return arg_error("%s: no offsets for %d experts", what, experts);
+  if (off_by(offsets, offsets_dtype == HEXMOE_I64 ? 8 : 4)) return arg_error("%s: offsets not aligned", what);
+  if (ld_x < k || ld_w < k || stride_w < 0 || ld_out < n) return arg_error("%s: a row stride is shorter than its row", what);
+  if (rows == 0) return HEXMOE_OK;
+  if (!x || !w || !w_scale || !out || (!quantizes && !x_scale) || off_by(w_scale, 4) || off_by(x_scale, 4) ||
+      off_by(out, out_dtype == HEXMOE_F32 ? 4 : 2) || (quantizes && off_by(x, x_dtype == HEXMOE_F32 ? 4 : 2)))
+    return arg_error("%s: null pointer, or one not aligned to its element", what);
+  if (!int8_stack(w, ld_w, stride_w, experts) || (!quantizes && !int8_rows(x, ld_x)))
+    return arg_error("%s: 8-bit rows must begin and repeat on multiples of 16 bytes", what);
+  if (off_by(workspace, 16)) return arg_error("%s: workspace not 16-byte aligned", what);
+  const MmScratch s(workspace, rows, experts, n, k, quantizes);
+  if (quantizes && (!workspace || workspace_bytes < s.used))
+    return arg_error("%s: a workspace of %zu bytes is needed", what, s.used);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  Int8Product d{};
+  d.x = static_cast<const int8_t*>(x); d.ld_x = ld_x; d.x_scale = x_scale;
+  if (quantizes) {
+    RowsParams p{};
+    p.x = x; p.ld_x = ld_x; p.rows = rows; p.cols = k; p.q = s.q; p.ld_q = pitch16(k); p.scale = s.scale;
+    const cudaError_t e = launch_rows(p, x_dtype, st);
+    if (e != cudaSuccess) return report_cuda_error(e, what);
+    d.x = s.q; d.ld_x = p.ld_q; d.x_scale = s.scale;
+  }
+  d.w = w; d.ld_w = ld_w; d.stride_w = stride_w; d.w_scale = w_scale;
+  d.rows = rows; d.experts = experts; d.n = n; d.k = k;
+  d.offsets = offsets; d.offsets64 = offsets_dtype == HEXMOE_I64;
+  d.out = out; d.ld_out = ld_out; d.out_dtype = out_dtype;
+  if (workspace && workspace_bytes >= s.used) { d.workspace = s.partial; d.workspace_bytes = s.partial_bytes; }
+  return run_int8_product(what, d, st);
+}
+
+size_t hexmoe_int8_forward_workspace_bytes(int64_t tokens, int32_t topk, int32_t experts, int32_t hidden, int32_t inter) {
+  if (tokens <= 0 || topk <= 0 || experts <= 0 || hidden <= 0 || inter <= 0) return 0;
+  return LayerScratch(nullptr, tokens * topk, experts, hidden, inter).used;
+}
+
+int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t tokens, int32_t hidden, int32_t inter, int32_t topk,
+                        const float* topk_weights, const void* topk_ids, int32_t ids_dtype, int32_t experts,
+                        const int8_t* w13, int64_t ld_w13, int64_t stride_w13, const float* w13_scale, const int8_t* w2,
+                        int64_t ld_w2, int64_t stride_w2, const float* w2_scale, void* out, int32_t out_dtype,
+                        void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "hexmoe_int8_forward";
+  if (!known_dtype(x_dtype) || (out_dtype != x_dtype && out_dtype != HEXMOE_F32))
+    return report_error(HEXMOE_E_DTYPE, "hexmoe_int8_forward: x is F32, BF16 or F16, out the same or F32");
+  if (ids_dtype != HEXMOE_I32 && ids_dtype != HEXMOE_I64) return report_error(HEXMOE_E_DTYPE, "hexmoe_int8_forward: ids are I32 or I64");
+  if (tokens < 0 || topk <= 0 || topk > 1024 || tokens * topk >= (1ll << 31) - 512)
+    return arg_error("%s: %lld tokens, topk %d", what, static_cast<long long>(tokens), topk);
+  if (experts <= 0 || experts > kMaxExperts) return arg_error("%s: %d experts outside 1..%d", what, experts, kMaxExperts);
+  if (hidden <= 0 || inter <= 0 || hidden % 16 || inter % 16 || hidden > kMaxSum || inter > kMaxSum)
+    return arg_error("%s: hidden %d, inter %d (multiples of 16, at most %lld)", what, hidden, inter, static_cast<long long>(kMaxSum));
+  if (ld_x < hidden || ld_w13 < hidden || ld_w2 < inter || stride_w13 < 0 || stride_w2 < 0)
+    return arg_error("%s: a row stride is shorter than its row", what);
+  if (tokens == 0) return HEXMOE_OK;
+  if (!x || !topk_weights || !topk_ids || !w13 || !w13_scale || !w2 || !w2_scale || !out || off_by(x, x_dtype == HEXMOE_F32 ? 4 : 2) ||
+      off_by(topk_weights, 4) || off_by(topk_ids, ids_dtype == HEXMOE_I64 ? 8 : 4) || off_by(w13_scale, 4) || off_by(w2_scale, 4))
+    return arg_error("%s: null pointer, or one not aligned to its element", what);
+  if (off_by(out, 16)) return arg_error("%s: out not 16-byte aligned", what);
+  if (!int8_stack(w13, ld_w13, stride_w13, experts) || !int8_stack(w2, ld_w2, stride_w2, experts))
+    return arg_error("%s: 8-bit rows must begin and repeat on multiples of 16 bytes", what);
+  const int64_t slots = tokens * topk;
+  const LayerScratch s(workspace, slots, experts, hidden, inter);
+  if (!workspace || off_by(workspace, 256) || workspace_bytes < s.used)
+    return arg_error("%s: a workspace of %zu bytes is needed, on a multiple of 256", what, s.used);
+  int32_t* dev_err = device_error_word();
+  if (!dev_err) return report_error(HEXMOE_E_CUDA, "device error word unavailable");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = launch_plan(topk_ids, ids_dtype == HEXMOE_I64, slots, experts, s.offsets, s.places, dev_err, st);
+  if (e != cudaSuccess) return report_cuda_error(e, what);
+  RowsParams p{};
+  p.x = x; p.ld_x = ld_x; p.rows = tokens; p.cols = hidden; p.q = s.xq; p.ld_q = hidden; p.scale = s.x_scale;
+  p.places = s.places; p.topk = topk; p.weights = topk_weights; p.row_weight = s.weight;
+  e = launch_rows(p, x_dtype, st);
+  if (e != cudaSuccess) return report_cuda_error(e, what);
+  Int8Product d{};
+  d.x = s.xq; d.ld_x = hidden; d.x_scale = s.x_scale;
+  d.w = w13; d.ld_w = ld_w13; d.stride_w = stride_w13; d.w_scale = w13_scale;
+  d.rows = slots; d.experts = experts; d.n = 2 * inter; d.k = hidden;
+  d.offsets = s.offsets;
+  d.out = s.act; d.ld_out = inter; d.out_dtype = HEXMOE_F32; d.glu = 1;
+  if (int rc = run_int8_product(what, d, st)) return rc;
+  p = RowsParams{};
+  p.x = s.act; p.ld_x = inter; p.rows = slots; p.cols = inter; p.q = s.actq; p.ld_q = inter; p.scale = s.act_scale;
+  p.factor = s.weight; p.count = s.offsets + experts;
+  e = launch_rows(p, HEXMOE_F32, st);
+  if (e != cudaSuccess) return report_cuda_error(e, what);
+  const int32_t y_dtype = x_dtype == HEXMOE_F16 ? HEXMOE_F16 : HEXMOE_BF16;
+  d = Int8Product{};
+  d.x = s.actq; d.ld_x = inter; d.x_scale = s.act_scale;
+  d.w = w2; d.ld_w = ld_w2; d.stride_w = stride_w2; d.w_scale = w2_scale;
+  d.rows = slots; d.experts = experts; d.n = hidden; d.k = inter;
+  d.offsets = s.offsets;
+  d.out = s.y; d.ld_out = hidden; d.out_dtype = y_dtype;
+  d.workspace = s.partial; d.workspace_bytes = s.partial_bytes;
+  if (int rc = run_int8_product(what, d, st)) return rc;
+  e = launch_combine(s.y, y_dtype, tokens, topk, hidden, hidden, s.places, slots, out, out_dtype, st, true);
+  return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
+}
+
+}  // extern "C"

@@ -177,6 +177,29 @@ cudaError_t launch_gather_rows(const void* x, int x_dtype, int64_t T, int32_t H,
                                cudaStream_t st, bool pdl, const int32_t* slot_row = nullptr);
 cudaError_t launch_route_topk(const void* logits, int dtype, int64_t T, int32_t E, int32_t k, int renorm, float* w,
                               int32_t* ids, cudaStream_t st);
+// Products of 8-bit rows in groups with their experts' 8-bit matrices (grouped.cu); glu: of [gate | up] matrices (n rows
+// in all, a multiple of 32), silu(gate) up in f32 [rows, n / 2].  x and w must pass int8_rows and int8_stack.
+struct Int8Product {
+  const int8_t* x;
+  int64_t ld_x;
+  const float* x_scale;    // [rows]
+  const int8_t* w;         // [experts, n, k]
+  int64_t ld_w, stride_w;
+  const float* w_scale;    // [experts, n]
+  int64_t rows;
+  int32_t experts, n, k;
+  const void* offsets;     // [experts + 1]; null: one group of all rows
+  int32_t offsets64;
+  void* out;
+  int64_t ld_out;
+  int32_t out_dtype, glu;
+  void* workspace;         // int8_partial_bytes, or null
+  size_t workspace_bytes;
+};
+int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st);
+size_t int8_partial_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k);
+bool int8_rows(const void* p, int64_t ld);
+bool int8_stack(const void* p, int64_t ld, int64_t stride, int32_t count);
 // The layer's description (api.cu).
 const hexmoe_layer_desc* layer_desc(const hexmoe_layer* layer);
 // The layer forward up to its per-slot rows y[num_slots, hidden] (16-bit) over

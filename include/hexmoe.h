@@ -54,7 +54,7 @@ enum hexmoe_status {
 };
 
 /* Element types of activations / outputs. */
-enum hexmoe_dtype { HEXMOE_F32 = 0, HEXMOE_BF16 = 1, HEXMOE_F16 = 2 };
+enum hexmoe_dtype { HEXMOE_F32 = 0, HEXMOE_BF16 = 1, HEXMOE_F16 = 2, HEXMOE_I8 = 3 /* 8-bit products only */ };
 /* Element types of expert-id tensors. */
 enum hexmoe_index_dtype { HEXMOE_I32 = 0, HEXMOE_I64 = 1 };
 
@@ -439,6 +439,91 @@ HEXMOE_API int hexmoe_clip_grad_norm(int32_t tensors, const void* const* src, co
                                      const int32_t* src_dtypes, void* const* dst, const int32_t* dst_dtypes,
                                      float max_norm, int32_t inf_norm, float* norm_out, void* workspace,
                                      size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * The router with all that routers do, and its gradient.  hexmoe_route_topk
+ * above is the plain softmax form.
+ * ------------------------------------------------------------------------- */
+enum hexmoe_scoring { HEXMOE_SOFTMAX = 0, HEXMOE_SIGMOID = 1 };
+
+/* Every token's topk experts and their weights.  Scores s = softmax(l) over all
+ * experts or sigmoid(l) of logits l [tokens, num_experts] (F32, BF16 or F16, row
+ * stride ld_logits); c = s + bias (f32 [num_experts]), or l without a bias, whose
+ * order is the scores'.  The experts form `groups` runs of equal length (at most
+ * 32); the topk_groups runs with the largest sums of their group_top (1 or 2)
+ * largest s + bias are open.  topk_ids int32 [tokens, topk]: the largest c of the
+ * open groups in order, ties to the lower id (groups as well), as exact
+ * arithmetic decides.  topk_weights f32 [tokens, topk]: scale * s, over the sum of
+ * the token's chosen s with renormalize != 0.  A logit of -infinity masks its
+ * expert: score 0, taken after all others of the open groups; a token with
+ * nothing else has weights 0.  NaN logits make NaN weights of valid ids.  At most
+ * 2048 experts, topk at most 32 and at most the experts of topk_groups groups. */
+HEXMOE_API int hexmoe_route(const void* logits, int32_t logits_dtype, int64_t ld_logits, int64_t tokens,
+                            int32_t num_experts, int32_t topk, int32_t scoring, const float* bias, int32_t groups,
+                            int32_t topk_groups, int32_t group_top, int32_t renormalize, float scale,
+                            float* topk_weights, int32_t* topk_ids, void* stream);
+
+/* The gradient of hexmoe_route's weights for the logits: dlogits [tokens,
+ * num_experts] (logits_dtype, row stride ld_dlogits) from dweights f32 and
+ * topk_ids (ids_dtype) [tokens, topk].  The choice has no gradient.  An expert
+ * that stands among a token's ids more than once has the sum of its places; ids
+ * outside 0..num_experts-1 have no part. */
+HEXMOE_API int hexmoe_route_backward(const float* dweights, const void* logits, int32_t logits_dtype,
+                                     int64_t ld_logits, int64_t tokens, int32_t num_experts, int32_t topk,
+                                     const void* topk_ids, int32_t ids_dtype, int32_t scoring, int32_t renormalize,
+                                     float scale, void* dlogits, int64_t ld_dlogits, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * Experts in 8-bit integers, with a scale for each row of activations (token)
+ * and each row of a matrix (channel): a MoE layer at twice the tensor-core rate
+ * of 16 bits and half its bytes, for a HEX layer's prefill where memory allows
+ * a copy of the experts in 8 bits.  No counterpart in the reference.
+ * ------------------------------------------------------------------------- */
+
+/* Rows x [rows, cols] (F32, BF16 or F16, row stride ld_x) in 8 bits:
+ *   scale[r] = max |x[r]| / 127,  q[r, i] = round(127 x[r, i] / max |x[r]|)
+ * ties to even, the quotient as exact arithmetic has it.  A row of zeros has
+ * scale 0, one with an infinity or NaN scale NaN and zeros.  q: row stride ld_q
+ * (a multiple of 16 for the products below).  The rows of a stack of matrices
+ * are its channels. */
+HEXMOE_API int hexmoe_quantize_rows(const void* x, int32_t x_dtype, int64_t ld_x, int64_t rows, int32_t cols,
+                                    int8_t* q, int64_t ld_q, float* scale, void* stream);
+
+/* out[r, j] = x_scale[r] w_scale[e, j] sum_i x[r, i] w[e, j, i] for every row r of
+ * group e (offsets as for hexmoe_grouped_mm; NULL with one expert: all rows are
+ * its).  x [rows, k]: I8 with x_scale [rows], or F32, BF16 or F16, quantized on the
+ * way as hexmoe_quantize_rows does (x_scale is not read).  w I8 [experts, n, k], w_scale
+ * f32 [experts, n].  Sums are exact (k at most 131071); out F32, BF16 or F16 is
+ * rounded once, or split reductions of few rows once for each of their parts in f32.  8-bit
+ * rows begin and repeat on multiples of 16 bytes.  Rows of no group are set to
+ * zero.  workspace (256-byte aligned): hexmoe_grouped_mm_int8_workspace_bytes,
+ * needed where x is quantized here, elsewhere as for hexmoe_grouped_mm. */
+HEXMOE_API size_t hexmoe_grouped_mm_int8_workspace_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k,
+                                                         int32_t x_dtype);
+HEXMOE_API int hexmoe_grouped_mm_int8(const void* x, int32_t x_dtype, int64_t ld_x, const float* x_scale,
+                                      const int8_t* w, int64_t ld_w, int64_t stride_w, const float* w_scale,
+                                      int64_t rows, int32_t experts, int32_t n, int32_t k, const void* offsets,
+                                      int32_t offsets_dtype, void* out, int64_t ld_out, int32_t out_dtype,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* Routed-expert output of a SwiGLU layer with 8-bit experts, out[t] = sum_j
+ * topk_weights[t, j] down_e(silu(gate_e x_t) * up_e x_t), e = topk_ids[t, j]: the
+ * rows of x and of the activation are quantized, the products are those above.
+ * x [tokens, hidden] (F32, BF16 or F16, row stride ld_x), out [tokens, hidden] in
+ * x_dtype or F32; w13 I8 [experts, 2 * inter, hidden] (gate rows, then up) with
+ * scales [experts, 2 * inter], w2 I8 [experts, hidden, inter] with scales
+ * [experts, hidden].  hidden and inter are multiples of 16.  The activation stays
+ * in f32 until it is quantized; a slot's row is rounded to 16 bits (BF16 for F32
+ * x) before a token's rows are summed in f32, as in hexmoe_forward.  Ids outside 0..experts-1 add
+ * nothing and set the device error word. */
+HEXMOE_API size_t hexmoe_int8_forward_workspace_bytes(int64_t tokens, int32_t topk, int32_t experts, int32_t hidden,
+                                                      int32_t inter);
+HEXMOE_API int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t tokens, int32_t hidden,
+                                   int32_t inter, int32_t topk, const float* topk_weights, const void* topk_ids,
+                                   int32_t ids_dtype, int32_t experts, const int8_t* w13, int64_t ld_w13,
+                                   int64_t stride_w13, const float* w13_scale, const int8_t* w2, int64_t ld_w2,
+                                   int64_t stride_w2, const float* w2_scale, void* out, int32_t out_dtype,
+                                   void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
