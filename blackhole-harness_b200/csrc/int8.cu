@@ -41,12 +41,14 @@ cudaLaunchConfig_t launch_config(dim3 grid, int threads, size_t smem, cudaStream
 }
 
 // ------------------------------------------------------------------- rows to 8 bits
-// scale = max |x| / 127, q = round(127 x / max |x|), ties to even, of every row.  The quotient is that of real numbers: it
-// is computed in f32, which is off by less than 2^-16 at 127, and where that leaves a border in doubt, in f64
-// (127 x is exact there, and half a step is met exactly: x = max / 2 is 63.5).  A row of zeros has scale 0; one that holds
-// an infinity or NaN has scale NaN and zeros, so that what is made of it is NaN.
-// Bound by HBM.  TPR threads take a row and keep its first kPieces 16-byte pieces each in registers; what a longer row has
-// behind those is read again.
+// scale = max |x| / 127, q = round(127 x / max |x|), ties to even, of every row.  The quotient is that of real numbers (x =
+// max / 2, which 16-bit rows hold often, is 63.5 to the last bit): it is computed in f32, off by less than 2^-16 at 127, and
+// an f32 x that close to a border n + 1/2 is decided by the sign of 254 |x| - (2 n + 1) max, which f32 products with their
+// rounding errors (by FMA) give exactly; 16 bits need less (see byte()).  A row of zeros has scale 0; one that holds an
+// infinity or NaN has scale NaN and zeros, so that what is made of it is NaN.
+// Bound by HBM; the arithmetic is kept to some ten instructions a value, no conversions among them (they run at an eighth
+// of the rate).  TPR threads take a row and keep its first kPieces 16-byte pieces each in registers; what a longer row
+// has behind those is read again.
 constexpr int kRowThreads = 256;
 constexpr int kPieces = 8;
 
@@ -67,54 +69,84 @@ struct RowsParams {
   float* row_weight;
 };
 
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4& v, float (&x)[16 / sizeof(T)]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (std::is_same_v<T, float>) {
-      x[i] = __uint_as_float(w[i]);
-    } else if constexpr (std::is_same_v<T, __half>) {
-      x[2 * i] = __half2float(__ushort_as_half(static_cast<uint16_t>(w[i])));
-      x[2 * i + 1] = __half2float(__ushort_as_half(static_cast<uint16_t>(w[i] >> 16)));
-    } else {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
-}
-
-// Values a piece: 16 bytes of them, or one (rows that are not aligned to 16 bytes, or of odd lengths).
+// A row's values as they lie, 16 bytes at a time, or one by one (rows that are not aligned to 16 bytes, or of odd
+// lengths): the largest magnitude's bits, and the values in f32.
 template <typename T, bool VEC>
 struct Piece {
-  static constexpr int kValues = VEC ? 16 / sizeof(T) : 1;
-  float x[kValues];
+  static constexpr int kValues = VEC ? 16 / sizeof(T) : 1, kWords = VEC ? 4 : 1;
+  uint32_t w[kWords];
   __device__ __forceinline__ void load(const T* row, int i) {
     if constexpr (VEC) {
-      unpack<T>(reinterpret_cast<const uint4*>(row)[i], x);
+      const uint4 v = reinterpret_cast<const uint4*>(row)[i];
+      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (sizeof(T) == 4) {
+      w[0] = reinterpret_cast<const uint32_t*>(row)[i];
     } else {
-      if constexpr (std::is_same_v<T, float>) x[0] = row[i];
-      else if constexpr (std::is_same_v<T, __half>) x[0] = __half2float(row[i]);
-      else x[0] = __bfloat162float(row[i]);
+      w[0] = reinterpret_cast<const uint16_t*>(row)[i];
     }
   }
+  // The largest magnitude so far: f32 bits, or two of 16 bits.
+  __device__ __forceinline__ uint32_t see(uint32_t most) const {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+      most = sizeof(T) == 4 ? max(most, w[i] & 0x7fffffffu) : __vmaxu2(most, w[i] & 0x7fff7fffu);
+    return most;
+  }
+  __device__ __forceinline__ float value(int j) const {
+    if constexpr (std::is_same_v<T, float>) return __uint_as_float(w[j]);
+    else if constexpr (std::is_same_v<T, __half>) return __half2float(__ushort_as_half(static_cast<uint16_t>(w[j / 2] >> j % 2 * 16)));
+    else return __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+  }
 };
+// The f32 bits of see()'s magnitude.
+template <typename T>
+__device__ __forceinline__ uint32_t f32_bits(uint32_t most) {
+  if constexpr (sizeof(T) == 4) return most;
+  const uint32_t v = max(most & 0xffffu, most >> 16);
+  if constexpr (std::is_same_v<T, __half>) return __float_as_uint(__half2float(__ushort_as_half(static_cast<uint16_t>(v))));
+  else return v << 16;
+}
 
 struct RowScale {
-  float largest, inverse;
-  bool plain;   // f32 is enough but for borders
+  float largest;   // as it is
+  float fit, most, inverse;   // a power of two that keeps what follows in range, the largest times it, 127 / that
   __device__ __forceinline__ explicit RowScale(uint32_t bits) {
     largest = __uint_as_float(bits);
-    plain = largest > 1e-30f && largest < 1e30f;
-    inverse = plain ? 127.f / largest : 0.f;
+    fit = largest > 0x1p96f ? 0x1p-60f : largest < 0x1p-90f ? 0x1p100f : 1.f;
+    most = largest * fit;
+    inverse = largest == 0.f || !finite() ? 0.f : 127.f / most;
   }
   __device__ __forceinline__ bool finite() const { return __float_as_uint(largest) < 0x7f800000u; }
   __device__ __forceinline__ float scale() const { return finite() ? largest / 127.f : __uint_as_float(0x7fc00000u); }
-  __device__ __forceinline__ int32_t operator()(float x) const {
-    const float t = x * inverse, r = rintf(t);
-    if (plain && fabsf(t - r) < 0.49998f) return static_cast<int32_t>(r);
-    if (!finite() || largest == 0.f) return 0;
-    return static_cast<int32_t>(rint(static_cast<double>(x) * 127.0 / static_cast<double>(largest)));
+  // 127 x / largest rounded, as the low byte of a word.
+  //   16-bit x: the quotient's nearest border n + 1/2 is met exactly or missed by 2^-19 of it (254 x and (2 n + 1) largest
+  //     are whole multiples of a common unit, of at most 11 + 8 bits), so rounding it to 20 bits first takes its f32 error
+  //     away and leaves exact halves to the rounding to even.
+  //   f32: doubt is the distance from the whole number, the largest so far; what near_border() says goes by exact_byte().
+  template <typename T>
+  __device__ __forceinline__ uint32_t byte(float x, float& doubt) const {
+    constexpr float kWhole = 12582912.f;   // 1.5 x 2^23: f32 values here are whole numbers
+    float t = __fmul_rn(__fmul_rn(x, fit), inverse);   // each rounded by itself: no FMA made of two
+    if constexpr (sizeof(T) == 2) {
+      const float wide = __fmul_rn(t, 17.f);
+      t = __fsub_rn(wide, __fsub_rn(wide, t));
+    }
+    const float r = t + kWhole;
+    if constexpr (sizeof(T) == 4) doubt = fmaxf(doubt, fabsf(t - (r - kWhole)));
+    return __float_as_uint(r);
+  }
+  static __device__ __forceinline__ bool near_border(float doubt) { return doubt > 0.49998f; }
+  __device__ __forceinline__ uint32_t exact_byte(float x) const {
+    const float v = fabsf(x * fit), n = floorf(v * inverse + 0x1p-10f);
+    if (!(fabsf(v * inverse - n - 0.5f) < 0x1p-10f)) {
+      float ignore = 0.f;
+      return byte<float>(x, ignore);
+    }
+    const float odd = 2.f * n + 1.f, p = odd * most;
+    const float over = fmaf(254.f, v, -p), lost = fmaf(odd, most, -p);   // 254 v - odd most = over - lost, both exact
+    const bool up = over > lost || (over == lost && (static_cast<int>(n) & 1));
+    const int32_t q = static_cast<int>(n) + up;
+    return static_cast<uint32_t>(x < 0.f ? -q : q);
   }
 };
 
@@ -131,24 +163,21 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsPa
   const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
   const int n = p.cols / V;
   P held[kPieces];
-  uint32_t bits = 0;
-  auto see = [&](const P& v) {
-#pragma unroll
-    for (int j = 0; j < V; ++j) bits = max(bits, __float_as_uint(v.x[j]) & 0x7fffffffu);
-  };
+  uint32_t most = 0;
   if (live) {
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
       if (lane + i * TPR < n) held[i].load(x, lane + i * TPR);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
-      if (lane + i * TPR < n) see(held[i]);
+      if (lane + i * TPR < n) most = held[i].see(most);
     for (int c = lane + kPieces * TPR; c < n; c += TPR) {
       P v;
       v.load(x, c);
-      see(v);
+      most = v.see(most);
     }
   }
+  uint32_t bits = f32_bits<T>(most);
 #pragma unroll
   for (int o = (TPR < 32 ? TPR : 32) / 2; o > 0; o >>= 1) bits = max(bits, __shfl_xor_sync(kAll, bits, o));
   if constexpr (TPR > 32) {
@@ -160,12 +189,20 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsPa
   if (!live) return;
   const RowScale to(bits);
   auto write = [&](const P& v, int c) {
-    int32_t q[V];
+    uint32_t q[V];
+    float doubt = 0.f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) q[j] = to(v.x[j]);
-    uint32_t w[2] = {};
+    for (int j = 0; j < V; ++j) q[j] = to.byte<T>(v.value(j), doubt);
+    if (!to.finite()) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) w[j / 4] |= (static_cast<uint32_t>(q[j]) & 0xffu) << j % 4 * 8;
+      for (int j = 0; j < V; ++j) q[j] = 0;
+    } else if (sizeof(T) == 4 && RowScale::near_border(doubt)) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) q[j] = to.exact_byte(v.value(j));
+    }
+    uint32_t w[V / 4 + 1];
+#pragma unroll
+    for (int j = 0; j + 3 < V; j += 4) w[j / 4] = prmt(prmt(q[j], q[j + 1], 0x0040), prmt(q[j + 2], q[j + 3], 0x0040), 0x5410);
     auto put = [&](int64_t at) {
       int8_t* dst = p.q + at * p.ld_q + static_cast<int64_t>(c) * V;
       if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
@@ -201,6 +238,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsPa
   }
 }
 
+// The threads of a row: as few as hold it in registers.
 template <typename T, bool VEC>
 cudaError_t launch_rows_vec(const RowsParams& p, cudaStream_t st) {
   const int n = p.cols / Piece<T, VEC>::kValues;
@@ -214,6 +252,7 @@ cudaError_t launch_rows_vec(const RowsParams& p, cudaStream_t st) {
   };
   if (n <= 8 * kPieces) return go(std::integral_constant<int, 8>{}, quantize_rows_kernel<T, VEC, 8>);
   if (n <= 32 * kPieces) return go(std::integral_constant<int, 32>{}, quantize_rows_kernel<T, VEC, 32>);
+  if (n <= 64 * kPieces) return go(std::integral_constant<int, 64>{}, quantize_rows_kernel<T, VEC, 64>);
   return go(std::integral_constant<int, 256>{}, quantize_rows_kernel<T, VEC, 256>);
 }
 

@@ -88,6 +88,20 @@ def test_quantize_rows_far_from_one(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+def test_quantize_rows_at_borders(dtype):
+    """Values next to every border n + 1/2 of many largest ones, and on them, above and below."""
+    g = torch.Generator().manual_seed(4)
+    largest = (torch.rand(300, 1, generator=g).double() + 0.5) * 2.0 ** torch.randint(-12, 8, (300, 1), generator=g)
+    largest = largest.to(dtype).double()
+    near = ((torch.arange(127) + 0.5) / 127 * largest).to(dtype)
+    step = torch.finfo(dtype).eps * near
+    x = torch.cat([largest.to(dtype), near, near + step, -(near - step), -near, near + step / 2], 1)
+    q, _ = int8.quantize_rows(x.to(DEV))
+    assert torch.equal(q.cpu().double(), quantized(x)[0])
+
+
+@pytest.mark.gpu
 def test_quantize_rows_of_views_and_stacks():
     x = normal((40, 300), BF16, 5).to(DEV)
     for view in (x[:, 3:250], x[::2, 8:136], x.t(), x[0], x[:1, :64], x[:, :1].expand(40, 32), x[:0]):
