@@ -38,6 +38,7 @@ try:
 except ImportError:   # not built, or built for another torch: every call goes through Python and libhexmoe.so
     class _call:
         grouped_mm = grouped_wgrad = swiglu = swiglu_backward = clip_grad_norm = staticmethod(lambda *args: None)
+        route = route_backward = grouped_mm_int8 = int8_moe = staticmethod(lambda *args: None)
 
 _16BIT = (torch.bfloat16, torch.float16)
 _INDEX = {torch.int32: _lib.I32, torch.int64: _lib.I64}

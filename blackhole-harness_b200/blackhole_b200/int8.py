@@ -21,7 +21,7 @@ from __future__ import annotations
 import torch
 
 from blackhole_b200 import _lib
-from blackhole_b200.experts import _INDEX, _check_groups, _recorded, _rows2d, _run, _workspace, _written
+from blackhole_b200.experts import _INDEX, _call, _check_groups, _recorded, _rows2d, _run, _workspace, _written
 from blackhole_b200.hex_moe import _DT, _ptr
 
 MAX_K = 131071   # longest sum of products of 8-bit integers that int32 holds
@@ -82,6 +82,10 @@ def grouped_mm_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, off
     (quantize_rows).  The result is in out_dtype (f32, bf16 or fp16; x's, or bf16 for an int8 x), rounded once from exact sums
     (K at most 131071).  Rows of no group come back as zero.  Stacks whose rows do not begin on multiples of 16 bytes are
     copied at each call; quantize_rows makes them so that they do."""
+    if out is None and out_dtype is None and x_scale is None and offsets is not None:
+        res = _call.grouped_mm_int8(x, w, w_scale, offsets)
+        if res is not None:
+            return res
     if not x.is_cuda:
         raise ValueError("grouped_mm_int8 runs on CUDA only")
     dev = x.device
@@ -136,6 +140,9 @@ def int8_moe(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor
     [E, H] (quantize_rows makes them).  x [T, H] f32, bf16 or fp16; topk_weights and topk_ids [T, k] as hex_moe takes
     them: an id of no expert adds nothing and sets the device error word.  H and I are multiples of 16.  The rows of x
     and of the activation are quantized on the way."""
+    out = _call.int8_moe(x, topk_weights, topk_ids, w13, w13_scale, w2, w2_scale)
+    if out is not None:
+        return out
     if not x.is_cuda:
         raise ValueError("int8_moe runs on CUDA only")
     dev = x.device

@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from blackhole_b200 import _lib
-from blackhole_b200.experts import _INDEX, _recorded, _rows2d, _run
+from blackhole_b200.experts import _INDEX, _call, _recorded, _rows2d, _run
 from blackhole_b200.hex_moe import _DT, _ptr
 
 SCORING = {"softmax": _lib.SOFTMAX, "sigmoid": _lib.SIGMOID}
@@ -67,6 +67,9 @@ def route(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bias: torch
     lower id, as 64-bit arithmetic decides.  An expert whose logit is -inf is masked: it is taken after all others
     of the open groups, with weight 0; a token with nothing else has weights 0.  NaN logits make NaN weights of
     valid ids."""
+    res = _call.route(logits, k, SCORING.get(scoring), bias, groups, topk_groups, group_top, renormalize, scale)
+    if res is not None:
+        return res
     options = dict(scoring=scoring, bias=bias, groups=groups, topk_groups=topk_groups, group_top=group_top,
                    renormalize=renormalize, scale=scale)
     if _recorded(logits):
@@ -90,6 +93,9 @@ def route_backward(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tens
     """The gradient of route's weights for the logits: dlogits [T, E] in their type, from dweights float32 [T, k]
     and the ids [T, k] (int32 or int64) that route gave, with the same scoring, renormalize and scale.  The choice
     itself (bias, groups) has no gradient.  ids outside 0..E-1 have no part.  Not differentiable itself."""
+    dlogits = _call.route_backward(dweights, logits, ids, SCORING.get(scoring), renormalize, scale)
+    if dlogits is not None:
+        return dlogits
     logits, ld, code = _check("route_backward", logits, scoring)
     T, E = logits.shape
     dev = logits.device

@@ -1,5 +1,5 @@
-// call.cpp — the Python module blackhole_b200._call: the calls of experts.py for
-// arguments that need no second look.
+// call.cpp — the Python module blackhole_b200._call: the calls of experts.py, router.py
+// and int8.py for arguments that need no second look.
 //
 // A small product or activation is over on the GPU in 2 to 10 us; reading a dozen
 // tensor attributes, allocating the result and passing the arguments through
@@ -9,7 +9,7 @@
 // returns the result; or it returns None, having done nothing, where anything is
 // out of the ordinary (another device than the current one, a stride that wants a
 // copy, a type or shape that does not fit, inputs that autograd follows, arguments that the call refuses), and
-// experts.py takes the call from there, with its checks and messages.  A call that
+// the Python function takes the call from there, with its checks and messages.  A call that
 // failed on the way, with some of its work perhaps done, raises.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -248,14 +248,149 @@ PyObject* clip_grad_norm(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
   });
 }
 
+// A plain int argument that fits; false where it is something else.
+bool integer(PyObject* o, int32_t* v) {
+  if (!PyLong_CheckExact(o)) return false;
+  int overflow = 0;
+  const long long n = PyLong_AsLongLongAndOverflow(o, &overflow);
+  if (overflow || n < INT32_MIN || n > INT32_MAX) return false;
+  *v = static_cast<int32_t>(n);
+  return true;
+}
+bool truth(PyObject* o, int32_t* v) {
+  *v = o == Py_True;
+  return o == Py_True || o == Py_False;
+}
+// float32 of these sizes, contiguous, here
+bool scales(const at::Tensor* t, at::IntArrayRef sizes) {
+  return t && here(*t) && t->scalar_type() == at::kFloat && t->sizes() == sizes && t->is_contiguous();
+}
+// int8 matrices whose rows begin and repeat on multiples of 16 bytes, here
+bool int8_stack(const at::Tensor& t) {
+  return here(t) && t.scalar_type() == at::kChar && t.dim() == 3 && t.stride(2) == 1 && t.stride(1) >= t.size(2) &&
+         t.stride(1) % 16 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+         (t.size(0) == 1 || (t.stride(0) >= t.stride(1) && t.stride(0) % 16 == 0)) && t.size(0) <= INT32_MAX &&
+         t.size(1) <= INT32_MAX && t.size(2) <= INT32_MAX;
+}
+
+// (logits, k, scoring, bias or None, groups, topk_groups or None, group_top, renormalize, scale): (weights, ids)
+PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* l = n_args == 9 ? tensor(a[0]) : nullptr;
+    int32_t k, scoring, groups, open_groups, group_top, renorm;
+    if (!l || !here(*l) || code_of(l->scalar_type()) < 0 || !matrix(*l) || recorded(*l) || !integer(a[1], &k) ||
+        !integer(a[2], &scoring) || !integer(a[4], &groups) || !integer(a[6], &group_top) || !truth(a[7], &renorm) ||
+        !PyFloat_CheckExact(a[8]))
+      Py_RETURN_NONE;
+    if (a[5] == Py_None) open_groups = groups;
+    else if (!integer(a[5], &open_groups)) Py_RETURN_NONE;
+    const int64_t T = l->size(0), E = l->size(1);
+    const at::Tensor* bias = a[3] == Py_None ? nullptr : tensor(a[3]);
+    if ((a[3] != Py_None && !scales(bias, {E})) || E > INT32_MAX || k < 1) Py_RETURN_NONE;
+    const auto f32 = l->options().dtype(at::kFloat);
+    at::Tensor weights = at::empty({T, k}, f32), ids = at::empty({T, k}, f32.dtype(at::kInt));
+    const int rc = hexmoe_route(l->data_ptr(), code_of(l->scalar_type()), l->stride(0), T, static_cast<int32_t>(E), k, scoring,
+                                bias ? bias->data_ptr<float>() : nullptr, groups, open_groups, group_top, renorm,
+                                static_cast<float>(PyFloat_AS_DOUBLE(a[8])), weights.data_ptr<float>(), ids.data_ptr<int32_t>(),
+                                stream_of(*l));
+    if (refused(rc, "hexmoe_route")) Py_RETURN_NONE;
+    PyObject* first = THPVariable_Wrap(std::move(weights));
+    if (!first) return nullptr;
+    PyObject* second = THPVariable_Wrap(std::move(ids));
+    if (!second) {
+      Py_DECREF(first);
+      return nullptr;
+    }
+    PyObject* both = PyTuple_Pack(2, first, second);
+    Py_DECREF(first);
+    Py_DECREF(second);
+    return both;
+  });
+}
+
+// (dweights, logits, ids, scoring, renormalize, scale)
+PyObject* route_backward(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *d = n_args == 6 ? tensor(a[0]) : nullptr, *l = d ? tensor(a[1]) : nullptr, *ids = l ? tensor(a[2]) : nullptr;
+    int32_t scoring, renorm;
+    if (!ids || !here(*l) || !here(*ids) || code_of(l->scalar_type()) < 0 || !matrix(*l) || ids->dim() != 2 ||
+        ids->size(0) != l->size(0) || ids->size(1) > INT32_MAX || !ids->is_contiguous() || !scales(d, ids->sizes()) ||
+        (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) || !integer(a[3], &scoring) || !truth(a[4], &renorm) ||
+        !PyFloat_CheckExact(a[5]) || l->size(1) > INT32_MAX)
+      Py_RETURN_NONE;
+    const int64_t T = l->size(0), E = l->size(1);
+    at::Tensor out = at::empty({T, E}, l->options());
+    const int rc = hexmoe_route_backward(d->data_ptr<float>(), l->data_ptr(), code_of(l->scalar_type()), l->stride(0), T,
+                                         static_cast<int32_t>(E), static_cast<int32_t>(ids->size(1)), ids->data_ptr(),
+                                         ids->scalar_type() == at::kLong ? HEXMOE_I64 : HEXMOE_I32, scoring, renorm,
+                                         static_cast<float>(PyFloat_AS_DOUBLE(a[5])), out.data_ptr(), E, stream_of(*l));
+    if (refused(rc, "hexmoe_route_backward")) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// (x, w, w_scale, offsets): x of f32, bf16 or fp16, the result in its type
+PyObject* grouped_mm_int8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *x = n_args == 4 ? tensor(a[0]) : nullptr, *w = x ? tensor(a[1]) : nullptr, *s = w ? tensor(a[2]) : nullptr,
+                     *off = s ? tensor(a[3]) : nullptr;
+    if (!off || !here(*x) || code_of(x->scalar_type()) < 0 || !matrix(*x) || recorded(*x) || !int8_stack(*w) ||
+        !scales(s, w->sizes().slice(0, 2)) || recorded(*s) || x->size(1) != w->size(2))
+      Py_RETURN_NONE;
+    const int64_t E = w->size(0), N = w->size(1), K = w->size(2), R = x->size(0);
+    const int code = code_of(x->scalar_type()), index = offsets_code(*off, E);
+    if (index < 0) Py_RETURN_NONE;
+    at::Tensor out = at::empty({R, N}, x->options()), ws;
+    const size_t bytes = hexmoe_grouped_mm_int8_workspace_bytes(R, E, N, K, code);
+    if (bytes) ws = workspace(bytes, *x);
+    const int rc = hexmoe_grouped_mm_int8(x->data_ptr(), code, x->stride(0), nullptr, w->data_ptr<int8_t>(), w->stride(1), w->stride(0),
+                                          s->data_ptr<float>(), R, E, N, K, off->data_ptr(), index, out.data_ptr(), N, code,
+                                          bytes ? ws.data_ptr() : nullptr, bytes, stream_of(*x));
+    if (refused(rc, "hexmoe_grouped_mm_int8")) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// (x, topk_weights, topk_ids, w13, w13_scale, w2, w2_scale)
+PyObject* int8_moe(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* t[7] = {};
+    for (int i = 0; i < 7; ++i)
+      if (n_args != 7 || !(t[i] = tensor(a[i]))) Py_RETURN_NONE;
+    const at::Tensor &x = *t[0], &weights = *t[1], &ids = *t[2], &w13 = *t[3], &s13 = *t[4], &w2 = *t[5], &s2 = *t[6];
+    if (!here(x) || code_of(x.scalar_type()) < 0 || !matrix(x) || !here(ids) || ids.dim() != 2 || !ids.is_contiguous() ||
+        (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong) || !scales(&weights, ids.sizes()) ||
+        !int8_stack(w13) || !int8_stack(w2) || !scales(&s13, w13.sizes().slice(0, 2)) || !scales(&s2, w2.sizes().slice(0, 2)) ||
+        recorded(x) || recorded(weights) || recorded(s13) || recorded(s2))
+      Py_RETURN_NONE;
+    const int64_t T = ids.size(0), k = ids.size(1), E = w2.size(0), H = w2.size(1), I = w2.size(2);
+    if (x.size(0) != T || x.size(1) != H || w13.size(0) != E || w13.size(1) != 2 * I || w13.size(2) != H || T == 0 || k == 0 || k > 1024)
+      Py_RETURN_NONE;
+    at::Tensor out = at::empty({T, H}, x.options());
+    const int code = code_of(x.scalar_type());
+    const size_t bytes = hexmoe_int8_forward_workspace_bytes(T, k, E, H, I);
+    at::Tensor ws = workspace(bytes, x);
+    const int rc = hexmoe_int8_forward(x.data_ptr(), code, x.stride(0), T, H, I, k, weights.data_ptr<float>(), ids.data_ptr(),
+                                       ids.scalar_type() == at::kLong ? HEXMOE_I64 : HEXMOE_I32, E, w13.data_ptr<int8_t>(), w13.stride(1),
+                                       w13.stride(0), s13.data_ptr<float>(), w2.data_ptr<int8_t>(), w2.stride(1), w2.stride(0),
+                                       s2.data_ptr<float>(), out.data_ptr(), code, ws.data_ptr(), bytes, stream_of(x));
+    if (refused(rc, "hexmoe_int8_forward")) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 PyMethodDef methods[] = {
     {"grouped_mm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(grouped_mm)), METH_FASTCALL, nullptr},
     {"grouped_wgrad", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(grouped_wgrad)), METH_FASTCALL, nullptr},
     {"swiglu", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(swiglu)), METH_FASTCALL, nullptr},
     {"swiglu_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(swiglu_backward)), METH_FASTCALL, nullptr},
     {"clip_grad_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(clip_grad_norm)), METH_FASTCALL, nullptr},
+    {"route", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(route)), METH_FASTCALL, nullptr},
+    {"route_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(route_backward)), METH_FASTCALL, nullptr},
+    {"grouped_mm_int8", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(grouped_mm_int8)), METH_FASTCALL, nullptr},
+    {"int8_moe", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(int8_moe)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
-PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_call", "Calls of blackhole_b200.experts for ordinary arguments.", -1, methods};
+PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_call", "Calls of blackhole_b200.experts, router and int8 for ordinary arguments.", -1, methods};
 
 }  // namespace
 

@@ -395,6 +395,9 @@ constexpr bool k_major(int mode) { return mode == kRowsK || is_int8(mode); }   /
 //            takes the issuing warp some 450 cycles, more than narrow products run: twice the step
 //            (one token on 96 experts, 1536 x 2048: 64 wide 14.5 us, 128 wide 13.1, 12.6 with the fifth step).
 //   kMiddle  up to 128: 4 steps of 48 KB, 128 wide
+// 8-bit products take kOne for all wide tiles: their products run half as long, so that kTwo's drain between tiles shows
+// (96 experts x 341 rows, 1536 x 2048 with SwiGLU: 109 us, kTwo 140; 2048 x 768: 71 and 89).  Three steps of 64 KB instead
+// of six of 32: 116 and 73.
 enum PairShape { kOne = 0, kTwo = 1, kNarrow = 2, kMiddle = 3 };
 constexpr int subs_of(int shape) { return shape >= kNarrow ? 2 : 1; }   // 64-wide blocks of a step
 constexpr int span_of(int shape) {                                      // most rows of a tile
@@ -1138,9 +1141,8 @@ int sm_count(int* sms) {
                           PAIR_KERNELS(kRowsK, kMiddle), PAIR_KERNELS(kRowsMN, kOne), PAIR_KERNELS(kRowsMN, kTwo),
                           PAIR_KERNELS(kRowsMN, kNarrow), PAIR_KERNELS(kRowsMN, kMiddle), PAIR_KERNELS(kWgrad, kOne),
                           PAIR_KERNELS(kWgrad, kMiddle), PAIR_KERNELS(kWgradT, kOne), PAIR_KERNELS(kWgradT, kMiddle),
-                          INT8_KERNEL(kInt8, kOne), INT8_KERNEL(kInt8, kTwo), INT8_KERNEL(kInt8, kNarrow),
-                          INT8_KERNEL(kInt8, kMiddle), INT8_KERNEL(kInt8Glu, kOne), INT8_KERNEL(kInt8Glu, kTwo),
-                          INT8_KERNEL(kInt8Glu, kNarrow), INT8_KERNEL(kInt8Glu, kMiddle)}) {
+                          INT8_KERNEL(kInt8, kNarrow), INT8_KERNEL(kInt8, kMiddle), INT8_KERNEL(kInt8, kOne),
+                          INT8_KERNEL(kInt8Glu, kNarrow), INT8_KERNEL(kInt8Glu, kMiddle), INT8_KERNEL(kInt8Glu, kOne)}) {
       e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
       if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
     }
@@ -1214,6 +1216,10 @@ PairShape rows_shape(int64_t rows, int32_t experts, int32_t m_len) {
   if (rows <= 128 || rows <= 96ll * experts || row_tiles(rows, experts, m_len, kMiddle) <= kPairsPlanned) return kMiddle;
   const bool fills = static_cast<int64_t>(experts) * ((m_len + 255) / 256) >= 2 * kPairsPlanned;
   return rows > 256ll * experts && rows <= 512ll * experts && fills ? kTwo : kOne;
+}
+PairShape int8_shape(int64_t rows, int32_t experts, int32_t m_len) {
+  const PairShape shape = rows_shape(rows, experts, m_len);
+  return shape == kTwo ? kOne : shape;
 }
 int rows_splits(int64_t rows, int32_t experts, int32_t m_len, int32_t red) {
   const PairShape shape = rows_shape(rows, experts, m_len);
@@ -1372,7 +1378,7 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
   q.stride_split = d.rows * pitch;
   q.f32 = split || f32; q.bf16 = bf16;
   q.dev_err = dev_err;
-  const PairShape shape = rows_shape(d.rows, d.experts, d.n);
+  const PairShape shape = int8_shape(d.rows, d.experts, d.n);
   const int64_t tiles = row_tiles(d.rows, d.experts, d.n, shape) * q.splits;
   if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
   constexpr CUtensorMapDataType kBytes = CU_TENSOR_MAP_DATA_TYPE_UINT8;
@@ -1399,7 +1405,6 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
     constexpr int MODE = decltype(mode)::value;
     return shape == kNarrow   ? launch_pair<MODE, kNarrow>(q, tiles, sms, st)
            : shape == kMiddle ? launch_pair<MODE, kMiddle>(q, tiles, sms, st)
-           : shape == kTwo    ? launch_pair<MODE, kTwo>(q, tiles, sms, st)
                               : launch_pair<MODE, kOne>(q, tiles, sms, st);
   };
   cudaError_t e = d.glu ? launch(std::integral_constant<int, kInt8Glu>{}) : launch(std::integral_constant<int, kInt8>{});

@@ -8,8 +8,8 @@
 // experts in order.  Bound by latency and issue, not by bytes: a token's row is a few hundred.
 //
 // Order is decided as in 64 bits.  What is compared without a bias are the logits themselves, which nothing has rounded.
-// Sums s + b and groups' values are computed in f32 first; where two that a decision lies between are nearer than their
-// errors' bound (a token in a hundred), the warp computes them again in f64 and decides by those.
+// Sums s + b and groups' values are computed in f32 first, with fast exponentials; where two that a decision lies between
+// are nearer than their errors' bound (a token in a thousand), the warp chooses again in f64 (choose_exact).
 #include <cstdarg>
 #include <cstdio>
 #include <type_traits>
@@ -43,6 +43,8 @@ struct RouteParams {
   void* dlogits;          // backward
   int64_t tokens, ld, ld_d;
   int32_t experts, topk, groups, topk_groups, group_top, renorm, ids64;
+  int32_t vec;            // rows (and biases) begin on 16 bytes and are whole pieces of 16 bytes
+  int32_t group_lanes;    // lanes whose experts make a group, where they are whole lanes and a power of two; else 0
   float scale;
 };
 
@@ -87,77 +89,104 @@ __device__ __forceinline__ double value_of(uint64_t k) {
   return k <= 1 ? __longlong_as_double(0x7ff8000000000000ll)
                 : __longlong_as_double(static_cast<long long>(k ^ (k >> 63 ? 1ull << 63 : ~0ull)));
 }
-__device__ __forceinline__ uint32_t warp_max_key(uint32_t k) { return __reduce_max_sync(kAll, k); }
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
   const uint32_t hi = __reduce_max_sync(kAll, static_cast<uint32_t>(k >> 32));
   const uint32_t lo = __reduce_max_sync(kAll, static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
   return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
-__device__ __forceinline__ float exp_of(float v) { return expf(v); }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
-
 // 1 / (1 + e^-l) without an overflow, and without a cancellation at either end.
-template <typename F>
-__device__ __forceinline__ F sigmoid(F l) {
-  const F e = exp_of(l < F(0) ? l : -l), r = F(1) / (F(1) + e);
-  return l < F(0) ? e * r : r;
+__device__ __forceinline__ float sigmoid(float l) {
+  const float e = expf(l < 0.f ? l : -l), r = 1.f / (1.f + e);
+  return l < 0.f ? e * r : r;
 }
 
-// A token's logits, one warp: NI to a lane, -inf past the last expert; largest is their largest, ignoring NaN.
+// A token's values (logits, biases), NI to a lane, `none` past the last expert; in pieces of 16 bytes where p.vec says
+// that rows begin on such.
 template <typename T, int NI>
-__device__ __forceinline__ void load_row(const RouteParams& p, int64_t t, float (&l)[NI]) {
-  const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+__device__ __forceinline__ void load_row(const RouteParams& p, const T* row, float none, float (&l)[NI]) {
   const int e0 = threadIdx.x % 32 * NI;
+  if constexpr (NI * sizeof(T) % 16 == 0) {
+    if (p.vec) {
+      constexpr int kWords = NI * sizeof(T) / 4, kPer = 4 / sizeof(T);
+      uint32_t w[kWords];
 #pragma unroll
-  for (int i = 0; i < NI; ++i) l[i] = e0 + i < p.experts ? widen(row[e0 + i]) : -INFINITY;
+      for (int i = 0; i < kWords; i += 4) {
+        if (e0 + i * kPer < p.experts) {   // whole pieces: experts are a multiple of a piece
+          const uint4 v = *reinterpret_cast<const uint4*>(row + e0 + i * kPer);
+          w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        if constexpr (sizeof(T) == 4) l[i] = __uint_as_float(w[i]);
+        else if constexpr (std::is_same_v<T, __half>) l[i] = __half2float(__ushort_as_half(static_cast<uint16_t>(w[i / 2] >> i % 2 * 16)));
+        else l[i] = __uint_as_float(i % 2 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        if (e0 + i >= p.experts) l[i] = none;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NI; ++i) l[i] = e0 + i < p.experts ? widen(row[e0 + i]) : none;
 }
 template <int NI>
-__device__ __forceinline__ float largest_of(const float (&l)[NI]) {
+__device__ __forceinline__ float largest_of(const float (&l)[NI]) {   // ignoring NaN
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < NI; ++i) m = fmaxf(m, l[i]);
   return warp_max(m);
 }
+// e^x and 1 / x to 2 units in the last place, and the rounding of x log2 e (|x| 2^-24 of the result).
+__device__ __forceinline__ float fast_exp(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x * 1.44269504f));
+  return r;
+}
+__device__ __forceinline__ float fast_inverse(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 
-// The scores of a row.  Masked experts (-inf) have 0, also where every one is masked.
-template <typename F, int NI, bool SIGMOID>
-__device__ __forceinline__ void scores_of(const float (&l)[NI], float largest, F (&s)[NI], F& sum) {
-  sum = F(1);
+// The scores of a row, for comparing.  Masked experts (-inf) have 0, also where every one is masked.  Returns the largest.
+template <int NI, bool SIGMOID>
+__device__ __forceinline__ float scores_of(const float (&l)[NI], float largest, float (&s)[NI]) {
   if constexpr (SIGMOID) {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) s[i] = l[i] == -INFINITY ? F(0) : sigmoid(F(l[i]));
+    for (int i = 0; i < NI; ++i) s[i] = fast_inverse(1.f + fast_exp(-l[i]));
+    return 1.f;
   } else {
-    F part = F(0);
+    float part = 0.f;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      s[i] = l[i] == -INFINITY ? F(0) : exp_of(F(l[i]) - F(largest));
+      s[i] = l[i] == -INFINITY ? 0.f : fast_exp(l[i] - largest);
       part += s[i];
     }
-    sum = warp_sum(part);
-    const F inv = sum > F(0) || sum != sum ? F(1) / sum : F(0);
+    const float sum = warp_sum(part), inv = sum == 0.f ? 0.f : fast_inverse(sum);
 #pragma unroll
     for (int i = 0; i < NI; ++i) s[i] *= inv;
+    return inv;
   }
 }
 
 // What a selection finds: lane j holds the j-th expert and its key; next: the key behind the last one.
-template <typename K>
 struct Picked {
   int32_t id;
-  K key, next;
+  uint32_t key, next;
 };
 
 // The k largest of a warp's keys, equal ones by lane and place.  Keys that are chosen become 0.
-template <typename K, int NI>
-__device__ __forceinline__ Picked<K> pick(K (&key)[NI], int k, bool want_next) {
+template <int NI>
+__device__ __forceinline__ Picked pick(uint32_t (&key)[NI], int k, bool want_next) {
   const int lane = threadIdx.x % 32;
-  Picked<K> got{0, 0, 0};
-  for (int j = 0; j < k + (want_next ? 1 : 0); ++j) {
-    K best = key[0];
+  Picked got{0, 0, 0};
+  for (int j = 0;; ++j) {
+    if (j == k && !want_next) break;
+    uint32_t best = key[0];
 #pragma unroll
-    for (int i = 1; i < NI; ++i) best = key[i] > best ? key[i] : best;
-    const K top = warp_max_key(best);
+    for (int i = 1; i < NI; ++i) best = max(best, key[i]);
+    const uint32_t top = __reduce_max_sync(kAll, best);
     if (j == k) {
       got.next = top;
       break;
@@ -168,7 +197,7 @@ __device__ __forceinline__ Picked<K> pick(K (&key)[NI], int k, bool want_next) {
     for (int i = NI - 1; i >= 0; --i) at = key[i] == top ? i : at;
     if (lane == owner) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i) key[i] = i == at ? K(0) : key[i];
+      for (int i = 0; i < NI; ++i) key[i] = i == at ? 0u : key[i];
     }
     const int id = __shfl_sync(kAll, lane * NI + at, owner);
     if (lane == j) {
@@ -179,105 +208,210 @@ __device__ __forceinline__ Picked<K> pick(K (&key)[NI], int k, bool want_next) {
   return got;
 }
 
-// The open groups as a bit each, from the values s + b (as keys).  near: whether a decision lay between two values
-// less than `tau` apart.
-template <typename F, typename K, int NI>
-__device__ __forceinline__ uint32_t open_groups(const RouteParams& p, const K (&key)[NI], F tau, bool& near) {
-  const int lane = threadIdx.x % 32, per = p.experts / p.groups, e0 = lane * NI;
-  F mine = F(0);
-  for (int g = 0; g < p.groups; ++g) {
-    K first = 0, second = 0;   // of this lane's experts in the group
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const K k = e0 + i >= g * per && e0 + i < (g + 1) * per ? key[i] : K(0);
-      if (k > first) {
-        second = first;
-        first = k;
-      } else if (k > second) {
-        second = k;
-      }
-    }
-    const K top = warp_max_key(first);
-    F v = value_of(top);
-    if (p.group_top > 1 && per > 1) {
-      const int owner = __ffs(__ballot_sync(kAll, first == top)) - 1;
-      v += value_of(warp_max_key(lane == owner ? second : first));
-    }
-    if (lane == g) mine = v;
-  }
-  int ahead = 0;
-  const K my_key = lane < p.groups ? key_of(mine) : K(0);
-  for (int g = 0; g < p.groups; ++g) {
-    const K other = __shfl_sync(kAll, my_key, g);
-    ahead += other > my_key || (other == my_key && g < lane);
-  }
-  const bool open = lane < p.groups && ahead < p.topk_groups;
-  if (near) {   // asked for: the last open value and the first closed one
-    const F last = value_of(__shfl_sync(kAll, my_key, __ffs(__ballot_sync(kAll, lane < p.groups && ahead == p.topk_groups - 1)) - 1));
-    const F next = value_of(__shfl_sync(kAll, my_key, __ffs(__ballot_sync(kAll, lane < p.groups && ahead == p.topk_groups)) - 1));
-    near = !(last - next > tau);
-  }
-  return __ballot_sync(kAll, open);
+__device__ __forceinline__ void add_top(uint32_t key, uint32_t& first, uint32_t& second) {
+  const uint32_t less = min(first, key);
+  first = max(first, key);
+  second = max(second, less);
 }
 
-// One token's choice in type F (float, double).  near: set where f32 could not decide.
-template <typename F, int NI, bool SIGMOID>
-__device__ __forceinline__ int32_t choose(const RouteParams& p, const float (&l)[NI], float largest, bool& near) {
-  using K = std::conditional_t<std::is_same_v<F, float>, uint32_t, uint64_t>;
-  const int e0 = threadIdx.x % 32 * NI, lane = threadIdx.x % 32;
-  const bool grouped = p.topk_groups < p.groups;
-  K key[NI];
-  F tau = F(0);
-  if (p.bias || grouped) {
-    F s[NI], sum;
-    scores_of<F, NI, SIGMOID>(l, largest, s, sum);
-    float widest = 0.f;
+// The open groups as a bit each, from the values s + b (as keys).  near: a decision lay between two values no more
+// than `tau` apart.
+template <int NI>
+__device__ __forceinline__ uint32_t open_groups(const RouteParams& p, const uint32_t (&key)[NI], float tau, bool& near) {
+  const int lane = threadIdx.x % 32, per = p.experts / p.groups;
+  const bool two = p.group_top > 1 && per > 1;
+  float mine = 0.f;
+  if (p.group_lanes) {   // a group is so many whole lanes, a power of two
+    uint32_t first = 0, second = 0;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      F c = s[i];
-      if (e0 + i < p.experts) {
-        if (p.bias) c = l[i] == -INFINITY ? F(-INFINITY) : c + F(p.bias[e0 + i]);
-        key[i] = key_of(c);
-      } else {
-        key[i] = 0;
+    for (int i = 0; i < NI; ++i) add_top(key[i], first, second);
+    for (int o = 1; o < p.group_lanes; o <<= 1) {
+      const uint32_t f = __shfl_xor_sync(kAll, first, o), g = __shfl_xor_sync(kAll, second, o);
+      add_top(f, first, second);
+      second = max(second, g);
+    }
+    const float v = two ? value_of(first) + value_of(second) : value_of(first);
+    mine = __shfl_sync(kAll, v, lane * p.group_lanes);
+  } else {
+    const int e0 = lane * NI;
+    for (int g = 0; g < p.groups; ++g) {
+      uint32_t first = 0, second = 0;   // of this lane's experts in the group
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        add_top(e0 + i >= g * per && e0 + i < (g + 1) * per ? key[i] : 0u, first, second);
+      const uint32_t top = __reduce_max_sync(kAll, first);
+      float v = value_of(top);
+      if (two) {
+        const int owner = __ffs(__ballot_sync(kAll, first == top)) - 1;
+        v += value_of(__reduce_max_sync(kAll, lane == owner ? second : first));
       }
-      if (fabs(c) < F(INFINITY)) widest = fmaxf(widest, static_cast<float>(fabs(c)));
+      if (lane == g) mine = v;
     }
-    if constexpr (std::is_same_v<F, float>) {
-      // f32 errors, in units of 2^-24: a sigmoid 8 of itself (the exponential 4, the sum, the divide); a softmax score
-      // 40 (the exponent's rounding, up to 30 where the score counts, the exponential, the divide) and one for each
-      // addition of its sum; the addition of the bias 1.  Two of each stand on the sides of a decision, and twice as
-      // many where a group's value adds two.
-      const float top = SIGMOID ? 1.f : (sum > 0.f ? 1.f / sum : 0.f);
-      tau = 0x1p-23f * ((SIGMOID ? 8.f : 45.f + NI) * top + 2.f * warp_max(widest));
+  }
+  int ahead = 0;
+  const uint32_t my_key = lane < p.groups ? key_of(mine) : 0u;
+  for (int g = 0; g < p.groups; ++g) {
+    const uint32_t other = __shfl_sync(kAll, my_key, g);
+    ahead += other > my_key || (other == my_key && g < lane);
+  }
+  const bool in = lane < p.groups;
+  // the last open value and the first closed one
+  const uint32_t last = __shfl_sync(kAll, my_key, __ffs(__ballot_sync(kAll, in && ahead == p.topk_groups - 1)) - 1);
+  const uint32_t next = __shfl_sync(kAll, my_key, __ffs(__ballot_sync(kAll, in && ahead == p.topk_groups)) - 1);
+  near = !(value_of(last) - value_of(next) > tau);
+  return __ballot_sync(kAll, in && ahead < p.topk_groups);
+}
+
+// One token's experts, lane j the j-th.  near: f32 could not decide.
+template <int NI, bool SIGMOID>
+__device__ __forceinline__ int32_t choose(const RouteParams& p, const float (&l)[NI], float largest, bool& near) {
+  const int lane = threadIdx.x % 32, e0 = lane * NI;
+  const bool grouped = p.topk_groups < p.groups;
+  near = false;
+  uint32_t key[NI];
+  float tau = 0.f;
+  if (p.bias || grouped) {
+    float c[NI], widest = 0.f;
+    const float top = scores_of<NI, SIGMOID>(l, largest, c);
+    if (p.bias) {
+      float b[NI];
+      load_row(p, p.bias, 0.f, b);
+#pragma unroll
+      for (int i = 0; i < NI; ++i) c[i] = l[i] == -INFINITY ? -INFINITY : c[i] + b[i];
     }
-    uint32_t open = kAll;
-    if (grouped) {
-      near = std::is_same_v<F, float>;
-      open = open_groups<F>(p, key, F(2) * tau, near);
-      if (near) return 0;
-    }
-    const int per = p.experts / p.groups;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      if (!p.bias) key[i] = e0 + i < p.experts ? K(key_of(F(l[i]))) : K(0);
-      if (grouped && !(open >> ((e0 + i) / per & 31) & 1)) key[i] = 0;
+      key[i] = e0 + i < p.experts ? key_of(c[i]) : 0u;
+      const float size = fabsf(c[i]);
+      widest = fmaxf(widest, size < INFINITY ? size : 0.f);
+    }
+    // Errors of the values, in units of 2^-24: a sigmoid 16 of 1 (of s (1 - s) times the exponential's 4 and its
+    // argument's |l|, of s the sum's 1 and the reciprocal's 4); a softmax score, of the largest one, 48 (the exponential's
+    // 4, its argument's two roundings, which count as much as |x| e^x, the reciprocal's 4, the product) and one for each
+    // addition of a lane's sum and five of the warp's; the addition of the bias 1.  Two of each stand on the sides of a
+    // decision, and twice as many where a group's value adds two.
+    tau = 0x1p-23f * ((SIGMOID ? 16.f : 48.f + NI) * top + 2.f * __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(widest))));
+    if (grouped) {
+      const uint32_t open = open_groups(p, key, 2.f * tau, near);
+      if (near) return 0;
+      if (!p.bias) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) key[i] = e0 + i < p.experts ? key_of(l[i]) : 0u;
+      }
+      if (p.group_lanes) {
+        if (!(open >> lane / p.group_lanes & 1)) {
+#pragma unroll
+          for (int i = 0; i < NI; ++i) key[i] = 0;
+        }
+      } else {
+        const int per = p.experts / p.groups;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          if (!(open >> ((e0 + i) / per & 31) & 1)) key[i] = 0;
+      }
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < NI; ++i) key[i] = e0 + i < p.experts ? K(key_of(F(l[i]))) : K(0);
+    for (int i = 0; i < NI; ++i) key[i] = e0 + i < p.experts ? key_of(l[i]) : 0u;
   }
-  const bool check = std::is_same_v<F, float> && p.bias;
-  const Picked<K> got = pick(key, p.topk, check);
-  near = false;
-  if (check) {
-    const K behind = __shfl_down_sync(kAll, got.key, 1);
-    const F v = value_of(got.key), next = value_of(lane == p.topk - 1 ? got.next : behind);
-    // nothing chosen lies behind the last one, or both are masked: by their ids, whatever their errors
-    const bool sure = (lane == p.topk - 1 && got.next == 0) || (v == F(-INFINITY) && next == F(-INFINITY));
+  const Picked got = pick(key, p.topk, p.bias != nullptr);
+  if (p.bias) {
+    const uint32_t behind = __shfl_down_sync(kAll, got.key, 1);
+    const bool end = lane == p.topk - 1;
+    const float v = value_of(got.key), next = value_of(end ? got.next : behind);
+    // nothing lies behind the last one, or both are masked: by their ids, whatever their errors
+    const bool sure = (end && got.next == 0) || (v == -INFINITY && next == -INFINITY);
     near = __any_sync(kAll, lane < p.topk && !sure && !(v - next > tau));
   }
   return got.id;
+}
+
+// The same choice with everything in f64.  Rolled loops over local memory and one exponential: tokens come here one by
+// one, and what they wait for is mostly the code.
+template <typename T, bool SIGMOID>
+__device__ __noinline__ int32_t choose_exact(const RouteParams& p, int64_t t, float largest) {
+  const int lane = threadIdx.x % 32, held = (p.experts + 31) / 32, e0 = lane * held, per = p.experts / p.groups;
+  const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+  uint64_t key[kMaxExperts / 32];
+  double sum = 0.0;
+#pragma unroll 1
+  for (int i = 0; i < held; ++i) {
+    const float l = e0 + i < p.experts ? widen(row[e0 + i]) : -INFINITY;
+    double s = 0.0;
+    if (l != -INFINITY) {
+      const double d = l, e = exp(SIGMOID ? (d < 0 ? d : -d) : d - static_cast<double>(largest));
+      s = SIGMOID ? (d < 0 ? e : 1.0) / (1.0 + e) : e;
+    }
+    sum += s;
+    key[i] = static_cast<uint64_t>(__double_as_longlong(s));
+  }
+  if constexpr (SIGMOID) sum = 1.0;
+  else sum = warp_sum(sum);
+#pragma unroll 1
+  for (int i = 0; i < held; ++i) {
+    const int e = e0 + i;
+    if (e >= p.experts) {
+      key[i] = 0;
+      continue;
+    }
+    double c = __longlong_as_double(static_cast<long long>(key[i]));
+    if (!SIGMOID && sum != 0.0) c /= sum;
+    if (p.bias) c = widen(row[e]) == -INFINITY ? -INFINITY : c + static_cast<double>(p.bias[e]);
+    key[i] = key_of(c);
+  }
+  if (p.topk_groups < p.groups) {
+    uint64_t mine = 0;
+#pragma unroll 1
+    for (int g = 0; g < p.groups; ++g) {
+      uint64_t first = 0, second = 0;
+#pragma unroll 1
+      for (int i = 0; i < held; ++i) {
+        const int e = e0 + i;
+        if (e < g * per || e >= (g + 1) * per) continue;
+        second = max(second, min(first, key[i]));
+        first = max(first, key[i]);
+      }
+      const uint64_t top = warp_max_key(first);
+      double v = value_of(top);
+      if (p.group_top > 1 && per > 1) {
+        const int owner = __ffs(__ballot_sync(kAll, first == top)) - 1;
+        v += value_of(warp_max_key(lane == owner ? second : first));
+      }
+      if (lane == g) mine = key_of(v);
+    }
+    int ahead = 0;
+#pragma unroll 1
+    for (int g = 0; g < p.groups; ++g) {
+      const uint64_t other = __shfl_sync(kAll, mine, g);
+      ahead += other > mine || (other == mine && g < lane);
+    }
+    const uint32_t open = __ballot_sync(kAll, lane < p.groups && ahead < p.topk_groups);
+#pragma unroll 1
+    for (int i = 0; i < held; ++i) {
+      const int e = e0 + i;
+      if (e >= p.experts) continue;
+      if (!p.bias) key[i] = key_of(static_cast<double>(widen(row[e])));
+      if (!(open >> (e / per) & 1)) key[i] = 0;
+    }
+  }
+  int32_t id = 0;
+#pragma unroll 1
+  for (int j = 0; j < p.topk; ++j) {
+    uint64_t best = 0;
+    int at = 0;
+#pragma unroll 1
+    for (int i = 0; i < held; ++i) {
+      if (key[i] > best) {
+        best = key[i];
+        at = i;
+      }
+    }
+    const uint64_t top = warp_max_key(best);
+    const int owner = __ffs(__ballot_sync(kAll, best == top)) - 1, found = __shfl_sync(kAll, e0 + at, owner);
+    if (lane == owner) key[at] = 0;
+    if (lane == j) id = found;
+  }
+  return id;
 }
 
 // The share of every chosen score (lane j < k: logit l, else used = false) in their sum.
@@ -300,11 +434,11 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
   pdl_wait();
   if (t >= p.tokens) return;
   float l[NI];
-  load_row<T>(p, t, l);
-  const float largest = largest_of(l);
-  bool near = false;
-  int32_t id = choose<float, NI, SIGMOID>(p, l, largest, near);
-  if (near) id = choose<double, NI, SIGMOID>(p, l, largest, near);
+  load_row(p, static_cast<const T*>(p.logits) + t * p.ld, -INFINITY, l);
+  const float largest = SIGMOID ? 0.f : largest_of(l);
+  bool near;
+  int32_t id = choose<NI, SIGMOID>(p, l, largest, near);
+  if (near) id = choose_exact<T, SIGMOID>(p, t, largest);
   const bool used = lane < p.topk;
   const float mine = used ? widen(static_cast<const T*>(p.logits)[t * p.ld + id]) : -INFINITY;
   float w;
@@ -357,11 +491,19 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
   const bool dense = !SIGMOID && !p.renorm;
   float value;
   if (dense) {
-    float l[NI], s[NI], sum;
-    load_row<T>(p, t, l);
+    float l[NI], s[NI];
+    load_row(p, row, -INFINITY, l);
     const float largest = largest_of(l);
-    scores_of<float, NI, false>(l, largest, s, sum);
-    const float score = mine == -INFINITY ? 0.f : expf(mine - largest) / sum;
+    float part = 0.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      s[i] = l[i] == -INFINITY ? 0.f : expf(l[i] - largest);
+      part += s[i];
+    }
+    const float sum = warp_sum(part), inv = sum == 0.f ? 0.f : 1.f / sum;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) s[i] *= inv;
+    const float score = mine == -INFINITY ? 0.f : expf(mine - largest) * inv;
     const float dot = warp_sum(score * d);
 #pragma unroll
     for (int i = 0; i < NI; ++i)
@@ -396,7 +538,11 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
 }
 
 template <typename T, int NI, bool SIGMOID>
-cudaError_t launch_one(const RouteParams& p, bool backward, cudaStream_t st) {
+cudaError_t launch_one(RouteParams p, bool backward, cudaStream_t st) {
+  const int per = p.experts / p.groups, lanes = per / NI;
+  p.group_lanes = per % NI == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
+  p.vec = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld * sizeof(T) % 16 == 0 && p.experts * sizeof(T) % 16 == 0 &&
+          reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && (!p.bias || p.experts % 4 == 0);
   // a token a warp: blocks of one warp until every SM has some
   const int warps = p.tokens <= 148 * 8 ? 1 : kRouteThreads / 32;
   const int64_t blocks = (p.tokens + warps - 1) / warps;
