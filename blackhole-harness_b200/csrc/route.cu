@@ -8,8 +8,10 @@
 // experts in order.  Bound by latency and issue, not by bytes: a token's row is a few hundred.
 //
 // Order is decided as in 64 bits.  What is compared without a bias are the logits themselves, which nothing has rounded.
-// Sums s + b and groups' values are computed in f32 first, with fast exponentials; where two that a decision lies between
-// are nearer than their errors' bound (a token in a thousand), the warp chooses again in f64 (choose_exact).
+// Sums s + b and groups' values are computed in f32 first, with fast exponentials.  Where two that a decision lies between
+// are nearer than their errors' bound (a token in a thousand), the values in question alone are computed again in f64, an
+// expert a lane: a warp that took its whole row through f64 would keep the kernel waiting (8192 tokens: 28 us of which 15
+// were such rows').  Only where more than 32 experts are that near does the whole row go through choose_exact.
 #include <cstdarg>
 #include <cstdio>
 #include <type_traits>
@@ -89,6 +91,7 @@ __device__ __forceinline__ double value_of(uint64_t k) {
   return k <= 1 ? __longlong_as_double(0x7ff8000000000000ll)
                 : __longlong_as_double(static_cast<long long>(k ^ (k >> 63 ? 1ull << 63 : ~0ull)));
 }
+constexpr uint32_t kMasked = 0x007fffffu;   // the key of -inf; NaN lies below
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
   const uint32_t hi = __reduce_max_sync(kAll, static_cast<uint32_t>(k >> 32));
   const uint32_t lo = __reduce_max_sync(kAll, static_cast<uint32_t>(k >> 32) == hi ? static_cast<uint32_t>(k) : 0u);
@@ -170,26 +173,59 @@ __device__ __forceinline__ float scores_of(const float (&l)[NI], float largest, 
   }
 }
 
-// What a selection finds: lane j holds the j-th expert and its key; next: the key behind the last one.
-struct Picked {
-  int32_t id;
-  uint32_t key, next;
-};
+// What is left of a row's softmax in f64: 1 for a sigmoid, the sum of e^(l - largest) otherwise.
+template <typename T, bool SIGMOID>
+__device__ __noinline__ double exact_sum(const RouteParams& p, const T* row, float largest) {
+  if constexpr (SIGMOID) return 1.0;
+  double part = 0.0;
+#pragma unroll 1
+  for (int e = threadIdx.x % 32; e < p.experts; e += 32) {
+    const float l = widen(row[e]);
+    if (l != -INFINITY) part += exp(static_cast<double>(l) - static_cast<double>(largest));
+  }
+  return warp_sum(part);
+}
+// s + b of one expert in f64.
+template <typename T, bool SIGMOID>
+__device__ __noinline__ double exact_value(const RouteParams& p, const T* row, int e, float largest, double sum) {
+  const float l = widen(row[e]);
+  const double d = l;
+  double s = 0.0;
+  if (l != -INFINITY) {
+    const double x = exp(SIGMOID ? (d < 0 ? d : -d) : d - static_cast<double>(largest));
+    s = SIGMOID ? (d < 0 ? x : 1.0) / (1.0 + x) : x / sum;
+  }
+  if (!p.bias) return s;
+  return l == -INFINITY ? -INFINITY : s + static_cast<double>(p.bias[e]);
+}
 
-// The k largest of a warp's keys, equal ones by lane and place.  Keys that are chosen become 0.
+// The k largest of a warp's keys in order, equal ones by lane and place, and as many behind them as lie no more than tau
+// apart from one to the next.  Keys that are chosen become 0.
+struct Picked {
+  int32_t id, count;   // lane j: the j-th expert; how many there are
+  uint32_t key;
+  bool near;           // two of them, or the last and what follows, lie no more than tau apart
+};
 template <int NI>
-__device__ __forceinline__ Picked pick(uint32_t (&key)[NI], int k, bool want_next) {
+__device__ __forceinline__ Picked pick(uint32_t (&key)[NI], int k, bool compare, float tau) {
   const int lane = threadIdx.x % 32;
-  Picked got{0, 0, 0};
+  Picked got{0, k, 0, false};
+  uint32_t before = 0;
   for (int j = 0;; ++j) {
-    if (j == k && !want_next) break;
+    if (j >= k && !compare) break;
     uint32_t best = key[0];
 #pragma unroll
     for (int i = 1; i < NI; ++i) best = max(best, key[i]);
     const uint32_t top = __reduce_max_sync(kAll, best);
-    if (j == k) {
-      got.next = top;
-      break;
+    if (compare) {
+      // masked ones (-inf, and NaN) are told apart by their ids, whatever their errors
+      const bool close = j > 0 && top > kMasked && !(value_of(before) - value_of(top) > tau);
+      got.near |= close;
+      if (j >= k && (!close || j == 32)) {
+        got.count = close ? 33 : j;
+        break;
+      }
+      before = top;
     }
     const int owner = __ffs(__ballot_sync(kAll, best == top)) - 1;
     int at = 0;
@@ -214,12 +250,11 @@ __device__ __forceinline__ void add_top(uint32_t key, uint32_t& first, uint32_t&
   second = max(second, less);
 }
 
-// The open groups as a bit each, from the values s + b (as keys).  near: a decision lay between two values no more
-// than `tau` apart.
-template <int NI>
-__device__ __forceinline__ uint32_t open_groups(const RouteParams& p, const uint32_t (&key)[NI], float tau, bool& near) {
+// The open groups as a bit each, from the values s + b (as keys); tau: what two groups' values may be off by together.
+template <typename T, int NI, bool SIGMOID>
+__device__ __forceinline__ uint32_t open_groups(const RouteParams& p, const T* row, const uint32_t (&key)[NI], float tau, float largest) {
   const int lane = threadIdx.x % 32, per = p.experts / p.groups;
-  const bool two = p.group_top > 1 && per > 1;
+  const bool two = p.group_top > 1 && per > 1, in = lane < p.groups;
   float mine = 0.f;
   if (p.group_lanes) {   // a group is so many whole lanes, a power of two
     uint32_t first = 0, second = 0;
@@ -248,26 +283,57 @@ __device__ __forceinline__ uint32_t open_groups(const RouteParams& p, const uint
       if (lane == g) mine = v;
     }
   }
-  int ahead = 0;
-  const uint32_t my_key = lane < p.groups ? key_of(mine) : 0u;
-  for (int g = 0; g < p.groups; ++g) {
-    const uint32_t other = __shfl_sync(kAll, my_key, g);
-    ahead += other > my_key || (other == my_key && g < lane);
+  auto rank = [&](auto k) {
+    int ahead = 0;
+#pragma unroll 4
+    for (int g = 0; g < p.groups; ++g) {
+      const auto other = __shfl_sync(kAll, k, g);
+      ahead += other > k || (other == k && g < lane);
+    }
+    return ahead;
+  };
+  const uint32_t my_key = in ? key_of(mine) : 0u;
+  int ahead = rank(my_key);
+  // the last open group and the first closed one
+  const float last = value_of(__shfl_sync(kAll, my_key, __ffs(__ballot_sync(kAll, in && ahead == p.topk_groups - 1)) - 1));
+  const float next = value_of(__shfl_sync(kAll, my_key, __ffs(__ballot_sync(kAll, in && ahead == p.topk_groups)) - 1));
+  if (!(last - next > tau) && !(last == -INFINITY && next == -INFINITY)) {
+    // groups that near to the border: their values in f64, a warp on each
+    const float away = fminf(fabsf(mine - last), fabsf(mine - next));
+    const double sum = exact_sum<T, SIGMOID>(p, row, largest);
+    double value = mine;
+    uint32_t doubt = __ballot_sync(kAll, in && !(away > 2.f * tau));
+    while (doubt) {
+      const int g = __ffs(doubt) - 1;
+      doubt &= doubt - 1;
+      uint64_t first = 0, second = 0;
+#pragma unroll 1
+      for (int e = g * per + lane; e < (g + 1) * per; e += 32) {
+        const uint64_t k = key_of(exact_value<T, SIGMOID>(p, row, e, largest, sum));
+        second = max(second, min(first, k));
+        first = max(first, k);
+      }
+      const uint64_t top = warp_max_key(first);
+      double v = value_of(top);
+      if (two) {
+        const int owner = __ffs(__ballot_sync(kAll, first == top)) - 1;
+        v += value_of(warp_max_key(lane == owner ? second : first));
+      }
+      if (lane == g) value = v;
+    }
+    ahead = rank(in ? key_of(value) : 0ull);
   }
-  const bool in = lane < p.groups;
-  // the last open value and the first closed one
-  const uint32_t last = __shfl_sync(kAll, my_key, __ffs(__ballot_sync(kAll, in && ahead == p.topk_groups - 1)) - 1);
-  const uint32_t next = __shfl_sync(kAll, my_key, __ffs(__ballot_sync(kAll, in && ahead == p.topk_groups)) - 1);
-  near = !(value_of(last) - value_of(next) > tau);
   return __ballot_sync(kAll, in && ahead < p.topk_groups);
 }
 
-// One token's experts, lane j the j-th.  near: f32 could not decide.
-template <int NI, bool SIGMOID>
-__device__ __forceinline__ int32_t choose(const RouteParams& p, const float (&l)[NI], float largest, bool& near) {
+template <typename T, bool SIGMOID>
+__device__ int32_t choose_exact(const RouteParams& p, const T* row, float largest);
+
+// One token's experts, lane j the j-th.
+template <typename T, int NI, bool SIGMOID>
+__device__ __forceinline__ int32_t choose(const RouteParams& p, const T* row, const float (&l)[NI], float largest) {
   const int lane = threadIdx.x % 32, e0 = lane * NI;
   const bool grouped = p.topk_groups < p.groups;
-  near = false;
   uint32_t key[NI];
   float tau = 0.f;
   if (p.bias || grouped) {
@@ -292,8 +358,7 @@ __device__ __forceinline__ int32_t choose(const RouteParams& p, const float (&l)
     // decision, and twice as many where a group's value adds two.
     tau = 0x1p-23f * ((SIGMOID ? 16.f : 48.f + NI) * top + 2.f * __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(widest))));
     if (grouped) {
-      const uint32_t open = open_groups(p, key, 2.f * tau, near);
-      if (near) return 0;
+      const uint32_t open = open_groups<T, NI, SIGMOID>(p, row, key, 2.f * tau, largest);
       if (!p.bias) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) key[i] = e0 + i < p.experts ? key_of(l[i]) : 0u;
@@ -314,51 +379,37 @@ __device__ __forceinline__ int32_t choose(const RouteParams& p, const float (&l)
 #pragma unroll
     for (int i = 0; i < NI; ++i) key[i] = e0 + i < p.experts ? key_of(l[i]) : 0u;
   }
-  const Picked got = pick(key, p.topk, p.bias != nullptr);
-  if (p.bias) {
-    const uint32_t behind = __shfl_down_sync(kAll, got.key, 1);
-    const bool end = lane == p.topk - 1;
-    const float v = value_of(got.key), next = value_of(end ? got.next : behind);
-    // nothing lies behind the last one, or both are masked: by their ids, whatever their errors
-    const bool sure = (end && got.next == 0) || (v == -INFINITY && next == -INFINITY);
-    near = __any_sync(kAll, lane < p.topk && !sure && !(v - next > tau));
+  const Picked got = pick(key, p.topk, p.bias != nullptr, tau);
+  if (!got.near) return got.id;
+  if (got.count > 32) return choose_exact<T, SIGMOID>(p, row, largest);
+  // in order of their values in f64, an expert a lane
+  const double sum = exact_sum<T, SIGMOID>(p, row, largest);
+  const uint64_t mine = lane < got.count ? key_of(exact_value<T, SIGMOID>(p, row, got.id, largest, sum)) : 0ull;
+  int place = 0;
+#pragma unroll 1
+  for (int j = 0; j < got.count; ++j) {
+    const uint64_t other = __shfl_sync(kAll, mine, j);
+    const int32_t id = __shfl_sync(kAll, got.id, j);
+    place += other > mine || (other == mine && id < got.id);
   }
-  return got.id;
+  int32_t id = 0;
+#pragma unroll 1
+  for (int j = 0; j < got.count; ++j) {
+    const int at = __shfl_sync(kAll, place, j);
+    const int32_t e = __shfl_sync(kAll, got.id, j);
+    if (at == lane) id = e;
+  }
+  return id;
 }
 
-// The same choice with everything in f64.  Rolled loops over local memory and one exponential: tokens come here one by
-// one, and what they wait for is mostly the code.
+// The whole choice in f64, in rolled loops over local memory.
 template <typename T, bool SIGMOID>
-__device__ __noinline__ int32_t choose_exact(const RouteParams& p, int64_t t, float largest) {
+__device__ __noinline__ int32_t choose_exact(const RouteParams& p, const T* row, float largest) {
   const int lane = threadIdx.x % 32, held = (p.experts + 31) / 32, e0 = lane * held, per = p.experts / p.groups;
-  const T* row = static_cast<const T*>(p.logits) + t * p.ld;
   uint64_t key[kMaxExperts / 32];
-  double sum = 0.0;
+  const double sum = exact_sum<T, SIGMOID>(p, row, largest);
 #pragma unroll 1
-  for (int i = 0; i < held; ++i) {
-    const float l = e0 + i < p.experts ? widen(row[e0 + i]) : -INFINITY;
-    double s = 0.0;
-    if (l != -INFINITY) {
-      const double d = l, e = exp(SIGMOID ? (d < 0 ? d : -d) : d - static_cast<double>(largest));
-      s = SIGMOID ? (d < 0 ? e : 1.0) / (1.0 + e) : e;
-    }
-    sum += s;
-    key[i] = static_cast<uint64_t>(__double_as_longlong(s));
-  }
-  if constexpr (SIGMOID) sum = 1.0;
-  else sum = warp_sum(sum);
-#pragma unroll 1
-  for (int i = 0; i < held; ++i) {
-    const int e = e0 + i;
-    if (e >= p.experts) {
-      key[i] = 0;
-      continue;
-    }
-    double c = __longlong_as_double(static_cast<long long>(key[i]));
-    if (!SIGMOID && sum != 0.0) c /= sum;
-    if (p.bias) c = widen(row[e]) == -INFINITY ? -INFINITY : c + static_cast<double>(p.bias[e]);
-    key[i] = key_of(c);
-  }
+  for (int i = 0; i < held; ++i) key[i] = e0 + i < p.experts ? key_of(exact_value<T, SIGMOID>(p, row, e0 + i, largest, sum)) : 0ull;
   if (p.topk_groups < p.groups) {
     uint64_t mine = 0;
 #pragma unroll 1
@@ -387,12 +438,8 @@ __device__ __noinline__ int32_t choose_exact(const RouteParams& p, int64_t t, fl
     }
     const uint32_t open = __ballot_sync(kAll, lane < p.groups && ahead < p.topk_groups);
 #pragma unroll 1
-    for (int i = 0; i < held; ++i) {
-      const int e = e0 + i;
-      if (e >= p.experts) continue;
-      if (!p.bias) key[i] = key_of(static_cast<double>(widen(row[e])));
-      if (!(open >> (e / per) & 1)) key[i] = 0;
-    }
+    for (int i = 0; i < held; ++i)
+      if (e0 + i < p.experts && !(open >> (e0 + i) / per & 1)) key[i] = 0;
   }
   int32_t id = 0;
 #pragma unroll 1
@@ -434,13 +481,12 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
   pdl_wait();
   if (t >= p.tokens) return;
   float l[NI];
-  load_row(p, static_cast<const T*>(p.logits) + t * p.ld, -INFINITY, l);
+  const T* row = static_cast<const T*>(p.logits) + t * p.ld;
+  load_row(p, row, -INFINITY, l);
   const float largest = SIGMOID ? 0.f : largest_of(l);
-  bool near;
-  int32_t id = choose<NI, SIGMOID>(p, l, largest, near);
-  if (near) id = choose_exact<T, SIGMOID>(p, t, largest);
+  const int32_t id = choose<T, NI, SIGMOID>(p, row, l, largest);
   const bool used = lane < p.topk;
-  const float mine = used ? widen(static_cast<const T*>(p.logits)[t * p.ld + id]) : -INFINITY;
+  const float mine = used ? widen(row[id]) : -INFINITY;
   float w;
   if (p.renorm) {
     w = share_of<SIGMOID>(mine, largest, used);
