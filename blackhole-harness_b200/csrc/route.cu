@@ -12,6 +12,7 @@
 // are nearer than their errors' bound (a token in a thousand), the values in question alone are computed again in f64, an
 // expert a lane: a warp that took its whole row through f64 would keep the kernel waiting (8192 tokens: 28 us of which 15
 // were such rows').  Only where more than 32 experts are that near does the whole row go through choose_exact.
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <type_traits>
@@ -26,6 +27,7 @@ constexpr int kRouteThreads = 256;
 constexpr int kMaxTopk = 32;       // a lane a weight
 constexpr int kMaxGroups = 32;     // a lane a group
 constexpr int kMaxExperts = 2048;  // 64 a lane
+constexpr size_t kRowsBytes = 40960;   // of keys, a block
 constexpr unsigned kAll = 0xffffffffu;
 
 int arg_error(const char* fmt, ...) {
@@ -90,6 +92,10 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 __device__ __forceinline__ double value_of(uint64_t k) {
   return k <= 1 ? __longlong_as_double(0x7ff8000000000000ll)
                 : __longlong_as_double(static_cast<long long>(k ^ (k >> 63 ? 1ull << 63 : ~0ull)));
+}
+__device__ __forceinline__ uint32_t plain_key(float v) {   // of what is no NaN
+  const uint32_t b = __float_as_uint(v + 0.f);
+  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
 }
 constexpr uint32_t kMasked = 0x007fffffu;   // the key of -inf; NaN lies below
 __device__ __forceinline__ uint64_t warp_max_key(uint64_t k) {
@@ -199,17 +205,22 @@ __device__ __noinline__ double exact_value(const RouteParams& p, const T* row, i
   return l == -INFINITY ? -INFINITY : s + static_cast<double>(p.bias[e]);
 }
 
-// The k largest of a warp's keys in order, equal ones by lane and place, and as many behind them as lie no more than tau
-// apart from one to the next.  Keys that are chosen become 0.
+// What a selection finds.
 struct Picked {
-  int32_t id, count;   // lane j: the j-th expert; how many there are
-  uint32_t key;
-  bool near;           // two of them, or the last and what follows, lie no more than tau apart
+  int32_t id, count;   // lane j: the j-th expert; how many there are, 33 where they are too many for a warp
+  bool near;           // two of the k first, or the last of them and what follows, lie no more than tau apart
 };
+__device__ __forceinline__ bool close_by(uint32_t above, uint32_t below, float tau) {
+  // masked ones (-inf, NaN) are told apart by their ids, whatever their errors
+  return below > kMasked && !(value_of(above) - value_of(below) > tau);
+}
+
+// The k largest of a warp's keys in order, equal ones by lane and place, one after the other; with `compare` as many
+// behind them as lie no more than tau apart from one to the next.
 template <int NI>
-__device__ __forceinline__ Picked pick(uint32_t (&key)[NI], int k, bool compare, float tau) {
+__device__ __noinline__ Picked pick_each(uint32_t (&key)[NI], int k, bool compare, float tau) {
   const int lane = threadIdx.x % 32;
-  Picked got{0, k, 0, false};
+  Picked got{0, k, false};
   uint32_t before = 0;
   for (int j = 0;; ++j) {
     if (j >= k && !compare) break;
@@ -218,8 +229,7 @@ __device__ __forceinline__ Picked pick(uint32_t (&key)[NI], int k, bool compare,
     for (int i = 1; i < NI; ++i) best = max(best, key[i]);
     const uint32_t top = __reduce_max_sync(kAll, best);
     if (compare) {
-      // masked ones (-inf, and NaN) are told apart by their ids, whatever their errors
-      const bool close = j > 0 && top > kMasked && !(value_of(before) - value_of(top) > tau);
+      const bool close = j > 0 && close_by(before, top, tau);
       got.near |= close;
       if (j >= k && (!close || j == 32)) {
         got.count = close ? 33 : j;
@@ -236,11 +246,76 @@ __device__ __forceinline__ Picked pick(uint32_t (&key)[NI], int k, bool compare,
       for (int i = 0; i < NI; ++i) key[i] = i == at ? 0u : key[i];
     }
     const int id = __shfl_sync(kAll, lane * NI + at, owner);
-    if (lane == j) {
-      got.id = id;
-      got.key = top;
+    if (lane == j) got.id = id;
+  }
+  return got;
+}
+
+// The same at a third of the instructions: the k-th largest of the lanes' largest keys bounds the k-th largest key from
+// below, and few more than k keys reach it (or come within tau of it).  Those go through shared memory to a lane each, in
+// the order of their ids, and are ranked by counting.  Where more than 32 do, or keys are equal too often, one by one.
+struct Found {
+  uint32_t key[32];
+  int32_t id[32];
+};
+template <int NI>
+__device__ __forceinline__ Picked pick(uint32_t (&key)[NI], int k, bool compare, float tau, Found& found) {
+  const int lane = threadIdx.x % 32;
+  uint32_t best = key[0];
+#pragma unroll
+  for (int i = 1; i < NI; ++i) best = max(best, key[i]);
+  uint32_t bound = 0;
+  for (int j = 0; j < k; ++j) {   // lanes of the same largest key leave together: the bound only falls
+    bound = __reduce_max_sync(kAll, best);
+    if (best == bound) best = 0;
+  }
+  if (compare && bound > kMasked) bound = key_of(value_of(bound) - tau);
+  bound = max(bound, 1u);
+  int mine = 0;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) mine += key[i] >= bound;
+  int upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(kAll, upto, o);
+    if (lane >= o) upto += v;
+  }
+  const int count = __shfl_sync(kAll, upto, 31);
+  if (count > 32) {
+    uint32_t copy[NI];   // what is handed on lives in memory: not the keys themselves
+#pragma unroll
+    for (int i = 0; i < NI; ++i) copy[i] = key[i];
+    return pick_each(copy, k, compare, tau);
+  }
+  int at = upto - mine;
+  if (mine) {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      if (key[i] >= bound) {
+        found.key[at] = key[i];
+        found.id[at++] = lane * NI + i;
+      }
     }
   }
+  __syncwarp();
+  const uint32_t my_key = lane < count ? found.key[lane] : 0u;
+  const int32_t my_id = lane < count ? found.id[lane] : 0;
+  int place = 0;
+#pragma unroll 4
+  for (int j = 0; j < count; ++j) {
+    const uint32_t other = __shfl_sync(kAll, my_key, j);
+    place += other > my_key || (other == my_key && j < lane);
+  }
+  __syncwarp();
+  if (lane < count) {
+    found.key[place] = my_key;
+    found.id[place] = my_id;
+  }
+  __syncwarp();
+  Picked got{0, count, false};
+  if (lane < count) got.id = found.id[lane];
+  if (compare) got.near = __any_sync(kAll, lane < k && lane + 1 < count && close_by(found.key[lane], found.key[lane + 1], tau));
+  __syncwarp();   // the next row of this warp's may come
   return got;
 }
 
@@ -250,39 +325,36 @@ __device__ __forceinline__ void add_top(uint32_t key, uint32_t& first, uint32_t&
   second = max(second, less);
 }
 
-// The open groups as a bit each, from the values s + b (as keys); tau: what two groups' values may be off by together.
+// The open groups as a bit each, from the values s + b (as keys); tau: what two groups' values may be off by together;
+// keys: room for a row.
 template <typename T, int NI, bool SIGMOID>
-__device__ __forceinline__ uint32_t open_groups(const RouteParams& p, const T* row, const uint32_t (&key)[NI], float tau, float largest) {
+__device__ __forceinline__ uint32_t open_groups(const RouteParams& p, const T* row, const uint32_t (&key)[NI], float tau, float largest,
+                                                uint32_t* keys) {
   const int lane = threadIdx.x % 32, per = p.experts / p.groups;
   const bool two = p.group_top > 1 && per > 1, in = lane < p.groups;
-  float mine = 0.f;
-  if (p.group_lanes) {   // a group is so many whole lanes, a power of two
-    uint32_t first = 0, second = 0;
+  // a lane's part of a group, or a lane's groups: lanes [g lanes, (g + 1) lanes) hold group g's two largest
+  int lanes = p.group_lanes;
+  uint32_t first = 0, second = 0;
+  if (lanes) {   // a group is so many whole lanes, a power of two
 #pragma unroll
     for (int i = 0; i < NI; ++i) add_top(key[i], first, second);
-    for (int o = 1; o < p.group_lanes; o <<= 1) {
-      const uint32_t f = __shfl_xor_sync(kAll, first, o), g = __shfl_xor_sync(kAll, second, o);
-      add_top(f, first, second);
-      second = max(second, g);
-    }
-    const float v = two ? value_of(first) + value_of(second) : value_of(first);
-    mine = __shfl_sync(kAll, v, lane * p.group_lanes);
-  } else {
-    const int e0 = lane * NI;
-    for (int g = 0; g < p.groups; ++g) {
-      uint32_t first = 0, second = 0;   // of this lane's experts in the group
+  } else {       // by way of shared memory
+    lanes = 32 >> (32 - __clz(p.groups - 1));
 #pragma unroll
-      for (int i = 0; i < NI; ++i)
-        add_top(e0 + i >= g * per && e0 + i < (g + 1) * per ? key[i] : 0u, first, second);
-      const uint32_t top = __reduce_max_sync(kAll, first);
-      float v = value_of(top);
-      if (two) {
-        const int owner = __ffs(__ballot_sync(kAll, first == top)) - 1;
-        v += value_of(__reduce_max_sync(kAll, lane == owner ? second : first));
-      }
-      if (lane == g) mine = v;
-    }
+    for (int i = 0; i < NI; ++i)
+      if (lane * NI + i < p.experts) keys[lane * NI + i] = key[i];
+    __syncwarp();
+    const int g = lane / lanes;
+    if (g < p.groups)
+      for (int i = lane % lanes; i < per; i += lanes) add_top(keys[g * per + i], first, second);
+    __syncwarp();
   }
+  for (int o = 1; o < lanes; o <<= 1) {
+    const uint32_t f = __shfl_xor_sync(kAll, first, o), g = __shfl_xor_sync(kAll, second, o);
+    add_top(f, first, second);
+    second = max(second, g);
+  }
+  const float mine = __shfl_sync(kAll, two ? value_of(first) + value_of(second) : value_of(first), lane * lanes);
   auto rank = [&](auto k) {
     int ahead = 0;
 #pragma unroll 4
@@ -331,34 +403,53 @@ __device__ int32_t choose_exact(const RouteParams& p, const T* row, float larges
 
 // One token's experts, lane j the j-th.
 template <typename T, int NI, bool SIGMOID>
-__device__ __forceinline__ int32_t choose(const RouteParams& p, const T* row, const float (&l)[NI], float largest) {
+__device__ __forceinline__ int32_t choose(const RouteParams& p, const T* row, const float (&l)[NI], float largest, Found& found,
+                                          uint32_t* keys) {
   const int lane = threadIdx.x % 32, e0 = lane * NI;
   const bool grouped = p.topk_groups < p.groups;
   uint32_t key[NI];
   float tau = 0.f;
   if (p.bias || grouped) {
-    float c[NI], widest = 0.f;
+    float c[NI];
     const float top = scores_of<NI, SIGMOID>(l, largest, c);
     if (p.bias) {
       float b[NI];
       load_row(p, p.bias, 0.f, b);
 #pragma unroll
-      for (int i = 0; i < NI; ++i) c[i] = l[i] == -INFINITY ? -INFINITY : c[i] + b[i];
+      for (int i = 0; i < NI; ++i) c[i] += b[i];
     }
+    // all logits and values finite, as a rule: then a key is their bits turned to their order
+    uint32_t most = 0;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      key[i] = e0 + i < p.experts ? key_of(c[i]) : 0u;
-      const float size = fabsf(c[i]);
-      widest = fmaxf(widest, size < INFINITY ? size : 0.f);
+    for (int i = 0; i < NI; ++i) most = max(most, max(__float_as_uint(c[i]) & 0x7fffffffu, __float_as_uint(l[i]) & 0x7fffffffu));
+    float widest;
+    if (__reduce_max_sync(kAll, p.experts == 32 * NI ? most : 0xffffffffu) < 0x7f800000u) {
+      uint32_t wide = 0;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        wide = max(wide, __float_as_uint(c[i]) & 0x7fffffffu);
+        key[i] = plain_key(c[i]);
+      }
+      widest = __uint_as_float(__reduce_max_sync(kAll, wide));
+    } else {
+      widest = 0.f;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        if (p.bias && l[i] == -INFINITY) c[i] = -INFINITY;
+        key[i] = e0 + i < p.experts ? key_of(c[i]) : 0u;
+        const float size = fabsf(c[i]);
+        widest = fmaxf(widest, size < INFINITY ? size : 0.f);
+      }
+      widest = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(widest)));
     }
     // Errors of the values, in units of 2^-24: a sigmoid 16 of 1 (of s (1 - s) times the exponential's 4 and its
     // argument's |l|, of s the sum's 1 and the reciprocal's 4); a softmax score, of the largest one, 48 (the exponential's
     // 4, its argument's two roundings, which count as much as |x| e^x, the reciprocal's 4, the product) and one for each
     // addition of a lane's sum and five of the warp's; the addition of the bias 1.  Two of each stand on the sides of a
     // decision, and twice as many where a group's value adds two.
-    tau = 0x1p-23f * ((SIGMOID ? 16.f : 48.f + NI) * top + 2.f * __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(widest))));
+    tau = 0x1p-23f * ((SIGMOID ? 16.f : 48.f + NI) * top + 2.f * widest);
     if (grouped) {
-      const uint32_t open = open_groups<T, NI, SIGMOID>(p, row, key, 2.f * tau, largest);
+      const uint32_t open = open_groups<T, NI, SIGMOID>(p, row, key, 2.f * tau, largest, keys);
       if (!p.bias) {
 #pragma unroll
         for (int i = 0; i < NI; ++i) key[i] = e0 + i < p.experts ? key_of(l[i]) : 0u;
@@ -379,7 +470,7 @@ __device__ __forceinline__ int32_t choose(const RouteParams& p, const T* row, co
 #pragma unroll
     for (int i = 0; i < NI; ++i) key[i] = e0 + i < p.experts ? key_of(l[i]) : 0u;
   }
-  const Picked got = pick(key, p.topk, p.bias != nullptr, tau);
+  const Picked got = pick(key, p.topk, p.bias != nullptr, tau, found);
   if (!got.near) return got.id;
   if (got.count > 32) return choose_exact<T, SIGMOID>(p, row, largest);
   // in order of their values in f64, an expert a lane
@@ -476,6 +567,8 @@ __device__ __forceinline__ float share_of(float l, float largest, bool used) {
 
 template <typename T, int NI, bool SIGMOID>
 __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams p) {
+  __shared__ Found found[kRouteThreads / 32];
+  extern __shared__ __align__(16) uint8_t keys[];
   const int lane = threadIdx.x % 32;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
   pdl_wait();
@@ -484,7 +577,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
   const T* row = static_cast<const T*>(p.logits) + t * p.ld;
   load_row(p, row, -INFINITY, l);
   const float largest = SIGMOID ? 0.f : largest_of(l);
-  const int32_t id = choose<T, NI, SIGMOID>(p, row, l, largest);
+  const int32_t id = choose<T, NI, SIGMOID>(p, row, l, largest, found[threadIdx.x / 32],
+                                            reinterpret_cast<uint32_t*>(keys) + threadIdx.x / 32 * p.experts);
   const bool used = lane < p.topk;
   const float mine = used ? widen(row[id]) : -INFINITY;
   float w;
@@ -589,12 +683,15 @@ cudaError_t launch_one(RouteParams p, bool backward, cudaStream_t st) {
   p.group_lanes = per % NI == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
   p.vec = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld * sizeof(T) % 16 == 0 && p.experts * sizeof(T) % 16 == 0 &&
           reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && (!p.bias || p.experts % 4 == 0);
-  // a token a warp: blocks of one warp until every SM has some
-  const int warps = p.tokens <= 148 * 8 ? 1 : kRouteThreads / 32;
+  // a token a warp: blocks of one warp until every SM has some, and no more than their rows of keys leave room for
+  const size_t row = !backward && p.topk_groups < p.groups && !p.group_lanes ? sizeof(uint32_t) * p.experts : 0;
+  int warps = p.tokens <= 148 * 8 ? 1 : kRouteThreads / 32;
+  if (row) warps = std::min(warps, static_cast<int>(kRowsBytes / row));
   const int64_t blocks = (p.tokens + warps - 1) / warps;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
   cfg.blockDim = dim3(warps * 32);
+  cfg.dynamicSmemBytes = row * warps;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
