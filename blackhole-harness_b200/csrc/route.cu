@@ -181,7 +181,7 @@ __device__ __forceinline__ float scores_of(const float (&l)[NI], float largest, 
 
 // What is left of a row's softmax in f64: 1 for a sigmoid, the sum of e^(l - largest) otherwise.
 template <typename T, bool SIGMOID>
-__device__ __noinline__ double exact_sum(const RouteParams& p, const T* row, float largest) {
+__device__ double exact_sum(const RouteParams& p, const T* row, float largest) {
   if constexpr (SIGMOID) return 1.0;
   double part = 0.0;
 #pragma unroll 1
@@ -193,7 +193,7 @@ __device__ __noinline__ double exact_sum(const RouteParams& p, const T* row, flo
 }
 // s + b of one expert in f64.
 template <typename T, bool SIGMOID>
-__device__ __noinline__ double exact_value(const RouteParams& p, const T* row, int e, float largest, double sum) {
+__device__ double exact_value(const RouteParams& p, const T* row, int e, float largest, double sum) {
   const float l = widen(row[e]);
   const double d = l;
   double s = 0.0;
@@ -203,6 +203,12 @@ __device__ __noinline__ double exact_value(const RouteParams& p, const T* row, i
   }
   if (!p.bias) return s;
   return l == -INFINITY ? -INFINITY : s + static_cast<double>(p.bias[e]);
+}
+
+__device__ __forceinline__ void add_top(uint32_t key, uint32_t& first, uint32_t& second) {
+  const uint32_t less = min(first, key);
+  first = max(first, key);
+  second = max(second, less);
 }
 
 // What a selection finds.
@@ -218,7 +224,7 @@ __device__ __forceinline__ bool close_by(uint32_t above, uint32_t below, float t
 // The k largest of a warp's keys in order, equal ones by lane and place, one after the other; with `compare` as many
 // behind them as lie no more than tau apart from one to the next.
 template <int NI>
-__device__ __noinline__ Picked pick_each(uint32_t (&key)[NI], int k, bool compare, float tau) {
+__device__ Picked pick_each(uint32_t (&key)[NI], int k, bool compare, float tau) {
   const int lane = threadIdx.x % 32;
   Picked got{0, k, false};
   uint32_t before = 0;
@@ -261,13 +267,21 @@ struct Found {
 template <int NI>
 __device__ __forceinline__ Picked pick(uint32_t (&key)[NI], int k, bool compare, float tau, Found& found) {
   const int lane = threadIdx.x % 32;
-  uint32_t best = key[0];
+  uint32_t best = key[0], second = 0;
+  if (k <= 8) {
 #pragma unroll
-  for (int i = 1; i < NI; ++i) best = max(best, key[i]);
+    for (int i = 1; i < NI; ++i) best = max(best, key[i]);
+  } else {   // more than the lanes of an open group or two may hold: two of each
+#pragma unroll
+    for (int i = 1; i < NI; ++i) add_top(key[i], best, second);
+  }
   uint32_t bound = 0;
   for (int j = 0; j < k; ++j) {   // lanes of the same largest key leave together: the bound only falls
     bound = __reduce_max_sync(kAll, best);
-    if (best == bound) best = 0;
+    if (best == bound) {
+      best = second;
+      second = 0;
+    }
   }
   if (compare && bound > kMasked) bound = key_of(value_of(bound) - tau);
   bound = max(bound, 1u);
@@ -319,11 +333,10 @@ __device__ __forceinline__ Picked pick(uint32_t (&key)[NI], int k, bool compare,
   return got;
 }
 
-__device__ __forceinline__ void add_top(uint32_t key, uint32_t& first, uint32_t& second) {
-  const uint32_t less = min(first, key);
-  first = max(first, key);
-  second = max(second, less);
-}
+
+// Where an expert's key stands in shared memory: a lane's even number of them one place on, in other banks.
+template <int NI>
+__device__ __forceinline__ int place_of(int e) { return NI % 2 ? e : e + e / NI; }
 
 // The open groups as a bit each, from the values s + b (as keys); tau: what two groups' values may be off by together;
 // keys: room for a row.
@@ -342,11 +355,11 @@ __device__ __forceinline__ uint32_t open_groups(const RouteParams& p, const T* r
     lanes = 32 >> (32 - __clz(p.groups - 1));
 #pragma unroll
     for (int i = 0; i < NI; ++i)
-      if (lane * NI + i < p.experts) keys[lane * NI + i] = key[i];
+      if (lane * NI + i < p.experts) keys[place_of<NI>(lane * NI + i)] = key[i];
     __syncwarp();
     const int g = lane / lanes;
     if (g < p.groups)
-      for (int i = lane % lanes; i < per; i += lanes) add_top(keys[g * per + i], first, second);
+      for (int i = lane % lanes; i < per; i += lanes) add_top(keys[place_of<NI>(g * per + i)], first, second);
     __syncwarp();
   }
   for (int o = 1; o < lanes; o <<= 1) {
@@ -419,18 +432,18 @@ __device__ __forceinline__ int32_t choose(const RouteParams& p, const T* row, co
       for (int i = 0; i < NI; ++i) c[i] += b[i];
     }
     // all logits and values finite, as a rule: then a key is their bits turned to their order
-    uint32_t most = 0;
+    const bool full = p.experts == 32 * NI;
+    uint32_t most = 0, wide = 0;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) most = max(most, max(__float_as_uint(c[i]) & 0x7fffffffu, __float_as_uint(l[i]) & 0x7fffffffu));
-    float widest;
-    if (__reduce_max_sync(kAll, p.experts == 32 * NI ? most : 0xffffffffu) < 0x7f800000u) {
-      uint32_t wide = 0;
+    for (int i = 0; i < NI; ++i) {
+      wide = max(wide, __float_as_uint(c[i]) & 0x7fffffffu);
+      most = max(most, full || e0 + i < p.experts ? __float_as_uint(l[i]) & 0x7fffffffu : 0u);
+    }
+    wide = __reduce_max_sync(kAll, wide);
+    float widest = __uint_as_float(wide);
+    if (max(wide, __reduce_max_sync(kAll, most)) < 0x7f800000u) {
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        wide = max(wide, __float_as_uint(c[i]) & 0x7fffffffu);
-        key[i] = plain_key(c[i]);
-      }
-      widest = __uint_as_float(__reduce_max_sync(kAll, wide));
+      for (int i = 0; i < NI; ++i) key[i] = full || e0 + i < p.experts ? plain_key(c[i]) : 0u;
     } else {
       widest = 0.f;
 #pragma unroll
@@ -495,7 +508,7 @@ __device__ __forceinline__ int32_t choose(const RouteParams& p, const T* row, co
 
 // The whole choice in f64, in rolled loops over local memory.
 template <typename T, bool SIGMOID>
-__device__ __noinline__ int32_t choose_exact(const RouteParams& p, const T* row, float largest) {
+__device__ int32_t choose_exact(const RouteParams& p, const T* row, float largest) {
   const int lane = threadIdx.x % 32, held = (p.experts + 31) / 32, e0 = lane * held, per = p.experts / p.groups;
   uint64_t key[kMaxExperts / 32];
   const double sum = exact_sum<T, SIGMOID>(p, row, largest);
@@ -578,7 +591,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
   load_row(p, row, -INFINITY, l);
   const float largest = SIGMOID ? 0.f : largest_of(l);
   const int32_t id = choose<T, NI, SIGMOID>(p, row, l, largest, found[threadIdx.x / 32],
-                                            reinterpret_cast<uint32_t*>(keys) + threadIdx.x / 32 * p.experts);
+                                            reinterpret_cast<uint32_t*>(keys) + threadIdx.x / 32 * (p.experts + 32));
   const bool used = lane < p.topk;
   const float mine = used ? widen(row[id]) : -INFINITY;
   float w;
@@ -684,7 +697,7 @@ cudaError_t launch_one(RouteParams p, bool backward, cudaStream_t st) {
   p.vec = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld * sizeof(T) % 16 == 0 && p.experts * sizeof(T) % 16 == 0 &&
           reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && (!p.bias || p.experts % 4 == 0);
   // a token a warp: blocks of one warp until every SM has some, and no more than their rows of keys leave room for
-  const size_t row = !backward && p.topk_groups < p.groups && !p.group_lanes ? sizeof(uint32_t) * p.experts : 0;
+  const size_t row = !backward && p.topk_groups < p.groups && !p.group_lanes ? sizeof(uint32_t) * (p.experts + 32) : 0;
   int warps = p.tokens <= 148 * 8 ? 1 : kRouteThreads / 32;
   if (row) warps = std::min(warps, static_cast<int>(kRowsBytes / row));
   const int64_t blocks = (p.tokens + warps - 1) / warps;
