@@ -362,7 +362,8 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 //
 // 12 warps a CTA: 0 loads, 1 issues the products (the leader's), 2 and 3 zero tails
 // (weight gradient, the leader's), 4..11 write results.  Each walks the groups' offsets by
-// itself, so that no size is known on the host.
+// itself, so that no size is known on the host.  8-bit products run half as long as 16-bit ones and are not to wait for
+// the issue of their loads: warp 2 loads the rows, in one box a step, and warp 0 the matrix.
 //
 // Measured, bf16, 96 experts, 1536 x 2048, a call at a time and (in brackets) back to back, where the power cap
 // lowers the clock at the same number of cycles: 512 rows 91..93 us (93: HBM, 6.5 TB/s); 32768 rows 174..178 us
@@ -380,6 +381,7 @@ constexpr uint32_t kStoreBytes = 2048;                 // a writer's staging til
 constexpr uint32_t kRingBytes = 200 * 1024;            // 6 steps of A and B, 4 of A and two Bs, 5 narrow ones
 constexpr uint32_t kPairSmem = 1024 + kRingBytes + kWriters * kStoreBytes + 1024;
 constexpr int kBoxes = 4;                              // row boxes of 16, 32, 64, 128
+constexpr int kBoxes8 = 8;                             // 8-bit rows: of 16, 32, 48 .. 128
 
 // kInt8: y = x W^T of 8-bit integers with scales; kInt8Glu: SwiGLU of such products with gate and up rows; kWgradT: M
 // side k, N side n.
@@ -406,7 +408,7 @@ constexpr int span_of(int shape) {                                      // most 
 
 struct PairParams {
   CUtensorMap a;             // W (3-D: reduction or features, ..., expert); weight gradient: dy, or x in kWgradT
-  CUtensorMap b[kBoxes];     // the rows, by box height; weight gradient: [0] is the other of x and dy
+  CUtensorMap b[kBoxes8];    // the rows, by box height; weight gradient: [0] is the other of x and dy
   CUtensorMap out;           // boxes of 32 rows x 64 B; f32 of kWgradT: 16 rows x 128 B
   Groups g;
   int32_t m_len;             // M side: output features; weight gradient: n, or k in kWgradT
@@ -797,7 +799,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   volatile int* abort = &c->abort;
   if (warp == 0) {   // a barrier a lane
     if (lane < kMaxStages) {
-      mbar_init(&c->full[lane], 2);    // one arrival of each CTA
+      mbar_init(&c->full[lane], is_int8(MODE) ? 4 : 2);    // an arrival of each warp that loads, in each CTA
       mbar_init(&c->empty[lane], 1);   // the products' commit
       mbar_init(&c->tail[lane], 2);
     } else if (lane < kMaxStages + 2) {
@@ -824,8 +826,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   const int32_t first = blockIdx.x / 2, stride = gridDim.x / 2;
   Walker<MODE, SHAPE, RUNS> walk;
   Tile t;
-  if (warp == 0) {
+  if (warp == 0 || (is_int8(MODE) && warp == 2)) {
     // ---------------------------------------------------------------- loads
+    const bool loads_a = !is_int8(MODE) || warp == 0, loads_b = !is_int8(MODE) || warp == 2;
     uint32_t it = 0, st = 0, phase = 1;
     uint32_t tails = 0, tail_odd = 0;   // a bit a stage: whether it has held a tail, whether an odd number of them
     bool ok = true;
@@ -833,7 +836,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       const int32_t halves[2] = {t.columns(0) / 2, WIDE && t.parts > 1 ? t.columns(1) / 2 : 0};
       const int32_t m = t.m0 + static_cast<int32_t>(rank) * 128;
       const uint32_t bytes =
-          kOperandBytes + (MODE >= kWgrad ? kBBytes : static_cast<uint32_t>(halves[0] + halves[1]) * kStepK * 2);
+          (loads_a ? kOperandBytes : 0) +
+          (loads_b ? (MODE >= kWgrad ? kBBytes : static_cast<uint32_t>(halves[0] + halves[1]) * kStepK * 2) : 0);
       for (int32_t s = 0; s < t.steps; ++s, ++it) {
         ok = warp_wait(&c->empty[st], phase, abort, p.dev_err);
         if (!ok) break;
@@ -851,7 +855,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           for (int sub = 0; sub < kSubs; ++sub) {
             if (sub >= subs) break;
             const int32_t r = ((t.first + s) * kSubs + sub) * kStepK;   // where the block begins in the reduction
-            if constexpr (MODE == kRowsK) {
+            if (!loads_a) {
+            } else if constexpr (MODE == kRowsK) {
               pair_load_3d(a, &p.a, bar, r, m, t.e);
             } else if constexpr (MODE == kInt8) {
               pair_load_3d(a, &p.a, bar, 2 * r, m, t.e);
@@ -865,7 +870,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
               pair_load_2d(a, &p.a, bar, m, y);
               pair_load_2d(a + kChunkBytes, &p.a, bar, m + 64, y);
             }
-            if constexpr (MODE >= kWgrad) {
+            if constexpr (is_int8(MODE)) {
+              if (loads_b)
+                pair_load_2d(b, &p.b[halves[0] / 16 - 1], bar, 2 * r, static_cast<int32_t>(t.row0) + static_cast<int32_t>(rank) * halves[0]);
+            } else if constexpr (MODE >= kWgrad) {
               const int32_t y = static_cast<int32_t>(t.row0) + r, x = t.n0 + static_cast<int32_t>(rank) * halves[0];
               pair_load_2d(b, &p.b[0], bar, x, y);
               if constexpr (kBBytes > kChunkBytes) pair_load_2d(b + kChunkBytes, &p.b[0], bar, x + 64, y);
@@ -879,7 +887,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
 #pragma unroll
                 for (int i = kBoxes - 1; i >= 0; --i) {   // the rows' number in boxes of 128, 64, 32, 16
                   if (half & (16 << i)) {
-                    pair_load_2d(to, &p.b[i], bar, is_int8(MODE) ? 2 * r : r, y);
+                    pair_load_2d(to, &p.b[i], bar, r, y);
                     to += (16 << i) * kStepK * 2;
                     y += 16 << i;
                   }
@@ -1386,8 +1394,8 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
                      : make_map(&q.a, d.w, kBytes, 3, d.k, d.n, d.experts, d.ld_w, d.experts == 1 ? d.ld_w : d.stride_w, 128, 128))
     return rc;
   const int64_t half = (std::min<int64_t>(d.rows, 256) + 31) / 32 * 16;
-  for (int i = 0; i < kBoxes && 16 << i <= half; ++i)
-    if (int rc = make_map(&q.b[i], d.x, kBytes, 2, d.k, d.rows, 1, d.ld_x, 0, 128, 16u << i)) return rc;
+  for (int i = 0; i < kBoxes8 && 16 * (i + 1) <= half; ++i)
+    if (int rc = make_map(&q.b[i], d.x, kBytes, 2, d.k, d.rows, 1, d.ld_x, 0, 128, 16 * (i + 1))) return rc;
   if (d.glu) {
     q.tma_out = 1;
     if (d.rows >= 32)
