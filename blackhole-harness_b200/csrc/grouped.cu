@@ -379,7 +379,7 @@ constexpr int kWriters = 8;
 constexpr uint32_t kAccCols = 256;
 constexpr uint32_t kStoreBytes = 2048;                 // a writer's staging tile: 32 lines of 64 B
 constexpr uint32_t kRingBytes = 200 * 1024;            // 6 steps of A and B, 4 of A and two Bs, 5 narrow ones
-constexpr uint32_t kPairSmem = 1024 + kRingBytes + kWriters * kStoreBytes + 1024;
+constexpr uint32_t kPairSmem = 1024 + kRingBytes + kWriters * kStoreBytes + 9 * 1024;
 constexpr int kBoxes = 4;                              // row boxes of 16, 32, 64, 128
 constexpr int kBoxes8 = 8;                             // 8-bit rows: of 16, 32, 48 .. 128
 
@@ -535,15 +535,16 @@ struct Walker {
 };
 
 // Writes 32 x 32 pieces of an accumulator: one writer warp's M rows by 32 columns.
-template <int MODE, bool RUNS>
+template <int MODE, bool RUNS, bool TWO>
 struct Writer {
   const PairParams& p;
   uint8_t* stage;    // 32 lines of 64 B (their 16-byte pieces permuted as SWIZZLE_64B), or 16 plain ones of 128 B
   int lane;
+  uint32_t flip = 0;   // TWO: the other staging tile's distance, kStoreBytes or minus that
   int32_t e = 0, m = 0, cols = 0;   // which result (expert, run of the reduction); first M row; columns there are
   bool add = false;                 // to what is there
   int64_t n0 = 0;                   // column 0 in the output: row products: its row; weight gradient: its column
-  float w_scale = 0.f;              // 8-bit products: of this lane's matrix row
+  float w_scale = 0.f, ws[4] = {};  // 8-bit products: of this lane's matrix row, and of a fragment's four
 
   // The lane's matrix row is one of the tile's: kInt8 in order, kInt8Glu 8 of gate, the 8 of up.
   __device__ __forceinline__ void load_w_scale(int32_t expert) {
@@ -553,6 +554,8 @@ struct Writer {
       const int32_t f = m / 2 + lane / 16 * 8 + lane % 8;
       w_scale = f < p.out_len ? p.w_scale[static_cast<int64_t>(expert) * p.m_len + (lane % 16 < 8 ? 0 : p.out_len) + f] : 0.f;
     }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ws[i] = __shfl_sync(0xffffffffu, w_scale, lane / 4 + 8 * i);
   }
   // The scale of row `col + lane` of the tile, read while the accumulator is.
   __device__ __forceinline__ float load_x_scale(int32_t col) const {
@@ -562,10 +565,8 @@ struct Writer {
   // int32 sums as scaled f32 values, in place.  Fragments: register 16 h + 4 i + 2 b + c is matrix row 16 h + 8 b + g
   // and tile row 8 i + 2 q + c.
   __device__ __forceinline__ void scale_fragments(uint32_t (&r)[32], float x) const {
-    const int g = lane / 4, q = lane % 4;
-    float ws[4], xs[8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) ws[i] = __shfl_sync(0xffffffffu, w_scale, g + 8 * i);
+    const int q = lane % 4;
+    float xs[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) xs[i] = __shfl_sync(0xffffffffu, x, i / 2 * 8 + 2 * q + i % 2);
 #pragma unroll
@@ -584,10 +585,19 @@ struct Writer {
     if (add) atomicAdd(dst, v);
     else *dst = v;
   }
-  // The staging tile is free once the store before has read it.
+  // The staging tile is free once the store before has read it, or of two the one before that.
   __device__ __forceinline__ void stage_free() const {
-    if (elect_one()) bulk_wait_read();
+    if (elect_one()) {
+      if constexpr (TWO) bulk_wait_read_but_one();
+      else bulk_wait_read();
+    }
     __syncwarp();
+  }
+  __device__ __forceinline__ void stage_used() {   // by a store
+    if constexpr (TWO) {
+      stage += static_cast<int32_t>(flip);
+      flip = -flip;
+    }
   }
   __device__ __forceinline__ bool f32() const { return RUNS || p.f32; }
   // Row products that leave by TMA take fragments, everything else a row of 32 columns a lane.
@@ -632,6 +642,7 @@ struct Writer {
         else tma_store_2d(&p.out, stage, m, static_cast<int32_t>(n0) + col);
         bulk_commit();
       }
+      stage_used();
     } else {   // the group's last rows: the next ones are another group's
       __syncwarp();
       uint16_t* dst = static_cast<uint16_t*>(p.dst) + (n0 + col) * p.ld + m;
@@ -657,7 +668,7 @@ struct Writer {
     for (int j = 0; j < 16; ++j) {   // j = 8 h + 2 i + c
       const int h = j / 8, line = j % 8 / 2 * 8 + 2 * q + j % 2, at = 16 * h + j % 8 / 2 * 4 + j % 2;
       const float gate = __uint_as_float(r[at]), up = __uint_as_float(r[at + 2]);
-      const float act = gate / (1.f + __expf(-gate)) * up;
+      const float act = __fdividef(gate, 1.f + __expf(-gate)) * up;   // 0 where the denominator passes 2^126
       const int feature = 8 * h + g;
       *reinterpret_cast<float*>(stage + line * 64 + ((feature / 4 ^ (line >> 1 & 3)) << 4) + feature % 4 * 4) = act;
     }
@@ -668,6 +679,7 @@ struct Writer {
         tma_store_2d(&p.out, stage, f, static_cast<int32_t>(n0) + col);
         bulk_commit();
       }
+      stage_used();
     } else {   // the group's last rows: the next ones are another group's
       __syncwarp();
       float* dst = static_cast<float*>(p.dst) + (n0 + col) * p.ld + f;
@@ -791,8 +803,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   extern __shared__ uint8_t raw[];
   uint8_t* base = raw + (1024 - smem_u32(raw) % 1024) % 1024;
   uint8_t* ring = base;
-  uint8_t* staging = ring + kRingBytes;
-  PairCtrl* c = reinterpret_cast<PairCtrl*>(staging + kWriters * kStoreBytes);
+  // a second staging tile a writer where the ring leaves room: 8-bit tiles come twice as often
+  constexpr bool kTwoStages = is_int8(MODE) && SHAPE != kNarrow;
+  constexpr uint32_t kRing = kTwoStages ? kStages * kStageBytes : kRingBytes;
+  static_assert(1024 + kRing + kWriters * kStoreBytes * (kTwoStages ? 2 : 1) + sizeof(PairCtrl) <= kPairSmem);
+  uint8_t* staging = ring + kRing;
+  PairCtrl* c = reinterpret_cast<PairCtrl*>(staging + kWriters * kStoreBytes * (kTwoStages ? 2 : 1));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
@@ -1004,7 +1020,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   } else if (warp >= 4) {
     // -------------------------------------------------------------- results
     const int quad = warp % 4, part = (warp - 4) / 4;   // 32 of the CTA's M rows, every other 32 columns
-    Writer<MODE, RUNS> out{p, staging + (warp - 4) * kStoreBytes, lane};
+    Writer<MODE, RUNS, kTwoStages> out{p, staging + (warp - 4) * kStoreBytes * (kTwoStages ? 2 : 1), lane};
+    out.flip = kStoreBytes;
     uint32_t n = 0;
     bool ok = true;
     for (int32_t tile = first; ok && walk.next(p, tile, stride, t);) {
