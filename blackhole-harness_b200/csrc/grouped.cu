@@ -415,7 +415,8 @@ struct PairParams {
   int32_t n_len;             // weight gradient: k, or n in kWgradT
   int32_t red;               // row products: reduction length (8-bit: in pairs)
   int32_t out_len;           // row products: columns of the result
-  const float* x_scale;      // 8-bit products: [rows]
+  int32_t stream;            // 8-bit products: the matrices pass through L2 without staying
+  const float* x_scale;      // [rows]
   const float* w_scale;      // [experts, matrix rows]
   int32_t m_tiles, n_tiles, tile_n;   // n_tiles, tile_n: weight gradient
   int32_t splits;            // runs that the reduction of a tile is cut into, over several pairs
@@ -546,16 +547,24 @@ struct Writer {
   int64_t n0 = 0;                   // column 0 in the output: row products: its row; weight gradient: its column
   float w_scale = 0.f, ws[4] = {};  // 8-bit products: of this lane's matrix row, and of a fragment's four
 
+  float w_ahead = 0.f, x_ahead = 0.f;   // of the next tile: the scale of this lane's matrix row, and of its first tile row
+
   // The lane's matrix row is one of the tile's: kInt8 in order, kInt8Glu 8 of gate, the 8 of up.
-  __device__ __forceinline__ void load_w_scale(int32_t expert) {
-    if constexpr (MODE == kInt8) {
-      w_scale = m + lane < p.m_len ? p.w_scale[static_cast<int64_t>(expert) * p.m_len + m + lane] : 0.f;
-    } else if constexpr (MODE == kInt8Glu) {
-      const int32_t f = m / 2 + lane / 16 * 8 + lane % 8;
-      w_scale = f < p.out_len ? p.w_scale[static_cast<int64_t>(expert) * p.m_len + (lane % 16 < 8 ? 0 : p.out_len) + f] : 0.f;
+  __device__ __forceinline__ void read_ahead(const Tile& t, uint32_t rank, int quad, int part) {
+    const int32_t m0 = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
+    int32_t row = m0 + lane;
+    if constexpr (MODE == kInt8Glu) {
+      const int32_t f = m0 / 2 + lane / 16 * 8 + lane % 8;
+      row = f < p.out_len ? (lane % 16 < 8 ? 0 : p.out_len) + f : p.m_len;
     }
+    w_ahead = row < p.m_len ? p.w_scale[static_cast<int64_t>(t.e) * p.m_len + row] : 0.f;
+    x_ahead = part * 32 + lane < min(t.width, t.valid) ? p.x_scale[t.row0 + part * 32 + lane] : 0.f;
+  }
+  __device__ __forceinline__ float take_ahead() {
+    w_scale = w_ahead;
 #pragma unroll
     for (int i = 0; i < 4; ++i) ws[i] = __shfl_sync(0xffffffffu, w_scale, lane / 4 + 8 * i);
+    return x_ahead;
   }
   // The scale of row `col + lane` of the tile, read while the accumulator is.
   __device__ __forceinline__ float load_x_scale(int32_t col) const {
@@ -836,8 +845,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = c->tmem;
+  if constexpr (is_int8(MODE)) pdl_launch_dependents();   // a layer's next kernel may be under way before this one's inputs are there
   pdl_wait();
-  pdl_launch_dependents();   // one wave: whoever waits for this grid may take its place on the SMs as they fall free
+  if constexpr (!is_int8(MODE))
+    pdl_launch_dependents();   // one wave: whoever waits for this grid may take its place on the SMs as they fall free
 
   const int32_t first = blockIdx.x / 2, stride = gridDim.x / 2;
   Walker<MODE, SHAPE, RUNS> walk;
@@ -845,6 +856,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   if (warp == 0 || (is_int8(MODE) && warp == 2)) {
     // ---------------------------------------------------------------- loads
     const bool loads_a = !is_int8(MODE) || warp == 0, loads_b = !is_int8(MODE) || warp == 2;
+    const uint64_t policy = is_int8(MODE) && p.stream ? l2_policy_evict_first() : l2_policy_evict_normal();
     uint32_t it = 0, st = 0, phase = 1;
     uint32_t tails = 0, tail_odd = 0;   // a bit a stage: whether it has held a tail, whether an odd number of them
     bool ok = true;
@@ -875,9 +887,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             } else if constexpr (MODE == kRowsK) {
               pair_load_3d(a, &p.a, bar, r, m, t.e);
             } else if constexpr (MODE == kInt8) {
-              pair_load_3d(a, &p.a, bar, 2 * r, m, t.e);
+              pair_load_3d_hint(a, &p.a, bar, 2 * r, m, t.e, policy);
             } else if constexpr (MODE == kInt8Glu) {   // 8 rows of gate, the 8 of up, and so on
-              pair_load_5d(a, &p.a, bar, 2 * r, 0, 0, m / 16, t.e);
+              pair_load_5d_hint(a, &p.a, bar, 2 * r, 0, 0, m / 16, t.e, policy);
             } else if constexpr (MODE == kRowsMN) {
               pair_load_3d(a, &p.a, bar, m, r, t.e);
               pair_load_3d(a + kChunkBytes, &p.a, bar, m + 64, r, t.e);
@@ -1024,11 +1036,22 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     out.flip = kStoreBytes;
     uint32_t n = 0;
     bool ok = true;
-    for (int32_t tile = first; ok && walk.next(p, tile, stride, t);) {
+    // 8-bit tiles are short: the next one is found and its scales are read while this one is written
+    int32_t tile = first;
+    Tile ahead;
+    bool more = walk.next(p, tile, stride, ahead);
+    if (is_int8(MODE) && more) out.read_ahead(ahead, rank, quad, part);
+    while (ok && more) {
+      t = ahead;
       out.e = MODE >= kWgrad ? t.split * p.g.experts + t.e : t.split;
       out.m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
       out.add = p.accumulate || (RUNS && t.add);
-      if constexpr (is_int8(MODE)) out.load_w_scale(t.e);
+      float x0 = 0.f;
+      if constexpr (is_int8(MODE)) {
+        x0 = out.take_ahead();
+        more = walk.next(p, tile, stride, ahead);
+        if (more) out.read_ahead(ahead, rank, quad, part);
+      }
       if (RUNS && t.add && p.tma_out) {   // the stores of the run before have arrived: additions to the same values stay in order
         if (elect_one()) bulk_wait_all();
         __syncwarp();
@@ -1049,7 +1072,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           continue;
         }
         const uint32_t buf = n % 2, acc = tmem + buf * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16) + part * 32;
-        float x0 = out.load_x_scale(part * 32);   // read while the products run
         ok = warp_wait(&c->acc_full[buf], (n / 2) & 1, abort, p.dev_err);
         if (!ok) break;
         tc_fence_after();
@@ -1077,6 +1099,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           out.write(col + 64 * (i + 1), r1, x1);
         }
       }
+      if constexpr (!is_int8(MODE)) more = walk.next(p, tile, stride, ahead);
     }
     if (p.tma_out && elect_one()) bulk_wait_all();
     if (MODE < kWgrad && ok) {   // rows of no group
@@ -1373,6 +1396,8 @@ int make_glu_map(CUtensorMap* m, const int8_t* w, int64_t k, int64_t inter, int6
 
 }  // namespace
 
+constexpr int64_t kL2Kept = 64 << 20;   // half of L2
+
 size_t int8_partial_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k) {
   const int splits = rows_splits(rows, experts, n, (k + 1) / 2);
   return splits > 1 ? splits * rows * pitch4(n) * sizeof(float) : 0;
@@ -1404,6 +1429,10 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
   q.f32 = split || f32; q.bf16 = bf16;
   q.dev_err = dev_err;
   const PairShape shape = int8_shape(d.rows, d.experts, d.n);
+  // Matrices that are read once each, and are more than L2 keeps for the next call, make no room among what it should
+  // keep: 96 experts, 1536 x 2048: 512 rows 47.4 us against 49.9, 4096 rows 47.8 against 53.1.  Where a group has more
+  // than one tile (32768 rows: 113 against 110) or the matrices are few (8 rows: 9.5 against 8.5, from L2) it costs.
+  q.stream = shape != kOne && std::min<int64_t>(d.experts, d.rows) * d.n * d.k > kL2Kept;
   const int64_t tiles = row_tiles(d.rows, d.experts, d.n, shape) * q.splits;
   if (tiles >= (1ll << 30)) return arg_error("%s: too many tiles", what);
   constexpr CUtensorMapDataType kBytes = CU_TENSOR_MAP_DATA_TYPE_UINT8;

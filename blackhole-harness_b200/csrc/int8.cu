@@ -69,6 +69,21 @@ struct RowsParams {
   float* row_weight;
 };
 
+template <typename T>
+__device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {   // 16 bits
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same_v<T, __half>) {
+      x[2 * i] = __half2float(__ushort_as_half(static_cast<uint16_t>(w[i])));
+      x[2 * i + 1] = __half2float(__ushort_as_half(static_cast<uint16_t>(w[i] >> 16)));
+    } else {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+}
+
 // A row's values as they lie, 16 bytes at a time, or one by one (rows that are not aligned to 16 bytes, or of odd
 // lengths): the largest magnitude's bits, and the values in f32.
 template <typename T, bool VEC>
@@ -157,8 +172,8 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsPa
   __shared__ uint32_t part[kRowThreads / 32];
   const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + slot;
-  pdl_wait();
   pdl_launch_dependents();
+  pdl_wait();
   const bool live = row < p.rows && (!p.count || row < *p.count);
   const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
   const int n = p.cols / V;
@@ -286,8 +301,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
   __shared__ int32_t hist[kMaxExperts], first[kMaxExperts], sums[32];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
-  pdl_wait();
   pdl_launch_dependents();
+  pdl_wait();
   for (int e = threadIdx.x; e < experts; e += kPlanThreads) hist[e] = 0;
   __syncthreads();
   const int64_t chunk = (slots + ctas - 1) / ctas, begin = rank * chunk, end = min(begin + chunk, slots);
@@ -361,6 +376,91 @@ cudaError_t launch_plan(const void* ids, int32_t ids64, int64_t slots, int32_t e
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.numAttrs = 2;
   return cudaLaunchKernelEx(&cfg, plan_kernel, ids, ids64, slots, experts, offsets, places, dev_err);
+}
+
+// ------------------------------------------------------------------- sum
+// out[t] = sum over j of y[places[t topk + j]], f32 in j's order, rounded once; a slot without a row adds nothing.  Bound by
+// HBM: a thread has eight 16-byte loads in flight, of as many of a token's rows as there are and so many pieces of each.
+constexpr int kSumThreads = 256;
+
+struct SumParams {
+  const void* y;   // [rows, hidden] of Y
+  const int32_t* places;
+  void* out;
+  int64_t tokens;
+  int32_t topk, hidden;
+};
+
+template <typename Y, typename T, int ROWS>
+__global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const SumParams p) {
+  constexpr int kEach = 8 / ROWS;
+  const int32_t pieces = p.hidden / 8, spans = (pieces + 32 * kEach - 1) / (32 * kEach), lane = threadIdx.x % 32;
+  const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kSumThreads / 32) + threadIdx.x / 32;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t t = unit / spans;
+  if (t >= p.tokens) return;
+  const int32_t first = static_cast<int32_t>(unit % spans) * 32 * kEach + lane;
+  float sum[kEach][8] = {};
+  for (int j0 = 0; j0 < p.topk; j0 += ROWS) {
+    uint4 v[ROWS][kEach];
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j) {
+      const int32_t at = j0 + j < p.topk ? p.places[t * p.topk + j0 + j] : -1;
+      const uint4* row = static_cast<const uint4*>(p.y) + static_cast<int64_t>(at) * pieces;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        v[j][i] = at >= 0 && first + 32 * i < pieces ? row[first + 32 * i] : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int j = 0; j < ROWS; ++j)
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        float f[8];
+        unpack<Y>(v[j][i], f);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) sum[i][q] += f[q];
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    if (first + 32 * i >= pieces) continue;
+    T* out = static_cast<T*>(p.out) + t * p.hidden + (first + 32 * i) * 8;
+    if constexpr (std::is_same_v<T, float>) {
+      reinterpret_cast<float4*>(out)[0] = make_float4(sum[i][0], sum[i][1], sum[i][2], sum[i][3]);
+      reinterpret_cast<float4*>(out)[1] = make_float4(sum[i][4], sum[i][5], sum[i][6], sum[i][7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if constexpr (std::is_same_v<T, __half>) {
+          const __half2 h = __floats2half2_rn(sum[i][2 * q], sum[i][2 * q + 1]);
+          w[q] = reinterpret_cast<const uint32_t&>(h);
+        } else {
+          const __nv_bfloat162 h = __floats2bfloat162_rn(sum[i][2 * q], sum[i][2 * q + 1]);
+          w[q] = reinterpret_cast<const uint32_t&>(h);
+        }
+      }
+      *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+template <typename Y, typename T>
+cudaError_t launch_sum(const SumParams& p, cudaStream_t st) {
+  auto go = [&](auto rows, auto* kernel) {
+    constexpr int kEach = 8 / decltype(rows)::value;
+    const int64_t spans = (p.hidden / 8 + 32 * kEach - 1) / (32 * kEach);
+    const int64_t blocks = (p.tokens * spans + kSumThreads / 32 - 1) / (kSumThreads / 32);
+    if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = launch_config(dim3(static_cast<unsigned>(blocks)), kSumThreads, 0, st, &attr);
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+  };
+  if (p.topk == 1) return go(std::integral_constant<int, 1>{}, sum_rows_kernel<Y, T, 1>);
+  if (p.topk == 2) return go(std::integral_constant<int, 2>{}, sum_rows_kernel<Y, T, 2>);
+  if (p.topk <= 4) return go(std::integral_constant<int, 4>{}, sum_rows_kernel<Y, T, 4>);
+  return go(std::integral_constant<int, 8>{}, sum_rows_kernel<Y, T, 8>);
 }
 
 bool is16(int32_t dt) { return dt == HEXMOE_BF16 || dt == HEXMOE_F16; }
@@ -553,7 +653,10 @@ int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t to
   d.out = s.y; d.ld_out = hidden; d.out_dtype = y_dtype;
   d.workspace = s.partial; d.workspace_bytes = s.partial_bytes;
   if (int rc = run_int8_product(what, d, st)) return rc;
-  e = launch_combine(s.y, y_dtype, tokens, topk, hidden, hidden, s.places, slots, out, out_dtype, st, true);
+  const SumParams sum = {s.y, s.places, out, tokens, topk, hidden};
+  e = y_dtype == HEXMOE_F16 ? (out_dtype == HEXMOE_F32 ? launch_sum<__half, float>(sum, st) : launch_sum<__half, __half>(sum, st))
+      : out_dtype == HEXMOE_F32 ? launch_sum<__nv_bfloat16, float>(sum, st)
+                                : launch_sum<__nv_bfloat16, __nv_bfloat16>(sum, st);
   return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
 }
 
