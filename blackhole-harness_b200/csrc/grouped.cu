@@ -845,10 +845,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = c->tmem;
-  if constexpr (is_int8(MODE)) pdl_launch_dependents();   // a layer's next kernel may be under way before this one's inputs are there
   pdl_wait();
-  if constexpr (!is_int8(MODE))
-    pdl_launch_dependents();   // one wave: whoever waits for this grid may take its place on the SMs as they fall free
+  pdl_launch_dependents();   // one wave: whoever waits for this grid may take its place on the SMs as they fall free
 
   const int32_t first = blockIdx.x / 2, stride = gridDim.x / 2;
   Walker<MODE, SHAPE, RUNS> walk;
@@ -856,7 +854,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   if (warp == 0 || (is_int8(MODE) && warp == 2)) {
     // ---------------------------------------------------------------- loads
     const bool loads_a = !is_int8(MODE) || warp == 0, loads_b = !is_int8(MODE) || warp == 2;
-    const uint64_t policy = is_int8(MODE) && p.stream ? l2_policy_evict_first() : l2_policy_evict_normal();
+    const uint64_t policy = is_int8(MODE) ? l2_policy_evict_first() : 0;
     uint32_t it = 0, st = 0, phase = 1;
     uint32_t tails = 0, tail_odd = 0;   // a bit a stage: whether it has held a tail, whether an odd number of them
     bool ok = true;
@@ -887,9 +885,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             } else if constexpr (MODE == kRowsK) {
               pair_load_3d(a, &p.a, bar, r, m, t.e);
             } else if constexpr (MODE == kInt8) {
-              pair_load_3d_hint(a, &p.a, bar, 2 * r, m, t.e, policy);
+              if (p.stream) pair_load_3d_hint(a, &p.a, bar, 2 * r, m, t.e, policy);
+              else pair_load_3d(a, &p.a, bar, 2 * r, m, t.e);
             } else if constexpr (MODE == kInt8Glu) {   // 8 rows of gate, the 8 of up, and so on
-              pair_load_5d_hint(a, &p.a, bar, 2 * r, 0, 0, m / 16, t.e, policy);
+              if (p.stream) pair_load_5d_hint(a, &p.a, bar, 2 * r, 0, 0, m / 16, t.e, policy);
+              else pair_load_5d(a, &p.a, bar, 2 * r, 0, 0, m / 16, t.e);
             } else if constexpr (MODE == kRowsMN) {
               pair_load_3d(a, &p.a, bar, m, r, t.e);
               pair_load_3d(a + kChunkBytes, &p.a, bar, m + 64, r, t.e);
@@ -1036,22 +1036,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     out.flip = kStoreBytes;
     uint32_t n = 0;
     bool ok = true;
-    // 8-bit tiles are short: the next one is found and its scales are read while this one is written
-    int32_t tile = first;
-    Tile ahead;
-    bool more = walk.next(p, tile, stride, ahead);
-    if (is_int8(MODE) && more) out.read_ahead(ahead, rank, quad, part);
-    while (ok && more) {
-      t = ahead;
+    auto write_tile = [&](float x0) {
       out.e = MODE >= kWgrad ? t.split * p.g.experts + t.e : t.split;
       out.m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
       out.add = p.accumulate || (RUNS && t.add);
-      float x0 = 0.f;
-      if constexpr (is_int8(MODE)) {
-        x0 = out.take_ahead();
-        more = walk.next(p, tile, stride, ahead);
-        if (more) out.read_ahead(ahead, rank, quad, part);
-      }
       if (RUNS && t.add && p.tma_out) {   // the stores of the run before have arrived: additions to the same values stay in order
         if (elect_one()) bulk_wait_all();
         __syncwarp();
@@ -1099,7 +1087,20 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           out.write(col + 64 * (i + 1), r1, x1);
         }
       }
-      if constexpr (!is_int8(MODE)) more = walk.next(p, tile, stride, ahead);
+    };
+    if constexpr (is_int8(MODE)) {   // short tiles: the next one is found and its scales are read before this one is written
+      Tile ahead;
+      float x0 = 0.f;
+      bool more = true;
+      for (int32_t tile = first, n_tiles = 0; ok && more; ++n_tiles) {
+        more = walk.next(p, tile, stride, ahead);
+        if (more) out.read_ahead(ahead, rank, quad, part);
+        if (n_tiles) write_tile(x0);
+        t = ahead;
+        x0 = out.take_ahead();
+      }
+    } else {
+      for (int32_t tile = first; ok && walk.next(p, tile, stride, t);) write_tile(0.f);
     }
     if (p.tma_out && elect_one()) bulk_wait_all();
     if (MODE < kWgrad && ok) {   // rows of no group

@@ -172,8 +172,8 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsPa
   __shared__ uint32_t part[kRowThreads / 32];
   const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + slot;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   const bool live = row < p.rows && (!p.count || row < *p.count);
   const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
   const int n = p.cols / V;
@@ -301,8 +301,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
   __shared__ int32_t hist[kMaxExperts], first[kMaxExperts], sums[32];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   for (int e = threadIdx.x; e < experts; e += kPlanThreads) hist[e] = 0;
   __syncthreads();
   const int64_t chunk = (slots + ctas - 1) / ctas, begin = rank * chunk, end = min(begin + chunk, slots);
@@ -396,8 +396,8 @@ __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const SumParams p
   constexpr int kEach = 8 / ROWS;
   const int32_t pieces = p.hidden / 8, spans = (pieces + 32 * kEach - 1) / (32 * kEach), lane = threadIdx.x % 32;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kSumThreads / 32) + threadIdx.x / 32;
-  pdl_launch_dependents();
   pdl_wait();
+  pdl_launch_dependents();
   const int64_t t = unit / spans;
   if (t >= p.tokens) return;
   const int32_t first = static_cast<int32_t>(unit % spans) * 32 * kEach + lane;

@@ -74,6 +74,14 @@ __device__ __forceinline__ void pair_load_3d(void* dst, const CUtensorMap* map, 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+__device__ __forceinline__ void pair_load_5d(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y,
+                                             int32_t z, int32_t u, int32_t v) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, "
+      "%5, %6, %7}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(u), "r"(v)
+      : "memory");
+}
 // The same with an L2 policy (createpolicy) for the lines read.
 __device__ __forceinline__ void pair_load_3d_hint(void* dst, const CUtensorMap* map, uint32_t bar, int32_t x, int32_t y,
                                                   int32_t z, uint64_t policy) {
