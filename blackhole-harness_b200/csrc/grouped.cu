@@ -547,24 +547,18 @@ struct Writer {
   int64_t n0 = 0;                   // column 0 in the output: row products: its row; weight gradient: its column
   float w_scale = 0.f, ws[4] = {};  // 8-bit products: of this lane's matrix row, and of a fragment's four
 
-  float w_ahead = 0.f, x_ahead = 0.f;   // of the next tile: the scale of this lane's matrix row, and of its first tile row
-
   // The lane's matrix row is one of the tile's: kInt8 in order, kInt8Glu 8 of gate, the 8 of up.
-  __device__ __forceinline__ void read_ahead(const Tile& t, uint32_t rank, int quad, int part) {
-    const int32_t m0 = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
-    int32_t row = m0 + lane;
+  __device__ __forceinline__ void load_w_scale(int32_t expert) {
+    int32_t row = m + lane;
     if constexpr (MODE == kInt8Glu) {
-      const int32_t f = m0 / 2 + lane / 16 * 8 + lane % 8;
+      const int32_t f = m / 2 + lane / 16 * 8 + lane % 8;
       row = f < p.out_len ? (lane % 16 < 8 ? 0 : p.out_len) + f : p.m_len;
     }
-    w_ahead = row < p.m_len ? p.w_scale[static_cast<int64_t>(t.e) * p.m_len + row] : 0.f;
-    x_ahead = part * 32 + lane < min(t.width, t.valid) ? p.x_scale[t.row0 + part * 32 + lane] : 0.f;
+    w_scale = row < p.m_len ? p.w_scale[static_cast<int64_t>(expert) * p.m_len + row] : 0.f;
   }
-  __device__ __forceinline__ float take_ahead() {
-    w_scale = w_ahead;
+  __device__ __forceinline__ void spread_w_scale() {   // once it is needed: what is loaded beside it does not wait
 #pragma unroll
     for (int i = 0; i < 4; ++i) ws[i] = __shfl_sync(0xffffffffu, w_scale, lane / 4 + 8 * i);
-    return x_ahead;
   }
   // The scale of row `col + lane` of the tile, read while the accumulator is.
   __device__ __forceinline__ float load_x_scale(int32_t col) const {
@@ -1036,7 +1030,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     out.flip = kStoreBytes;
     uint32_t n = 0;
     bool ok = true;
-    auto write_tile = [&](float x0) {
+    for (int32_t tile = first; ok && walk.next(p, tile, stride, t);) {
       out.e = MODE >= kWgrad ? t.split * p.g.experts + t.e : t.split;
       out.m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
       out.add = p.accumulate || (RUNS && t.add);
@@ -1044,9 +1038,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         if (elect_one()) bulk_wait_all();
         __syncwarp();
       }
+      if constexpr (is_int8(MODE)) out.load_w_scale(t.e);
       for (int acc_n = 0; acc_n < (WIDE ? t.parts : 1); ++acc_n) {
         const int32_t cols = MODE >= kWgrad ? min(t.width, p.n_len - t.n0) : min(t.width, t.valid - acc_n * t.width);
-        const int chunks = out.m < p.m_len && cols > part * 32 ? (cols - part * 32 + 63) / 64 : 0;
+        // 8-bit tiles are short, and one of up to 32 columns is one warp's of each two: in turn
+        const int col = (is_int8(MODE) ? (part + n) % 2 : part) * 32;
+        const int chunks = out.m < p.m_len && cols > col ? (cols - col + 63) / 64 : 0;
         out.cols = cols;
         out.n0 = MODE >= kWgrad ? t.n0 : t.row0 + acc_n * t.width;
         uint32_t r0[32], r1[32];
@@ -1055,11 +1052,12 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           for (int i = 0; i < chunks; ++i) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) r0[j] = 0;
-            out.write(part * 32 + 64 * i, r0, 0.f);
+            out.write(col + 64 * i, r0, 0.f);
           }
           continue;
         }
-        const uint32_t buf = n % 2, acc = tmem + buf * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16) + part * 32;
+        const uint32_t buf = n % 2, acc = tmem + buf * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16) + col;
+        float x0 = out.load_x_scale(col);   // read while the products run
         ok = warp_wait(&c->acc_full[buf], (n / 2) & 1, abort, p.dev_err);
         if (!ok) break;
         tc_fence_after();
@@ -1070,9 +1068,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           __syncwarp();
           if (lane == 0) pair_arrive(peer_addr(&c->acc_empty[buf], 0));
         };
-        const int32_t col = part * 32;
         if (chunks == 0) release();
         else out.load(acc, r0);
+        if constexpr (is_int8(MODE)) out.spread_w_scale();
         for (int i = 0; i < chunks; i += 2) {
           tmem_ld_wait_for(r0);
           const float x1 = i + 1 < chunks ? out.load_x_scale(col + 64 * (i + 1)) : 0.f;
@@ -1087,20 +1085,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           out.write(col + 64 * (i + 1), r1, x1);
         }
       }
-    };
-    if constexpr (is_int8(MODE)) {   // short tiles: the next one is found and its scales are read before this one is written
-      Tile ahead;
-      float x0 = 0.f;
-      bool more = true;
-      for (int32_t tile = first, n_tiles = 0; ok && more; ++n_tiles) {
-        more = walk.next(p, tile, stride, ahead);
-        if (more) out.read_ahead(ahead, rank, quad, part);
-        if (n_tiles) write_tile(x0);
-        t = ahead;
-        x0 = out.take_ahead();
-      }
-    } else {
-      for (int32_t tile = first; ok && walk.next(p, tile, stride, t);) write_tile(0.f);
     }
     if (p.tma_out && elect_one()) bulk_wait_all();
     if (MODE < kWgrad && ok) {   // rows of no group
