@@ -448,6 +448,7 @@ struct Walker {
   int64_t carry = 0, lo = 0;
   int32_t upto = 0, mine = 0, total = 0;
   int64_t begin = 0, end = 0;
+  int32_t row = 0, size = 0, tiles = 0, parts = 1, width = 0;   // row products: of this lane's group, and of its tiles
   bool bad = false;
   int32_t left = 0, per = 0, end_tail = 0;   // of the tile's steps: to come, in a run, and its last one
 
@@ -487,7 +488,15 @@ struct Walker {
       if (base == 0) lo = __shfl_sync(0xffffffffu, begin, 0);
       const int lane = threadIdx.x % 32;
       if constexpr (MODE >= kWgrad) mine = base + lane < p.g.experts ? p.m_tiles * p.n_tiles : 0;
-      else mine = static_cast<int32_t>((end - begin + kSpan - 1) / kSpan) * p.m_tiles;
+      else {
+        row = static_cast<int32_t>(begin);
+        size = static_cast<int32_t>(end - begin);
+        tiles = (size + kSpan - 1) / kSpan;
+        const int32_t span = tiles > 1 ? (size + tiles - 1) / tiles : size;
+        parts = SHAPE == kTwo && span > 256 ? 2 : 1;
+        width = ((span + parts - 1) / parts + 31) / 32 * 32;
+        mine = tiles * p.m_tiles;
+      }
       upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -498,11 +507,11 @@ struct Walker {
       total = __shfl_sync(0xffffffffu, upto, 31);
     }
     const int src = __ffs(__ballot_sync(0xffffffffu, tile < upto)) - 1;
-    const int64_t b = __shfl_sync(0xffffffffu, begin, src), e = __shfl_sync(0xffffffffu, end, src);
     const int32_t local = tile - __shfl_sync(0xffffffffu, upto - mine, src);
     t.e = base + src;
     constexpr int32_t kWidth = kStepK * subs_of(SHAPE);
     if constexpr (MODE >= kWgrad) {
+      const int64_t b = __shfl_sync(0xffffffffu, begin, src), e = __shfl_sync(0xffffffffu, end, src);
       t.m0 = local / p.n_tiles * 256;
       t.n0 = local % p.n_tiles * p.tile_n;
       t.width = t.valid = p.tile_n;
@@ -511,14 +520,15 @@ struct Walker {
       t.steps = static_cast<int32_t>((e - b + kWidth - 1) / kWidth);
       t.tail = static_cast<int32_t>((e - b) % kWidth);
     } else {
-      const int32_t size = static_cast<int32_t>(e - b), tiles = (size + kSpan - 1) / kSpan;
-      const int32_t span = (size + tiles - 1) / tiles;
-      const int32_t parts = SHAPE == kTwo && span > 256 ? 2 : 1;
-      t.width = ((span + parts - 1) / parts + 31) / 32 * 32;
-      t.m0 = local / tiles * 256;
-      t.n0 = local % tiles * parts * t.width;
-      t.row0 = b + t.n0;
-      t.valid = min(parts * t.width, size - t.n0);
+      const int32_t group_tiles = __shfl_sync(0xffffffffu, tiles, src), group_size = __shfl_sync(0xffffffffu, size, src);
+      const int32_t across = SHAPE == kTwo ? __shfl_sync(0xffffffffu, parts, src) : 1;
+      // one tile of a group's rows is the rule where tiles are short: no division then
+      const int32_t m = group_tiles == 1 ? local : local / group_tiles, n = local - m * group_tiles;
+      t.width = __shfl_sync(0xffffffffu, width, src);
+      t.m0 = m * 256;
+      t.n0 = n * across * t.width;
+      t.row0 = __shfl_sync(0xffffffffu, row, src) + t.n0;
+      t.valid = min(across * t.width, group_size - t.n0);
       t.parts = t.valid > t.width ? 2 : 1;   // the last tile of a group may end within its first accumulator
       t.steps = (p.red + kWidth - 1) / kWidth;
       t.tail = p.red % kWidth;
