@@ -1048,7 +1048,6 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         if (elect_one()) bulk_wait_all();
         __syncwarp();
       }
-      if constexpr (is_int8(MODE)) out.load_w_scale(t.e);
       for (int acc_n = 0; acc_n < (WIDE ? t.parts : 1); ++acc_n) {
         const int32_t cols = MODE >= kWgrad ? min(t.width, p.n_len - t.n0) : min(t.width, t.valid - acc_n * t.width);
         // 8-bit tiles are short, and one of up to 32 columns is one warp's of each two: in turn
@@ -1067,7 +1066,11 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
           continue;
         }
         const uint32_t buf = n % 2, acc = tmem + buf * kAccCols + (static_cast<uint32_t>(quad) * 32 << 16) + col;
-        float x0 = out.load_x_scale(col);   // read while the products run
+        float x0 = 0.f;
+        if (is_int8(MODE) && chunks) {   // read while the products run
+          out.load_w_scale(t.e);
+          x0 = out.load_x_scale(col);
+        }
         ok = warp_wait(&c->acc_full[buf], (n / 2) & 1, abort, p.dev_err);
         if (!ok) break;
         tc_fence_after();
@@ -1080,7 +1083,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         };
         if (chunks == 0) release();
         else out.load(acc, r0);
-        if constexpr (is_int8(MODE)) out.spread_w_scale();
+        if (is_int8(MODE) && chunks) out.spread_w_scale();
         for (int i = 0; i < chunks; i += 2) {
           tmem_ld_wait_for(r0);
           const float x1 = i + 1 < chunks ? out.load_x_scale(col + 64 * (i + 1)) : 0.f;

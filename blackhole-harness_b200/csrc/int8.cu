@@ -165,16 +165,14 @@ struct RowScale {
   }
 };
 
-template <typename T, bool VEC, int TPR>
-__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsParams p) {
+// One row, by the TPR threads of it (lane: which); PLACES: into the rows of its slots, which this kernel may have
+// written (they are read past L1).  Every thread of the block calls it where TPR > 32; live: whether there is a row.  The
+// pieces are turned into bytes in registers and stored from there: what is unrolled eight times stays short, for a kernel of a
+// few microseconds waits for its instructions more than for anything else.
+template <typename T, bool VEC, int TPR, bool PLACES>
+__device__ __forceinline__ void quantize_row(const RowsParams& p, int64_t row, bool live, int lane, uint32_t* part) {
   using P = Piece<T, VEC>;
-  constexpr int kRows = kRowThreads / TPR, V = P::kValues;
-  __shared__ uint32_t part[kRowThreads / 32];
-  const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + slot;
-  pdl_wait();
-  pdl_launch_dependents();
-  const bool live = row < p.rows && (!p.count || row < *p.count);
+  constexpr int V = P::kValues, kWords = V > 4 ? V / 4 : 1;
   const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
   const int n = p.cols / V;
   P held[kPieces];
@@ -198,59 +196,79 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsPa
   if constexpr (TPR > 32) {
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = bits;
     __syncthreads();
+    const int slot = threadIdx.x / TPR;
 #pragma unroll
     for (int i = 0; i < TPR / 32; ++i) bits = max(bits, part[slot * (TPR / 32) + i]);
   }
   if (!live) return;
   const RowScale to(bits);
-  auto write = [&](const P& v, int c) {
+  const bool finite = to.finite();
+  auto bytes = [&](const P& v, uint32_t (&w)[kWords]) {
     uint32_t q[V];
     float doubt = 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) q[j] = to.byte<T>(v.value(j), doubt);
-    if (!to.finite()) {
-#pragma unroll
-      for (int j = 0; j < V; ++j) q[j] = 0;
-    } else if (sizeof(T) == 4 && RowScale::near_border(doubt)) {
+    if (sizeof(T) == 4 && __builtin_expect(RowScale::near_border(doubt), 0)) {
 #pragma unroll
       for (int j = 0; j < V; ++j) q[j] = to.exact_byte(v.value(j));
     }
-    uint32_t w[V / 4 + 1];
+    if constexpr (V == 1) w[0] = q[0];
 #pragma unroll
     for (int j = 0; j + 3 < V; j += 4) w[j / 4] = prmt(prmt(q[j], q[j + 1], 0x0040), prmt(q[j + 2], q[j + 3], 0x0040), 0x5410);
-    auto put = [&](int64_t at) {
-      int8_t* dst = p.q + at * p.ld_q + static_cast<int64_t>(c) * V;
-      if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-      else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
-      else *dst = static_cast<int8_t>(q[0]);
-    };
-    if (!p.places) {
-      put(row);
-    } else {
-      for (int j = 0; j < p.topk; ++j) {
-        const int32_t at = p.places[row * p.topk + j];
-        if (at >= 0) put(at);
-      }
+    if (!finite) {
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) w[j] = 0;
     }
   };
+  auto put = [&](int64_t at, int c, const uint32_t (&w)[kWords]) {
+    int8_t* dst = p.q + at * p.ld_q + static_cast<int64_t>(c) * V;
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    else if constexpr (V == 4) *reinterpret_cast<uint32_t*>(dst) = w[0];
+    else *dst = static_cast<int8_t>(w[0]);
+  };
+  uint32_t w[kPieces][kWords];
 #pragma unroll
-  for (int i = 0; i < kPieces; ++i)
-    if (lane + i * TPR < n) write(held[i], lane + i * TPR);
+  for (int i = 0; i < kPieces; ++i) {
+    if (lane + i * TPR < n) bytes(held[i], w[i]);
+  }
+  const int copies = PLACES ? p.topk : 1;
+#pragma unroll 1
+  for (int j = 0; j < copies; ++j) {
+    const int64_t at = PLACES ? __ldcg(p.places + row * p.topk + j) : row;
+    if (PLACES && at < 0) continue;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i)
+      if (lane + i * TPR < n) put(at, lane + i * TPR, w[i]);
+    if (lane == 0) {
+      if constexpr (PLACES) {
+        p.scale[at] = to.scale();
+        p.row_weight[at] = p.weights[row * p.topk + j];
+      } else {
+        p.scale[at] = p.factor ? to.scale() * p.factor[row] : to.scale();
+      }
+    }
+  }
   for (int c = lane + kPieces * TPR; c < n; c += TPR) {
     P v;
     v.load(x, c);
-    write(v, c);
-  }
-  if (!p.places) {
-    if (lane == 0) p.scale[row] = p.factor ? to.scale() * p.factor[row] : to.scale();
-  } else {
-    for (int j = lane; j < p.topk; j += TPR) {
-      const int32_t at = p.places[row * p.topk + j];
-      if (at < 0) continue;
-      p.scale[at] = to.scale();
-      p.row_weight[at] = p.weights[row * p.topk + j];
+    bytes(v, w[0]);
+#pragma unroll 1
+    for (int j = 0; j < copies; ++j) {
+      const int64_t at = PLACES ? __ldcg(p.places + row * p.topk + j) : row;
+      if (!PLACES || at >= 0) put(at, c, w[0]);
     }
   }
+}
+
+template <typename T, bool VEC, int TPR, bool PLACES>
+__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsParams p) {
+  constexpr int kRows = kRowThreads / TPR;
+  __shared__ uint32_t part[kRowThreads / 32];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
+  pdl_wait();
+  pdl_launch_dependents();
+  const bool live = row < p.rows && (!p.count || row < *p.count);
+  quantize_row<T, VEC, TPR, PLACES>(p, row, live, threadIdx.x % TPR, part);
 }
 
 // The threads of a row: as few as hold it in registers.
@@ -265,18 +283,25 @@ cudaError_t launch_rows_vec(const RowsParams& p, cudaStream_t st) {
     const cudaLaunchConfig_t cfg = launch_config(dim3(static_cast<unsigned>(blocks)), kRowThreads, 0, st, &attr);
     return cudaLaunchKernelEx(&cfg, kernel, p);
   };
-  if (n <= 8 * kPieces) return go(std::integral_constant<int, 8>{}, quantize_rows_kernel<T, VEC, 8>);
-  if (n <= 32 * kPieces) return go(std::integral_constant<int, 32>{}, quantize_rows_kernel<T, VEC, 32>);
-  if (n <= 64 * kPieces) return go(std::integral_constant<int, 64>{}, quantize_rows_kernel<T, VEC, 64>);
-  return go(std::integral_constant<int, 256>{}, quantize_rows_kernel<T, VEC, 256>);
+  auto pick = [&](auto tpr) {
+    constexpr int TPR = decltype(tpr)::value;
+    return p.places ? go(tpr, quantize_rows_kernel<T, VEC, TPR, true>) : go(tpr, quantize_rows_kernel<T, VEC, TPR, false>);
+  };
+  if (n <= 8 * kPieces) return pick(std::integral_constant<int, 8>{});
+  if (n <= 32 * kPieces) return pick(std::integral_constant<int, 32>{});
+  if (n <= 64 * kPieces) return pick(std::integral_constant<int, 64>{});
+  return pick(std::integral_constant<int, 256>{});
 }
 
 template <typename T>
-cudaError_t launch_rows_type(const RowsParams& p, cudaStream_t st) {
+bool rows_aligned(const RowsParams& p) {   // rows of whole pieces of 16 bytes
   constexpr int V = 16 / sizeof(T);
-  const bool vec = p.cols % V == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ld_x % V == 0 &&
-                   reinterpret_cast<uintptr_t>(p.q) % V == 0 && p.ld_q % V == 0;
-  return vec ? launch_rows_vec<T, true>(p, st) : launch_rows_vec<T, false>(p, st);
+  return p.cols % V == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.ld_x % V == 0 &&
+         reinterpret_cast<uintptr_t>(p.q) % V == 0 && p.ld_q % V == 0;
+}
+template <typename T>
+cudaError_t launch_rows_type(const RowsParams& p, cudaStream_t st) {
+  return rows_aligned<T>(p) ? launch_rows_vec<T, true>(p, st) : launch_rows_vec<T, false>(p, st);
 }
 
 cudaError_t launch_rows(const RowsParams& p, int32_t dtype, cudaStream_t st) {
@@ -291,43 +316,85 @@ cudaError_t launch_rows(const RowsParams& p, int32_t dtype, cudaStream_t st) {
 // rows come in whatever order the counting finds: no value of the layer depends on it (a row's sums are whole
 // numbers and its own).  One cluster: each CTA counts its slots in shared memory, the counts of the CTAs before it come
 // over distributed shared memory, and nothing has to be cleared or handed on between kernels.
+// Few tokens are quantized by the same kernel once their rows are known, a warp a token: one launch less (2 tokens of
+// 416, the layer: 18.9 us against 22.3), as long as one SM can write the rows (22 tokens of 2816, top 6, by eight: 43 us
+// against 40).
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;
+constexpr int kPlanHeld = 4;        // slots a thread keeps in registers
 constexpr int kMaxExperts = 2048;
+constexpr int64_t kTogether = 32, kTogetherBytes = 1 << 17;   // tokens, and bytes of all slots' rows
 
-__global__ void __launch_bounds__(kPlanThreads, 1)
-    plan_kernel(const void* ids, int32_t ids64, int64_t slots, int32_t experts, int32_t* offsets, int32_t* places,
-                int32_t* dev_err) {
+struct PlanParams {
+  const void* ids;
+  int32_t ids64, experts;
+  int64_t slots;
+  int32_t* offsets;
+  int32_t* places;
+  int32_t* dev_err;
+};
+
+// The experts of kPlanHeld slots, `step` apart from s on, all loads issued before the first is used; -1: of none.
+__device__ __forceinline__ void plan_experts(const PlanParams& p, int64_t s, int64_t step, int64_t end, int32_t (&e)[kPlanHeld]) {
+  int64_t v[kPlanHeld];
+#pragma unroll
+  for (int i = 0; i < kPlanHeld; ++i) {
+    const int64_t at = s + i * step;
+    v[i] = at < end ? (p.ids64 ? static_cast<const int64_t*>(p.ids)[at] : static_cast<const int32_t*>(p.ids)[at]) : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < kPlanHeld; ++i) e[i] = v[i] >= 0 && v[i] < p.experts ? static_cast<int32_t>(v[i]) : -1;
+}
+
+// T: the tokens' type where they are quantized here (by one CTA), else void.
+template <typename T, bool VEC, int CTAS>
+__global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanParams p, const RowsParams rows) {
   __shared__ int32_t hist[kMaxExperts], first[kMaxExperts], sums[32];
   cg::cluster_group cluster = cg::this_cluster();
-  const int rank = static_cast<int>(cluster.block_rank()), ctas = static_cast<int>(cluster.num_blocks());
+  const int rank = CTAS > 1 ? static_cast<int>(cluster.block_rank()) : 0;
+  auto sync = [&] {
+    if constexpr (CTAS > 1) cluster.sync();
+    else __syncthreads();
+  };
+  for (int e = threadIdx.x; e < p.experts; e += kPlanThreads) hist[e] = 0;
   pdl_wait();
   pdl_launch_dependents();
-  for (int e = threadIdx.x; e < experts; e += kPlanThreads) hist[e] = 0;
   __syncthreads();
-  const int64_t chunk = (slots + ctas - 1) / ctas, begin = rank * chunk, end = min(begin + chunk, slots);
-  auto expert = [&](int64_t s) -> int64_t {
-    const int64_t e = ids64 ? static_cast<const int64_t*>(ids)[s] : static_cast<const int32_t*>(ids)[s];
-    return e >= 0 && e < experts ? e : -1;
-  };
+  const int64_t chunk = (p.slots + CTAS - 1) / CTAS, begin = rank * chunk, end = min(begin + chunk, p.slots);
+  const int64_t s0 = begin + threadIdx.x;
+  int32_t held_e[kPlanHeld], held_at[kPlanHeld];   // of the first slots; those behind wait in places
   bool bad = false;
-  for (int64_t s = begin + threadIdx.x; s < end; s += kPlanThreads) {
-    const int64_t e = expert(s);
-    places[s] = e < 0 ? -1 : atomicAdd(&hist[e], 1);
-    bad |= e < 0;
+  for (int64_t s = s0; s < end; s += kPlanHeld * kPlanThreads) {
+    int32_t e[kPlanHeld];
+    plan_experts(p, s, kPlanThreads, end, e);
+#pragma unroll
+    for (int i = 0; i < kPlanHeld; ++i) {
+      const int64_t at = s + i * kPlanThreads;
+      const int32_t n = e[i] >= 0 ? atomicAdd(&hist[e[i]], 1) : -1;
+      bad |= at < end && e[i] < 0;
+      if (s == s0) {
+        held_e[i] = e[i];
+        held_at[i] = n;
+      } else if (at < end) {
+        p.places[at] = n;
+      }
+    }
   }
-  if (bad) atomicOr(dev_err, kDevErrExpertId);
-  cluster.sync();
+  if (bad) atomicOr(p.dev_err, kDevErrExpertId);
+  sync();
   // every CTA: each expert's count over all of them, and before this one
-  const int per = (experts + kPlanThreads - 1) / kPlanThreads;   // 1 or 2 a thread
+  const int per = (p.experts + kPlanThreads - 1) / kPlanThreads;   // 1 or 2 a thread
   int32_t total[2] = {}, before[2] = {}, mine = 0;
   for (int i = 0; i < per; ++i) {
     const int e = static_cast<int>(threadIdx.x) * per + i;
-    if (e >= experts) break;
-    for (int c = 0; c < ctas; ++c) {
-      const int32_t v = cluster.map_shared_rank(hist, c)[e];
-      total[i] += v;
-      if (c < rank) before[i] += v;
+    if (e >= p.experts) break;
+    int32_t v[CTAS];
+#pragma unroll
+    for (int c = 0; c < CTAS; ++c) v[c] = CTAS > 1 ? cluster.map_shared_rank(hist, c)[e] : hist[e];
+#pragma unroll
+    for (int c = 0; c < CTAS; ++c) {
+      total[i] += v[c];
+      if (c < rank) before[i] += v[c];
     }
     mine += total[i];
   }
@@ -353,29 +420,53 @@ __global__ void __launch_bounds__(kPlanThreads, 1)
   int32_t at = upto - mine + (warp ? sums[warp - 1] : 0);
   for (int i = 0; i < per; ++i) {
     const int e = static_cast<int>(threadIdx.x) * per + i;
-    if (e >= experts) break;
+    if (e >= p.experts) break;
     first[e] = at + before[i];
-    if (rank == 0) offsets[e] = at;
+    if (rank == 0) p.offsets[e] = at;
     at += total[i];
-    if (rank == 0 && e == experts - 1) offsets[experts] = at;
+    if (rank == 0 && e == p.experts - 1) p.offsets[p.experts] = at;
   }
-  cluster.sync();   // `first` is whole, and no CTA leaves while its counts are read
-  for (int64_t s = begin + threadIdx.x; s < end; s += kPlanThreads) {
-    const int64_t e = expert(s);
-    if (e >= 0) places[s] += first[e];
+  sync();   // `first` is whole, and no CTA leaves while its counts are read
+#pragma unroll
+  for (int i = 0; i < kPlanHeld; ++i)
+    if (s0 + i * kPlanThreads < end) p.places[s0 + i * kPlanThreads] = held_e[i] < 0 ? -1 : held_at[i] + first[held_e[i]];
+  for (int64_t s = s0 + kPlanHeld * kPlanThreads; s < end; s += kPlanHeld * kPlanThreads) {
+    int32_t e[kPlanHeld];
+    plan_experts(p, s, kPlanThreads, end, e);
+#pragma unroll
+    for (int i = 0; i < kPlanHeld; ++i)
+      if (e[i] >= 0) p.places[s + i * kPlanThreads] += first[e[i]];
+  }
+  if constexpr (!std::is_void_v<T>) {
+    sync();   // every token's places
+    if (warp < rows.rows) quantize_row<T, VEC, 32, true>(rows, warp, true, lane, nullptr);
   }
 }
 
-cudaError_t launch_plan(const void* ids, int32_t ids64, int64_t slots, int32_t experts, int32_t* offsets, int32_t* places,
-                        int32_t* dev_err, cudaStream_t st) {
+template <typename T, bool VEC, int CTAS>
+cudaError_t launch_plan_one(const PlanParams& p, const RowsParams& rows, cudaStream_t st) {
   cudaLaunchAttribute attr[2];
-  const int ctas = slots > 2 * kPlanThreads ? kPlanCtas : 1;
-  cudaLaunchConfig_t cfg = launch_config(dim3(ctas), kPlanThreads, 0, st, attr);
+  cudaLaunchConfig_t cfg = launch_config(dim3(CTAS), kPlanThreads, 0, st, attr);
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.x = CTAS;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, plan_kernel, ids, ids64, slots, experts, offsets, places, dev_err);
+  return cudaLaunchKernelEx(&cfg, plan_kernel<T, VEC, CTAS>, p, rows);
+}
+
+// The plan, and the tokens quantized into their rows: one kernel or two.
+cudaError_t launch_plan(const PlanParams& p, const RowsParams& rows, int32_t x_dtype, cudaStream_t st) {
+  const int64_t bytes = p.slots * rows.cols;
+  if (rows.rows <= kTogether && bytes <= kTogetherBytes && p.slots <= kPlanHeld * kPlanThreads) {
+    auto go = [&](auto t) {
+      using T = decltype(t);
+      return rows_aligned<T>(rows) ? launch_plan_one<T, true, 1>(p, rows, st) : launch_plan_one<T, false, 1>(p, rows, st);
+    };
+    return x_dtype == HEXMOE_F32 ? go(float{}) : x_dtype == HEXMOE_F16 ? go(__half{}) : go(__nv_bfloat16{});
+  }
+  const cudaError_t e = p.slots > 2 * kPlanThreads ? launch_plan_one<void, false, kPlanCtas>(p, rows, st)
+                                                   : launch_plan_one<void, false, 1>(p, rows, st);
+  return e == cudaSuccess ? launch_rows(rows, x_dtype, st) : e;
 }
 
 // ------------------------------------------------------------------- sum
@@ -625,12 +716,11 @@ int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t to
   int32_t* dev_err = device_error_word();
   if (!dev_err) return report_error(HEXMOE_E_CUDA, "device error word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = launch_plan(topk_ids, ids_dtype == HEXMOE_I64, slots, experts, s.offsets, s.places, dev_err, st);
-  if (e != cudaSuccess) return report_cuda_error(e, what);
+  const PlanParams plan = {topk_ids, ids_dtype == HEXMOE_I64, experts, slots, s.offsets, s.places, dev_err};
   RowsParams p{};
   p.x = x; p.ld_x = ld_x; p.rows = tokens; p.cols = hidden; p.q = s.xq; p.ld_q = hidden; p.scale = s.x_scale;
   p.places = s.places; p.topk = topk; p.weights = topk_weights; p.row_weight = s.weight;
-  e = launch_rows(p, x_dtype, st);
+  cudaError_t e = launch_plan(plan, p, x_dtype, st);
   if (e != cudaSuccess) return report_cuda_error(e, what);
   Int8Product d{};
   d.x = s.xq; d.ld_x = hidden; d.x_scale = s.x_scale;
