@@ -545,6 +545,17 @@ struct Walker {
   }
 };
 
+// Two products in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  unsigned long long p, q, r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a.x), "f"(a.y));
+  asm("mov.b64 %0, {%1, %2};" : "=l"(q) : "f"(b.x), "f"(b.y));
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(p), "l"(q));
+  float2 y;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(y.x), "=f"(y.y) : "l"(r));
+  return y;
+}
+
 // Writes 32 x 32 pieces of an accumulator: one writer warp's M rows by 32 columns.
 template <int MODE, bool RUNS, bool TWO>
 struct Writer {
@@ -579,12 +590,18 @@ struct Writer {
   // and tile row 8 i + 2 q + c.
   __device__ __forceinline__ void scale_fragments(uint32_t (&r)[32], float x) const {
     const int q = lane % 4;
-    float xs[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) xs[i] = __shfl_sync(0xffffffffu, x, i / 2 * 8 + 2 * q + i % 2);
+    for (int i = 0; i < 4; ++i) {
+      const float2 xs = make_float2(__shfl_sync(0xffffffffu, x, 8 * i + 2 * q), __shfl_sync(0xffffffffu, x, 8 * i + 2 * q + 1));
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      r[j] = __float_as_uint(static_cast<float>(static_cast<int32_t>(r[j])) * (ws[j / 16 * 2 + j / 2 % 2] * xs[j / 4 % 4 * 2 + j % 2]));
+      for (int h = 0; h < 4; ++h) {   // matrix rows 8 h + g
+        const int at = h / 2 * 16 + i * 4 + h % 2 * 2;
+        const float2 v = make_float2(static_cast<float>(static_cast<int32_t>(r[at])), static_cast<float>(static_cast<int32_t>(r[at + 1])));
+        const float2 y = mul2(v, mul2(make_float2(ws[h], ws[h]), xs));
+        r[at] = __float_as_uint(y.x);
+        r[at + 1] = __float_as_uint(y.y);
+      }
+    }
   }
   __device__ __forceinline__ void scale_columns(uint32_t (&r)[32], float x) const {
 #pragma unroll
