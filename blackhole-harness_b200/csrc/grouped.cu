@@ -545,6 +545,16 @@ struct Walker {
   }
 };
 
+__device__ __forceinline__ float fast_exp2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float fast_inverse(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 // Two products in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   unsigned long long p, q, r;
@@ -695,13 +705,19 @@ struct Writer {
     const int g = lane / 4, q = lane % 4;
     stage_free();
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {   // j = 8 h + 2 i + c
-      const int h = j / 8, line = j % 8 / 2 * 8 + 2 * q + j % 2, at = 16 * h + j % 8 / 2 * 4 + j % 2;
-      const float gate = __uint_as_float(r[at]), up = __uint_as_float(r[at + 2]);
-      const float act = __fdividef(gate, 1.f + __expf(-gate)) * up;   // 0 where the denominator passes 2^126
-      const int feature = 8 * h + g;
-      *reinterpret_cast<float*>(stage + line * 64 + ((feature / 4 ^ (line >> 1 & 3)) << 4) + feature % 4 * 4) = act;
-    }
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {   // features 8 h + g of rows 8 i + 2 q and the next
+        const int at = 16 * h + 4 * i, line = 8 * i + 2 * q;
+        const float2 gate = make_float2(__uint_as_float(r[at]), __uint_as_float(r[at + 1]));
+        const float2 up = make_float2(__uint_as_float(r[at + 2]), __uint_as_float(r[at + 3]));
+        // 1 / (1 + e^-gate): where e^-gate leaves f32's range, below gates of -88, it is 0
+        const float2 t = mul2(gate, make_float2(-1.44269504f, -1.44269504f));
+        const float2 act = mul2(mul2(gate, make_float2(fast_inverse(1.f + fast_exp2(t.x)), fast_inverse(1.f + fast_exp2(t.y)))), up);
+        float* to = reinterpret_cast<float*>(stage + line * 64 + (((8 * h + g) / 4 ^ (line >> 1 & 3)) << 4)) + g % 4;
+        to[0] = act.x;
+        to[16] = act.y;   // the next line's pieces lie in the same order
+      }
     if (rows == 32) {
       fence_proxy_async_smem();
       __syncwarp();
