@@ -363,7 +363,8 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 // 12 warps a CTA: 0 loads, 1 issues the products (the leader's), 2 and 3 zero tails
 // (weight gradient, the leader's), 4..11 write results.  Each walks the groups' offsets by
 // itself, so that no size is known on the host.  8-bit products run half as long as 16-bit ones and are not to wait for
-// the issue of their loads: warp 2 loads the rows, in one box a step, and warp 0 the matrix.
+// the issue of their loads: warp 2 loads the rows, in one box a step, and warp 0 the matrix; nor for the walk: warp 3 of
+// each CTA walks and hands the tiles to the others.
 //
 // Measured, bf16, 96 experts, 1536 x 2048, a call at a time and (in brackets) back to back, where the power cap
 // lowers the clock at the same number of cycles: 512 rows 91..93 us (93: HBM, 6.5 TB/s); 32768 rows 174..178 us
@@ -830,11 +831,48 @@ struct Writer {
   }
 };
 
+// A tile as one warp of a CTA hands it to the others (8-bit products).
+struct TileRecord {
+  int32_t e, m0, n0, width;
+  int32_t first, steps, tail, split;
+  int32_t row0, valid, more, end_row;   // more = 0: no tile; the groups' rows are row0 .. end_row - 1
+};
+constexpr int kRecords = 4;
+
 struct PairCtrl {
   uint64_t full[kMaxStages], empty[kMaxStages], tail[kMaxStages];
   uint64_t acc_full[2], acc_empty[2], done;
+  uint64_t rec_full[kRecords], rec_empty[kRecords];
   uint32_t tmem;
   int abort;
+  __align__(16) TileRecord rec[kRecords];
+};
+
+// The tiles in order, for a warp that does not look for them itself.  Looking takes some 500 cycles a tile, and every
+// role's own code for it: with short reductions (n 2816, k 160, 132 rows of 97 groups) that was 40 % of each role's time.
+struct TileReader {
+  PairCtrl* c;
+  uint32_t slot = 0, phase = 0;
+  int64_t lo = 0, carry = 0;
+  bool ended = false;
+  __device__ __forceinline__ bool next(const PairParams& p, int32_t&, int32_t, Tile& t) {
+    if (!warp_wait(&c->rec_full[slot], phase, &c->abort, p.dev_err)) return false;
+    const int4* r = reinterpret_cast<const int4*>(&c->rec[slot]);
+    const int4 a = r[0], b = r[1], d = r[2];
+    __syncwarp();
+    if (threadIdx.x % 32 == 0) mbar_arrive(&c->rec_empty[slot]);
+    if (++slot == kRecords) { slot = 0; phase ^= 1; }
+    t.e = a.x; t.m0 = a.y; t.n0 = a.z; t.width = a.w;
+    t.first = b.x; t.steps = b.y; t.tail = b.z; t.split = b.w;
+    t.row0 = d.x; t.valid = d.y;
+    t.parts = 1;
+    if (!d.z) {
+      ended = true;
+      lo = d.x;
+      carry = d.w;
+    }
+    return d.z;
+  }
 };
 
 template <int MODE, int SHAPE, bool RUNS>
@@ -870,6 +908,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     } else if (lane == kMaxStages + 2) {
       mbar_init(&c->done, 1);
       c->abort = 0;
+    } else if (is_int8(MODE) && lane < kMaxStages + 3 + kRecords) {
+      mbar_init(&c->rec_full[lane - kMaxStages - 3], 1);
+      mbar_init(&c->rec_empty[lane - kMaxStages - 3], 2 + kWriters + leader);   // two that load, the writers, the leader's products
     }
     fence_mbar_init();
   } else if (warp == 1) {
@@ -886,7 +927,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   pdl_launch_dependents();   // one wave: whoever waits for this grid may take its place on the SMs as they fall free
 
   const int32_t first = blockIdx.x / 2, stride = gridDim.x / 2;
-  Walker<MODE, SHAPE, RUNS> walk;
+  std::conditional_t<is_int8(MODE), TileReader, Walker<MODE, SHAPE, RUNS>> walk;
+  if constexpr (is_int8(MODE)) walk.c = c;
   Tile t;
   if (warp == 0 || (is_int8(MODE) && warp == 2)) {
     // ---------------------------------------------------------------- loads
@@ -967,7 +1009,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
         if (++st == kStages) { st = 0; phase ^= 1; }
       }
     }
-    if (walk.bad && blockIdx.x == 0) atomicOr(p.dev_err, kDevErrOffsets);
+    if constexpr (!is_int8(MODE))
+      if (walk.bad && blockIdx.x == 0) atomicOr(p.dev_err, kDevErrOffsets);
     if (ok && lane == 0) {   // the last steps are released to both CTAs before either leaves
       for (uint32_t back = 0; back < kStages && back < it; ++back) {
         const uint32_t j = it - 1 - back;
@@ -1035,6 +1078,25 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       pair_umma_commit(&c->done);
       mbar_wait(&c->done, 0, &ignore, p.dev_err);
     }
+  } else if (is_int8(MODE) && warp == 3) {
+    // ---------------------------------------------------------------- tiles
+    Walker<MODE, SHAPE, RUNS> look;
+    uint32_t slot = 0, phase = 1;
+    bool more = true;
+    for (int32_t tile = first; more;) {
+      more = look.next(p, tile, stride, t);
+      if (!warp_wait(&c->rec_empty[slot], phase, abort, p.dev_err)) break;
+      if (lane == 0) {
+        int4* r = reinterpret_cast<int4*>(&c->rec[slot]);
+        r[0] = make_int4(t.e, t.m0, t.n0, t.width);
+        r[1] = make_int4(t.first, t.steps, t.tail, t.split);
+        r[2] = make_int4(static_cast<int32_t>(more ? t.row0 : look.lo), t.valid, more, static_cast<int32_t>(look.carry));
+        mbar_arrive(&c->rec_full[slot]);
+      }
+      __syncwarp();
+      if (++slot == kRecords) { slot = 0; phase ^= 1; }
+    }
+    if (look.bad && blockIdx.x == 0) atomicOr(p.dev_err, kDevErrOffsets);
   } else if ((warp == 2 || warp == 3) && MODE >= kWgrad && leader) {
     // ---------------------------------------------------------------- tails
     // A warp for each CTA's shared memory, both in the leader: what they clear reaches the products by way of an
@@ -1133,6 +1195,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       }
     }
     if (p.tma_out && elect_one()) bulk_wait_all();
+    if constexpr (is_int8(MODE)) ok = ok && walk.ended;
     if (MODE < kWgrad && ok) {   // rows of no group
       const int64_t gap = walk.lo + (p.g.rows - walk.carry);
       for (int64_t j = blockIdx.x; j < gap * p.splits; j += gridDim.x) {
