@@ -47,7 +47,7 @@ struct RouteParams {
   void* dlogits;          // backward
   int64_t tokens, ld, ld_d;
   int32_t experts, topk, groups, topk_groups, group_top, renorm, ids64;
-  int32_t vec;            // rows (and biases) begin on 16 bytes and are whole pieces of 16 bytes
+  int32_t vec;            // rows (of logits, of their gradients, and biases) begin on 16 bytes and are whole pieces of 16 bytes
   int32_t group_lanes;    // lanes whose experts make a group, where they are whole lanes and a power of two; else 0
   float scale;
 };
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
 // once among the ids has the sum of its places; ids outside 0..E-1 have no part.
 template <typename T, int NI, bool SIGMOID>
 __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const RouteParams p) {
-  const int lane = threadIdx.x % 32, e0 = lane * NI;
+  const int lane = threadIdx.x % 32;
   const int64_t t = static_cast<int64_t>(blockIdx.x) * (blockDim.x / 32) + threadIdx.x / 32;
   pdl_wait();
   if (t >= p.tokens) return;
@@ -644,23 +644,22 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
   const bool dense = !SIGMOID && !p.renorm;
   float value;
   if (dense) {
-    float l[NI], s[NI];
-    load_row(p, row, -INFINITY, l);
-    const float largest = largest_of(l);
+    float s[NI];   // of experts lane, lane + 32 ...: no order is asked for here
+#pragma unroll
+    for (int i = 0; i < NI; ++i) s[i] = lane + 32 * i < p.experts ? widen(row[lane + 32 * i]) : -INFINITY;
+    const float largest = largest_of(s);
     float part = 0.f;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      s[i] = l[i] == -INFINITY ? 0.f : expf(l[i] - largest);
+      s[i] = s[i] == -INFINITY ? 0.f : expf(s[i] - largest);
       part += s[i];
     }
     const float sum = warp_sum(part), inv = sum == 0.f ? 0.f : 1.f / sum;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) s[i] *= inv;
     const float score = mine == -INFINITY ? 0.f : expf(mine - largest) * inv;
     const float dot = warp_sum(score * d);
 #pragma unroll
     for (int i = 0; i < NI; ++i)
-      if (e0 + i < p.experts) out[e0 + i] = narrow<T>(-s[i] * dot);
+      if (lane + 32 * i < p.experts) out[lane + 32 * i] = narrow<T>(-(s[i] * inv) * dot);
     float all = 0.f;   // of this expert's places
     for (int j = 0; j < p.topk; ++j) {
       const float dj = __shfl_sync(kAll, d, j);
@@ -668,7 +667,11 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
     }
     value = score * (all - dot);
   } else {
-    for (int e = lane; e < p.experts; e += 32) out[e] = narrow<T>(0.f);
+    if (p.vec) {
+      for (int e = lane; e < p.experts * static_cast<int>(sizeof(T)) / 16; e += 32) reinterpret_cast<uint4*>(out)[e] = make_uint4(0, 0, 0, 0);
+    } else {
+      for (int e = lane; e < p.experts; e += 32) out[e] = narrow<T>(0.f);
+    }
     if (p.renorm) {
       const float r = share_of<SIGMOID>(mine, SIGMOID ? 0.f : warp_max(mine), used);
       float away = 0.f;
@@ -695,7 +698,8 @@ cudaError_t launch_one(RouteParams p, bool backward, cudaStream_t st) {
   const int per = p.experts / p.groups, lanes = per / NI;
   p.group_lanes = per % NI == 0 && (lanes & (lanes - 1)) == 0 ? lanes : 0;
   p.vec = reinterpret_cast<uintptr_t>(p.logits) % 16 == 0 && p.ld * sizeof(T) % 16 == 0 && p.experts * sizeof(T) % 16 == 0 &&
-          reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && (!p.bias || p.experts % 4 == 0);
+          reinterpret_cast<uintptr_t>(p.bias) % 16 == 0 && (!p.bias || p.experts % 4 == 0) &&
+          reinterpret_cast<uintptr_t>(p.dlogits) % 16 == 0 && p.ld_d * sizeof(T) % 16 == 0;
   // a token a warp: blocks of one warp until every SM has some, and no more than their rows of keys leave room for
   const size_t row = !backward && p.topk_groups < p.groups && !p.group_lanes ? sizeof(uint32_t) * (p.experts + 32) : 0;
   int warps = p.tokens <= 148 * 8 ? 1 : kRouteThreads / 32;
