@@ -496,7 +496,7 @@ HEXMOE_API int hexmoe_quantize_rows(const void* x, int32_t x_dtype, int64_t ld_x
  * f32 [experts, n].  Sums are exact (k at most 131071); out F32, BF16 or F16 is
  * rounded once, or split reductions of few rows once for each of their parts in f32.  8-bit
  * rows begin and repeat on multiples of 16 bytes.  Rows of no group are set to
- * zero.  workspace (256-byte aligned): hexmoe_grouped_mm_int8_workspace_bytes,
+ * zero.  workspace (16-byte aligned): hexmoe_grouped_mm_int8_workspace_bytes,
  * needed where x is quantized here, elsewhere as for hexmoe_grouped_mm. */
 HEXMOE_API size_t hexmoe_grouped_mm_int8_workspace_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k,
                                                          int32_t x_dtype);

@@ -338,6 +338,35 @@ def test_int8_moe_views_streams_and_graphs():
 
 
 @pytest.mark.gpu
+def test_ordinary_calls_and_the_checked_ones_agree():
+    """What _call takes and what goes through Python's checks is the same call: an `out`, or ids that are not
+    contiguous, send it there."""
+    x, weights, ids, w13, w2 = layer_inputs(6, 128, 64, F16, 70, 3, 100)
+    xd, wd, idd = x.to(DEV), weights.to(DEV), ids.to(DEV)
+    want = int8.int8_moe(xd, wd, idd, *w13, *w2)
+    assert torch.equal(int8.int8_moe(xd, wd, idd.t().contiguous().t(), *w13, *w2), want)
+    assert torch.equal(int8.int8_moe(xd, wd.double(), idd.short(), *w13, *w2), want)
+    off = offsets_of([20, 0, 50, 0, 0, 0]).to(DEV)
+    out = torch.empty(70, 128, dtype=F16, device=DEV)
+    assert torch.equal(int8.grouped_mm_int8(xd, *w13, off), int8.grouped_mm_int8(xd, *w13, off, out=out))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,E,k,H,I", [(31, 5, 4, 1024, 32), (32, 5, 4, 1024, 32), (33, 5, 4, 1024, 32), (8, 5, 33, 64, 32), (1, 3, 200, 32, 16)])
+def test_few_tokens_quantized_with_the_plan(tokens, E, k, H, I):
+    """Up to 32 tokens whose slots' rows are up to 128 KB go through the plan's kernel, the next ones through two; more
+    slots a token than a warp has lanes."""
+    g = torch.Generator().manual_seed(110)
+    x, weights = normal((tokens, H), BF16, 111), torch.rand(tokens, k, generator=g) / k
+    ids = torch.randint(0, E, (tokens, k), generator=g)
+    w13 = int8.quantize_rows(normal((E, 2 * I, H), F32, 112, H ** -0.5).to(DEV))
+    w2 = int8.quantize_rows(normal((E, H, I), F32, 113, I ** -0.5).to(DEV))
+    for rows in (x.to(DEV), torch.cat([x, x], 1).to(DEV)[:, 1:H + 1]):     # and rows that do not begin on 16 bytes
+        got = int8.int8_moe(rows, weights.to(DEV), ids.to(DEV), *w13, *w2)
+        assert_layer(got, rows.cpu(), weights, ids, w13, w2)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("slots", [1, 2047, 2048, 2049, 9001, 40000])
 def test_plan_of_many_slots_and_experts(slots):
     """Routing to up to 2048 experts, from one slot to more than one block counts: every token finds its expert."""

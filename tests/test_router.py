@@ -264,6 +264,49 @@ def test_strides_streams_and_graphs():
 
 
 @pytest.mark.gpu
+def test_ordinary_calls_and_the_checked_ones_agree():
+    """What _call takes and what goes through Python's checks is the same call: a scale that is no float, or a strided
+    bias or gradient, send it there."""
+    logits, bias = normal((30, 40), F32, 44).to(DEV), normal((80,), F32, 45, 0.1).to(DEV)
+    want = router.route(logits, 4, bias=bias[::2].contiguous(), scale=2.0)
+    for got in (router.route(logits, 4, bias=bias[::2], scale=2.0), router.route(logits, 4, bias=bias[::2].contiguous(), scale=2)):
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    d = normal((4, 30), F32, 46).to(DEV)
+    assert torch.equal(router.route_backward(d.t(), logits, want[1]), router.route_backward(d.t().contiguous(), logits, want[1]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", [(2040, 8, 8, 3), (2048, 32, 2, 1), (1000, 20, 25, 11), (300, 16, 5, 2), (512, 32, 1, 1)], ids=str)
+def test_many_tokens_of_many_experts(case):
+    """Rows of keys that go through shared memory, selections longer than a lane's experts, and blocks of several tokens."""
+    E, k, groups, open_groups = case
+    logits, bias = normal((1500, E), BF16, 47), normal((E,), F32, 48, 0.1)
+    how = dict(scoring="softmax", bias=bias, groups=groups, topk_groups=open_groups)
+    some = torch.arange(0, 1500, 29)
+    want, gap = choice_of(logits[some], k, **how)
+    assert gap > 1e-14
+    weights, ids = router.route(logits.to(DEV), k, **{**how, "bias": bias.to(DEV)})
+    assert torch.equal(ids.cpu()[some].long(), want)
+    assert_weights(weights.cpu()[some], weights_of(logits[some], want), logits, 1.0)
+    assert all(len(set(row)) == k for row in ids.tolist())
+
+
+@pytest.mark.gpu
+def test_rows_of_equal_values():
+    """Every choice alike, or many: more candidates than lanes, in the order of their ids."""
+    for E, k in ((96, 8), (512, 32), (40, 20)):
+        logits = torch.zeros(5, E)
+        logits[1, ::3] = 1
+        logits[2] = torch.arange(E) // 40
+        logits[3] = torch.linspace(0, 1e-9, E)
+        for bias in (None, torch.zeros(E)):
+            for scoring in ("softmax", "sigmoid"):
+                want, _ = choice_of(logits, k, scoring, bias)
+                _, ids = router.route(logits.to(DEV), k, scoring=scoring, bias=None if bias is None else bias.to(DEV))
+                assert torch.equal(ids.cpu().long(), want)
+
+
+@pytest.mark.gpu
 def test_agrees_with_route_topk():
     from blackhole_b200.hex_moe import route_topk
     logits = normal((300, 96), F32, 50).to(DEV)
