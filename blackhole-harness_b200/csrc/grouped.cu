@@ -4,6 +4,7 @@
 #include <algorithm>
 #include <cstdarg>
 #include <cstdio>
+#include <initializer_list>
 #include <type_traits>
 
 #include <atomic>
@@ -30,14 +31,13 @@ int arg_error(const char* fmt, ...) {
 // and to no less than the one before, so that whatever the array holds the
 // groups are disjoint row ranges.  `bad` says that something was clamped.
 struct Groups {
-  const void* offsets;   // int32 or int64 [experts + 1]; null (8-bit products): one group of all rows
+  const void* offsets;   // int32 or int64 [experts + 1]; null (8-bit products): Int8Params::whole
   int32_t is64;
   int32_t experts;
   int64_t rows;
 };
 
 __device__ __forceinline__ int64_t raw_offset(const Groups& g, int e) {
-  if (!g.offsets) return e ? g.rows : 0;
   return g.is64 ? static_cast<const int64_t*>(g.offsets)[e] : static_cast<const int32_t*>(g.offsets)[e];
 }
 
@@ -380,7 +380,6 @@ constexpr int kWriters = 8;
 constexpr uint32_t kAccCols = 256;
 constexpr uint32_t kStoreBytes = 2048;                 // a writer's staging tile: 32 lines of 64 B
 constexpr uint32_t kRingBytes = 200 * 1024;            // 6 steps of A and B, 4 of A and two Bs, 5 narrow ones
-constexpr uint32_t kPairSmem = 1024 + kRingBytes + kWriters * kStoreBytes + 9 * 1024;
 constexpr int kBoxes = 4;                              // row boxes of 16, 32, 64, 128
 constexpr int kBoxes8 = 8;                             // 8-bit rows: of 16, 32, 48 .. 128
 
@@ -389,6 +388,9 @@ constexpr int kBoxes8 = 8;                             // 8-bit rows: of 16, 32,
 enum PairMode { kRowsK = 0, kRowsMN = 1, kInt8 = 2, kInt8Glu = 3, kWgrad = 4, kWgradT = 5 };
 constexpr bool is_int8(int mode) { return mode == kInt8 || mode == kInt8Glu; }
 constexpr bool k_major(int mode) { return mode == kRowsK || is_int8(mode); }   // the matrix as it lies is reduction-major
+
+// Two staging tiles a writer in 8-bit products, which leave that much of the ring.
+constexpr uint32_t pair_smem(int mode) { return 1024 + kRingBytes + kWriters * kStoreBytes + (is_int8(mode) ? 9 * 1024 : 1024); }
 
 // Shapes of a tile's N side and of the ring that fits it.
 //   kOne     up to 256 columns: 6 steps of 32 KB
@@ -409,16 +411,13 @@ constexpr int span_of(int shape) {                                      // most 
 
 struct PairParams {
   CUtensorMap a;             // W (3-D: reduction or features, ..., expert); weight gradient: dy, or x in kWgradT
-  CUtensorMap b[kBoxes8];    // the rows, by box height; weight gradient: [0] is the other of x and dy
+  CUtensorMap b[kBoxes];     // the rows, by box height; weight gradient: [0] is the other of x and dy
   CUtensorMap out;           // boxes of 32 rows x 64 B; f32 of kWgradT: 16 rows x 128 B
   Groups g;
   int32_t m_len;             // M side: output features; weight gradient: n, or k in kWgradT
   int32_t n_len;             // weight gradient: k, or n in kWgradT
   int32_t red;               // row products: reduction length (8-bit: in pairs)
   int32_t out_len;           // row products: columns of the result
-  int32_t stream;            // 8-bit products: the matrices pass through L2 without staying
-  const float* x_scale;      // [rows]
-  const float* w_scale;      // [experts, matrix rows]
   int32_t m_tiles, n_tiles, tile_n;   // n_tiles, tile_n: weight gradient
   int32_t splits;            // runs that the reduction of a tile is cut into, over several pairs
   int32_t run;               // RUNS: most steps that one accumulator sums
@@ -427,6 +426,25 @@ struct PairParams {
   int32_t f32, bf16, accumulate, tma_out;
   int32_t* dev_err;
 };
+
+// What 8-bit products take beside that (16-bit ones start sooner without it: one token on 96 experts 10.8 us, not 11.4).
+struct Int8Params : PairParams {
+  CUtensorMap rows[kBoxes8];   // in boxes of 16 (i + 1)
+  const float* x_scale;        // [rows]
+  const float* w_scale;        // [experts, matrix rows]
+  int32_t stream;              // the matrices pass through L2 without staying
+  int32_t whole[2];            // the offsets of one group of all rows
+};
+template <int MODE>
+using Params = std::conditional_t<is_int8(MODE), Int8Params, PairParams>;
+// (A test for null at each offset, instead, kept the loads apart: 0.7 us a kernel.)
+template <int MODE>
+__device__ __forceinline__ Groups groups_of(const Params<MODE>& p) {
+  Groups g = p.g;
+  if constexpr (is_int8(MODE))
+    if (!g.offsets) g.offsets = p.whole;
+  return g;
+}
 
 // One tile: expert, M offset, N offset (a row offset within the group in the row
 // products) and width, of `parts` accumulators side by side; row0 its first row,
@@ -454,7 +472,7 @@ struct Walker {
   int32_t left = 0, per = 0, end_tail = 0;   // of the tile's steps: to come, in a run, and its last one
 
   // The next run of a tile's reduction: all of it, or with RUNS pieces of at most p.run steps one after the other.
-  __device__ __forceinline__ bool next(const PairParams& p, int32_t& unit, int32_t stride, Tile& t) {
+  __device__ __forceinline__ bool next(const Params<MODE>& p, int32_t& unit, int32_t stride, Tile& t) {
     if (!RUNS || left == 0) {
       if (!find(p, unit, t)) return false;
       unit += stride;
@@ -476,13 +494,13 @@ struct Walker {
     return true;
   }
 
-  __device__ __forceinline__ bool find(const PairParams& p, int32_t unit, Tile& t) {
+  __device__ __forceinline__ bool find(const Params<MODE>& p, int32_t unit, Tile& t) {
     constexpr int32_t kSpan = span_of(SHAPE);
     const int32_t tile = p.splits > 1 ? unit / p.splits : unit;
     while (tile >= total) {
       if (base + 32 >= p.g.experts) return false;
       base += 32;
-      const GroupScan s = scan_groups(p.g, base, carry);
+      const GroupScan s = scan_groups(groups_of<MODE>(p), base, carry);
       bad |= s.bad;
       begin = s.begin;
       end = s.end;
@@ -570,7 +588,7 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
 // Writes 32 x 32 pieces of an accumulator: one writer warp's M rows by 32 columns.
 template <int MODE, bool RUNS, bool TWO>
 struct Writer {
-  const PairParams& p;
+  const Params<MODE>& p;
   uint8_t* stage;    // 32 lines of 64 B (their 16-byte pieces permuted as SWIZZLE_64B), or 16 plain ones of 128 B
   int lane;
   uint32_t flip = 0;   // TWO: the other staging tile's distance, kStoreBytes or minus that
@@ -586,7 +604,7 @@ struct Writer {
       const int32_t f = m / 2 + lane / 16 * 8 + lane % 8;
       row = f < p.out_len ? (lane % 16 < 8 ? 0 : p.out_len) + f : p.m_len;
     }
-    w_scale = row < p.m_len ? p.w_scale[static_cast<int64_t>(expert) * p.m_len + row] : 0.f;
+    if constexpr (is_int8(MODE)) w_scale = row < p.m_len ? p.w_scale[static_cast<int64_t>(expert) * p.m_len + row] : 0.f;
   }
   __device__ __forceinline__ void spread_w_scale() {   // once it is needed: what is loaded beside it does not wait
 #pragma unroll
@@ -877,7 +895,7 @@ struct TileReader {
 
 template <int MODE, int SHAPE, bool RUNS>
 __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
-    grouped_pair_kernel(const __grid_constant__ PairParams p) {
+    grouped_pair_kernel(const __grid_constant__ Params<MODE> p) {
   constexpr bool WIDE = SHAPE == kTwo;
   constexpr int kSubs = subs_of(SHAPE);
   constexpr uint32_t kStages = SHAPE == kOne ? 6 : SHAPE == kNarrow ? 5 : 4;
@@ -890,7 +908,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   // a second staging tile a writer where the ring leaves room: 8-bit tiles come twice as often
   constexpr bool kTwoStages = is_int8(MODE) && SHAPE != kNarrow;
   constexpr uint32_t kRing = kTwoStages ? kStages * kStageBytes : kRingBytes;
-  static_assert(1024 + kRing + kWriters * kStoreBytes * (kTwoStages ? 2 : 1) + sizeof(PairCtrl) <= kPairSmem);
+  static_assert(1024 + kRing + kWriters * kStoreBytes * (kTwoStages ? 2 : 1) + sizeof(PairCtrl) <= pair_smem(MODE));
   uint8_t* staging = ring + kRing;
   PairCtrl* c = reinterpret_cast<PairCtrl*>(staging + kWriters * kStoreBytes * (kTwoStages ? 2 : 1));
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -916,7 +934,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   } else if (warp == 1) {
     if (lane == 0) {
       prefetch_tmap(&p.a);
-      prefetch_tmap(&p.b[0]);
+      if constexpr (!is_int8(MODE)) prefetch_tmap(&p.b[0]);
     }
   } else if (warp == 2) pair_tmem_alloc(&c->tmem, 512);
   tc_fence_before();
@@ -979,7 +997,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             }
             if constexpr (is_int8(MODE)) {
               if (loads_b)
-                pair_load_2d(b, &p.b[halves[0] / 16 - 1], bar, 2 * r, static_cast<int32_t>(t.row0) + static_cast<int32_t>(rank) * halves[0]);
+                pair_load_2d(b, &p.rows[halves[0] / 16 - 1], bar, 2 * r, static_cast<int32_t>(t.row0) + static_cast<int32_t>(rank) * halves[0]);
             } else if constexpr (MODE >= kWgrad) {
               const int32_t y = static_cast<int32_t>(t.row0) + r, x = t.n0 + static_cast<int32_t>(rank) * halves[0];
               pair_load_2d(b, &p.b[0], bar, x, y);
@@ -1279,15 +1297,18 @@ int sm_count(int* sms) {
   if (dev < 0 || dev >= 64) return report_error(HEXMOE_E_DEVICE, "device ordinal out of range");
   int v = cached[dev].load(std::memory_order_acquire);
   if (!v) {   // first call on this device: the kernels' shared memory as well
-    for (const void* k : {PAIR_KERNELS(kRowsK, kOne), PAIR_KERNELS(kRowsK, kTwo), PAIR_KERNELS(kRowsK, kNarrow),
-                          PAIR_KERNELS(kRowsK, kMiddle), PAIR_KERNELS(kRowsMN, kOne), PAIR_KERNELS(kRowsMN, kTwo),
-                          PAIR_KERNELS(kRowsMN, kNarrow), PAIR_KERNELS(kRowsMN, kMiddle), PAIR_KERNELS(kWgrad, kOne),
-                          PAIR_KERNELS(kWgrad, kMiddle), PAIR_KERNELS(kWgradT, kOne), PAIR_KERNELS(kWgradT, kMiddle),
-                          INT8_KERNEL(kInt8, kNarrow), INT8_KERNEL(kInt8, kMiddle), INT8_KERNEL(kInt8, kOne),
-                          INT8_KERNEL(kInt8Glu, kNarrow), INT8_KERNEL(kInt8Glu, kMiddle), INT8_KERNEL(kInt8Glu, kOne)}) {
-      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem);
-      if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
-    }
+    const auto room = [&](std::initializer_list<const void*> kernels, int mode) {
+      for (const void* k : kernels)
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, pair_smem(mode));
+    };
+    room({PAIR_KERNELS(kRowsK, kOne), PAIR_KERNELS(kRowsK, kTwo), PAIR_KERNELS(kRowsK, kNarrow), PAIR_KERNELS(kRowsK, kMiddle),
+          PAIR_KERNELS(kRowsMN, kOne), PAIR_KERNELS(kRowsMN, kTwo), PAIR_KERNELS(kRowsMN, kNarrow), PAIR_KERNELS(kRowsMN, kMiddle),
+          PAIR_KERNELS(kWgrad, kOne), PAIR_KERNELS(kWgrad, kMiddle), PAIR_KERNELS(kWgradT, kOne), PAIR_KERNELS(kWgradT, kMiddle)},
+         kRowsK);
+    room({INT8_KERNEL(kInt8, kNarrow), INT8_KERNEL(kInt8, kMiddle), INT8_KERNEL(kInt8, kOne), INT8_KERNEL(kInt8Glu, kNarrow),
+          INT8_KERNEL(kInt8Glu, kMiddle), INT8_KERNEL(kInt8Glu, kOne)},
+         kInt8);
+    if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
     e = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
     if (e != cudaSuccess) return report_cuda_error(e, "cudaDeviceGetAttribute");
     cached[dev].store(v, std::memory_order_release);
@@ -1297,11 +1318,11 @@ int sm_count(int* sms) {
 }
 
 template <int MODE, int SHAPE>
-cudaError_t launch_pair(const PairParams& p, int64_t tiles, int sms, cudaStream_t st) {
+cudaError_t launch_pair(const Params<MODE>& p, int64_t tiles, int sms, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(sms / 2, tiles))));
   cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.dynamicSmemBytes = pair_smem(MODE);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -1505,12 +1526,13 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
   if (!dev_err) return report_error(HEXMOE_E_CUDA, "device error word unavailable");
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
-  PairParams q{};
-  q.g = {d.offsets, d.offsets64, d.experts, d.rows};
+  Int8Params q{};
+  q.g = {d.offsets, d.offsets ? d.offsets64 : 0, d.experts, d.rows};
   q.m_len = d.n;
   q.out_len = d.glu ? d.n / 2 : d.n;
   q.red = (d.k + 1) / 2;
   q.m_tiles = (d.n + 255) / 256;
+  q.whole[1] = static_cast<int32_t>(d.rows);
   q.x_scale = d.x_scale;
   q.w_scale = d.w_scale;
   q.splits = d.glu ? 1 : rows_splits(d.rows, d.experts, d.n, q.red);
@@ -1535,7 +1557,7 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
     return rc;
   const int64_t half = (std::min<int64_t>(d.rows, 256) + 31) / 32 * 16;
   for (int i = 0; i < kBoxes8 && 16 * (i + 1) <= half; ++i)
-    if (int rc = make_map(&q.b[i], d.x, kBytes, 2, d.k, d.rows, 1, d.ld_x, 0, 128, 16 * (i + 1))) return rc;
+    if (int rc = make_map(&q.rows[i], d.x, kBytes, 2, d.k, d.rows, 1, d.ld_x, 0, 128, 16 * (i + 1))) return rc;
   if (d.glu) {
     q.tma_out = 1;
     if (d.rows >= 32)
