@@ -304,6 +304,35 @@ def test_int8_moe_without_tokens_and_with_bad_ids():
 
 
 @pytest.mark.gpu
+def test_tokens_that_are_no_numbers_stay_among_themselves():
+    x, weights, ids, w13, w2 = layer_inputs(4, 64, 32, BF16, 40, 2, 75)
+    x[7, 3], x[20] = math.nan, math.inf
+    got = int8.int8_moe(x.to(DEV), weights.to(DEV), ids.to(DEV), *w13, *w2)
+    fine = torch.ones(40, dtype=torch.bool)
+    fine[[7, 20]] = False
+    assert got[7].isnan().all() and got[20].isnan().all()
+    assert_layer(got.cpu()[fine], x[fine], weights[fine], ids[fine], w13, w2)
+
+
+@pytest.mark.gpu
+def test_a_stack_that_streams_through_l2():
+    """Matrices of more than 64 MB read once, and the same product of a part of them that is not: bit for bit."""
+    E, n, k = 40, 1024, 2048
+    w = torch.randint(-127, 128, (E, n, k), dtype=torch.int8, device=DEV)
+    ws = torch.rand(E, n, device=DEV)
+    x = normal((80, k), BF16, 120).to(DEV)
+    off = torch.arange(0, 81, 2, dtype=torch.int32, device=DEV)
+    got = int8.grouped_mm_int8(x, w, ws, off)
+    for e in (0, 7, 39):
+        rows = slice(2 * e, 2 * e + 2)
+        one = int8.grouped_mm_int8(x[rows], w[e:e + 1], ws[e:e + 1], torch.tensor([0, 2], device=DEV), out_dtype=F32)
+        q, scale, _ = quantized(x[rows].cpu())
+        want, mass = product(q, scale, w[e:e + 1].cpu(), ws[e:e + 1].cpu(), torch.tensor([0, 2]), 2)
+        assert_product(one, want, mass, F32)
+        assert_product(got[rows], want, mass, BF16)
+
+
+@pytest.mark.gpu
 def test_int8_moe_views_streams_and_graphs():
     x, weights, ids, w13, w2 = layer_inputs(6, 128, 64, BF16, 90, 3, 80)
     xd, wd, idd = x.to(DEV), weights.to(DEV), ids.to(DEV)
