@@ -454,9 +454,11 @@ cudaError_t launch_plan_one(const PlanParams& p, const RowsParams& rows, cudaStr
 }
 
 // The plan, and the tokens quantized into their rows: one kernel or two.
+bool plan_quantizes(const PlanParams& p, const RowsParams& rows) {
+  return rows.rows <= kTogether && p.slots * rows.cols <= kTogetherBytes && p.slots <= kPlanHeld * kPlanThreads;
+}
 cudaError_t launch_plan(const PlanParams& p, const RowsParams& rows, int32_t x_dtype, cudaStream_t st) {
-  const int64_t bytes = p.slots * rows.cols;
-  if (rows.rows <= kTogether && bytes <= kTogetherBytes && p.slots <= kPlanHeld * kPlanThreads) {
+  if (plan_quantizes(p, rows)) {
     auto go = [&](auto t) {
       using T = decltype(t);
       return rows_aligned<T>(rows) ? launch_plan_one<T, true, 1>(p, rows, st) : launch_plan_one<T, false, 1>(p, rows, st);
@@ -671,6 +673,7 @@ int hexmoe_grouped_mm_int8(const void* x, int32_t x_dtype, int64_t ld_x, const f
     const cudaError_t e = launch_rows(p, x_dtype, st);
     if (e != cudaSuccess) return report_cuda_error(e, what);
     d.x = s.q; d.ld_x = p.ld_q; d.x_scale = s.scale;
+    d.early = 1;
   }
   d.w = w; d.ld_w = ld_w; d.stride_w = stride_w; d.w_scale = w_scale;
   d.rows = rows; d.experts = experts; d.n = n; d.k = k;
@@ -727,6 +730,7 @@ int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t to
   d.rows = slots; d.experts = experts; d.n = 2 * inter; d.k = hidden;
   d.offsets = s.offsets;
   d.out = s.act; d.ld_out = inter; d.out_dtype = HEXMOE_F32; d.glu = 1;
+  d.early = !plan_quantizes(plan, p);   // else the kernel before makes the offsets too
   if (int rc = run_int8_product(what, d, st)) return rc;
   p = RowsParams{};
   p.x = s.act; p.ld_x = inter; p.rows = slots; p.cols = inter; p.q = s.actq; p.ld_q = inter; p.scale = s.act_scale;
@@ -740,6 +744,7 @@ int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t to
   d.rows = slots; d.experts = experts; d.n = hidden; d.k = inter;
   d.offsets = s.offsets;
   d.out = s.y; d.ld_out = hidden; d.out_dtype = y_dtype;
+  d.early = 1;
   d.workspace = s.partial; d.workspace_bytes = s.partial_bytes;
   if (int rc = run_int8_product(what, d, st)) return rc;
   const SumParams sum = {s.y, s.places, out, tokens, topk, hidden};

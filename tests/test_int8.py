@@ -333,6 +333,52 @@ def test_a_stack_that_streams_through_l2():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows,E,n,k", [(3, 5, 96, 160), (300, 40, 320, 1104), (2500, 7, 512, 256)])
+def test_operands_written_just_before(rows, E, n, k):
+    """Rows, matrices, scales and offsets rewritten on the stream before each product, by calls not waited for."""
+    g = torch.Generator().manual_seed(rows)
+    sets = []
+    for i in range(4):
+        cuts = torch.randint(0, rows + 1, (E - 1,), generator=g).sort().values
+        off = torch.cat([torch.zeros(1, dtype=torch.int64), cuts, torch.tensor([rows])]).int()
+        sets.append((normal((rows, k), BF16, 200 + i), torch.randint(-127, 128, (E, n, k), generator=g).to(torch.int8),
+                     torch.rand(E, n, generator=g), off))
+    sets = [tuple(t.to(DEV) for t in s) for s in sets]
+    alone = []
+    for s in sets:
+        alone.append(int8.grouped_mm_int8(*(t.clone() for t in s)))
+        torch.cuda.synchronize()
+    q, scale, _ = quantized(sets[0][0].cpu())
+    want, mass = product(q, scale, sets[0][1].cpu(), sets[0][2].cpu(), sets[0][3].long().cpu(), rows)
+    assert_product(alone[0], want, mass, BF16)
+    held = [torch.empty_like(t) for t in sets[0]]
+    order = [i % 4 for i in range(0, 60, 3)] + [0, 0, 2, 1, 3, 1]
+    got = []
+    for i in order:
+        for h, t in zip(held, sets[i]):
+            h.copy_(t)
+        got.append(int8.grouped_mm_int8(*held))
+    for i, y in zip(order, got):
+        assert torch.equal(y, alone[i])
+
+
+@pytest.mark.gpu
+def test_int8_moe_written_just_before():
+    args = [layer_inputs(6, 128, 64, BF16, 64, 3, seed) for seed in (90, 95)]
+    a, b = ([x.to(DEV), w.to(DEV), ids.to(DEV), *(t.to(DEV) for t in (*w13, *w2))] for x, w, ids, w13, w2 in args)
+    alone = [int8.int8_moe(*(t.clone() for t in s)) for s in (a, b)]
+    torch.cuda.synchronize()
+    held = [torch.empty_like(t) for t in a]
+    got = []
+    for i in (0, 1) * 10:
+        for h, t in zip(held, (a, b)[i]):
+            h.copy_(t)
+        got.append(int8.int8_moe(*held))
+    for i, y in enumerate(got):
+        assert torch.equal(y, alone[i % 2])
+
+
+@pytest.mark.gpu
 def test_int8_moe_views_streams_and_graphs():
     x, weights, ids, w13, w2 = layer_inputs(6, 128, 64, BF16, 90, 3, 80)
     xd, wd, idd = x.to(DEV), weights.to(DEV), ids.to(DEV)
