@@ -90,14 +90,15 @@ template <typename T, bool VEC>
 struct Piece {
   static constexpr int kValues = VEC ? 16 / sizeof(T) : 1, kWords = VEC ? 4 : 1;
   uint32_t w[kWords];
+  // Past L1: it is read once, or before the wait.
   __device__ __forceinline__ void load(const T* row, int i) {
     if constexpr (VEC) {
-      const uint4 v = reinterpret_cast<const uint4*>(row)[i];
+      const uint4 v = __ldcg(reinterpret_cast<const uint4*>(row) + i);
       w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
     } else if constexpr (sizeof(T) == 4) {
-      w[0] = reinterpret_cast<const uint32_t*>(row)[i];
+      w[0] = __ldcg(reinterpret_cast<const uint32_t*>(row) + i);
     } else {
-      w[0] = reinterpret_cast<const uint16_t*>(row)[i];
+      w[0] = __ldcg(reinterpret_cast<const uint16_t*>(row) + i);
     }
   }
   // The largest magnitude so far: f32 bits, or two of 16 bits.
@@ -165,11 +166,22 @@ struct RowScale {
   }
 };
 
-// One row, by the TPR threads of it (lane: which); PLACES: into the rows of its slots.  Every thread of the block calls it
-// where TPR > 32; live: whether there is a row.  The pieces are turned into bytes in registers and stored from there: what is
-// unrolled eight times stays short, for a kernel of a few microseconds waits for its instructions more than for anything else.
+// A row to TPR threads.  PLACES: into the rows of its slots, which the kernel before makes; it lets this one start when
+// everything before it is done, so that the row may be read and turned into bytes before the wait (the layer of 1 token on 96
+// experts: 24.0 us, 24.9 when it waits first, 26.9 when few tokens are quantized by that kernel itself).  The pieces are
+// turned into bytes in registers and stored from there: what is unrolled eight times stays short, for a kernel of a few
+// microseconds waits for its instructions more than for anything else.
 template <typename T, bool VEC, int TPR, bool PLACES>
-__device__ __forceinline__ void quantize_row(const RowsParams& p, int64_t row, bool live, int lane, uint32_t* part) {
+__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsParams p) {
+  constexpr int kRows = kRowThreads / TPR;
+  __shared__ uint32_t part[kRowThreads / 32];
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
+  const int lane = threadIdx.x % TPR;
+  if constexpr (!PLACES) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
+  const bool live = row < p.rows && (!p.count || row < *p.count);
   using P = Piece<T, VEC>;
   constexpr int V = P::kValues, kWords = V > 4 ? V / 4 : 1;
   const T* x = static_cast<const T*>(p.x) + row * p.ld_x;
@@ -199,7 +211,6 @@ __device__ __forceinline__ void quantize_row(const RowsParams& p, int64_t row, b
 #pragma unroll
     for (int i = 0; i < TPR / 32; ++i) bits = max(bits, part[slot * (TPR / 32) + i]);
   }
-  if (!live) return;
   const RowScale to(bits);
   const bool finite = to.finite();
   auto bytes = [&](const P& v, uint32_t (&w)[kWords]) {
@@ -228,8 +239,13 @@ __device__ __forceinline__ void quantize_row(const RowsParams& p, int64_t row, b
   uint32_t w[kPieces][kWords];
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
-    if (lane + i * TPR < n) bytes(held[i], w[i]);
+    if (live && lane + i * TPR < n) bytes(held[i], w[i]);
   }
+  if constexpr (PLACES) {
+    pdl_wait();
+    pdl_launch_dependents();
+  }
+  if (!live) return;
   const int copies = PLACES ? p.topk : 1;
 #pragma unroll 1
   for (int j = 0; j < copies; ++j) {
@@ -257,17 +273,6 @@ __device__ __forceinline__ void quantize_row(const RowsParams& p, int64_t row, b
       if (!PLACES || at >= 0) put(at, c, w[0]);
     }
   }
-}
-
-template <typename T, bool VEC, int TPR, bool PLACES>
-__global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsParams p) {
-  constexpr int kRows = kRowThreads / TPR;
-  __shared__ uint32_t part[kRowThreads / 32];
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
-  pdl_wait();
-  pdl_launch_dependents();
-  const bool live = row < p.rows && (!p.count || row < *p.count);
-  quantize_row<T, VEC, TPR, PLACES>(p, row, live, threadIdx.x % TPR, part);
 }
 
 // The threads of a row: as few as hold it in registers.
@@ -315,14 +320,10 @@ cudaError_t launch_rows(const RowsParams& p, int32_t dtype, cudaStream_t st) {
 // rows come in whatever order the counting finds: no value of the layer depends on it (a row's sums are whole
 // numbers and its own).  One cluster: each CTA counts its slots in shared memory, the counts of the CTAs before it come
 // over distributed shared memory, and nothing has to be cleared or handed on between kernels.
-// Few tokens are quantized by the same kernel once their rows are known, a warp a token: one launch less (2 tokens of
-// 416, the layer: 18.9 us against 22.3), as long as one SM can write the rows (22 tokens of 2816, top 6, by eight: 43 us
-// against 40).
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanCtas = 8;
 constexpr int kPlanHeld = 4;        // slots a thread keeps in registers
 constexpr int kMaxExperts = 2048;
-constexpr int64_t kTogether = 32, kTogetherBytes = 1 << 17;   // tokens, and bytes of all slots' rows
 
 struct PlanParams {
   const void* ids;
@@ -345,9 +346,8 @@ __device__ __forceinline__ void plan_experts(const PlanParams& p, int64_t s, int
   for (int i = 0; i < kPlanHeld; ++i) e[i] = v[i] >= 0 && v[i] < p.experts ? static_cast<int32_t>(v[i]) : -1;
 }
 
-// T: the tokens' type where they are quantized here (by one CTA), else void.
-template <typename T, bool VEC, int CTAS>
-__global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanParams p, const RowsParams rows) {
+template <int CTAS>
+__global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanParams p) {
   __shared__ int32_t hist[kMaxExperts], first[kMaxExperts], sums[32];
   cg::cluster_group cluster = cg::this_cluster();
   const int rank = CTAS > 1 ? static_cast<int>(cluster.block_rank()) : 0;
@@ -436,38 +436,20 @@ __global__ void __launch_bounds__(kPlanThreads, 1) plan_kernel(const PlanParams 
     for (int i = 0; i < kPlanHeld; ++i)
       if (e[i] >= 0) p.places[s + i * kPlanThreads] += first[e[i]];
   }
-  if constexpr (!std::is_void_v<T>) {
-    sync();   // every token's places
-    if (warp < rows.rows) quantize_row<T, VEC, 32, true>(rows, warp, true, lane, nullptr);
-  }
 }
 
-template <typename T, bool VEC, int CTAS>
-cudaError_t launch_plan_one(const PlanParams& p, const RowsParams& rows, cudaStream_t st) {
+template <int CTAS>
+cudaError_t launch_plan_of(const PlanParams& p, cudaStream_t st) {
   cudaLaunchAttribute attr[2];
   cudaLaunchConfig_t cfg = launch_config(dim3(CTAS), kPlanThreads, 0, st, attr);
   attr[1].id = cudaLaunchAttributeClusterDimension;
   attr[1].val.clusterDim.x = CTAS;
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.numAttrs = 2;
-  return cudaLaunchKernelEx(&cfg, plan_kernel<T, VEC, CTAS>, p, rows);
+  return cudaLaunchKernelEx(&cfg, plan_kernel<CTAS>, p);
 }
-
-// The plan, and the tokens quantized into their rows: one kernel or two.
-bool plan_quantizes(const PlanParams& p, const RowsParams& rows) {
-  return rows.rows <= kTogether && p.slots * rows.cols <= kTogetherBytes && p.slots <= kPlanHeld * kPlanThreads;
-}
-cudaError_t launch_plan(const PlanParams& p, const RowsParams& rows, int32_t x_dtype, cudaStream_t st) {
-  if (plan_quantizes(p, rows)) {
-    auto go = [&](auto t) {
-      using T = decltype(t);
-      return rows_aligned<T>(rows) ? launch_plan_one<T, true, 1>(p, rows, st) : launch_plan_one<T, false, 1>(p, rows, st);
-    };
-    return x_dtype == HEXMOE_F32 ? go(float{}) : x_dtype == HEXMOE_F16 ? go(__half{}) : go(__nv_bfloat16{});
-  }
-  const cudaError_t e = p.slots > 2 * kPlanThreads ? launch_plan_one<void, false, kPlanCtas>(p, rows, st)
-                                                   : launch_plan_one<void, false, 1>(p, rows, st);
-  return e == cudaSuccess ? launch_rows(rows, x_dtype, st) : e;
+cudaError_t launch_plan(const PlanParams& p, cudaStream_t st) {
+  return p.slots > 2 * kPlanThreads ? launch_plan_of<kPlanCtas>(p, st) : launch_plan_of<1>(p, st);
 }
 
 // ------------------------------------------------------------------- sum
@@ -722,7 +704,8 @@ int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t to
   RowsParams p{};
   p.x = x; p.ld_x = ld_x; p.rows = tokens; p.cols = hidden; p.q = s.xq; p.ld_q = hidden; p.scale = s.x_scale;
   p.places = s.places; p.topk = topk; p.weights = topk_weights; p.row_weight = s.weight;
-  cudaError_t e = launch_plan(plan, p, x_dtype, st);
+  cudaError_t e = launch_plan(plan, st);
+  if (e == cudaSuccess) e = launch_rows(p, x_dtype, st);
   if (e != cudaSuccess) return report_cuda_error(e, what);
   Int8Product d{};
   d.x = s.xq; d.ld_x = hidden; d.x_scale = s.x_scale;
@@ -730,7 +713,7 @@ int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t to
   d.rows = slots; d.experts = experts; d.n = 2 * inter; d.k = hidden;
   d.offsets = s.offsets;
   d.out = s.act; d.ld_out = inter; d.out_dtype = HEXMOE_F32; d.glu = 1;
-  d.early = !plan_quantizes(plan, p);   // else the kernel before makes the offsets too
+  d.early = 1;
   if (int rc = run_int8_product(what, d, st)) return rc;
   p = RowsParams{};
   p.x = s.act; p.ld_x = inter; p.rows = slots; p.cols = inter; p.q = s.actq; p.ld_q = inter; p.scale = s.act_scale;
