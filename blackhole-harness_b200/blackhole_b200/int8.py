@@ -25,6 +25,8 @@ from blackhole_b200.experts import _INDEX, _call, _check_groups, _recorded, _row
 from blackhole_b200.hex_moe import _DT, _ptr
 
 MAX_K = 131071   # longest sum of products of 8-bit integers that int32 holds
+MAX_SIZE = 1 << 24   # of every other dimension of a stack
+MAX_ROW = 1 << 30
 
 _quantize_rows, _grouped_mm_int8, _int8_forward = (_lib.lib.hexmoe_quantize_rows, _lib.lib.hexmoe_grouped_mm_int8,
                                                    _lib.lib.hexmoe_int8_forward)
@@ -47,6 +49,8 @@ def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _check_stack(what: str, w: torch.Tensor, scale: torch.Tensor, dev: torch.device, name: str) -> None:
+    if w.dim() and (w.shape[-1] > MAX_K or max(w.shape) > MAX_SIZE):
+        raise ValueError(f"{what}: {name} {tuple(w.shape)}: rows have at most {MAX_K} values, every other size is at most {MAX_SIZE}")
     if w.dtype != torch.int8 or w.device != dev:
         raise ValueError(f"{what}: {name} must be int8 on {dev}, got {w.dtype} on {w.device}")
     if scale.dtype != torch.float32 or scale.shape != w.shape[:-1] or scale.device != dev:
@@ -63,7 +67,7 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         raise ValueError("quantize_rows runs on CUDA only")
     if x.dtype not in _DT:
         raise ValueError(f"quantize_rows: unsupported dtype {x.dtype}")
-    if x.dim() == 0 or x.shape[-1] == 0:
+    if x.dim() == 0 or not 0 < x.shape[-1] <= MAX_ROW:
         raise ValueError(f"quantize_rows: x must have rows of values, got {tuple(x.shape)}")
     shape, K = x.shape, x.shape[-1]
     rows, ld = _rows2d(x.detach().reshape(-1, K), "x")
@@ -162,6 +166,8 @@ def int8_moe(x: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor
         raise ValueError(f"x must be [T, {H}], got {tuple(x.shape)}")
     if topk_ids.dim() != 2 or topk_ids.shape[0] != x.shape[0] or topk_weights.shape != topk_ids.shape:
         raise ValueError("topk_weights / topk_ids / x disagree on T or k")
+    if topk_ids.shape[1] > 1024:
+        raise ValueError(f"int8_moe: topk {topk_ids.shape[1]}, at most 1024")
     if topk_weights.device != dev or topk_ids.device != dev:
         raise ValueError(f"int8_moe: x is on {dev}, topk_weights on {topk_weights.device}, topk_ids on {topk_ids.device}")
     T, k = topk_ids.shape

@@ -20,6 +20,7 @@ from blackhole_b200.experts import _INDEX, _call, _recorded, _rows2d, _run
 from blackhole_b200.hex_moe import _DT, _ptr
 
 SCORING = {"softmax": _lib.SOFTMAX, "sigmoid": _lib.SIGMOID}
+MAX_EXPERTS, MAX_TOPK = 2048, 32
 
 _route, _route_backward = _lib.lib.hexmoe_route, _lib.lib.hexmoe_route_backward
 
@@ -32,6 +33,8 @@ def _check(what: str, logits: torch.Tensor, scoring: str) -> tuple[torch.Tensor,
         raise ValueError(f"{what}: unsupported logits dtype {logits.dtype}")
     if scoring not in SCORING:
         raise ValueError(f"{what}: scoring must be one of {sorted(SCORING)}, got {scoring!r}")
+    if logits.dim() == 2 and logits.shape[1] > MAX_EXPERTS:
+        raise ValueError(f"{what}: {logits.shape[1]} experts, at most {MAX_EXPERTS}")
     return *_rows2d(logits, "logits"), SCORING[scoring]
 
 
@@ -77,14 +80,18 @@ def route(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bias: torch
     logits, ld, code = _check("route", logits, scoring)
     T, E = logits.shape
     dev = logits.device
+    open_groups = groups if topk_groups is None else topk_groups
+    for name, value in (("k", k), ("groups", groups), ("topk_groups", open_groups), ("group_top", group_top)):
+        if not 1 <= value <= MAX_TOPK:
+            raise ValueError(f"route: {name} {value} outside 1..{MAX_TOPK}")
     if bias is not None:
         if bias.dtype != torch.float32 or bias.shape != (E,) or bias.device != dev:
             raise ValueError(f"route: bias must be float32 [{E}] on {dev}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}")
         bias = bias.detach().contiguous()
-    weights = torch.empty(T, max(k, 0), dtype=torch.float32, device=dev)
-    ids = torch.empty(T, max(k, 0), dtype=torch.int32, device=dev)
+    weights = torch.empty(T, k, dtype=torch.float32, device=dev)
+    ids = torch.empty(T, k, dtype=torch.int32, device=dev)
     _run(_route, dev, logits.data_ptr(), _DT[logits.dtype], ld, T, E, k, code, _ptr(bias), groups,
-         groups if topk_groups is None else topk_groups, group_top, renormalize, scale, weights.data_ptr(), ids.data_ptr())
+         open_groups, group_top, renormalize, scale, weights.data_ptr(), ids.data_ptr())
     return weights, ids
 
 
@@ -99,8 +106,8 @@ def route_backward(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tens
     logits, ld, code = _check("route_backward", logits, scoring)
     T, E = logits.shape
     dev = logits.device
-    if ids.dtype not in _INDEX or ids.dim() != 2 or ids.shape[0] != T or ids.device != dev:
-        raise ValueError(f"route_backward: ids must be int32 or int64 [{T}, k] on {dev}, got {ids.dtype} {tuple(ids.shape)} "
+    if ids.dtype not in _INDEX or ids.dim() != 2 or ids.shape[0] != T or ids.shape[1] > MAX_TOPK or ids.device != dev:
+        raise ValueError(f"route_backward: ids must be int32 or int64 [{T}, k <= {MAX_TOPK}] on {dev}, got {ids.dtype} {tuple(ids.shape)} "
                          f"on {ids.device}")
     if dweights.dtype != torch.float32 or dweights.shape != ids.shape or dweights.device != dev:
         raise ValueError(f"route_backward: dweights must be float32 {list(ids.shape)} on {dev}, got {dweights.dtype} "

@@ -286,7 +286,7 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     else if (!integer(a[5], &open_groups)) Py_RETURN_NONE;
     const int64_t T = l->size(0), E = l->size(1);
     const at::Tensor* bias = a[3] == Py_None ? nullptr : tensor(a[3]);
-    if ((a[3] != Py_None && !scales(bias, {E})) || E > INT32_MAX || k < 1) Py_RETURN_NONE;
+    if ((a[3] != Py_None && !scales(bias, {E})) || E > INT32_MAX || k < 1 || k > 32) Py_RETURN_NONE;
     const auto f32 = l->options().dtype(at::kFloat);
     at::Tensor weights = at::empty({T, k}, f32), ids = at::empty({T, k}, f32.dtype(at::kInt));
     const int rc = hexmoe_route(l->data_ptr(), code_of(l->scalar_type()), l->stride(0), T, static_cast<int32_t>(E), k, scoring,
@@ -335,7 +335,7 @@ PyObject* grouped_mm_int8(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const at::Tensor *x = n_args == 4 ? tensor(a[0]) : nullptr, *w = x ? tensor(a[1]) : nullptr, *s = w ? tensor(a[2]) : nullptr,
                      *off = s ? tensor(a[3]) : nullptr;
     if (!off || !here(*x) || code_of(x->scalar_type()) < 0 || !matrix(*x) || recorded(*x) || !int8_stack(*w) ||
-        !scales(s, w->sizes().slice(0, 2)) || recorded(*s) || x->size(1) != w->size(2))
+        !scales(s, w->sizes().slice(0, 2)) || recorded(*s) || x->size(1) != w->size(2) || w->size(2) > 131071)
       Py_RETURN_NONE;
     const int64_t E = w->size(0), N = w->size(1), K = w->size(2), R = x->size(0);
     const int code = code_of(x->scalar_type()), index = offsets_code(*off, E);

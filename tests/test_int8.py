@@ -543,3 +543,26 @@ def test_refusals_on_the_device():
             call()
     with torch.no_grad():
         mm(x, w, s, off)
+
+
+@pytest.mark.gpu
+def test_sizes_past_32_bits_are_refused():
+    """Views without the memory: none of these sizes may be cut to its low bits, or allocated first."""
+    wide = 2 ** 32 + 16
+    one = torch.zeros(1, 1, dtype=BF16, device=DEV)
+    w, s, off = torch.zeros(1, 1, 1, dtype=torch.int8, device=DEV), torch.zeros(1, 1, device=DEV), offsets_of([1]).to(DEV)
+    tw, ids = torch.zeros(1, 1, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    x, w13, s13, w2, s2 = one.expand(1, 16), w.expand(1, 32, 16), s.expand(1, 32), w.expand(1, 16, 16), s.expand(1, 16)
+    bad = [lambda: int8.quantize_rows(one.expand(1, wide)), lambda: int8.grouped_mm_int8(one.expand(1, wide), w.expand(1, 1, wide), s, off),
+           lambda: int8.grouped_mm_int8(one.expand(1, 131072), w.expand(1, 1, 131072), s, off),
+           lambda: int8.grouped_mm_int8(x, w.expand(1, wide, 16), s.expand(1, wide), off),
+           lambda: int8.int8_moe(x, tw.expand(1, wide), ids.expand(1, wide), w13, s13, w2, s2),
+           lambda: int8.int8_moe(x, tw, ids, w.expand(1, 2 * wide, 16), s.expand(1, 2 * wide), w.expand(1, 16, wide), s2),
+           lambda: int8.int8_moe(one.expand(1, wide), tw, ids, w.expand(1, 32, wide), s13, w.expand(1, wide, 16), s.expand(1, wide))]
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"case {i} was taken")
+    assert torch.cuda.max_memory_allocated() <= before + (1 << 20)

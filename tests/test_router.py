@@ -377,3 +377,22 @@ def test_refusals_on_the_device():
         with pytest.raises(ValueError):
             call()
             pytest.fail(f"case {i} was taken")
+
+
+@pytest.mark.gpu
+def test_sizes_past_32_bits_are_refused():
+    """Views without the memory: none of these sizes may be cut to its low bits, or allocated first."""
+    x, ids = torch.zeros(4, 8, device=DEV), torch.zeros(4, 2, dtype=torch.int32, device=DEV)
+    wide = 2 ** 32 + 8
+    bad = [lambda: router.route(x, 2 ** 32 + 2), lambda: router.route(x, 33), lambda: router.route(x, 1 << 30),
+           lambda: router.route(x, 2, groups=2 ** 32 + 1), lambda: router.route(x, 2, groups=2, topk_groups=2 ** 32 + 1),
+           lambda: router.route(x, 2, group_top=2 ** 32 + 2), lambda: router.route(x[:1, :1].expand(1, wide), 2),
+           lambda: router.route_backward(x[:1, :2], x[:1, :1].expand(1, wide), ids[:1]),
+           lambda: router.route_backward(x[:1, :1].expand(1, wide), x[:1], ids[:1, :1].expand(1, wide))]
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            pytest.fail(f"case {i} was taken")
+    assert torch.cuda.max_memory_allocated() <= before + (1 << 20)
