@@ -629,7 +629,8 @@ struct Writer {
     if constexpr (is_int8(MODE)) return col + lane < cols ? p.x_scale[n0 + col + lane] : 0.f;
     return 0.f;
   }
-  // int32 sums as scaled f32 values, in place.  Fragments: register 16 h + 4 i + 2 b + c is matrix row 16 h + 8 b + g
+  // int32 sums as scaled f32 values, in place; the matrix's scale first, for the product of two small scales would leave the
+  // normal numbers before the result does.  Fragments: register 16 h + 4 i + 2 b + c is matrix row 16 h + 8 b + g
   // and tile row 8 i + 2 q + c.
   __device__ __forceinline__ void scale_fragments(uint32_t (&r)[32], float x) const {
     const int q = lane % 4;
@@ -640,7 +641,7 @@ struct Writer {
       for (int h = 0; h < 4; ++h) {   // matrix rows 8 h + g
         const int at = h / 2 * 16 + i * 4 + h % 2 * 2;
         const float2 v = make_float2(static_cast<float>(static_cast<int32_t>(r[at])), static_cast<float>(static_cast<int32_t>(r[at + 1])));
-        const float2 y = mul2(v, mul2(make_float2(ws[h], ws[h]), xs));
+        const float2 y = mul2(mul2(v, make_float2(ws[h], ws[h])), xs);
         r[at] = __float_as_uint(y.x);
         r[at + 1] = __float_as_uint(y.y);
       }
@@ -649,7 +650,7 @@ struct Writer {
   __device__ __forceinline__ void scale_columns(uint32_t (&r)[32], float x) const {
 #pragma unroll
     for (int j = 0; j < 32; ++j)
-      r[j] = __float_as_uint(static_cast<float>(static_cast<int32_t>(r[j])) * (w_scale * __shfl_sync(0xffffffffu, x, j)));
+      r[j] = __float_as_uint(static_cast<float>(static_cast<int32_t>(r[j])) * w_scale * __shfl_sync(0xffffffffu, x, j));
   }
 
   // An f32 result, or its addition without waiting for what is there.  Each value has one writer, whose additions

@@ -315,6 +315,19 @@ def test_tokens_that_are_no_numbers_stay_among_themselves():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_scales_whose_product_is_no_normal_number(dtype):
+    x = (normal((40, 512), F32, 130) * 1e-35).to(dtype)
+    w, ws = int8_stack((2, 96, 512), 131)
+    ws, off = torch.full_like(ws, 1e-5), offsets_of([17, 23])
+    q, scale, _ = quantized(x)
+    assert float((scale.max() * ws.max())) < 2.0 ** -130
+    want, mass = product(q, scale, w, ws, off, 40)
+    got = int8.grouped_mm_int8(x.to(DEV), w.to(DEV), ws.to(DEV), off.to(DEV), out_dtype=dtype)
+    assert_product(got, want, mass, dtype)
+
+
+@pytest.mark.gpu
 def test_a_stack_that_streams_through_l2():
     """Matrices of more than 64 MB read once, and the same product of a part of them that is not: bit for bit."""
     E, n, k = 40, 1024, 2048
