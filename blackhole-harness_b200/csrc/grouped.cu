@@ -392,10 +392,11 @@ constexpr uint32_t kRingBytes = 200 * 1024;            // 6 steps of A and B, 4 
 constexpr int kBoxes = 4;                              // row boxes of 16, 32, 64, 128
 constexpr int kBoxes8 = 8;                             // 8-bit rows: of 16, 32, 48 .. 128
 
-// kInt8: y = x W^T of 8-bit integers with scales; kInt8Glu: SwiGLU of such products with gate and up rows; kWgradT: M
-// side k, N side n.
-enum PairMode { kRowsK = 0, kRowsMN = 1, kInt8 = 2, kInt8Glu = 3, kWgrad = 4, kWgradT = 5 };
-constexpr bool is_int8(int mode) { return mode == kInt8 || mode == kInt8Glu; }
+// kInt8: y = x W^T of 8-bit integers with scales; kInt8F32: the same to f32 rows that TMA can store (a kernel of its own: as a
+// branch of kInt8 it took registers from the 16-bit results, 2047 tokens with Zipf 1.2, 2048 x 768: 48.3 us against 46.4);
+// kInt8Glu: SwiGLU of such products with gate and up rows; kWgradT: M side k, N side n.
+enum PairMode { kRowsK = 0, kRowsMN = 1, kInt8 = 2, kInt8F32 = 3, kInt8Glu = 4, kWgrad = 5, kWgradT = 6 };
+constexpr bool is_int8(int mode) { return mode >= kInt8 && mode <= kInt8Glu; }
 constexpr bool k_major(int mode) { return mode == kRowsK || is_int8(mode); }   // the matrix as it lies is reduction-major
 
 // Two staging tiles a writer in 8-bit products, which leave that much of the ring.
@@ -676,7 +677,7 @@ struct Writer {
   __device__ __forceinline__ bool f32() const { return RUNS || p.f32; }
   // Row products that leave by TMA take fragments, everything else a row of 32 columns a lane.
   __device__ __forceinline__ void load(uint32_t acc, uint32_t (&r)[32]) const {
-    if (MODE == kInt8Glu || (MODE != kWgrad && p.tma_out && (MODE < kWgrad || !f32()))) {
+    if (MODE == kInt8Glu || MODE == kInt8F32 || (MODE != kWgrad && p.tma_out && (MODE < kWgrad || !f32()))) {
       tmem_ld_fragments<0>(acc, r);
       tmem_ld_fragments<16>(acc + (16u << 16), r);
     } else {
@@ -688,8 +689,10 @@ struct Writer {
       if (p.tma_out) scale_fragments(r, x);
       else scale_columns(r, x);
     }
+    if constexpr (MODE == kInt8F32) scale_fragments(r, x);
     if constexpr (MODE == kWgrad) write_gradient(col, r);
     else if constexpr (MODE == kInt8Glu) write_glu(col, r, x);
+    else if constexpr (MODE == kInt8F32) write_f32(col, r);
     else if (MODE == kWgradT && p.tma_out && f32()) write_lines(col, r);
     else if (p.tma_out) write_rows(col, r);
     else write_elements(col, r);
@@ -735,7 +738,7 @@ struct Writer {
   // on other whole numbers often enough to change the layer's result by 0.8 %, five times its own rounding; fp16 0.3 %.)
   __device__ __forceinline__ void write_glu(int32_t col, uint32_t (&r)[32], float x) {
     scale_fragments(r, x);
-    const int32_t rows = min(32, cols - col), f = m / 2;
+    const int32_t f = m / 2;
     const int g = lane / 4, q = lane % 4;
     stage_free();
 #pragma unroll
@@ -748,10 +751,21 @@ struct Writer {
         // 1 / (1 + e^-gate): where e^-gate leaves f32's range, below gates of -88, it is 0
         const float2 t = mul2(gate, make_float2(-1.44269504f, -1.44269504f));
         const float2 act = mul2(mul2(gate, make_float2(fast_inverse(1.f + fast_exp2(t.x)), fast_inverse(1.f + fast_exp2(t.y)))), up);
-        float* to = reinterpret_cast<float*>(stage + line * 64 + (((8 * h + g) / 4 ^ (line >> 1 & 3)) << 4)) + g % 4;
+        float* to = line_of(line, 8 * h + g);
         to[0] = act.x;
-        to[16] = act.y;   // the next line's pieces lie in the same order
+        to[16] = act.y;
       }
+    store_lines(col, f);
+  }
+
+  // The place of a value in the staging tile, as lines of 16 f32 features of a row; the next row's line has its pieces in the
+  // same order where `line` is even.
+  __device__ __forceinline__ float* line_of(int line, int feature) const {
+    return reinterpret_cast<float*>(stage + line * 64 + ((feature / 4 ^ (line >> 1 & 3)) << 4)) + feature % 4;
+  }
+  // 16 f32 features from f on of 32 rows leave the staging tile: by TMA where the rows are all the group's.
+  __device__ __forceinline__ void store_lines(int32_t col, int32_t f) {
+    const int32_t rows = min(32, cols - col);
     if (rows == 32) {
       fence_proxy_async_smem();
       __syncwarp();
@@ -762,14 +776,35 @@ struct Writer {
       stage_used();
     } else {   // the group's last rows: the next ones are another group's
       __syncwarp();
+      const int q = lane % 4;
       float* dst = static_cast<float*>(p.dst) + (n0 + col) * p.ld + f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int line = 8 * i + lane / 4;
-        const float4 v = *reinterpret_cast<const float4*>(stage + line * 64 + ((q ^ (line >> 1 & 3)) << 4));
-        if (line < rows) *reinterpret_cast<float4*>(dst + line * p.ld + q * 4) = v;
+        const float4 v = *reinterpret_cast<const float4*>(line_of(line, 4 * q));
+        if (line < rows && f + 4 * q < p.out_len) *reinterpret_cast<float4*>(dst + line * p.ld + q * 4) = v;
       }
       __syncwarp();
+    }
+  }
+
+  // Scaled products in f32, 16 features at a time (the layer of 4096 tokens, 96 experts of 2048 x 768, whose down product
+  // writes 268 MB so: 287 us; by write_elements 365).
+  __device__ __forceinline__ void write_f32(int32_t col, uint32_t (&r)[32]) {
+    const int g = lane / 4, q = lane % 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (m + 16 * h >= p.m_len) break;
+      stage_free();
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          float* to = line_of(8 * i + 2 * q, 8 * b + g);
+          to[0] = __uint_as_float(r[16 * h + 4 * i + 2 * b]);
+          to[16] = __uint_as_float(r[16 * h + 4 * i + 2 * b + 1]);
+        }
+      store_lines(col, m + 16 * h);
     }
   }
 
@@ -1003,7 +1038,7 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
             if (!loads_a) {
             } else if constexpr (MODE == kRowsK) {
               pair_load_3d(a, &p.a, bar, r, m, t.e);
-            } else if constexpr (MODE == kInt8) {
+            } else if constexpr (MODE == kInt8 || MODE == kInt8F32) {
               if (p.stream) pair_load_3d_hint(a, &p.a, bar, 2 * r, m, t.e, policy);
               else pair_load_3d(a, &p.a, bar, 2 * r, m, t.e);
             } else if constexpr (MODE == kInt8Glu) {   // 8 rows of gate, the 8 of up, and so on
@@ -1327,8 +1362,9 @@ int sm_count(int* sms) {
           PAIR_KERNELS(kRowsMN, kOne), PAIR_KERNELS(kRowsMN, kTwo), PAIR_KERNELS(kRowsMN, kNarrow), PAIR_KERNELS(kRowsMN, kMiddle),
           PAIR_KERNELS(kWgrad, kOne), PAIR_KERNELS(kWgrad, kMiddle), PAIR_KERNELS(kWgradT, kOne), PAIR_KERNELS(kWgradT, kMiddle)},
          kRowsK);
-    room({INT8_KERNEL(kInt8, kNarrow), INT8_KERNEL(kInt8, kMiddle), INT8_KERNEL(kInt8, kOne), INT8_KERNEL(kInt8Glu, kNarrow),
-          INT8_KERNEL(kInt8Glu, kMiddle), INT8_KERNEL(kInt8Glu, kOne)},
+    room({INT8_KERNEL(kInt8, kNarrow), INT8_KERNEL(kInt8, kMiddle), INT8_KERNEL(kInt8, kOne), INT8_KERNEL(kInt8F32, kNarrow),
+          INT8_KERNEL(kInt8F32, kMiddle), INT8_KERNEL(kInt8F32, kOne), INT8_KERNEL(kInt8Glu, kNarrow), INT8_KERNEL(kInt8Glu, kMiddle),
+          INT8_KERNEL(kInt8Glu, kOne)},
          kInt8);
     if (e != cudaSuccess) return report_cuda_error(e, "grouped product kernel");
     e = cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev);
@@ -1588,10 +1624,13 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
                             CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
   } else {
-    q.tma_out = !q.f32 && tma_rows(d.out, d.ld_out, 2) && d.n % 8 == 0;
+    const int z = f32 ? 4 : 2;
+    q.tma_out = !split && tma_rows(d.out, d.ld_out, z) && d.n * z % 16 == 0;
     if (q.tma_out && d.rows >= 32)
-      if (int rc = make_map(&q.out, d.out, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, d.n,
-                            d.rows, 1, 2 * d.ld_out, 0, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B))
+      if (int rc = make_map(&q.out, d.out, f32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                           : bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                  : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                            2, d.n, d.rows, 1, z * d.ld_out, 0, 64 / z, 32, CU_TENSOR_MAP_SWIZZLE_64B))
         return rc;
   }
   auto launch = [&](auto mode) {
@@ -1600,7 +1639,9 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
            : shape == kMiddle ? launch_pair<MODE, kMiddle>(q, tiles, sms, st)
                               : launch_pair<MODE, kOne>(q, tiles, sms, st);
   };
-  cudaError_t e = d.glu ? launch(std::integral_constant<int, kInt8Glu>{}) : launch(std::integral_constant<int, kInt8>{});
+  cudaError_t e = d.glu                ? launch(std::integral_constant<int, kInt8Glu>{})
+                  : q.tma_out && q.f32 ? launch(std::integral_constant<int, kInt8F32>{})
+                                       : launch(std::integral_constant<int, kInt8>{});
   if (e == cudaSuccess && split) {
     JoinParams j{};
     j.part = static_cast<const float*>(d.workspace);

@@ -59,30 +59,11 @@ struct RowsParams {
   int8_t* q;              // [rows, ld_q], or with `places` [places..., ld_q]
   int64_t ld_q;
   float* scale;
-  const float* factor;    // [rows], what every scale is multiplied with; or null
   const int32_t* count;   // on the device: rows that exist, of `rows`; or null
-  // The layer's tokens, each to the rows of its topk slots: slot s has row places[s] (-1: none), and its
-  // routing weight is copied to row_weight.
+  // The layer's tokens, each to the rows of its topk slots: slot s has row places[s] (-1: none).
   const int32_t* places;
   int32_t topk;
-  const float* weights;
-  float* row_weight;
 };
-
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4& v, float (&x)[8]) {   // 16 bits
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (std::is_same_v<T, __half>) {
-      x[2 * i] = __half2float(__ushort_as_half(static_cast<uint16_t>(w[i])));
-      x[2 * i + 1] = __half2float(__ushort_as_half(static_cast<uint16_t>(w[i] >> 16)));
-    } else {
-      x[2 * i] = __uint_as_float(w[i] << 16);
-      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-  }
-}
 
 // A row's values as they lie, 16 bytes at a time, or one by one (rows that are not aligned to 16 bytes, or of odd
 // lengths): the largest magnitude's bits, and the values in f32.
@@ -254,14 +235,7 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsPa
 #pragma unroll
     for (int i = 0; i < kPieces; ++i)
       if (lane + i * TPR < n) put(at, lane + i * TPR, w[i]);
-    if (lane == 0) {
-      if constexpr (PLACES) {
-        p.scale[at] = to.scale();
-        p.row_weight[at] = p.weights[row * p.topk + j];
-      } else {
-        p.scale[at] = p.factor ? to.scale() * p.factor[row] : to.scale();
-      }
-    }
+    if (lane == 0) p.scale[at] = to.scale();
   }
   for (int c = lane + kPieces * TPR; c < n; c += TPR) {
     P v;
@@ -453,88 +427,90 @@ cudaError_t launch_plan(const PlanParams& p, cudaStream_t st) {
 }
 
 // ------------------------------------------------------------------- sum
-// out[t] = sum over j of y[places[t topk + j]], f32 in j's order, rounded once; a slot without a row adds nothing.  Bound by
-// HBM: a thread has eight 16-byte loads in flight, of as many of a token's rows as there are and so many pieces of each.
+// out[t] = sum over j of weights[t topk + j] y[places[t topk + j]], in f32 in j's order, rounded once; a slot without a row
+// adds nothing.  Products are rounded by themselves (no FMA): slots that are each other's negatives leave 0.  Slots' rows are f32: in 16 bits, where they would be half the bytes, the layer's result was off by
+// 0.23 % where its own rounding to bf16 costs 0.17, fp16 rows could leave the type's range where their sum does not, and a
+// caller with f32 rows got eight bits.  (4096 tokens, 96 experts of 2048 x 768: 287 us in a
+// graph, 239 with 16-bit rows; 16 tokens 67 and 69.)  The
+// routing weight is taken here, not with the activation's scale: the product of two small ones would leave the normal numbers
+// before the result does.  Bound by HBM: a thread has eight 16-byte loads in flight, of as many of a token's rows as there
+// are and so many pieces of each.
 constexpr int kSumThreads = 256;
 
 struct SumParams {
-  const void* y;   // [rows, hidden] of Y
+  const float* y;   // [rows, hidden]
   const int32_t* places;
+  const float* weights;
   void* out;
   int64_t tokens;
   int32_t topk, hidden;
 };
 
-template <typename Y, typename T, int ROWS>
+template <typename T, int ROWS>
 __global__ void __launch_bounds__(kSumThreads) sum_rows_kernel(const SumParams p) {
   constexpr int kEach = 8 / ROWS;
-  const int32_t pieces = p.hidden / 8, spans = (pieces + 32 * kEach - 1) / (32 * kEach), lane = threadIdx.x % 32;
+  const int32_t pieces = p.hidden / 4, spans = (pieces + 32 * kEach - 1) / (32 * kEach), lane = threadIdx.x % 32;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * (kSumThreads / 32) + threadIdx.x / 32;
   pdl_wait();
   pdl_launch_dependents();
   const int64_t t = unit / spans;
   if (t >= p.tokens) return;
   const int32_t first = static_cast<int32_t>(unit % spans) * 32 * kEach + lane;
-  float sum[kEach][8] = {};
+  float4 sum[kEach] = {};
   for (int j0 = 0; j0 < p.topk; j0 += ROWS) {
-    uint4 v[ROWS][kEach];
+    float4 v[ROWS][kEach];
+    float weight[ROWS];
 #pragma unroll
     for (int j = 0; j < ROWS; ++j) {
-      const int32_t at = j0 + j < p.topk ? p.places[t * p.topk + j0 + j] : -1;
-      const uint4* row = static_cast<const uint4*>(p.y) + static_cast<int64_t>(at) * pieces;
+      const int64_t slot = t * p.topk + j0 + j;
+      const int32_t at = j0 + j < p.topk ? p.places[slot] : -1;
+      weight[j] = at >= 0 ? p.weights[slot] : 0.f;
+      const float4* row = reinterpret_cast<const float4*>(p.y) + static_cast<int64_t>(at) * pieces;
 #pragma unroll
       for (int i = 0; i < kEach; ++i)
-        v[j][i] = at >= 0 && first + 32 * i < pieces ? row[first + 32 * i] : make_uint4(0, 0, 0, 0);
+        v[j][i] = at >= 0 && first + 32 * i < pieces ? row[first + 32 * i] : make_float4(0.f, 0.f, 0.f, 0.f);
     }
 #pragma unroll
     for (int j = 0; j < ROWS; ++j)
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        float f[8];
-        unpack<Y>(v[j][i], f);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) sum[i][q] += f[q];
+        sum[i].x += __fmul_rn(weight[j], v[j][i].x);
+        sum[i].y += __fmul_rn(weight[j], v[j][i].y);
+        sum[i].z += __fmul_rn(weight[j], v[j][i].z);
+        sum[i].w += __fmul_rn(weight[j], v[j][i].w);
       }
   }
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
     if (first + 32 * i >= pieces) continue;
-    T* out = static_cast<T*>(p.out) + t * p.hidden + (first + 32 * i) * 8;
+    T* out = static_cast<T*>(p.out) + t * p.hidden + (first + 32 * i) * 4;
     if constexpr (std::is_same_v<T, float>) {
-      reinterpret_cast<float4*>(out)[0] = make_float4(sum[i][0], sum[i][1], sum[i][2], sum[i][3]);
-      reinterpret_cast<float4*>(out)[1] = make_float4(sum[i][4], sum[i][5], sum[i][6], sum[i][7]);
+      *reinterpret_cast<float4*>(out) = sum[i];
+    } else if constexpr (std::is_same_v<T, __half>) {
+      const __half2 lo = __floats2half2_rn(sum[i].x, sum[i].y), hi = __floats2half2_rn(sum[i].z, sum[i].w);
+      *reinterpret_cast<uint2*>(out) = make_uint2(reinterpret_cast<const uint32_t&>(lo), reinterpret_cast<const uint32_t&>(hi));
     } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if constexpr (std::is_same_v<T, __half>) {
-          const __half2 h = __floats2half2_rn(sum[i][2 * q], sum[i][2 * q + 1]);
-          w[q] = reinterpret_cast<const uint32_t&>(h);
-        } else {
-          const __nv_bfloat162 h = __floats2bfloat162_rn(sum[i][2 * q], sum[i][2 * q + 1]);
-          w[q] = reinterpret_cast<const uint32_t&>(h);
-        }
-      }
-      *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+      const __nv_bfloat162 lo = __floats2bfloat162_rn(sum[i].x, sum[i].y), hi = __floats2bfloat162_rn(sum[i].z, sum[i].w);
+      *reinterpret_cast<uint2*>(out) = make_uint2(reinterpret_cast<const uint32_t&>(lo), reinterpret_cast<const uint32_t&>(hi));
     }
   }
 }
 
-template <typename Y, typename T>
+template <typename T>
 cudaError_t launch_sum(const SumParams& p, cudaStream_t st) {
   auto go = [&](auto rows, auto* kernel) {
     constexpr int kEach = 8 / decltype(rows)::value;
-    const int64_t spans = (p.hidden / 8 + 32 * kEach - 1) / (32 * kEach);
+    const int64_t spans = (p.hidden / 4 + 32 * kEach - 1) / (32 * kEach);
     const int64_t blocks = (p.tokens * spans + kSumThreads / 32 - 1) / (kSumThreads / 32);
     if (blocks > 0x7fffffffll) return cudaErrorInvalidConfiguration;
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg = launch_config(dim3(static_cast<unsigned>(blocks)), kSumThreads, 0, st, &attr);
     return cudaLaunchKernelEx(&cfg, kernel, p);
   };
-  if (p.topk == 1) return go(std::integral_constant<int, 1>{}, sum_rows_kernel<Y, T, 1>);
-  if (p.topk == 2) return go(std::integral_constant<int, 2>{}, sum_rows_kernel<Y, T, 2>);
-  if (p.topk <= 4) return go(std::integral_constant<int, 4>{}, sum_rows_kernel<Y, T, 4>);
-  return go(std::integral_constant<int, 8>{}, sum_rows_kernel<Y, T, 8>);
+  if (p.topk == 1) return go(std::integral_constant<int, 1>{}, sum_rows_kernel<T, 1>);
+  if (p.topk == 2) return go(std::integral_constant<int, 2>{}, sum_rows_kernel<T, 2>);
+  if (p.topk <= 4) return go(std::integral_constant<int, 4>{}, sum_rows_kernel<T, 4>);
+  return go(std::integral_constant<int, 8>{}, sum_rows_kernel<T, 8>);
 }
 
 bool is16(int32_t dt) { return dt == HEXMOE_BF16 || dt == HEXMOE_F16; }
@@ -572,21 +548,20 @@ struct MmScratch {
 
 struct LayerScratch {
   int32_t *offsets, *places;
-  float *x_scale, *weight, *act, *act_scale;
+  float *x_scale, *act, *act_scale, *y;
   int8_t *xq, *actq;
-  uint8_t *y, *partial;
+  uint8_t* partial;
   size_t partial_bytes, used;
   LayerScratch(void* ws, int64_t slots, int32_t experts, int32_t hidden, int32_t inter) {
     Carve c{static_cast<uint8_t*>(ws)};
     offsets = c.take<int32_t>(experts + 1);
     places = c.take<int32_t>(slots);
     x_scale = c.take<float>(slots);
-    weight = c.take<float>(slots);
     act_scale = c.take<float>(slots);
     xq = c.take<int8_t>(slots * hidden);
     act = c.take<float>(slots * inter);
     actq = c.take<int8_t>(slots * inter);
-    y = c.take<uint8_t>(2 * slots * hidden);
+    y = c.take<float>(slots * hidden);
     partial_bytes = int8_partial_bytes(slots, experts, hidden, inter);
     partial = c.take<uint8_t>(partial_bytes);
     used = c.used;
@@ -703,7 +678,7 @@ int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t to
   const PlanParams plan = {topk_ids, ids_dtype == HEXMOE_I64, experts, slots, s.offsets, s.places, dev_err};
   RowsParams p{};
   p.x = x; p.ld_x = ld_x; p.rows = tokens; p.cols = hidden; p.q = s.xq; p.ld_q = hidden; p.scale = s.x_scale;
-  p.places = s.places; p.topk = topk; p.weights = topk_weights; p.row_weight = s.weight;
+  p.places = s.places; p.topk = topk;
   cudaError_t e = launch_plan(plan, st);
   if (e == cudaSuccess) e = launch_rows(p, x_dtype, st);
   if (e != cudaSuccess) return report_cuda_error(e, what);
@@ -717,23 +692,22 @@ int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t to
   if (int rc = run_int8_product(what, d, st)) return rc;
   p = RowsParams{};
   p.x = s.act; p.ld_x = inter; p.rows = slots; p.cols = inter; p.q = s.actq; p.ld_q = inter; p.scale = s.act_scale;
-  p.factor = s.weight; p.count = s.offsets + experts;
+  p.count = s.offsets + experts;
   e = launch_rows(p, HEXMOE_F32, st);
   if (e != cudaSuccess) return report_cuda_error(e, what);
-  const int32_t y_dtype = x_dtype == HEXMOE_F16 ? HEXMOE_F16 : HEXMOE_BF16;
   d = Int8Product{};
   d.x = s.actq; d.ld_x = inter; d.x_scale = s.act_scale;
   d.w = w2; d.ld_w = ld_w2; d.stride_w = stride_w2; d.w_scale = w2_scale;
   d.rows = slots; d.experts = experts; d.n = hidden; d.k = inter;
   d.offsets = s.offsets;
-  d.out = s.y; d.ld_out = hidden; d.out_dtype = y_dtype;
+  d.out = s.y; d.ld_out = hidden; d.out_dtype = HEXMOE_F32;
   d.early = 1;
   d.workspace = s.partial; d.workspace_bytes = s.partial_bytes;
   if (int rc = run_int8_product(what, d, st)) return rc;
-  const SumParams sum = {s.y, s.places, out, tokens, topk, hidden};
-  e = y_dtype == HEXMOE_F16 ? (out_dtype == HEXMOE_F32 ? launch_sum<__half, float>(sum, st) : launch_sum<__half, __half>(sum, st))
-      : out_dtype == HEXMOE_F32 ? launch_sum<__nv_bfloat16, float>(sum, st)
-                                : launch_sum<__nv_bfloat16, __nv_bfloat16>(sum, st);
+  const SumParams sum = {s.y, s.places, topk_weights, out, tokens, topk, hidden};
+  e = out_dtype == HEXMOE_F32   ? launch_sum<float>(sum, st)
+      : out_dtype == HEXMOE_F16 ? launch_sum<__half>(sum, st)
+                                : launch_sum<__nv_bfloat16>(sum, st);
   return e == cudaSuccess ? HEXMOE_OK : report_cuda_error(e, what);
 }
 

@@ -513,9 +513,9 @@ HEXMOE_API int hexmoe_grouped_mm_int8(const void* x, int32_t x_dtype, int64_t ld
  * x_dtype or F32; w13 I8 [experts, 2 * inter, hidden] (gate rows, then up) with
  * scales [experts, 2 * inter], w2 I8 [experts, hidden, inter] with scales
  * [experts, hidden].  hidden and inter are multiples of 16.  The activation stays
- * in f32 until it is quantized; a slot's row is rounded to 16 bits (BF16 for F32
- * x) before a token's rows are summed in f32, as in hexmoe_forward.  Ids outside 0..experts-1 add
- * nothing and set the device error word. */
+ * in f32 until it is quantized, and a slot's row until a token's rows are summed,
+ * times their routing weights; the sum is rounded once.  Ids outside 0..experts-1
+ * add nothing and set the device error word. */
 HEXMOE_API size_t hexmoe_int8_forward_workspace_bytes(int64_t tokens, int32_t topk, int32_t experts, int32_t hidden,
                                                       int32_t inter);
 HEXMOE_API int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t tokens, int32_t hidden,
