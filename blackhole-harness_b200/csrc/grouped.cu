@@ -37,14 +37,8 @@ struct Groups {
   int64_t rows;
 };
 
-// FROM_L2: past L1, for a warp that reads before it waits for the kernels ahead (Int8Params::early).
-template <bool FROM_L2>
 __device__ __forceinline__ int64_t raw_offset(const Groups& g, int e) {
-  if constexpr (FROM_L2) {
-    return g.is64 ? __ldcg(static_cast<const long long*>(g.offsets) + e) : __ldcg(static_cast<const int32_t*>(g.offsets) + e);
-  } else {
-    return g.is64 ? static_cast<const int64_t*>(g.offsets)[e] : static_cast<const int32_t*>(g.offsets)[e];
-  }
+  return g.is64 ? static_cast<const int64_t*>(g.offsets)[e] : static_cast<const int32_t*>(g.offsets)[e];
 }
 
 // A warp's walk over the groups, 32 at a time: lane l of a step holds group
@@ -53,11 +47,10 @@ struct GroupScan {
   int64_t begin, end;   // this lane's group (empty past the last expert)
   bool bad;
 };
-template <bool FROM_L2 = false>
 __device__ __forceinline__ GroupScan scan_groups(const Groups& g, int base, int64_t& carry) {
   const int lane = threadIdx.x % 32, e = base + lane;
   const bool in = e < g.experts;
-  const int64_t raw0 = raw_offset<FROM_L2>(g, min(e, g.experts)), raw1 = raw_offset<FROM_L2>(g, min(e + 1, g.experts));
+  const int64_t raw0 = raw_offset(g, min(e, g.experts)), raw1 = raw_offset(g, min(e + 1, g.experts));
   GroupScan s;
   s.bad = in && (raw0 < 0 || raw1 < raw0 || raw1 > g.rows);
   s.begin = raw0;
@@ -445,10 +438,6 @@ struct Int8Params : PairParams {
   int32_t stream;              // the matrices pass through L2 without staying
   int32_t whole[2];            // the offsets of one group of all rows
   int32_t boxes;               // of rows, that there are
-  // The kernel before this one only makes the rows and their scales, and lets this one start when everything before it is
-  // done (it waits, then launches): offsets and matrices may be read before it ends.  One token on 96 experts, quantized
-  // and multiplied: 9.9 us without, 9.15 with; 64 tokens 52.2, 49.7; the layer of 16 tokens 74.7, 69.8.
-  int32_t early;
 };
 template <int MODE>
 using Params = std::conditional_t<is_int8(MODE), Int8Params, PairParams>;
@@ -515,7 +504,7 @@ struct Walker {
     while (tile >= total) {
       if (base + 32 >= p.g.experts) return false;
       base += 32;
-      const GroupScan s = scan_groups<is_int8(MODE)>(groups_of<MODE>(p), base, carry);
+      const GroupScan s = scan_groups(groups_of<MODE>(p), base, carry);
       bad |= s.bad;
       begin = s.begin;
       end = s.end;
@@ -994,12 +983,8 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
   cluster_sync();
   tc_fence_after();
   const uint32_t tmem = c->tmem;
-  bool waits = true;
-  if constexpr (is_int8(MODE)) waits = !(p.early && (warp == 0 || warp == 3));   // the matrix's loads, the walk
-  if (waits) {
-    pdl_wait();
-    pdl_launch_dependents();   // one wave: whoever waits for this grid may take its place on the SMs as they fall free
-  }
+  pdl_wait();   // every warp: what a kernel ahead wrote is only visible to a thread that has waited
+  pdl_launch_dependents();   // one wave: whoever waits for this grid may take its place on the SMs as they fall free
 
   const int32_t first = blockIdx.x / 2, stride = gridDim.x / 2;
   std::conditional_t<is_int8(MODE), TileReader, Walker<MODE, SHAPE, RUNS>> walk;
@@ -1591,7 +1576,6 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
   q.red = (d.k + 1) / 2;
   q.m_tiles = (d.n + 255) / 256;
   q.whole[1] = static_cast<int32_t>(d.rows);
-  q.early = d.early;
   q.x_scale = d.x_scale;
   q.w_scale = d.w_scale;
   q.splits = d.glu ? 1 : rows_splits(d.rows, d.experts, d.n, q.red);

@@ -71,7 +71,7 @@ template <typename T, bool VEC>
 struct Piece {
   static constexpr int kValues = VEC ? 16 / sizeof(T) : 1, kWords = VEC ? 4 : 1;
   uint32_t w[kWords];
-  // Past L1: it is read once, or before the wait.
+  // Past L1: it is read once.
   __device__ __forceinline__ void load(const T* row, int i) {
     if constexpr (VEC) {
       const uint4 v = __ldcg(reinterpret_cast<const uint4*>(row) + i);
@@ -147,21 +147,17 @@ struct RowScale {
   }
 };
 
-// A row to TPR threads.  PLACES: into the rows of its slots, which the kernel before makes; it lets this one start when
-// everything before it is done, so that the row may be read and turned into bytes before the wait (the layer of 1 token on 96
-// experts: 24.0 us, 24.9 when it waits first, 26.9 when few tokens are quantized by that kernel itself).  The pieces are
-// turned into bytes in registers and stored from there: what is unrolled eight times stays short, for a kernel of a few
-// microseconds waits for its instructions more than for anything else.
+// A row to TPR threads.  PLACES: into the rows of its slots, which the kernel before has found.  The pieces are turned into
+// bytes in registers and stored from there: what is unrolled eight times stays short, for a kernel of a few microseconds waits
+// for its instructions more than for anything else.
 template <typename T, bool VEC, int TPR, bool PLACES>
 __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsParams p) {
   constexpr int kRows = kRowThreads / TPR;
   __shared__ uint32_t part[kRowThreads / 32];
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + threadIdx.x / TPR;
   const int lane = threadIdx.x % TPR;
-  if constexpr (!PLACES) {
-    pdl_wait();
-    pdl_launch_dependents();
-  }
+  pdl_wait();
+  pdl_launch_dependents();
   const bool live = row < p.rows && (!p.count || row < *p.count);
   using P = Piece<T, VEC>;
   constexpr int V = P::kValues, kWords = V > 4 ? V / 4 : 1;
@@ -221,10 +217,6 @@ __global__ void __launch_bounds__(kRowThreads) quantize_rows_kernel(const RowsPa
 #pragma unroll
   for (int i = 0; i < kPieces; ++i) {
     if (live && lane + i * TPR < n) bytes(held[i], w[i]);
-  }
-  if constexpr (PLACES) {
-    pdl_wait();
-    pdl_launch_dependents();
   }
   if (!live) return;
   const int copies = PLACES ? p.topk : 1;
@@ -630,7 +622,6 @@ int hexmoe_grouped_mm_int8(const void* x, int32_t x_dtype, int64_t ld_x, const f
     const cudaError_t e = launch_rows(p, x_dtype, st);
     if (e != cudaSuccess) return report_cuda_error(e, what);
     d.x = s.q; d.ld_x = p.ld_q; d.x_scale = s.scale;
-    d.early = 1;
   }
   d.w = w; d.ld_w = ld_w; d.stride_w = stride_w; d.w_scale = w_scale;
   d.rows = rows; d.experts = experts; d.n = n; d.k = k;
@@ -688,7 +679,6 @@ int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t to
   d.rows = slots; d.experts = experts; d.n = 2 * inter; d.k = hidden;
   d.offsets = s.offsets;
   d.out = s.act; d.ld_out = inter; d.out_dtype = HEXMOE_F32; d.glu = 1;
-  d.early = 1;
   if (int rc = run_int8_product(what, d, st)) return rc;
   p = RowsParams{};
   p.x = s.act; p.ld_x = inter; p.rows = slots; p.cols = inter; p.q = s.actq; p.ld_q = inter; p.scale = s.act_scale;
@@ -701,7 +691,6 @@ int hexmoe_int8_forward(const void* x, int32_t x_dtype, int64_t ld_x, int64_t to
   d.rows = slots; d.experts = experts; d.n = hidden; d.k = inter;
   d.offsets = s.offsets;
   d.out = s.y; d.ld_out = hidden; d.out_dtype = HEXMOE_F32;
-  d.early = 1;
   d.workspace = s.partial; d.workspace_bytes = s.partial_bytes;
   if (int rc = run_int8_product(what, d, st)) return rc;
   const SumParams sum = {s.y, s.places, topk_weights, out, tokens, topk, hidden};

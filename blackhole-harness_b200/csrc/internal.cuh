@@ -193,8 +193,6 @@ struct Int8Product {
   void* out;
   int64_t ld_out;
   int32_t out_dtype, glu;
-  int32_t early;           // the launch before this one makes x and x_scale and nothing else that is read here, and waits
-                           // for what comes before it, then launches its dependents
   void* workspace;         // int8_partial_bytes, or null
   size_t workspace_bytes;
 };
