@@ -424,7 +424,7 @@ struct PairParams {
   int32_t m_tiles, n_tiles, tile_n;   // n_tiles, tile_n: weight gradient
   int32_t splits;            // runs that the reduction of a tile is cut into, over several pairs
   int32_t run;               // RUNS: most steps that one accumulator sums
-  void* dst;                 // splits > 1: fp32 partials, one result a run
+  void* dst;                 // splits > 1: fp32 (8-bit products: int32) partials, one result a run
   int64_t ld, stride_e, stride_split;
   int32_t f32, bf16, accumulate, tma_out;
   int32_t* dev_err;
@@ -435,6 +435,7 @@ struct Int8Params : PairParams {
   CUtensorMap rows[kBoxes8];   // in boxes of 16 (i + 1)
   const float* x_scale;        // [rows]
   const float* w_scale;        // [experts, matrix rows]
+  int32_t* row_expert;         // [rows], splits > 1: the expert of every row, -1 of no group, for what adds the parts up
   int32_t stream;              // the matrices pass through L2 without staying
   int32_t whole[2];            // the offsets of one group of all rows
   int32_t boxes;               // of rows, that there are
@@ -676,7 +677,7 @@ struct Writer {
   __device__ __forceinline__ void write(int32_t col, uint32_t (&r)[32], float x) {
     if constexpr (MODE == kInt8) {
       if (p.tma_out) scale_fragments(r, x);
-      else scale_columns(r, x);
+      else if (p.splits == 1) scale_columns(r, x);   // parts of a split reduction stay whole numbers
     }
     if constexpr (MODE == kInt8F32) scale_fragments(r, x);
     if constexpr (MODE == kWgrad) write_gradient(col, r);
@@ -1199,6 +1200,10 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
       out.e = MODE >= kWgrad ? t.split * p.g.experts + t.e : t.split;
       out.m = t.m0 + static_cast<int32_t>(rank) * 128 + quad * 32;
       out.add = p.accumulate || (RUNS && t.add);
+      if constexpr (MODE == kInt8) {
+        if (p.splits > 1 && t.split == 0 && out.m == 0 && part == 0)
+          for (int32_t i = lane; i < t.valid; i += 32) p.row_expert[t.row0 + i] = t.e;
+      }
       if (RUNS && t.add && p.tma_out) {   // the stores of the run before have arrived: additions to the same values stay in order
         if (elect_one()) bulk_wait_all();
         __syncwarp();
@@ -1259,7 +1264,9 @@ __global__ void __launch_bounds__(kPairThreads, 1) __cluster_dims__(2, 1, 1)
     if (MODE < kWgrad && ok) {   // rows of no group
       const int64_t gap = walk.lo + (p.g.rows - walk.carry);
       for (int64_t j = blockIdx.x; j < gap * p.splits; j += gridDim.x) {
-        const int64_t i = j % gap, at = j / gap * p.stride_split + (i < walk.lo ? i : i - walk.lo + walk.carry) * p.ld;
+        const int64_t i = j % gap, row = i < walk.lo ? i : i - walk.lo + walk.carry, at = j / gap * p.stride_split + row * p.ld;
+        if constexpr (MODE == kInt8)
+          if (p.splits > 1 && j < gap && threadIdx.x == 128) p.row_expert[row] = -1;
         for (int32_t f = threadIdx.x - 128; f < p.out_len; f += kWriters * 32) {
           if (p.f32) static_cast<float*>(p.dst)[at + f] = 0.f;
           else static_cast<uint16_t*>(p.dst)[at + f] = 0;
@@ -1471,15 +1478,23 @@ int wgrad_splits(int64_t rows, int32_t experts, int32_t n, int32_t k) {
 }
 
 struct JoinParams {
-  const float* part;   // [splits][rows][pitch]
+  const void* part;    // [splits][rows][pitch], f32 or (8-bit products) int32
   int64_t rows, pitch;
   int32_t splits, cols;
   void* out;           // row r: matrix r / inner, its row r % inner
   int64_t ld, stride;
   int32_t inner, f32, bf16, accumulate, vec;
 };
+// Whole numbers are added and then scaled as they are where a reduction is not split: the same bits, whatever the number of
+// parts.  (As scaled f32 parts, each was off by its own roundings, which is more than the result's where parts cancel.)
+struct Int8JoinParams : JoinParams {
+  const int32_t* row_expert;
+  const float *x_scale, *w_scale;
+};
 
-__global__ void __launch_bounds__(256) grouped_join_kernel(const JoinParams p) {
+template <typename P>
+__global__ void __launch_bounds__(256) grouped_join_kernel(const P p) {
+  constexpr bool kWhole = std::is_same_v<P, Int8JoinParams>;
   pdl_wait();
   pdl_launch_dependents();
   const int32_t pieces = static_cast<int32_t>(p.pitch / 4);
@@ -1487,17 +1502,30 @@ __global__ void __launch_bounds__(256) grouped_join_kernel(const JoinParams p) {
   if (i >= p.rows * pieces) return;
   const int64_t row = i / pieces;
   const int32_t col = static_cast<int32_t>(i % pieces) * 4;
+  const int count = min(4, p.cols - col);
   float v[4] = {};
+  std::conditional_t<kWhole, int32_t, float> sum[4] = {};
 #pragma unroll 4
   for (int s = 0; s < p.splits; ++s) {
-    const float4 f = *reinterpret_cast<const float4*>(p.part + (s * p.rows + row) * p.pitch + col);
-    v[0] += f.x;
-    v[1] += f.y;
-    v[2] += f.z;
-    v[3] += f.w;
+    const auto f = *reinterpret_cast<const std::conditional_t<kWhole, int4, float4>*>(
+        static_cast<const float*>(p.part) + (s * p.rows + row) * p.pitch + col);
+    sum[0] += f.x;
+    sum[1] += f.y;
+    sum[2] += f.z;
+    sum[3] += f.w;
+  }
+  if constexpr (kWhole) {
+    const int32_t e = p.row_expert[row];
+    if (e >= 0) {   // else a row of no group: 0, whatever its scale
+      const float x = p.x_scale[row], *w = p.w_scale + static_cast<int64_t>(e) * p.cols + col;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(__fmul_rn(static_cast<float>(sum[j]), j < count ? w[j] : 0.f), x);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = sum[j];
   }
   const int64_t at = row / p.inner * p.stride + row % p.inner * p.ld + col;
-  const int count = min(4, p.cols - col);
   if (p.f32) {
     float* o = static_cast<float*>(p.out) + at;
 #pragma unroll
@@ -1515,7 +1543,8 @@ __global__ void __launch_bounds__(256) grouped_join_kernel(const JoinParams p) {
   }
 }
 
-cudaError_t launch_join(const JoinParams& p, cudaStream_t st) {
+template <typename P>
+cudaError_t launch_join(const P& p, cudaStream_t st) {
   const int64_t blocks = (p.rows * (p.pitch / 4) + 255) / 256;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(blocks));
@@ -1526,7 +1555,7 @@ cudaError_t launch_join(const JoinParams& p, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, grouped_join_kernel, p);
+  return cudaLaunchKernelEx(&cfg, grouped_join_kernel<P>, p);
 }
 
 int check_groups(const char* what, int64_t rows, int32_t experts, const void* offsets, int32_t offsets_dtype) {
@@ -1558,7 +1587,7 @@ constexpr int64_t kL2Kept = 64 << 20;   // half of L2
 
 size_t int8_partial_bytes(int64_t rows, int32_t experts, int32_t n, int32_t k) {
   const int splits = rows_splits(rows, experts, n, (k + 1) / 2);
-  return splits > 1 ? splits * rows * pitch4(n) * sizeof(float) : 0;
+  return splits > 1 ? (splits * rows * pitch4(n) + rows) * sizeof(int32_t) : 0;   // the parts, and the rows' experts
 }
 
 bool int8_rows(const void* p, int64_t ld) { return tma_rows(p, ld, 1); }
@@ -1580,12 +1609,13 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
   q.w_scale = d.w_scale;
   q.splits = d.glu ? 1 : rows_splits(d.rows, d.experts, d.n, q.red);
   const int64_t pitch = pitch4(d.n);
-  if (d.workspace_bytes < q.splits * d.rows * pitch * sizeof(float) || !d.workspace) q.splits = 1;
+  if (d.workspace_bytes < int8_partial_bytes(d.rows, d.experts, d.n, d.k) || !d.workspace) q.splits = 1;
   const bool split = q.splits > 1, f32 = d.out_dtype == HEXMOE_F32, bf16 = d.out_dtype == HEXMOE_BF16;
   q.dst = split ? d.workspace : d.out;
   q.ld = split ? pitch : d.ld_out;
   q.stride_split = d.rows * pitch;
   q.f32 = split || f32; q.bf16 = bf16;
+  if (split) q.row_expert = static_cast<int32_t*>(d.workspace) + q.splits * d.rows * pitch;
   q.dev_err = dev_err;
   const PairShape shape = int8_shape(d.rows, d.experts, d.n);
   // Matrices that are read once each, and are more than L2 keeps for the next call, make no room among what it should
@@ -1627,8 +1657,9 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
                   : q.tma_out && q.f32 ? launch(std::integral_constant<int, kInt8F32>{})
                                        : launch(std::integral_constant<int, kInt8>{});
   if (e == cudaSuccess && split) {
-    JoinParams j{};
-    j.part = static_cast<const float*>(d.workspace);
+    Int8JoinParams j{};
+    j.part = d.workspace;
+    j.row_expert = q.row_expert; j.x_scale = d.x_scale; j.w_scale = d.w_scale;
     j.rows = d.rows; j.pitch = pitch; j.splits = q.splits; j.cols = d.n;
     j.out = d.out; j.ld = d.ld_out; j.inner = static_cast<int32_t>(d.rows);
     j.f32 = f32; j.bf16 = bf16; j.vec = d.ld_out % 4 == 0 && !off_by(d.out, 8);
@@ -1740,7 +1771,7 @@ int hexmoe_grouped_mm(const void* x, int64_t ld_x, const void* w, int64_t ld_w, 
                               : launch(std::integral_constant<int, kRowsK>{});
     if (e == cudaSuccess && split) {
       JoinParams j{};
-      j.part = static_cast<const float*>(workspace);
+      j.part = workspace;
       j.rows = rows; j.pitch = pitch; j.splits = q.splits; j.cols = width_out;
       j.out = out; j.ld = ld_out; j.inner = static_cast<int32_t>(rows);
       j.f32 = f32; j.bf16 = bf16; j.vec = ld_out % 4 == 0 && !off_by(out, 8);
@@ -1824,7 +1855,7 @@ int hexmoe_grouped_wgrad(const void* dy, int64_t ld_dy, const void* x, int64_t l
                                     : launch_pair<kWgrad, kMiddle>(q, tiles, sms, st);
     if (e == cudaSuccess && split) {
       JoinParams j{};
-      j.part = static_cast<const float*>(workspace);
+      j.part = workspace;
       j.rows = lines; j.pitch = pitch; j.splits = q.splits; j.cols = k;
       j.out = out; j.ld = ld_out; j.stride = stride_out; j.inner = n;
       j.f32 = f32; j.bf16 = bf16; j.accumulate = accumulate != 0;

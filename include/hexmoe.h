@@ -493,8 +493,9 @@ HEXMOE_API int hexmoe_quantize_rows(const void* x, int32_t x_dtype, int64_t ld_x
  * group e (offsets as for hexmoe_grouped_mm; NULL with one expert: all rows are
  * its).  x [rows, k]: I8 with x_scale [rows], or F32, BF16 or F16, quantized on the
  * way as hexmoe_quantize_rows does (x_scale is not read).  w I8 [experts, n, k], w_scale
- * f32 [experts, n].  Sums are exact (k at most 131071); out F32, BF16 or F16 is
- * rounded once, or split reductions of few rows once for each of their parts in f32.  8-bit
+ * f32 [experts, n].  Sums are exact (k at most 131071), however a reduction
+ * of few rows is split; one becomes f32 and is multiplied by w_scale and x_scale
+ * (each a rounding of 2^-24), then rounded to out's type, F32, BF16 or F16.  8-bit
  * rows begin and repeat on multiples of 16 bytes.  Rows of no group are set to
  * zero.  workspace (16-byte aligned): hexmoe_grouped_mm_int8_workspace_bytes,
  * needed where x is quantized here, elsewhere as for hexmoe_grouped_mm. */

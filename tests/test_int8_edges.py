@@ -76,3 +76,68 @@ def test_routing_weights_of_any_size():
     s13[:, 16:] = 2.0 ** -100
     got = int8.int8_moe(*(t.to(DEV) for t in (x, weights * 2.0 ** -60, ids, w13, s13, w2, s2)))
     assert ((got.double().cpu() - y.sum(1)).abs() <= 9 * 2.0 ** -24 * y.abs().sum(1)).all()
+
+
+# ------------------------------------------------------------------ split reductions
+def assert_exact(got, want, dtype):
+    """Sums are whole numbers, exact; one becomes f32, is multiplied by two scales (3 roundings of 2^-24) and rounded to
+    the type, whatever number of pairs its reduction was split over."""
+    f32 = 3.01 * 2.0 ** -24 * want.abs()
+    assert got.dtype == dtype and got.shape == want.shape
+    assert ((got.double().cpu() - want).abs() <= f32 + 1.01 * ROUND[dtype] * (want.abs() + f32) + HALF_STEP[dtype]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("rows,n,k", [(1, 512, 4096), (7, 776, 1624), (300, 512, 4096), (129, 24, 8000), (5, 2049, 33), (3, 7, 131071),
+                                      (900, 700, 640)])
+def test_sums_of_parts_are_whole_numbers(rows, n, k, dtype):
+    """Parts that cancel: halves of every sum with opposite signs, but for what the last values add."""
+    x, x_scale = int8_stack((rows, k), 21)
+    w, w_scale = int8_stack((n, k), 22)
+    half = k // 2
+    x[:, half:2 * half], w[:, half:2 * half] = x[:, :half], -w[:, :half].clamp(min=-127)
+    w[:, :half] = w[:, :half].clamp(min=-127)
+    w[:, :3] += (w[:, :3] < 100).to(torch.int8)
+    x_scale, w_scale = x_scale * 0.01, w_scale * 0.01     # fp16 holds the results
+    want, mass = product(x, x_scale, w[None], w_scale[None], torch.tensor([0, rows]), rows)
+    assert k < 100 or float(want.abs().median()) < 1e-3 * float(mass.median())
+    got = int8.grouped_mm_int8(x.to(DEV), w.to(DEV), w_scale.to(DEV), x_scale=x_scale.to(DEV), out_dtype=dtype)
+    assert_exact(got, want, dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("sizes,first,n,k", [([3, 0, 20, 5, 1], 4, 200, 4096), ([40, 1, 90], 0, 136, 2048), ([1] * 40, 2, 64, 1500)], ids=str)
+def test_rows_alone_and_among_others(sizes, first, n, k, dtype):
+    """The same row in batches that split differently, in groups with gaps before and behind: the same bits."""
+    rows = first + sum(sizes) + 3
+    x, x_scale = int8_stack((rows, k), 23)
+    w, w_scale = int8_stack((len(sizes), n, k), 24)
+    if first:
+        x_scale[:first] = float("nan")
+    x_scale[-3:] = float("inf")
+    off = offsets_of(sizes, first)
+    xd, sd, wd, ws = x.to(DEV), x_scale.to(DEV), w.to(DEV), w_scale.to(DEV)
+    got = int8.grouped_mm_int8(xd, wd, ws, off.to(DEV), x_scale=sd, out_dtype=dtype)
+    want, _ = product(x, torch.nan_to_num(x_scale, 0, 0, 0), w, w_scale, off, rows)
+    assert_exact(got, want, dtype)
+    for e, size in enumerate(sizes):
+        part = slice(int(off[e]), int(off[e + 1]))
+        many = torch.cat([xd[part]] * 30), torch.cat([sd[part]] * 30)
+        assert torch.equal(int8.grouped_mm_int8(xd[part], wd[e], ws[e], x_scale=sd[part], out_dtype=dtype), got[part])
+        assert torch.equal(int8.grouped_mm_int8(many[0], wd[e], ws[e], x_scale=many[1], out_dtype=dtype)[:size], got[part])
+
+
+@pytest.mark.gpu
+def test_matrices_that_stream_through_l2_bit_for_bit():
+    """Matrices of more than 64 MB read once, and each of them alone, which stays in L2."""
+    E, n, k = 40, 1024, 2048
+    w = torch.randint(-127, 128, (E, n, k), dtype=torch.int8, device=DEV)
+    ws = torch.rand(E, n, device=DEV)
+    x = normal((80, k), BF16, 120).to(DEV)
+    got = int8.grouped_mm_int8(x, w, ws, torch.arange(0, 81, 2, dtype=torch.int32, device=DEV))
+    for e in range(E):
+        rows = slice(2 * e, 2 * e + 2)
+        one = int8.grouped_mm_int8(x[rows], w[e:e + 1], ws[e:e + 1], torch.tensor([0, 2], device=DEV))
+        assert torch.equal(one, got[rows])
