@@ -67,8 +67,9 @@ def route(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bias: torch
     scale        a factor on the weights
 
     The experts come in the order of their scores, bias included (without a bias: of their logits), ties by the
-    lower id, as 64-bit arithmetic decides.  An expert whose logit is -inf is masked: it is taken after all others
-    of the open groups, with weight 0; a token with nothing else has weights 0.  NaN logits make NaN weights of
+    lower id, as 64-bit arithmetic decides.  An expert whose logit is -inf is masked: its score is 0,
+    which is also what its group is valued by (with its bias), and it is taken after all others of the open groups; a
+    token with nothing else there has weights 0.  NaN logits make NaN weights of
     valid ids."""
     res = _call.route(logits, k, SCORING.get(scoring), bias, groups, topk_groups, group_top, renormalize, scale)
     if res is not None:

@@ -3,6 +3,7 @@
 //   s = softmax(l) or sigmoid(l);   c = s + b with a balancing bias, else l (which has the scores' order)
 //   a group's value: the sum of its 1 or 2 largest s + b; the topk_groups groups of largest value are open
 //   ids: the k largest c of the open groups;   w = scale s[ids], over their sum where renormalised
+//   l = -inf masks an expert: s = 0, which is what its group is valued by; among the open groups' experts it comes last
 //
 // Ties go to the lower id.  A warp takes a token; lane l holds experts l NI .. l NI + NI - 1, so that lanes in order are
 // experts in order.  Bound by latency and issue, not by bytes: a token's row is a few hundred.  8192 tokens of 256 experts
@@ -193,7 +194,7 @@ __device__ double exact_sum(const RouteParams& p, const T* row, float largest) {
   }
   return warp_sum(part);
 }
-// s + b of one expert in f64.
+// s + b of one expert in f64; a masked one's s is 0.
 template <typename T, bool SIGMOID>
 __device__ double exact_value(const RouteParams& p, const T* row, int e, float largest, double sum) {
   const float l = widen(row[e]);
@@ -203,8 +204,7 @@ __device__ double exact_value(const RouteParams& p, const T* row, int e, float l
     const double x = exp(SIGMOID ? (d < 0 ? d : -d) : d - static_cast<double>(largest));
     s = SIGMOID ? (d < 0 ? x : 1.0) / (1.0 + x) : x / sum;
   }
-  if (!p.bias) return s;
-  return l == -INFINITY ? -INFINITY : s + static_cast<double>(p.bias[e]);
+  return p.bias ? s + static_cast<double>(p.bias[e]) : s;
 }
 
 __device__ __forceinline__ void add_top(uint32_t key, uint32_t& first, uint32_t& second) {
@@ -442,14 +442,14 @@ __device__ __forceinline__ int32_t choose(const RouteParams& p, const T* row, co
     }
     wide = __reduce_max_sync(kAll, wide);
     float widest = __uint_as_float(wide);
-    if (max(wide, __reduce_max_sync(kAll, most)) < 0x7f800000u) {
+    const bool finite = max(wide, __reduce_max_sync(kAll, most)) < 0x7f800000u;
+    if (finite) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) key[i] = full || e0 + i < p.experts ? plain_key(c[i]) : 0u;
     } else {
       widest = 0.f;
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        if (p.bias && l[i] == -INFINITY) c[i] = -INFINITY;
         key[i] = e0 + i < p.experts ? key_of(c[i]) : 0u;
         const float size = fabsf(c[i]);
         widest = fmaxf(widest, size < INFINITY ? size : 0.f);
@@ -480,6 +480,11 @@ __device__ __forceinline__ int32_t choose(const RouteParams& p, const T* row, co
           if (!(open >> ((e0 + i) / per & 31) & 1)) key[i] = 0;
       }
     }
+    if (!finite) {   // what is masked, behind all others of the open groups
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        if (l[i] == -INFINITY && key[i] > kMasked) key[i] = kMasked;
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < NI; ++i) key[i] = e0 + i < p.experts ? key_of(l[i]) : 0u;
@@ -489,7 +494,9 @@ __device__ __forceinline__ int32_t choose(const RouteParams& p, const T* row, co
   if (got.count > 32) return choose_exact<T, SIGMOID>(p, row, largest);
   // in order of their values in f64, an expert a lane
   const double sum = exact_sum<T, SIGMOID>(p, row, largest);
-  const uint64_t mine = lane < got.count ? key_of(exact_value<T, SIGMOID>(p, row, got.id, largest, sum)) : 0ull;
+  uint64_t mine = 0;
+  if (lane < got.count)
+    mine = key_of(widen(row[got.id]) == -INFINITY ? -INFINITY : exact_value<T, SIGMOID>(p, row, got.id, largest, sum));
   int place = 0;
 #pragma unroll 1
   for (int j = 0; j < got.count; ++j) {
@@ -546,6 +553,9 @@ __device__ int32_t choose_exact(const RouteParams& p, const T* row, float larges
     for (int i = 0; i < held; ++i)
       if (e0 + i < p.experts && !(open >> (e0 + i) / per & 1)) key[i] = 0;
   }
+#pragma unroll 1
+  for (int i = 0; i < held; ++i)   // what is masked, behind all others
+    if (key[i] && widen(row[e0 + i]) == -INFINITY) key[i] = key_of(-static_cast<double>(INFINITY));
   int32_t id = 0;
 #pragma unroll 1
   for (int j = 0; j < p.topk; ++j) {

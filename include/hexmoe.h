@@ -455,8 +455,8 @@ enum hexmoe_scoring { HEXMOE_SOFTMAX = 0, HEXMOE_SIGMOID = 1 };
  * open groups in order, ties to the lower id (groups as well), as exact
  * arithmetic decides.  topk_weights f32 [tokens, topk]: scale * s, over the sum of
  * the token's chosen s with renormalize != 0.  A logit of -infinity masks its
- * expert: score 0, taken after all others of the open groups; a token with
- * nothing else has weights 0.  NaN logits make NaN weights of valid ids.  At most
+ * expert: score 0 (its group is valued by that, and the bias), taken after all
+ * others of the open groups; a token with nothing else there has weights 0.  NaN logits make NaN weights of valid ids.  At most
  * 2048 experts, topk at most 32 and at most the experts of topk_groups groups. */
 HEXMOE_API int hexmoe_route(const void* logits, int32_t logits_dtype, int64_t ld_logits, int64_t tokens,
                             int32_t num_experts, int32_t topk, int32_t scoring, const float* bias, int32_t groups,

@@ -1,0 +1,81 @@
+"""The router where logits are masked, no numbers or far apart: against 64-bit restatements written from the definition."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+from test_experts import BF16, DEV, F16, F32, device_word, normal  # noqa: F401
+from test_router import INF, assert_weights, scores_of, weights_of
+
+from blackhole_b200 import router
+
+
+# ------------------------------------------------------------------ masked experts in groups
+def masked_choice(logits, k, scoring, bias, groups, topk_groups, group_top):
+    """ids [T, k] from the definition: a group's value is the sum of its group_top largest s + b, where a masked expert's s
+    is 0; in the open groups masked experts come after all others.  And the smallest distance a decision rested on."""
+    T, E = logits.shape
+    per, scores = E // groups, scores_of(logits, scoring)
+    biased = scores + (0.0 if bias is None else bias.double())
+    ids, gap = [], INF
+    for t in range(T):
+        values = [sum(sorted(biased[t, g * per:(g + 1) * per].tolist())[-group_top:]) for g in range(groups)]
+        order = sorted(range(groups), key=lambda g: (-values[g], g))
+        rank = [(float(logits[t, e]) == -INF, -float(logits[t, e] if bias is None else biased[t, e]), e)
+                for g in order[:topk_groups] for e in range(g * per, (g + 1) * per)]
+        rank = sorted((m, 0.0 if m else v, e) for m, v, e in rank)
+        steps = [values[order[topk_groups - 1]] - values[order[topk_groups]]] if topk_groups < groups else []
+        if bias is not None:
+            steps += [b[1] - a[1] for a, b in zip(rank[:k], rank[1:k + 1]) if not b[0]]
+        gap = min([gap] + [s for s in steps if s])
+        ids.append([e for _, _, e in rank[:k]])
+    return torch.tensor(ids), gap
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("bias", [None, "zeros", "some", "large"])
+@pytest.mark.parametrize("group_top", [1, 2])
+@pytest.mark.parametrize("E,k,groups,open_groups", [(4, 1, 2, 1), (24, 3, 2, 1), (40, 4, 4, 2), (96, 8, 8, 4), (256, 8, 8, 4), (500, 16, 20, 7)])
+def test_masked_experts_in_groups(E, k, groups, open_groups, group_top, bias, scoring):
+    """Seven of ten experts masked, groups with one expert left, groups with none, and rows with next to none."""
+    g = torch.Generator().manual_seed(E + k)
+    logits = normal((40, E), F32, E, 1.5)
+    logits[torch.rand(40, E, generator=g) < 0.7] = -INF
+    logits[1:6, :E // groups] = -INF
+    logits[2] = -INF
+    logits[3] = -INF
+    logits[3, E - 1] = 5.0
+    logits[4, E // groups:] = -INF
+    b = None if bias is None else torch.zeros(E) if bias == "zeros" else normal((E,), F32, 3, 0.1 if bias == "some" else 3.0)
+    how = dict(scoring=scoring, groups=groups, topk_groups=open_groups, group_top=group_top)
+    want, gap = masked_choice(logits, k, bias=b, **how)
+    assert gap > 1e-13
+    for renormalize in (True, False):
+        weights, ids = router.route(logits.to(DEV), k, bias=None if b is None else b.to(DEV), renormalize=renormalize, **how)
+        assert torch.equal(ids.cpu().long(), want)
+        assert_weights(weights, weights_of(logits, want, scoring, renormalize), logits[:1], 1.0)
+    if bias == "zeros":   # a bias of nothing changes nothing
+        assert torch.equal(router.route(logits.to(DEV), k, **how)[1].cpu().long()[3], want[3])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_masked_experts_in_groups_nearer_than_f32_tells(scoring):
+    """Groups' values that only 64 bits tell apart, with masked experts in every group, and more equal ones than lanes."""
+    E, k, how = 64, 6, dict(scoring=scoring, groups=8, topk_groups=3, group_top=2)
+    logits = normal((1, E), F32, 5, 1.0) + normal((200, E), F32, 6, 1e-7)
+    logits[:, ::3] = -INF
+    logits[7, 1::8], logits[7, 2::8] = -INF, -INF
+    bias = (0.9 - scores_of(logits[:1], scoring)[0]).float()
+    want, gap = masked_choice(logits, k, bias=bias, **how)
+    assert gap > 2e-15
+    assert torch.equal(router.route(logits.to(DEV), k, bias=bias.to(DEV), **how)[1].cpu().long(), want)
+    flat = torch.zeros(3, 512)
+    flat[0, ::2], flat[1, 5:], flat[2, 40:90] = -INF, -INF, -INF
+    for bias in (None, torch.zeros(512), torch.full((512,), 0.25)):
+        want, _ = masked_choice(flat, 20, scoring, bias, 4, 2, 2)
+        got = router.route(flat.to(DEV), 20, scoring=scoring, bias=None if bias is None else bias.to(DEV), groups=4, topk_groups=2)[1]
+        assert torch.equal(got.cpu().long(), want)
