@@ -67,10 +67,9 @@ def route(logits: torch.Tensor, k: int, *, scoring: str = "softmax", bias: torch
     scale        a factor on the weights
 
     The experts come in the order of their scores, bias included (without a bias: of their logits), ties by the
-    lower id, as 64-bit arithmetic decides.  An expert whose logit is -inf is masked: its score is 0,
-    which is also what its group is valued by (with its bias), and it is taken after all others of the open groups; a
-    token with nothing else there has weights 0.  NaN logits make NaN weights of
-    valid ids."""
+    lower id, as 64-bit arithmetic decides.  An expert whose logit is -inf is masked: its score is 0, which is
+    also what its group is valued by (with its bias), and it is taken after all others of the open groups; a token with
+    nothing else there has weights 0.  A row with a NaN (softmax: or +inf) has NaN weights of valid ids."""
     res = _call.route(logits, k, SCORING.get(scoring), bias, groups, topk_groups, group_top, renormalize, scale)
     if res is not None:
         return res
@@ -100,7 +99,8 @@ def route_backward(dweights: torch.Tensor, logits: torch.Tensor, ids: torch.Tens
                    renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
     """The gradient of route's weights for the logits: dlogits [T, E] in their type, from dweights float32 [T, k]
     and the ids [T, k] (int32 or int64) that route gave, with the same scoring, renormalize and scale.  The choice
-    itself (bias, groups) has no gradient.  ids outside 0..E-1 have no part.  Not differentiable itself."""
+    itself (bias, groups) has no gradient.  ids outside 0..E-1 have no part.  A softmax's row with a NaN or +inf has a
+    NaN gradient; with sigmoid scores only the chosen logits are looked at.  Not differentiable itself."""
     dlogits = _call.route_backward(dweights, logits, ids, SCORING.get(scoring), renormalize, scale)
     if dlogits is not None:
         return dlogits

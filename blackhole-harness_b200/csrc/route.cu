@@ -149,6 +149,15 @@ __device__ __forceinline__ float largest_of(const float (&l)[NI]) {   // ignorin
   for (int i = 0; i < NI; ++i) m = fmaxf(m, l[i]);
   return warp_max(m);
 }
+// Whether a row has no scores: it holds a NaN or, under a softmax, +inf (`largest`).  Its weights are all NaN, and a softmax's
+// gradients: of the chosen logits alone neither would show where the NaN was not chosen.
+template <int NI, bool SIGMOID>
+__device__ __forceinline__ bool undefined(const float (&l)[NI], float largest) {
+  bool nan = !SIGMOID && largest == INFINITY;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) nan |= l[i] != l[i];
+  return __any_sync(kAll, nan);
+}
 // e^x and 1 / x to 2 units in the last place, and the rounding of x log2 e (|x| 2^-24 of the result).
 __device__ __forceinline__ float fast_exp(float x) {
   float r;
@@ -601,6 +610,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
   const T* row = static_cast<const T*>(p.logits) + t * p.ld;
   load_row(p, row, -INFINITY, l);
   const float largest = SIGMOID ? 0.f : largest_of(l);
+  const bool no_scores = undefined<NI, SIGMOID>(l, largest);
   const int32_t id = choose<T, NI, SIGMOID>(p, row, l, largest, found[threadIdx.x / 32],
                                             reinterpret_cast<uint32_t*>(keys) + threadIdx.x / 32 * (p.experts + 32));
   const bool used = lane < p.topk;
@@ -618,7 +628,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
     w = mine == -INFINITY && sum == sum ? 0.f : expf(mine - largest) / sum;
   }
   if (used) {
-    p.weights[t * p.topk + lane] = w * p.scale;
+    p.weights[t * p.topk + lane] = no_scores ? __uint_as_float(0x7fc00000u) : w * p.scale;
     static_cast<int32_t*>(p.ids)[t * p.topk + lane] = id;
   }
 }
@@ -631,7 +641,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
 //   sigmoid                dl_j = d_j s_j (1 - s_j)
 // d_j - dot is summed as r_i (d_j - d_i): a share near 1 leaves no cancellation.  The row is written as what every
 // expert has (0, or -s_e sum) and the chosen ones' values over it, by the same warp.  An expert that stands more than
-// once among the ids has the sum of its places; ids outside 0..E-1 have no part.
+// once among the ids has the sum of its places; ids outside 0..E-1 have no part.  A softmax's row with a NaN or +inf has a
+// gradient of NaN, renormalised or not; a sigmoid's chosen logits stand for themselves.
 template <typename T, int NI, bool SIGMOID>
 __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const RouteParams p) {
   const int lane = threadIdx.x % 32;
@@ -678,6 +689,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
     }
     value = score * (all - dot);
   } else {
+    float l[NI];
+    if constexpr (!SIGMOID) load_row(p, row, -INFINITY, l);   // only to see whether they are numbers
     if (p.vec) {
       for (int e = lane; e < p.experts * static_cast<int>(sizeof(T)) / 16; e += 32) reinterpret_cast<uint4*>(out)[e] = make_uint4(0, 0, 0, 0);
     } else {
@@ -699,6 +712,13 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
       if (__shfl_sync(kAll, id, j) == id) all += vj;
     }
     value = all;
+    if constexpr (!SIGMOID) {
+      if (undefined<NI, SIGMOID>(l, largest_of(l))) {
+        __syncwarp();   // over the zeros
+        for (int e = lane; e < p.experts; e += 32) out[e] = narrow<T>(__uint_as_float(0x7fc00000u));
+        return;
+      }
+    }
   }
   __syncwarp();   // the row's zeros (or common part) come before the chosen ones' values
   if (used) out[id] = narrow<T>(value);

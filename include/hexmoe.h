@@ -456,7 +456,8 @@ enum hexmoe_scoring { HEXMOE_SOFTMAX = 0, HEXMOE_SIGMOID = 1 };
  * arithmetic decides.  topk_weights f32 [tokens, topk]: scale * s, over the sum of
  * the token's chosen s with renormalize != 0.  A logit of -infinity masks its
  * expert: score 0 (its group is valued by that, and the bias), taken after all
- * others of the open groups; a token with nothing else there has weights 0.  NaN logits make NaN weights of valid ids.  At most
+ * others of the open groups; a token with nothing else there has weights 0.  A
+ * row with a NaN (softmax: or +infinity) has NaN weights of valid ids.  At most
  * 2048 experts, topk at most 32 and at most the experts of topk_groups groups. */
 HEXMOE_API int hexmoe_route(const void* logits, int32_t logits_dtype, int64_t ld_logits, int64_t tokens,
                             int32_t num_experts, int32_t topk, int32_t scoring, const float* bias, int32_t groups,
@@ -467,7 +468,8 @@ HEXMOE_API int hexmoe_route(const void* logits, int32_t logits_dtype, int64_t ld
  * num_experts] (logits_dtype, row stride ld_dlogits) from dweights f32 and
  * topk_ids (ids_dtype) [tokens, topk].  The choice has no gradient.  An expert
  * that stands among a token's ids more than once has the sum of its places; ids
- * outside 0..num_experts-1 have no part. */
+ * outside 0..num_experts-1 have no part.  A softmax's row with a NaN or +infinity
+ * has a NaN gradient; with sigmoid scores only the chosen logits are looked at. */
 HEXMOE_API int hexmoe_route_backward(const float* dweights, const void* logits, int32_t logits_dtype,
                                      int64_t ld_logits, int64_t tokens, int32_t num_experts, int32_t topk,
                                      const void* topk_ids, int32_t ids_dtype, int32_t scoring, int32_t renormalize,

@@ -79,3 +79,48 @@ def test_masked_experts_in_groups_nearer_than_f32_tells(scoring):
         want, _ = masked_choice(flat, 20, scoring, bias, 4, 2, 2)
         got = router.route(flat.to(DEV), 20, scoring=scoring, bias=None if bias is None else bias.to(DEV), groups=4, topk_groups=2)[1]
         assert torch.equal(got.cpu().long(), want)
+
+
+# ------------------------------------------------------------------ logits that are no numbers
+@pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("E,groups", [(20, 1), (20, 4), (96, 1), (256, 8), (1000, 10)])
+def test_one_logit_that_is_no_number(E, groups, renormalize, scoring):
+    """A row with a NaN, or under a softmax with +inf, whose scores are not defined: weights are all NaN, wherever it stands,
+    ids valid and distinct; other rows are not touched."""
+    logits = normal((12, E), F32, 12).index_fill(0, torch.tensor([3]), 2.0)
+    bad = {1: (E - 1, math.nan), 3: (E // 2, math.nan), 4: (0, math.nan), 8: (E - 2, INF), 9: (1, INF)}
+    clean = logits.clone()
+    for t, (e, v) in bad.items():
+        logits[t, e] = v
+    logits[4, 1:5] = -INF
+    rows = torch.tensor([t for t, (_, v) in bad.items() if v != INF or scoring == "softmax"])
+    rest = torch.tensor([t for t in range(12) if t not in bad])
+    for bias in (None, torch.zeros(E, device=DEV), normal((E,), F32, 13, 0.1).to(DEV)):
+        how = dict(scoring=scoring, bias=bias, groups=groups, topk_groups=min(2, groups), renormalize=renormalize)
+        weights, ids = router.route(logits.to(DEV), 5, **how)
+        assert weights.cpu()[rows].isnan().all() and 0 <= int(ids.min()) and int(ids.max()) < E
+        assert all(len(set(row)) == 5 for row in ids.tolist())
+        want, want_ids = router.route(clean.to(DEV), 5, **how)
+        assert torch.equal(weights.cpu()[rest], want.cpu()[rest]) and torch.equal(ids.cpu()[rest], want_ids.cpu()[rest])
+        if scoring == "sigmoid":   # +inf is a score of 1
+            top = (ids.cpu()[8] == E - 2).nonzero()
+            assert weights[8:10].isfinite().all() and (bias is not None or groups > 1 or top.tolist() == [[0]])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=str)
+@pytest.mark.parametrize("renormalize", [False, True])
+@pytest.mark.parametrize("E", [20, 96, 256, 1000])
+def test_gradient_of_a_row_with_one_logit_that_is_no_number(E, renormalize, dtype):
+    """Softmax: the whole row's gradient is NaN, as the formula's, also where the NaN (or +inf) was not chosen."""
+    logits = normal((9, E), dtype, 14)
+    ids = torch.arange(3).expand(9, 3) + torch.arange(9)[:, None]
+    d = normal((9, 3), F32, 15).to(DEV)
+    want = router.route_backward(d, logits.to(DEV), ids.to(DEV), renormalize=renormalize)
+    logits[2, E - 1], logits[5, 18], logits[6, 6] = math.nan, INF, math.nan
+    got = router.route_backward(d, logits.to(DEV), ids.to(DEV), renormalize=renormalize)
+    bad = torch.tensor([2, 5, 6])
+    rest = torch.tensor([0, 1, 3, 4, 7, 8])
+    assert got.cpu()[bad].isnan().all() and torch.equal(got.cpu()[rest], want.cpu()[rest])
