@@ -639,7 +639,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
 //   renormalised sigmoid   dl_j = r_j (1 - s_j) (d_j - dot)
 //   softmax                dl_e = s_e (d_e - sum_j s_j d_j), d_e = 0 where not chosen
 //   sigmoid                dl_j = d_j s_j (1 - s_j)
-// d_j - dot is summed as r_i (d_j - d_i): a share near 1 leaves no cancellation.  The row is written as what every
+// d_j - dot is summed as r_i (d_j - d_i), for the softmax s_i (d_j - d_i) over the chosen experts and d_j times what the
+// others' scores sum to: a share or score near 1 leaves no cancellation.  The row is written as what every
 // expert has (0, or -s_e sum) and the chosen ones' values over it, by the same warp.  An expert that stands more than
 // once among the ids has the sum of its places; ids outside 0..E-1 have no part.  A softmax's row with a NaN or +inf has a
 // gradient of NaN, renormalised or not; a sigmoid's chosen logits stand for themselves.
@@ -651,13 +652,13 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
   if (t >= p.tokens) return;
   const T* row = static_cast<const T*>(p.logits) + t * p.ld;
   T* out = static_cast<T*>(p.dlogits) + t * p.ld_d;
-  int64_t id = -1 - lane;   // no two alike where there is none
+  int32_t id = -1 - lane;   // no two alike where there is none
   float d = 0.f;
   if (lane < p.topk) {
     const int64_t v = p.ids64 ? static_cast<const int64_t*>(p.ids)[t * p.topk + lane]
                               : static_cast<const int32_t*>(p.ids)[t * p.topk + lane];
     if (v >= 0 && v < p.experts) {
-      id = v;
+      id = static_cast<int32_t>(v);
       d = p.weights[t * p.topk + lane] * p.scale;
     }
   }
@@ -683,11 +684,22 @@ __global__ void __launch_bounds__(kRouteThreads) route_backward_kernel(const Rou
     for (int i = 0; i < NI; ++i)
       if (lane + 32 * i < p.experts) out[lane + 32 * i] = narrow<T>(-(s[i] * inv) * dot);
     float all = 0.f;   // of this expert's places
+    bool again = false;   // it stands in a place before this one
+    std::conditional_t<(NI > 32), uint64_t, uint32_t> chosen = 0;   // of the experts s holds
     for (int j = 0; j < p.topk; ++j) {
       const float dj = __shfl_sync(kAll, d, j);
-      if (__shfl_sync(kAll, id, j) == id) all += dj;
+      const int32_t other = __shfl_sync(kAll, id, j);
+      all += other == id ? dj : 0.f;
+      again |= other == id && j < lane;
+      if (other >= 0 && (other & 31) == lane) chosen |= decltype(chosen){1} << (other >> 5);
     }
-    value = score * (all - dot);
+    float rest = 0.f, away = 0.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) rest += chosen >> i & 1 ? 0.f : s[i];
+    rest = warp_sum(rest) * inv;
+    const float once = again ? 0.f : score;
+    for (int j = 0; j < p.topk; ++j) away += __shfl_sync(kAll, once, j) * (all - __shfl_sync(kAll, all, j));
+    value = score * (away + all * rest);
   } else {
     float l[NI];
     if constexpr (!SIGMOID) load_row(p, row, -INFINITY, l);   // only to see whether they are numbers

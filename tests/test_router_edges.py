@@ -124,3 +124,39 @@ def test_gradient_of_a_row_with_one_logit_that_is_no_number(E, renormalize, dtyp
     bad = torch.tensor([2, 5, 6])
     rest = torch.tensor([0, 1, 3, 4, 7, 8])
     assert got.cpu()[bad].isnan().all() and torch.equal(got.cpu()[rest], want.cpu()[rest])
+
+
+# ------------------------------------------------------------------ gradients next to a score of 1
+def gradient_and_mass(logits, ids, d, scale):
+    """The plain softmax's gradient in 64 bits without a difference of near values, dl_e = s_e sum_i s_i (a_e - a_i) with a
+    the sum of an expert's places (0 where not chosen), and the sum of the magnitudes of its terms."""
+    s = torch.softmax(logits.double(), 1)
+    a = torch.zeros_like(s).scatter_add_(1, ids, d.double() * scale)
+    away = s[:, None, :] * (a[:, :, None] - a[:, None, :])
+    return s * away.sum(2), s * away.abs().sum(2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gap", [0, 5, 10, 15, 17, 20, 30, 60])
+@pytest.mark.parametrize("E,k", [(1, 1), (2, 1), (8, 1), (8, 2), (33, 4), (96, 8), (256, 1), (1000, 32)])
+def test_softmax_gradient_next_to_a_score_of_one(E, k, gap):
+    """One expert ahead of all others, among the chosen ones or not, and ids that stand twice.  A term s_e s_i (a_e - a_i) is
+    off by its two scores (exponents rounded, |l - m| 2^-24; exponentials and sums, E / 32 + 24 units) and its sum of k + E / 32
+    + 5 additions; twice over."""
+    T = 9
+    logits, d = normal((T, E), F32, E + k), normal((T, k), F32, 21)
+    ids = torch.stack([torch.randperm(E, generator=torch.Generator().manual_seed(t))[:k] for t in range(T)])
+    logits.scatter_add_(1, ids[:, :1], torch.full((T, 1), float(gap)))
+    ids[3] = ids[3, 0]                 # one expert in every place
+    ids[4] = ids[4].flip(0)
+    if k > 1:
+        ids[5, 0] = ids[5, 1]          # the one ahead is not chosen
+        ids[6, 1] = ids[6, 0]
+    want, mass = gradient_and_mass(logits, ids, d, 1.5)
+    got = router.route_backward(d.to(DEV), logits.to(DEV), ids.to(DEV), renormalize=False, scale=1.5).double().cpu()
+    span = float(logits.max() - logits.min())
+    bound = 2 * (2 * (span + E / 32 + 24) + k + E / 32 + 5) * 2.0 ** -24 * mass + 2.0 ** -120
+    assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / mass.clamp(min=1e-300)).max())
+    ref = logits.double().requires_grad_()
+    (torch.softmax(ref, 1).gather(1, ids) * 1.5 * d.double()).sum().backward()
+    assert ((want - ref.grad).abs() <= 2.0 ** -48 * d.double().abs().sum(1, keepdim=True)).all()
