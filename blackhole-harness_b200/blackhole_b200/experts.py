@@ -17,7 +17,8 @@ Rows lie in expert order: group e is rows offsets[e] .. offsets[e + 1] - 1
 sm_100 device; there is no CPU path.  Calls run on the current stream of the
 inputs' device, synchronise nothing and can be captured in CUDA graphs.
 
-grouped_mm, grouped_wgrad, swiglu and expert_mlp are differentiable (once).  What is written
+grouped_mm, grouped_wgrad, swiglu and expert_mlp are differentiable (once, and backwards only:
+tensors with a tangent of forward-mode differentiation are refused).  What is written
 into an `out` stays outside autograd's graph, as do swiglu_backward and clip_grad_norm, and
 an `out` overlaps no input (swiglu_backward's may be h).
 """
@@ -29,6 +30,7 @@ from array import array
 from operator import attrgetter
 
 import torch
+from torch.autograd import forward_ad
 
 from blackhole_b200 import _lib
 from blackhole_b200.hex_moe import _DT, _aligned, _ptr, align, combine_rows
@@ -115,8 +117,12 @@ def _output(out, shape: tuple, like: torch.Tensor, out_dtype, what: str) -> torc
 
 
 def _recorded(*tensors) -> bool:
-    """Whether autograd is to see the call."""
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether autograd is to see the call: an input requires a gradient, or has a tangent of forward-mode
+    differentiation (which nothing here computes: the autograd functions say so)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def _workspace(nbytes: int, like: torch.Tensor) -> tuple[torch.Tensor | None, int]:

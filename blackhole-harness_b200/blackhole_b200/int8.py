@@ -13,7 +13,8 @@ Stacks come from 16-bit ones (hex_moe.dequant_all, or what expert_mlp has traine
     out = int8_moe(x, *router.route(logits, 8), *w13, *w2)
 
 Inputs must be CUDA tensors on an sm_100 device; there is no CPU path.  Calls run on the current stream of the
-inputs' device, synchronise nothing and can be captured in CUDA graphs.  Nothing here is differentiable.
+inputs' device, synchronise nothing and can be captured in CUDA graphs.  Nothing here is differentiable: the products
+refuse inputs that require a gradient or have a tangent; what quantize_rows returns has neither.
 """
 
 from __future__ import annotations

@@ -15,6 +15,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
@@ -47,8 +48,11 @@ int code_of(at::ScalarType t) {
 bool here(const at::Tensor& t) {
   return t.is_cuda() && t.layout() == at::kStrided && t.get_device() == c10::cuda::current_device();
 }
-// Autograd is to see a call with this input.
-bool recorded(const at::Tensor& t) { return c10::GradMode::is_enabled() && t.requires_grad(); }
+// Autograd is to see a call with this input: it requires a gradient, or has a tangent of forward-mode differentiation.
+bool recorded(const at::Tensor& t) {
+  return (c10::GradMode::is_enabled() && t.requires_grad()) ||
+         (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined());
+}
 void* stream_of(const at::Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 bool matrix(const at::Tensor& t) { return t.dim() == 2 && t.stride(1) == 1 && t.stride(0) >= t.size(1); }
 
