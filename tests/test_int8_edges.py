@@ -141,3 +141,20 @@ def test_matrices_that_stream_through_l2_bit_for_bit():
         rows = slice(2 * e, 2 * e + 2)
         one = int8.grouped_mm_int8(x[rows], w[e:e + 1], ws[e:e + 1], torch.tensor([0, 2], device=DEV))
         assert torch.equal(one, got[rows])
+
+
+# ------------------------------------------------------------------ gates far below zero
+@pytest.mark.gpu
+def test_gates_far_below_zero():
+    """silu is a normal f32 number down to gates of -91, where 1 + e^-gate is none; one column of the activation, so that
+    its 8-bit value is 127 whatever its error (a fast exponential's, 1.2 |g| + 2 units of 2^-23, twice over)."""
+    gates = torch.tensor([-1.0, -40, -80, -87, -88, -88.5, -89, -90, -91])
+    x, w13, w2 = torch.zeros(1, 16), torch.zeros(9, 32, 16, dtype=torch.int8), torch.zeros(9, 16, 16, dtype=torch.int8)
+    x[0, 0], w13[:, 0, 0], w13[:, 16, 0], w2[:, :, 0] = 127, 1, 1, 1
+    s13, s2 = torch.ones(9, 32), torch.ones(9, 16)
+    s13[:, 0], s13[:, 16] = gates / 127, 2.0 ** 20 / 127
+    weights, ids = torch.ones(9, 1), torch.arange(9)[:, None]
+    g = (s13[:, 0].double() * 127)
+    want = g * torch.sigmoid(g) * (s13[:, 16].double() * 127)
+    got = int8.int8_moe(*(t.to(DEV) for t in (x.expand(9, 16), weights, ids, w13, s13, w2, s2))).double().cpu()
+    assert ((got - want[:, None]).abs() <= (16 + 3 * g.abs()[:, None]) * 2.0 ** -23 * want.abs()[:, None]).all(), (got[:, 0], want)
