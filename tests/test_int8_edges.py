@@ -158,3 +158,55 @@ def test_gates_far_below_zero():
     want = g * torch.sigmoid(g) * (s13[:, 16].double() * 127)
     got = int8.int8_moe(*(t.to(DEV) for t in (x.expand(9, 16), weights, ids, w13, s13, w2, s2))).double().cpu()
     assert ((got - want[:, None]).abs() <= (16 + 3 * g.abs()[:, None]) * 2.0 ** -23 * want.abs()[:, None]).all(), (got[:, 0], want)
+
+
+# ------------------------------------------------------------------ groups and plans
+def clamped(offsets, rows):
+    """The groups that any offsets stand for: each entry within 0..rows and no less than the one before."""
+    return torch.cummax(offsets.clamp(0, rows), 0).values
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [32, 4096])
+@pytest.mark.parametrize("at", [0, 1, 30, 31, 32, 33, 63, 64, 65, 69, 70])
+def test_offsets_that_are_none(at, k):
+    """One bad entry among 70 groups, before, at and behind a step of 32: the clamped groups' products, and the error word."""
+    from blackhole_b200.hex_moe import device_status
+    E, n, rows = 70, 48, 210
+    x, x_scale = int8_stack((rows, k), 31)
+    w, w_scale = int8_stack((E, n, k), 32)
+    args = x.to(DEV), w.to(DEV), w_scale.to(DEV)
+    for bad in (-7, 500, 2 ** 40, 0, 209):
+        off = torch.arange(0, rows + 1, 3)
+        if int(off[at]) == bad:
+            continue
+        off[at] = bad
+        real = clamped(off, rows)
+        want, mass = product(x, x_scale, w, w_scale, real, rows)
+        got = int8.grouped_mm_int8(*args, off.to(DEV), x_scale=x_scale.to(DEV), out_dtype=F32)
+        assert ((got.double().cpu() - want).abs() <= 2.0 ** -24 * (4 * want.abs() + 19 * mass)).all()
+        assert device_status(0) == (0 if torch.equal(real, off) else 8)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=str)
+@pytest.mark.parametrize("H", [16, 512, 528, 2048, 2064, 4112, 16400, 20000])
+def test_tokens_of_any_length(H, dtype):
+    """Rows that 8, 32, 64 and 256 threads take, at the borders between them, and rows longer than their registers."""
+    x, weights, ids, w13, w2 = layer_inputs(3, H, 16, dtype, 6, 2, 41)
+    got = int8.int8_moe(x.to(DEV), weights.to(DEV), ids.to(DEV), *w13, *w2)
+    assert_layer(got, x, weights, ids, w13, w2)
+    wide = torch.cat([x, x], 1).to(DEV)[:, 1:H + 1]      # rows that do not begin on 16 bytes, read one by one
+    assert_layer(int8.int8_moe(wide, weights.to(DEV), ids.to(DEV), *w13, *w2), wide.cpu(), weights, ids, w13, w2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,k", [(1, 1), (1024, 2), (683, 3), (4097, 2), (5, 1024)])
+def test_slots_on_both_sides_of_a_cluster(T, k):
+    """2048 slots are placed by one block, the next ones by eight; as many slots a token as there may be."""
+    x, weights, ids, w13, w2 = layer_inputs(7, 32, 16, BF16, T, min(k, 7), 51)
+    if k > 7:
+        ids, weights = ids.repeat(1, k // 7 + 1)[:, :k], weights.repeat(1, k // 7 + 1)[:, :k] / (k / 7)
+    some = torch.arange(0, T, max(1, T // 150))
+    got = int8.int8_moe(x.to(DEV), weights.to(DEV), ids.to(DEV), *w13, *w2)
+    assert_layer(got.cpu()[some], x[some], weights[some], ids[some], w13, w2)
