@@ -585,12 +585,14 @@ __device__ int32_t choose_exact(const RouteParams& p, const T* row, float larges
   return id;
 }
 
-// The share of every chosen score (lane j < k: logit l, else used = false) in their sum.
+// The share of every chosen score (lane j < k: logit l, else used = false) in their sum.  Where all of them are small, as a
+// bias may choose, they are taken relative to their largest, or the smallest would be no normal numbers above a share of
+// 2^-126; a sigmoid there is e^l but for 2^-24 of it.
 template <bool SIGMOID>
 __device__ __forceinline__ float share_of(float l, float largest, bool used) {
   float x = !used || l == -INFINITY ? 0.f : SIGMOID ? sigmoid(l) : expf(l - largest);
   float sum = warp_sum(x);
-  if (sum < 1e-30f) {   // scores below f32's range: there a sigmoid is e^l too
+  if (sum < 0x1p-24f) {
     const float top = warp_max(used ? l : -INFINITY);
     x = !used || l == -INFINITY ? 0.f : expf(l - top);
     sum = warp_sum(x);

@@ -160,3 +160,23 @@ def test_softmax_gradient_next_to_a_score_of_one(E, k, gap):
     ref = logits.double().requires_grad_()
     (torch.softmax(ref, 1).gather(1, ids) * 1.5 * d.double()).sum().backward()
     assert ((want - ref.grad).abs() <= 2.0 ** -48 * d.double().abs().sum(1, keepdim=True)).all()
+
+
+# ------------------------------------------------------------------ weights of scores far below others
+@pytest.mark.gpu
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,k,groups", [(20, 7, 1), (96, 8, 8), (500, 16, 20), (1000, 32, 1)])
+def test_weights_of_scores_far_below_others(E, k, groups, scoring):
+    """Experts that a bias picks although their scores are f32's smallest, and scores that are all small: renormalised weights
+    are as near as any others (what is below 2^-126 may be off by that)."""
+    logits = normal((60, E), F32, E, 30.0)
+    if scoring == "sigmoid":
+        logits = -logits.abs() - torch.arange(60)[:, None]
+    bias = normal((E,), F32, 3, 3.0)
+    how = dict(scoring=scoring, groups=groups, topk_groups=max(1, groups // 2), group_top=1)
+    for b in (None, bias):
+        want, gap = masked_choice(logits, k, bias=b, **how)
+        assert b is None or gap > 1e-13   # without: decisions between numbers of any size, as near as their own size
+        weights, ids = router.route(logits.to(DEV), k, bias=None if b is None else b.to(DEV), **how)
+        assert torch.equal(ids.cpu().long(), want)
+        assert_weights(weights, weights_of(logits, want, scoring), logits, 1.0)
