@@ -371,8 +371,8 @@ __global__ void group_offsets_kernel(const int32_t* expert_ids, int64_t max_bloc
 // (206..228 at 1.12 GHz; HBM and tensor cores, each of which alone takes 145); the weight gradient of those 203..209 us
 // (229..260 at 1.27 GHz; tensor cores 52 % busy, 604 MB written, which takes a plain fill 157).  A single product of
 // 8192 x 8192 x 2048: 174 us (1580 TFLOP/s).
-// 8 bits, the same experts: 8 rows 7.6 us, 512 rows 47.3 (6.4 TB/s), 32768 rows 104..110 (without products 88, without loads
-// 60, without writes 90: HBM, which takes reads and writes mixed at 5.3 TB/s); 8192 x 8192 x 8192: 352 us (3120 TOPS).
+// 8 bits, the same experts: 8 rows 7.6 us, 512 rows 47.3 (6.4 TB/s), 32768 rows 103..107 (without products 88, without loads
+// 60, without writes 90: HBM, which takes reads and writes mixed at 5.3 TB/s), to f32 118; 8192 x 8192 x 8192: 363 us (3030 TOPS).
 constexpr int kMaxStages = 6;
 constexpr int kStepK = 64;
 constexpr uint32_t kOperandBytes = 128 * kStepK * 2;   // one operand's share of a CTA and step
@@ -404,8 +404,8 @@ constexpr uint32_t pair_smem(int mode) { return 1024 + kRingBytes + kWriters * k
 //            (one token on 96 experts, 1536 x 2048: 64 wide 14.5 us, 128 wide 13.1, 12.6 with the fifth step).
 //   kMiddle  up to 128: 4 steps of 48 KB, 128 wide
 // 8-bit products take kOne for all wide tiles: their products run half as long, so that kTwo's drain between tiles shows
-// (the layer of 4096 tokens, 96 experts of 2048 x 768: 267 us with kOne, 296 with kTwo; three steps of 64 KB instead of six of
-// 32: 276 against 274).
+// (the layer of 4096 tokens, 96 experts of 2048 x 768, its slots still in 16 bits: 267 us with kOne, 296 with kTwo; three steps
+// of 64 KB instead of six of 32: 276 against 274).
 enum PairShape { kOne = 0, kTwo = 1, kNarrow = 2, kMiddle = 3 };
 constexpr int subs_of(int shape) { return shape >= kNarrow ? 2 : 1; }   // 64-wide blocks of a step
 constexpr int span_of(int shape) {                                      // most rows of a tile
@@ -1444,6 +1444,7 @@ PairShape rows_shape(int64_t rows, int32_t experts, int32_t m_len) {
   const bool fills = static_cast<int64_t>(experts) * ((m_len + 255) / 256) >= 2 * kPairsPlanned;
   return rows > 256ll * experts && rows <= 512ll * experts && fills ? kTwo : kOne;
 }
+// 8-bit products go by the same thresholds, whose figures are of 16 bits; for 8 only kTwo against kOne was measured.
 PairShape int8_shape(int64_t rows, int32_t experts, int32_t m_len) {
   const PairShape shape = rows_shape(rows, experts, m_len);
   return shape == kTwo ? kOne : shape;
