@@ -1504,6 +1504,7 @@ struct JoinParams {
 // parts.  (As scaled f32 parts, each was off by its own roundings, which is more than the result's where parts cancel.)
 struct Int8JoinParams : JoinParams {
   const int32_t* row_expert;
+  int32_t experts;
   const float *x_scale, *w_scale;
 };
 
@@ -1531,7 +1532,7 @@ __global__ void __launch_bounds__(256) grouped_join_kernel(const P p) {
   }
   if constexpr (kWhole) {
     const int32_t e = p.row_expert[row];
-    if (e >= 0) {   // else a row of no group: 0, whatever its scale
+    if (e >= 0 && e < p.experts) {   // else a row of no group: 0, whatever its scale; or one whose product gave up before
       const float x = p.x_scale[row], *w = p.w_scale + static_cast<int64_t>(e) * p.cols + col;
 #pragma unroll
       for (int j = 0; j < 4; ++j) v[j] = __fmul_rn(__fmul_rn(static_cast<float>(sum[j]), j < count ? w[j] : 0.f), x);
@@ -1674,7 +1675,7 @@ int run_int8_product(const char* what, const Int8Product& d, cudaStream_t st) {
   if (e == cudaSuccess && split) {
     Int8JoinParams j{};
     j.part = d.workspace;
-    j.row_expert = q.row_expert; j.x_scale = d.x_scale; j.w_scale = d.w_scale;
+    j.row_expert = q.row_expert; j.experts = d.experts; j.x_scale = d.x_scale; j.w_scale = d.w_scale;
     j.rows = d.rows; j.pitch = pitch; j.splits = q.splits; j.cols = d.n;
     j.out = d.out; j.ld = d.ld_out; j.inner = static_cast<int32_t>(d.rows);
     j.f32 = f32; j.bf16 = bf16; j.vec = d.ld_out % 4 == 0 && !off_by(d.out, 8);
