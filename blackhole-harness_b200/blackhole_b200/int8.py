@@ -84,9 +84,10 @@ def grouped_mm_int8(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, off
     """out[r, n] = x_scale[r] w_scale[e, n] sum_k x[r, k] w[e, n, k] for every row r of group e, rows offsets[e] ..
     offsets[e + 1] - 1: x [R, K], w int8 [E, N, K] with w_scale float32 [E, N] -> [R, N].  Without offsets w is one
     matrix [N, K] for all rows.  x is int8 with x_scale float32 [R], or f32, bf16 or fp16 and quantized on the way
-    (quantize_rows).  The result is in out_dtype (f32, bf16 or fp16; x's, or bf16 for an int8 x): sums
-    are exact (K at most 131071), become f32, are multiplied by both scales there and rounded to the type.  Rows of no group come back as zero.  Stacks whose rows do not begin on multiples of 16 bytes are
-    copied at each call; quantize_rows makes them so that they do."""
+    (quantize_rows).  The result is in out_dtype (f32, bf16 or fp16; x's, or bf16 for an int8 x): sums are exact (K at
+    most 131071), become f32, are multiplied by both scales there and rounded to the type.  Rows of no group come back as
+    zero.  `out` overlaps no input.  Stacks whose rows do not begin on multiples of 16 bytes are copied at each call;
+    quantize_rows makes them so that they do."""
     if out is None and out_dtype is None and x_scale is None and offsets is not None:
         res = _call.grouped_mm_int8(x, w, w_scale, offsets)
         if res is not None:
